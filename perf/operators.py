@@ -249,7 +249,9 @@ class _Framework:
         self.lens[s] += n
 
     def fork(self, s):
-        return self.cache.fork([s], 1)
+        kids = self.cache.fork([s], 1)
+        self.lens[kids[0]] = self.lens[s]
+        return kids
 
     def close(self, s):
         self.cache.free([s])
