@@ -531,6 +531,75 @@ int infllm_shard_refill(infllm_shard_cache* cache, const int32_t* ids, int n, vo
 int infllm_ctx_save(infllm_ctx* ctx, const char* path, void* stream);
 int infllm_ctx_load(infllm_ctx* ctx, const char* path, void* stream);
 
+/* ------------------------------------------------------- paged cache, and attention over shared pages
+ * (No counterpart in the reference, whose caches hold one stream each.)  Several continuations of one prompt: sequences
+ * of tokens in pages of a pool that the caller owns; a fork shares its parent's full pages, and the attention reads what
+ * several sequences of a batch share once for all of them.
+ *
+ * Which pages a sequence has is known on the host at once; the device has a copy of the table.  What does not fit is
+ * refused (INFLLM_E_CAPACITY) before anything changes.  Pages and sequence numbers are taken lowest first, for one sequence
+ * after the other.  All calls on a cache belong on one stream, or are ordered by the caller; one host thread at a time.
+ *
+ * d_pages (n_layers, 2: keys and values, n_pages, n_kv_heads, page_size, head_dim), d_table (max_sequences, max_pages);
+ * head_dim 64 or 128, page_size 16, 32, 64 or 128.  device < 0: bookkeeping only, without a GPU. */
+typedef struct infllm_pages infllm_pages;
+typedef struct infllm_page_batch infllm_page_batch;
+typedef struct infllm_pages_config {
+  int32_t n_layers, n_kv_heads, head_dim, page_size, n_pages, max_sequences, max_pages, dtype, device, pad;
+  void* d_pages;
+  int32_t* d_table;
+} infllm_pages_config;
+/* Rows (batch, heads, tokens, head_dim): strides in elements, multiples of 8; the base 16-byte aligned. */
+typedef struct infllm_page_rows {
+  const void* d;
+  int64_t bs, hs, ts;
+} infllm_page_rows;
+
+int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages** out);
+int infllm_pages_destroy(infllm_pages* p);
+int infllm_pages_open(infllm_pages* p, int n, int32_t* out); /* n empty sequences */
+/* n_each continuations of each sequence: out (n, n_each).  Full pages are shared, a last page that is not full is copied. */
+int infllm_pages_fork(infllm_pages* p, const int32_t* seqs, int n, int n_each, int32_t* out, void* stream);
+/* Copies that share nothing, in `into`: the same cache, or another one whose pages have the same shape. */
+int infllm_pages_copy(infllm_pages* p, const int32_t* seqs, int n, infllm_pages* into, int32_t* out, void* stream);
+/* Cuts sequences to lengths; pages that no sequence has any more are free.  No device work. */
+int infllm_pages_truncate(infllm_pages* p, const int32_t* seqs, const int64_t* lengths, int n);
+int infllm_pages_free(infllm_pages* p, const int32_t* seqs, int n);
+/* Of each sequence only the tokens of its n_spans[i] spans [start, stop) stay (spans: all of them in a row, ascending within
+ * a sequence).  They close up; the position that its next token is rotated to stays.  Pages at the front of which every
+ * token stays are kept, the rest of the tokens goes to pages of its own. */
+int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n, const int64_t* spans, const int32_t* n_spans, void* stream);
+int infllm_pages_info(const infllm_pages* p, int32_t seq, int64_t* length, int64_t* position);
+int infllm_pages_row(const infllm_pages* p, int32_t seq, int32_t* out, int cap, int* n); /* its pages */
+int infllm_pages_free_count(const infllm_pages* p); /* free pages */
+
+/* A batch: sequences, and of each a count of newest tokens that the calls are about.  The tensors of a call have as many
+ * tokens as the largest count; a sequence with fewer has its own at the end, the rows before them are not read, or written
+ * as zeros.
+ *   extend    room for counts[i] more tokens, which become the newest
+ *   retract   takes counts[i] tokens back (no token is newest then)
+ *   select    the newest counts[i] tokens that are there
+ *   write     a layer's keys and values of the newest tokens into their pages, and q to d_q_out (batch, tokens, n_heads,
+ *             head_dim); with d_cos / d_sin (table_len, head_dim / 2) keys and queries rotated to the tokens' positions.
+ *             q may be NULL.
+ *   attend    attention of the newest tokens: each sees its sequence's tokens up to itself.  d_out (batch, tokens, n_heads,
+ *             head_dim), d_lse (batch, tokens, n_heads) fp32 log-sum-exp of the scores (natural logarithm), or NULL.
+ *             d_plan and d_scratch are the caller's, 16-byte aligned, of the sizes that infllm_page_batch_plan gives; that
+ *             call also works out the plan, which holds for all layers until a sequence of the cache changes.  d_plan is
+ *             uploaded by the attend call with `upload` set: the first one after the plan. */
+int infllm_page_batch_create(infllm_pages* p, const int32_t* seqs, int n, infllm_page_batch** out);
+int infllm_page_batch_destroy(infllm_page_batch* b);
+int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* counts, void* stream);
+int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* counts);
+int infllm_page_batch_select(infllm_page_batch* b, const int32_t* counts);
+int64_t infllm_page_batch_reach(const infllm_page_batch* b); /* rows that the tables have to have: the largest next position */
+int infllm_page_batch_write(infllm_page_batch* b, int layer, const infllm_page_rows* k, const infllm_page_rows* v,
+                            const infllm_page_rows* q, void* d_q_out, int n_heads, const float* d_cos, const float* d_sin,
+                            int64_t table_len, void* stream);
+int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* plan_bytes, int64_t* scratch_bytes, int* fresh);
+int infllm_page_batch_attend(infllm_page_batch* b, int layer, const infllm_page_rows* q, void* d_out, float* d_lse, int n_heads,
+                             float scale, void* d_plan, int upload, void* d_scratch, void* stream);
+
 /* ----------------------------------------------------- host logic, GPU-free
  * The LRU table alone (context_manager.py:246-265, 495-515): dict-ordered ids with stamps.
  * Exposed so that the eviction order can be tested without a device. */

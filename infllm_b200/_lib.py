@@ -69,6 +69,17 @@ class ShardCache(ctypes.Structure):
     ]
 
 
+class PagesConfig(ctypes.Structure):
+    """infllm_pages_config of include/infllm_b200.h."""
+    _fields_ = [(n, c_int32) for n in ("n_layers", "n_kv_heads", "head_dim", "page_size", "n_pages", "max_sequences", "max_pages",
+                                       "dtype", "device", "pad")] + [("d_pages", c_void_p), ("d_table", c_void_p)]
+
+
+class PageRows(ctypes.Structure):
+    """infllm_page_rows of include/infllm_b200.h."""
+    _fields_ = [("d", c_void_p), ("bs", c_int64), ("hs", c_int64), ("ts", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 class ShardToken(ctypes.Structure):
     """infllm_shard_token of include/infllm_b200.h."""
@@ -190,6 +201,28 @@ SIGNATURES = {
     "infllm_ctx_get_block_k": (c_int, [c_void_p, c_int64, c_int64, c_void_p]),
     "infllm_ctx_load_synthetic": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_void_p, c_void_p]),
+    "infllm_pages_create": (c_int, [POINTER(PagesConfig), POINTER(c_void_p)]),
+    "infllm_pages_destroy": (c_int, [c_void_p]),
+    "infllm_pages_open": (c_int, [c_void_p, c_int, POINTER(c_int32)]),
+    "infllm_pages_fork": (c_int, [c_void_p, POINTER(c_int32), c_int, c_int, POINTER(c_int32), c_void_p]),
+    "infllm_pages_copy": (c_int, [c_void_p, POINTER(c_int32), c_int, c_void_p, POINTER(c_int32), c_void_p]),
+    "infllm_pages_truncate": (c_int, [c_void_p, POINTER(c_int32), POINTER(c_int64), c_int]),
+    "infllm_pages_free": (c_int, [c_void_p, POINTER(c_int32), c_int]),
+    "infllm_pages_compact": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_int64), POINTER(c_int32), c_void_p]),
+    "infllm_pages_info": (c_int, [c_void_p, c_int32, POINTER(c_int64), POINTER(c_int64)]),
+    "infllm_pages_row": (c_int, [c_void_p, c_int32, POINTER(c_int32), c_int, POINTER(c_int)]),
+    "infllm_pages_free_count": (c_int, [c_void_p]),
+    "infllm_page_batch_create": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_void_p)]),
+    "infllm_page_batch_destroy": (c_int, [c_void_p]),
+    "infllm_page_batch_extend": (c_int, [c_void_p, POINTER(c_int32), c_void_p]),
+    "infllm_page_batch_retract": (c_int, [c_void_p, POINTER(c_int32)]),
+    "infllm_page_batch_select": (c_int, [c_void_p, POINTER(c_int32)]),
+    "infllm_page_batch_reach": (c_int64, [c_void_p]),
+    "infllm_page_batch_write": (c_int, [c_void_p, c_int, POINTER(PageRows), POINTER(PageRows), POINTER(PageRows), c_void_p, c_int,
+                                        c_void_p, c_void_p, c_int64, c_void_p]),
+    "infllm_page_batch_plan": (c_int, [c_void_p, c_int, POINTER(c_int64), POINTER(c_int64), POINTER(c_int)]),
+    "infllm_page_batch_attend": (c_int, [c_void_p, c_int, POINTER(PageRows), c_void_p, c_void_p, c_int, c_float, c_void_p, c_int,
+                                         c_void_p, c_void_p]),
     "infllm_lru_create": (c_int, [c_int, POINTER(c_void_p)]),
     "infllm_lru_destroy": (c_int, [c_void_p]),
     "infllm_lru_plan": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_int32), POINTER(c_int)]),

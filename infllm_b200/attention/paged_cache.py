@@ -1,0 +1,254 @@
+"""A paged key/value cache for several continuations of one prompt, and attention that reads shared pages once.
+
+The reference's caches hold one stream each (inf_llm/attention/context_manager.py:196-816, stream_llm.py:6-111); this
+one is for a program that samples many answers to a long prompt, keeps beams, or puts many questions to one document:
+
+    cache = PagedCache(n_layers, n_kv_heads, head_dim, n_pages)
+    root = cache.open()[0]
+    prompt = cache.batch([root])
+    prompt.extend(len_prompt)                              # once per step ...
+    q = prompt.write(layer, k, v, q, rope)                 # ... then in every layer
+    o = prompt.attend(layer, q)
+    answers = cache.batch(cache.fork([root], 64))          # 64 sequences that share the prompt's pages
+    answers.extend(1); ...
+
+Tensors are (batch, heads, tokens, head_dim) views with any strides whose rows are 16-byte aligned, as the other
+attention types take them.  Work goes to the current stream; all calls on a cache belong on one stream, or are ordered by
+the caller."""
+import ctypes
+import math
+from ctypes import c_int32, c_int64
+
+import torch
+
+from .. import _lib
+from .rope import RotaryEmbeddingESM
+
+_lib_call = _lib.lib
+
+
+def _ids(seqs):
+    return (c_int32 * len(seqs))(*seqs)
+
+
+class PagedCache:
+    """`n_pages` pages of `page_size` tokens (16, 32, 64 or 128), each with the keys and values of all layers, and up to
+    `max_sequences` sequences of up to `max_tokens` tokens over them.  head_dim is 64 or 128, dtype bfloat16 or float16.
+
+    `pages` (n_layers, 2, n_pages, n_kv_heads, page_size, head_dim) and `table` (max_sequences, max_pages) are the device's
+    memory of it.  Sequences are named by small numbers.  What does not fit raises InfLLMCapacityError and changes nothing."""
+
+    def __init__(self, n_layers, n_kv_heads, head_dim, n_pages, page_size=128, max_sequences=256, max_tokens=131072,
+                 dtype=torch.bfloat16, device=None):
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError(f"a CUDA device is needed, got {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.n_layers, self.n_kv_heads, self.head_dim = int(n_layers), int(n_kv_heads), int(head_dim)
+        self.n_pages, self.page_size, self.max_sequences = int(n_pages), int(page_size), int(max_sequences)
+        self.dtype = dtype
+        if min(self.n_layers, self.n_kv_heads, self.head_dim, self.n_pages, self.page_size, self.max_sequences, int(max_tokens)) < 1:
+            raise ValueError("sizes of a paged cache are positive")
+        max_pages = -(-int(max_tokens) // self.page_size)
+        self.pages = torch.zeros((self.n_layers, 2, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim), dtype=dtype,
+                                 device=self.device)
+        self.table = torch.zeros((self.max_sequences, max_pages), dtype=torch.int32, device=self.device)
+        cfg = _lib.PagesConfig(self.n_layers, self.n_kv_heads, self.head_dim, self.page_size, self.n_pages, self.max_sequences,
+                               max_pages, _lib.dtype_code(dtype), self.device.index, 0, self.pages.data_ptr(), self.table.data_ptr())
+        self.handle = ctypes.c_void_p()
+        _lib.check(_lib_call.infllm_pages_create(ctypes.byref(cfg), ctypes.byref(self.handle)))
+
+    def __del__(self):
+        try:
+            if self.handle:
+                _lib_call.infllm_pages_destroy(self.handle)
+        except Exception:
+            pass
+        self.handle = None
+
+    # -- sequences
+    def open(self, n=1):
+        """n new, empty sequences: their numbers, the lowest that are not in use."""
+        out = (c_int32 * n)()
+        _lib.check(_lib_call.infllm_pages_open(self.handle, n, out))
+        return list(out)
+
+    def fork(self, seqs, n=1):
+        """n continuations of each of `seqs`, one sequence's after the other's.  They share its full pages; a last page that is not
+        full is copied, in all layers."""
+        out = (c_int32 * (len(seqs) * n))()
+        _lib.check(_lib_call.infllm_pages_fork(self.handle, _ids(seqs), len(seqs), n, out, _lib.raw_stream(self.device)))
+        return list(out)
+
+    def copy(self, seqs, into=None):
+        """Copies of `seqs` that share no pages, here or `into` another PagedCache with pages of the same shape."""
+        into = self if into is None else into
+        out = (c_int32 * len(seqs))()
+        _lib.check(_lib_call.infllm_pages_copy(self.handle, _ids(seqs), len(seqs), into.handle, out, _lib.raw_stream(self.device)))
+        return list(out)
+
+    def truncate(self, seqs, lengths):
+        """Cuts each sequence to a length."""
+        if len(seqs) != len(lengths):
+            raise ValueError(f"{len(seqs)} sequences and {len(lengths)} lengths")
+        _lib.check(_lib_call.infllm_pages_truncate(self.handle, _ids(seqs), (c_int64 * len(seqs))(*lengths), len(seqs)))
+
+    def free(self, seqs):
+        """Ends sequences; pages that no other one shares are free."""
+        _lib.check(_lib_call.infllm_pages_free(self.handle, _ids(seqs), len(seqs)))
+
+    def compact(self, seqs, keep):
+        """Of each sequence only the tokens of keep[i], a list of ascending (start, stop), stay, and close up.  Keys keep the
+        rotation that they were written with, and position() goes on from where it was.  Pages at the front that stay whole
+        are kept, and stay shared; the other tokens move to pages of the sequence's own."""
+        if len(seqs) != len(keep):
+            raise ValueError(f"{len(seqs)} sequences and {len(keep)} lists of spans")
+        flat = [x for spans in keep for span in spans for x in span]
+        counts = _ids([len(spans) for spans in keep])
+        if len(flat) != 2 * sum(counts):
+            raise ValueError("spans are pairs (start, stop)")
+        _lib.check(_lib_call.infllm_pages_compact(self.handle, _ids(seqs), len(seqs), (c_int64 * len(flat))(*flat), counts,
+                                                  _lib.raw_stream(self.device)))
+
+    def batch(self, seqs):
+        return PagedBatch(self, seqs)
+
+    # -- what there is
+    def _info(self, seq):
+        length, position = c_int64(), c_int64()
+        _lib.check(_lib_call.infllm_pages_info(self.handle, seq, ctypes.byref(length), ctypes.byref(position)))
+        return length.value, position.value
+
+    def length(self, seq):
+        """Tokens of a sequence."""
+        return self._info(seq)[0]
+
+    def position(self, seq):
+        """The position that its next token is rotated to: the tokens that it has had (compact() takes none of them back)."""
+        return self._info(seq)[1]
+
+    def page_ids(self, seq):
+        n = ctypes.c_int()
+        out = (c_int32 * self.table.size(1))()
+        _lib.check(_lib_call.infllm_pages_row(self.handle, seq, out, len(out), ctypes.byref(n)))
+        return out[:n.value]
+
+    @property
+    def free_pages(self):
+        return _lib_call.infllm_pages_free_count(self.handle)
+
+
+class PagedBatch:
+    """Sequences that take a step together.  extend(), or plan(), says how many of each one's newest tokens the step is about;
+    write() and attend() are then called in every layer.  Tensors have as many tokens as the largest of those counts; a
+    sequence with fewer has its own at the end, and what is before them is not read, and zero in what is returned."""
+
+    def __init__(self, cache, seqs):
+        self.cache, self.seqs = cache, list(seqs)
+        self._n = len(self.seqs)
+        self.tokens = 0  # of the step's tensors
+        self._plan = None
+        self._sizes = c_int64(), c_int64(), ctypes.c_int()
+        self._size_refs = tuple(ctypes.byref(x) for x in self._sizes)
+        self.handle = ctypes.c_void_p()
+        _lib.check(_lib_call.infllm_page_batch_create(cache.handle, _ids(self.seqs), self._n, ctypes.byref(self.handle)))
+
+    def __del__(self):
+        try:
+            if self.handle:
+                _lib_call.infllm_page_batch_destroy(self.handle)
+        except Exception:
+            pass
+        self.handle = None
+
+    def _counts(self, n):
+        if isinstance(n, int):
+            return (c_int32 * self._n)(*[n] * self._n), n
+        if len(n) != self._n:
+            raise ValueError(f"{self._n} sequences and {len(n)} counts")
+        return _ids(n), max(n)
+
+    def extend(self, n):
+        """Room for n more tokens of every sequence, or for n[i]: they are the step's."""
+        counts, most = self._counts(n)
+        _lib.check(_lib_call.infllm_page_batch_extend(self.handle, counts, _lib.raw_stream(self.cache.device)))
+        self.tokens = most
+
+    def plan(self, n):
+        """The newest n tokens of every sequence, or n[i], that are there already, are the step's."""
+        counts, most = self._counts(n)
+        _lib.check(_lib_call.infllm_page_batch_select(self.handle, counts))
+        self.tokens = most
+
+    def retract(self, n):
+        """Takes the newest n tokens of every sequence, or n[i], back, as a speculative decoder does with drafts."""
+        counts, _ = self._counts(n)
+        _lib.check(_lib_call.infllm_page_batch_retract(self.handle, counts))
+        self.tokens = 0
+
+    def _rows(self, t, heads, what):
+        """(batch, heads, tokens, head_dim) as the library takes it, and the tensor that has to live until the call."""
+        c = self.cache
+        if t.device != c.device:
+            raise RuntimeError(f"{what} must be on {c.device}: infllm_b200 has no CPU path")
+        if t.dtype != c.dtype:
+            raise TypeError(f"{what} is {t.dtype}, the cache {c.dtype}")
+        if t.shape != (self._n, heads, self.tokens, c.head_dim):
+            raise ValueError(f"{what} is {tuple(t.shape)}, not {(self._n, heads, self.tokens, c.head_dim)}")
+        bs, hs, ts, ds = t.stride()
+        at = t.data_ptr()
+        if ds != 1 or (bs | hs | ts) % 8 or at % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+            bs, hs, ts, _ = t.stride()
+            at = t.data_ptr()
+        return _lib.PageRows(at, bs, hs, ts), t
+
+    def write(self, layer, k, v, q=None, rope=None):
+        """The step's keys and values (batch, n_kv_heads, tokens, head_dim) into a layer's pages.  With `rope`, a
+        RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q)."""
+        c = self.cache
+        rk, k = self._rows(k, c.n_kv_heads, "k")
+        rv, v = self._rows(v, c.n_kv_heads, "v")
+        rq = out = cos = sin = None
+        heads = rows = at = 0
+        if q is not None:
+            heads = q.size(1)
+            rq, q = self._rows(q, heads, "q")
+            out = torch.empty((self._n, self.tokens, heads, c.head_dim), dtype=c.dtype, device=c.device)
+            at = out.data_ptr()
+            rq = ctypes.byref(rq)
+        if rope is not None:
+            if not isinstance(rope, RotaryEmbeddingESM) or rope.dim != c.head_dim:
+                raise ValueError(f"rope must be a RotaryEmbeddingESM of {c.head_dim} dimensions")
+            cos, sin = rope._tables(max(_lib_call.infllm_page_batch_reach(self.handle), 1), c.device)
+            rows, cos, sin = cos.size(0), cos.data_ptr(), sin.data_ptr()
+        _lib.check(_lib_call.infllm_page_batch_write(self.handle, layer, ctypes.byref(rk), ctypes.byref(rv), rq, at, heads, cos, sin, rows,
+                                                     _lib.raw_stream(c.device)))
+        return None if out is None else out.permute(0, 2, 1, 3)
+
+    def attend(self, layer, q, scale=None, return_lse=False):
+        """Attention of the step's queries (batch, n_heads, tokens, head_dim) to their sequences' keys up to their own places.
+        `scale` of the scores: 1 / sqrt(head_dim) if not given.  Returns (batch, n_heads, tokens, head_dim), a view of
+        (batch, tokens, n_heads, head_dim); with return_lse also the scores' log-sum-exps (batch, n_heads, tokens), fp32."""
+        c = self.cache
+        heads = q.size(1) if q.dim() == 4 else 0
+        rq, q = self._rows(q, heads, "q")
+        rc = _lib_call.infllm_page_batch_plan(self.handle, heads, *self._size_refs)
+        if rc:
+            _lib.check(rc)
+        plan_bytes, scratch_bytes, fresh = (x.value for x in self._sizes)
+        if fresh or self._plan is None:  # (memory of its own: the last plan may still be in use)
+            fresh = 1
+            self._plan = torch.empty(max(plan_bytes, 16), dtype=torch.uint8, device=c.device)
+        scratch = torch.empty(max(scratch_bytes, 16), dtype=torch.uint8, device=c.device)
+        out = torch.empty((self._n, self.tokens, heads, c.head_dim), dtype=c.dtype, device=c.device)
+        lse = torch.empty((self._n, self.tokens, heads), dtype=torch.float32, device=c.device) if return_lse else None
+        rc = _lib_call.infllm_page_batch_attend(self.handle, layer, ctypes.byref(rq), out.data_ptr(), lse.data_ptr() if return_lse else None,
+                                                heads, 1.0 / math.sqrt(c.head_dim) if scale is None else scale, self._plan.data_ptr(), fresh,
+                                                scratch.data_ptr(), _lib.raw_stream(c.device))
+        if rc:
+            self._plan = None
+            _lib.check(rc)
+        out = out.permute(0, 2, 1, 3)
+        return (out, lse.permute(0, 2, 1)) if return_lse else out

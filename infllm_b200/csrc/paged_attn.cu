@@ -1,0 +1,547 @@
+// Attention of a batch of sequences over a paged cache (pages.cu), with what several of them share read once for all.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij) / sum_j exp(s_ij),  s_ij = scale q_i . k_j,  over the keys j up to query i's place
+//
+// A batch's pages form a tree: a node is a stretch of pages that the same sequences have.  The queries of all sequences
+// under a node, of all query heads of a KV head, are the rows of one product with the node's keys; a query's row appears in
+// every node on the way to its sequence, and the parts are joined by their log-sum-exps,
+//   M = max_p lse_p,   o = sum_p 2^(lse_p - M) o_p / sum_p 2^(lse_p - M)   (logarithms to base 2).
+// A node ends before the newest tokens of its sequences, so that only a sequence's own last stretch (a leaf) has keys that
+// some of its queries do not see.
+//
+// The host knows the tree and all lengths: it cuts every node's rows into tiles and its keys into units of about equal work.
+#include <algorithm>
+#include <cstring>
+
+#include "decode_warp.cuh"
+#include "pages.cuh"
+
+namespace infllm {
+
+using namespace mma;
+
+constexpr int kSeeAll = 1 << 30;
+
+struct alignas(16) AttnUnit {
+  int32_t row;        // of the page table: one of the node's sequences
+  int32_t key0, keys; // keys of the sequence; key0 is the first token of a page
+  int32_t lim0;       // a row of token i sees the keys below lim0 + i
+  int32_t row0, rows; // of the node's rows: (sequence of the node, token, query head of the KV head)
+  int32_t node_seq;   // where the node's sequences are listed
+  int32_t part;       // where the unit's partial rows begin: part * n_kv_heads + kv head * rows; -1: they are whole, and go to the output
+};
+struct alignas(16) AttnSeq {   // of a sequence of the batch, for the join
+  int32_t path, n_path;        // its nodes
+  int32_t count, pad;
+};
+struct alignas(16) AttnPath {
+  int32_t span, tile;          // the node's first row tile's span, rows of a tile
+  int32_t at, pad;             // place of the sequence in the node
+};
+struct alignas(16) AttnSpan {  // of a row tile of a node: n partials, one behind the other
+  int32_t part, n, rows, pad;
+};
+
+struct PagedParams {
+  const char* pages;  // keys of the layer
+  int64_t plane;      // bytes from keys to values
+  const int32_t* table;
+  const char* q;
+  int64_t q_bs, q_hs, q_ts;  // bytes
+  char* out;
+  float* lse;
+  float *part_o, *part_lse;
+  const AttnUnit* unit;
+  const AttnSeq* seq;
+  const AttnPath* path;
+  const AttnSpan* span;
+  const int32_t* node_seq;
+  int32_t max_pages, page, n_kv, group, most, batch;
+  float scale_log2;
+};
+
+// where a row of a node is in the batch
+struct RowAt {
+  int32_t b, i, h;  // sequence, token, query head of the KV head
+};
+__device__ __forceinline__ RowAt row_at(const PagedParams& P, int node_seq, int r) {
+  RowAt a;
+  const int t = r / P.group;
+  a.h = r - t * P.group;
+  const int j = t / P.most;
+  a.i = t - j * P.most;
+  a.b = __ldg(P.node_seq + node_seq + j);
+  return a;
+}
+
+// ------------------------------------------------------------------------------------------------------- few rows
+// Up to 16 rows: a unit's keys in groups of 16, a warp per group; keys and values go from global memory straight into the
+// registers that are the operands of the m16n8k16 products (decode_warp.cuh has the same arrangement for eight rows of 128
+// dimensions).  It is bound by the bytes of the keys and values.
+constexpr int kRowWarps = 4;
+constexpr int kRowTile = 16;
+
+template <typename T, int kDim, int kNt>  // kNt: tiles of eight rows
+__global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid_constant__ PagedParams P) {
+  constexpr int kJ = kDim / 32;   // 16-byte pieces of a row that a thread has as scores' operands
+  constexpr int kH = kDim / 64;   // of a value's row
+  constexpr int kPitch = kDim + 4;
+  __shared__ __align__(16) float sm_o[kRowWarps][8 * kNt][kPitch];
+  __shared__ float sm_m[kRowWarps][8 * kNt], sm_l[kRowWarps][8 * kNt];
+  chain_enter();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const AttnUnit U = P.unit[blockIdx.x];
+  const int hkv = blockIdx.y;
+  uint4 qf[kNt][kJ];
+  int lim[kNt];
+#pragma unroll
+  for (int x = 0; x < kNt; ++x) {
+    const int r = x * 8 + g;
+    lim[x] = 0;
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) qf[x][j] = make_uint4(0, 0, 0, 0);
+    if (r < U.rows) {
+      const RowAt a = row_at(P, U.node_seq, U.row0 + r);
+      // (a row without a token sees nothing)
+      lim[x] = a.i < P.most - __ldg(&P.seq[a.b].count) ? 0 : min(U.lim0 + a.i, U.key0 + U.keys);
+      const char* qp = P.q + a.b * P.q_bs + (int64_t)(hkv * P.group + a.h) * P.q_hs + a.i * P.q_ts;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) qf[x][j] = __ldg(reinterpret_cast<const uint4*>(qp + j * 64 + t * 16));
+    }
+  }
+  float ot[8][kNt][4], m[kNt], l[kNt];
+#pragma unroll
+  for (int x = 0; x < kNt; ++x) {
+    m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ot[i][x][0] = ot[i][x][1] = ot[i][x][2] = ot[i][x][3] = 0.f;
+  }
+  const int32_t* row = P.table + (int64_t)U.row * P.max_pages;
+  const int n_groups = (U.keys + 15) / 16;
+#pragma unroll 1
+  for (int it = warp; it < n_groups; it += kRowWarps) {
+    const int j0 = U.key0 + it * 16, nk = min(16, U.key0 + U.keys - j0);
+    const char* kb = P.pages + (((int64_t)__ldg(row + j0 / P.page) * P.n_kv + hkv) * P.page + j0 % P.page) * (kDim * 2);
+    const char* vb = kb + P.plane;
+    uint4 kr[2][kJ], vr[4][kH];
+    // (what lies behind the last key is not read: it is not a number in the worst case, and 0 times that is none)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const int r = nt * 8 + g;
+      const char* rp = kb + (r < nk ? r : nk - 1) * (kDim * 2) + t * 16;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) kr[nt][j] = ld_stream16(rp + j * 64);
+    }
+#pragma unroll
+    for (int ki = 0; ki < 4; ++ki) {
+      const int r = 2 * t + (ki & 1) + (ki >> 1) * 8;
+      const char* rp = vb + (r < nk ? r : nk - 1) * (kDim * 2) + g * 16;
+#pragma unroll
+      for (int j = 0; j < kH; ++j) vr[ki][j] = ld_stream16(rp + j * 128);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        const uint32_t a0[4] = {qf[0][j].x, kNt > 1 ? qf[kNt - 1][j].x : 0u, qf[0][j].y, kNt > 1 ? qf[kNt - 1][j].y : 0u};
+        mma16816<T>(s[nt], a0, kr[nt][j].x, kr[nt][j].y);
+        const uint32_t a1[4] = {qf[0][j].z, kNt > 1 ? qf[kNt - 1][j].z : 0u, qf[0][j].w, kNt > 1 ? qf[kNt - 1][j].w : 0u};
+        mma16816<T>(s[nt], a1, kr[nt][j].z, kr[nt][j].w);
+      }
+    }
+    uint32_t pb[kNt][2];
+#pragma unroll
+    for (int x = 0; x < kNt; ++x) {  // row x * 8 + g: keys nt * 8 + 2t + e
+      float v[4], mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = j0 + (k >> 1) * 8 + 2 * t + (k & 1);
+        v[k] = key < lim[x] ? s[k >> 1][x * 2 + (k & 1)] * P.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, v[k]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[x], mx), ms = mn == -INFINITY ? 0.f : mn;
+      const float al = exp2f(m[x] - ms);
+      m[x] = mn;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = exp2f(v[k] - ms);
+      l[x] = l[x] * al + (v[0] + v[1]) + (v[2] + v[3]);
+      pb[x][0] = pack2<T>(v[0], v[1]), pb[x][1] = pack2<T>(v[2], v[3]);
+      // this thread's columns of O^T are rows 2t and 2t + 1
+      const float a0 = __shfl_sync(0xffffffffu, al, (2 * t) * 4), a1 = __shfl_sync(0xffffffffu, al, (2 * t + 1) * 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ot[i][x][0] *= a0;
+        ot[i][x][1] *= a1;
+        ot[i][x][2] *= a0;
+        ot[i][x][3] *= a1;
+      }
+    }
+    const uint32_t* w[4][kH];
+#pragma unroll
+    for (int ki = 0; ki < 4; ++ki)
+#pragma unroll
+      for (int j = 0; j < kH; ++j) w[ki][j] = reinterpret_cast<const uint32_t*>(&vr[ki][j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i >> 1;
+      const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;  // the high or the low 16 bits of both words
+      uint32_t a[4];
+      a[0] = __byte_perm(w[0][0][r], w[1][0][r], sel);  // dimension g*8+i of keys 2t, 2t+1
+      a[2] = __byte_perm(w[2][0][r], w[3][0][r], sel);  // of keys 2t+8, 2t+9
+      a[1] = kH > 1 ? __byte_perm(w[0][kH - 1][r], w[1][kH - 1][r], sel) : 0u;  // dimension 64+g*8+i
+      a[3] = kH > 1 ? __byte_perm(w[2][kH - 1][r], w[3][kH - 1][r], sel) : 0u;
+#pragma unroll
+      for (int x = 0; x < kNt; ++x) mma16816<T>(ot[i][x], a, pb[x][0], pb[x][1]);
+    }
+  }
+  // the warps' results meet in shared memory; dimension half*64 + g*8 + i at half*64 + i*8 + g, for the banks' sake
+#pragma unroll
+  for (int x = 0; x < kNt; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    if (t == 0) sm_m[warp][x * 8 + g] = m[x], sm_l[warp][x * 8 + g] = l[x];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sm_o[warp][x * 8 + 2 * t + e][i * 8 + g] = ot[i][x][e];
+        if (kH > 1) sm_o[warp][x * 8 + 2 * t + e][64 % kDim + i * 8 + g] = ot[i][x][2 + e];
+      }
+  }
+  __syncthreads();
+  for (int idx = tid; idx < U.rows * (kDim / 2); idx += kRowWarps * 32) {  // two neighbouring dimensions each
+    const int r = idx / (kDim / 2), d = idx % (kDim / 2) * 2;
+    const int p0 = (d & 64) | ((d & 7) << 3) | ((d >> 3) & 7), p1 = p0 + 8;
+    float mx = sm_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kRowWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
+    float den = 0.f, n0 = 0.f, n1 = 0.f;
+    if (mx != -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) {
+        const float wt = exp2f(sm_m[w][r] - mx);
+        den = fmaf(wt, sm_l[w][r], den);
+        n0 = fmaf(wt, sm_o[w][r][p0], n0);
+        n1 = fmaf(wt, sm_o[w][r][p1], n1);
+      }
+      n0 /= den, n1 /= den;
+    }
+    const float lse = mx == -INFINITY ? -INFINITY : mx + log2f(den);
+    if (U.part >= 0) {
+      const int64_t pr = (int64_t)U.part * P.n_kv + hkv * U.rows + r;
+      *reinterpret_cast<float2*>(P.part_o + pr * kDim + d) = make_float2(n0, n1);
+      if (d == 0) P.part_lse[pr] = lse;
+    } else {
+      const RowAt a = row_at(P, U.node_seq, U.row0 + r);
+      const int64_t orow = ((int64_t)a.b * P.most + a.i) * (P.n_kv * P.group) + hkv * P.group + a.h;
+      *reinterpret_cast<uint32_t*>(P.out + (orow * kDim + d) * 2) = pack2<T>(n0, n1);
+      if (P.lse && d == 0) P.lse[orow] = lse * (1.f / kLog2e);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- the join
+// A warp per query head and token: its parts of all nodes of its sequence.  Bound by the latency of two loads behind one
+// another and by the bytes of the partial rows.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams P) {
+  constexpr int kPer = kDim / 32;
+  chain_enter();
+  const int64_t orow = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, heads = P.n_kv * P.group;
+  if (orow >= (int64_t)P.batch * P.most * heads) return;
+  const int h = (int)(orow % heads), i = (int)(orow / heads % P.most), b = (int)(orow / heads / P.most);
+  const int hkv = h / P.group;
+  const AttnSeq S = P.seq[b];
+  float mx = -INFINITY;
+  const bool is = i >= P.most - S.count;  // (a row without a token: zeros)
+  auto parts = [&](auto&& f) {
+    for (int k = 0; k < S.n_path; ++k) {
+      const AttnPath A = P.path[S.path + k];
+      const int r = (A.at * P.most + i) * P.group + h % P.group, tile = r / A.tile;
+      const AttnSpan Z = P.span[A.span + tile];
+      f((int64_t)Z.part * P.n_kv + hkv * Z.rows + (r - tile * A.tile), Z.n, (int64_t)Z.rows * P.n_kv);
+    }
+  };
+  bool whole = false;  // written by the unit that had all of it
+  if (is)
+    parts([&](int64_t at, int n, int64_t step) {
+      whole |= n < 0;
+      for (int c = lane; c < n; c += 32) mx = fmaxf(mx, P.part_lse[at + c * step]);
+    });
+  if (whole) return;
+  mx = warp_max(mx);
+  float den = 0.f, acc[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+  if (mx != -INFINITY)
+    parts([&](int64_t at, int n, int64_t step) {
+#pragma unroll 4
+      for (int c = 0; c < n; ++c) {
+        const float w = exp2f(P.part_lse[at + c * step] - mx);
+        const float* o = P.part_o + (at + c * step) * kDim + lane * kPer;
+        den += w;
+        if (kPer == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(o);
+          acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]), acc[2 % kPer] = fmaf(w, v.z, acc[2 % kPer]), acc[3 % kPer] = fmaf(w, v.w, acc[3 % kPer]);
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(o);
+          acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]);
+        }
+      }
+    });
+  const float inv = mx != -INFINITY ? 1.f / den : 0.f;
+  uint32_t* to = reinterpret_cast<uint32_t*>(P.out + (orow * kDim + lane * kPer) * 2);
+#pragma unroll
+  for (int k = 0; k < kPer; k += 2) to[k / 2] = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
+  if (P.lse && lane == 0) P.lse[orow] = mx != -INFINITY ? (mx + log2f(den)) * (1.f / kLog2e) : -INFINITY;
+}
+
+// ----------------------------------------------------------------------------------------------------------- the plan
+namespace {
+
+struct Node {
+  int64_t key0, key1;
+  std::vector<int32_t> seqs;  // of the batch
+};
+
+// the batch's sequences in the order of their pages, and how many first pages each shares with the one before
+void order_batch(infllm_page_batch* b) {
+  const infllm_pages* p = b->cache;
+  const int n = (int)b->seqs.size();
+  auto pages = [&](int i) -> const std::vector<int32_t>& { return p->seqs[b->seqs[i]].pages; };
+  b->order.resize(n);
+  for (int i = 0; i < n; ++i) b->order[i] = i;
+  std::stable_sort(b->order.begin(), b->order.end(), [&](int x, int y) { return pages(x) < pages(y); });
+  b->common.assign(n, 0);
+  for (int i = 1; i < n; ++i) {
+    const std::vector<int32_t>&x = pages(b->order[i - 1]), &y = pages(b->order[i]);
+    const size_t most = std::min(x.size(), y.size());
+    b->common[i] = (int32_t)(std::mismatch(x.begin(), x.begin() + most, y.begin()).first - x.begin());
+  }
+}
+
+struct Tree {
+  const infllm_page_batch* b;
+  std::vector<Node> nodes;
+  std::vector<std::vector<int32_t>> path;  // nodes of a sequence of the batch
+
+  int64_t length(int i) const { return b->cache->seqs[b->seqs[i]].length; }
+  void add(int64_t key0, int64_t key1, std::vector<int32_t> seqs) {
+    for (int32_t i : seqs) path[i].push_back((int32_t)nodes.size());
+    nodes.push_back({key0, key1, std::move(seqs)});
+  }
+  // sequences that share `at` pages; common[k]: pages that seqs[k] shares with seqs[k - 1]
+  void build(const std::vector<int32_t>& seqs, const std::vector<int32_t>& common, int32_t at) {
+    const int page = b->cache->cfg.page_size;
+    size_t k = 0;
+    while (k < seqs.size()) {
+      // a run of neighbours that have page `at` in common, where it holds none of their newest tokens
+      auto whole = [&](size_t x) { return (int32_t)((length(seqs[x]) - b->count[seqs[x]]) / page); };
+      std::vector<int32_t> run, with;
+      int32_t link = INT32_MAX;
+      size_t e = k;
+      for (; e < seqs.size(); ++e) {
+        if (e > k) link = std::min(link, common[e]);
+        if (link <= at) break;
+        if (whole(e) > at) {
+          run.push_back(seqs[e]);
+          with.push_back(run.size() == 1 ? 0 : link);
+          link = INT32_MAX;
+        } else if (length(seqs[e]) > (int64_t)at * page) {
+          add((int64_t)at * page, length(seqs[e]), {seqs[e]});
+        }
+      }
+      k = e;
+      if (run.size() == 1) {
+        add((int64_t)at * page, length(run[0]), run);
+      } else if (run.size() > 1) {
+        int32_t to = INT32_MAX;
+        for (size_t x = 0; x < run.size(); ++x) {
+          to = std::min(to, (int32_t)((length(run[x]) - b->count[run[x]]) / page));
+          if (x > 0) to = std::min(to, with[x]);
+        }
+        add((int64_t)at * page, (int64_t)to * page, run);
+        build(run, with, to);
+      }
+    }
+  }
+};
+
+template <typename V>
+int64_t append(std::vector<int32_t>* plan, const std::vector<V>& v) {
+  plan->resize((plan->size() + 3) / 4 * 4);
+  const int64_t at = (int64_t)plan->size();
+  plan->resize(plan->size() + v.size() * sizeof(V) / 4);
+  if (!v.empty()) memcpy(plan->data() + at, v.data(), v.size() * sizeof(V));
+  return at;
+}
+
+int make_plan(infllm_page_batch* b, int n_heads) {
+  const infllm_pages* p = b->cache;
+  const int n = (int)b->seqs.size(), group = n_heads / p->cfg.n_kv_heads, most = b->most;
+  if (b->order_of != p->reshape) {
+    order_batch(b);
+    b->order_of = p->reshape;
+  }
+  Tree tree{b, {}, std::vector<std::vector<int32_t>>(n)};
+  tree.build(b->order, b->common, 0);
+
+  // row tiles
+  struct Tile {
+    int32_t node, row0, rows;
+    int64_t key1;
+  };
+  std::vector<Tile> tiles;
+  std::vector<int32_t> first_tile;
+  int64_t work = 0;
+  for (size_t x = 0; x < tree.nodes.size(); ++x) {
+    const Node& N = tree.nodes[x];
+    const bool leaf = N.seqs.size() == 1;
+    const int64_t rows = (int64_t)N.seqs.size() * most * group;
+    first_tile.push_back((int32_t)tiles.size());
+    for (int64_t r = 0; r < rows; r += kRowTile) {
+      Tile t{(int32_t)x, (int32_t)r, (int32_t)std::min<int64_t>(kRowTile, rows - r), N.key1};
+      if (leaf) t.key1 = N.key1 - most + (r + t.rows - 1) / group + 1;  // up to the last row's token
+      tiles.push_back(t);
+      work += std::max<int64_t>(0, ceil_div(t.key1 - N.key0, 16)) * p->cfg.n_kv_heads;
+    }
+  }
+  // units of equal work: four blocks per SM, a warp's groups of 16 keys at least
+  const int64_t chunk = std::max<int64_t>(kRowWarps, ceil_div(ceil_div(work, 148 * 4), kRowWarps) * kRowWarps) * 16;
+  std::vector<AttnUnit> units;
+  std::vector<AttnSpan> spans;
+  std::vector<int32_t> node_seq, node_seq_at;
+  for (const Node& N : tree.nodes) {
+    node_seq_at.push_back((int32_t)node_seq.size());
+    node_seq.insert(node_seq.end(), N.seqs.begin(), N.seqs.end());
+  }
+  int64_t part = 0;
+  bool join = false;
+  for (const Tile& t : tiles) {
+    const Node& N = tree.nodes[t.node];
+    const bool leaf = N.seqs.size() == 1, alone = leaf && tree.path[N.seqs[0]].size() == 1;
+    const int64_t keys = std::max<int64_t>(0, t.key1 - N.key0);
+    const int64_t cut = std::max<int64_t>(1, ceil_div(keys, chunk)), each = ceil_div(ceil_div(keys, 16), cut) * 16;
+    AttnSpan z{(int32_t)part, 0, t.rows, 0};
+    for (int64_t k = 0; k < keys || (alone && k == 0); k += std::max<int64_t>(each, 1)) {
+      const bool whole = alone && keys <= each;
+      AttnUnit u{b->seqs[N.seqs[0]], (int32_t)(N.key0 + k), (int32_t)std::max<int64_t>(0, std::min(each, keys - k)),
+                 leaf ? (int32_t)(N.key1 - most + 1) : kSeeAll, t.row0, t.rows, node_seq_at[t.node], whole ? -1 : (int32_t)part};
+      units.push_back(u);
+      if (whole) {
+        z.n = -1;
+        break;
+      }
+      ++z.n;
+      part += t.rows;
+    }
+    join |= z.n >= 0;
+    spans.push_back(z);
+  }
+  if (part * p->cfg.n_kv_heads > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_plan: too many partial rows");
+  std::vector<AttnSeq> seqs;
+  std::vector<AttnPath> paths;
+  for (int i = 0; i < n; ++i) {
+    seqs.push_back({(int32_t)paths.size(), (int32_t)tree.path[i].size(), b->count[i], 0});
+    join |= tree.path[i].empty();
+    for (int32_t x : tree.path[i]) {
+      const Node& N = tree.nodes[x];
+      paths.push_back({first_tile[x], kRowTile, (int32_t)(std::find(N.seqs.begin(), N.seqs.end(), i) - N.seqs.begin()), 0});
+    }
+  }
+  b->plan.clear();
+  b->off_unit = append(&b->plan, units);
+  b->off_seq = append(&b->plan, seqs);
+  b->off_path = append(&b->plan, paths);
+  b->off_span = append(&b->plan, spans);
+  b->off_node_seq = append(&b->plan, node_seq);
+  b->n_row_units = (int32_t)units.size();
+  b->join = join;
+  b->part_rows = part * p->cfg.n_kv_heads;
+  return INFLLM_OK;
+}
+
+}  // namespace
+
+int pages_encode_map(infllm_pages* p) {
+  (void)p;
+  return INFLLM_OK;
+}
+
+}  // namespace infllm
+
+using namespace infllm;
+
+extern "C" int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* plan_bytes, int64_t* scratch_bytes, int* fresh) {
+  return guarded("page_batch_plan", [&]() -> int {
+    INFLLM_TRY(batch_alive(b, "page_batch_plan"));
+    const infllm_pages* p = b->cache;
+    if (!plan_bytes || !scratch_bytes || !fresh) return fail(INFLLM_E_BADARG, "page_batch_plan: null pointer");
+    if (n_heads < 1 || n_heads % p->cfg.n_kv_heads) return fail(INFLLM_E_BADARG, "page_batch_plan: %d query heads over %d KV heads", n_heads, p->cfg.n_kv_heads);
+    if ((int64_t)b->most * n_heads * (int64_t)b->seqs.size() > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_plan: more than 2^31 query rows");
+    *fresh = b->plan_of != p->change || b->plan_heads != n_heads;
+    if (*fresh) {
+      for (size_t i = 0; i < b->seqs.size(); ++i)
+        if (b->count[i] > p->seqs[b->seqs[i]].length)
+          return fail(INFLLM_E_BADARG, "page_batch_plan: the newest %d tokens of sequence %d, which has %lld", b->count[i], b->seqs[i],
+                      (long long)p->seqs[b->seqs[i]].length);
+      b->plan_of = ~0ull;
+      INFLLM_TRY(make_plan(b, n_heads));
+      b->plan_of = p->change;
+      b->plan_heads = n_heads;
+    }
+    *plan_bytes = (int64_t)b->plan.size() * 4;
+    *scratch_bytes = b->part_rows * (p->cfg.head_dim + 4) * 4;
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const infllm_page_rows* q, void* d_out, float* d_lse, int n_heads,
+                                        float scale, void* d_plan, int upload, void* d_scratch, void* stream) {
+  return guarded("page_batch_attend", [&]() -> int {
+    INFLLM_TRY(batch_alive(b, "page_batch_attend"));
+    const infllm_pages* p = b->cache;
+    const infllm_pages_config& c = p->cfg;
+    if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_attend: a cache without a device");
+    if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_attend: layer %d of %d", layer, c.n_layers);
+    if (b->most == 0) return INFLLM_OK;
+    if (b->plan_of != p->change || b->plan_heads != n_heads) return fail(INFLLM_E_BADARG, "page_batch_attend: the plan is of another state of the cache");
+    if (!q || !q->d || !d_out || !d_plan || (b->part_rows > 0 && !d_scratch)) return fail(INFLLM_E_BADARG, "page_batch_attend: null pointer");
+    if (((uintptr_t)q->d | (uintptr_t)d_out | (uintptr_t)d_plan | (uintptr_t)d_scratch) % 16 || (q->bs | q->hs | q->ts) % 8)
+      return fail(INFLLM_E_BADARG, "page_batch_attend: rows must be 16-byte aligned");
+    DeviceScope scope(c.device);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (upload) INFLLM_CUDA_OK(cudaMemcpyAsync(d_plan, b->plan.data(), b->plan.size() * 4, cudaMemcpyHostToDevice, s));
+    PagedParams P;
+    P.plane = (int64_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim * 2;
+    P.pages = (const char*)c.d_pages + 2 * layer * P.plane;
+    P.table = c.d_table;
+    P.q = (const char*)q->d, P.q_bs = q->bs * 2, P.q_hs = q->hs * 2, P.q_ts = q->ts * 2;
+    P.out = (char*)d_out, P.lse = d_lse;
+    P.part_o = (float*)d_scratch, P.part_lse = P.part_o + b->part_rows * c.head_dim;
+    const int32_t* plan = (const int32_t*)d_plan;
+    P.unit = (const AttnUnit*)(plan + b->off_unit), P.seq = (const AttnSeq*)(plan + b->off_seq);
+    P.path = (const AttnPath*)(plan + b->off_path), P.span = (const AttnSpan*)(plan + b->off_span), P.node_seq = plan + b->off_node_seq;
+    P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.group = n_heads / c.n_kv_heads, P.most = b->most;
+    P.batch = (int)b->seqs.size();
+    P.scale_log2 = scale * kLog2e;
+    INFLLM_DISPATCH_DTYPE(c.dtype, T, {
+      if (b->n_row_units > 0) {
+        auto kern = c.head_dim == 128 ? paged_rows_kernel<T, 128, 2> : paged_rows_kernel<T, 64, 2>;
+        launch_chained(kern, dim3(b->n_row_units, c.n_kv_heads), dim3(kRowWarps * 32), 0, s, P);
+        INFLLM_LAUNCH_OK("paged_rows_kernel");
+      }
+      if (b->join) {
+        const int64_t rows = (int64_t)P.batch * P.most * n_heads;
+        launch_chained(c.head_dim == 128 ? paged_join_kernel<T, 128> : paged_join_kernel<T, 64>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, s, P);
+        INFLLM_LAUNCH_OK("paged_join_kernel");
+      }
+    });
+    return INFLLM_OK;
+  });
+}

@@ -1,0 +1,687 @@
+// A paged key/value cache: sequences of tokens in pages of a pool, several of which may share pages (the continuations of
+// one prompt).  Which pages a sequence has is known on the host, exactly and at once: what does not fit is refused before
+// anything changes, and a call's grid follows from sizes that the host has.  The device has a copy of the page table.
+//
+// Layout: a page of one layer holds its tokens' keys, (n_kv_heads, page_size, head_dim), and in another plane their values;
+// a page's plane is one stretch of memory, and so are the rows of one head.  Rows of a page that are in use are never
+// written again while two sequences share it: a sequence has its last page, where that is not full, to itself (fork copies
+// it; where truncation left it shared, it is copied before the next token is written).
+#include <algorithm>
+#include <cstring>
+
+#include "pages.cuh"
+
+namespace infllm {
+
+// ---------------------------------------------------------------------------------------------------------- changes
+// One kernel makes all changes of a call: items [0, n_rows) copy a row of the table (a: from row, b: to row, c: entries),
+// the next n_edits set entries (a: index, b: page, and c, d another one, index -1: none), the rest move tokens
+// (a: from page, b: to page, c: from place | to place << 16, d: tokens) in all layers, keys and values.
+// Pages that are written were free before the call and rows that are written belong to sequences that were not read from, so the order of the blocks does not matter.
+// It is bound by the bytes of the tokens that it moves, read and written once.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveAhead = 4;  // 16-byte loads of a thread in flight
+
+template <int kItems>
+struct PageChanges {
+  const char* from;  // the pools that tokens are moved from and to, of from_pages and to_pages pages
+  char* to;
+  int32_t* table;
+  int32_t n_rows, n_edits, max_pages, parts;  // parts: blocks of a move
+  int32_t planes, from_pages, to_pages, n_kv, page, dim16;  // dim16: 16-byte pieces of a row
+  PageItem item[kItems];
+};
+
+template <int kItems>
+__global__ void __launch_bounds__(kMoveThreads) page_change_kernel(const __grid_constant__ PageChanges<kItems> P) {
+  int b = blockIdx.x;
+  if (b < P.n_rows) {
+    const PageItem it = P.item[b];
+    const int32_t* from = P.table + (int64_t)it.a * P.max_pages;
+    int32_t* to = P.table + (int64_t)it.b * P.max_pages;
+    for (int i = threadIdx.x; i < it.c; i += kMoveThreads) to[i] = from[i];
+    return;
+  }
+  b -= P.n_rows;
+  if (P.n_edits > 0 && b-- == 0) {
+    for (int i = threadIdx.x; i < P.n_edits; i += kMoveThreads) {
+      const PageItem it = P.item[P.n_rows + i];
+      P.table[it.a] = it.b;
+      if (it.c >= 0) P.table[it.c] = it.d;
+    }
+    return;
+  }
+  const PageItem it = P.item[P.n_rows + P.n_edits + b / P.parts];
+  const int part = b % P.parts;
+  const int from = it.c & 0xffff, to = it.c >> 16;
+  // 16-byte pieces of the move: (plane, head, token, piece); rows of a head are one stretch on both sides
+  const int strip = it.d * P.dim16;
+  const uint32_t total = (uint32_t)P.planes * P.n_kv * strip;
+  const uint32_t share = (total + P.parts - 1) / P.parts, end = min(total, (part + 1) * share);
+  const uint4* src = reinterpret_cast<const uint4*>(P.from);
+  uint4* dst = reinterpret_cast<uint4*>(P.to);
+  const int head = P.page * P.dim16;  // pieces of a head's rows of a page
+  for (uint32_t i = part * share + threadIdx.x; i < end; i += kMoveThreads * kMoveAhead) {
+    uint4 v[kMoveAhead];
+    int64_t at[kMoveAhead];
+#pragma unroll
+    for (int k = 0; k < kMoveAhead; ++k) {
+      const uint32_t j = i + k * kMoveThreads;
+      if (j >= end) continue;
+      const uint32_t s = j / strip, r = j - s * strip, plane = s / P.n_kv, h = s - plane * P.n_kv;
+      v[k] = src[(((int64_t)plane * P.from_pages + it.a) * P.n_kv + h) * head + from * P.dim16 + r];
+      at[k] = (((int64_t)plane * P.to_pages + it.b) * P.n_kv + h) * head + to * P.dim16 + r;
+    }
+#pragma unroll
+    for (int k = 0; k < kMoveAhead; ++k)
+      if (i + k * kMoveThreads < end) dst[at[k]] = v[k];
+  }
+}
+
+template <int kItems>
+static int launch_changes(infllm_pages* p, const infllm_pages* from, size_t r0, size_t r1, size_t e0, size_t e1, size_t m0, size_t m1, cudaStream_t s) {
+  const infllm_pages_config& c = p->cfg;
+  const int n_moves = (int)(m1 - m0);
+  PageChanges<kItems> P;
+  P.from = (const char*)from->cfg.d_pages, P.to = (char*)c.d_pages;
+  P.table = c.d_table;
+  P.n_rows = (int)(r1 - r0), P.n_edits = (int)(e1 - e0), P.max_pages = c.max_pages;
+  P.planes = 2 * c.n_layers, P.from_pages = from->cfg.n_pages, P.to_pages = c.n_pages;
+  P.n_kv = c.n_kv_heads, P.page = c.page_size, P.dim16 = c.head_dim / 8;
+  if (r1 > r0) memcpy(P.item, &p->rows[r0], (r1 - r0) * sizeof(PageItem));
+  if (e1 > e0) memcpy(P.item + P.n_rows, &p->edits[e0], (e1 - e0) * sizeof(PageItem));
+  if (m1 > m0) memcpy(P.item + P.n_rows + P.n_edits, &p->moves[m0], (m1 - m0) * sizeof(PageItem));
+  // blocks of a move: two rounds of a block's loads each
+  int32_t most = 0;
+  for (size_t i = m0; i < m1; ++i) most = std::max(most, p->moves[i].d);
+  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div((int64_t)P.planes * P.n_kv * most * P.dim16, 2 * kMoveThreads * kMoveAhead), 65535));
+  const int64_t blocks = P.n_rows + (P.n_edits > 0) + (int64_t)n_moves * P.parts;
+  page_change_kernel<kItems><<<(unsigned)blocks, kMoveThreads, 0, s>>>(P);
+  INFLLM_LAUNCH_OK("page_change_kernel");
+  return INFLLM_OK;
+}
+
+// makes the changes that a call has listed; tokens are moved from the pages of `from`
+static int flush(infllm_pages* p, const infllm_pages* from, cudaStream_t s) {
+  constexpr size_t kSmall = 60, kLarge = 1000;  // of 16 bytes each: a kernel's arguments, up to 4 KB and up to 32
+  int rc = INFLLM_OK;
+  if (p->cfg.device >= 0) {
+    size_t r = 0, e = 0, m = 0;
+    while (rc == INFLLM_OK && r + e + m < p->rows.size() + p->edits.size() + p->moves.size()) {
+      const size_t left = p->rows.size() + p->edits.size() + p->moves.size() - r - e - m;
+      size_t room = left <= kSmall ? kSmall : kLarge;
+      const size_t r1 = std::min(p->rows.size(), r + room);
+      room -= r1 - r;
+      const size_t e1 = std::min(p->edits.size(), e + room);
+      room -= e1 - e;
+      const size_t m1 = std::min(p->moves.size(), m + room);
+      rc = left <= kSmall ? launch_changes<kSmall>(p, from, r, r1, e, e1, m, m1, s)
+                          : launch_changes<kLarge>(p, from, r, r1, e, e1, m, m1, s);
+      r = r1, e = e1, m = m1;
+    }
+  }
+  p->rows.clear();
+  p->edits.clear();
+  p->moves.clear();
+  return rc;
+}
+
+// ------------------------------------------------------------------------------------------------------ bookkeeping
+static int check_seqs(const infllm_pages* p, const int32_t* seqs, int n, const char* what) {
+  if (!p || n < 0 || (n > 0 && !seqs)) return fail(INFLLM_E_BADARG, "%s: null pointer or a negative count", what);
+  for (int i = 0; i < n; ++i)
+    if (seqs[i] < 0 || seqs[i] >= (int)p->seqs.size() || !p->seqs[seqs[i]].open)
+      return fail(INFLLM_E_BADARG, "%s: %d is not a sequence of this cache", what, seqs[i]);
+  return INFLLM_OK;
+}
+
+static int check_once(const infllm_pages* p, const int32_t* seqs, int n, const char* what) {
+  INFLLM_TRY(check_seqs(p, seqs, n, what));
+  std::vector<char> seen(p->seqs.size(), 0);
+  for (int i = 0; i < n; ++i)
+    if (seen[seqs[i]]++) return fail(INFLLM_E_BADARG, "%s: sequence %d is named twice", what, seqs[i]);
+  return INFLLM_OK;
+}
+
+static int32_t take_page(infllm_pages* p) {
+  const int32_t page = p->free_pages.top();
+  p->free_pages.pop();
+  p->uses[page] = 1;
+  return page;
+}
+
+static void drop_page(infllm_pages* p, int32_t page) {
+  if (--p->uses[page] == 0) p->free_pages.push(page);
+}
+
+static void set_entry(infllm_pages* p, int32_t row, size_t at, int32_t page) {
+  const int32_t index = row * p->cfg.max_pages + (int32_t)at;
+  if (!p->edits.empty() && p->edits.back().c < 0) p->edits.back().c = index, p->edits.back().d = page;
+  else p->edits.push_back({index, page, -1, 0});
+}
+
+static void move_tokens(infllm_pages* p, int32_t from, int32_t from_at, int32_t to, int32_t to_at, int32_t n) {
+  p->moves.push_back({from, to, from_at | to_at << 16, n});
+}
+
+static int need_pages(const infllm_pages* p, int64_t n, const char* what) {
+  if (n > (int64_t)p->free_pages.size())
+    return fail(INFLLM_E_CAPACITY, "%s: %lld pages are needed, %zu of %d are free", what, (long long)n, p->free_pages.size(), p->cfg.n_pages);
+  return INFLLM_OK;
+}
+
+// the lowest numbers that no sequence has
+static int need_seqs(const infllm_pages* p, int64_t n, std::vector<int32_t>* out, const char* what) {
+  for (size_t i = 0; i < p->seqs.size() && (int64_t)out->size() < n; ++i)
+    if (!p->seqs[i].open) out->push_back((int32_t)i);
+  if ((int64_t)out->size() < n)
+    return fail(INFLLM_E_CAPACITY, "%s: %lld new sequences, and room for %zu", what, (long long)n, out->size());
+  return INFLLM_OK;
+}
+
+static void open_seq(infllm_pages* p, int32_t seq) {
+  PageSeq& s = p->seqs[seq];
+  s.open = true;
+  ++s.generation;
+  s.length = s.position = 0;
+}
+
+static void cut(infllm_pages* p, int32_t seq, int64_t length) {
+  PageSeq& s = p->seqs[seq];
+  s.position -= s.length - length;
+  s.length = length;
+  const size_t left = (size_t)p->pages_of(length);
+  while (s.pages.size() > left) {
+    drop_page(p, s.pages.back());
+    s.pages.pop_back();
+  }
+}
+
+// room for count[i] more tokens of each sequence
+static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* count, int n, const char* what) {
+  const int page = p->cfg.page_size;
+  int64_t need = 0;
+  for (int i = 0; i < n; ++i) {
+    const PageSeq& s = p->seqs[seqs[i]];
+    if (count[i] < 0) return fail(INFLLM_E_BADARG, "%s: %d tokens", what, count[i]);
+    if (s.length + count[i] > (int64_t)p->cfg.max_pages * page)
+      return fail(INFLLM_E_CAPACITY, "%s: sequence %d would have %lld tokens, and rows of the page table are for %lld", what, seqs[i],
+                  (long long)(s.length + count[i]), (long long)p->cfg.max_pages * page);
+    if (s.position + count[i] > INT32_MAX) return fail(INFLLM_E_CAPACITY, "%s: positions beyond 31 bits", what);
+    need += p->pages_of(s.length + count[i]) - (int64_t)s.pages.size();
+    // (as many as would be copied if each of several that share their last page had to: the last one may keep it)
+    if (count[i] > 0 && s.length % page && p->uses[s.pages.back()] > 1) ++need;
+  }
+  INFLLM_TRY(need_pages(p, need, what));
+  ++p->change;
+  for (int i = 0; i < n; ++i) {
+    PageSeq& s = p->seqs[seqs[i]];
+    if (count[i] > 0 && s.length % page && p->uses[s.pages.back()] > 1) {
+      const int32_t old = s.pages.back();
+      s.pages.back() = take_page(p);
+      set_entry(p, seqs[i], s.pages.size() - 1, s.pages.back());
+      move_tokens(p, old, 0, s.pages.back(), 0, (int32_t)(s.length % page));
+      drop_page(p, old);  // (another one has it still)
+      ++p->reshape;
+    }
+    s.length += count[i];
+    s.position += count[i];
+    const size_t want = (size_t)p->pages_of(s.length);
+    while (s.pages.size() < want) {
+      s.pages.push_back(take_page(p));
+      set_entry(p, seqs[i], s.pages.size() - 1, s.pages.back());
+    }
+  }
+  return INFLLM_OK;
+}
+
+int batch_alive(const infllm_page_batch* b, const char* what) {
+  if (!b) return fail(INFLLM_E_BADARG, "%s: null pointer", what);
+  for (size_t i = 0; i < b->seqs.size(); ++i) {
+    const PageSeq& s = b->cache->seqs[b->seqs[i]];
+    if (!s.open || s.generation != b->generation[i]) return fail(INFLLM_E_BADARG, "%s: sequence %d of the batch has been freed", what, b->seqs[i]);
+  }
+  return INFLLM_OK;
+}
+
+// ------------------------------------------------------------------------------------------------------------ writes
+// New tokens' keys and values into their pages, keys and queries rotated to the tokens' positions on the way.  A block has
+// a token; a thread has 8 dimensions of the first half of a row and the 8 that go with them in the second, so that it needs
+// one stretch of the tables for all its rows, and keeps it.  Bound by the bytes of q, k and v, read and written once.
+constexpr int kWriteThreads = 256;
+constexpr int kWriteSeqs = 128;  // of a launch
+
+struct WriteParams {
+  const char *k, *v, *q;
+  char* q_out;                                      // (B, L, n_heads, dim)
+  int64_t k_bs, k_hs, k_ts, v_bs, v_hs, v_ts, q_bs, q_hs, q_ts;  // bytes
+  char* pages;                                      // of the layer
+  const int32_t* table;
+  const float *cos_t, *sin_t;                       // null: nothing is rotated
+  int64_t plane;                                    // bytes from keys to values
+  int32_t max_pages, page, n_kv, n_heads, most, b0, pad;
+  BatchSeq seq[kWriteSeqs];
+};
+
+template <typename T, int kDim, bool kRope>
+__device__ __forceinline__ void rotate8(uint4& lo, uint4& hi, const float* cs, const float* sn) {
+  T *a = reinterpret_cast<T*>(&lo), *b = reinterpret_cast<T*>(&hi);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // each product rounded to fp32 first, and the sum to 16 bits: as the rotary embedding of the other attention types
+    const float x1 = Act<T>::to_f(a[i]), x2 = Act<T>::to_f(b[i]);
+    a[i] = Act<T>::from_f(__fadd_rn(__fmul_rn(x1, cs[i]), __fmul_rn(-x2, sn[i])));
+    b[i] = Act<T>::from_f(__fadd_rn(__fmul_rn(x2, cs[i]), __fmul_rn(x1, sn[i])));
+  }
+}
+
+template <typename T, int kDim, bool kRope>
+__global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const __grid_constant__ WriteParams P) {
+  constexpr int kPer = kDim / 16;  // threads of a row
+  const int i = blockIdx.x % P.most, b = blockIdx.x / P.most;
+  const BatchSeq S = P.seq[b];
+  const int at = i - (P.most - S.count);  // of the new tokens (the shorter sequences' stand at the end)
+  const int c = threadIdx.x % kPer, n_rows = P.n_heads + 2 * P.n_kv;
+  const int64_t bb = P.b0 + b;
+  float cs[8], sn[8];
+  if (kRope && at >= 0) {
+    const int64_t o = (int64_t)(S.position + at) * (kDim / 2) + c * 8;
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      *reinterpret_cast<float4*>(cs + k) = __ldg(reinterpret_cast<const float4*>(P.cos_t + o + k));
+      *reinterpret_cast<float4*>(sn + k) = __ldg(reinterpret_cast<const float4*>(P.sin_t + o + k));
+    }
+  }
+  const int place = S.length - S.count + at;
+  char* const page_at = at >= 0 ? P.pages + ((int64_t)__ldg(P.table + (int64_t)S.row * P.max_pages + place / P.page) * P.n_kv * P.page + place % P.page) * kDim * 2
+                                : nullptr;
+  for (int r = threadIdx.x / kPer; r < n_rows; r += kWriteThreads / kPer) {
+    const char* src;
+    char* dst;
+    bool turn = kRope;
+    if (r < P.n_heads) {
+      src = P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts;
+      dst = P.q_out + ((bb * P.most + i) * P.n_heads + r) * (int64_t)(kDim * 2);
+    } else {
+      const bool val = r >= P.n_heads + P.n_kv;
+      const int h = r - P.n_heads - (val ? P.n_kv : 0);
+      src = val ? P.v + bb * P.v_bs + h * P.v_hs + i * P.v_ts : P.k + bb * P.k_bs + h * P.k_hs + i * P.k_ts;
+      dst = page_at + (int64_t)h * P.page * kDim * 2 + (val ? P.plane : 0);
+      turn = kRope && !val;
+      if (at < 0) continue;
+    }
+    uint4 lo = *reinterpret_cast<const uint4*>(src + c * 16), hi = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
+    if (r < P.n_heads && at < 0) lo = hi = make_uint4(0, 0, 0, 0);  // (no token: its query is not one)
+    else if (turn) rotate8<T, kDim, kRope>(lo, hi, cs, sn);
+    *reinterpret_cast<uint4*>(dst + c * 16) = lo;
+    *reinterpret_cast<uint4*>(dst + kDim + c * 16) = hi;
+  }
+}
+
+}  // namespace infllm
+
+// ------------------------------------------------------------------------------------------------------- entry points
+using namespace infllm;
+
+extern "C" int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages** out) {
+  return guarded("pages_create", [&]() -> int {
+    if (!cfg || !out) return fail(INFLLM_E_BADARG, "pages_create: null pointer");
+    const infllm_pages_config& c = *cfg;
+    if (c.n_layers < 1 || c.n_kv_heads < 1 || c.n_pages < 1 || c.max_sequences < 1 || c.max_pages < 1)
+      return fail(INFLLM_E_BADARG, "pages_create: %d layers, %d KV heads, %d pages, %d sequences of %d pages", c.n_layers, c.n_kv_heads,
+                  c.n_pages, c.max_sequences, c.max_pages);
+    if (c.head_dim != 64 && c.head_dim != 128) return fail(INFLLM_E_UNSUPPORTED, "pages_create: head_dim %d (64 and 128 are built)", c.head_dim);
+    if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128)
+      return fail(INFLLM_E_UNSUPPORTED, "pages_create: pages of %d tokens (16, 32, 64 or 128)", c.page_size);
+    if (c.dtype != INFLLM_BF16 && c.dtype != INFLLM_FP16) return fail(INFLLM_E_UNSUPPORTED, "dtype code %d", c.dtype);
+    if ((int64_t)c.max_sequences * c.max_pages > INT32_MAX || (int64_t)c.n_layers * 2 * c.n_pages > INT32_MAX ||
+        (int64_t)c.n_layers * 2 * c.n_kv_heads * c.page_size * 16 > INT32_MAX || (int64_t)c.max_pages * c.page_size > INT32_MAX)
+      return fail(INFLLM_E_BADARG, "pages_create: a page table or a pool beyond 31 bits");
+    if (c.device >= 0 && (!c.d_pages || !c.d_table || (uintptr_t)c.d_pages % 16 || (uintptr_t)c.d_table % 4))
+      return fail(INFLLM_E_BADARG, "pages_create: the pool has to be 16-byte aligned");
+    infllm_pages* p = new infllm_pages();
+    p->cfg = c;
+    int rc = guarded("pages_create", [&]() -> int {
+      p->seqs.resize(c.max_sequences);
+      p->uses.resize(c.n_pages, 0);
+      std::vector<int32_t> all(c.n_pages);
+      for (int32_t i = 0; i < c.n_pages; ++i) all[i] = i;
+      p->free_pages = decltype(p->free_pages)(std::greater<int32_t>(), std::move(all));
+      DeviceScope scope(c.device);
+      if (!scope.ok()) return fail(INFLLM_E_CUDA, "pages_create: no device %d", c.device);
+      return c.device >= 0 ? pages_encode_map(p) : INFLLM_OK;
+    });
+    if (rc != INFLLM_OK) {
+      delete p;
+      return rc;
+    }
+    *out = p;
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_pages_destroy(infllm_pages* p) {
+  delete p;
+  return INFLLM_OK;
+}
+
+extern "C" int infllm_pages_open(infllm_pages* p, int n, int32_t* out) {
+  return guarded("pages_open", [&]() -> int {
+    if (!p || n < 0 || (n > 0 && !out)) return fail(INFLLM_E_BADARG, "pages_open: null pointer or a negative count");
+    std::vector<int32_t> got;
+    INFLLM_TRY(need_seqs(p, n, &got, "pages_open"));
+    for (int i = 0; i < n; ++i) open_seq(p, out[i] = got[i]);
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_pages_fork(infllm_pages* p, const int32_t* seqs, int n, int n_each, int32_t* out, void* stream) {
+  return guarded("pages_fork", [&]() -> int {
+    INFLLM_TRY(check_seqs(p, seqs, n, "pages_fork"));
+    if (n_each < 0 || ((int64_t)n * n_each > 0 && !out)) return fail(INFLLM_E_BADARG, "pages_fork: null pointer or a negative count");
+    std::vector<int32_t> got;
+    INFLLM_TRY(need_seqs(p, (int64_t)n * n_each, &got, "pages_fork"));
+    const int page = p->cfg.page_size;
+    int64_t need = 0;
+    for (int i = 0; i < n; ++i) need += p->seqs[seqs[i]].length % page ? n_each : 0;
+    INFLLM_TRY(need_pages(p, need, "pages_fork"));
+    DeviceScope scope(p->cfg.device);
+    ++p->change;
+    int at = 0;
+    for (int i = 0; i < n; ++i) {
+      const PageSeq& s = p->seqs[seqs[i]];
+      const int32_t full = (int32_t)(s.length / page);
+      for (int j = 0; j < n_each; ++j, ++at) {
+        open_seq(p, got[at]);
+        PageSeq& c = p->seqs[got[at]];
+        c.length = s.length, c.position = s.position;
+        c.pages.assign(s.pages.begin(), s.pages.begin() + full);
+        if (full) p->rows.push_back({seqs[i], got[at], full, 0});
+        if (s.length % page) {
+          c.pages.push_back(take_page(p));
+          set_entry(p, got[at], full, c.pages.back());
+          move_tokens(p, s.pages[full], 0, c.pages.back(), 0, page);
+        }
+      }
+      for (int32_t k = 0; k < full; ++k) p->uses[s.pages[k]] += n_each;
+    }
+    std::copy(got.begin(), got.end(), out);
+    return flush(p, p, (cudaStream_t)stream);
+  });
+}
+
+extern "C" int infllm_pages_copy(infllm_pages* p, const int32_t* seqs, int n, infllm_pages* into, int32_t* out, void* stream) {
+  return guarded("pages_copy", [&]() -> int {
+    INFLLM_TRY(check_seqs(p, seqs, n, "pages_copy"));
+    if (!into || (n > 0 && !out)) return fail(INFLLM_E_BADARG, "pages_copy: null pointer");
+    const infllm_pages_config &a = p->cfg, &b = into->cfg;
+    if (a.n_layers != b.n_layers || a.n_kv_heads != b.n_kv_heads || a.head_dim != b.head_dim || a.page_size != b.page_size || a.dtype != b.dtype || a.device != b.device)
+      return fail(INFLLM_E_BADARG, "pages_copy: the caches' pages or devices differ");
+    std::vector<int32_t> got;
+    INFLLM_TRY(need_seqs(into, n, &got, "pages_copy"));
+    int64_t need = 0;
+    for (int i = 0; i < n; ++i) {
+      const int64_t m = (int64_t)p->seqs[seqs[i]].pages.size();
+      if (m > b.max_pages) return fail(INFLLM_E_CAPACITY, "pages_copy: sequence %d has %lld pages, and rows of the page table are for %d", seqs[i], (long long)m, b.max_pages);
+      need += m;
+    }
+    INFLLM_TRY(need_pages(into, need, "pages_copy"));
+    DeviceScope scope(b.device);
+    ++into->change;
+    for (int i = 0; i < n; ++i) {
+      const PageSeq& s = p->seqs[seqs[i]];
+      open_seq(into, got[i]);
+      PageSeq& c = into->seqs[got[i]];
+      c.length = s.length, c.position = s.position;
+      for (size_t k = 0; k < s.pages.size(); ++k) {
+        c.pages.push_back(take_page(into));
+        set_entry(into, got[i], k, c.pages.back());
+        move_tokens(into, s.pages[k], 0, c.pages.back(), 0, (int32_t)std::min<int64_t>(a.page_size, s.length - (int64_t)k * a.page_size));
+      }
+    }
+    std::copy(got.begin(), got.end(), out);
+    return flush(into, p, (cudaStream_t)stream);
+  });
+}
+
+extern "C" int infllm_pages_truncate(infllm_pages* p, const int32_t* seqs, const int64_t* lengths, int n) {
+  return guarded("pages_truncate", [&]() -> int {
+    INFLLM_TRY(check_once(p, seqs, n, "pages_truncate"));
+    if (n > 0 && !lengths) return fail(INFLLM_E_BADARG, "pages_truncate: null pointer");
+    for (int i = 0; i < n; ++i)
+      if (lengths[i] < 0 || lengths[i] > p->seqs[seqs[i]].length)
+        return fail(INFLLM_E_BADARG, "pages_truncate: %lld of the %lld tokens of sequence %d", (long long)lengths[i],
+                    (long long)p->seqs[seqs[i]].length, seqs[i]);
+    ++p->change, ++p->reshape;
+    for (int i = 0; i < n; ++i) cut(p, seqs[i], lengths[i]);
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_pages_free(infllm_pages* p, const int32_t* seqs, int n) {
+  return guarded("pages_free", [&]() -> int {
+    INFLLM_TRY(check_once(p, seqs, n, "pages_free"));
+    ++p->change, ++p->reshape;
+    for (int i = 0; i < n; ++i) {
+      cut(p, seqs[i], 0);
+      p->seqs[seqs[i]].open = false;
+    }
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n, const int64_t* spans, const int32_t* n_spans, void* stream) {
+  return guarded("pages_compact", [&]() -> int {
+    INFLLM_TRY(check_once(p, seqs, n, "pages_compact"));
+    if (n > 0 && !n_spans) return fail(INFLLM_E_BADARG, "pages_compact: null pointer");
+    const int page = p->cfg.page_size;
+    struct Kept {
+      int64_t length;
+      int32_t stay;  // pages at the front of which every token stays where it is
+    };
+    std::vector<Kept> kept(n);
+    int64_t need = 0;
+    const int64_t* span = spans;
+    for (int i = 0; i < n; ++i) {
+      if (n_spans[i] < 0 || (n_spans[i] > 0 && !spans)) return fail(INFLLM_E_BADARG, "pages_compact: null pointer or a negative count");
+      int64_t at = 0, same = 0, total = 0;
+      for (int k = 0; k < n_spans[i]; ++k, span += 2) {
+        if (span[0] < at || span[1] < span[0] || span[1] > p->seqs[seqs[i]].length)
+          return fail(INFLLM_E_BADARG, "pages_compact: [%lld, %lld) behind %lld, of the %lld tokens of sequence %d", (long long)span[0],
+                      (long long)span[1], (long long)at, (long long)p->seqs[seqs[i]].length, seqs[i]);
+        if (span[0] == total) same = total + span[1] - span[0];  // (nothing has been left out so far)
+        total += span[1] - span[0];
+        at = span[1];
+      }
+      kept[i] = {total, (int32_t)(same / page)};
+      need += p->pages_of(total) - kept[i].stay;
+    }
+    INFLLM_TRY(need_pages(p, need, "pages_compact"));
+    DeviceScope scope(p->cfg.device);
+    ++p->change, ++p->reshape;
+    std::vector<int32_t> gone;
+    span = spans;
+    for (int i = 0; i < n; ++i) {
+      PageSeq& s = p->seqs[seqs[i]];
+      const int32_t stay = kept[i].stay;
+      std::vector<int32_t> now(s.pages.begin(), s.pages.begin() + stay);
+      while ((int64_t)now.size() < p->pages_of(kept[i].length)) {
+        now.push_back(take_page(p));
+        set_entry(p, seqs[i], now.size() - 1, now.back());
+      }
+      int64_t to = 0;
+      for (int k = 0; k < n_spans[i]; ++k, span += 2) {
+        int64_t from = span[0];
+        while (from < span[1]) {  // up to the end of a page on either side
+          const int64_t m = std::min({span[1] - from, page - from % page, page - to % page});
+          if (to / page >= stay)
+            move_tokens(p, s.pages[from / page], (int32_t)(from % page), now[to / page], (int32_t)(to % page), (int32_t)m);
+          from += m, to += m;
+        }
+      }
+      gone.insert(gone.end(), s.pages.begin() + stay, s.pages.end());
+      s.pages = std::move(now);
+      s.length = kept[i].length;
+    }
+    // (only now: what one sequence leaves must not be taken by the next while it is still to be read)
+    for (int32_t g : gone) drop_page(p, g);
+    return flush(p, p, (cudaStream_t)stream);
+  });
+}
+
+extern "C" int infllm_pages_info(const infllm_pages* p, int32_t seq, int64_t* length, int64_t* position) {
+  INFLLM_TRY(check_seqs(p, &seq, 1, "pages_info"));
+  if (length) *length = p->seqs[seq].length;
+  if (position) *position = p->seqs[seq].position;
+  return INFLLM_OK;
+}
+
+extern "C" int infllm_pages_row(const infllm_pages* p, int32_t seq, int32_t* out, int cap, int* n) {
+  INFLLM_TRY(check_seqs(p, &seq, 1, "pages_row"));
+  if (!n || cap < 0 || (cap > 0 && !out)) return fail(INFLLM_E_BADARG, "pages_row: null pointer");
+  const std::vector<int32_t>& row = p->seqs[seq].pages;
+  *n = (int)row.size();
+  std::copy(row.begin(), row.begin() + std::min<size_t>(row.size(), (size_t)cap), out);
+  return INFLLM_OK;
+}
+
+extern "C" int infllm_pages_free_count(const infllm_pages* p) { return p ? (int)p->free_pages.size() : fail(INFLLM_E_BADARG, "pages_free_count: null pointer"); }
+
+extern "C" int infllm_page_batch_create(infllm_pages* p, const int32_t* seqs, int n, infllm_page_batch** out) {
+  return guarded("page_batch_create", [&]() -> int {
+    if (!out) return fail(INFLLM_E_BADARG, "page_batch_create: null pointer");
+    INFLLM_TRY(check_once(p, seqs, n, "page_batch_create"));
+    if (n < 1) return fail(INFLLM_E_BADARG, "page_batch_create: no sequences");
+    infllm_page_batch* b = new infllm_page_batch();
+    int rc = guarded("page_batch_create", [&]() -> int {
+      b->cache = p;
+      b->seqs.assign(seqs, seqs + n);
+      b->count.assign(n, 0);
+      for (int i = 0; i < n; ++i) b->generation.push_back(p->seqs[seqs[i]].generation);
+      return INFLLM_OK;
+    });
+    if (rc != INFLLM_OK) {
+      delete b;
+      return rc;
+    }
+    *out = b;
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_page_batch_destroy(infllm_page_batch* b) {
+  delete b;
+  return INFLLM_OK;
+}
+
+static void set_counts(infllm_page_batch* b, const int32_t* counts) {
+  b->most = 0;
+  for (size_t i = 0; i < b->seqs.size(); ++i) {
+    b->count[i] = counts[i];
+    b->most = std::max(b->most, counts[i]);
+  }
+  b->plan_of = ~0ull;
+}
+
+extern "C" int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* counts, void* stream) {
+  return guarded("page_batch_extend", [&]() -> int {
+    INFLLM_TRY(batch_alive(b, "page_batch_extend"));
+    if (!counts) return fail(INFLLM_E_BADARG, "page_batch_extend: null pointer");
+    DeviceScope scope(b->cache->cfg.device);
+    INFLLM_TRY(extend(b->cache, b->seqs.data(), counts, (int)b->seqs.size(), "page_batch_extend"));
+    set_counts(b, counts);
+    return flush(b->cache, b->cache, (cudaStream_t)stream);
+  });
+}
+
+extern "C" int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* counts) {
+  return guarded("page_batch_retract", [&]() -> int {
+    INFLLM_TRY(batch_alive(b, "page_batch_retract"));
+    if (!counts) return fail(INFLLM_E_BADARG, "page_batch_retract: null pointer");
+    infllm_pages* p = b->cache;
+    for (size_t i = 0; i < b->seqs.size(); ++i)
+      if (counts[i] < 0 || counts[i] > p->seqs[b->seqs[i]].length)
+        return fail(INFLLM_E_BADARG, "page_batch_retract: %d of the %lld tokens of sequence %d", counts[i],
+                    (long long)p->seqs[b->seqs[i]].length, b->seqs[i]);
+    ++p->change, ++p->reshape;
+    for (size_t i = 0; i < b->seqs.size(); ++i) cut(p, b->seqs[i], p->seqs[b->seqs[i]].length - counts[i]);
+    set_counts(b, std::vector<int32_t>(b->seqs.size(), 0).data());
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int infllm_page_batch_select(infllm_page_batch* b, const int32_t* counts) {
+  return guarded("page_batch_select", [&]() -> int {
+    INFLLM_TRY(batch_alive(b, "page_batch_select"));
+    if (!counts) return fail(INFLLM_E_BADARG, "page_batch_select: null pointer");
+    for (size_t i = 0; i < b->seqs.size(); ++i)
+      if (counts[i] < 0 || counts[i] > b->cache->seqs[b->seqs[i]].length)
+        return fail(INFLLM_E_BADARG, "page_batch_select: the newest %d of the %lld tokens of sequence %d", counts[i],
+                    (long long)b->cache->seqs[b->seqs[i]].length, b->seqs[i]);
+    set_counts(b, counts);
+    return INFLLM_OK;
+  });
+}
+
+extern "C" int64_t infllm_page_batch_reach(const infllm_page_batch* b) {
+  INFLLM_TRY(batch_alive(b, "page_batch_reach"));
+  int64_t most = 0;
+  for (int32_t s : b->seqs) most = std::max(most, b->cache->seqs[s].position);
+  return most;
+}
+
+extern "C" int infllm_page_batch_write(infllm_page_batch* b, int layer, const infllm_page_rows* k, const infllm_page_rows* v,
+                                       const infllm_page_rows* q, void* d_q_out, int n_heads, const float* d_cos, const float* d_sin,
+                                       int64_t table_len, void* stream) {
+  return guarded("page_batch_write", [&]() -> int {
+    INFLLM_TRY(batch_alive(b, "page_batch_write"));
+    const infllm_pages_config& c = b->cache->cfg;
+    if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_write: a cache without a device");
+    if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_write: layer %d of %d", layer, c.n_layers);
+    if (!k || !v || !k->d || !v->d || (q && (!q->d || !d_q_out || n_heads < 1)) || (!d_cos) != (!d_sin))
+      return fail(INFLLM_E_BADARG, "page_batch_write: null pointer");
+    const infllm_page_rows* all[3] = {k, v, q};
+    for (const infllm_page_rows* r : all)
+      if (r && ((uintptr_t)r->d % 16 || (r->bs | r->hs | r->ts) % 8)) return fail(INFLLM_E_BADARG, "page_batch_write: rows must be 16-byte aligned");
+    if (q && (uintptr_t)d_q_out % 16) return fail(INFLLM_E_BADARG, "page_batch_write: rows must be 16-byte aligned");
+    if (b->most == 0) return INFLLM_OK;
+    DeviceScope scope(c.device);
+    WriteParams P;
+    P.k = (const char*)k->d, P.v = (const char*)v->d, P.q = q ? (const char*)q->d : nullptr;
+    P.q_out = (char*)d_q_out;
+    P.k_bs = k->bs * 2, P.k_hs = k->hs * 2, P.k_ts = k->ts * 2;
+    P.v_bs = v->bs * 2, P.v_hs = v->hs * 2, P.v_ts = v->ts * 2;
+    P.q_bs = q ? q->bs * 2 : 0, P.q_hs = q ? q->hs * 2 : 0, P.q_ts = q ? q->ts * 2 : 0;
+    P.plane = (int64_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim * 2;
+    P.pages = (char*)c.d_pages + 2 * layer * P.plane;
+    P.table = c.d_table;
+    P.cos_t = d_cos, P.sin_t = d_sin;
+    P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.n_heads = q ? n_heads : 0, P.most = b->most;
+    const int n = (int)b->seqs.size();
+    for (int i = 0; i < n; ++i) {
+      const PageSeq& s = b->cache->seqs[b->seqs[i]];
+      if (d_cos && s.position > table_len) return fail(INFLLM_E_BADARG, "page_batch_write: a rotary table of %lld rows, position %lld", (long long)table_len, (long long)s.position - 1);
+      // pages that another sequence has too are not written: a batch that was cut back and selected again is not extended
+      if (b->count[i] > 0)
+        for (int64_t g = (s.length - b->count[i]) / c.page_size; g < (int64_t)s.pages.size(); ++g)
+          if (b->cache->uses[s.pages[g]] > 1) return fail(INFLLM_E_BADARG, "page_batch_write: sequence %d shares the pages of the tokens to be written", b->seqs[i]);
+    }
+    for (P.b0 = 0; P.b0 < n; P.b0 += kWriteSeqs) {
+      const int m = std::min(n - P.b0, kWriteSeqs);
+      for (int i = 0; i < m; ++i) {
+        const int e = P.b0 + i;
+        const PageSeq& s = b->cache->seqs[b->seqs[e]];
+        P.seq[i] = {b->seqs[e], (int32_t)s.length, b->count[e], (int32_t)(s.position - b->count[e])};
+      }
+      const int64_t blocks = (int64_t)m * b->most;
+      if (blocks > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_write: %lld tokens", (long long)blocks);
+      INFLLM_DISPATCH_DTYPE(c.dtype, T, {
+        auto kern = c.head_dim == 128 ? (d_cos ? page_write_kernel<T, 128, true> : page_write_kernel<T, 128, false>)
+                                      : (d_cos ? page_write_kernel<T, 64, true> : page_write_kernel<T, 64, false>);
+        kern<<<(unsigned)blocks, kWriteThreads, 0, (cudaStream_t)stream>>>(P);
+      });
+      INFLLM_LAUNCH_OK("page_write_kernel");
+    }
+    return INFLLM_OK;
+  });
+}

@@ -1,0 +1,99 @@
+// The paged cache's bookkeeping (pages.cu) and a batch's view of it, as the attention over its pages (paged_attn.cu) uses them.
+#pragma once
+#include <exception>
+#include <functional>
+#include <new>
+#include <queue>
+#include <vector>
+
+#include "tc_common.cuh"
+
+namespace infllm {
+
+struct PageSeq {
+  bool open = false;
+  uint32_t generation = 0;  // counts the sequences that had this number
+  int64_t length = 0, position = 0;
+  std::vector<int32_t> pages;
+};
+
+// One launch's worth of changes: rows of the table that are copied, entries that are set, tokens that are moved.
+struct PageItem {
+  int32_t a, b, c, d;
+};
+
+// A batch's tokens as the kernels get them.
+struct BatchSeq {
+  int32_t row;       // of the table
+  int32_t length;    // tokens, the newest included
+  int32_t count;     // of them the newest that the call is about
+  int32_t position;  // of the first of those, for the rotary embedding
+};
+
+// the current device for a call's duration
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    if (device >= 0 && cudaGetDevice(&before_) == cudaSuccess && before_ != device) ok_ = cudaSetDevice(device) == cudaSuccess;
+    else before_ = -1;
+  }
+  ~DeviceScope() {
+    if (before_ >= 0) cudaSetDevice(before_);
+  }
+  bool ok() const { return ok_; }
+
+ private:
+  int before_ = -1;
+  bool ok_ = true;
+};
+
+// nothing is thrown across the C boundary
+template <typename F>
+int guarded(const char* what, F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(INFLLM_E_NOMEM, "%s: no host memory", what);
+  } catch (const std::exception& e) {
+    return fail(INFLLM_E_NOMEM, "%s: %s", what, e.what());
+  }
+}
+
+}  // namespace infllm
+
+struct infllm_pages {
+  infllm_pages_config cfg;
+  std::vector<infllm::PageSeq> seqs;
+  std::vector<int32_t> uses;  // sequences that have a page
+  std::priority_queue<int32_t, std::vector<int32_t>, std::greater<int32_t>> free_pages;
+  uint64_t change = 0;   // any change of what sequences hold
+  uint64_t reshape = 0;  // of the pages that a sequence had before
+  std::vector<infllm::PageItem> rows, edits, moves;  // of the call that is being made
+  CUtensorMap map;       // of all pages (paged_attn.cu)
+
+  int32_t pages_of(int64_t tokens) const { return (int32_t)((tokens + cfg.page_size - 1) / cfg.page_size); }
+};
+
+struct infllm_page_batch {
+  infllm_pages* cache;
+  std::vector<int32_t> seqs;
+  std::vector<uint32_t> generation;
+  std::vector<int32_t> count;  // newest tokens of each sequence that calls are about
+  int32_t most = 0;            // the largest of them: the tokens of a call's tensors
+  // the order of the sequences by their pages, and how many pages each shares with the one before: as of `reshape`
+  uint64_t order_of = ~0ull;
+  std::vector<int32_t> order, common;
+  // the plan of the attention (paged_attn.cu), as of `change` and for n_heads
+  uint64_t plan_of = ~0ull;
+  int32_t plan_heads = 0;
+  std::vector<int32_t> plan;
+  int32_t n_row_units = 0;
+  bool join = false;
+  int64_t part_rows = 0;
+  int64_t off_unit = 0, off_seq = 0, off_path = 0, off_span = 0, off_node_seq = 0;  // sections of the plan
+};
+
+namespace infllm {
+int batch_alive(const infllm_page_batch* b, const char* what);
+int pages_encode_map(infllm_pages* p);  // paged_attn.cu
+}  // namespace infllm

@@ -1,0 +1,335 @@
+"""PagedBatch.attend and write against the formulas in 64 bits.
+
+Tolerances, per output: u of |o| for the rounding to the 16-bit type (u = 2^-8 for bf16, 2^-11 for fp16), u of
+sum_j p_j |v_j| for the probabilities, which are 16-bit operands of the product, and for what is held in 32 bits 2^-16 of that
+sum (a dot product of 128 terms, and sums over 4096 keys in parts).  Of a log-sum-exp: 2^-16 of the largest sum_d |q_d k_d| of a row, scaled."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+NAN = float("nan")
+
+
+def make(n_pages, page, kv, dim, dtype=torch.bfloat16, layers=1, **more):
+    from infllm_b200.attention import PagedCache
+
+    c = PagedCache(layers, kv, dim, n_pages, page_size=page, dtype=dtype, **more)
+    c.pages.fill_(NAN)  # what no token was written to is not read
+    return c
+
+
+def rand(g, *shape, dtype=torch.bfloat16, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+class Kept:
+    """A cache, and the keys and values of every sequence as one tensor each."""
+
+    def __init__(self, cache, seed):
+        self.c, self.g, self.k, self.v = cache, torch.Generator(device="cuda").manual_seed(seed), {}, {}
+
+    def open(self):
+        s = self.c.open()[0]
+        self.k[s] = self.v[s] = torch.empty((self.c.n_kv_heads, 0, self.c.head_dim), dtype=self.c.dtype, device="cuda")
+        return s
+
+    def grow(self, seqs, counts):
+        b, most = self.c.batch(seqs), max(counts)
+        b.extend(counts)
+        k, v = (rand(self.g, len(seqs), self.c.n_kv_heads, most, self.c.head_dim, dtype=self.c.dtype) for _ in range(2))
+        b.write(0, k, v)
+        for i, (s, n) in enumerate(zip(seqs, counts)):
+            self.k[s] = torch.cat((self.k[s], k[i, :, most - n:]), 1)
+            self.v[s] = torch.cat((self.v[s], v[i, :, most - n:]), 1)
+        return b
+
+    def fork(self, s, n):
+        kids = self.c.fork([s], n)
+        for x in kids:
+            self.k[x], self.v[x] = self.k[s], self.v[s]
+        return kids
+
+    def check(self, b, counts, heads, scale=None, lean=1.0):
+        c, most = self.c, max(counts)
+        q = rand(self.g, len(b.seqs), heads, most, c.head_dim, dtype=c.dtype, scale=lean)
+        out, lse = b.attend(0, q, scale=scale, return_lse=True)
+        alone = b.attend(0, q, scale=scale)
+        assert torch.equal(out, alone)
+        scale = 1 / math.sqrt(c.head_dim) if scale is None else scale
+        u, group = U[c.dtype], heads // c.n_kv_heads
+        assert out.shape == q.shape and out.dtype == c.dtype and lse.shape == q.shape[:3]
+        for i, (s, n) in enumerate(zip(b.seqs, counts)):
+            assert (out[i, :, :most - n] == 0).all() and (lse[i, :, :most - n] == -math.inf).all()
+            if n == 0:
+                continue
+            k, v = (x[s].double().repeat_interleave(group, 0) for x in (self.k, self.v))
+            length = k.size(1)
+            x = q[i, :, most - n:].double()
+            sc = x @ k.transpose(1, 2) * scale
+            hidden = torch.ones((n, length), dtype=torch.bool, device="cuda").triu(length - n + 1)
+            sc = sc.masked_fill(hidden, -math.inf)
+            p = torch.softmax(sc, -1)
+            want, mass = p @ v, p @ v.abs()
+            err = (out[i, :, most - n:].double() - want).abs()
+            tol = u * want.abs() + (u + 2.0 ** -16) * mass
+            assert (err <= tol).all(), (i, s, n, (err / tol).max().item())
+            big = (x.abs() @ k.abs().transpose(1, 2)).amax() * abs(scale)
+            assert ((lse[i, :, most - n:].double() - torch.logsumexp(sc, -1)).abs() <= 2.0 ** -16 * (1 + big)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim,kv,group", [(16, 128, 2, 4), (128, 128, 8, 4), (32, 64, 4, 7), (64, 64, 1, 16), (128, 128, 3, 1), (64, 128, 2, 24)])
+@pytest.mark.parametrize("prefix,tails", [(0, (1,)), (1, (1, 1)), (15, (2, 1, 17)), (300, (1, 5, 129, 64)), (1024, (1,) * 5), (2000, (3, 200) * 20)])
+def test_one_token_each(dtype, page, dim, kv, group, prefix, tails):
+    total = prefix + sum(t + 2 * page for t in tails)
+    x = Kept(make(total // page + 2, page, kv, dim, dtype, max_tokens=8192), prefix + len(tails))
+    root = x.open()
+    if prefix:
+        x.grow([root], [prefix])
+    seqs = x.fork(root, len(tails))
+    x.grow(seqs, list(tails))
+    b = x.grow(seqs, [1] * len(tails))
+    x.check(b, [1] * len(tails), kv * group)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim,kv,group", [(16, 128, 2, 4), (128, 128, 4, 1), (32, 64, 2, 7), (64, 128, 1, 8)])
+@pytest.mark.parametrize("prefix,counts", [(0, (1000,)), (700, (33,)), (129, (7, 1, 0, 40)), (1500, (48,) * 6), (40, (300, 2, 129)), (2500, (128, 128))])
+def test_several_tokens_each(dtype, page, dim, kv, group, prefix, counts):
+    total = prefix + sum(t + 2 * page for t in counts)
+    x = Kept(make(total // page + 2, page, kv, dim, dtype, max_tokens=8192), prefix + sum(counts))
+    root = x.open()
+    if prefix:
+        x.grow([root], [prefix])
+    seqs = x.fork(root, len(counts))
+    b = x.grow(seqs, list(counts))
+    x.check(b, list(counts), kv * group)
+    some = [min(n, 5) for n in counts]
+    b.plan(some)  # the newest tokens, asked again
+    x.check(b, some, kv * group)
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_a_tree_of_forks_and_strangers(page):
+    x = Kept(make(4000 // page + 60, page, 2, 128), 3)
+    a, other, empty = x.open(), x.open(), x.open()
+    x.grow([a, other], [page * 3 + 5, 77])
+    kids = x.fork(a, 3)
+    x.grow(kids, [page * 2, page * 2 + 1, 9])
+    grand = x.fork(kids[0], 2) + x.fork(kids[1], 3)
+    x.grow(grand, [1, 300, 2, page, 5])
+    seqs = [grand[3], other, kids[2], empty, grand[0], a, grand[4], kids[1], grand[1], grand[2], kids[0]]
+    b = x.c.batch(seqs)
+    counts = [1, 1, 1, 0, 1, 1, 1, 1, 1, 1, 1]
+    b.plan(counts)
+    x.check(b, counts, 8)
+    counts = [min(n, x.c.length(s)) for n, s in zip([3, 70, 9, 0, 150, 2, 5, 1, 33, 2, 2], seqs)]  # newest tokens that lie in shared pages
+    b.plan(counts)
+    x.check(b, counts, 8)
+    x.c.truncate([kids[1], grand[2]], [page * 3 + 9, page * 4])  # inside a page that others share
+    for s, n in ((kids[1], page * 3 + 9), (grand[2], page * 4)):
+        x.k[s], x.v[s] = x.k[s][:, :n], x.v[s][:, :n]
+    counts = [1, 1, 1, 0, 1, 1, 1, 2, 1, 2, 1]
+    b.plan(counts)
+    x.check(b, counts, 8)
+    b = x.grow([kids[1], grand[2], kids[0]], [1, 2, 3])  # written into a copy of it
+    x.check(b, [1, 2, 3], 8)
+    b = x.c.batch(seqs)
+    b.plan(counts)
+    x.check(b, counts, 8)
+
+
+@pytest.mark.parametrize("lean", [0.0, 8.0, 60.0])
+def test_flat_and_peaked_scores(lean):
+    x = Kept(make(200, 32, 2, 128), 5)
+    root = x.open()
+    x.grow([root], [3000])
+    seqs = x.fork(root, 40)
+    b = x.grow(seqs, [4] * 40)
+    x.check(b, [4] * 40, 8, lean=lean)
+    x.check(b, [4] * 40, 8, scale=0.01, lean=lean)
+
+
+def test_strided_queries_and_another_layer():
+    c = make(40, 16, 2, 128, layers=3)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    s = c.open(2)
+    b = c.batch(s)
+    b.extend([100, 30])
+    qkv = rand(g, 2, 100, 12 * 128 + 8)  # one projection of all heads
+    q, k, v = (qkv[..., a * 128:e * 128].view(2, 100, e - a, 128).permute(0, 2, 1, 3) for a, e in ((0, 8), (8, 10), (10, 12)))
+    b.write(2, k, v)
+    o = b.attend(2, q)
+    b.write(1, k.contiguous(), v.contiguous())
+    assert torch.equal(o, b.attend(1, q.contiguous()))
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")[1:].view(q.shape)  # not 16-byte aligned
+    odd.copy_(q)
+    assert torch.equal(o, b.attend(1, odd))
+    torch.cuda.synchronize()
+    assert torch.isnan(c.pages[0]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,page,kv,heads", [(128, 16, 2, 8), (64, 64, 4, 4), (128, 128, 1, 0)])
+def test_write_rotates_to_the_tokens_positions(dtype, dim, page, kv, heads):
+    """Bit for bit the rotary embedding of the other attention types, at the tokens' places; nothing else is touched."""
+    from infllm_b200.attention import RotaryEmbeddingESM
+
+    c = make(60, page, kv, dim, dtype)
+    rope, g = RotaryEmbeddingESM(dim, 1e4, 1.0), torch.Generator(device="cuda").manual_seed(dim)
+    s = c.open(3)
+    b = c.batch(s)
+    pasts = [0, 21, page]
+    b.extend(pasts)
+    counts = [5, 37, 0]
+    b.extend(counts)
+    k, v = (rand(g, 3, kv, 37, dim, dtype=dtype) for _ in range(2))
+    q = rand(g, 3, heads, 37, dim, dtype=dtype) if heads else None
+    got = b.write(0, k, v, q, rope)
+    assert (got is None) == (heads == 0)
+    touched = torch.zeros_like(c.pages, dtype=torch.bool)
+    for i, (n, past) in enumerate(zip(counts, pasts)):
+        if n == 0:
+            continue
+        turned = rope.apply_rotary_pos_emb(k[i, :, 37 - n:], n, past + n)
+        row = c.page_ids(s[i])
+        for t in range(n):
+            p, o = row[(past + t) // page], (past + t) % page
+            assert torch.equal(c.pages[0, 0, p, :, o], turned[:, t]) and torch.equal(c.pages[0, 1, p, :, o], v[i, :, 37 - n + t])
+            touched[0, :, p, :, o] = True
+        if heads:
+            assert torch.equal(got[i, :, 37 - n:], rope.apply_rotary_pos_emb(q[i, :, 37 - n:], n, past + n))
+            assert (got[i, :, :37 - n] == 0).all()
+    assert torch.isnan(c.pages[~touched]).all()
+
+
+def test_positions_go_on_after_compaction():
+    from infllm_b200.attention import RotaryEmbeddingESM
+
+    c = make(20, 16, 1, 64)
+    rope = RotaryEmbeddingESM(64, 1e4, 1.0)
+    s = c.open()
+    b = c.batch(s)
+    b.extend(50)
+    c.compact(s, [[(0, 3), (30, 50)]])
+    assert (c.length(s[0]), c.position(s[0])) == (23, 50)
+    b.extend(2)
+    k = rand(torch.Generator(device="cuda").manual_seed(0), 1, 1, 2, 64)
+    b.write(0, k, k, None, rope)
+    at = c.page_ids(s[0])[1]
+    assert torch.equal(c.pages[0, 0, at, :, 7:9], rope.apply_rotary_pos_emb(k[0], 2, 52))
+
+
+@pytest.mark.parametrize("page,layers,kv,dim", [(16, 2, 2, 64), (128, 3, 1, 128), (32, 1, 4, 128)])
+def test_fork_copy_and_compact_move_what_they_say(page, layers, kv, dim):
+    from infllm_b200.attention import PagedCache
+
+    c = make(100 * 128 // page, page, kv, dim, layers=layers)
+    g = torch.Generator(device="cuda").manual_seed(page)
+    c.pages.copy_(rand(g, *c.pages.shape))
+    s = c.open(2)
+    c.batch(s).extend([5 * page + 3, 2 * page])
+
+    def tokens(cache, seq):
+        ids = torch.tensor(cache.page_ids(seq), device="cuda", dtype=torch.long)
+        assert cache.table[seq, :len(ids)].tolist() == ids.tolist()
+        x = cache.pages[:, :, ids].movedim(3, 2)
+        return x.reshape(layers, 2, kv, -1, dim)[:, :, :, :cache.length(seq)]
+
+    before, was = [tokens(c, x).clone() for x in s], c.pages.clone()
+    kids = c.fork(s, 70)  # more changes than a small launch takes
+    for i, k in enumerate(kids):
+        assert torch.equal(tokens(c, k), before[i // 70])
+    assert c.page_ids(kids[0])[:5] == c.page_ids(s[0])[:5] and c.page_ids(kids[0])[5] != c.page_ids(s[0])[5]
+    spans = [[(0, page), (page + 3, 2 * page + 1), (4 * page, 5 * page + 3)], [(1, 2), (3, 3), (5, 2 * page)]]
+    c.compact([kids[3], kids[75]], spans)
+    for k, i, sp in ((kids[3], 0, spans[0]), (kids[75], 1, spans[1])):
+        assert torch.equal(tokens(c, k), torch.cat([before[i][:, :, :, a:b] for a, b in sp], 3))
+    assert c.page_ids(kids[3])[0] == c.page_ids(s[0])[0]
+    for i, k in enumerate(s):
+        assert torch.equal(tokens(c, k), before[i])
+    other = PagedCache(layers, kv, dim, 30, page_size=page, max_sequences=4, max_tokens=6 * page)
+    moved = c.copy([kids[3], s[1]], into=other)
+    assert torch.equal(tokens(other, moved[0]), tokens(c, kids[3])) and torch.equal(tokens(other, moved[1]), before[1])
+    again = c.copy([s[0]])[0]
+    assert torch.equal(tokens(c, again), before[0]) and not set(c.page_ids(again)) & set(c.page_ids(s[0]))
+    c.compact([again], [[]])
+    assert c.length(again) == 0 and c.page_ids(again) == []
+    c.free(kids + [again])
+    assert torch.equal(was[:, :, c.page_ids(s[0])], c.pages[:, :, c.page_ids(s[0])])
+    assert c.free_pages == c.n_pages - 8
+
+
+def test_refusals():
+    from infllm_b200 import _lib as L
+    from infllm_b200.attention import PagedCache, RotaryEmbeddingESM
+
+    c = make(6, 16, 2, 64, max_sequences=4, max_tokens=64)
+    s = c.open(2)
+    b = c.batch(s)
+    b.extend([20, 4])
+    k = torch.zeros((2, 2, 20, 64), dtype=torch.bfloat16, device="cuda")
+    b.write(0, k, k)
+    with pytest.raises(L.InfLLMCapacityError):
+        b.extend(40)  # pages
+    with pytest.raises(L.InfLLMCapacityError):
+        b.extend([45, 0])  # the row of the table
+    assert c.length(s[0]) == 20 and c.free_pages == 3
+    q = torch.zeros((2, 4, 20, 64), dtype=torch.bfloat16, device="cuda")
+    for call, error in ((lambda: b.write(1, k, k), L.InfLLMError), (lambda: b.attend(-1, q), L.InfLLMError), (lambda: b.attend(0, q[:, :3]), L.InfLLMError),
+                        (lambda: b.attend(0, q[:, :, :3]), ValueError), (lambda: b.attend(0, q.half()), TypeError), (lambda: b.attend(0, q.cpu()), RuntimeError),
+                        (lambda: b.write(0, k, k[..., :32]), ValueError), (lambda: b.write(0, k, k, q, RotaryEmbeddingESM(128)), ValueError),
+                        (lambda: c.batch([s[0], s[0]]), L.InfLLMError), (lambda: c.batch([]), L.InfLLMError), (lambda: b.plan([30, 1]), L.InfLLMError),
+                        (lambda: b.plan([1]), ValueError), (lambda: b.retract([21, 0]), L.InfLLMError), (lambda: c.truncate(s, [1]), ValueError),
+                        (lambda: c.compact(s, [[(0, 1)]]), ValueError), (lambda: c.compact(s, [[(0, 1, 2)], []]), ValueError),
+                        (lambda: PagedCache(1, 2, 96, 4), L.InfLLMError), (lambda: PagedCache(1, 2, 64, 4, page_size=24), L.InfLLMError),
+                        (lambda: PagedCache(1, 2, 64, 4, dtype=torch.float32), TypeError), (lambda: PagedCache(1, 2, 64, 4, device="cpu"), ValueError),
+                        (lambda: PagedCache(0, 2, 64, 4), ValueError)):
+        with pytest.raises(error):
+            call()
+    kid = c.fork([s[0]], 1)
+    both = c.batch([s[0], kid[0]])
+    both.plan([20, 20])
+    with pytest.raises(L.InfLLMError):  # shared pages are not written
+        both.write(0, k, k)
+    b.plan(1)
+    assert b.attend(0, q[:, :, :1]).shape == (2, 4, 1, 64)
+    c.free([s[1]])
+    with pytest.raises(L.InfLLMError):
+        b.attend(0, q[:, :, :1])
+    b = c.batch([s[0]])
+    b.extend(1)
+    b.retract(1)
+    assert b.attend(0, q[:1, :, :0]).shape == (1, 4, 0, 64)  # no token is newest
+
+
+def test_drafts_are_taken_back():
+    x = Kept(make(60, 16, 2, 128), 9)
+    root = x.open()
+    x.grow([root], [100])
+    seqs = x.fork(root, 3)
+    x.grow(seqs, [5, 6, 7])
+    b = x.c.batch(seqs)
+    free = x.c.free_pages
+    b.extend(30)
+    junk = rand(x.g, 3, 2, 30, 128)
+    b.write(0, junk, junk)
+    b.retract(30)
+    assert x.c.free_pages == free
+    b = x.grow(seqs, [2, 2, 2])
+    x.check(b, [2, 2, 2], 8)
+
+
+def test_another_stream_than_the_default():
+    x = Kept(make(60, 16, 2, 128), 11)
+    root = x.open()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        x.grow([root], [500])
+        seqs = x.fork(root, 6)
+        b = x.grow(seqs, [1] * 6)
+        x.check(b, [1] * 6, 8)

@@ -1,0 +1,260 @@
+"""The paged cache's bookkeeping, without a GPU, against a restatement of its rules: pages and numbers lowest first, shared
+full pages, what is refused and that a refusal changes nothing."""
+import ctypes
+import random
+from ctypes import c_int, c_int32, c_int64
+
+import pytest
+
+from infllm_b200 import _lib as L
+
+
+class Cache:
+    def __init__(self, n_pages=40, page=16, max_sequences=12, max_pages=10):
+        cfg = L.PagesConfig(1, 2, 64, page, n_pages, max_sequences, max_pages, L.BF16, -1, 0, None, None)
+        self.h = ctypes.c_void_p()
+        L.check(L.lib.infllm_pages_create(ctypes.byref(cfg), ctypes.byref(self.h)))
+
+    def __del__(self):
+        L.lib.infllm_pages_destroy(self.h)
+
+    def ids(self, x):
+        return (c_int32 * len(x))(*x)
+
+    def open(self, n=1):
+        out = (c_int32 * n)()
+        L.check(L.lib.infllm_pages_open(self.h, n, out))
+        return list(out)
+
+    def fork(self, seqs, n):
+        out = (c_int32 * (len(seqs) * n))()
+        L.check(L.lib.infllm_pages_fork(self.h, self.ids(seqs), len(seqs), n, out, None))
+        return list(out)
+
+    def copy(self, seqs, into):
+        out = (c_int32 * len(seqs))()
+        L.check(L.lib.infllm_pages_copy(self.h, self.ids(seqs), len(seqs), into.h, out, None))
+        return list(out)
+
+    def extend(self, seqs, counts):
+        b = ctypes.c_void_p()
+        L.check(L.lib.infllm_page_batch_create(self.h, self.ids(seqs), len(seqs), ctypes.byref(b)))
+        try:
+            L.check(L.lib.infllm_page_batch_extend(b, self.ids(counts), None))
+        finally:
+            L.lib.infllm_page_batch_destroy(b)
+
+    def truncate(self, seqs, lengths):
+        L.check(L.lib.infllm_pages_truncate(self.h, self.ids(seqs), (c_int64 * len(lengths))(*lengths), len(seqs)))
+
+    def free(self, seqs):
+        L.check(L.lib.infllm_pages_free(self.h, self.ids(seqs), len(seqs)))
+
+    def compact(self, seqs, keep):
+        flat = [x for spans in keep for s in spans for x in s]
+        L.check(L.lib.infllm_pages_compact(self.h, self.ids(seqs), len(seqs), (c_int64 * len(flat))(*flat),
+                                           self.ids([len(k) for k in keep]), None))
+
+    def row(self, s):
+        n, out = c_int(), (c_int32 * 64)()
+        L.check(L.lib.infllm_pages_row(self.h, s, out, 64, ctypes.byref(n)))
+        return list(out[:n.value])
+
+    def info(self, s):
+        a, b = c_int64(), c_int64()
+        L.check(L.lib.infllm_pages_info(self.h, s, ctypes.byref(a), ctypes.byref(b)))
+        return a.value, b.value
+
+    @property
+    def n_free(self):
+        return L.lib.infllm_pages_free_count(self.h)
+
+
+class Model:
+    """The rules, as plainly as they can be said; a page also knows which tokens are in it, so that moves can be followed."""
+
+    def __init__(self, n_pages=40, page=16, max_sequences=12, max_pages=10):
+        self.page, self.n_pages, self.max_pages, self.max_sequences = page, n_pages, max_pages, max_sequences
+        self.uses = [0] * n_pages
+        self.seqs = {}  # number -> [pages, length, position]
+
+    def free_pages(self):
+        return [i for i in range(self.n_pages) if not self.uses[i]]
+
+    def take(self):
+        p = self.free_pages()[0]
+        self.uses[p] = 1
+        return p
+
+    def numbers(self, n):
+        got = [i for i in range(self.max_sequences) if i not in self.seqs][:n]
+        return got if len(got) == n else None
+
+    def pages_of(self, n):
+        return -(-n // self.page)
+
+    def open(self, n=1):
+        got = self.numbers(n)
+        if got is None:
+            return None
+        for g in got:
+            self.seqs[g] = [[], 0, 0]
+        return got
+
+    def extend(self, seqs, counts):
+        need = 0
+        for s, c in zip(seqs, counts):
+            pages, length, _ = self.seqs[s]
+            if length + c > self.max_pages * self.page:
+                return None
+            need += self.pages_of(length + c) - len(pages)
+            need += bool(c and length % self.page and self.uses[pages[-1]] > 1)
+        if need > len(self.free_pages()):
+            return None
+        for s, c in zip(seqs, counts):
+            q = self.seqs[s]
+            if c and q[1] % self.page and self.uses[q[0][-1]] > 1:
+                old, q[0][-1] = q[0][-1], self.take()
+                self.uses[old] -= 1
+            q[1] += c
+            q[2] += c
+            while len(q[0]) < self.pages_of(q[1]):
+                q[0].append(self.take())
+        return True
+
+    def fork(self, seqs, n):
+        got = self.numbers(len(seqs) * n)
+        if got is None or sum(n * bool(self.seqs[s][1] % self.page) for s in seqs) > len(self.free_pages()):
+            return None
+        at = iter(got)
+        for s in seqs:
+            pages, length, position = self.seqs[s]
+            full = pages[:length // self.page]
+            for _ in range(n):
+                for p in full:
+                    self.uses[p] += 1
+                self.seqs[next(at)] = [full + ([self.take()] if length % self.page else []), length, position]
+        return got
+
+    def cut(self, s, length):
+        q = self.seqs[s]
+        q[2] -= q[1] - length
+        q[1] = length
+        while len(q[0]) > self.pages_of(length):
+            self.uses[q[0].pop()] -= 1
+
+    def compact(self, seqs, keep):
+        plans, need = [], 0
+        for s, spans in zip(seqs, keep):
+            place = [i for a, b in spans for i in range(a, b)]
+            stay = 0
+            while (stay + 1) * self.page <= len(place) and place[(stay + 1) * self.page - 1] == (stay + 1) * self.page - 1:
+                stay += 1
+            need += self.pages_of(len(place)) - stay
+            plans.append((len(place), stay))
+        if need > len(self.free_pages()):
+            return None
+        gone = []
+        for s, (n, stay) in zip(seqs, plans):
+            q = self.seqs[s]
+            gone += q[0][stay:]
+            q[0] = q[0][:stay] + [self.take() for _ in range(self.pages_of(n) - stay)]
+            q[1] = n
+        for g in gone:
+            self.uses[g] -= 1
+        return True
+
+
+def same(c, m):
+    assert c.n_free == len(m.free_pages())
+    for s, (pages, length, position) in m.seqs.items():
+        assert c.row(s) == pages and c.info(s) == (length, position), s
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("page,n_pages", [(16, 40), (32, 9)])
+def test_random_steps_follow_the_rules(seed, page, n_pages):
+    r = random.Random(seed)
+    c, m = Cache(n_pages, page), Model(n_pages, page)
+    refused = done = 0
+    for _ in range(400):
+        live = sorted(m.seqs)
+        what = r.choice(["open", "extend", "extend", "fork", "cut", "free", "compact"])
+        some = r.sample(live, r.randint(1, min(3, len(live)))) if live else []
+        if what != "open" and not live:
+            continue
+        if what == "open":
+            want, call = m.open(2), lambda: c.open(2)
+        elif what == "extend":
+            counts = [r.choice([0, 1, 3, page, 2 * page + 1]) for _ in some]
+            want, call = m.extend(some, counts), lambda: c.extend(some, counts)
+        elif what == "fork":
+            n = r.randint(0, 3)
+            want, call = m.fork(some, n), lambda: c.fork(some, n)
+        elif what == "cut":
+            lengths = [r.randint(0, m.seqs[s][1]) for s in some]
+            for s, n in zip(some, lengths):
+                m.cut(s, n)
+            want, call = True, lambda: c.truncate(some, lengths)
+        elif what == "free":
+            for s in some:
+                m.cut(s, 0)
+                del m.seqs[s]
+            want, call = True, lambda: c.free(some)
+        else:
+            keep = []
+            for s in some:
+                cuts = sorted(r.sample(range(m.seqs[s][1] + 1), min(m.seqs[s][1] + 1, 2 * r.randint(0, 3)) // 2 * 2))
+                keep.append(list(zip(cuts[::2], cuts[1::2])))
+            want, call = m.compact(some, keep), lambda: c.compact(some, keep)
+        if want is None:
+            with pytest.raises(L.InfLLMCapacityError):
+                call()
+            refused += 1
+        else:
+            got = call()
+            assert got is None or got == want
+            done += 1
+        same(c, m)
+    assert done > 100 and refused > 5
+
+
+def test_copies_share_nothing():
+    a, b = Cache(), Cache(n_pages=7)
+    s = a.open()[0]
+    a.extend([s], [35])
+    k = a.fork([s], 1)[0]
+    t = a.copy([k, s], a)
+    assert len(set(a.row(t[0]) + a.row(t[1])) & set(a.row(s) + a.row(k))) == 0 and not set(a.row(t[0])) & set(a.row(t[1]))
+    assert [a.info(x) for x in t] == [(35, 35)] * 2
+    u = b.copy([], b) + a.copy([s, k], b)
+    assert b.row(u[0]) == [0, 1, 2] and b.row(u[1]) == [3, 4, 5] and b.n_free == 1
+    with pytest.raises(L.InfLLMCapacityError):
+        a.copy([s], b)
+    assert b.n_free == 1 and b.info(u[0]) == (35, 35)
+
+
+def test_refusals():
+    c = Cache()
+    s = c.open()[0]
+    c.extend([s], [20])
+    for call in (lambda: c.free([5]), lambda: c.free([s, s]), lambda: c.free([-1]), lambda: c.fork([3], 1), lambda: c.truncate([s], [21]),
+                 lambda: c.truncate([s], [-1]), lambda: c.extend([s], [-1]), lambda: c.compact([s], [[(0, 21)]]),
+                 lambda: c.compact([s], [[(5, 7), (6, 9)]]), lambda: c.compact([s], [[(5, 4)]]), lambda: c.row(99)):
+        with pytest.raises(L.InfLLMError) as e:
+            call()
+        assert e.value.code == L.E_BADARG
+        assert c.info(s) == (20, 20) and c.n_free == 38
+    b = ctypes.c_void_p()
+    L.check(L.lib.infllm_page_batch_create(c.h, c.ids([s]), 1, ctypes.byref(b)))
+    c.free([s])
+    assert c.open() == [s]  # the same number, another sequence
+    assert L.lib.infllm_page_batch_extend(b, c.ids([1]), None) == L.E_BADARG and b"freed" in L.lib.infllm_last_error()
+    L.lib.infllm_page_batch_destroy(b)
+    out = ctypes.c_void_p()
+    for change in (dict(head_dim=96), dict(page_size=48), dict(dtype=2), dict(n_pages=0), dict(max_pages=1 << 30)):
+        cfg = L.PagesConfig(n_layers=1, n_kv_heads=2, head_dim=64, page_size=16, n_pages=4, max_sequences=4, max_pages=4, dtype=0, device=-1)
+        for k, v in change.items():
+            setattr(cfg, k, v)
+        assert L.lib.infllm_pages_create(ctypes.byref(cfg), ctypes.byref(out)) in (L.E_BADARG, L.E_UNSUPPORTED)
+    assert L.lib.infllm_pages_create(None, None) == L.E_BADARG
