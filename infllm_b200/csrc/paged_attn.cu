@@ -14,65 +14,12 @@
 #include <cstring>
 
 #include "decode_warp.cuh"
-#include "pages.cuh"
+#include "attn_tc.cuh"
+#include "paged_attn.cuh"
 
 namespace infllm {
 
 using namespace mma;
-
-constexpr int kSeeAll = 1 << 30;
-
-struct alignas(16) AttnUnit {
-  int32_t row;        // of the page table: one of the node's sequences
-  int32_t key0, keys; // keys of the sequence; key0 is the first token of a page
-  int32_t lim0;       // a row of token i sees the keys below lim0 + i
-  int32_t row0, rows; // of the node's rows: (sequence of the node, token, query head of the KV head)
-  int32_t node_seq;   // where the node's sequences are listed
-  int32_t part;       // where the unit's partial rows begin: part * n_kv_heads + kv head * rows; -1: they are whole, and go to the output
-};
-struct alignas(16) AttnSeq {   // of a sequence of the batch, for the join
-  int32_t path, n_path;        // its nodes
-  int32_t count, pad;
-};
-struct alignas(16) AttnPath {
-  int32_t span, tile;          // the node's first row tile's span, rows of a tile
-  int32_t at, pad;             // place of the sequence in the node
-};
-struct alignas(16) AttnSpan {  // of a row tile of a node: n partials, one behind the other
-  int32_t part, n, rows, pad;
-};
-
-struct PagedParams {
-  const char* pages;  // keys of the layer
-  int64_t plane;      // bytes from keys to values
-  const int32_t* table;
-  const char* q;
-  int64_t q_bs, q_hs, q_ts;  // bytes
-  char* out;
-  float* lse;
-  float *part_o, *part_lse;
-  const AttnUnit* unit;
-  const AttnSeq* seq;
-  const AttnPath* path;
-  const AttnSpan* span;
-  const int32_t* node_seq;
-  int32_t max_pages, page, n_kv, group, most, batch;
-  float scale_log2;
-};
-
-// where a row of a node is in the batch
-struct RowAt {
-  int32_t b, i, h;  // sequence, token, query head of the KV head
-};
-__device__ __forceinline__ RowAt row_at(const PagedParams& P, int node_seq, int r) {
-  RowAt a;
-  const int t = r / P.group;
-  a.h = r - t * P.group;
-  const int j = t / P.most;
-  a.i = t - j * P.most;
-  a.b = __ldg(P.node_seq + node_seq + j);
-  return a;
-}
 
 // ------------------------------------------------------------------------------------------------------- few rows
 // Up to 16 rows: a unit's keys in groups of 16, a warp per group; keys and values go from global memory straight into the
@@ -232,7 +179,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid
     }
     const float lse = mx == -INFINITY ? -INFINITY : mx + log2f(den);
     if (U.part >= 0) {
-      const int64_t pr = (int64_t)U.part * P.n_kv + hkv * U.rows + r;
+      const int64_t pr = (int64_t)U.part + hkv * U.part_kv + r;
       *reinterpret_cast<float2*>(P.part_o + pr * kDim + d) = make_float2(n0, n1);
       if (d == 0) P.part_lse[pr] = lse;
     } else {
@@ -263,8 +210,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     for (int k = 0; k < S.n_path; ++k) {
       const AttnPath A = P.path[S.path + k];
       const int r = (A.at * P.most + i) * P.group + h % P.group, tile = r / A.tile;
-      const AttnSpan Z = P.span[A.span + tile];
-      f((int64_t)Z.part * P.n_kv + hkv * Z.rows + (r - tile * A.tile), Z.n, (int64_t)Z.rows * P.n_kv);
+      const AttnSpan Z = P.span[(A.span + tile) * P.n_kv + hkv];
+      f((int64_t)Z.part + (r - tile * A.tile), Z.n, (int64_t)Z.rows);
     }
   };
   bool whole = false;  // written by the unit that had all of it
@@ -383,7 +330,7 @@ int64_t append(std::vector<int32_t>* plan, const std::vector<V>& v) {
 
 int make_plan(infllm_page_batch* b, int n_heads) {
   const infllm_pages* p = b->cache;
-  const int n = (int)b->seqs.size(), group = n_heads / p->cfg.n_kv_heads, most = b->most;
+  const int n = (int)b->seqs.size(), n_kv = p->cfg.n_kv_heads, group = n_heads / n_kv, most = b->most;
   if (b->order_of != p->reshape) {
     order_batch(b);
     b->order_of = p->reshape;
@@ -391,59 +338,101 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   Tree tree{b, {}, std::vector<std::vector<int32_t>>(n)};
   tree.build(b->order, b->common, 0);
 
-  // row tiles
+  // row tiles: of up to 256 rows for the tensor cores, of up to 16 for nodes that have no more
   struct Tile {
-    int32_t node, row0, rows;
-    int64_t key1;
+    AttnUnit unit;  // of all its keys
+    bool many, alone;
   };
   std::vector<Tile> tiles;
-  std::vector<int32_t> first_tile;
-  int64_t work = 0;
-  for (size_t x = 0; x < tree.nodes.size(); ++x) {
-    const Node& N = tree.nodes[x];
+  std::vector<int32_t> first_tile, node_seq;
+  int64_t few_work = 0, many_work = 0;  // groups of 16 keys, and tiles of 128 by up to 128 rows
+  for (const Node& N : tree.nodes) {
     const bool leaf = N.seqs.size() == 1;
     const int64_t rows = (int64_t)N.seqs.size() * most * group;
+    const bool many = rows > kRowTile;
+    const int size = many ? kTileRows : kRowTile;
     first_tile.push_back((int32_t)tiles.size());
-    for (int64_t r = 0; r < rows; r += kRowTile) {
-      Tile t{(int32_t)x, (int32_t)r, (int32_t)std::min<int64_t>(kRowTile, rows - r), N.key1};
-      if (leaf) t.key1 = N.key1 - most + (r + t.rows - 1) / group + 1;  // up to the last row's token
-      tiles.push_back(t);
-      work += std::max<int64_t>(0, ceil_div(t.key1 - N.key0, 16)) * p->cfg.n_kv_heads;
+    for (int64_t r = 0; r < rows; r += size) {
+      const int32_t in = (int32_t)std::min<int64_t>(size, rows - r);
+      // (of a leaf up to the last row's token)
+      const int64_t end = leaf ? N.key1 - most + (r + in - 1) / group + 1 : N.key1;
+      const int64_t keys = std::max<int64_t>(0, end - N.key0);
+      AttnUnit u{b->seqs[N.seqs[0]], (int32_t)N.key0, (int32_t)keys, leaf ? (int32_t)(N.key1 - most + 1) : kSeeAll, (int32_t)r, in, (int32_t)node_seq.size(), 0, 0, -1, {0, 0}};
+      tiles.push_back({u, many, leaf && tree.path[N.seqs[0]].size() == 1});
+      if (many) many_work += ceil_div(keys, 128) * (in > 128 ? 2 : 1) * n_kv;
+      else few_work += ceil_div(keys, 16) * n_kv;
     }
-  }
-  // units of equal work: four blocks per SM, a warp's groups of 16 keys at least
-  const int64_t chunk = std::max<int64_t>(kRowWarps, ceil_div(ceil_div(work, 148 * 4), kRowWarps) * kRowWarps) * 16;
-  std::vector<AttnUnit> units;
-  std::vector<AttnSpan> spans;
-  std::vector<int32_t> node_seq, node_seq_at;
-  for (const Node& N : tree.nodes) {
-    node_seq_at.push_back((int32_t)node_seq.size());
     node_seq.insert(node_seq.end(), N.seqs.begin(), N.seqs.end());
   }
+
+  std::vector<AttnUnit> few, large;
+  std::vector<int32_t> cta{0};
+  std::vector<AttnSpan> spans(tiles.size() * n_kv);
   int64_t part = 0;
   bool join = false;
-  for (const Tile& t : tiles) {
-    const Node& N = tree.nodes[t.node];
-    const bool leaf = N.seqs.size() == 1, alone = leaf && tree.path[N.seqs[0]].size() == 1;
-    const int64_t keys = std::max<int64_t>(0, t.key1 - N.key0);
-    const int64_t cut = std::max<int64_t>(1, ceil_div(keys, chunk)), each = ceil_div(ceil_div(keys, 16), cut) * 16;
-    AttnSpan z{(int32_t)part, 0, t.rows, 0};
-    for (int64_t k = 0; k < keys || (alone && k == 0); k += std::max<int64_t>(each, 1)) {
-      const bool whole = alone && keys <= each;
-      AttnUnit u{b->seqs[N.seqs[0]], (int32_t)(N.key0 + k), (int32_t)std::max<int64_t>(0, std::min(each, keys - k)),
-                 leaf ? (int32_t)(N.key1 - most + 1) : kSeeAll, t.row0, t.rows, node_seq_at[t.node], whole ? -1 : (int32_t)part};
-      units.push_back(u);
-      if (whole) {
-        z.n = -1;
-        break;
-      }
-      ++z.n;
-      part += t.rows;
+  // few rows: units of equal work, four blocks per SM, a warp's groups of 16 keys at least
+  const int64_t chunk = std::max<int64_t>(kRowWarps, ceil_div(ceil_div(few_work, p->n_sm * 4), kRowWarps) * kRowWarps) * 16;
+  for (size_t x = 0; x < tiles.size(); ++x) {
+    const Tile& t = tiles[x];
+    if (t.many) continue;
+    const int64_t keys = t.unit.keys, cut = ceil_div(keys, chunk), each = cut ? ceil_div(ceil_div(keys, 16), cut) * 16 : 0;
+    AttnUnit u = t.unit;
+    const bool whole = t.alone && cut <= 1;
+    if (whole) {
+      few.push_back(u);
+      for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h].n = -1;
+      continue;
     }
-    join |= z.n >= 0;
-    spans.push_back(z);
+    u.part_kv = (int32_t)(cut * u.rows);
+    for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h] = {(int32_t)(part + h * cut * u.rows), (int32_t)cut, u.rows, 0};
+    for (int64_t k = 0; k < keys; k += each) {
+      u.key0 = t.unit.key0 + (int32_t)k, u.keys = (int32_t)std::min(each, keys - k), u.part = (int32_t)(part + k / each * u.rows);
+      few.push_back(u);
+    }
+    part += cut * u.rows * n_kv;
+    join = true;
   }
-  if (part * p->cfg.n_kv_heads > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_plan: too many partial rows");
+  // many rows: one list of all key tiles, cut into as many stretches of equal work as there are SMs, or fewer of four tiles
+  const int64_t n_cta = std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / 4));
+  int64_t done = 0;  // work that has been dealt out
+  for (size_t x = 0; x < tiles.size(); ++x) {
+    const Tile& t = tiles[x];
+    if (!t.many) continue;
+    const int64_t n_tiles = ceil_div(t.unit.keys, 128), weight = t.unit.rows > 128 ? 2 : 1;
+    for (int h = 0; h < n_kv; ++h) {
+      AttnUnit u = t.unit;
+      u.hkv = h;
+      const size_t first = large.size();
+      for (int64_t k = 0; k < n_tiles || (k == 0 && t.alone);) {
+        // up to the end of the block's share; what is left of one tile or less goes along
+        const int64_t share = ceil_div(many_work * (int64_t)cta.size(), n_cta);
+        int64_t take = std::min(n_tiles - k, std::max<int64_t>(0, (share - done) / weight));
+        if (n_tiles - k - take <= 1) take = n_tiles - k;
+        if (take > 0 || n_tiles == 0) {
+          u.key0 = t.unit.key0 + (int32_t)k * 128;
+          u.keys = (int32_t)std::min<int64_t>(take * 128, t.unit.keys - k * 128);
+          large.push_back(u);
+        }
+        k += take, done += take * weight;
+        if (n_tiles == 0) break;
+        if (k < n_tiles || done >= share) {
+          if ((int64_t)cta.size() < n_cta) cta.push_back((int32_t)large.size());
+        }
+      }
+      const size_t cut = large.size() - first;
+      AttnSpan& z = spans[x * n_kv + h];
+      if (cut == 1 && t.alone) {
+        z.n = -1;
+        continue;
+      }
+      z = {(int32_t)part, (int32_t)cut, u.rows, 0};
+      for (size_t k = first; k < large.size(); ++k, part += u.rows) large[k].part = (int32_t)part;
+      join = true;
+    }
+  }
+  if (part > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_plan: too many partial rows");
+  b->n_ctas = large.empty() ? 0 : (int32_t)cta.size();
+  cta.push_back((int32_t)large.size());
   std::vector<AttnSeq> seqs;
   std::vector<AttnPath> paths;
   for (int i = 0; i < n; ++i) {
@@ -451,27 +440,25 @@ int make_plan(infllm_page_batch* b, int n_heads) {
     join |= tree.path[i].empty();
     for (int32_t x : tree.path[i]) {
       const Node& N = tree.nodes[x];
-      paths.push_back({first_tile[x], kRowTile, (int32_t)(std::find(N.seqs.begin(), N.seqs.end(), i) - N.seqs.begin()), 0});
+      const int32_t tile = (int64_t)N.seqs.size() * most * group > kRowTile ? kTileRows : kRowTile;
+      paths.push_back({first_tile[x], tile, (int32_t)(std::find(N.seqs.begin(), N.seqs.end(), i) - N.seqs.begin()), 0});
     }
   }
   b->plan.clear();
-  b->off_unit = append(&b->plan, units);
+  b->off_unit = append(&b->plan, few);
+  b->off_tile_unit = append(&b->plan, large);
+  b->off_cta = append(&b->plan, cta);
   b->off_seq = append(&b->plan, seqs);
   b->off_path = append(&b->plan, paths);
   b->off_span = append(&b->plan, spans);
   b->off_node_seq = append(&b->plan, node_seq);
-  b->n_row_units = (int32_t)units.size();
+  b->n_row_units = (int32_t)few.size();
   b->join = join;
-  b->part_rows = part * p->cfg.n_kv_heads;
+  b->part_rows = part;
   return INFLLM_OK;
 }
 
 }  // namespace
-
-int pages_encode_map(infllm_pages* p) {
-  (void)p;
-  return INFLLM_OK;
-}
 
 }  // namespace infllm
 
@@ -527,9 +514,14 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const i
     const int32_t* plan = (const int32_t*)d_plan;
     P.unit = (const AttnUnit*)(plan + b->off_unit), P.seq = (const AttnSeq*)(plan + b->off_seq);
     P.path = (const AttnPath*)(plan + b->off_path), P.span = (const AttnSpan*)(plan + b->off_span), P.node_seq = plan + b->off_node_seq;
+    P.map = p->map;
+    P.tile_unit = (const AttnUnit*)(plan + b->off_tile_unit), P.cta_unit = plan + b->off_cta;
+    P.page0 = 2 * layer * c.n_pages, P.n_pages = c.n_pages;
+    INFLLM_TRY(tc_get_error_ptr(&P.err));
     P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.group = n_heads / c.n_kv_heads, P.most = b->most;
     P.batch = (int)b->seqs.size();
     P.scale_log2 = scale * kLog2e;
+    if (b->n_ctas > 0) INFLLM_TRY(paged_tc_launch(P, c.dtype, c.head_dim, b->n_ctas, s));
     INFLLM_DISPATCH_DTYPE(c.dtype, T, {
       if (b->n_row_units > 0) {
         auto kern = c.head_dim == 128 ? paged_rows_kernel<T, 128, 2> : paged_rows_kernel<T, 64, 2>;

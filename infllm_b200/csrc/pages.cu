@@ -349,7 +349,9 @@ extern "C" int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages*
       p->free_pages = decltype(p->free_pages)(std::greater<int32_t>(), std::move(all));
       DeviceScope scope(c.device);
       if (!scope.ok()) return fail(INFLLM_E_CUDA, "pages_create: no device %d", c.device);
-      return c.device >= 0 ? pages_encode_map(p) : INFLLM_OK;
+      if (c.device < 0) return INFLLM_OK;
+      INFLLM_CUDA_OK(cudaDeviceGetAttribute(&p->n_sm, cudaDevAttrMultiProcessorCount, c.device));
+      return pages_encode_map(p);
     });
     if (rc != INFLLM_OK) {
       delete p;

@@ -69,7 +69,8 @@ struct infllm_pages {
   uint64_t change = 0;   // any change of what sequences hold
   uint64_t reshape = 0;  // of the pages that a sequence had before
   std::vector<infllm::PageItem> rows, edits, moves;  // of the call that is being made
-  CUtensorMap map;       // of all pages (paged_attn.cu)
+  CUtensorMap map;       // of all pages (paged_tc.cu)
+  int32_t n_sm = 148;
 
   int32_t pages_of(int64_t tokens) const { return (int32_t)((tokens + cfg.page_size - 1) / cfg.page_size); }
 };
@@ -87,13 +88,13 @@ struct infllm_page_batch {
   uint64_t plan_of = ~0ull;
   int32_t plan_heads = 0;
   std::vector<int32_t> plan;
-  int32_t n_row_units = 0;
+  int32_t n_row_units = 0, n_ctas = 0;
   bool join = false;
   int64_t part_rows = 0;
-  int64_t off_unit = 0, off_seq = 0, off_path = 0, off_span = 0, off_node_seq = 0;  // sections of the plan
+  int64_t off_unit = 0, off_tile_unit = 0, off_cta = 0, off_seq = 0, off_path = 0, off_span = 0, off_node_seq = 0;  // sections of the plan
 };
 
 namespace infllm {
 int batch_alive(const infllm_page_batch* b, const char* what);
-int pages_encode_map(infllm_pages* p);  // paged_attn.cu
+int pages_encode_map(infllm_pages* p);  // paged_tc.cu
 }  // namespace infllm
