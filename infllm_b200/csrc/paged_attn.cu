@@ -192,64 +192,125 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid
 }
 
 // ----------------------------------------------------------------------------------------------------------- the join
-// A warp per query head and token: its parts of all nodes of its sequence.  Bound by the latency of two loads behind one
-// another and by the bytes of the partial rows.
-template <typename T, int kDim>
+// kWarps warps per query head and token share the parts of all nodes of its sequence.  Bound by the latency of loads one behind
+// the other: where the parts are is looked up before the kernels before on the stream have ended (it is the plan's), and a
+// part's row is asked for together with its log-sum-exp, four parts at a time.
+template <typename T, int kDim, int kWarps>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams P) {
-  constexpr int kPer = kDim / 32;
-  chain_enter();
-  const int64_t orow = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, heads = P.n_kv * P.group;
-  if (orow >= (int64_t)P.batch * P.most * heads) return;
-  const int h = (int)(orow % heads), i = (int)(orow / heads % P.most), b = (int)(orow / heads / P.most);
+  constexpr int kPer = kDim / 32, kRows = 8 / kWarps, kAhead = 4;
+  __shared__ float sm[8][kDim + 4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = P.n_kv * P.group;
+  const int64_t orow = (int64_t)blockIdx.x * kRows + warp / kWarps;
+  const bool in = orow < (int64_t)P.batch * P.most * heads;
+  const int h = in ? (int)(orow % heads) : 0, i = in ? (int)(orow / heads % P.most) : 0, b = in ? (int)(orow / heads / P.most) : 0;
   const int hkv = h / P.group;
   const AttnSeq S = P.seq[b];
-  float mx = -INFINITY;
-  const bool is = i >= P.most - S.count;  // (a row without a token: zeros)
-  auto parts = [&](auto&& f) {
-    for (int k = 0; k < S.n_path; ++k) {
-      const AttnPath A = P.path[S.path + k];
-      const int r = (A.at * P.most + i) * P.group + h % P.group, tile = r / A.tile;
-      const AttnSpan Z = P.span[(A.span + tile) * P.n_kv + hkv];
-      f((int64_t)Z.part + (r - tile * A.tile), Z.n, (int64_t)Z.rows);
-    }
+  const bool is = in && i >= P.most - S.count;  // (a row without a token: zeros)
+  auto span_of = [&](const AttnPath& A, int* row) {
+    const int r = (A.at * P.most + i) * P.group + h % P.group, tile = r / A.tile;
+    *row = r - tile * A.tile;
+    return P.span[(A.span + tile) * P.n_kv + hkv];
   };
-  bool whole = false;  // written by the unit that had all of it
-  if (is)
-    parts([&](int64_t at, int n, int64_t step) {
-      whole |= n < 0;
-      for (int c = lane; c < n; c += 32) mx = fmaxf(mx, P.part_lse[at + c * step]);
-    });
-  if (whole) return;
-  mx = warp_max(mx);
-  float den = 0.f, acc[kPer];
+  int at[kNearPath], n[kNearPath], step[kNearPath];
+#pragma unroll
+  for (int k = 0; k < kNearPath; ++k) {
+    at[k] = n[k] = step[k] = 0;
+    if (is && k < S.n_path) {
+      int r;
+      const AttnSpan Z = span_of(S.near_path[k], &r);
+      at[k] = Z.part + r, n[k] = Z.n, step[k] = Z.rows;
+    }
+  }
+  chain_enter();
+  const bool whole = n[0] < 0;  // written by the unit that had all of it
+  float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  if (mx != -INFINITY)
-    parts([&](int64_t at, int n, int64_t step) {
-#pragma unroll 4
-      for (int c = 0; c < n; ++c) {
-        const float w = exp2f(P.part_lse[at + c * step] - mx);
-        const float* o = P.part_o + (at + c * step) * kDim + lane * kPer;
-        den += w;
-        if (kPer == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(o);
-          acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]), acc[2 % kPer] = fmaf(w, v.z, acc[2 % kPer]), acc[3 % kPer] = fmaf(w, v.w, acc[3 % kPer]);
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(o);
-          acc[0] = fmaf(w, v.x, acc[0]), acc[1] = fmaf(w, v.y, acc[1]);
-        }
+  auto fold = [&](int first, int count, int stride) {  // this warp's of `count` parts
+    for (int c0 = warp % kWarps; c0 < count; c0 += kWarps * kAhead) {
+      float lse[kAhead], v[kAhead][kPer];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int c = c0 + e * kWarps;
+        lse[e] = -INFINITY;
+        if (c >= count) continue;
+        const int64_t row = (int64_t)first + (int64_t)c * stride;
+        lse[e] = P.part_lse[row];
+        const float* o = P.part_o + row * kDim + lane * kPer;
+        if (kPer == 4) *reinterpret_cast<float4*>(v[e]) = *reinterpret_cast<const float4*>(o);
+        else *reinterpret_cast<float2*>(v[e]) = *reinterpret_cast<const float2*>(o);
       }
-    });
-  const float inv = mx != -INFINITY ? 1.f / den : 0.f;
+      float mx = m;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) mx = fmaxf(mx, lse[e]);
+      if (mx == -INFINITY) continue;
+      const float a = exp2f(m - mx);
+      l *= a;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] *= a;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        if (lse[e] == -INFINITY) continue;
+        const float w = exp2f(lse[e] - mx);
+        l += w;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(w, v[e][k], acc[k]);
+      }
+      m = mx;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kNearPath; ++k) fold(at[k], n[k], step[k]);
+  for (int k = kNearPath; is && k < S.n_path; ++k) {
+    int r;
+    const AttnSpan Z = span_of(P.path[S.path + k - kNearPath], &r);
+    fold(Z.part + r, Z.n, Z.rows);
+  }
+  if (kWarps > 1) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) sm[warp][lane * kPer + k] = acc[k];
+    if (lane == 0) sm[warp][kDim] = m, sm[warp][kDim + 1] = l;
+    __syncthreads();
+    if (warp % kWarps) return;
+    float mx = m;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[warp + w][kDim]);
+    const float ms = mx == -INFINITY ? 0.f : mx, a = exp2f(m - ms);
+    l *= a;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) acc[k] *= a;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      const float wt = exp2f(sm[warp + w][kDim] - ms);
+      l = fmaf(wt, sm[warp + w][kDim + 1], l);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] = fmaf(wt, sm[warp + w][lane * kPer + k], acc[k]);
+    }
+    m = mx;
+  }
+  if (!in || whole) return;
+  const float inv = m != -INFINITY ? 1.f / l : 0.f;
   uint32_t* to = reinterpret_cast<uint32_t*>(P.out + (orow * kDim + lane * kPer) * 2);
 #pragma unroll
   for (int k = 0; k < kPer; k += 2) to[k / 2] = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
-  if (P.lse && lane == 0) P.lse[orow] = mx != -INFINITY ? (mx + log2f(den)) * (1.f / kLog2e) : -INFINITY;
+  if (P.lse && lane == 0) P.lse[orow] = m != -INFINITY ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
+}
+
+template <typename T, int kDim>
+static int join_launch(const PagedParams& P, cudaStream_t s) {
+  // eight warps to a row while that still is one wave of blocks, and one where there are rows enough
+  const int64_t rows = (int64_t)P.batch * P.most * P.n_kv * P.group;
+  if (rows <= 148 * 8) launch_chained(paged_join_kernel<T, kDim, 8>, dim3((unsigned)rows), dim3(256), 0, s, P);
+  else if (rows <= 148 * 32) launch_chained(paged_join_kernel<T, kDim, 4>, dim3((unsigned)ceil_div(rows, 2)), dim3(256), 0, s, P);
+  else launch_chained(paged_join_kernel<T, kDim, 1>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, s, P);
+  INFLLM_LAUNCH_OK("paged_join_kernel");
+  return INFLLM_OK;
 }
 
 // ----------------------------------------------------------------------------------------------------------- the plan
 namespace {
+
+constexpr int kUnitWork = 6;  // what a unit of many rows takes besides its tiles, in tiles of 128 rows
 
 struct Node {
   int64_t key0, key1;
@@ -345,7 +406,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   };
   std::vector<Tile> tiles;
   std::vector<int32_t> first_tile, node_seq;
-  int64_t few_work = 0, many_work = 0;  // groups of 16 keys, and tiles of 128 by up to 128 rows
+  int64_t few_work = 0, many_work = 0, many_units = 0;  // groups of 16 keys, and tiles of 128 by up to 128 rows
   for (const Node& N : tree.nodes) {
     const bool leaf = N.seqs.size() == 1;
     const int64_t rows = (int64_t)N.seqs.size() * most * group;
@@ -359,7 +420,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
       const int64_t keys = std::max<int64_t>(0, end - N.key0);
       AttnUnit u{b->seqs[N.seqs[0]], (int32_t)N.key0, (int32_t)keys, leaf ? (int32_t)(N.key1 - most + 1) : kSeeAll, (int32_t)r, in, (int32_t)node_seq.size(), 0, 0, -1, {0, 0}};
       tiles.push_back({u, many, leaf && tree.path[N.seqs[0]].size() == 1});
-      if (many) many_work += ceil_div(keys, 128) * (in > 128 ? 2 : 1) * n_kv;
+      if (many) many_work += ceil_div(keys, 128) * (in > 128 ? 2 : 1) * n_kv, many_units += keys > 0 ? n_kv : 0;
       else few_work += ceil_div(keys, 16) * n_kv;
     }
     node_seq.insert(node_seq.end(), N.seqs.begin(), N.seqs.end());
@@ -392,8 +453,10 @@ int make_plan(infllm_page_batch* b, int n_heads) {
     part += cut * u.rows * n_kv;
     join = true;
   }
-  // many rows: one list of all key tiles, cut into as many stretches of equal work as there are SMs, or fewer of four tiles
+  // many rows: one list of all key tiles, cut into as many stretches of equal work as there are SMs, or fewer of four tiles;
+  // a unit's begin and end are as long as some tiles
   const int64_t n_cta = std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / 4));
+  many_work += kUnitWork * (many_units + n_cta);
   int64_t done = 0;  // work that has been dealt out
   for (size_t x = 0; x < tiles.size(); ++x) {
     const Tile& t = tiles[x];
@@ -406,14 +469,14 @@ int make_plan(infllm_page_batch* b, int n_heads) {
       for (int64_t k = 0; k < n_tiles || (k == 0 && t.alone);) {
         // up to the end of the block's share; what is left of one tile or less goes along
         const int64_t share = ceil_div(many_work * (int64_t)cta.size(), n_cta);
-        int64_t take = std::min(n_tiles - k, std::max<int64_t>(0, (share - done) / weight));
+        int64_t take = std::min(n_tiles - k, std::max<int64_t>(0, (share - done - kUnitWork) / weight));
         if (n_tiles - k - take <= 1) take = n_tiles - k;
         if (take > 0 || n_tiles == 0) {
           u.key0 = t.unit.key0 + (int32_t)k * 128;
           u.keys = (int32_t)std::min<int64_t>(take * 128, t.unit.keys - k * 128);
           large.push_back(u);
         }
-        k += take, done += take * weight;
+        k += take, done += take > 0 ? take * weight + kUnitWork : 0;
         if (n_tiles == 0) break;
         if (k < n_tiles || done >= share) {
           if ((int64_t)cta.size() < n_cta) cta.push_back((int32_t)large.size());
@@ -436,13 +499,18 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   std::vector<AttnSeq> seqs;
   std::vector<AttnPath> paths;
   for (int i = 0; i < n; ++i) {
-    seqs.push_back({(int32_t)paths.size(), (int32_t)tree.path[i].size(), b->count[i], 0});
+    AttnSeq q{};
+    q.count = b->count[i], q.path = (int32_t)paths.size();
     join |= tree.path[i].empty();
     for (int32_t x : tree.path[i]) {
       const Node& N = tree.nodes[x];
       const int32_t tile = (int64_t)N.seqs.size() * most * group > kRowTile ? kTileRows : kRowTile;
-      paths.push_back({first_tile[x], tile, (int32_t)(std::find(N.seqs.begin(), N.seqs.end(), i) - N.seqs.begin()), 0});
+      const AttnPath a{first_tile[x], tile, (int32_t)(std::find(N.seqs.begin(), N.seqs.end(), i) - N.seqs.begin())};
+      if (q.n_path < kNearPath) q.near_path[q.n_path] = a;
+      else paths.push_back(a);
+      ++q.n_path;
     }
+    seqs.push_back(q);
   }
   b->plan.clear();
   b->off_unit = append(&b->plan, few);
@@ -528,11 +596,7 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const i
         launch_chained(kern, dim3(b->n_row_units, c.n_kv_heads), dim3(kRowWarps * 32), 0, s, P);
         INFLLM_LAUNCH_OK("paged_rows_kernel");
       }
-      if (b->join) {
-        const int64_t rows = (int64_t)P.batch * P.most * n_heads;
-        launch_chained(c.head_dim == 128 ? paged_join_kernel<T, 128> : paged_join_kernel<T, 64>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, s, P);
-        INFLLM_LAUNCH_OK("paged_join_kernel");
-      }
+      if (b->join) INFLLM_TRY((c.head_dim == 128 ? join_launch<T, 128>(P, s) : join_launch<T, 64>(P, s)));
     });
     return INFLLM_OK;
   });

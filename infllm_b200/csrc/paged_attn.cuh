@@ -17,14 +17,17 @@ struct alignas(16) AttnUnit {
   int32_t part;       // first partial row; -1: the rows are whole, and go to the output
   int32_t pad[2];
 };
-struct alignas(16) AttnSeq {   // of a sequence of the batch, for the join
-  int32_t path, n_path;        // its nodes
-  int32_t count, pad;
+struct AttnPath {
+  int32_t span, tile;  // the node's first row tile, rows of a tile
+  int32_t at;          // place of the sequence in the node
 };
-struct alignas(16) AttnPath {
-  int32_t span, tile;          // the node's first row tile, rows of a tile
-  int32_t at, pad;             // place of the sequence in the node
+constexpr int kNearPath = 4;
+struct alignas(16) AttnSeq {   // of a sequence of the batch, for the join: its nodes,
+  int32_t count, n_path, path; // the first of them here, the others at `path` behind one another
+  AttnPath near_path[kNearPath];
+  int32_t pad;
 };
+static_assert(sizeof(AttnSeq) == 64, "");
 struct alignas(16) AttnSpan {  // of a row tile of a node and a KV head: n partials of `rows` rows, one behind the other
   int32_t part, n, rows, pad;
 };

@@ -237,17 +237,30 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
       const int rows = works ? min(128, U.rows - team * 128) : 0, step = two ? 1 : 2;
       // ---- queries: 16-byte pieces of rows, swizzled as TMA would have
       if (works && n > 0) {
-        constexpr int kPer = kDim / 8;
-        const int c = tid % kPer;
+        constexpr int kPer = kDim / 8, kStep = 128 / kPer;
+        const int c = tid % kPer, r0 = tid / kPer;
         unsigned char* to = smem + L::kQ + team * L::kTileBytes + (c >> 3) * kSubTileBytes;
-#pragma unroll 4
-        for (int r = tid / kPer; r < 128; r += 128 / kPer) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < rows) {
-            const RowAt a = row_at(P, U.node_seq, U.row0 + team * 128 + r);
-            v = __ldg(reinterpret_cast<const uint4*>(P.q + a.b * P.q_bs + (int64_t)(U.hkv * P.group + a.h) * P.q_hs + a.i * P.q_ts + c * 16));
+        // (all rows' places, then all rows, in two rounds of eight: loads one behind the other are what a unit's begin waits for)
+#pragma unroll
+        for (int g = 0; g < kPer; g += 8) {
+          const char* from[8];
+          uint4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = r0 + (g + k) * kStep;
+            from[k] = nullptr;
+            if (r < rows) {
+              const RowAt a = row_at(P, U.node_seq, U.row0 + team * 128 + r);
+              from[k] = P.q + a.b * P.q_bs + (int64_t)(U.hkv * P.group + a.h) * P.q_hs + a.i * P.q_ts + c * 16;
+            }
           }
-          *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = from[k] ? __ldg(reinterpret_cast<const uint4*>(from[k])) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = r0 + (g + k) * kStep;
+            *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
