@@ -541,7 +541,9 @@ int infllm_ctx_load(infllm_ctx* ctx, const char* path, void* stream);
  * after the other.  All calls on a cache belong on one stream, or are ordered by the caller; one host thread at a time.
  *
  * d_pages (n_layers, 2: keys and values, n_pages, n_kv_heads, page_size, head_dim), d_table (max_sequences, max_pages);
- * head_dim 64 or 128, page_size 16, 32, 64 or 128.  device < 0: bookkeeping only, without a GPU. */
+ * head_dim 64 or 128, page_size 16, 32, 64 or 128.  device < 0: bookkeeping only, without a GPU.
+ * Tensors of a batch's calls are (batch, heads, tokens, head_dim) with strides in elements (bs, hs, ts) that are multiples of 8;
+ * their bases are 16-byte aligned. */
 typedef struct infllm_pages infllm_pages;
 typedef struct infllm_page_batch infllm_page_batch;
 typedef struct infllm_pages_config {
@@ -549,12 +551,6 @@ typedef struct infllm_pages_config {
   void* d_pages;
   int32_t* d_table;
 } infllm_pages_config;
-/* Rows (batch, heads, tokens, head_dim): strides in elements, multiples of 8; the base 16-byte aligned. */
-typedef struct infllm_page_rows {
-  const void* d;
-  int64_t bs, hs, ts;
-} infllm_page_rows;
-
 int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages** out);
 int infllm_pages_destroy(infllm_pages* p);
 int infllm_pages_open(infllm_pages* p, int n, int32_t* out); /* n empty sequences */
@@ -579,26 +575,28 @@ int infllm_pages_free_count(const infllm_pages* p); /* free pages */
  *   extend    room for counts[i] more tokens, which become the newest
  *   retract   takes counts[i] tokens back (no token is newest then)
  *   select    the newest counts[i] tokens that are there
+ *             (counts NULL: `same` for every sequence; *reach, if given: the rows that a rotary table has to have)
  *   write     a layer's keys and values of the newest tokens into their pages, and q to d_q_out (batch, tokens, n_heads,
  *             head_dim); with d_cos / d_sin (table_len, head_dim / 2) keys and queries rotated to the tokens' positions.
  *             q may be NULL.
  *   attend    attention of the newest tokens: each sees its sequence's tokens up to itself.  d_out (batch, tokens, n_heads,
  *             head_dim), d_lse (batch, tokens, n_heads) fp32 log-sum-exp of the scores (natural logarithm), or NULL.
- *             d_plan and d_scratch are the caller's, 16-byte aligned, of the sizes that infllm_page_batch_plan gives; that
- *             call also works out the plan, which holds for all layers until a sequence of the cache changes.  d_plan is
- *             uploaded by the attend call with `upload` set: the first one after the plan. */
+ *             d_work is the caller's, 16-byte aligned, of the size that infllm_page_batch_plan gives.  That call works out
+ *             the plan, which holds for all layers until a sequence of the cache changes: attend returns
+ *             INFLLM_PAGES_NO_PLAN where there is none for n_heads.  The first attend call after it uploads the plan to
+ *             d_work, which the later ones have to be given too. */
+#define INFLLM_PAGES_NO_PLAN 1
 int infllm_page_batch_create(infllm_pages* p, const int32_t* seqs, int n, infllm_page_batch** out);
 int infllm_page_batch_destroy(infllm_page_batch* b);
-int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* counts, void* stream);
-int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* counts);
-int infllm_page_batch_select(infllm_page_batch* b, const int32_t* counts);
-int64_t infllm_page_batch_reach(const infllm_page_batch* b); /* rows that the tables have to have: the largest next position */
-int infllm_page_batch_write(infllm_page_batch* b, int layer, const infllm_page_rows* k, const infllm_page_rows* v,
-                            const infllm_page_rows* q, void* d_q_out, int n_heads, const float* d_cos, const float* d_sin,
-                            int64_t table_len, void* stream);
-int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* plan_bytes, int64_t* scratch_bytes, int* fresh);
-int infllm_page_batch_attend(infllm_page_batch* b, int layer, const infllm_page_rows* q, void* d_out, float* d_lse, int n_heads,
-                             float scale, void* d_plan, int upload, void* d_scratch, void* stream);
+int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* counts, int32_t same, int64_t* reach, void* stream);
+int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* counts, int32_t same);
+int infllm_page_batch_select(infllm_page_batch* b, const int32_t* counts, int32_t same, int64_t* reach);
+int infllm_page_batch_write(infllm_page_batch* b, int layer, const void* d_k, int64_t k_bs, int64_t k_hs, int64_t k_ts, const void* d_v,
+                            int64_t v_bs, int64_t v_hs, int64_t v_ts, const void* d_q, int64_t q_bs, int64_t q_hs, int64_t q_ts,
+                            void* d_q_out, int n_heads, const float* d_cos, const float* d_sin, int64_t table_len, void* stream);
+int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* work_bytes);
+int infllm_page_batch_attend(infllm_page_batch* b, int layer, const void* d_q, int64_t q_bs, int64_t q_hs, int64_t q_ts, void* d_out,
+                             float* d_lse, int n_heads, float scale, void* d_work, void* stream);
 
 /* ----------------------------------------------------- host logic, GPU-free
  * The LRU table alone (context_manager.py:246-265, 495-515): dict-ordered ids with stamps.

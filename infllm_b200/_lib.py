@@ -15,6 +15,7 @@ BF16, FP16 = 0, 1
 CACHE_LRU, CACHE_LRU_S = 0, 1
 MASK_NONE, MASK_WINDOW, MASK_COMPLEMENT = 0, 1, 2
 MAX_SEGMENTS = 80
+PAGES_NO_PLAN = 1
 PROF_ATTN, PROF_COLSUM, PROF_DECODE, PROF_TOPK, PROF_SLOTS = 0, 1, 2, 3, 4
 
 
@@ -73,11 +74,6 @@ class PagesConfig(ctypes.Structure):
     """infllm_pages_config of include/infllm_b200.h."""
     _fields_ = [(n, c_int32) for n in ("n_layers", "n_kv_heads", "head_dim", "page_size", "n_pages", "max_sequences", "max_pages",
                                        "dtype", "device", "pad")] + [("d_pages", c_void_p), ("d_table", c_void_p)]
-
-
-class PageRows(ctypes.Structure):
-    """infllm_page_rows of include/infllm_b200.h."""
-    _fields_ = [("d", c_void_p), ("bs", c_int64), ("hs", c_int64), ("ts", c_int64)]
 
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -214,14 +210,13 @@ SIGNATURES = {
     "infllm_pages_free_count": (c_int, [c_void_p]),
     "infllm_page_batch_create": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_void_p)]),
     "infllm_page_batch_destroy": (c_int, [c_void_p]),
-    "infllm_page_batch_extend": (c_int, [c_void_p, POINTER(c_int32), c_void_p]),
-    "infllm_page_batch_retract": (c_int, [c_void_p, POINTER(c_int32)]),
-    "infllm_page_batch_select": (c_int, [c_void_p, POINTER(c_int32)]),
-    "infllm_page_batch_reach": (c_int64, [c_void_p]),
-    "infllm_page_batch_write": (c_int, [c_void_p, c_int, POINTER(PageRows), POINTER(PageRows), POINTER(PageRows), c_void_p, c_int,
-                                        c_void_p, c_void_p, c_int64, c_void_p]),
-    "infllm_page_batch_plan": (c_int, [c_void_p, c_int, POINTER(c_int64), POINTER(c_int64), POINTER(c_int)]),
-    "infllm_page_batch_attend": (c_int, [c_void_p, c_int, POINTER(PageRows), c_void_p, c_void_p, c_int, c_float, c_void_p, c_int,
+    "infllm_page_batch_extend": (c_int, [c_void_p, POINTER(c_int32), c_int32, POINTER(c_int64), c_void_p]),
+    "infllm_page_batch_retract": (c_int, [c_void_p, POINTER(c_int32), c_int32]),
+    "infllm_page_batch_select": (c_int, [c_void_p, POINTER(c_int32), c_int32, POINTER(c_int64)]),
+    "infllm_page_batch_write": (c_int, [c_void_p, c_int] + [c_void_p, c_int64, c_int64, c_int64] * 3 +
+                                [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "infllm_page_batch_plan": (c_int, [c_void_p, c_int, POINTER(c_int64)]),
+    "infllm_page_batch_attend": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_float,
                                          c_void_p, c_void_p]),
     "infllm_lru_create": (c_int, [c_int, POINTER(c_void_p)]),
     "infllm_lru_destroy": (c_int, [c_void_p]),

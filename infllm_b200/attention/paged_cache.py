@@ -148,9 +148,10 @@ class PagedBatch:
         self.cache, self.seqs = cache, list(seqs)
         self._n = len(self.seqs)
         self.tokens = 0  # of the step's tensors
-        self._plan = None
-        self._sizes = c_int64(), c_int64(), ctypes.c_int()
-        self._size_refs = tuple(ctypes.byref(x) for x in self._sizes)
+        self._work, self._work_at = None, 0  # the plan on the device, and room for partial results
+        self._reach = c_int64()  # rows that a rotary table has to have
+        self._reach_ref = ctypes.byref(self._reach)
+        self._scale = 1.0 / math.sqrt(cache.head_dim)
         self.handle = ctypes.c_void_p()
         _lib.check(_lib_call.infllm_page_batch_create(cache.handle, _ids(self.seqs), self._n, ctypes.byref(self.handle)))
 
@@ -164,67 +165,72 @@ class PagedBatch:
 
     def _counts(self, n):
         if isinstance(n, int):
-            return (c_int32 * self._n)(*[n] * self._n), n
+            return None, n, n
         if len(n) != self._n:
             raise ValueError(f"{self._n} sequences and {len(n)} counts")
-        return _ids(n), max(n)
+        return _ids(n), 0, max(n)
 
     def extend(self, n):
         """Room for n more tokens of every sequence, or for n[i]: they are the step's."""
-        counts, most = self._counts(n)
-        _lib.check(_lib_call.infllm_page_batch_extend(self.handle, counts, _lib.raw_stream(self.cache.device)))
+        counts, same, most = self._counts(n)
+        rc = _lib_call.infllm_page_batch_extend(self.handle, counts, same, self._reach_ref, _lib.raw_stream(self.cache.device))
+        if rc:
+            _lib.check(rc)
         self.tokens = most
 
     def plan(self, n):
         """The newest n tokens of every sequence, or n[i], that are there already, are the step's."""
-        counts, most = self._counts(n)
-        _lib.check(_lib_call.infllm_page_batch_select(self.handle, counts))
+        counts, same, most = self._counts(n)
+        _lib.check(_lib_call.infllm_page_batch_select(self.handle, counts, same, self._reach_ref))
         self.tokens = most
 
     def retract(self, n):
         """Takes the newest n tokens of every sequence, or n[i], back, as a speculative decoder does with drafts."""
-        counts, _ = self._counts(n)
-        _lib.check(_lib_call.infllm_page_batch_retract(self.handle, counts))
+        counts, same, _ = self._counts(n)
+        rc = _lib_call.infllm_page_batch_retract(self.handle, counts, same)
+        if rc:
+            _lib.check(rc)
         self.tokens = 0
 
     def _rows(self, t, heads, what):
-        """(batch, heads, tokens, head_dim) as the library takes it, and the tensor that has to live until the call."""
+        """A tensor (batch, heads, tokens, head_dim) with 16-byte aligned rows, copied if it has others; address and strides."""
         c = self.cache
-        if t.device != c.device:
-            raise RuntimeError(f"{what} must be on {c.device}: infllm_b200 has no CPU path")
-        if t.dtype != c.dtype:
-            raise TypeError(f"{what} is {t.dtype}, the cache {c.dtype}")
         if t.shape != (self._n, heads, self.tokens, c.head_dim):
             raise ValueError(f"{what} is {tuple(t.shape)}, not {(self._n, heads, self.tokens, c.head_dim)}")
+        if t.dtype != c.dtype:
+            raise TypeError(f"{what} is {t.dtype}, the cache {c.dtype}")
+        if t.device != c.device:
+            raise RuntimeError(f"{what} must be on {c.device}: infllm_b200 has no CPU path")
         bs, hs, ts, ds = t.stride()
         at = t.data_ptr()
         if ds != 1 or (bs | hs | ts) % 8 or at % 16:
             t = t.clone(memory_format=torch.contiguous_format)
             bs, hs, ts, _ = t.stride()
             at = t.data_ptr()
-        return _lib.PageRows(at, bs, hs, ts), t
+        return t, at, bs, hs, ts
 
     def write(self, layer, k, v, q=None, rope=None):
         """The step's keys and values (batch, n_kv_heads, tokens, head_dim) into a layer's pages.  With `rope`, a
         RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q)."""
         c = self.cache
-        rk, k = self._rows(k, c.n_kv_heads, "k")
-        rv, v = self._rows(v, c.n_kv_heads, "v")
-        rq = out = cos = sin = None
-        heads = rows = at = 0
+        k, k_at, k_bs, k_hs, k_ts = self._rows(k, c.n_kv_heads, "k")
+        v, v_at, v_bs, v_hs, v_ts = self._rows(v, c.n_kv_heads, "v")
+        out = q_at = at = cos = sin = None
+        q_bs = q_hs = q_ts = heads = rows = 0
         if q is not None:
             heads = q.size(1)
-            rq, q = self._rows(q, heads, "q")
+            q, q_at, q_bs, q_hs, q_ts = self._rows(q, heads, "q")
             out = torch.empty((self._n, self.tokens, heads, c.head_dim), dtype=c.dtype, device=c.device)
             at = out.data_ptr()
-            rq = ctypes.byref(rq)
         if rope is not None:
             if not isinstance(rope, RotaryEmbeddingESM) or rope.dim != c.head_dim:
                 raise ValueError(f"rope must be a RotaryEmbeddingESM of {c.head_dim} dimensions")
-            cos, sin = rope._tables(max(_lib_call.infllm_page_batch_reach(self.handle), 1), c.device)
+            cos, sin = rope._tables(max(self._reach.value, 1), c.device)
             rows, cos, sin = cos.size(0), cos.data_ptr(), sin.data_ptr()
-        _lib.check(_lib_call.infllm_page_batch_write(self.handle, layer, ctypes.byref(rk), ctypes.byref(rv), rq, at, heads, cos, sin, rows,
-                                                     _lib.raw_stream(c.device)))
+        rc = _lib_call.infllm_page_batch_write(self.handle, layer, k_at, k_bs, k_hs, k_ts, v_at, v_bs, v_hs, v_ts, q_at, q_bs, q_hs, q_ts,
+                                               at, heads, cos, sin, rows, _lib.raw_stream(c.device))
+        if rc:
+            _lib.check(rc)
         return None if out is None else out.permute(0, 2, 1, 3)
 
     def attend(self, layer, q, scale=None, return_lse=False):
@@ -232,23 +238,25 @@ class PagedBatch:
         `scale` of the scores: 1 / sqrt(head_dim) if not given.  Returns (batch, n_heads, tokens, head_dim), a view of
         (batch, tokens, n_heads, head_dim); with return_lse also the scores' log-sum-exps (batch, n_heads, tokens), fp32."""
         c = self.cache
-        heads = q.size(1) if q.dim() == 4 else 0
-        rq, q = self._rows(q, heads, "q")
-        rc = _lib_call.infllm_page_batch_plan(self.handle, heads, *self._size_refs)
-        if rc:
-            _lib.check(rc)
-        plan_bytes, scratch_bytes, fresh = (x.value for x in self._sizes)
-        if fresh or self._plan is None:  # (memory of its own: the last plan may still be in use)
-            fresh = 1
-            self._plan = torch.empty(max(plan_bytes, 16), dtype=torch.uint8, device=c.device)
-        scratch = torch.empty(max(scratch_bytes, 16), dtype=torch.uint8, device=c.device)
+        heads = q.size(1)
+        q, at, bs, hs, ts = self._rows(q, heads, "q")
         out = torch.empty((self._n, self.tokens, heads, c.head_dim), dtype=c.dtype, device=c.device)
-        lse = torch.empty((self._n, self.tokens, heads), dtype=torch.float32, device=c.device) if return_lse else None
-        rc = _lib_call.infllm_page_batch_attend(self.handle, layer, ctypes.byref(rq), out.data_ptr(), lse.data_ptr() if return_lse else None,
-                                                heads, 1.0 / math.sqrt(c.head_dim) if scale is None else scale, self._plan.data_ptr(), fresh,
-                                                scratch.data_ptr(), _lib.raw_stream(c.device))
+        lse = lse_at = None
+        if return_lse:
+            lse = torch.empty((self._n, self.tokens, heads), dtype=torch.float32, device=c.device)
+            lse_at = lse.data_ptr()
+        scale = self._scale if scale is None else scale
+        stream = _lib.raw_stream(c.device)
+        rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at, stream)
+        if rc == _lib.PAGES_NO_PLAN:  # the first layer of a step
+            size = c_int64()
+            _lib.check(_lib_call.infllm_page_batch_plan(self.handle, heads, ctypes.byref(size)))
+            # (memory of its own: the last plan may still be in use)
+            self._work = torch.empty(max(size.value, 16), dtype=torch.uint8, device=c.device)
+            self._work_at = self._work.data_ptr()
+            rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at,
+                                                    stream)
         if rc:
-            self._plan = None
             _lib.check(rc)
         out = out.permute(0, 2, 1, 3)
         return (out, lse.permute(0, 2, 1)) if return_lse else out

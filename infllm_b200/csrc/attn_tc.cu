@@ -75,7 +75,6 @@ constexpr int kXmax = kTmax + 4 * 1024;          // per team: the reference its 
 constexpr int kXsum = kXmax + 2 * 512;           // per team: row sums
 constexpr int kPlan = kXsum + 2 * 512;
 constexpr int kTotal = kPlan + 32 + kMaxSeg * 32;
-constexpr int kPolyEvery = 8;
 enum { T3_Q_FULL0 = 0, T3_K_FULL0 = 2, T3_K_EMPTY0 = 6, T3_V_FULL0 = 10, T3_V_EMPTY0 = 14, T3_S_FULL0 = 18,
        T3_P_FULL0 = 21, T3_PV_DONE0 = 24, T3_O_FULL = 27, T3_N_BARS };
 constexpr int kWarpTma = 8, kWarpPv = 9, kWarpQk = 10;  // behind the eight softmax warps
@@ -172,45 +171,11 @@ __device__ __forceinline__ uint64_t look_word(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ void leave_word(uint32_t addr, uint64_t v) { asm volatile("st.volatile.shared.b64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
-// exponentials of 32 columns of a row, packed; sums into rs
-template <typename T, bool kExact>
-__device__ __forceinline__ void exp_chunk(const float2* a, float2* rs, uint32_t* pk) {
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    float2 p;
-    if (k % kPolyEvery == kPolyEvery - 1) {
-      p = ex2_poly2<kExact ? 5 : 3>(a[k]);  // one pair in kPolyEvery off the special-function unit
-    } else {
-      p = make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
-    }
-    rs[k & 3] = fadd2(rs[k & 3], p);
-    typename Act<T>::T2 v = Act<T>::from_f2(p.x, p.y);
-    pk[k] = *reinterpret_cast<uint32_t*>(&v);
-  }
-}
-// 32 columns of scores into exponents; what they were loaded into may be loaded into again behind it
-__device__ __forceinline__ void arg_chunk(const float* s, float sc, float neg_m, float2* a) {
-  const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    a[k] = ffma2(s[2 * k], s[2 * k + 1], sc2, nm2);
-    asm volatile("" : "+f"(a[k].x), "+f"(a[k].y));
-  }
-}
 // a row's reference maximum behind a tile whose maximum is m_tile.  Lazy: it only moves when the maximum grew by more than
 // 2^8 - or, kExact, at all, so that the largest probabilities of a row are the ones that a 16-bit P holds without a rounding
 template <bool kExact>
 __device__ __forceinline__ float next_ref(float m, float m_tile) {
   return m_tile - m > (kExact ? 0.f : 8.f) ? m_tile : m;  // (from -inf: any number)
-}
-__device__ __forceinline__ void max_chunk(const float* s, float* mx) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    mx[0] = fmax3(mx[0], s[i], s[i + 1]);
-    mx[1] = fmax3(mx[1], s[i + 2], s[i + 3]);
-    mx[2] = fmax3(mx[2], s[i + 4], s[i + 5]);
-    mx[3] = fmax3(mx[3], s[i + 6], s[i + 7]);
-  }
 }
 }  // namespace tc3
 
@@ -563,7 +528,7 @@ __global__ void __launch_bounds__(tc3::kThreads, 1) attn_tc3_kernel(const __grid
           uint32_t pk[16];
           arg_chunk(sa, P.scale_log2, neg_m, e);
           tmem_ld32_if(c < 3, tS + 32 * c + 32, ua);
-          exp_chunk<T, kExact>(e, rs, pk);
+          exp_chunk<T, kExact ? 5 : 3>(e, rs, pk);
           tmem_st16(tS + 16 * c, pk);
           tmem_wait_ld32(ua);
         }

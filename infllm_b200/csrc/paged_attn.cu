@@ -13,150 +13,39 @@
 #include <algorithm>
 #include <cstring>
 
-#include "decode_warp.cuh"
 #include "attn_tc.cuh"
-#include "paged_attn.cuh"
+#include "paged_rows.cuh"
 
 namespace infllm {
 
 using namespace mma;
 
 // ------------------------------------------------------------------------------------------------------- few rows
-// Up to 16 rows: a unit's keys in groups of 16, a warp per group; keys and values go from global memory straight into the
-// registers that are the operands of the m16n8k16 products (decode_warp.cuh has the same arrangement for eight rows of 128
-// dimensions).  It is bound by the bytes of the keys and values.
-constexpr int kRowWarps = 4;
-constexpr int kRowTile = 16;
-
-template <typename T, int kDim, int kNt>  // kNt: tiles of eight rows
+// Four warps share a unit's groups of 16 keys and meet in shared memory.
+template <typename T, int kDim, int kNt>
 __global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid_constant__ PagedParams P) {
-  constexpr int kJ = kDim / 32;   // 16-byte pieces of a row that a thread has as scores' operands
-  constexpr int kH = kDim / 64;   // of a value's row
-  constexpr int kPitch = kDim + 4;
+  constexpr int kH = kDim / 64, kPitch = kDim + 4;
   __shared__ __align__(16) float sm_o[kRowWarps][8 * kNt][kPitch];
   __shared__ float sm_m[kRowWarps][8 * kNt], sm_l[kRowWarps][8 * kNt];
-  chain_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const AttnUnit U = P.unit[blockIdx.x];
   const int hkv = blockIdx.y;
-  uint4 qf[kNt][kJ];
-  int lim[kNt];
+  RowsWarp<T, kDim, kNt> W;
+  W.find(P, U, hkv);
+  chain_enter();
+  W.begin(P);
+  W.template groups<false>(P, U, hkv, warp, kRowWarps);
+  W.sums();
+  // dimension half*64 + g*8 + i at half*64 + i*8 + g, for the banks' sake
 #pragma unroll
   for (int x = 0; x < kNt; ++x) {
-    const int r = x * 8 + g;
-    lim[x] = 0;
-#pragma unroll
-    for (int j = 0; j < kJ; ++j) qf[x][j] = make_uint4(0, 0, 0, 0);
-    if (r < U.rows) {
-      const RowAt a = row_at(P, U.node_seq, U.row0 + r);
-      // (a row without a token sees nothing)
-      lim[x] = a.i < P.most - __ldg(&P.seq[a.b].count) ? 0 : min(U.lim0 + a.i, U.key0 + U.keys);
-      const char* qp = P.q + a.b * P.q_bs + (int64_t)(hkv * P.group + a.h) * P.q_hs + a.i * P.q_ts;
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) qf[x][j] = __ldg(reinterpret_cast<const uint4*>(qp + j * 64 + t * 16));
-    }
-  }
-  float ot[8][kNt][4], m[kNt], l[kNt];
-#pragma unroll
-  for (int x = 0; x < kNt; ++x) {
-    m[x] = -INFINITY, l[x] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ot[i][x][0] = ot[i][x][1] = ot[i][x][2] = ot[i][x][3] = 0.f;
-  }
-  const int32_t* row = P.table + (int64_t)U.row * P.max_pages;
-  const int n_groups = (U.keys + 15) / 16;
-#pragma unroll 1
-  for (int it = warp; it < n_groups; it += kRowWarps) {
-    const int j0 = U.key0 + it * 16, nk = min(16, U.key0 + U.keys - j0);
-    const char* kb = P.pages + (((int64_t)__ldg(row + j0 / P.page) * P.n_kv + hkv) * P.page + j0 % P.page) * (kDim * 2);
-    const char* vb = kb + P.plane;
-    uint4 kr[2][kJ], vr[4][kH];
-    // (what lies behind the last key is not read: it is not a number in the worst case, and 0 times that is none)
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const int r = nt * 8 + g;
-      const char* rp = kb + (r < nk ? r : nk - 1) * (kDim * 2) + t * 16;
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) kr[nt][j] = ld_stream16(rp + j * 64);
-    }
-#pragma unroll
-    for (int ki = 0; ki < 4; ++ki) {
-      const int r = 2 * t + (ki & 1) + (ki >> 1) * 8;
-      const char* rp = vb + (r < nk ? r : nk - 1) * (kDim * 2) + g * 16;
-#pragma unroll
-      for (int j = 0; j < kH; ++j) vr[ki][j] = ld_stream16(rp + j * 128);
-    }
-    float s[2][4];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        const uint32_t a0[4] = {qf[0][j].x, kNt > 1 ? qf[kNt - 1][j].x : 0u, qf[0][j].y, kNt > 1 ? qf[kNt - 1][j].y : 0u};
-        mma16816<T>(s[nt], a0, kr[nt][j].x, kr[nt][j].y);
-        const uint32_t a1[4] = {qf[0][j].z, kNt > 1 ? qf[kNt - 1][j].z : 0u, qf[0][j].w, kNt > 1 ? qf[kNt - 1][j].w : 0u};
-        mma16816<T>(s[nt], a1, kr[nt][j].z, kr[nt][j].w);
-      }
-    }
-    uint32_t pb[kNt][2];
-#pragma unroll
-    for (int x = 0; x < kNt; ++x) {  // row x * 8 + g: keys nt * 8 + 2t + e
-      float v[4], mx = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = j0 + (k >> 1) * 8 + 2 * t + (k & 1);
-        v[k] = key < lim[x] ? s[k >> 1][x * 2 + (k & 1)] * P.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, v[k]);
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[x], mx), ms = mn == -INFINITY ? 0.f : mn;
-      const float al = exp2f(m[x] - ms);
-      m[x] = mn;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = exp2f(v[k] - ms);
-      l[x] = l[x] * al + (v[0] + v[1]) + (v[2] + v[3]);
-      pb[x][0] = pack2<T>(v[0], v[1]), pb[x][1] = pack2<T>(v[2], v[3]);
-      // this thread's columns of O^T are rows 2t and 2t + 1
-      const float a0 = __shfl_sync(0xffffffffu, al, (2 * t) * 4), a1 = __shfl_sync(0xffffffffu, al, (2 * t + 1) * 4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ot[i][x][0] *= a0;
-        ot[i][x][1] *= a1;
-        ot[i][x][2] *= a0;
-        ot[i][x][3] *= a1;
-      }
-    }
-    const uint32_t* w[4][kH];
-#pragma unroll
-    for (int ki = 0; ki < 4; ++ki)
-#pragma unroll
-      for (int j = 0; j < kH; ++j) w[ki][j] = reinterpret_cast<const uint32_t*>(&vr[ki][j]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i >> 1;
-      const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;  // the high or the low 16 bits of both words
-      uint32_t a[4];
-      a[0] = __byte_perm(w[0][0][r], w[1][0][r], sel);  // dimension g*8+i of keys 2t, 2t+1
-      a[2] = __byte_perm(w[2][0][r], w[3][0][r], sel);  // of keys 2t+8, 2t+9
-      a[1] = kH > 1 ? __byte_perm(w[0][kH - 1][r], w[1][kH - 1][r], sel) : 0u;  // dimension 64+g*8+i
-      a[3] = kH > 1 ? __byte_perm(w[2][kH - 1][r], w[3][kH - 1][r], sel) : 0u;
-#pragma unroll
-      for (int x = 0; x < kNt; ++x) mma16816<T>(ot[i][x], a, pb[x][0], pb[x][1]);
-    }
-  }
-  // the warps' results meet in shared memory; dimension half*64 + g*8 + i at half*64 + i*8 + g, for the banks' sake
-#pragma unroll
-  for (int x = 0; x < kNt; ++x) {
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-    if (t == 0) sm_m[warp][x * 8 + g] = m[x], sm_l[warp][x * 8 + g] = l[x];
+    if (t == 0) sm_m[warp][x * 8 + g] = W.m[x], sm_l[warp][x * 8 + g] = W.l[x];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        sm_o[warp][x * 8 + 2 * t + e][i * 8 + g] = ot[i][x][e];
-        if (kH > 1) sm_o[warp][x * 8 + 2 * t + e][64 % kDim + i * 8 + g] = ot[i][x][2 + e];
+        sm_o[warp][x * 8 + 2 * t + e][i * 8 + g] = W.ot[i][x][e];
+        if (kH > 1) sm_o[warp][x * 8 + 2 * t + e][64 % kDim + i * 8 + g] = W.ot[i][x][2 + e];
       }
   }
   __syncthreads();
@@ -243,15 +132,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
       float mx = m;
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) mx = fmaxf(mx, lse[e]);
-      if (mx == -INFINITY) continue;
-      const float a = exp2f(m - mx);
+      const float ref = mx == -INFINITY ? 0.f : mx;  // (a part that is no number is not seen by the maximum)
+      const float a = exp2f(m - ref);
       l *= a;
 #pragma unroll
       for (int k = 0; k < kPer; ++k) acc[k] *= a;
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
         if (lse[e] == -INFINITY) continue;
-        const float w = exp2f(lse[e] - mx);
+        const float w = exp2f(lse[e] - ref);
         l += w;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) acc[k] = fmaf(w, v[e][k], acc[k]);
@@ -289,11 +178,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     m = mx;
   }
   if (!in || whole) return;
-  const float inv = m != -INFINITY ? 1.f / l : 0.f;
+  const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
   uint32_t* to = reinterpret_cast<uint32_t*>(P.out + (orow * kDim + lane * kPer) * 2);
 #pragma unroll
   for (int k = 0; k < kPer; k += 2) to[k / 2] = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
-  if (P.lse && lane == 0) P.lse[orow] = m != -INFINITY ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
+  if (P.lse && lane == 0) P.lse[orow] = l > 0.f ? (m + log2f(l)) * (1.f / kLog2e) : l == 0.f ? -INFINITY : l;
 }
 
 template <typename T, int kDim>
@@ -310,6 +199,7 @@ static int join_launch(const PagedParams& P, cudaStream_t s) {
 // ----------------------------------------------------------------------------------------------------------- the plan
 namespace {
 
+constexpr int kGroupWork = 2;  // what a group of 16 keys of few rows takes a warp beside the products, in tiles of 128 rows
 constexpr int kUnitWork = 6;  // what a unit of many rows takes besides its tiles, in tiles of 128 rows
 
 struct Node {
@@ -431,14 +321,21 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   std::vector<AttnSpan> spans(tiles.size() * n_kv);
   int64_t part = 0;
   bool join = false;
-  // few rows: units of equal work, four blocks per SM, a warp's groups of 16 keys at least
-  const int64_t chunk = std::max<int64_t>(kRowWarps, ceil_div(ceil_div(few_work, p->n_sm * 4), kRowWarps) * kRowWarps) * 16;
+  // few rows: units of equal work.  Beside a kernel of many rows two warps of each of its blocks take them, one unit each, as
+  // long as that takes no longer than the products (a group of 16 keys about two tiles of 128 rows); otherwise blocks of
+  // four warps, four per SM.
+  const int64_t n_cta = many_units ? std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / 4)) : 0;
+  const bool beside = n_cta > 0 && few_work * kGroupWork <= 2 * (many_work + kUnitWork * (many_units + n_cta));
+  const int64_t warps = beside ? 1 : kRowWarps, units = beside ? 2 * n_cta : p->n_sm * 4;
+  const int64_t chunk = std::max<int64_t>(warps, ceil_div(ceil_div(few_work, units), warps) * warps) * 16;
+  int32_t most_rows = 0;
   for (size_t x = 0; x < tiles.size(); ++x) {
     const Tile& t = tiles[x];
     if (t.many) continue;
     const int64_t keys = t.unit.keys, cut = ceil_div(keys, chunk), each = cut ? ceil_div(ceil_div(keys, 16), cut) * 16 : 0;
     AttnUnit u = t.unit;
-    const bool whole = t.alone && cut <= 1;
+    most_rows = std::max(most_rows, u.rows);
+    const bool whole = t.alone && cut <= 1 && !beside;
     if (whole) {
       few.push_back(u);
       for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h].n = -1;
@@ -455,7 +352,6 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   }
   // many rows: one list of all key tiles, cut into as many stretches of equal work as there are SMs, or fewer of four tiles;
   // a unit's begin and end are as long as some tiles
-  const int64_t n_cta = std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / 4));
   many_work += kUnitWork * (many_units + n_cta);
   int64_t done = 0;  // work that has been dealt out
   for (size_t x = 0; x < tiles.size(); ++x) {
@@ -521,6 +417,8 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   b->off_span = append(&b->plan, spans);
   b->off_node_seq = append(&b->plan, node_seq);
   b->n_row_units = (int32_t)few.size();
+  b->beside = beside;
+  b->most_rows = most_rows;
   b->join = join;
   b->part_rows = part;
   return INFLLM_OK;
@@ -532,54 +430,54 @@ int make_plan(infllm_page_batch* b, int n_heads) {
 
 using namespace infllm;
 
-extern "C" int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* plan_bytes, int64_t* scratch_bytes, int* fresh) {
+static int64_t plan_room(const infllm_page_batch* b) { return ((int64_t)b->plan.size() * 4 + 255) / 256 * 256; }
+
+extern "C" int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* work_bytes) {
   return guarded("page_batch_plan", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_plan"));
     const infllm_pages* p = b->cache;
-    if (!plan_bytes || !scratch_bytes || !fresh) return fail(INFLLM_E_BADARG, "page_batch_plan: null pointer");
+    if (!work_bytes) return fail(INFLLM_E_BADARG, "page_batch_plan: null pointer");
     if (n_heads < 1 || n_heads % p->cfg.n_kv_heads) return fail(INFLLM_E_BADARG, "page_batch_plan: %d query heads over %d KV heads", n_heads, p->cfg.n_kv_heads);
     if ((int64_t)b->most * n_heads * (int64_t)b->seqs.size() > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_plan: more than 2^31 query rows");
-    *fresh = b->plan_of != p->change || b->plan_heads != n_heads;
-    if (*fresh) {
-      for (size_t i = 0; i < b->seqs.size(); ++i)
-        if (b->count[i] > p->seqs[b->seqs[i]].length)
-          return fail(INFLLM_E_BADARG, "page_batch_plan: the newest %d tokens of sequence %d, which has %lld", b->count[i], b->seqs[i],
-                      (long long)p->seqs[b->seqs[i]].length);
-      b->plan_of = ~0ull;
-      INFLLM_TRY(make_plan(b, n_heads));
-      b->plan_of = p->change;
-      b->plan_heads = n_heads;
-    }
-    *plan_bytes = (int64_t)b->plan.size() * 4;
-    *scratch_bytes = b->part_rows * (p->cfg.head_dim + 4) * 4;
+    for (size_t i = 0; i < b->seqs.size(); ++i)
+      if (b->count[i] > p->seqs[b->seqs[i]].length)
+        return fail(INFLLM_E_BADARG, "page_batch_plan: the newest %d tokens of sequence %d, which has %lld", b->count[i], b->seqs[i],
+                    (long long)p->seqs[b->seqs[i]].length);
+    b->plan_of = ~0ull;
+    INFLLM_TRY(make_plan(b, n_heads));
+    b->plan_of = p->change;
+    b->plan_heads = n_heads;
+    b->upload = true;
+    *work_bytes = plan_room(b) + b->part_rows * (p->cfg.head_dim + 4) * 4;
     return INFLLM_OK;
   });
 }
 
-extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const infllm_page_rows* q, void* d_out, float* d_lse, int n_heads,
-                                        float scale, void* d_plan, int upload, void* d_scratch, void* stream) {
+extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const void* d_q, int64_t q_bs, int64_t q_hs, int64_t q_ts, void* d_out,
+                                        float* d_lse, int n_heads, float scale, void* d_work, void* stream) {
   return guarded("page_batch_attend", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_attend"));
     const infllm_pages* p = b->cache;
     const infllm_pages_config& c = p->cfg;
     if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_attend: a cache without a device");
     if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_attend: layer %d of %d", layer, c.n_layers);
+    if (b->plan_of != p->change || b->plan_heads != n_heads) return INFLLM_PAGES_NO_PLAN;
     if (b->most == 0) return INFLLM_OK;
-    if (b->plan_of != p->change || b->plan_heads != n_heads) return fail(INFLLM_E_BADARG, "page_batch_attend: the plan is of another state of the cache");
-    if (!q || !q->d || !d_out || !d_plan || (b->part_rows > 0 && !d_scratch)) return fail(INFLLM_E_BADARG, "page_batch_attend: null pointer");
-    if (((uintptr_t)q->d | (uintptr_t)d_out | (uintptr_t)d_plan | (uintptr_t)d_scratch) % 16 || (q->bs | q->hs | q->ts) % 8)
+    if (!d_q || !d_out || !d_work) return fail(INFLLM_E_BADARG, "page_batch_attend: null pointer");
+    if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_work) % 16 || (q_bs | q_hs | q_ts) % 8)
       return fail(INFLLM_E_BADARG, "page_batch_attend: rows must be 16-byte aligned");
     DeviceScope scope(c.device);
     cudaStream_t s = (cudaStream_t)stream;
-    if (upload) INFLLM_CUDA_OK(cudaMemcpyAsync(d_plan, b->plan.data(), b->plan.size() * 4, cudaMemcpyHostToDevice, s));
+    if (b->upload) INFLLM_CUDA_OK(cudaMemcpyAsync(d_work, b->plan.data(), b->plan.size() * 4, cudaMemcpyHostToDevice, s));
+    b->upload = false;
     PagedParams P;
     P.plane = (int64_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim * 2;
     P.pages = (const char*)c.d_pages + 2 * layer * P.plane;
     P.table = c.d_table;
-    P.q = (const char*)q->d, P.q_bs = q->bs * 2, P.q_hs = q->hs * 2, P.q_ts = q->ts * 2;
+    P.q = (const char*)d_q, P.q_bs = q_bs * 2, P.q_hs = q_hs * 2, P.q_ts = q_ts * 2;
     P.out = (char*)d_out, P.lse = d_lse;
-    P.part_o = (float*)d_scratch, P.part_lse = P.part_o + b->part_rows * c.head_dim;
-    const int32_t* plan = (const int32_t*)d_plan;
+    P.part_o = (float*)((char*)d_work + plan_room(b)), P.part_lse = P.part_o + b->part_rows * c.head_dim;
+    const int32_t* plan = (const int32_t*)d_work;
     P.unit = (const AttnUnit*)(plan + b->off_unit), P.seq = (const AttnSeq*)(plan + b->off_seq);
     P.path = (const AttnPath*)(plan + b->off_path), P.span = (const AttnSpan*)(plan + b->off_span), P.node_seq = plan + b->off_node_seq;
     P.map = p->map;
@@ -588,11 +486,13 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const i
     INFLLM_TRY(tc_get_error_ptr(&P.err));
     P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.group = n_heads / c.n_kv_heads, P.most = b->most;
     P.batch = (int)b->seqs.size();
+    P.n_beside = b->beside ? b->n_row_units * c.n_kv_heads : 0;
     P.scale_log2 = scale * kLog2e;
     if (b->n_ctas > 0) INFLLM_TRY(paged_tc_launch(P, c.dtype, c.head_dim, b->n_ctas, s));
     INFLLM_DISPATCH_DTYPE(c.dtype, T, {
-      if (b->n_row_units > 0) {
-        auto kern = c.head_dim == 128 ? paged_rows_kernel<T, 128, 2> : paged_rows_kernel<T, 64, 2>;
+      if (b->n_row_units > 0 && !b->beside) {
+        auto kern = c.head_dim == 128 ? (b->most_rows <= 8 ? paged_rows_kernel<T, 128, 1> : paged_rows_kernel<T, 128, 2>)
+                                      : (b->most_rows <= 8 ? paged_rows_kernel<T, 64, 1> : paged_rows_kernel<T, 64, 2>);
         launch_chained(kern, dim3(b->n_row_units, c.n_kv_heads), dim3(kRowWarps * 32), 0, s, P);
         INFLLM_LAUNCH_OK("paged_rows_kernel");
       }

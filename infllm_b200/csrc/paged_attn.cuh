@@ -52,6 +52,7 @@ struct PagedParams {
   const AttnSpan* span;
   const int32_t* node_seq;
   int32_t max_pages, page, n_kv, group, most, batch;
+  int32_t n_beside;  // units of few rows, by KV heads, for the blocks of many rows
   float scale_log2;
 };
 

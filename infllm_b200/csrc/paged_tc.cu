@@ -7,10 +7,12 @@
 // two buffers in turn, so that the next product runs while it works; such units are bound by the bytes of the keys.
 // A warp asks for pages, one box of a page and operand (boxes of 16 to 64 tokens: one per lane), through a ring of tiles in
 // the order K0 K1 V0 K2 V1 ..; another warp issues the products.  Blocks work through a list of units of about equal work.
+// Two more warps take units of few rows (paged_rows.cuh), whose loads fit in beside the products.
 // The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
+#include <atomic>
 #include <type_traits>
 
-#include "paged_attn.cuh"
+#include "paged_rows.cuh"
 #include "attn_tc.cuh"
 #include "ring.cuh"
 #include "tc_softmax.cuh"
@@ -19,8 +21,8 @@ namespace infllm {
 
 namespace ptc {
 constexpr int kStages = 5;
-constexpr int kThreads = 10 * 32;
-constexpr int kWarpTma = 8, kWarpMma = 9;
+constexpr int kThreads = 12 * 32;
+constexpr int kWarpTma = 8, kWarpMma = 9, kWarpRows = 10;  // the last two: units of few rows
 enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, Q_FULL0 = EMPTY0 + kStages, S_FULL0 = Q_FULL0 + 2, P_FULL0 = S_FULL0 + 3, PV_DONE0 = P_FULL0 + 3, N_BARS = PV_DONE0 + 3 };
 // Scores and what follows from them go by channels: 0 and 1 are the teams' with the buffer of the same number, 2 is the first
 // team's with the second buffer.  (The second team may be a unit ahead, one that it has no part in: on a barrier that both
@@ -64,14 +66,15 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  chain_enter();
   const uint32_t tmem = *tmem_slot;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   constexpr uint32_t idesc_qk = make_idesc(kBf16, 128, 128, false), idesc_pv = make_idesc(kBf16, 128, kDim, true);
   const int u0 = P.cta_unit[blockIdx.x], u1 = P.cta_unit[blockIdx.x + 1];
 
+  // (the plan is there: the roles wait for the kernels before on the stream where they first need what those have written)
   if (warp == kWarpTma) {
     // ======================================================================================================== pages
+    chain_enter();
     const bool lead = elect_one();
     const int per = 128 / P.page;  // pages of a tile
     int slot = 0;
@@ -223,9 +226,23 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
       base += 2 * n;
     }
     __syncwarp();
+  } else if (warp >= kWarpRows) {
+    // ===================================================================================================== few rows
+    chain_wait();
+    for (int j = blockIdx.x * 2 + warp - kWarpRows; j < P.n_beside; j += gridDim.x * 2) {
+      const AttnUnit U = P.unit[j / P.n_kv];
+      if (U.rows <= 8) {
+        RowsWarp<T, kDim, 1> W;
+        W.alone(P, U, j % P.n_kv);
+      } else {
+        RowsWarp<T, kDim, 2> W;
+        W.alone(P, U, j % P.n_kv);
+      }
+    }
+    __syncwarp();
   } else {
     // ====================================================================================================== softmax
-    const int quad = warp & 3, team = warp >> 2, row = quad * 32 + lane, tid = threadIdx.x & 127;
+    const int quad = warp & 3, team = warp >> 2, row = quad * 32 + lane;
     const uint32_t lane_base = ((uint32_t)(quad * 32)) << 16;
     const uint32_t tO = tmem + 256 + team * 128 + lane_base;
     int ns[3] = {0, 0, 0};  // tiles so far of each channel
@@ -235,46 +252,43 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
       const int n = (U.keys + 127) / 128;
       const bool two = U.rows > 128, works = two || team == 0;
       const int rows = works ? min(128, U.rows - team * 128) : 0, step = two ? 1 : 2;
-      // ---- queries: 16-byte pieces of rows, swizzled as TMA would have
-      if (works && n > 0) {
-        constexpr int kPer = kDim / 8, kStep = 128 / kPer;
-        const int c = tid % kPer, r0 = tid / kPer;
-        unsigned char* to = smem + L::kQ + team * L::kTileBytes + (c >> 3) * kSubTileBytes;
-        // (all rows' places, then all rows, in two rounds of eight: loads one behind the other are what a unit's begin waits for)
-#pragma unroll
-        for (int g = 0; g < kPer; g += 8) {
-          const char* from[8];
-          uint4 v[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = r0 + (g + k) * kStep;
-            from[k] = nullptr;
-            if (r < rows) {
-              const RowAt a = row_at(P, U.node_seq, U.row0 + team * 128 + r);
-              from[k] = P.q + a.b * P.q_bs + (int64_t)(U.hkv * P.group + a.h) * P.q_hs + a.i * P.q_ts + c * 16;
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = from[k] ? __ldg(reinterpret_cast<const uint4*>(from[k])) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = r0 + (g + k) * kStep;
-            *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
-      }
       if (works) {
         const int end = U.key0 + U.keys;
         int lim = end;  // rows that are none are not masked, so that whole tiles stay whole: nothing of them is written
         RowAt at = {0, 0, 0};
+        const char* from = nullptr;
         if (row < rows) {
           at = row_at(P, U.node_seq, U.row0 + team * 128 + row);
           lim = at.i < P.most - __ldg(&P.seq[at.b].count) ? 0 : min(end, U.lim0 + at.i);
+          from = P.q + at.b * P.q_bs + (int64_t)(U.hkv * P.group + at.h) * P.q_hs + at.i * P.q_ts;
         }
         const int all = __reduce_min_sync(0xffffffffu, lim);
+        unsigned char* const mine = smem + L::kQ + team * L::kTileBytes + quad * 32 * 128;  // this warp's rows of the queries' tiles
+        chain_wait();
+        if (n > 0) {
+          // ---- the warp's 32 rows of queries, swizzled as TMA would have them: some rows at once, 16 bytes a lane.  (Rolled: code
+          // that runs once waits for its instructions; unrolled it took 13 us instead of 3.)
+          constexpr int kPer = kDim / 8, kAt = 32 / kPer, kRound = kPer / 2;
+          const int c = lane % kPer, r0 = lane / kPer;
+          unsigned char* to = mine + (c >> 3) * kSubTileBytes;
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            uint4 v[kRound];
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) {
+              const char* p = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), (g * kRound + k) * kAt + r0));
+              v[k] = p ? __ldg(reinterpret_cast<const uint4*>(p + c * 16)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) {
+              const int r = (g * kRound + k) * kAt + r0;
+              *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
+        }
         float m = -INFINITY, l = 0.f;
         for (int i = 0; i < n && ok; ++i) {
           const int ch = channel(two, team, i);
@@ -282,24 +296,39 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
           ok = warp_wait(bar(S_FULL0 + ch), (ns[ch] + i / step) & 1, abort_flag, P.err, 720);
           if (!ok) break;
           tc_fence_after();
-          uint32_t us[128];
-          float* s = reinterpret_cast<float*>(us);
-#pragma unroll
-          for (int c = 0; c < 128; c += 32) tmem_ld32(tS + c, us + c);
-#pragma unroll
-          for (int c = 0; c < 128; c += 32) tmem_wait_ld32(us + c);
           const int j0 = U.key0 + i * 128;
           if (all < j0 + 128) {
+            // what a row does not see is taken out of the scores where they are
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              const int hi = lim - j0 - c;
+              if (__all_sync(0xffffffffu, hi >= 32)) continue;
+              uint32_t w[32];
+              tmem_ld32(tS + c, w);
+              tmem_wait_ld32(w);
 #pragma unroll
-            for (int k = 0; k < 128; ++k) s[k] = j0 + k < lim ? s[k] : -INFINITY;
+              for (int k = 0; k < 32; ++k) w[k] = k < hi ? w[k] : 0xff800000u;
+              tmem_st32(tS + c, w);
+            }
+            tmem_wait_st();
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int k = 0; k < 128; k += 8) {
-            mx[0] = fmax3(mx[0], s[k], s[k + 1]);
-            mx[1] = fmax3(mx[1], s[k + 2], s[k + 3]);
-            mx[2] = fmax3(mx[2], s[k + 4], s[k + 5]);
-            mx[3] = fmax3(mx[3], s[k + 6], s[k + 7]);
+          float s[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint32_t* us = reinterpret_cast<uint32_t*>(s);
+          {
+            float b[32];
+            uint32_t* ub = reinterpret_cast<uint32_t*>(b);
+            tmem_ld32(tS + 32, ub);
+            tmem_ld32(tS + 64, us);
+            tmem_wait_ld32(ub);
+            tmem_wait_ld32(us);
+            max_chunk(b, mx);
+            tmem_ld32(tS + 96, ub);
+            max_chunk(s, mx);
+            tmem_ld32(tS, us);
+            tmem_wait_ld32(ub);
+            tmem_wait_ld32(us);
+            max_chunk(b, mx);
+            max_chunk(s, mx);
           }
           const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.scale_log2;
           const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
@@ -308,23 +337,21 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
           l *= alpha;
           m = mn;
           const float nm = m == -INFINITY ? 0.f : -m;
-          const float2 sc2 = make_float2(P.scale_log2, P.scale_log2), nm2 = make_float2(nm, nm);
           float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
+          // P, packed, takes the place of scores that have been read: 16 columns for 32
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
+            float2 e[16];
             uint32_t pk[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float2 a = ffma2(s[c * 32 + 2 * k], s[c * 32 + 2 * k + 1], sc2, nm2);
-              const float2 p = make_float2(ex2_approx(a.x), ex2_approx(a.y));
-              rs[k & 3] = fadd2(rs[k & 3], p);
-              typename Act<T>::T2 v = Act<T>::from_f2(p.x, p.y);
-              pk[k] = *reinterpret_cast<uint32_t*>(&v);
-            }
+            arg_chunk(s, P.scale_log2, nm, e);
+            tmem_ld32_if(c < 3, tS + 32 * c + 32, us);
+            exp_chunk<T, 5>(e, rs, pk);
             tmem_st16(tS + 16 * c, pk);
+            tmem_wait_ld32(us);
           }
           const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
-          l += r.x + r.y;
+          const float sum = r.x + r.y;
+          l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
           if (scale_o) {
             // O has the products up to the tile before: wait for the last of them
             const int pb = channel(two, team, i - 1);
@@ -361,9 +388,14 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
           const bool whole = U.part < 0;
           const int64_t prow = (int64_t)U.part + team * 128 + row;
           const int64_t orow = ((int64_t)at.b * P.most + at.i) * (P.n_kv * P.group) + U.hkv * P.group + at.h;
+          // 32 columns of the warp's rows at a time through its part of the queries' tile, which no product reads any more, so that
+          // rows are written 128 or 64 bytes at once
+          const char* to = whole ? P.out + orow * (kDim * 2) : reinterpret_cast<const char*>(P.part_o + prow * kDim);
+          const int n_rows = min(32, rows - quad * 32);
 #pragma unroll 1
           for (int c = 0; c < kDim; c += 32) {
             uint32_t o[32];
+            float* f = reinterpret_cast<float*>(o);
             if (n > 0) {
               tmem_ld32(tO + c, o);
               tmem_wait_ld32(o);
@@ -371,28 +403,24 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] = 0;
             }
-            if (row < rows) {
-              float* f = reinterpret_cast<float*>(o);
+            uint4* stage = reinterpret_cast<uint4*>(mine);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) f[k] *= inv;
+            for (int k = 0; k < 8; ++k) reinterpret_cast<float4*>(stage)[lane * 8 + (k ^ (lane & 7))] = make_float4(f[4 * k] * inv, f[4 * k + 1] * inv, f[4 * k + 2] * inv, f[4 * k + 3] * inv);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int r = k * 4 + (lane >> 3), p = lane & 7;
+              const float4 v = reinterpret_cast<float4*>(stage)[r * 8 + (p ^ (r & 7))];
+              char* dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r));
+              if (r >= n_rows) continue;
               if (!whole) {
-                float4* to = reinterpret_cast<float4*>(P.part_o + prow * kDim + c);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) to[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+                *reinterpret_cast<float4*>(dst + (c + p * 4) * 4) = v;
               } else {
-                uint4* to = reinterpret_cast<uint4*>(P.out + (orow * kDim + c) * 2);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    typename Act<T>::T2 v = Act<T>::from_f2(f[8 * k + 2 * e], f[8 * k + 2 * e + 1]);
-                    w[e] = *reinterpret_cast<uint32_t*>(&v);
-                  }
-                  to[k] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+                typename Act<T>::T2 v01 = Act<T>::from_f2(v.x, v.y), v23 = Act<T>::from_f2(v.z, v.w);
+                *reinterpret_cast<uint2*>(dst + (c + p * 4) * 2) = make_uint2(*reinterpret_cast<uint32_t*>(&v01), *reinterpret_cast<uint32_t*>(&v23));
               }
             }
+            __syncwarp();
           }
           if (row < rows) {
             const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
@@ -416,8 +444,14 @@ int paged_tc_launch(const PagedParams& P, int dtype, int head_dim, int n_ctas, c
   INFLLM_DISPATCH_DTYPE(dtype, T, {
     auto kern = head_dim == 128 ? paged_tc_kernel<T, 128> : paged_tc_kernel<T, 64>;
     const int smem = (head_dim == 128 ? ptc::Smem<128>::kTotal : ptc::Smem<64>::kTotal) + 1024;
-    // (set for every launch: it is per device, costs 0.1 us, and remembers nothing)
-    INFLLM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> set[2];  // devices that know it, per head_dim (and, by the dispatch, type)
+    int dev = 0;
+    INFLLM_CUDA_OK(cudaGetDevice(&dev));
+    std::atomic<uint64_t>& there = set[head_dim == 128];
+    if (dev >= 64 || !(there.load(std::memory_order_relaxed) >> dev & 1)) {
+      INFLLM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (dev < 64) there.fetch_or(1ull << dev);
+    }
     launch_chained(kern, dim3(n_ctas), dim3(ptc::kThreads), smem, s, P);
   });
   INFLLM_LAUNCH_OK("paged_tc_kernel");

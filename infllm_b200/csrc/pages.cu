@@ -197,26 +197,28 @@ static void cut(infllm_pages* p, int32_t seq, int64_t length) {
   }
 }
 
-// room for count[i] more tokens of each sequence
-static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* count, int n, const char* what) {
+// room for counts[i] more tokens of each sequence, or for `same`
+static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* counts, int32_t same, int n, const char* what) {
   const int page = p->cfg.page_size;
   int64_t need = 0;
   for (int i = 0; i < n; ++i) {
     const PageSeq& s = p->seqs[seqs[i]];
-    if (count[i] < 0) return fail(INFLLM_E_BADARG, "%s: %d tokens", what, count[i]);
-    if (s.length + count[i] > (int64_t)p->cfg.max_pages * page)
+    const int32_t more = counts ? counts[i] : same;
+    if (more < 0) return fail(INFLLM_E_BADARG, "%s: %d tokens", what, more);
+    if (s.length + more > (int64_t)p->cfg.max_pages * page)
       return fail(INFLLM_E_CAPACITY, "%s: sequence %d would have %lld tokens, and rows of the page table are for %lld", what, seqs[i],
-                  (long long)(s.length + count[i]), (long long)p->cfg.max_pages * page);
-    if (s.position + count[i] > INT32_MAX) return fail(INFLLM_E_CAPACITY, "%s: positions beyond 31 bits", what);
-    need += p->pages_of(s.length + count[i]) - (int64_t)s.pages.size();
+                  (long long)(s.length + more), (long long)p->cfg.max_pages * page);
+    if (s.position + more > INT32_MAX) return fail(INFLLM_E_CAPACITY, "%s: positions beyond 31 bits", what);
+    need += p->pages_of(s.length + more) - (int64_t)s.pages.size();
     // (as many as would be copied if each of several that share their last page had to: the last one may keep it)
-    if (count[i] > 0 && s.length % page && p->uses[s.pages.back()] > 1) ++need;
+    if (more > 0 && s.length % page && p->uses[s.pages.back()] > 1) ++need;
   }
   INFLLM_TRY(need_pages(p, need, what));
   ++p->change;
   for (int i = 0; i < n; ++i) {
     PageSeq& s = p->seqs[seqs[i]];
-    if (count[i] > 0 && s.length % page && p->uses[s.pages.back()] > 1) {
+    const int32_t more = counts ? counts[i] : same;
+    if (more > 0 && s.length % page && p->uses[s.pages.back()] > 1) {
       const int32_t old = s.pages.back();
       s.pages.back() = take_page(p);
       set_entry(p, seqs[i], s.pages.size() - 1, s.pages.back());
@@ -224,8 +226,8 @@ static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* count, in
       drop_page(p, old);  // (another one has it still)
       ++p->reshape;
     }
-    s.length += count[i];
-    s.position += count[i];
+    s.length += more;
+    s.position += more;
     const size_t want = (size_t)p->pages_of(s.length);
     while (s.pages.size() < want) {
       s.pages.push_back(take_page(p));
@@ -576,89 +578,90 @@ extern "C" int infllm_page_batch_destroy(infllm_page_batch* b) {
   return INFLLM_OK;
 }
 
-static void set_counts(infllm_page_batch* b, const int32_t* counts) {
+static void set_counts(infllm_page_batch* b, const int32_t* counts, int32_t same) {
   b->most = 0;
   for (size_t i = 0; i < b->seqs.size(); ++i) {
-    b->count[i] = counts[i];
-    b->most = std::max(b->most, counts[i]);
+    b->count[i] = counts ? counts[i] : same;
+    b->most = std::max(b->most, b->count[i]);
   }
   b->plan_of = ~0ull;
 }
 
-extern "C" int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* counts, void* stream) {
+static void set_reach(const infllm_page_batch* b, int64_t* reach) {
+  if (!reach) return;
+  *reach = 0;
+  for (int32_t s : b->seqs) *reach = std::max(*reach, b->cache->seqs[s].position);
+}
+
+extern "C" int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* counts, int32_t same, int64_t* reach, void* stream) {
   return guarded("page_batch_extend", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_extend"));
-    if (!counts) return fail(INFLLM_E_BADARG, "page_batch_extend: null pointer");
     DeviceScope scope(b->cache->cfg.device);
-    INFLLM_TRY(extend(b->cache, b->seqs.data(), counts, (int)b->seqs.size(), "page_batch_extend"));
-    set_counts(b, counts);
+    INFLLM_TRY(extend(b->cache, b->seqs.data(), counts, same, (int)b->seqs.size(), "page_batch_extend"));
+    set_counts(b, counts, same);
+    set_reach(b, reach);
     return flush(b->cache, b->cache, (cudaStream_t)stream);
   });
 }
 
-extern "C" int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* counts) {
+// whether every sequence has as many tokens
+static int check_counts(const infllm_page_batch* b, const int32_t* counts, int32_t same, const char* what) {
+  for (size_t i = 0; i < b->seqs.size(); ++i) {
+    const int32_t n = counts ? counts[i] : same;
+    const int64_t length = b->cache->seqs[b->seqs[i]].length;
+    if (n < 0 || n > length) return fail(INFLLM_E_BADARG, "%s: the newest %d of the %lld tokens of sequence %d", what, n, (long long)length, b->seqs[i]);
+  }
+  return INFLLM_OK;
+}
+
+extern "C" int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* counts, int32_t same) {
   return guarded("page_batch_retract", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_retract"));
-    if (!counts) return fail(INFLLM_E_BADARG, "page_batch_retract: null pointer");
+    INFLLM_TRY(check_counts(b, counts, same, "page_batch_retract"));
     infllm_pages* p = b->cache;
-    for (size_t i = 0; i < b->seqs.size(); ++i)
-      if (counts[i] < 0 || counts[i] > p->seqs[b->seqs[i]].length)
-        return fail(INFLLM_E_BADARG, "page_batch_retract: %d of the %lld tokens of sequence %d", counts[i],
-                    (long long)p->seqs[b->seqs[i]].length, b->seqs[i]);
     ++p->change, ++p->reshape;
-    for (size_t i = 0; i < b->seqs.size(); ++i) cut(p, b->seqs[i], p->seqs[b->seqs[i]].length - counts[i]);
-    set_counts(b, std::vector<int32_t>(b->seqs.size(), 0).data());
+    for (size_t i = 0; i < b->seqs.size(); ++i) cut(p, b->seqs[i], p->seqs[b->seqs[i]].length - (counts ? counts[i] : same));
+    set_counts(b, nullptr, 0);
     return INFLLM_OK;
   });
 }
 
-extern "C" int infllm_page_batch_select(infllm_page_batch* b, const int32_t* counts) {
+extern "C" int infllm_page_batch_select(infllm_page_batch* b, const int32_t* counts, int32_t same, int64_t* reach) {
   return guarded("page_batch_select", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_select"));
-    if (!counts) return fail(INFLLM_E_BADARG, "page_batch_select: null pointer");
-    for (size_t i = 0; i < b->seqs.size(); ++i)
-      if (counts[i] < 0 || counts[i] > b->cache->seqs[b->seqs[i]].length)
-        return fail(INFLLM_E_BADARG, "page_batch_select: the newest %d of the %lld tokens of sequence %d", counts[i],
-                    (long long)b->cache->seqs[b->seqs[i]].length, b->seqs[i]);
-    set_counts(b, counts);
+    INFLLM_TRY(check_counts(b, counts, same, "page_batch_select"));
+    set_counts(b, counts, same);
+    set_reach(b, reach);
     return INFLLM_OK;
   });
 }
 
-extern "C" int64_t infllm_page_batch_reach(const infllm_page_batch* b) {
-  INFLLM_TRY(batch_alive(b, "page_batch_reach"));
-  int64_t most = 0;
-  for (int32_t s : b->seqs) most = std::max(most, b->cache->seqs[s].position);
-  return most;
-}
-
-extern "C" int infllm_page_batch_write(infllm_page_batch* b, int layer, const infllm_page_rows* k, const infllm_page_rows* v,
-                                       const infllm_page_rows* q, void* d_q_out, int n_heads, const float* d_cos, const float* d_sin,
+extern "C" int infllm_page_batch_write(infllm_page_batch* b, int layer, const void* d_k, int64_t k_bs, int64_t k_hs, int64_t k_ts,
+                                       const void* d_v, int64_t v_bs, int64_t v_hs, int64_t v_ts, const void* d_q, int64_t q_bs,
+                                       int64_t q_hs, int64_t q_ts, void* d_q_out, int n_heads, const float* d_cos, const float* d_sin,
                                        int64_t table_len, void* stream) {
   return guarded("page_batch_write", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_write"));
     const infllm_pages_config& c = b->cache->cfg;
     if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_write: a cache without a device");
     if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_write: layer %d of %d", layer, c.n_layers);
-    if (!k || !v || !k->d || !v->d || (q && (!q->d || !d_q_out || n_heads < 1)) || (!d_cos) != (!d_sin))
-      return fail(INFLLM_E_BADARG, "page_batch_write: null pointer");
-    const infllm_page_rows* all[3] = {k, v, q};
-    for (const infllm_page_rows* r : all)
-      if (r && ((uintptr_t)r->d % 16 || (r->bs | r->hs | r->ts) % 8)) return fail(INFLLM_E_BADARG, "page_batch_write: rows must be 16-byte aligned");
-    if (q && (uintptr_t)d_q_out % 16) return fail(INFLLM_E_BADARG, "page_batch_write: rows must be 16-byte aligned");
+    if (b->most > 0 && (!d_k || !d_v || (d_q && (!d_q_out || n_heads < 1)) || (!d_cos) != (!d_sin))) return fail(INFLLM_E_BADARG, "page_batch_write: null pointer");
+    if (((uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q | (uintptr_t)d_q_out | (uintptr_t)d_cos | (uintptr_t)d_sin) % 16 ||
+        (k_bs | k_hs | k_ts | v_bs | v_hs | v_ts | q_bs | q_hs | q_ts) % 8)
+      return fail(INFLLM_E_BADARG, "page_batch_write: rows must be 16-byte aligned");
     if (b->most == 0) return INFLLM_OK;
     DeviceScope scope(c.device);
     WriteParams P;
-    P.k = (const char*)k->d, P.v = (const char*)v->d, P.q = q ? (const char*)q->d : nullptr;
+    P.k = (const char*)d_k, P.v = (const char*)d_v, P.q = (const char*)d_q;
     P.q_out = (char*)d_q_out;
-    P.k_bs = k->bs * 2, P.k_hs = k->hs * 2, P.k_ts = k->ts * 2;
-    P.v_bs = v->bs * 2, P.v_hs = v->hs * 2, P.v_ts = v->ts * 2;
-    P.q_bs = q ? q->bs * 2 : 0, P.q_hs = q ? q->hs * 2 : 0, P.q_ts = q ? q->ts * 2 : 0;
+    P.k_bs = k_bs * 2, P.k_hs = k_hs * 2, P.k_ts = k_ts * 2;
+    P.v_bs = v_bs * 2, P.v_hs = v_hs * 2, P.v_ts = v_ts * 2;
+    P.q_bs = q_bs * 2, P.q_hs = q_hs * 2, P.q_ts = q_ts * 2;
     P.plane = (int64_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim * 2;
     P.pages = (char*)c.d_pages + 2 * layer * P.plane;
     P.table = c.d_table;
     P.cos_t = d_cos, P.sin_t = d_sin;
-    P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.n_heads = q ? n_heads : 0, P.most = b->most;
+    P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.n_heads = d_q ? n_heads : 0, P.most = b->most;
     const int n = (int)b->seqs.size();
     for (int i = 0; i < n; ++i) {
       const PageSeq& s = b->cache->seqs[b->seqs[i]];

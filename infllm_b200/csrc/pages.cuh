@@ -87,8 +87,11 @@ struct infllm_page_batch {
   // the plan of the attention (paged_attn.cu), as of `change` and for n_heads
   uint64_t plan_of = ~0ull;
   int32_t plan_heads = 0;
+  bool upload = false;  // it is not on the device yet
   std::vector<int32_t> plan;
   int32_t n_row_units = 0, n_ctas = 0;
+  int32_t most_rows = 0;  // of a unit of few rows
+  bool beside = false;    // units of few rows go to the blocks of many
   bool join = false;
   int64_t part_rows = 0;
   int64_t off_unit = 0, off_tile_unit = 0, off_cta = 0, off_seq = 0, off_path = 0, off_span = 0, off_node_seq = 0;  // sections of the plan

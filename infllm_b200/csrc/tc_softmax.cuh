@@ -112,4 +112,40 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
                               __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 
+constexpr int kPolyEvery = 8;
+// exponentials of 32 columns of a row, packed; sums into rs
+template <typename T, int kDegree>
+__device__ __forceinline__ void exp_chunk(const float2* a, float2* rs, uint32_t* pk) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    float2 p;
+    if (k % kPolyEvery == kPolyEvery - 1) {
+      p = ex2_poly2<kDegree>(a[k]);  // one pair in kPolyEvery off the special-function unit
+    } else {
+      p = make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
+    }
+    rs[k & 3] = fadd2(rs[k & 3], p);
+    typename Act<T>::T2 v = Act<T>::from_f2(p.x, p.y);
+    pk[k] = *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+// 32 columns of scores into exponents; what they were loaded into may be loaded into again behind it
+__device__ __forceinline__ void arg_chunk(const float* s, float sc, float neg_m, float2* a) {
+  const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    a[k] = ffma2(s[2 * k], s[2 * k + 1], sc2, nm2);
+    asm volatile("" : "+f"(a[k].x), "+f"(a[k].y));
+  }
+}
+__device__ __forceinline__ void max_chunk(const float* s, float* mx) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    mx[0] = fmax3(mx[0], s[i], s[i + 1]);
+    mx[1] = fmax3(mx[1], s[i + 2], s[i + 3]);
+    mx[2] = fmax3(mx[2], s[i + 4], s[i + 5]);
+    mx[3] = fmax3(mx[3], s[i + 6], s[i + 7]);
+  }
+}
+
 }  // namespace infllm

@@ -333,3 +333,34 @@ def test_another_stream_than_the_default():
         seqs = x.fork(root, 6)
         b = x.grow(seqs, [1] * 6)
         x.check(b, [1] * 6, 8)
+
+
+@pytest.mark.parametrize("n_seqs,n", [(3, 1), (40, 1), (3, 30)])
+@pytest.mark.parametrize("what", [NAN, math.inf])
+def test_what_is_no_number_stays_in_its_row(n_seqs, n, what):
+    """A query that is no number, and a key of a sequence's own that is none, reach that row and that sequence alone."""
+    c = make(400, 16, 2, 128)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    root = c.open()
+    b = c.batch(root)
+    b.extend(900)
+    b.write(0, rand(g, 1, 2, 900, 128), rand(g, 1, 2, 900, 128))
+    seqs = c.fork(root, n_seqs)
+    b = c.batch(seqs)
+    b.extend(n)
+    k, v, q = (rand(g, n_seqs, h, n, 128) for h in (2, 2, 8))
+    b.write(0, k, v)
+    fine = b.attend(0, q)
+    odd = q.clone()
+    odd[1, 5, 0, 3] = what
+    got = b.attend(0, odd)
+    bad = torch.zeros_like(fine, dtype=torch.bool)
+    bad[1, 5, 0] = True
+    assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], fine[~bad])
+    k[2, 1, 0, 7] = what
+    b.write(0, k, v)
+    got = b.attend(0, q)
+    bad = torch.zeros_like(fine, dtype=torch.bool)
+    bad[2, 4:] = True  # the KV head's query heads
+    assert torch.equal(got[~bad], fine[~bad])
+    assert (torch.isnan(got[bad]).any() if what == math.inf else torch.isnan(got[bad]).all())

@@ -40,7 +40,7 @@ class Cache:
         b = ctypes.c_void_p()
         L.check(L.lib.infllm_page_batch_create(self.h, self.ids(seqs), len(seqs), ctypes.byref(b)))
         try:
-            L.check(L.lib.infllm_page_batch_extend(b, self.ids(counts), None))
+            L.check(L.lib.infllm_page_batch_extend(b, self.ids(counts), 0, None, None))
         finally:
             L.lib.infllm_page_batch_destroy(b)
 
@@ -249,7 +249,7 @@ def test_refusals():
     L.check(L.lib.infllm_page_batch_create(c.h, c.ids([s]), 1, ctypes.byref(b)))
     c.free([s])
     assert c.open() == [s]  # the same number, another sequence
-    assert L.lib.infllm_page_batch_extend(b, c.ids([1]), None) == L.E_BADARG and b"freed" in L.lib.infllm_last_error()
+    assert L.lib.infllm_page_batch_extend(b, None, 1, None, None) == L.E_BADARG and b"freed" in L.lib.infllm_last_error()
     L.lib.infllm_page_batch_destroy(b)
     out = ctypes.c_void_p()
     for change in (dict(head_dim=96), dict(page_size=48), dict(dtype=2), dict(n_pages=0), dict(max_pages=1 << 30)):
