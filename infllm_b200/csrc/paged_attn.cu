@@ -32,7 +32,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid
   const int hkv = blockIdx.y;
   RowsWarp<T, kDim, kNt> W;
   W.find(P, U, hkv);
-  chain_enter();
+  // (the kernel before on the stream, where it is the one of many rows, has waited for what was before it by the time this one
+  // runs, and leaves other rows: it is waited for at the end, for the join's sake)
+  if (P.after_tiles) chain_trigger(); else chain_enter();
   W.begin(P);
   W.template groups<false>(P, U, hkv, warp, kRowWarps);
   W.sums();
@@ -78,6 +80,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid
       if (P.lse && d == 0) P.lse[orow] = lse * (1.f / kLog2e);
     }
   }
+  if (P.after_tiles) chain_wait();
 }
 
 // ----------------------------------------------------------------------------------------------------------- the join
@@ -101,13 +104,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     return P.span[(A.span + tile) * P.n_kv + hkv];
   };
   int at[kNearPath], n[kNearPath], step[kNearPath];
+  bool blocks[kNearPath];
 #pragma unroll
   for (int k = 0; k < kNearPath; ++k) {
-    at[k] = n[k] = step[k] = 0;
+    at[k] = n[k] = step[k] = 0, blocks[k] = false;
     if (is && k < S.n_path) {
       int r;
       const AttnSpan Z = span_of(S.near_path[k], &r);
-      at[k] = Z.part + r, n[k] = Z.n, step[k] = Z.rows;
+      at[k] = Z.part + r, n[k] = Z.n, step[k] = Z.rows, blocks[k] = Z.blocks;
     }
   }
   chain_enter();
@@ -115,7 +119,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  auto fold = [&](int first, int count, int stride) {  // this warp's of `count` parts
+  if (P.n_beside > 0 && blockIdx.x == 0 && threadIdx.x == 0) *P.next = 0;
+  auto fold = [&](int first, int count, int stride, bool in_blocks) {  // this warp's of `count` parts
     for (int c0 = warp % kWarps; c0 < count; c0 += kWarps * kAhead) {
       float lse[kAhead], v[kAhead][kPer];
 #pragma unroll
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         if (c >= count) continue;
         const int64_t row = (int64_t)first + (int64_t)c * stride;
         lse[e] = P.part_lse[row];
-        const float* o = P.part_o + row * kDim + lane * kPer;
+        const float* o = P.part_o + (in_blocks ? (row & ~(int64_t)31) * kDim + (lane * kPer / 4) * 128 + (row & 31) * 4 + lane * kPer % 4 : row * kDim + lane * kPer);
         if (kPer == 4) *reinterpret_cast<float4*>(v[e]) = *reinterpret_cast<const float4*>(o);
         else *reinterpret_cast<float2*>(v[e]) = *reinterpret_cast<const float2*>(o);
       }
@@ -149,11 +154,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     }
   };
 #pragma unroll
-  for (int k = 0; k < kNearPath; ++k) fold(at[k], n[k], step[k]);
+  for (int k = 0; k < kNearPath; ++k) fold(at[k], n[k], step[k], blocks[k]);
   for (int k = kNearPath; is && k < S.n_path; ++k) {
     int r;
     const AttnSpan Z = span_of(P.path[S.path + k - kNearPath], &r);
-    fold(Z.part + r, Z.n, Z.rows);
+    fold(Z.part + r, Z.n, Z.rows, Z.blocks);
   }
   if (kWarps > 1) {
 #pragma unroll
@@ -199,8 +204,10 @@ static int join_launch(const PagedParams& P, cudaStream_t s) {
 // ----------------------------------------------------------------------------------------------------------- the plan
 namespace {
 
-constexpr int kGroupWork = 2;  // what a group of 16 keys of few rows takes a warp beside the products, in tiles of 128 rows
-constexpr int kUnitWork = 6;  // what a unit of many rows takes besides its tiles, in tiles of 128 rows
+// Work, in what a tile of 128 rows by 128 keys takes (0.9 us where the products are the bound)
+constexpr int kUnitWork = 4;   // of a unit of many rows besides its tiles
+constexpr int kBlockWork = 4;  // worth a block
+constexpr int kGroupWork = 3;  // of a group of 16 keys for few rows by a warp beside the products
 
 struct Node {
   int64_t key0, key1;
@@ -321,38 +328,43 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   std::vector<AttnSpan> spans(tiles.size() * n_kv);
   int64_t part = 0;
   bool join = false;
-  // few rows: units of equal work.  Beside a kernel of many rows two warps of each of its blocks take them, one unit each, as
-  // long as that takes no longer than the products (a group of 16 keys about two tiles of 128 rows); otherwise blocks of
-  // four warps, four per SM.
-  const int64_t n_cta = many_units ? std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / 4)) : 0;
-  const bool beside = n_cta > 0 && few_work * kGroupWork <= 2 * (many_work + kUnitWork * (many_units + n_cta));
-  const int64_t warps = beside ? 1 : kRowWarps, units = beside ? 2 * n_cta : p->n_sm * 4;
-  const int64_t chunk = std::max<int64_t>(warps, ceil_div(ceil_div(few_work, units), warps) * warps) * 16;
+  // Few rows.  Two warps of each block of many rows take units of them, whoever is free the next, as much as is done by the time
+  // the products are; the rest goes to blocks of four warps, four per SM, in units of equal work.
+  const int64_t n_cta = many_units ? std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / kBlockWork)) : 0;
+  many_work += kUnitWork * (many_units + n_cta);
+  int64_t beside_left = n_cta ? 2 * many_work / kGroupWork : 0;
+  const int64_t beside_chunk = std::min<int64_t>(16, std::max<int64_t>(2, ceil_div(few_work, 8 * std::max<int64_t>(n_cta, 1)))) * 16;
+  const int64_t rest = std::max<int64_t>(0, few_work - beside_left);
+  const int64_t rest_chunk = std::max<int64_t>(kRowWarps, ceil_div(ceil_div(rest, p->n_sm * 4), kRowWarps) * kRowWarps) * 16;
+  std::vector<AttnUnit> by_four;
   int32_t most_rows = 0;
   for (size_t x = 0; x < tiles.size(); ++x) {
     const Tile& t = tiles[x];
     if (t.many) continue;
-    const int64_t keys = t.unit.keys, cut = ceil_div(keys, chunk), each = cut ? ceil_div(ceil_div(keys, 16), cut) * 16 : 0;
+    const int64_t keys = t.unit.keys, work = ceil_div(keys, 16) * n_kv;
+    const bool beside = work <= beside_left && !(t.alone && keys == 0);
+    const int64_t chunk = beside ? beside_chunk : rest_chunk, cut = ceil_div(keys, chunk), each = cut ? ceil_div(ceil_div(keys, 16), cut) * 16 : 0;
+    std::vector<AttnUnit>& to = beside ? few : by_four;
     AttnUnit u = t.unit;
-    most_rows = std::max(most_rows, u.rows);
-    const bool whole = t.alone && cut <= 1 && !beside;
-    if (whole) {
-      few.push_back(u);
+    if (!beside) most_rows = std::max(most_rows, u.rows);
+    if (!beside && t.alone && cut <= 1) {
+      to.push_back(u);
       for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h].n = -1;
       continue;
     }
+    if (beside) beside_left -= work;
     u.part_kv = (int32_t)(cut * u.rows);
     for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h] = {(int32_t)(part + h * cut * u.rows), (int32_t)cut, u.rows, 0};
     for (int64_t k = 0; k < keys; k += each) {
       u.key0 = t.unit.key0 + (int32_t)k, u.keys = (int32_t)std::min(each, keys - k), u.part = (int32_t)(part + k / each * u.rows);
-      few.push_back(u);
+      to.push_back(u);
     }
     part += cut * u.rows * n_kv;
     join = true;
   }
-  // many rows: one list of all key tiles, cut into as many stretches of equal work as there are SMs, or fewer of four tiles;
-  // a unit's begin and end are as long as some tiles
-  many_work += kUnitWork * (many_units + n_cta);
+  const size_t n_beside = few.size();
+  few.insert(few.end(), by_four.begin(), by_four.end());
+  // many rows: one list of all key tiles, cut into as many stretches of equal work as there are SMs, or fewer
   int64_t done = 0;  // work that has been dealt out
   for (size_t x = 0; x < tiles.size(); ++x) {
     const Tile& t = tiles[x];
@@ -384,8 +396,10 @@ int make_plan(infllm_page_batch* b, int n_heads) {
         z.n = -1;
         continue;
       }
-      z = {(int32_t)part, (int32_t)cut, u.rows, 0};
-      for (size_t k = first; k < large.size(); ++k, part += u.rows) large[k].part = (int32_t)part;
+      const int32_t room = (u.rows + 31) / 32 * 32;
+      part = (part + 31) / 32 * 32;
+      z = {(int32_t)part, (int32_t)cut, room, 1};
+      for (size_t k = first; k < large.size(); ++k, part += room) large[k].part = (int32_t)part;
       join = true;
     }
   }
@@ -408,7 +422,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
     }
     seqs.push_back(q);
   }
-  b->plan.clear();
+  b->plan.assign(4, 0);  // the number of the next unit of few rows, and nothing
   b->off_unit = append(&b->plan, few);
   b->off_tile_unit = append(&b->plan, large);
   b->off_cta = append(&b->plan, cta);
@@ -416,8 +430,8 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   b->off_path = append(&b->plan, paths);
   b->off_span = append(&b->plan, spans);
   b->off_node_seq = append(&b->plan, node_seq);
-  b->n_row_units = (int32_t)few.size();
-  b->beside = beside;
+  b->n_row_units = (int32_t)by_four.size();
+  b->n_beside = (int32_t)n_beside;
   b->most_rows = most_rows;
   b->join = join;
   b->part_rows = part;
@@ -486,11 +500,13 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     INFLLM_TRY(tc_get_error_ptr(&P.err));
     P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.group = n_heads / c.n_kv_heads, P.most = b->most;
     P.batch = (int)b->seqs.size();
-    P.n_beside = b->beside ? b->n_row_units * c.n_kv_heads : 0;
+    P.n_beside = b->n_beside * c.n_kv_heads;
+    P.next = (int32_t*)d_work;
     P.scale_log2 = scale * kLog2e;
     if (b->n_ctas > 0) INFLLM_TRY(paged_tc_launch(P, c.dtype, c.head_dim, b->n_ctas, s));
     INFLLM_DISPATCH_DTYPE(c.dtype, T, {
-      if (b->n_row_units > 0 && !b->beside) {
+      if (b->n_row_units > 0) {
+        P.unit += b->n_beside, P.after_tiles = b->n_ctas > 0;
         auto kern = c.head_dim == 128 ? (b->most_rows <= 8 ? paged_rows_kernel<T, 128, 1> : paged_rows_kernel<T, 128, 2>)
                                       : (b->most_rows <= 8 ? paged_rows_kernel<T, 64, 1> : paged_rows_kernel<T, 64, 2>);
         launch_chained(kern, dim3(b->n_row_units, c.n_kv_heads), dim3(kRowWarps * 32), 0, s, P);

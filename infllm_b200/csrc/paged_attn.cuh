@@ -29,7 +29,8 @@ struct alignas(16) AttnSeq {   // of a sequence of the batch, for the join: its 
 };
 static_assert(sizeof(AttnSeq) == 64, "");
 struct alignas(16) AttnSpan {  // of a row tile of a node and a KV head: n partials of `rows` rows, one behind the other
-  int32_t part, n, rows, pad;
+  int32_t part, n, rows;
+  int32_t blocks;     // the rows lie in blocks of 32, four columns of all of them side by side
 };
 
 struct PagedParams {
@@ -53,6 +54,8 @@ struct PagedParams {
   const int32_t* node_seq;
   int32_t max_pages, page, n_kv, group, most, batch;
   int32_t n_beside;  // units of few rows, by KV heads, for the blocks of many rows
+  int32_t after_tiles;
+  int32_t* next;     // of those, the next that nobody has taken; the join sets it back
   float scale_log2;
 };
 

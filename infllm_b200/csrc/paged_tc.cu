@@ -229,7 +229,12 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
   } else if (warp >= kWarpRows) {
     // ===================================================================================================== few rows
     chain_wait();
-    for (int j = blockIdx.x * 2 + warp - kWarpRows; j < P.n_beside; j += gridDim.x * 2) {
+    // (whoever is free takes the next: the products beside them keep some waiting longer)
+    while (true) {
+      int j = P.n_beside;
+      if (lane == 0 && j > 0) j = atomicAdd(P.next, 1);
+      j = __shfl_sync(0xffffffffu, j, 0);
+      if (j >= P.n_beside) break;
       const AttnUnit U = P.unit[j / P.n_kv];
       if (U.rows <= 8) {
         RowsWarp<T, kDim, 1> W;
@@ -245,194 +250,200 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
     const int quad = warp & 3, team = warp >> 2, row = quad * 32 + lane;
     const uint32_t lane_base = ((uint32_t)(quad * 32)) << 16;
     const uint32_t tO = tmem + 256 + team * 128 + lane_base;
+    struct Turn {  // a unit of this team's, and this thread's row of it
+      int u, n, key0, rows, lim, all;
+      bool two, whole;
+      int64_t out;  // row of the output, or of the partial results
+      const char* q;
+    };
+    auto find = [&](int u) {  // the team's next unit from u on: of the plan alone
+      Turn t{u, 0, 0, 0, 0, 0, false, false, 0, nullptr};
+      for (; t.u < u1; ++t.u)
+        if (team == 0 || __ldg(&P.tile_unit[t.u].rows) > 128) break;
+      if (t.u >= u1) return t;
+      const AttnUnit U = P.tile_unit[t.u];
+      t.n = (U.keys + 127) / 128, t.key0 = U.key0, t.two = U.rows > 128, t.whole = U.part < 0;
+      t.rows = min(128, U.rows - team * 128);
+      t.lim = U.key0 + U.keys;  // rows that are none are not masked, so that whole tiles stay whole: nothing of them is written
+      if (row < t.rows) {
+        const RowAt at = row_at(P, U.node_seq, U.row0 + team * 128 + row);
+        t.lim = at.i < P.most - __ldg(&P.seq[at.b].count) ? 0 : min(t.lim, U.lim0 + at.i);
+        t.q = P.q + at.b * P.q_bs + (int64_t)(U.hkv * P.group + at.h) * P.q_hs + at.i * P.q_ts;
+        t.out = t.whole ? ((int64_t)at.b * P.most + at.i) * (P.n_kv * P.group) + U.hkv * P.group + at.h : (int64_t)U.part + team * 128 + row;
+      }
+      t.all = __reduce_min_sync(0xffffffffu, t.lim);
+      return t;
+    };
+    auto queries = [&](const Turn& t) {
+      // The warp's 32 rows, 16 bytes a lane, swizzled as TMA would have them.  No product reads the last unit's any more: its
+      // scores have been seen.
+      constexpr int kPer = kDim / 8, kAt = 32 / kPer;
+      const int c = lane % kPer, r0 = lane / kPer;
+      unsigned char* to = smem + L::kQ + team * L::kTileBytes + quad * 32 * 128 + (c >> 3) * kSubTileBytes;
+      uint4 v[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const char* p = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(t.q), k * kAt + r0));
+        v[k] = p ? __ldg(reinterpret_cast<const uint4*>(p + c * 16)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int r = k * kAt + r0;
+        *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
+    };
     int ns[3] = {0, 0, 0};  // tiles so far of each channel
     bool ok = true;
-    for (int u = u0; u < u1 && ok; ++u) {
-      const AttnUnit U = P.tile_unit[u];
-      const int n = (U.keys + 127) / 128;
-      const bool two = U.rows > 128, works = two || team == 0;
-      const int rows = works ? min(128, U.rows - team * 128) : 0, step = two ? 1 : 2;
-      if (works) {
-        const int end = U.key0 + U.keys;
-        int lim = end;  // rows that are none are not masked, so that whole tiles stay whole: nothing of them is written
-        RowAt at = {0, 0, 0};
-        const char* from = nullptr;
-        if (row < rows) {
-          at = row_at(P, U.node_seq, U.row0 + team * 128 + row);
-          lim = at.i < P.most - __ldg(&P.seq[at.b].count) ? 0 : min(end, U.lim0 + at.i);
-          from = P.q + at.b * P.q_bs + (int64_t)(U.hkv * P.group + at.h) * P.q_hs + at.i * P.q_ts;
-        }
-        const int all = __reduce_min_sync(0xffffffffu, lim);
-        unsigned char* const mine = smem + L::kQ + team * L::kTileBytes + quad * 32 * 128;  // this warp's rows of the queries' tiles
-        chain_wait();
-        if (n > 0) {
-          // ---- the warp's 32 rows of queries, swizzled as TMA would have them: some rows at once, 16 bytes a lane.  (Rolled: code
-          // that runs once waits for its instructions; unrolled it took 13 us instead of 3.)
-          constexpr int kPer = kDim / 8, kAt = 32 / kPer, kRound = kPer / 2;
-          const int c = lane % kPer, r0 = lane / kPer;
-          unsigned char* to = mine + (c >> 3) * kSubTileBytes;
+    Turn now = find(u0);
+    chain_wait();
+    if (now.n > 0) queries(now);
+    while (now.u < u1 && ok) {
+      const Turn next = find(now.u + 1);
+      const int step = now.two ? 1 : 2;
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < now.n && ok; ++i) {
+        const int ch = channel(now.two, team, i);
+        const uint32_t tS = tmem + buffer(ch) * 128 + lane_base;
+        ok = warp_wait(bar(S_FULL0 + ch), (ns[ch] + i / step) & 1, abort_flag, P.err, 720);
+        if (!ok) break;
+        tc_fence_after();
+        const int j0 = now.key0 + i * 128;
+        if (now.all < j0 + 128) {
+          // what a row does not see is taken out of the scores where they are
 #pragma unroll 1
-          for (int g = 0; g < 2; ++g) {
-            uint4 v[kRound];
+          for (int c = 0; c < 128; c += 32) {
+            const int hi = now.lim - j0 - c;
+            if (__all_sync(0xffffffffu, hi >= 32)) continue;
+            uint32_t w[32];
+            tmem_ld32(tS + c, w);
+            tmem_wait_ld32(w);
 #pragma unroll
-            for (int k = 0; k < kRound; ++k) {
-              const char* p = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), (g * kRound + k) * kAt + r0));
-              v[k] = p ? __ldg(reinterpret_cast<const uint4*>(p + c * 16)) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int k = 0; k < kRound; ++k) {
-              const int r = (g * kRound + k) * kAt + r0;
-              *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
-        }
-        float m = -INFINITY, l = 0.f;
-        for (int i = 0; i < n && ok; ++i) {
-          const int ch = channel(two, team, i);
-          const uint32_t tS = tmem + buffer(ch) * 128 + lane_base;
-          ok = warp_wait(bar(S_FULL0 + ch), (ns[ch] + i / step) & 1, abort_flag, P.err, 720);
-          if (!ok) break;
-          tc_fence_after();
-          const int j0 = U.key0 + i * 128;
-          if (all < j0 + 128) {
-            // what a row does not see is taken out of the scores where they are
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-              const int hi = lim - j0 - c;
-              if (__all_sync(0xffffffffu, hi >= 32)) continue;
-              uint32_t w[32];
-              tmem_ld32(tS + c, w);
-              tmem_wait_ld32(w);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) w[k] = k < hi ? w[k] : 0xff800000u;
-              tmem_st32(tS + c, w);
-            }
-            tmem_wait_st();
-          }
-          float s[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          uint32_t* us = reinterpret_cast<uint32_t*>(s);
-          {
-            float b[32];
-            uint32_t* ub = reinterpret_cast<uint32_t*>(b);
-            tmem_ld32(tS + 32, ub);
-            tmem_ld32(tS + 64, us);
-            tmem_wait_ld32(ub);
-            tmem_wait_ld32(us);
-            max_chunk(b, mx);
-            tmem_ld32(tS + 96, ub);
-            max_chunk(s, mx);
-            tmem_ld32(tS, us);
-            tmem_wait_ld32(ub);
-            tmem_wait_ld32(us);
-            max_chunk(b, mx);
-            max_chunk(s, mx);
-          }
-          const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.scale_log2;
-          const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
-          const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
-          const bool scale_o = __any_sync(0xffffffffu, mn != m && m != -INFINITY) && i > 0;
-          l *= alpha;
-          m = mn;
-          const float nm = m == -INFINITY ? 0.f : -m;
-          float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          // P, packed, takes the place of scores that have been read: 16 columns for 32
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float2 e[16];
-            uint32_t pk[16];
-            arg_chunk(s, P.scale_log2, nm, e);
-            tmem_ld32_if(c < 3, tS + 32 * c + 32, us);
-            exp_chunk<T, 5>(e, rs, pk);
-            tmem_st16(tS + 16 * c, pk);
-            tmem_wait_ld32(us);
-          }
-          const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
-          const float sum = r.x + r.y;
-          l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
-          if (scale_o) {
-            // O has the products up to the tile before: wait for the last of them
-            const int pb = channel(two, team, i - 1);
-            ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (i - 1) / step) & 1, abort_flag, P.err, 721);
-            if (!ok) break;
-            tc_fence_after();
-            const float2 al = make_float2(alpha, alpha);
-#pragma unroll 1
-            for (int c = 0; c < kDim; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(tO + c, o);
-              tmem_wait_ld32(o);
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const float2 x = fmul2(make_float2(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), al);
-                o[k] = __float_as_uint(x.x), o[k + 1] = __float_as_uint(x.y);
-              }
-              tmem_st32(tO + c, o);
-            }
+            for (int k = 0; k < 32; ++k) w[k] = k < hi ? w[k] : 0xff800000u;
+            tmem_st32(tS + c, w);
           }
           tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(P_FULL0 + ch));
         }
-        // ---- out
-        if (ok && n > 0) {
-          const int pb = channel(two, team, n - 1);
-          ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (n - 1) / step) & 1, abort_flag, P.err, 722);
+        float s[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t* us = reinterpret_cast<uint32_t*>(s);
+        {
+          float b[32];
+          uint32_t* ub = reinterpret_cast<uint32_t*>(b);
+          tmem_ld32(tS + 32, ub);
+          tmem_ld32(tS + 64, us);
+          tmem_wait_ld32(ub);
+          tmem_wait_ld32(us);
+          max_chunk(b, mx);
+          tmem_ld32(tS + 96, ub);
+          max_chunk(s, mx);
+          tmem_ld32(tS, us);
+          tmem_wait_ld32(ub);
+          tmem_wait_ld32(us);
+          max_chunk(b, mx);
+          max_chunk(s, mx);
         }
-        if (ok) {
+        const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.scale_log2;
+        const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
+        const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
+        const bool scale_o = __any_sync(0xffffffffu, mn != m && m != -INFINITY) && i > 0;
+        l *= alpha;
+        m = mn;
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // P, packed, takes the place of scores that have been read: 16 columns for 32
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float2 e[16];
+          uint32_t pk[16];
+          arg_chunk(s, P.scale_log2, nm, e);
+          tmem_ld32_if(c < 3, tS + 32 * c + 32, us);
+          exp_chunk<T, 5>(e, rs, pk);
+          tmem_st16(tS + 16 * c, pk);
+          tmem_wait_ld32(us);
+        }
+        const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
+        const float sum = r.x + r.y;
+        l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
+        if (scale_o) {
+          // O has the products up to the tile before: wait for the last of them
+          const int pb = channel(now.two, team, i - 1);
+          ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (i - 1) / step) & 1, abort_flag, P.err, 721);
+          if (!ok) break;
           tc_fence_after();
-          const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
-          const bool whole = U.part < 0;
-          const int64_t prow = (int64_t)U.part + team * 128 + row;
-          const int64_t orow = ((int64_t)at.b * P.most + at.i) * (P.n_kv * P.group) + U.hkv * P.group + at.h;
-          // 32 columns of the warp's rows at a time through its part of the queries' tile, which no product reads any more, so that
-          // rows are written 128 or 64 bytes at once
-          const char* to = whole ? P.out + orow * (kDim * 2) : reinterpret_cast<const char*>(P.part_o + prow * kDim);
-          const int n_rows = min(32, rows - quad * 32);
+          const float2 al = make_float2(alpha, alpha);
 #pragma unroll 1
           for (int c = 0; c < kDim; c += 32) {
             uint32_t o[32];
-            float* f = reinterpret_cast<float*>(o);
-            if (n > 0) {
-              tmem_ld32(tO + c, o);
-              tmem_wait_ld32(o);
-            } else {
+            tmem_ld32(tO + c, o);
+            tmem_wait_ld32(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = 0;
+            for (int k = 0; k < 32; k += 2) {
+              const float2 x = fmul2(make_float2(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), al);
+              o[k] = __float_as_uint(x.x), o[k + 1] = __float_as_uint(x.y);
             }
-            uint4* stage = reinterpret_cast<uint4*>(mine);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) reinterpret_cast<float4*>(stage)[lane * 8 + (k ^ (lane & 7))] = make_float4(f[4 * k] * inv, f[4 * k + 1] * inv, f[4 * k + 2] * inv, f[4 * k + 3] * inv);
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int r = k * 4 + (lane >> 3), p = lane & 7;
-              const float4 v = reinterpret_cast<float4*>(stage)[r * 8 + (p ^ (r & 7))];
-              char* dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r));
-              if (r >= n_rows) continue;
-              if (!whole) {
-                *reinterpret_cast<float4*>(dst + (c + p * 4) * 4) = v;
-              } else {
-                typename Act<T>::T2 v01 = Act<T>::from_f2(v.x, v.y), v23 = Act<T>::from_f2(v.z, v.w);
-                *reinterpret_cast<uint2*>(dst + (c + p * 4) * 2) = make_uint2(*reinterpret_cast<uint32_t*>(&v01), *reinterpret_cast<uint32_t*>(&v23));
-              }
-            }
-            __syncwarp();
+            tmem_st32(tO + c, o);
           }
-          if (row < rows) {
-            const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
-            if (!whole) P.part_lse[prow] = lse;
-            else if (P.lse) P.lse[orow] = lse * (1.f / kLog2e);
-          }
-          tc_fence_before();
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(P_FULL0 + ch));
       }
-      if (two) ns[0] += n, ns[1] += n;
-      else ns[0] += (n + 1) / 2, ns[2] += n / 2;
+      // the next unit's queries first, so that its first scores are formed while this one's rows are written
+      if (ok && next.n > 0) queries(next);
+      if (ok && now.n > 0) {
+        const int pb = channel(now.two, team, now.n - 1);
+        ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (now.n - 1) / step) & 1, abort_flag, P.err, 722);
+      }
+      if (ok) {
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
+#pragma unroll 1
+        for (int c = 0; c < kDim; c += 32) {
+          uint32_t o[32];
+          float* f = reinterpret_cast<float*>(o);
+          if (now.n > 0) {
+            tmem_ld32(tO + c, o);
+            tmem_wait_ld32(o);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0;
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) f[k] *= inv;
+          if (row < now.rows && !now.whole) {
+            // partial rows lie in blocks of 32, four columns of all of them side by side: every store is one stretch
+            float4* to = reinterpret_cast<float4*>(P.part_o + (now.out - lane) * kDim) + (c / 4) * 32 + lane;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to[k * 32] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+          } else if (row < now.rows) {
+            uint4* to = reinterpret_cast<uint4*>(P.out + (now.out * kDim + c) * 2);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                typename Act<T>::T2 v = Act<T>::from_f2(f[8 * k + 2 * e], f[8 * k + 2 * e + 1]);
+                w[e] = *reinterpret_cast<uint32_t*>(&v);
+              }
+              to[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (row < now.rows) {
+          const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
+          if (!now.whole) P.part_lse[now.out] = lse;
+          else if (P.lse) P.lse[now.out] = lse * (1.f / kLog2e);
+        }
+        tc_fence_before();
+      }
+      if (now.two) ns[team] += now.n;
+      else ns[0] += (now.n + 1) / 2, ns[2] += now.n / 2;
       __syncwarp();
+      now = next;
     }
   }
   tc_fence_before();

@@ -90,8 +90,8 @@ struct infllm_page_batch {
   bool upload = false;  // it is not on the device yet
   std::vector<int32_t> plan;
   int32_t n_row_units = 0, n_ctas = 0;
-  int32_t most_rows = 0;  // of a unit of few rows
-  bool beside = false;    // units of few rows go to the blocks of many
+  int32_t n_beside = 0;   // units of few rows that go to the blocks of many, the first; the others:
+  int32_t most_rows = 0;  // of a unit
   bool join = false;
   int64_t part_rows = 0;
   int64_t off_unit = 0, off_tile_unit = 0, off_cta = 0, off_seq = 0, off_path = 0, off_span = 0, off_node_seq = 0;  // sections of the plan
