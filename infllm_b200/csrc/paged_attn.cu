@@ -205,9 +205,9 @@ static int join_launch(const PagedParams& P, cudaStream_t s) {
 namespace {
 
 // Work, in what a tile of 128 rows by 128 keys takes (0.9 us where the products are the bound)
-constexpr int kUnitWork = 4;   // of a unit of many rows besides its tiles
+constexpr int kUnitWork = 6;   // of a unit of many rows besides its tiles
 constexpr int kBlockWork = 4;  // worth a block
-constexpr int kGroupWork = 3;  // of a group of 16 keys for few rows by a warp beside the products
+constexpr int kGroupWork = 2;  // of a group of 16 keys for few rows by a warp beside the products
 
 struct Node {
   int64_t key0, key1;
@@ -480,6 +480,9 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     if (!d_q || !d_out || !d_work) return fail(INFLLM_E_BADARG, "page_batch_attend: null pointer");
     if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_work) % 16 || (q_bs | q_hs | q_ts) % 8)
       return fail(INFLLM_E_BADARG, "page_batch_attend: rows must be 16-byte aligned");
+    // (a row's place in the queries is counted in 16 bytes, in 31 bits)
+    const int64_t far = std::max<int64_t>((int64_t)b->seqs.size() - 1, 0) * q_bs + (int64_t)(n_heads - 1) * q_hs + (int64_t)(b->most - 1) * q_ts;
+    if (q_bs < 0 || q_hs < 0 || q_ts < 0 || far / 8 > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_attend: queries that lie %lld bytes apart", (long long)far * 2);
     DeviceScope scope(c.device);
     cudaStream_t s = (cudaStream_t)stream;
     if (b->upload) INFLLM_CUDA_OK(cudaMemcpyAsync(d_work, b->plan.data(), b->plan.size() * 4, cudaMemcpyHostToDevice, s));

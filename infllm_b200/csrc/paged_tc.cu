@@ -254,10 +254,10 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
       int u, n, key0, rows, lim, all;
       bool two, whole;
       int64_t out;  // row of the output, or of the partial results
-      const char* q;
+      int q;  // 16-byte pieces from the first query's first row to its own, -1: none
     };
     auto find = [&](int u) {  // the team's next unit from u on: of the plan alone
-      Turn t{u, 0, 0, 0, 0, 0, false, false, 0, nullptr};
+      Turn t{u, 0, 0, 0, 0, 0, false, false, 0, -1};
       for (; t.u < u1; ++t.u)
         if (team == 0 || __ldg(&P.tile_unit[t.u].rows) > 128) break;
       if (t.u >= u1) return t;
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
       if (row < t.rows) {
         const RowAt at = row_at(P, U.node_seq, U.row0 + team * 128 + row);
         t.lim = at.i < P.most - __ldg(&P.seq[at.b].count) ? 0 : min(t.lim, U.lim0 + at.i);
-        t.q = P.q + at.b * P.q_bs + (int64_t)(U.hkv * P.group + at.h) * P.q_hs + at.i * P.q_ts;
+        t.q = (int)((at.b * P.q_bs + (int64_t)(U.hkv * P.group + at.h) * P.q_hs + at.i * P.q_ts) / 16);
         t.out = t.whole ? ((int64_t)at.b * P.most + at.i) * (P.n_kv * P.group) + U.hkv * P.group + at.h : (int64_t)U.part + team * 128 + row;
       }
       t.all = __reduce_min_sync(0xffffffffu, t.lim);
@@ -276,21 +276,18 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
     };
     auto queries = [&](const Turn& t) {
       // The warp's 32 rows, 16 bytes a lane, swizzled as TMA would have them.  No product reads the last unit's any more: its
-      // scores have been seen.
+      // scores have been seen.  (Rolled, and past the registers: a unit waits for the instructions of what runs once, and
+      // for one load; unrolled over 16 registers this took 5 us instead of 1.5.)
       constexpr int kPer = kDim / 8, kAt = 32 / kPer;
-      const int c = lane % kPer, r0 = lane / kPer;
-      unsigned char* to = smem + L::kQ + team * L::kTileBytes + quad * 32 * 128 + (c >> 3) * kSubTileBytes;
-      uint4 v[kPer];
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const char* p = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(t.q), k * kAt + r0));
-        v[k] = p ? __ldg(reinterpret_cast<const uint4*>(p + c * 16)) : make_uint4(0, 0, 0, 0);
+      const int c = lane % kPer;
+      const uint32_t to = sQ + team * L::kTileBytes + quad * 32 * 128 + (c >> 3) * kSubTileBytes;
+#pragma unroll 1
+      for (int r = lane / kPer; r < 32; r += kAt) {
+        const int from = __shfl_sync(0xffffffffu, t.q, r);
+        mma::cp_async16(to + r * 128 + (((c & 7) ^ (r & 7)) << 4), P.q + (int64_t)max(from, 0) * 16 + c * 16, from >= 0);
       }
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int r = k * kAt + r0;
-        *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
-      }
+      mma::cp_async_commit();
+      mma::cp_async_wait<0>();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
