@@ -204,10 +204,11 @@ static int join_launch(const PagedParams& P, cudaStream_t s) {
 // ----------------------------------------------------------------------------------------------------------- the plan
 namespace {
 
-// Work, in what a tile of 128 rows by 128 keys takes (0.9 us where the products are the bound)
-constexpr int kUnitWork = 6;   // of a unit of many rows besides its tiles
-constexpr int kBlockWork = 4;  // worth a block
-constexpr int kGroupWork = 2;  // of a group of 16 keys for few rows by a warp beside the products
+// Work, in half microseconds
+int64_t tile_work(int64_t rows) { return rows > 128 ? 4 : 3; }  // of 128 keys: bound by the products, or by the keys' bytes
+constexpr int kUnitWork = 10;  // of a unit of many rows besides its tiles
+constexpr int kBlockWork = 8;  // worth a block
+constexpr int kGroupWork = 4;  // of a group of 16 keys for few rows, by a warp beside the products
 
 struct Node {
   int64_t key0, key1;
@@ -317,7 +318,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
       const int64_t keys = std::max<int64_t>(0, end - N.key0);
       AttnUnit u{b->seqs[N.seqs[0]], (int32_t)N.key0, (int32_t)keys, leaf ? (int32_t)(N.key1 - most + 1) : kSeeAll, (int32_t)r, in, (int32_t)node_seq.size(), 0, 0, -1, {0, 0}};
       tiles.push_back({u, many, leaf && tree.path[N.seqs[0]].size() == 1});
-      if (many) many_work += ceil_div(keys, 128) * (in > 128 ? 2 : 1) * n_kv, many_units += keys > 0 ? n_kv : 0;
+      if (many) many_work += ceil_div(keys, 128) * tile_work(in) * n_kv, many_units += keys > 0 ? n_kv : 0;
       else few_work += ceil_div(keys, 16) * n_kv;
     }
     node_seq.insert(node_seq.end(), N.seqs.begin(), N.seqs.end());
@@ -369,7 +370,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   for (size_t x = 0; x < tiles.size(); ++x) {
     const Tile& t = tiles[x];
     if (!t.many) continue;
-    const int64_t n_tiles = ceil_div(t.unit.keys, 128), weight = t.unit.rows > 128 ? 2 : 1;
+    const int64_t n_tiles = ceil_div(t.unit.keys, 128), weight = tile_work(t.unit.rows);
     for (int h = 0; h < n_kv; ++h) {
       AttnUnit u = t.unit;
       u.hkv = h;
