@@ -209,6 +209,12 @@ class PagedBatch:
             at = t.data_ptr()
         return t, at, bs, hs, ts
 
+    def _out(self, like, heads):
+        """(batch, heads, tokens, head_dim) over memory of (batch, tokens, heads, head_dim)."""
+        if self.tokens == 1:
+            return like.new_empty((self._n, heads, 1, self.cache.head_dim))
+        return like.new_empty((self._n, self.tokens, heads, self.cache.head_dim)).permute(0, 2, 1, 3)
+
     def write(self, layer, k, v, q=None, rope=None):
         """The step's keys and values (batch, n_kv_heads, tokens, head_dim) into a layer's pages.  With `rope`, a
         RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q)."""
@@ -220,7 +226,7 @@ class PagedBatch:
         if q is not None:
             heads = q.size(1)
             q, q_at, q_bs, q_hs, q_ts = self._rows(q, heads, "q")
-            out = torch.empty((self._n, self.tokens, heads, c.head_dim), dtype=c.dtype, device=c.device)
+            out = self._out(q, heads)
             at = out.data_ptr()
         if rope is not None:
             if not isinstance(rope, RotaryEmbeddingESM) or rope.dim != c.head_dim:
@@ -231,7 +237,7 @@ class PagedBatch:
                                                at, heads, cos, sin, rows, _lib.raw_stream(c.device))
         if rc:
             _lib.check(rc)
-        return None if out is None else out.permute(0, 2, 1, 3)
+        return out
 
     def attend(self, layer, q, scale=None, return_lse=False):
         """Attention of the step's queries (batch, n_heads, tokens, head_dim) to their sequences' keys up to their own places.
@@ -240,7 +246,7 @@ class PagedBatch:
         c = self.cache
         heads = q.size(1)
         q, at, bs, hs, ts = self._rows(q, heads, "q")
-        out = torch.empty((self._n, self.tokens, heads, c.head_dim), dtype=c.dtype, device=c.device)
+        out = self._out(q, heads)
         lse = lse_at = None
         if return_lse:
             lse = torch.empty((self._n, self.tokens, heads), dtype=torch.float32, device=c.device)
@@ -258,5 +264,4 @@ class PagedBatch:
                                                     stream)
         if rc:
             _lib.check(rc)
-        out = out.permute(0, 2, 1, 3)
         return (out, lse.permute(0, 2, 1)) if return_lse else out

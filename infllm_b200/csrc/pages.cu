@@ -15,19 +15,23 @@ namespace infllm {
 
 // ---------------------------------------------------------------------------------------------------------- changes
 // One kernel makes all changes of a call: items [0, n_rows) copy a row of the table (a: from row, b: to row, c: entries),
-// the next n_edits set entries (a: index, b: page, and c, d another one, index -1: none), the rest move tokens
-// (a: from page, b: to page, c: from place | to place << 16, d: tokens) in all layers, keys and values.
-// Pages that are written were free before the call and rows that are written belong to sequences that were not read from, so the order of the blocks does not matter.
-// It is bound by the bytes of the tokens that it moves, read and written once.
+// the next n_edits set entries (a: index, b: page, and c, d another one, index -1: none), the next n_moves move tokens in all
+// layers, keys and values (a: from page, b: the first of the pages to move them to, c: from place | to place << 16, d: tokens |
+// pages << 16); those pages' numbers are behind them, four to an item.
+// Pages that are written were free before the call, and rows that are written belong to sequences that are not read from, so
+// that the order of the blocks does not matter.  It is bound by the bytes of the tokens, read once and written as often as there
+// are pages for them: half of two 65536-token sequences of four layers (2.1 GB) in 325 us, 6.6 TB/s; the last page of a sequence
+// for 64 forks in eight layers (268 MB written) in FORKTIME.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveAhead = 4;  // 16-byte loads of a thread in flight
+constexpr int kMostTo = 256;   // pages of a move
 
 template <int kItems>
 struct PageChanges {
   const char* from;  // the pools that tokens are moved from and to, of from_pages and to_pages pages
   char* to;
   int32_t* table;
-  int32_t n_rows, n_edits, max_pages, parts;  // parts: blocks of a move
+  int32_t n_rows, n_edits, n_moves, max_pages, parts;       // parts: blocks of a move
   int32_t planes, from_pages, to_pages, n_kv, page, dim16;  // dim16: 16-byte pieces of a row
   PageItem item[kItems];
 };
@@ -52,15 +56,17 @@ __global__ void __launch_bounds__(kMoveThreads) page_change_kernel(const __grid_
     return;
   }
   const PageItem it = P.item[P.n_rows + P.n_edits + b / P.parts];
-  const int part = b % P.parts;
+  const int32_t* pages = reinterpret_cast<const int32_t*>(P.item + P.n_rows + P.n_edits + P.n_moves) + it.b;
+  const int part = b % P.parts, n_to = it.d >> 16;
   const int from = it.c & 0xffff, to = it.c >> 16;
   // 16-byte pieces of the move: (plane, head, token, piece); rows of a head are one stretch on both sides
-  const int strip = it.d * P.dim16;
+  const int strip = (it.d & 0xffff) * P.dim16;
   const uint32_t total = (uint32_t)P.planes * P.n_kv * strip;
   const uint32_t share = (total + P.parts - 1) / P.parts, end = min(total, (part + 1) * share);
   const uint4* src = reinterpret_cast<const uint4*>(P.from);
   uint4* dst = reinterpret_cast<uint4*>(P.to);
   const int head = P.page * P.dim16;  // pieces of a head's rows of a page
+  const int64_t page16 = (int64_t)P.n_kv * head;
   for (uint32_t i = part * share + threadIdx.x; i < end; i += kMoveThreads * kMoveAhead) {
     uint4 v[kMoveAhead];
     int64_t at[kMoveAhead];
@@ -69,33 +75,50 @@ __global__ void __launch_bounds__(kMoveThreads) page_change_kernel(const __grid_
       const uint32_t j = i + k * kMoveThreads;
       if (j >= end) continue;
       const uint32_t s = j / strip, r = j - s * strip, plane = s / P.n_kv, h = s - plane * P.n_kv;
-      v[k] = src[(((int64_t)plane * P.from_pages + it.a) * P.n_kv + h) * head + from * P.dim16 + r];
-      at[k] = (((int64_t)plane * P.to_pages + it.b) * P.n_kv + h) * head + to * P.dim16 + r;
+      v[k] = src[((int64_t)plane * P.from_pages + it.a) * page16 + h * head + from * P.dim16 + r];
+      at[k] = (int64_t)plane * P.to_pages * page16 + h * head + to * P.dim16 + r;
     }
+#pragma unroll 1
+    for (int x = 0; x < n_to; ++x) {
+      const int64_t page = pages[x] * page16;
 #pragma unroll
-    for (int k = 0; k < kMoveAhead; ++k)
-      if (i + k * kMoveThreads < end) dst[at[k]] = v[k];
+      for (int k = 0; k < kMoveAhead; ++k)
+        if (i + k * kMoveThreads < end) dst[at[k] + page] = v[k];
+    }
   }
 }
 
+// Items of one launch: a stretch of each list.
+struct ChangeSpan {
+  size_t r0, r1, e0, e1, m0, m1;
+};
+
 template <int kItems>
-static int launch_changes(infllm_pages* p, const infllm_pages* from, size_t r0, size_t r1, size_t e0, size_t e1, size_t m0, size_t m1, cudaStream_t s) {
-  const infllm_pages_config& c = p->cfg;
-  const int n_moves = (int)(m1 - m0);
+static int launch_changes(infllm_pages* p, const infllm_pages* from, const ChangeSpan& c, cudaStream_t s) {
+  const infllm_pages_config& g = p->cfg;
   PageChanges<kItems> P;
-  P.from = (const char*)from->cfg.d_pages, P.to = (char*)c.d_pages;
-  P.table = c.d_table;
-  P.n_rows = (int)(r1 - r0), P.n_edits = (int)(e1 - e0), P.max_pages = c.max_pages;
-  P.planes = 2 * c.n_layers, P.from_pages = from->cfg.n_pages, P.to_pages = c.n_pages;
-  P.n_kv = c.n_kv_heads, P.page = c.page_size, P.dim16 = c.head_dim / 8;
-  if (r1 > r0) memcpy(P.item, &p->rows[r0], (r1 - r0) * sizeof(PageItem));
-  if (e1 > e0) memcpy(P.item + P.n_rows, &p->edits[e0], (e1 - e0) * sizeof(PageItem));
-  if (m1 > m0) memcpy(P.item + P.n_rows + P.n_edits, &p->moves[m0], (m1 - m0) * sizeof(PageItem));
-  // blocks of a move: two rounds of a block's loads each
+  P.from = (const char*)from->cfg.d_pages, P.to = (char*)g.d_pages;
+  P.table = g.d_table;
+  P.n_rows = (int)(c.r1 - c.r0), P.n_edits = (int)(c.e1 - c.e0), P.n_moves = (int)(c.m1 - c.m0), P.max_pages = g.max_pages;
+  P.planes = 2 * g.n_layers, P.from_pages = from->cfg.n_pages, P.to_pages = g.n_pages;
+  P.n_kv = g.n_kv_heads, P.page = g.page_size, P.dim16 = g.head_dim / 8;
+  PageItem* at = P.item;
+  at = std::copy(p->rows.begin() + c.r0, p->rows.begin() + c.r1, at);
+  at = std::copy(p->edits.begin() + c.e0, p->edits.begin() + c.e1, at);
   int32_t most = 0;
-  for (size_t i = m0; i < m1; ++i) most = std::max(most, p->moves[i].d);
-  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div((int64_t)P.planes * P.n_kv * most * P.dim16, 2 * kMoveThreads * kMoveAhead), 65535));
-  const int64_t blocks = P.n_rows + (P.n_edits > 0) + (int64_t)n_moves * P.parts;
+  if (c.m1 > c.m0) {
+    const int32_t first = p->moves[c.m0].b, last = p->moves[c.m1 - 1].b + (p->moves[c.m1 - 1].d >> 16);
+    for (size_t i = c.m0; i < c.m1; ++i, ++at) {
+      *at = p->moves[i];
+      at->b -= first;
+      most = std::max(most, at->d & 0xffff);
+    }
+    std::copy(p->to_pages.begin() + first, p->to_pages.begin() + last, reinterpret_cast<int32_t*>(at));
+  }
+  // blocks of a move: a round or two of a block's loads each
+  const int64_t pieces = (int64_t)P.planes * P.n_kv * most * P.dim16, round = kMoveThreads * kMoveAhead;
+  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(pieces, P.n_moves * pieces > 2 * 148 * 8 * round ? 2 * round : round), 65535));
+  const int64_t blocks = P.n_rows + (P.n_edits > 0) + (int64_t)P.n_moves * P.parts;
   page_change_kernel<kItems><<<(unsigned)blocks, kMoveThreads, 0, s>>>(P);
   INFLLM_LAUNCH_OK("page_change_kernel");
   return INFLLM_OK;
@@ -103,26 +126,31 @@ static int launch_changes(infllm_pages* p, const infllm_pages* from, size_t r0, 
 
 // makes the changes that a call has listed; tokens are moved from the pages of `from`
 static int flush(infllm_pages* p, const infllm_pages* from, cudaStream_t s) {
-  constexpr size_t kSmall = 60, kLarge = 1000;  // of 16 bytes each: a kernel's arguments, up to 4 KB and up to 32
+  // items of 16 bytes: a kernel's arguments, of 1, 4 and 16 KB (a launch costs about 0.3 us more per KB)
+  constexpr size_t kSmall = 56, kMiddle = 250, kLarge = 1000;
+  static_assert(kLarge > 2 + kMostTo / 4, "");
   int rc = INFLLM_OK;
   if (p->cfg.device >= 0) {
-    size_t r = 0, e = 0, m = 0;
-    while (rc == INFLLM_OK && r + e + m < p->rows.size() + p->edits.size() + p->moves.size()) {
-      const size_t left = p->rows.size() + p->edits.size() + p->moves.size() - r - e - m;
-      size_t room = left <= kSmall ? kSmall : kLarge;
-      const size_t r1 = std::min(p->rows.size(), r + room);
-      room -= r1 - r;
-      const size_t e1 = std::min(p->edits.size(), e + room);
-      room -= e1 - e;
-      const size_t m1 = std::min(p->moves.size(), m + room);
-      rc = left <= kSmall ? launch_changes<kSmall>(p, from, r, r1, e, e1, m, m1, s)
-                          : launch_changes<kLarge>(p, from, r, r1, e, e1, m, m1, s);
-      r = r1, e = e1, m = m1;
+    ChangeSpan c{0, 0, 0, 0, 0, 0};
+    while (rc == INFLLM_OK && (c.r1 < p->rows.size() || c.e1 < p->edits.size() || c.m1 < p->moves.size())) {
+      size_t used = 0;
+      c.r0 = c.r1, c.e0 = c.e1, c.m0 = c.m1;
+      c.r1 = std::min(p->rows.size(), c.r0 + kLarge), used += c.r1 - c.r0;
+      c.e1 = std::min(p->edits.size(), c.e0 + kLarge - used), used += c.e1 - c.e0;
+      size_t to = 0;  // pages of the moves
+      while (c.m1 < p->moves.size()) {
+        const size_t more = to + (size_t)(p->moves[c.m1].d >> 16);
+        if (used + (c.m1 - c.m0 + 1) + (more + 3) / 4 > kLarge) break;
+        to = more, ++c.m1;
+      }
+      used += c.m1 - c.m0 + (to + 3) / 4;
+      rc = used <= kSmall ? launch_changes<kSmall>(p, from, c, s) : used <= kMiddle ? launch_changes<kMiddle>(p, from, c, s) : launch_changes<kLarge>(p, from, c, s);
     }
   }
   p->rows.clear();
   p->edits.clear();
   p->moves.clear();
+  p->to_pages.clear();
   return rc;
 }
 
@@ -160,8 +188,18 @@ static void set_entry(infllm_pages* p, int32_t row, size_t at, int32_t page) {
   else p->edits.push_back({index, page, -1, 0});
 }
 
+// (a move of the same tokens as the last one's is the last one, to another page too)
 static void move_tokens(infllm_pages* p, int32_t from, int32_t from_at, int32_t to, int32_t to_at, int32_t n) {
-  p->moves.push_back({from, to, from_at | to_at << 16, n});
+  const int32_t at = from_at | to_at << 16;
+  p->to_pages.push_back(to);
+  if (!p->moves.empty()) {
+    PageItem& m = p->moves.back();
+    if (m.a == from && m.c == at && (m.d & 0xffff) == n && (m.d >> 16) < kMostTo) {
+      m.d += 1 << 16;
+      return;
+    }
+  }
+  p->moves.push_back({from, (int32_t)p->to_pages.size() - 1, at, n | 1 << 16});
 }
 
 static int need_pages(const infllm_pages* p, int64_t n, const char* what) {
@@ -251,6 +289,7 @@ int batch_alive(const infllm_page_batch* b, const char* what) {
 // a token; a thread has 8 dimensions of the first half of a row and the 8 that go with them in the second, so that it needs
 // one stretch of the tables for all its rows, and keeps it.  Bound by the bytes of q, k and v, read and written once.
 constexpr int kWriteThreads = 256;
+constexpr int kWriteAhead = 3;   // rows of a thread in flight
 constexpr int kWriteSeqs = 128;  // of a launch
 
 struct WriteParams {
@@ -265,7 +304,7 @@ struct WriteParams {
   BatchSeq seq[kWriteSeqs];
 };
 
-template <typename T, int kDim, bool kRope>
+template <typename T>
 __device__ __forceinline__ void rotate8(uint4& lo, uint4& hi, const float* cs, const float* sn) {
   T *a = reinterpret_cast<T*>(&lo), *b = reinterpret_cast<T*>(&hi);
 #pragma unroll
@@ -297,26 +336,35 @@ __global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const __grid_
   const int place = S.length - S.count + at;
   char* const page_at = at >= 0 ? P.pages + ((int64_t)__ldg(P.table + (int64_t)S.row * P.max_pages + place / P.page) * P.n_kv * P.page + place % P.page) * kDim * 2
                                 : nullptr;
-  for (int r = threadIdx.x / kPer; r < n_rows; r += kWriteThreads / kPer) {
-    const char* src;
-    char* dst;
-    bool turn = kRope;
-    if (r < P.n_heads) {
-      src = P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts;
-      dst = P.q_out + ((bb * P.most + i) * P.n_heads + r) * (int64_t)(kDim * 2);
-    } else {
-      const bool val = r >= P.n_heads + P.n_kv;
-      const int h = r - P.n_heads - (val ? P.n_kv : 0);
-      src = val ? P.v + bb * P.v_bs + h * P.v_hs + i * P.v_ts : P.k + bb * P.k_bs + h * P.k_hs + i * P.k_ts;
-      dst = page_at + (int64_t)h * P.page * kDim * 2 + (val ? P.plane : 0);
-      turn = kRope && !val;
-      if (at < 0) continue;
+  constexpr int kStep = kWriteThreads / kPer;
+  for (int r0 = threadIdx.x / kPer; r0 < n_rows; r0 += kStep * kWriteAhead) {
+    uint4 lo[kWriteAhead], hi[kWriteAhead];
+    char* to[kWriteAhead];
+#pragma unroll
+    for (int k = 0; k < kWriteAhead; ++k) {
+      const int r = r0 + k * kStep;
+      to[k] = nullptr;
+      if (r >= n_rows) continue;
+      const char* src;
+      if (r < P.n_heads) {
+        src = P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts;
+        to[k] = P.q_out + ((bb * P.most + i) * P.n_heads + r) * (int64_t)(kDim * 2);
+      } else {
+        const bool val = r >= P.n_heads + P.n_kv;
+        const int h = r - P.n_heads - (val ? P.n_kv : 0);
+        src = val ? P.v + bb * P.v_bs + h * P.v_hs + i * P.v_ts : P.k + bb * P.k_bs + h * P.k_hs + i * P.k_ts;
+        if (at >= 0) to[k] = page_at + (int64_t)h * P.page * kDim * 2 + (val ? P.plane : 0);
+      }
+      lo[k] = hi[k] = make_uint4(0, 0, 0, 0);  // (no token: its query is not one)
+      if (at >= 0) lo[k] = *reinterpret_cast<const uint4*>(src + c * 16), hi[k] = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
     }
-    uint4 lo = *reinterpret_cast<const uint4*>(src + c * 16), hi = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
-    if (r < P.n_heads && at < 0) lo = hi = make_uint4(0, 0, 0, 0);  // (no token: its query is not one)
-    else if (turn) rotate8<T, kDim, kRope>(lo, hi, cs, sn);
-    *reinterpret_cast<uint4*>(dst + c * 16) = lo;
-    *reinterpret_cast<uint4*>(dst + kDim + c * 16) = hi;
+#pragma unroll
+    for (int k = 0; k < kWriteAhead; ++k) {
+      if (!to[k]) continue;
+      if (kRope && at >= 0 && r0 + k * kStep < P.n_heads + P.n_kv) rotate8<T>(lo[k], hi[k], cs, sn);
+      *reinterpret_cast<uint4*>(to[k] + c * 16) = lo[k];
+      *reinterpret_cast<uint4*>(to[k] + kDim + c * 16) = hi[k];
+    }
   }
 }
 

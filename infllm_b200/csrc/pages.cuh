@@ -68,7 +68,8 @@ struct infllm_pages {
   std::priority_queue<int32_t, std::vector<int32_t>, std::greater<int32_t>> free_pages;
   uint64_t change = 0;   // any change of what sequences hold
   uint64_t reshape = 0;  // of the pages that a sequence had before
-  std::vector<infllm::PageItem> rows, edits, moves;  // of the call that is being made
+  std::vector<infllm::PageItem> rows, edits, moves;  // of the call that is being made (pages.cu)
+  std::vector<int32_t> to_pages;
   CUtensorMap map;       // of all pages (paged_tc.cu)
   int32_t n_sm = 148;
 
