@@ -21,7 +21,7 @@ namespace infllm {
 // Pages that are written were free before the call, and rows that are written belong to sequences that are not read from, so
 // that the order of the blocks does not matter.  It is bound by the bytes of the tokens, read once and written as often as there
 // are pages for them: half of two 65536-token sequences of four layers (2.1 GB) in 325 us, 6.6 TB/s; the last page of a sequence
-// for 64 forks in eight layers (268 MB written) in FORKTIME.
+// for 64 forks in eight layers (268 MB written) in 50.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveAhead = 4;  // 16-byte loads of a thread in flight
 constexpr int kMostTo = 256;   // pages of a move
@@ -31,7 +31,8 @@ struct PageChanges {
   const char* from;  // the pools that tokens are moved from and to, of from_pages and to_pages pages
   char* to;
   int32_t* table;
-  int32_t n_rows, n_edits, n_moves, max_pages, parts;       // parts: blocks of a move
+  int32_t n_rows, n_edits, n_moves, max_pages;
+  int32_t parts, shares;  // blocks of a move: parts of its tokens by shares of the pages that they go to
   int32_t planes, from_pages, to_pages, n_kv, page, dim16;  // dim16: 16-byte pieces of a row
   PageItem item[kItems];
 };
@@ -55,9 +56,9 @@ __global__ void __launch_bounds__(kMoveThreads) page_change_kernel(const __grid_
     }
     return;
   }
-  const PageItem it = P.item[P.n_rows + P.n_edits + b / P.parts];
+  const PageItem it = P.item[P.n_rows + P.n_edits + b / (P.parts * P.shares)];
   const int32_t* pages = reinterpret_cast<const int32_t*>(P.item + P.n_rows + P.n_edits + P.n_moves) + it.b;
-  const int part = b % P.parts, n_to = it.d >> 16;
+  const int part = b % P.parts, to0 = b / P.parts % P.shares, n_to = it.d >> 16;
   const int from = it.c & 0xffff, to = it.c >> 16;
   // 16-byte pieces of the move: (plane, head, token, piece); rows of a head are one stretch on both sides
   const int strip = (it.d & 0xffff) * P.dim16;
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(kMoveThreads) page_change_kernel(const __grid_
       at[k] = (int64_t)plane * P.to_pages * page16 + h * head + to * P.dim16 + r;
     }
 #pragma unroll 1
-    for (int x = 0; x < n_to; ++x) {
+    for (int x = to0; x < n_to; x += P.shares) {
       const int64_t page = pages[x] * page16;
 #pragma unroll
       for (int k = 0; k < kMoveAhead; ++k)
@@ -105,20 +106,22 @@ static int launch_changes(infllm_pages* p, const infllm_pages* from, const Chang
   PageItem* at = P.item;
   at = std::copy(p->rows.begin() + c.r0, p->rows.begin() + c.r1, at);
   at = std::copy(p->edits.begin() + c.e0, p->edits.begin() + c.e1, at);
-  int32_t most = 0;
+  int32_t most = 0, most_to = 1;
   if (c.m1 > c.m0) {
     const int32_t first = p->moves[c.m0].b, last = p->moves[c.m1 - 1].b + (p->moves[c.m1 - 1].d >> 16);
     for (size_t i = c.m0; i < c.m1; ++i, ++at) {
       *at = p->moves[i];
       at->b -= first;
-      most = std::max(most, at->d & 0xffff);
+      most = std::max(most, at->d & 0xffff), most_to = std::max(most_to, at->d >> 16);
     }
     std::copy(p->to_pages.begin() + first, p->to_pages.begin() + last, reinterpret_cast<int32_t*>(at));
   }
-  // blocks of a move: a round or two of a block's loads each
-  const int64_t pieces = (int64_t)P.planes * P.n_kv * most * P.dim16, round = kMoveThreads * kMoveAhead;
-  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(pieces, P.n_moves * pieces > 2 * 148 * 8 * round ? 2 * round : round), 65535));
-  const int64_t blocks = P.n_rows + (P.n_edits > 0) + (int64_t)P.n_moves * P.parts;
+  // a round of a block's loads each, or two where there are many; and the pages of a move shared out until there are sixteen blocks
+  // per SM (64 forks of a page in eight layers, 268 MB written: 67 us by blocks that have all 64 pages, 50 so)
+  const int64_t pieces = (int64_t)P.planes * P.n_kv * most * P.dim16, round = kMoveThreads * kMoveAhead, enough = (int64_t)p->n_sm * 16;
+  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(pieces, P.n_moves * pieces > 2 * enough * round ? 2 * round : round), 65535));
+  P.shares = (int)std::max<int64_t>(1, std::min<int64_t>(most_to, enough / std::max<int64_t>(1, (int64_t)P.n_moves * P.parts)));
+  const int64_t blocks = P.n_rows + (P.n_edits > 0) + (int64_t)P.n_moves * P.parts * P.shares;
   page_change_kernel<kItems><<<(unsigned)blocks, kMoveThreads, 0, s>>>(P);
   INFLLM_LAUNCH_OK("page_change_kernel");
   return INFLLM_OK;
@@ -287,9 +290,10 @@ int batch_alive(const infllm_page_batch* b, const char* what) {
 // ------------------------------------------------------------------------------------------------------------ writes
 // New tokens' keys and values into their pages, keys and queries rotated to the tokens' positions on the way.  A block has
 // a token; a thread has 8 dimensions of the first half of a row and the 8 that go with them in the second, so that it needs
-// one stretch of the tables for all its rows, and keeps it.  Bound by the bytes of q, k and v, read and written once.
-constexpr int kWriteThreads = 256;
-constexpr int kWriteAhead = 3;   // rows of a thread in flight
+// one stretch of the tables for all its rows, and keeps it.  Bound by the bytes of q, k and v, read and written once: 8192 tokens
+// of 32 query and 8 KV heads (201 MB) in 40 us, 5.0 TB/s; with blocks of 256 threads 46, of 512 64, with three rows of a thread
+// in flight 79 (fewer loads at once for a token of 48 rows).
+constexpr int kWriteThreads = 128;
 constexpr int kWriteSeqs = 128;  // of a launch
 
 struct WriteParams {
@@ -336,35 +340,26 @@ __global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const __grid_
   const int place = S.length - S.count + at;
   char* const page_at = at >= 0 ? P.pages + ((int64_t)__ldg(P.table + (int64_t)S.row * P.max_pages + place / P.page) * P.n_kv * P.page + place % P.page) * kDim * 2
                                 : nullptr;
-  constexpr int kStep = kWriteThreads / kPer;
-  for (int r0 = threadIdx.x / kPer; r0 < n_rows; r0 += kStep * kWriteAhead) {
-    uint4 lo[kWriteAhead], hi[kWriteAhead];
-    char* to[kWriteAhead];
-#pragma unroll
-    for (int k = 0; k < kWriteAhead; ++k) {
-      const int r = r0 + k * kStep;
-      to[k] = nullptr;
-      if (r >= n_rows) continue;
-      const char* src;
-      if (r < P.n_heads) {
-        src = P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts;
-        to[k] = P.q_out + ((bb * P.most + i) * P.n_heads + r) * (int64_t)(kDim * 2);
-      } else {
-        const bool val = r >= P.n_heads + P.n_kv;
-        const int h = r - P.n_heads - (val ? P.n_kv : 0);
-        src = val ? P.v + bb * P.v_bs + h * P.v_hs + i * P.v_ts : P.k + bb * P.k_bs + h * P.k_hs + i * P.k_ts;
-        if (at >= 0) to[k] = page_at + (int64_t)h * P.page * kDim * 2 + (val ? P.plane : 0);
-      }
-      lo[k] = hi[k] = make_uint4(0, 0, 0, 0);  // (no token: its query is not one)
-      if (at >= 0) lo[k] = *reinterpret_cast<const uint4*>(src + c * 16), hi[k] = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
+  for (int r = threadIdx.x / kPer; r < n_rows; r += kWriteThreads / kPer) {
+    const char* src;
+    char* to;
+    const bool is_q = r < P.n_heads, val = r >= P.n_heads + P.n_kv;
+    if (is_q) {
+      src = P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts;
+      to = P.q_out + ((bb * P.most + i) * P.n_heads + r) * (int64_t)(kDim * 2);
+    } else {
+      if (at < 0) return;  // (queries come first: nothing is left of this token)
+      const int h = r - P.n_heads - (val ? P.n_kv : 0);
+      src = val ? P.v + bb * P.v_bs + h * P.v_hs + i * P.v_ts : P.k + bb * P.k_bs + h * P.k_hs + i * P.k_ts;
+      to = page_at + (int64_t)h * P.page * kDim * 2 + (val ? P.plane : 0);
     }
-#pragma unroll
-    for (int k = 0; k < kWriteAhead; ++k) {
-      if (!to[k]) continue;
-      if (kRope && at >= 0 && r0 + k * kStep < P.n_heads + P.n_kv) rotate8<T>(lo[k], hi[k], cs, sn);
-      *reinterpret_cast<uint4*>(to[k] + c * 16) = lo[k];
-      *reinterpret_cast<uint4*>(to[k] + kDim + c * 16) = hi[k];
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;  // (no token: its query is not one)
+    if (at >= 0) {
+      lo = *reinterpret_cast<const uint4*>(src + c * 16), hi = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
+      if (kRope && !val) rotate8<T>(lo, hi, cs, sn);
     }
+    *reinterpret_cast<uint4*>(to + c * 16) = lo;
+    *reinterpret_cast<uint4*>(to + kDim + c * 16) = hi;
   }
 }
 
