@@ -265,3 +265,31 @@ class PagedBatch:
         if rc:
             _lib.check(rc)
         return (out, lse.permute(0, 2, 1)) if return_lse else out
+
+
+class PagedLayer:
+    """What ATTN_FORWRAD["paged"] takes and returns as past_key_value: a layer of a step's sequences."""
+
+    def __init__(self, batch, layer):
+        self.batch, self.layer = batch, layer
+
+
+def paged_forward(*args, **kwargs):
+    """ATTN_FORWRAD["paged"]: full causal attention of several sequences over a PagedCache, behind the same
+    forward(self, query, key_value, position_bias, use_cache, past_key_value, project_q, project_k, project_v, attention_out,
+    dim_head, num_heads, num_heads_kv) as the other types (inf_llm/attention/inf_llm.py:20-32).  past_key_value is a
+    PagedLayer; its batch was extended by the step's tokens before the first layer."""
+
+    def forward(self, query, key_value, position_bias, use_cache, past_key_value, project_q, project_k, project_v,
+                attention_out, dim_head, num_heads, num_heads_kv):
+        if not isinstance(past_key_value, PagedLayer):
+            raise TypeError('attention type "paged" needs a PagedLayer as past_key_value')
+        n, tokens = query.size(0), query.size(1)
+        q, k, v = (project(x).view(n, tokens, heads, dim_head).permute(0, 2, 1, 3) for project, x, heads in (
+            (project_q, query, num_heads), (project_k, key_value, num_heads_kv), (project_v, key_value, num_heads_kv)))
+        batch, layer = past_key_value.batch, past_key_value.layer
+        o = batch.attend(layer, batch.write(layer, k, v, q, position_bias))
+        o = attention_out(o.permute(0, 2, 1, 3).reshape(n, tokens, num_heads * dim_head))
+        return (o, past_key_value) if use_cache else o
+
+    return forward

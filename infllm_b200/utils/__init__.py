@@ -3,5 +3,6 @@
 from .decoder import HeadGroupDecoder
 from .greedy_search import GreedySearch
 from .patch import patch_hf
+from .shared_prompt import SharedPromptDecoder
 
-__all__ = ["patch_hf", "GreedySearch", "HeadGroupDecoder"]
+__all__ = ["patch_hf", "GreedySearch", "HeadGroupDecoder", "SharedPromptDecoder"]

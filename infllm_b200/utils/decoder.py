@@ -27,22 +27,22 @@ class HeadGroupDecoder:
     """n_layers x (RMSNorm, context-memory attention, RMSNorm, SwiGLU feed-forward), final norm, LM head.
 
     `comm` is a HeadGroupComm when world > 1 (collective construction), `group` the torch.distributed group of the
-    all-reduces.  `attn_kwargs` are the keyword arguments of ATTN_FORWRAD["inf-llm"] (n_local, n_init, topk, ...)."""
+    all-reduces.  `attn_kwargs` are the keyword arguments of ATTN_FORWRAD[attn_type] (n_local, n_init, topk, ...)."""
 
     def __init__(self, n_layers, hidden, n_heads, n_kv_heads, head_dim, ffn, vocab, attn_kwargs, rank=0, world=1,
                  comm=None, group=None, seed=0, dtype=torch.bfloat16, device=None, rope_base=500000.0, eps=1e-5,
-                 init_std=0.02):
+                 init_std=0.02, attn_type="inf-llm"):
         assert n_heads % world == 0 and n_kv_heads % world == 0 and ffn % world == 0
-        assert world == 1 or comm is not None
+        assert world == 1 or comm is not None or attn_type != "inf-llm"  # (the others retrieve nothing)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.n_layers, self.hidden, self.head_dim, self.vocab, self.eps = n_layers, hidden, head_dim, vocab, eps
         self.heads, self.kv_heads = n_heads // world, n_kv_heads // world
         self.rank, self.world, self.group, self.dtype = rank, world, group, dtype
         self.rope = RotaryEmbeddingESM(head_dim, rope_base, 1.0)
         kwargs = dict(attn_kwargs)
-        if world > 1:
+        if comm is not None and world > 1:
             kwargs["head_group_comm"] = comm
-        self.forward = ATTN_FORWRAD["inf-llm"](**kwargs)
+        self.forward = ATTN_FORWRAD[attn_type](**kwargs)
 
         def draw(rows, cols, *key):  # the whole matrix, the same on every rank
             g = torch.Generator(device=self.device).manual_seed(zlib.crc32(repr((seed,) + key).encode()))
@@ -81,7 +81,7 @@ class HeadGroupDecoder:
 
     @torch.inference_mode()
     def step(self, ids):
-        """ids (1, L) -> logits (1, vocab) of the last position; the context memories advance by L tokens."""
+        """ids (B, L) -> logits (B, vocab) of the last position; the context memories advance by L tokens."""
         lin = torch.nn.functional.linear
         h = self.embed[ids]
         for layer in self.layers:
