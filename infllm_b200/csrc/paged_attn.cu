@@ -23,7 +23,7 @@ using namespace mma;
 // ------------------------------------------------------------------------------------------------------- few rows
 // Four warps share a unit's groups of 16 keys and meet in shared memory.
 template <typename T, int kDim, int kNt>
-__global__ void __launch_bounds__(kRowWarps * 32) paged_rows_kernel(const __grid_constant__ PagedParams P) {
+__global__ void __launch_bounds__(kRowWarps * 32, row_blocks(kNt)) paged_rows_kernel(const __grid_constant__ PagedParams P) {
   constexpr int kH = kDim / 64, kPitch = kDim + 4;
   __shared__ __align__(16) float sm_o[kRowWarps][8 * kNt][kPitch];
   __shared__ float sm_m[kRowWarps][8 * kNt], sm_l[kRowWarps][8 * kNt];
@@ -210,6 +210,42 @@ constexpr int kUnitWork = 10;  // of a unit of many rows besides its tiles
 constexpr int kBlockWork = 8;  // worth a block
 constexpr int kGroupWork = 4;  // of a group of 16 keys for few rows, by a warp beside the products
 
+// Groups of 16 keys of a block's unit, where nodes have groups[..] of them for each KV head: so that all blocks run in one, two or
+// some waves of as many as the machine holds, whichever is the shortest.  (A sequence of 131072 keys over 32 heads: 449 us by
+// 608 blocks where 592 run at once, 319 by 1184.)
+int64_t row_chunk(const std::vector<int64_t>& groups, int64_t n_kv, int64_t resident, bool join) {
+  // microseconds of a warp's group while all stream, of a block besides, and of the join where only a cut makes one necessary (128
+  // sequences of up to 300 keys: 32 us where some are cut, 25 where none is)
+  constexpr double kGroup = 3., kBlock = 4., kJoin = 7.;
+  int64_t most = kRowWarps, best = kRowWarps;
+  for (int64_t g : groups) most = std::max(most, ceil_div(g, kRowWarps) * kRowWarps);
+  double least = 1e300;
+  auto blocks = [&](int64_t c) {
+    int64_t n = 0;
+    for (int64_t g : groups) n += std::max<int64_t>(1, ceil_div(g, c * kRowWarps)) * n_kv;
+    return n;
+  };
+  for (int waves = 0; waves <= 6; ++waves) {  // (none: nothing is cut)
+    int64_t lo = waves ? 1 : most / kRowWarps, hi = most / kRowWarps;  // the smallest unit with which there are no more blocks than that
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (blocks(mid) <= waves * resident) hi = mid;
+      else lo = mid + 1;
+    }
+    // equal blocks run in waves; where they differ, the short ones fill up what the long ones leave
+    double sum = 0.;
+    for (int64_t g : groups) {
+      const int64_t n = std::max<int64_t>(1, ceil_div(g, lo * kRowWarps));
+      sum += (double)(n * n_kv) * ((double)ceil_div(g, n * kRowWarps) * kGroup + kBlock);
+    }
+    const double longest = lo * kGroup + kBlock;
+    const double cost = std::min((double)ceil_div(blocks(lo), resident) * longest, sum / (double)resident + .7 * longest) +
+                        (!join && lo * kRowWarps < most ? kJoin : 0.);
+    if (cost < least) least = cost, best = lo * kRowWarps;
+  }
+  return best;
+}
+
 struct Node {
   int64_t key0, key1;
   std::vector<int32_t> seqs;  // of the batch
@@ -330,30 +366,43 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   int64_t part = 0;
   bool join = false;
   // Few rows.  Two warps of each block of many rows take units of them, whoever is free the next, as much as is done by the time
-  // the products are; the rest goes to blocks of four warps, four per SM, in units of equal work.
+  // the products are; the rest goes to blocks of four warps, in units of about equal work.
   const int64_t n_cta = many_units ? std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / kBlockWork)) : 0;
   many_work += kUnitWork * (many_units + n_cta);
   int64_t beside_left = n_cta ? 2 * many_work / kGroupWork : 0;
   const int64_t beside_chunk = std::min<int64_t>(16, std::max<int64_t>(2, ceil_div(few_work, 8 * std::max<int64_t>(n_cta, 1)))) * 16;
-  const int64_t rest = std::max<int64_t>(0, few_work - beside_left);
-  const int64_t rest_chunk = std::max<int64_t>(kRowWarps, ceil_div(ceil_div(rest, p->n_sm * 4), kRowWarps) * kRowWarps) * 16;
-  std::vector<AttnUnit> by_four;
+  std::vector<char> is_beside(tiles.size(), 0);
+  std::vector<int64_t> rest;  // groups of the others
   int32_t most_rows = 0;
+  bool rest_joins = false;
   for (size_t x = 0; x < tiles.size(); ++x) {
     const Tile& t = tiles[x];
     if (t.many) continue;
-    const int64_t keys = t.unit.keys, work = ceil_div(keys, 16) * n_kv;
-    const bool beside = work <= beside_left && !(t.alone && keys == 0);
+    const int64_t groups = ceil_div(t.unit.keys, 16);
+    if (groups * n_kv <= beside_left && !(t.alone && groups == 0)) {
+      is_beside[x] = 1;
+      beside_left -= groups * n_kv;
+    } else {
+      rest.push_back(groups);
+      most_rows = std::max(most_rows, t.unit.rows);
+      rest_joins |= !t.alone;
+    }
+  }
+  const int64_t rest_chunk = row_chunk(rest, n_kv, (int64_t)p->n_sm * row_blocks(most_rows > 8 ? 2 : 1), rest_joins || many_units) * 16;
+  std::vector<AttnUnit> by_four;
+  for (size_t x = 0; x < tiles.size(); ++x) {
+    const Tile& t = tiles[x];
+    if (t.many) continue;
+    const int64_t keys = t.unit.keys;
+    const bool beside = is_beside[x];
     const int64_t chunk = beside ? beside_chunk : rest_chunk, cut = ceil_div(keys, chunk), each = cut ? ceil_div(ceil_div(keys, 16), cut) * 16 : 0;
     std::vector<AttnUnit>& to = beside ? few : by_four;
     AttnUnit u = t.unit;
-    if (!beside) most_rows = std::max(most_rows, u.rows);
     if (!beside && t.alone && cut <= 1) {
       to.push_back(u);
       for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h].n = -1;
       continue;
     }
-    if (beside) beside_left -= work;
     u.part_kv = (int32_t)(cut * u.rows);
     for (int h = 0; h < n_kv; ++h) spans[x * n_kv + h] = {(int32_t)(part + h * cut * u.rows), (int32_t)cut, u.rows, 0};
     for (int64_t k = 0; k < keys; k += each) {

@@ -13,6 +13,8 @@ namespace infllm {
 
 constexpr int kRowWarps = 4;
 constexpr int kRowTile = 16;
+// blocks of four warps per SM: as many as 128 or 168 registers a thread leave room for
+constexpr int row_blocks(int tiles_of_eight) { return tiles_of_eight > 1 ? 3 : 4; }
 
 template <typename T, int kDim, int kNt>  // kNt: tiles of eight rows
 struct RowsWarp {
