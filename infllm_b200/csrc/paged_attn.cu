@@ -193,10 +193,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 template <typename T, int kDim>
 static int join_launch(const PagedParams& P, cudaStream_t s) {
   // eight warps to a row while that still is one wave of blocks, and one where there are rows enough
-  const int64_t rows = (int64_t)P.batch * P.most * P.n_kv * P.group;
-  if (rows <= 148 * 8) launch_chained(paged_join_kernel<T, kDim, 8>, dim3((unsigned)rows), dim3(256), 0, s, P);
-  else if (rows <= 148 * 32) launch_chained(paged_join_kernel<T, kDim, 4>, dim3((unsigned)ceil_div(rows, 2)), dim3(256), 0, s, P);
-  else launch_chained(paged_join_kernel<T, kDim, 1>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, s, P);
+  const int64_t rows = (int64_t)P.batch * P.most * P.n_kv * P.group, warps = 148 * 32 / std::max<int64_t>(rows, 1);
+  auto launch = [&](auto kern, int per_row) { launch_chained(kern, dim3((unsigned)ceil_div(rows * per_row, 8)), dim3(256), 0, s, P); };
+  if (warps >= 8) launch(paged_join_kernel<T, kDim, 8>, 8);
+  else if (warps >= 4) launch(paged_join_kernel<T, kDim, 4>, 4);
+  else if (warps >= 2) launch(paged_join_kernel<T, kDim, 2>, 2);
+  else launch(paged_join_kernel<T, kDim, 1>, 1);
   INFLLM_LAUNCH_OK("paged_join_kernel");
   return INFLLM_OK;
 }
