@@ -372,7 +372,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   const int64_t n_cta = many_units ? std::max<int64_t>(1, std::min<int64_t>(p->n_sm, many_work / kBlockWork)) : 0;
   many_work += kUnitWork * (many_units + n_cta);
   int64_t beside_left = n_cta ? 2 * many_work / kGroupWork : 0;
-  const int64_t beside_chunk = std::min<int64_t>(16, std::max<int64_t>(2, ceil_div(few_work, 8 * std::max<int64_t>(n_cta, 1)))) * 16;
+  const int64_t beside_chunk = std::min<int64_t>(16, std::max<int64_t>(2, ceil_div(few_work, 4 * std::max<int64_t>(n_cta, 1)))) * 16;
   std::vector<char> is_beside(tiles.size(), 0);
   std::vector<int64_t> rest;  // groups of the others
   int32_t most_rows = 0;
