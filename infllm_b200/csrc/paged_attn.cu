@@ -212,6 +212,12 @@ constexpr int kUnitWork = 10;  // of a unit of many rows besides its tiles
 constexpr int kBlockWork = 8;  // worth a block
 constexpr int kGroupWork = 4;  // of a group of 16 keys for few rows, by a warp beside the products
 
+// Work of a batch, in groups of 16 keys by tiles of 16 rows and KV heads, up to which all of it goes to the kernel of few rows: that
+// is through before the tensor-core kernel has begun, and is one launch less where both would be needed.  (Eight tokens on 1000 keys,
+// 1100: 11.6 us instead of 22.6; 30 on 1000, 4500: 17.0, 24.2; 13 of 28/4 heads of 64 on 5000, 8700: 15.2, 16.5; 33 new tokens of a
+// sequence of 2000, 9100: 18.4, 18.5; five times 20 on 700, 9000: 29, 23; ten on 8000, 12300: 24.5, 18.8.)
+constexpr int64_t kLittle = 8800;
+
 // Groups of 16 keys of a block's unit, where nodes have groups[..] of them for each KV head: so that all blocks run in one, two or
 // some waves of as many as the machine holds, whichever is the shortest.  (A sequence of 131072 keys over 32 heads: 449 us by
 // 608 blocks where 592 run at once, 319 by 1184.)
@@ -335,7 +341,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   Tree tree{b, {}, std::vector<std::vector<int32_t>>(n)};
   tree.build(b->order, b->common, 0);
 
-  // row tiles: of up to 256 rows for the tensor cores, of up to 16 for nodes that have no more
+  // row tiles: of up to 256 rows for the tensor cores, of up to 16 for nodes that have no more, or where there is little of all
   struct Tile {
     AttnUnit unit;  // of all its keys
     bool many, alone;
@@ -343,10 +349,13 @@ int make_plan(infllm_page_batch* b, int n_heads) {
   std::vector<Tile> tiles;
   std::vector<int32_t> first_tile, node_seq;
   int64_t few_work = 0, many_work = 0, many_units = 0;  // groups of 16 keys, and tiles of 128 by up to 128 rows
+  int64_t by_sixteen = 0;
+  for (const Node& N : tree.nodes) by_sixteen += ceil_div((int64_t)N.seqs.size() * most * group, kRowTile) * ceil_div(N.key1 - N.key0, 16) * n_kv;
+  const bool little = by_sixteen <= kLittle;
   for (const Node& N : tree.nodes) {
     const bool leaf = N.seqs.size() == 1;
     const int64_t rows = (int64_t)N.seqs.size() * most * group;
-    const bool many = rows > kRowTile;
+    const bool many = rows > kRowTile && !little;
     const int size = many ? kTileRows : kRowTile;
     first_tile.push_back((int32_t)tiles.size());
     for (int64_t r = 0; r < rows; r += size) {
@@ -466,7 +475,7 @@ int make_plan(infllm_page_batch* b, int n_heads) {
     join |= tree.path[i].empty();
     for (int32_t x : tree.path[i]) {
       const Node& N = tree.nodes[x];
-      const int32_t tile = (int64_t)N.seqs.size() * most * group > kRowTile ? kTileRows : kRowTile;
+      const int32_t tile = (int64_t)N.seqs.size() * most * group > kRowTile && !little ? kTileRows : kRowTile;
       const AttnPath a{first_tile[x], tile, (int32_t)(std::find(N.seqs.begin(), N.seqs.end(), i) - N.seqs.begin())};
       if (q.n_path < kNearPath) q.near_path[q.n_path] = a;
       else paths.push_back(a);

@@ -61,6 +61,9 @@ class Kept:
         scale = 1 / math.sqrt(c.head_dim) if scale is None else scale
         u, group = U[c.dtype], heads // c.n_kv_heads
         assert out.shape == q.shape and out.dtype == c.dtype and lse.shape == q.shape[:3]
+        from infllm_b200._lib import device_error
+
+        assert device_error() == (0, 0)
         for i, (s, n) in enumerate(zip(b.seqs, counts)):
             assert (out[i, :, :most - n] == 0).all() and (lse[i, :, :most - n] == -math.inf).all()
             if n == 0:
@@ -114,9 +117,19 @@ def test_several_tokens_each(dtype, page, dim, kv, group, prefix, counts):
 
 @pytest.mark.parametrize("page", [16, 128])
 def test_a_tree_of_forks_and_strangers(page):
-    x = Kept(make(4000 // page + 60, page, 2, 128), 3)
+    _tree(page, 1)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_a_tree_of_long_forks(page):
+    """The same tree with 40 times the prompt: its nodes are the tensor-core kernel's."""
+    _tree(page, 40 * 128 // page)
+
+
+def _tree(page, long):
+    x = Kept(make(4000 // page + 60 + 3 * long, page, 2, 128), 3)
     a, other, empty = x.open(), x.open(), x.open()
-    x.grow([a, other], [page * 3 + 5, 77])
+    x.grow([a, other], [page * 3 * long + 5, 77])
     kids = x.fork(a, 3)
     x.grow(kids, [page * 2, page * 2 + 1, 9])
     grand = x.fork(kids[0], 2) + x.fork(kids[1], 3)
@@ -129,8 +142,9 @@ def test_a_tree_of_forks_and_strangers(page):
     counts = [min(n, x.c.length(s)) for n, s in zip([3, 70, 9, 0, 150, 2, 5, 1, 33, 2, 2], seqs)]  # newest tokens that lie in shared pages
     b.plan(counts)
     x.check(b, counts, 8)
-    x.c.truncate([kids[1], grand[2]], [page * 3 + 9, page * 4])  # inside a page that others share
-    for s, n in ((kids[1], page * 3 + 9), (grand[2], page * 4)):
+    ends = page * 3 * long + 9, page * (3 * long + 1)
+    x.c.truncate([kids[1], grand[2]], ends)  # inside a page that others share
+    for s, n in ((kids[1], ends[0]), (grand[2], ends[1])):
         x.k[s], x.v[s] = x.k[s][:, :n], x.v[s][:, :n]
     counts = [1, 1, 1, 0, 1, 1, 1, 2, 1, 2, 1]
     b.plan(counts)
@@ -140,6 +154,25 @@ def test_a_tree_of_forks_and_strangers(page):
     b = x.c.batch(seqs)
     b.plan(counts)
     x.check(b, counts, 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim,kv,group", [(16, 128, 2, 4), (128, 128, 4, 1), (32, 64, 2, 7), (64, 64, 1, 16), (64, 128, 1, 24)])
+@pytest.mark.parametrize("prefix,counts,tail", [(9000, (1,) * 40, 30), (16000, (1,) * 33, 0), (9001, (17, 0, 40, 33), 100), (0, (2000,), 0), (5000, (700, 3), 1),
+                                                (12345, (1,) * 70, 3), (3000, (65,) * 9, 0), (20000, (5,), 0)])
+def test_many_rows(dtype, page, dim, kv, group, prefix, counts, tail):
+    """Sizes of the tensor-core kernel: nodes of one and of several row tiles and units, whole and ragged last tiles of keys, leaves
+    of few rows beside them."""
+    total = prefix + sum(t + tail + 2 * page for t in counts)
+    x = Kept(make(total // page + 2, page, kv, dim, dtype, max_tokens=32768), prefix + sum(counts))
+    root = x.open()
+    if prefix:
+        x.grow([root], [prefix])
+    seqs = x.fork(root, len(counts))
+    if tail:
+        x.grow(seqs, [1 + (tail + 7 * i) % tail for i in range(len(seqs))])
+    b = x.grow(seqs, list(counts))
+    x.check(b, list(counts), kv * group)
 
 
 @pytest.mark.parametrize("lean", [0.0, 8.0, 60.0])
@@ -335,16 +368,16 @@ def test_another_stream_than_the_default():
         x.check(b, [1] * 6, 8)
 
 
-@pytest.mark.parametrize("n_seqs,n", [(3, 1), (40, 1), (3, 30)])
+@pytest.mark.parametrize("n_seqs,n,prefix", [(3, 1, 900), (40, 1, 900), (3, 30, 900), (40, 1, 9000), (3, 30, 9000)])
 @pytest.mark.parametrize("what", [NAN, math.inf])
-def test_what_is_no_number_stays_in_its_row(n_seqs, n, what):
+def test_what_is_no_number_stays_in_its_row(n_seqs, n, prefix, what):
     """A query that is no number, and a key of a sequence's own that is none, reach that row and that sequence alone."""
-    c = make(400, 16, 2, 128)
+    c = make(prefix // 16 + 400, 16, 2, 128)
     g = torch.Generator(device="cuda").manual_seed(2)
     root = c.open()
     b = c.batch(root)
-    b.extend(900)
-    b.write(0, rand(g, 1, 2, 900, 128), rand(g, 1, 2, 900, 128))
+    b.extend(prefix)
+    b.write(0, rand(g, 1, 2, prefix, 128), rand(g, 1, 2, prefix, 128))
     seqs = c.fork(root, n_seqs)
     b = c.batch(seqs)
     b.extend(n)
