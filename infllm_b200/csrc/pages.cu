@@ -21,9 +21,10 @@ namespace infllm {
 // Pages that are written were free before the call, and rows that are written belong to sequences that are not read from, so
 // that the order of the blocks does not matter.  It is bound by the bytes of the tokens, read once and written as often as there
 // are pages for them: half of two 65536-token sequences of four layers (2.1 GB) in 325 us, 6.6 TB/s; the last page of a sequence
-// for 64 forks in eight layers (268 MB written) in 50.
+// for 64 forks in eight layers (268 MB written) in 47.
 constexpr int kMoveThreads = 256;
-constexpr int kMoveAhead = 4;  // 16-byte loads of a thread in flight
+constexpr int kMoveAhead = 8;  // 16-byte loads of a thread in flight
+constexpr int kChunk = 256;    // 16-byte pieces that a warp takes at once
 constexpr int kMostTo = 256;   // pages of a move
 
 template <int kItems>
@@ -60,31 +61,28 @@ __global__ void __launch_bounds__(kMoveThreads) page_change_kernel(const __grid_
   const int32_t* pages = reinterpret_cast<const int32_t*>(P.item + P.n_rows + P.n_edits + P.n_moves) + it.b;
   const int part = b % P.parts, to0 = b / P.parts % P.shares, n_to = it.d >> 16;
   const int from = it.c & 0xffff, to = it.c >> 16;
-  // 16-byte pieces of the move: (plane, head, token, piece); rows of a head are one stretch on both sides
-  const int strip = (it.d & 0xffff) * P.dim16;
-  const uint32_t total = (uint32_t)P.planes * P.n_kv * strip;
-  const uint32_t share = (total + P.parts - 1) / P.parts, end = min(total, (part + 1) * share);
-  const uint4* src = reinterpret_cast<const uint4*>(P.from);
-  uint4* dst = reinterpret_cast<uint4*>(P.to);
+  // Rows of a head in a plane are one stretch on both sides; a warp takes up to 4 KB of one.
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int strip = (it.d & 0xffff) * P.dim16, chunks = (strip + kChunk - 1) / kChunk, units = P.planes * P.n_kv * chunks;
+  const int u1 = (int)((int64_t)units * (part + 1) / P.parts);
   const int head = P.page * P.dim16;  // pieces of a head's rows of a page
   const int64_t page16 = (int64_t)P.n_kv * head;
-  for (uint32_t i = part * share + threadIdx.x; i < end; i += kMoveThreads * kMoveAhead) {
-    uint4 v[kMoveAhead];
-    int64_t at[kMoveAhead];
-#pragma unroll
-    for (int k = 0; k < kMoveAhead; ++k) {
-      const uint32_t j = i + k * kMoveThreads;
-      if (j >= end) continue;
-      const uint32_t s = j / strip, r = j - s * strip, plane = s / P.n_kv, h = s - plane * P.n_kv;
-      v[k] = src[((int64_t)plane * P.from_pages + it.a) * page16 + h * head + from * P.dim16 + r];
-      at[k] = (int64_t)plane * P.to_pages * page16 + h * head + to * P.dim16 + r;
-    }
-#pragma unroll 1
-    for (int x = to0; x < n_to; x += P.shares) {
-      const int64_t page = pages[x] * page16;
+  for (int u = (int)((int64_t)units * part / P.parts) + warp; u < u1; u += kMoveThreads / 32) {
+    const int s = u / chunks, plane = s / P.n_kv, h = s - plane * P.n_kv, i0 = (u - s * chunks) * kChunk, i1 = min(strip, i0 + kChunk);
+    const uint4* src = reinterpret_cast<const uint4*>(P.from) + ((int64_t)plane * P.from_pages + it.a) * page16 + h * head + from * P.dim16;
+    uint4* dst = reinterpret_cast<uint4*>(P.to) + (int64_t)plane * P.to_pages * page16 + h * head + to * P.dim16;
+    for (int i = i0 + lane; i < i1; i += 32 * kMoveAhead) {
+      uint4 v[kMoveAhead];
 #pragma unroll
       for (int k = 0; k < kMoveAhead; ++k)
-        if (i + k * kMoveThreads < end) dst[at[k] + page] = v[k];
+        if (i + k * 32 < i1) v[k] = src[i + k * 32];
+#pragma unroll 1
+      for (int x = to0; x < n_to; x += P.shares) {
+        uint4* d = dst + pages[x] * page16;
+#pragma unroll
+        for (int k = 0; k < kMoveAhead; ++k)
+          if (i + k * 32 < i1) d[i + k * 32] = v[k];
+      }
     }
   }
 }
@@ -116,10 +114,10 @@ static int launch_changes(infllm_pages* p, const infllm_pages* from, const Chang
     }
     std::copy(p->to_pages.begin() + first, p->to_pages.begin() + last, reinterpret_cast<int32_t*>(at));
   }
-  // a round of a block's loads each, or two where there are many; and the pages of a move shared out until there are sixteen blocks
-  // per SM (64 forks of a page in eight layers, 268 MB written: 67 us by blocks that have all 64 pages, 50 so)
-  const int64_t pieces = (int64_t)P.planes * P.n_kv * most * P.dim16, round = kMoveThreads * kMoveAhead, enough = (int64_t)p->n_sm * 16;
-  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(pieces, P.n_moves * pieces > 2 * enough * round ? 2 * round : round), 65535));
+  // a piece of work for every warp of a block, or two where there are many; and the pages of a move shared out until there are sixteen
+  // blocks per SM (64 forks of a page in eight layers, 268 MB written: 67 us by blocks that have all 64 pages, 47 so)
+  const int64_t units = (int64_t)P.planes * P.n_kv * ceil_div(most * P.dim16, kChunk), warps = kMoveThreads / 32, enough = (int64_t)p->n_sm * 16;
+  P.parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(units, P.n_moves * units > 2 * enough * warps ? 2 * warps : warps), 65535));
   P.shares = (int)std::max<int64_t>(1, std::min<int64_t>(most_to, enough / std::max<int64_t>(1, (int64_t)P.n_moves * P.parts)));
   const int64_t blocks = P.n_rows + (P.n_edits > 0) + (int64_t)P.n_moves * P.parts * P.shares;
   page_change_kernel<kItems><<<(unsigned)blocks, kMoveThreads, 0, s>>>(P);
@@ -175,14 +173,13 @@ static int check_once(const infllm_pages* p, const int32_t* seqs, int n, const c
 }
 
 static int32_t take_page(infllm_pages* p) {
-  const int32_t page = p->free_pages.top();
-  p->free_pages.pop();
+  const int32_t page = p->free_pages.take();
   p->uses[page] = 1;
   return page;
 }
 
 static void drop_page(infllm_pages* p, int32_t page) {
-  if (--p->uses[page] == 0) p->free_pages.push(page);
+  if (--p->uses[page] == 0) p->free_pages.give(page);
 }
 
 static void set_entry(infllm_pages* p, int32_t row, size_t at, int32_t page) {
@@ -206,8 +203,8 @@ static void move_tokens(infllm_pages* p, int32_t from, int32_t from_at, int32_t 
 }
 
 static int need_pages(const infllm_pages* p, int64_t n, const char* what) {
-  if (n > (int64_t)p->free_pages.size())
-    return fail(INFLLM_E_CAPACITY, "%s: %lld pages are needed, %zu of %d are free", what, (long long)n, p->free_pages.size(), p->cfg.n_pages);
+  if (n > p->free_pages.count())
+    return fail(INFLLM_E_CAPACITY, "%s: %lld pages are needed, %d of %d are free", what, (long long)n, p->free_pages.count(), p->cfg.n_pages);
   return INFLLM_OK;
 }
 
@@ -289,7 +286,7 @@ int batch_alive(const infllm_page_batch* b, const char* what) {
 
 // ------------------------------------------------------------------------------------------------------------ writes
 // New tokens' keys and values into their pages, keys and queries rotated to the tokens' positions on the way.  A block has
-// a token; a thread has 8 dimensions of the first half of a row and the 8 that go with them in the second, so that it needs
+// a token, or some where a token's rows are few; a thread has 8 dimensions of the first half of a row and the 8 that go with them in the second, so that it needs
 // one stretch of the tables for all its rows, and keeps it.  Bound by the bytes of q, k and v, read and written once: 8192 tokens
 // of 32 query and 8 KV heads (201 MB) in 40 us, 5.0 TB/s; with blocks of 256 threads 46, of 512 64, with three rows of a thread
 // in flight 79 (fewer loads at once for a token of 48 rows).
@@ -304,7 +301,7 @@ struct WriteParams {
   const int32_t* table;
   const float *cos_t, *sin_t;                       // null: nothing is rotated
   int64_t plane;                                    // bytes from keys to values
-  int32_t max_pages, page, n_kv, n_heads, most, b0, pad;
+  int32_t max_pages, page, n_kv, n_heads, most, b0, tokens, per_block;  // tokens of the launch, and of a block
   BatchSeq seq[kWriteSeqs];
 };
 
@@ -323,10 +320,13 @@ __device__ __forceinline__ void rotate8(uint4& lo, uint4& hi, const float* cs, c
 template <typename T, int kDim, bool kRope>
 __global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const __grid_constant__ WriteParams P) {
   constexpr int kPer = kDim / 16;  // threads of a row
-  const int i = blockIdx.x % P.most, b = blockIdx.x / P.most;
+  const int n_rows = P.n_heads + 2 * P.n_kv, per = min(n_rows * kPer, kWriteThreads);  // threads of a token
+  const int sub = (int)threadIdx.x / per, of_token = (int)threadIdx.x - sub * per, token = (int)blockIdx.x * P.per_block + sub;
+  if (sub >= P.per_block || token >= P.tokens) return;
+  const int b = token / P.most, i = token - b * P.most;
   const BatchSeq S = P.seq[b];
   const int at = i - (P.most - S.count);  // of the new tokens (the shorter sequences' stand at the end)
-  const int c = threadIdx.x % kPer, n_rows = P.n_heads + 2 * P.n_kv;
+  const int c = of_token % kPer;
   const int64_t bb = P.b0 + b;
   float cs[8], sn[8];
   if (kRope && at >= 0) {
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const __grid_
   const int place = S.length - S.count + at;
   char* const page_at = at >= 0 ? P.pages + ((int64_t)__ldg(P.table + (int64_t)S.row * P.max_pages + place / P.page) * P.n_kv * P.page + place % P.page) * kDim * 2
                                 : nullptr;
-  for (int r = threadIdx.x / kPer; r < n_rows; r += kWriteThreads / kPer) {
+  for (int r = of_token / kPer; r < n_rows; r += per / kPer) {
     const char* src;
     char* to;
     const bool is_q = r < P.n_heads, val = r >= P.n_heads + P.n_kv;
@@ -389,9 +389,7 @@ extern "C" int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages*
     int rc = guarded("pages_create", [&]() -> int {
       p->seqs.resize(c.max_sequences);
       p->uses.resize(c.n_pages, 0);
-      std::vector<int32_t> all(c.n_pages);
-      for (int32_t i = 0; i < c.n_pages; ++i) all[i] = i;
-      p->free_pages = decltype(p->free_pages)(std::greater<int32_t>(), std::move(all));
+      p->free_pages.fill(c.n_pages);
       DeviceScope scope(c.device);
       if (!scope.ok()) return fail(INFLLM_E_CUDA, "pages_create: no device %d", c.device);
       if (c.device < 0) return INFLLM_OK;
@@ -521,7 +519,7 @@ extern "C" int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n,
   return guarded("pages_compact", [&]() -> int {
     INFLLM_TRY(check_once(p, seqs, n, "pages_compact"));
     if (n > 0 && !n_spans) return fail(INFLLM_E_BADARG, "pages_compact: null pointer");
-    const int page = p->cfg.page_size;
+    const int page = p->cfg.page_size, shift = __builtin_ctz(page);
     struct Kept {
       int64_t length;
       int32_t stay;  // pages at the front of which every token stays where it is
@@ -556,13 +554,15 @@ extern "C" int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n,
         now.push_back(take_page(p));
         set_entry(p, seqs[i], now.size() - 1, now.back());
       }
-      int64_t to = 0;
+      int32_t to = 0;
       for (int k = 0; k < n_spans[i]; ++k, span += 2) {
-        int64_t from = span[0];
-        while (from < span[1]) {  // up to the end of a page on either side
-          const int64_t m = std::min({span[1] - from, page - from % page, page - to % page});
-          if (to / page >= stay)
-            move_tokens(p, s.pages[from / page], (int32_t)(from % page), now[to / page], (int32_t)(to % page), (int32_t)m);
+        int32_t from = (int32_t)span[0];
+        const int32_t stop = (int32_t)span[1];
+        // (what stays where it is: up to the end of the pages that are kept)
+        if (const int32_t skip = std::min(stop - from, (stay << shift) - to); skip > 0) from += skip, to += skip;
+        while (from < stop) {  // up to the end of a page on either side
+          const int32_t m = std::min({stop - from, page - (from & (page - 1)), page - (to & (page - 1))});
+          move_tokens(p, s.pages[from >> shift], from & (page - 1), now[to >> shift], to & (page - 1), m);
           from += m, to += m;
         }
       }
@@ -592,7 +592,7 @@ extern "C" int infllm_pages_row(const infllm_pages* p, int32_t seq, int32_t* out
   return INFLLM_OK;
 }
 
-extern "C" int infllm_pages_free_count(const infllm_pages* p) { return p ? (int)p->free_pages.size() : fail(INFLLM_E_BADARG, "pages_free_count: null pointer"); }
+extern "C" int infllm_pages_free_count(const infllm_pages* p) { return p ? p->free_pages.count() : fail(INFLLM_E_BADARG, "pages_free_count: null pointer"); }
 
 extern "C" int infllm_page_batch_create(infllm_pages* p, const int32_t* seqs, int n, infllm_page_batch** out) {
   return guarded("page_batch_create", [&]() -> int {
@@ -721,8 +721,10 @@ extern "C" int infllm_page_batch_write(infllm_page_batch* b, int layer, const vo
         const PageSeq& s = b->cache->seqs[b->seqs[e]];
         P.seq[i] = {b->seqs[e], (int32_t)s.length, b->count[e], (int32_t)(s.position - b->count[e])};
       }
-      const int64_t blocks = (int64_t)m * b->most;
-      if (blocks > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_write: %lld tokens", (long long)blocks);
+      if ((int64_t)m * b->most > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_write: %lld tokens", (long long)m * b->most);
+      P.tokens = m * b->most;
+      P.per_block = std::max(1, kWriteThreads / ((P.n_heads + 2 * P.n_kv) * (c.head_dim / 16)));
+      const int64_t blocks = ceil_div(P.tokens, P.per_block);
       INFLLM_DISPATCH_DTYPE(c.dtype, T, {
         auto kern = c.head_dim == 128 ? (d_cos ? page_write_kernel<T, 128, true> : page_write_kernel<T, 128, false>)
                                       : (d_cos ? page_write_kernel<T, 64, true> : page_write_kernel<T, 64, false>);

@@ -1,9 +1,7 @@
 // The paged cache's bookkeeping (pages.cu) and a batch's view of it, as the attention over its pages (paged_attn.cu) uses them.
 #pragma once
 #include <exception>
-#include <functional>
 #include <new>
-#include <queue>
 #include <vector>
 
 #include "tc_common.cuh"
@@ -15,6 +13,35 @@ struct PageSeq {
   uint32_t generation = 0;  // counts the sequences that had this number
   int64_t length = 0, position = 0;
   std::vector<int32_t> pages;
+};
+
+// The pages that no sequence has: a bit each, taken lowest first.  No page below word `first_` is free.
+class FreePages {
+ public:
+  void fill(int32_t n) {
+    words_.assign((size_t)(n + 63) / 64, ~0ull);
+    if (n % 64) words_.back() = (1ull << (n % 64)) - 1;
+    first_ = 0, count_ = n;
+  }
+  int32_t count() const { return count_; }
+  int32_t take() {  // (of some)
+    while (!words_[first_]) ++first_;
+    const int bit = __builtin_ctzll(words_[first_]);
+    words_[first_] &= words_[first_] - 1;
+    --count_;
+    return (int32_t)(first_ * 64) + bit;
+  }
+  void give(int32_t page) {
+    const size_t at = (size_t)page / 64;
+    words_[at] |= 1ull << (page % 64);
+    if (at < first_) first_ = at;
+    ++count_;
+  }
+
+ private:
+  std::vector<uint64_t> words_;
+  size_t first_ = 0;
+  int32_t count_ = 0;
 };
 
 // One launch's worth of changes: rows of the table that are copied, entries that are set, tokens that are moved.
@@ -65,7 +92,7 @@ struct infllm_pages {
   infllm_pages_config cfg;
   std::vector<infllm::PageSeq> seqs;
   std::vector<int32_t> uses;  // sequences that have a page
-  std::priority_queue<int32_t, std::vector<int32_t>, std::greater<int32_t>> free_pages;
+  infllm::FreePages free_pages;
   uint64_t change = 0;   // any change of what sequences hold
   uint64_t reshape = 0;  // of the pages that a sequence had before
   std::vector<infllm::PageItem> rows, edits, moves;  // of the call that is being made (pages.cu)
