@@ -569,7 +569,7 @@ int infllm_pages_info(const infllm_pages* p, int32_t seq, int64_t* length, int64
 int infllm_pages_row(const infllm_pages* p, int32_t seq, int32_t* out, int cap, int* n); /* its pages */
 int infllm_pages_free_count(const infllm_pages* p); /* free pages */
 
-/* A batch: sequences, and of each a count of newest tokens that the calls are about.  The tensors of a call have as many
+/* A batch (destroyed before its cache): sequences, and of each a count of newest tokens that the calls are about.  The tensors of a call have as many
  * tokens as the largest count; a sequence with fewer has its own at the end, the rows before them are not read, or written
  * as zeros.
  *   extend    room for counts[i] more tokens, which become the newest
@@ -580,7 +580,8 @@ int infllm_pages_free_count(const infllm_pages* p); /* free pages */
  *             head_dim); with d_cos / d_sin (table_len, head_dim / 2) keys and queries rotated to the tokens' positions.
  *             q may be NULL.
  *   attend    attention of the newest tokens: each sees its sequence's tokens up to itself.  d_out (batch, tokens, n_heads,
- *             head_dim), d_lse (batch, tokens, n_heads) fp32 log-sum-exp of the scores (natural logarithm), or NULL.
+ *             head_dim), d_lse (batch, tokens, n_heads) fp32 log-sum-exp of the scores (natural logarithm), or NULL; scale is
+ *             not negative.
  *             d_work is the caller's, 16-byte aligned, of the size that infllm_page_batch_plan gives.  That call works out
  *             the plan, which holds for all layers until a sequence of the cache changes: attend returns
  *             INFLLM_PAGES_NO_PLAN where there is none for n_heads.  The first attend call after it uploads the plan to

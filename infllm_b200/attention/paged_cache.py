@@ -241,7 +241,7 @@ class PagedBatch:
 
     def attend(self, layer, q, scale=None, return_lse=False):
         """Attention of the step's queries (batch, n_heads, tokens, head_dim) to their sequences' keys up to their own places.
-        `scale` of the scores: 1 / sqrt(head_dim) if not given.  Returns (batch, n_heads, tokens, head_dim), a view of
+        `scale` of the scores, not negative: 1 / sqrt(head_dim) if not given.  Returns (batch, n_heads, tokens, head_dim), a view of
         (batch, tokens, n_heads, head_dim); with return_lse also the scores' log-sum-exps (batch, n_heads, tokens), fp32."""
         c = self.cache
         heads = q.size(1)

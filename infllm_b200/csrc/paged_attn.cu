@@ -536,6 +536,8 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     const infllm_pages_config& c = p->cfg;
     if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_attend: a cache without a device");
     if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_attend: layer %d of %d", layer, c.n_layers);
+    // (maxima are taken of the scores before they are scaled)
+    if (!(scale >= 0.f) || scale > 3e38f) return fail(INFLLM_E_BADARG, "page_batch_attend: a scale of %g", (double)scale);
     if (b->plan_of != p->change || b->plan_heads != n_heads) return INFLLM_PAGES_NO_PLAN;
     if (b->most == 0) return INFLLM_OK;
     if (!d_q || !d_out || !d_work) return fail(INFLLM_E_BADARG, "page_batch_attend: null pointer");

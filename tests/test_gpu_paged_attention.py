@@ -314,6 +314,7 @@ def test_refusals():
     q = torch.zeros((2, 4, 20, 64), dtype=torch.bfloat16, device="cuda")
     for call, error in ((lambda: b.write(1, k, k), L.InfLLMError), (lambda: b.attend(-1, q), L.InfLLMError), (lambda: b.attend(0, q[:, :3]), L.InfLLMError),
                         (lambda: b.attend(0, q[:, :, :3]), ValueError), (lambda: b.attend(0, q.half()), TypeError), (lambda: b.attend(0, q.cpu()), RuntimeError),
+                        (lambda: b.attend(0, q, scale=-1.0), L.InfLLMError), (lambda: b.attend(0, q, scale=NAN), L.InfLLMError),
                         (lambda: b.write(0, k, k[..., :32]), ValueError), (lambda: b.write(0, k, k, q, RotaryEmbeddingESM(128)), ValueError),
                         (lambda: c.batch([s[0], s[0]]), L.InfLLMError), (lambda: c.batch([]), L.InfLLMError), (lambda: b.plan([30, 1]), L.InfLLMError),
                         (lambda: b.plan([1]), ValueError), (lambda: b.retract([21, 0]), L.InfLLMError), (lambda: c.truncate(s, [1]), ValueError),
@@ -397,3 +398,34 @@ def test_what_is_no_number_stays_in_its_row(n_seqs, n, prefix, what):
     bad[2, 4:] = True  # the KV head's query heads
     assert torch.equal(got[~bad], fine[~bad])
     assert (torch.isnan(got[bad]).any() if what == math.inf else torch.isnan(got[bad]).all())
+
+
+def test_pages_far_into_a_large_pool():
+    """Offsets past 32 bits, in bytes and in elements: the last pages of 9 GB, of the second of two layers."""
+    n_pages = 9000
+    x = Kept(make(n_pages, 128, 8, 128, layers=2, max_tokens=n_pages * 128), 13)
+    c = x.c
+    filler = c.open()
+    c.batch(filler).extend((n_pages - 100) * 128)
+    root = x.open()
+    x.grow([root], [4000])
+    seqs = x.fork(root, 12)
+    b = x.grow(seqs, [1] * 12)
+    assert min(c.page_ids(seqs[0])) >= n_pages - 100
+    x.check(b, [1] * 12, 32)
+    b = x.c.batch(seqs[:2])
+    b.extend(40)
+    k, v, q = (rand(x.g, 2, h, 40, 128) for h in (8, 8, 32))
+    b.write(0, k, v)
+    b.write(1, k, v)
+    at = torch.tensor(c.page_ids(root), device="cuda")
+    c.pages[1, :, at] = c.pages[0, :, at]  # (the forks' shared and own pages, in the other layer too)
+    for s in seqs[:2]:
+        own = torch.tensor(c.page_ids(s)[31:], device="cuda")
+        c.pages[1, :, own] = c.pages[0, :, own]
+    assert torch.equal(b.attend(0, q), b.attend(1, q))
+    small = c.copy(seqs[:1])
+    ids = [torch.tensor(c.page_ids(s), device="cuda") for s in (seqs[0], small[0])]
+    n = c.length(seqs[0])
+    one, other = (c.pages[:, :, i].movedim(3, 2).reshape(2, 2, 8, -1, 128)[:, :, :, :n] for i in ids)
+    assert torch.equal(one, other)
