@@ -224,12 +224,14 @@ static void open_seq(infllm_pages* p, int32_t seq) {
   s.length = s.position = 0;
 }
 
+// (what sequences share is another thing only where a shared page goes)
 static void cut(infllm_pages* p, int32_t seq, int64_t length) {
   PageSeq& s = p->seqs[seq];
   s.position -= s.length - length;
   s.length = length;
   const size_t left = (size_t)p->pages_of(length);
   while (s.pages.size() > left) {
+    p->reshape += p->uses[s.pages.back()] > 1;
     drop_page(p, s.pages.back());
     s.pages.pop_back();
   }
@@ -497,7 +499,7 @@ extern "C" int infllm_pages_truncate(infllm_pages* p, const int32_t* seqs, const
       if (lengths[i] < 0 || lengths[i] > p->seqs[seqs[i]].length)
         return fail(INFLLM_E_BADARG, "pages_truncate: %lld of the %lld tokens of sequence %d", (long long)lengths[i],
                     (long long)p->seqs[seqs[i]].length, seqs[i]);
-    ++p->change, ++p->reshape;
+    ++p->change;
     for (int i = 0; i < n; ++i) cut(p, seqs[i], lengths[i]);
     return INFLLM_OK;
   });
@@ -506,7 +508,7 @@ extern "C" int infllm_pages_truncate(infllm_pages* p, const int32_t* seqs, const
 extern "C" int infllm_pages_free(infllm_pages* p, const int32_t* seqs, int n) {
   return guarded("pages_free", [&]() -> int {
     INFLLM_TRY(check_once(p, seqs, n, "pages_free"));
-    ++p->change, ++p->reshape;
+    ++p->change;
     for (int i = 0; i < n; ++i) {
       cut(p, seqs[i], 0);
       p->seqs[seqs[i]].open = false;
@@ -662,7 +664,7 @@ extern "C" int infllm_page_batch_retract(infllm_page_batch* b, const int32_t* co
     INFLLM_TRY(batch_alive(b, "page_batch_retract"));
     INFLLM_TRY(check_counts(b, counts, same, "page_batch_retract"));
     infllm_pages* p = b->cache;
-    ++p->change, ++p->reshape;
+    ++p->change;
     for (size_t i = 0; i < b->seqs.size(); ++i) cut(p, b->seqs[i], p->seqs[b->seqs[i]].length - (counts ? counts[i] : same));
     set_counts(b, nullptr, 0);
     return INFLLM_OK;

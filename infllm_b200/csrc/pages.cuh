@@ -94,7 +94,7 @@ struct infllm_pages {
   std::vector<int32_t> uses;  // sequences that have a page
   infllm::FreePages free_pages;
   uint64_t change = 0;   // any change of what sequences hold
-  uint64_t reshape = 0;  // of the pages that a sequence had before
+  uint64_t reshape = 0;  // of which pages sequences share, but for forks
   std::vector<infllm::PageItem> rows, edits, moves;  // of the call that is being made (pages.cu)
   std::vector<int32_t> to_pages;
   CUtensorMap map;       // of all pages (paged_tc.cu)

@@ -258,3 +258,50 @@ def test_refusals():
             setattr(cfg, k, v)
         assert L.lib.infllm_pages_create(ctypes.byref(cfg), ctypes.byref(out)) in (L.E_BADARG, L.E_UNSUPPORTED)
     assert L.lib.infllm_pages_create(None, None) == L.E_BADARG
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_plan_of_a_batch_that_has_lived(seed):
+    """What a batch keeps of its sequences' order is made anew where what they share has changed: its plan has the size of a new batch's."""
+    r = random.Random(seed)
+    c = Cache(n_pages=4000, max_sequences=100, max_pages=300)
+
+    def batch(seqs):
+        b = ctypes.c_void_p()
+        L.check(L.lib.infllm_page_batch_create(c.h, c.ids(seqs), len(seqs), ctypes.byref(b)))
+        return b
+
+    def plan(b, new):
+        if L.lib.infllm_page_batch_select(b, None, new, None) != 0:  # (one of them has fewer)
+            L.check(L.lib.infllm_page_batch_select(b, None, 0, None))
+        size = c_int64()
+        L.check(L.lib.infllm_page_batch_plan(b, 8, ctypes.byref(size)))
+        return size.value
+
+    seqs = c.open(r.randint(1, 2))
+    for _ in range(3):
+        b = batch(seqs)
+        L.check(L.lib.infllm_page_batch_extend(b, None, r.choice([5, 16, 100, 800]), None, None))
+        L.lib.infllm_page_batch_destroy(b)
+        seqs += c.fork([r.choice(seqs)], r.randint(1, 10))
+    b = batch(seqs)
+    for _ in range(20):
+        what = r.randrange(4)
+        if what == 0:
+            L.check(L.lib.infllm_page_batch_extend(b, c.ids([r.choice([0, 1, 3, 16, 40]) for _ in seqs]), 0, None, None))
+        elif what == 1:
+            n = r.choice([1, 16, 33])
+            L.check(L.lib.infllm_page_batch_extend(b, None, n, None, None))
+            plan(b, 1)
+            L.check(L.lib.infllm_page_batch_select(b, None, n, None))
+            L.check(L.lib.infllm_page_batch_retract(b, None, r.randint(0, n)))
+        elif what == 2:
+            for q in r.sample(seqs, r.randint(1, len(seqs))):
+                L.lib.infllm_pages_truncate(c.h, c.ids([q]), (c_int64 * 1)(r.choice([0, 16, 17, 100, 160, 800])), 1)  # (or refused)
+        else:
+            L.check(L.lib.infllm_pages_free(c.h, c.ids(c.fork([r.choice(seqs)], 1)), 1))
+        new = r.choice([1, 4])
+        fresh = batch(seqs)
+        assert plan(b, new) == plan(fresh, new)
+        L.lib.infllm_page_batch_destroy(fresh)
+    L.lib.infllm_page_batch_destroy(b)
