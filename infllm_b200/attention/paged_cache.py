@@ -149,6 +149,7 @@ class PagedBatch:
         self._n = len(self.seqs)
         self.tokens = 0  # of the step's tensors
         self._work, self._work_at = None, 0  # the plan on the device, and room for partial results
+        self._work_stream = None  # that its memory is of
         self._reach = c_int64()  # rows that a rotary table has to have
         self._reach_ref = ctypes.byref(self._reach)
         self._scale = 1.0 / math.sqrt(cache.head_dim)
@@ -242,7 +243,8 @@ class PagedBatch:
     def attend(self, layer, q, scale=None, return_lse=False):
         """Attention of the step's queries (batch, n_heads, tokens, head_dim) to their sequences' keys up to their own places.
         `scale` of the scores, not negative: 1 / sqrt(head_dim) if not given.  Returns (batch, n_heads, tokens, head_dim), a view of
-        (batch, tokens, n_heads, head_dim); with return_lse also the scores' log-sum-exps (batch, n_heads, tokens), fp32."""
+        (batch, tokens, n_heads, head_dim); with return_lse also the scores' log-sum-exps (batch, n_heads, tokens), fp32.  A batch's
+        calls share a workspace: on several streams, one waits for the other as for any tensor that both use."""
         c = self.cache
         heads = q.size(1)
         q, at, bs, hs, ts = self._rows(q, heads, "q")
@@ -259,9 +261,11 @@ class PagedBatch:
             _lib.check(_lib_call.infllm_page_batch_plan(self.handle, heads, ctypes.byref(size)))
             # (memory of its own: the last plan may still be in use)
             self._work = torch.empty(max(size.value, 16), dtype=torch.uint8, device=c.device)
-            self._work_at = self._work.data_ptr()
+            self._work_at, self._work_stream = self._work.data_ptr(), stream
             rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at,
                                                     stream)
+        elif stream != self._work_stream and self._work is not None:  # it is not to be given away before this stream is done with it
+            self._work.record_stream(torch.cuda.current_stream(c.device))
         if rc:
             _lib.check(rc)
         return (out, lse.permute(0, 2, 1)) if return_lse else out

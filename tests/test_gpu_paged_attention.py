@@ -429,3 +429,25 @@ def test_pages_far_into_a_large_pool():
     n = c.length(seqs[0])
     one, other = (c.pages[:, :, i].movedim(3, 2).reshape(2, 2, 8, -1, 128)[:, :, :, :n] for i in ids)
     assert torch.equal(one, other)
+
+
+def test_batch_goes_while_another_stream_reads_its_plan():
+    """The plan is made on one stream and read on another, which is held up meanwhile: its memory is not given away before."""
+    kept = Kept(make(200, 16, 2, 64), 77)
+    seqs = [kept.open()]
+    kept.grow(seqs, [700])
+    seqs += kept.fork(seqs[0], 5)
+    kept.grow(seqs, [3, 20, 1, 40, 9, 17])
+    b = kept.c.batch(seqs)
+    b.plan(1)
+    q = rand(kept.g, len(seqs), 8, 1, 64)
+    want = b.attend(0, q)
+    torch.cuda.synchronize()
+    stream, size = torch.cuda.Stream(), b._work.numel()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(100_000_000)  # (some 50 ms)
+        got = b.attend(0, q)
+    del b
+    filled = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all(not x.any() for x in filled)
