@@ -578,7 +578,7 @@ int infllm_pages_free_count(const infllm_pages* p); /* free pages */
  *             (counts NULL: `same` for every sequence; *reach, if given: the rows that a rotary table has to have)
  *   write     a layer's keys and values of the newest tokens into their pages, and q to d_q_out (batch, tokens, n_heads,
  *             head_dim); with d_cos / d_sin (table_len, head_dim / 2) keys and queries rotated to the tokens' positions.
- *             q may be NULL.
+ *             q may be NULL.  Refused where a sequence was cut, compacted or extended by another call since extend or select.
  *   attend    attention of the newest tokens: each sees its sequence's tokens up to itself.  d_out (batch, tokens, n_heads,
  *             head_dim), d_lse (batch, tokens, n_heads) fp32 log-sum-exp of the scores (natural logarithm), or NULL; scale is
  *             not negative.

@@ -218,7 +218,8 @@ class PagedBatch:
 
     def write(self, layer, k, v, q=None, rope=None):
         """The step's keys and values (batch, n_kv_heads, tokens, head_dim) into a layer's pages.  With `rope`, a
-        RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q)."""
+        RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q).  Refused where one
+        of the sequences was cut, compacted or extended by another call since the step began."""
         c = self.cache
         k, k_at, k_bs, k_hs, k_ts = self._rows(k, c.n_kv_heads, "k")
         v, v_at, v_bs, v_hs, v_ts = self._rows(v, c.n_kv_heads, "v")

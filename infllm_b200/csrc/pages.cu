@@ -227,6 +227,7 @@ static void open_seq(infllm_pages* p, int32_t seq) {
 // (what sequences share is another thing only where a shared page goes)
 static void cut(infllm_pages* p, int32_t seq, int64_t length) {
   PageSeq& s = p->seqs[seq];
+  s.changes += s.length != length;
   s.position -= s.length - length;
   s.length = length;
   const size_t left = (size_t)p->pages_of(length);
@@ -266,6 +267,7 @@ static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* counts, i
       drop_page(p, old);  // (another one has it still)
       ++p->reshape;
     }
+    s.changes += more > 0;
     s.length += more;
     s.position += more;
     const size_t want = (size_t)p->pages_of(s.length);
@@ -570,6 +572,7 @@ extern "C" int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n,
       }
       gone.insert(gone.end(), s.pages.begin() + stay, s.pages.end());
       s.pages = std::move(now);
+      s.changes += s.length != kept[i].length;
       s.length = kept[i].length;
     }
     // (only now: what one sequence leaves must not be taken by the next while it is still to be read)
@@ -606,7 +609,10 @@ extern "C" int infllm_page_batch_create(infllm_pages* p, const int32_t* seqs, in
       b->cache = p;
       b->seqs.assign(seqs, seqs + n);
       b->count.assign(n, 0);
-      for (int i = 0; i < n; ++i) b->generation.push_back(p->seqs[seqs[i]].generation);
+      for (int i = 0; i < n; ++i) {
+        b->generation.push_back(p->seqs[seqs[i]].generation);
+        b->as_of.push_back(p->seqs[seqs[i]].changes);
+      }
       return INFLLM_OK;
     });
     if (rc != INFLLM_OK) {
@@ -627,6 +633,7 @@ static void set_counts(infllm_page_batch* b, const int32_t* counts, int32_t same
   b->most = 0;
   for (size_t i = 0; i < b->seqs.size(); ++i) {
     b->count[i] = counts ? counts[i] : same;
+    b->as_of[i] = b->cache->seqs[b->seqs[i]].changes;
     b->most = std::max(b->most, b->count[i]);
   }
   b->plan_of = ~0ull;
@@ -687,6 +694,10 @@ extern "C" int infllm_page_batch_write(infllm_page_batch* b, int layer, const vo
                                        int64_t table_len, void* stream) {
   return guarded("page_batch_write", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_write"));
+    // (the tokens that the step is about may be gone, and the newest ones others; from here on no sequence is shorter than its count)
+    for (size_t i = 0; i < b->seqs.size(); ++i)
+      if (b->count[i] > 0 && b->cache->seqs[b->seqs[i]].changes != b->as_of[i])
+        return fail(INFLLM_E_BADARG, "page_batch_write: sequence %d has been cut or extended since the step began", b->seqs[i]);
     const infllm_pages_config& c = b->cache->cfg;
     if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_write: a cache without a device");
     if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_write: layer %d of %d", layer, c.n_layers);

@@ -11,6 +11,7 @@ namespace infllm {
 struct PageSeq {
   bool open = false;
   uint32_t generation = 0;  // counts the sequences that had this number
+  uint64_t changes = 0;     // of its tokens: some added, or taken away
   int64_t length = 0, position = 0;
   std::vector<int32_t> pages;
 };
@@ -108,6 +109,7 @@ struct infllm_page_batch {
   std::vector<int32_t> seqs;
   std::vector<uint32_t> generation;
   std::vector<int32_t> count;  // newest tokens of each sequence that calls are about
+  std::vector<uint64_t> as_of;  // each sequence's `changes` when they were set
   int32_t most = 0;            // the largest of them: the tokens of a call's tensors
   // the order of the sequences by their pages, and how many pages each shares with the one before: as of `reshape`
   uint64_t order_of = ~0ull;

@@ -451,3 +451,34 @@ def test_batch_goes_while_another_stream_reads_its_plan():
     filled = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(8)]
     torch.cuda.synchronize()
     assert torch.equal(got, want) and all(not x.any() for x in filled)
+
+
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("what", ["truncate", "compact", "retract"])
+def test_a_write_after_a_cut_touches_nothing(page, what):
+    """The step's tokens are gone, and their places in front of the sequence's pages another's: the write is refused."""
+    from infllm_b200 import _lib as L
+    from infllm_b200.attention import RotaryEmbeddingESM
+
+    c = make(12, page, 2, 64)
+    s = c.open(2)
+    c.batch(s[:1]).extend(page)
+    b = c.batch(s)
+    b.extend([1, 40])
+    k = torch.zeros((2, 2, 40, 64), dtype=torch.bfloat16, device="cuda")
+    if what == "truncate":
+        c.truncate(s[1:], [2])
+    elif what == "compact":
+        c.compact(s[1:], [[(3, 5)]])
+    else:
+        other = c.batch(s[1:])
+        other.plan(1)
+        other.retract(39)
+    for rope in (None, RotaryEmbeddingESM(64, 1e4, 1.0)):
+        with pytest.raises(L.InfLLMError, match="since the step began"):
+            b.write(0, k, k, None, rope)
+    torch.cuda.synchronize()
+    assert torch.isnan(c.pages).sum() == c.pages.numel()
+    b.extend(2)
+    b.write(0, k[:, :, :2], k[:, :, :2])
+    assert (~torch.isnan(c.pages)).sum() == 2 * 2 * 2 * 2 * 64

@@ -305,3 +305,51 @@ def test_plan_of_a_batch_that_has_lived(seed):
         assert plan(b, new) == plan(fresh, new)
         L.lib.infllm_page_batch_destroy(fresh)
     L.lib.infllm_page_batch_destroy(b)
+
+
+@pytest.mark.parametrize("what", ["truncate", "truncate a little", "compact", "retract of another batch", "extend of another batch", "free pages"])
+def test_write_is_refused_where_the_step_is_another(what):
+    """A step's counts are of the sequences as they were when it began.  A sequence that was cut since would be written in front of its
+    pages, one that was cut by less, or has grown, where other tokens are."""
+    c = Cache()
+    s, t = c.open(2)
+    b, other = ctypes.c_void_p(), ctypes.c_void_p()
+    L.check(L.lib.infllm_page_batch_create(c.h, c.ids([s, t]), 2, ctypes.byref(b)))
+    L.check(L.lib.infllm_page_batch_create(c.h, c.ids([t]), 1, ctypes.byref(other)))
+
+    def write():
+        rc = L.lib.infllm_page_batch_write(b, 0, None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, 0, None, 0, None, None, 0, None)
+        assert rc == L.E_BADARG  # (at the latest because there is no device)
+        return L.lib.infllm_last_error().decode()
+
+    L.check(L.lib.infllm_page_batch_extend(b, c.ids([3, 40]), 0, None, None))
+    assert "without a device" in write()
+    if what == "truncate":
+        c.truncate([t], [2])
+    elif what == "truncate a little":
+        c.truncate([t], [39])
+    elif what == "compact":
+        c.compact([t], [[(0, 1), (7, 9)]])
+    elif what == "retract of another batch":
+        L.check(L.lib.infllm_page_batch_select(other, None, 0, None))
+        L.check(L.lib.infllm_page_batch_retract(other, None, 40))
+    elif what == "extend of another batch":
+        L.check(L.lib.infllm_page_batch_extend(other, None, 1, None, None))
+    else:  # (what changes no token of theirs is no reason to refuse)
+        c.truncate([s, t], [3, 40])
+        c.compact([t], [[(0, 40)]])
+        L.check(L.lib.infllm_page_batch_extend(other, None, 0, None, None))
+        c.free(c.fork([s], 2))
+    got = write()
+    if what == "free pages":
+        assert "without a device" in got
+    else:
+        assert f"sequence {t}" in got and "step" in got
+        # a step that is about fewer sequences, or a new one, is not refused for it
+        L.check(L.lib.infllm_page_batch_select(b, c.ids([3, 0]), 0, None))
+        L.check(L.lib.infllm_page_batch_extend(other, None, 1, None, None))
+        assert "without a device" in write()
+        L.check(L.lib.infllm_page_batch_extend(b, None, 2, None, None))
+        assert "without a device" in write()
+    for x in (b, other):
+        L.lib.infllm_page_batch_destroy(x)
