@@ -256,11 +256,15 @@ class PagedBatch:
             lse_at = lse.data_ptr()
         scale = self._scale if scale is None else scale
         stream = _lib.raw_stream(c.device)
-        rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at, stream)
+        rc = _lib.PAGES_NO_PLAN
+        if self._work_at:
+            rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at,
+                                                    stream)
         if rc == _lib.PAGES_NO_PLAN:  # the first layer of a step
             size = c_int64()
+            # a plan goes with the memory that was made for it, or with none: the last one's may be too small for it
+            self._work, self._work_at = None, 0
             _lib.check(_lib_call.infllm_page_batch_plan(self.handle, heads, ctypes.byref(size)))
-            # (memory of its own: the last plan may still be in use)
             self._work = torch.empty(max(size.value, 16), dtype=torch.uint8, device=c.device)
             self._work_at, self._work_stream = self._work.data_ptr(), stream
             rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at,

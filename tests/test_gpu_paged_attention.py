@@ -482,3 +482,29 @@ def test_a_write_after_a_cut_touches_nothing(page, what):
     b.extend(2)
     b.write(0, k[:, :, :2], k[:, :, :2])
     assert (~torch.isnan(c.pages)).sum() == 2 * 2 * 2 * 2 * 64
+
+
+def test_attend_again_after_its_workspace_found_no_memory(monkeypatch):
+    """The next call plans anew, with memory of the size that the longer sequences need."""
+    x = Kept(make(300, 16, 2, 128), 21)
+    root = x.open()
+    x.grow([root], [40])
+    b = x.grow([root], [1])
+    x.check(b, [1], 8)
+    x.grow([root], [3000])
+    b.plan(200)
+    q = rand(x.g, 1, 8, 200, 128)
+    empty, small = torch.empty, b._work.numel()
+
+    def none(*a, **k):
+        if k.get("dtype") is torch.uint8:
+            raise torch.cuda.OutOfMemoryError("no memory")
+        return empty(*a, **k)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", none)
+        for _ in range(2):
+            with pytest.raises(torch.cuda.OutOfMemoryError):
+                b.attend(0, q)
+    x.check(b, [200], 8)
+    assert b._work.numel() > small

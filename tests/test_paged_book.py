@@ -353,3 +353,65 @@ def test_write_is_refused_where_the_step_is_another(what):
         assert "without a device" in write()
     for x in (b, other):
         L.lib.infllm_page_batch_destroy(x)
+
+
+def test_a_plan_that_found_no_memory_is_not_used_with_the_last_ones(monkeypatch):
+    """Where the workspace of a new plan cannot be had, the call fails, and the next one asks for it again: it is never made in the
+    last plan's memory, which may be too small.  (The library is stood in for by the rules of its attend and plan calls.)"""
+    import types
+
+    import torch
+
+    from infllm_b200.attention import paged_cache as M
+
+    class Library:
+        planned, need, seen = False, 1 << 12, []
+
+        def infllm_page_batch_create(self, *a):
+            return 0
+
+        infllm_page_batch_destroy = infllm_page_batch_extend = infllm_page_batch_create
+
+        def infllm_page_batch_plan(self, handle, heads, size):
+            size._obj.value, self.planned = self.need, True
+            return 0
+
+        def infllm_page_batch_attend(self, handle, layer, q, bs, hs, ts, out, lse, heads, scale, work, stream):
+            if not self.planned:
+                return L.PAGES_NO_PLAN
+            self.seen.append(work)
+            return 0 if work else L.E_BADARG
+
+    lib = Library()
+    monkeypatch.setattr(M, "_lib_call", lib)
+    monkeypatch.setattr(M._lib, "raw_stream", lambda device: 0)
+    cache = types.SimpleNamespace(handle=None, head_dim=64, dtype=torch.bfloat16, device=torch.device("cpu"), n_kv_heads=1)
+    empty, sizes, short = torch.empty, {}, [False]
+
+    def take(size, *a, **k):
+        if k.get("dtype") is not torch.uint8:
+            return empty(size, *a, **k)
+        if short[0]:
+            raise torch.cuda.OutOfMemoryError("no memory")
+        t = empty(size, *a, **k)
+        sizes[t.data_ptr()] = t.numel()
+        return t
+
+    monkeypatch.setattr(torch, "empty", take)
+    q = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16)
+    for before in (False, True):  # the batch's first plan, or a later one
+        b = M.PagedBatch(cache, [0])
+        b.extend(1)
+        lib.planned, lib.need = False, 1 << 12
+        if before:
+            b.attend(0, q)
+        lib.planned, lib.need, short[0] = False, 1 << 16, True
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            b.attend(0, q)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            b.attend(0, q)
+        short[0] = False
+        lib.seen.clear()
+        b.attend(0, q)
+        b.attend(1, q)
+        assert len(lib.seen) == 2 and all(sizes[w] >= 1 << 16 for w in lib.seen)
