@@ -581,7 +581,7 @@ int infllm_pages_free_count(const infllm_pages* p); /* free pages */
  *             q may be NULL.  Refused where a sequence was cut, compacted or extended by another call since extend or select.
  *   attend    attention of the newest tokens: each sees its sequence's tokens up to itself.  d_out (batch, tokens, n_heads,
  *             head_dim), d_lse (batch, tokens, n_heads) fp32 log-sum-exp of the scores (natural logarithm), or NULL; scale is
- *             not negative.
+ *             not negative, and scale * log2(e) a number in 32 bits.
  *             d_work is the caller's, 16-byte aligned, of the size that infllm_page_batch_plan gives.  That call works out
  *             the plan, which holds for all layers until a sequence of the cache changes: attend returns
  *             INFLLM_PAGES_NO_PLAN where there is none for n_heads.  The first attend call after it uploads the plan to

@@ -11,6 +11,7 @@
 //
 // The host knows the tree and all lengths: it cuts every node's rows into tiles and its keys into units of about equal work.
 #include <algorithm>
+#include <cfloat>
 #include <cstring>
 
 #include "attn_tc.cuh"
@@ -537,7 +538,7 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_attend: a cache without a device");
     if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_attend: layer %d of %d", layer, c.n_layers);
     // (maxima are taken of the scores before they are scaled)
-    if (!(scale >= 0.f) || scale > 3e38f) return fail(INFLLM_E_BADARG, "page_batch_attend: a scale of %g", (double)scale);
+    if (!(scale >= 0.f) || !(scale * kLog2e <= FLT_MAX)) return fail(INFLLM_E_BADARG, "page_batch_attend: a scale of %g", (double)scale);
     if (b->plan_of != p->change || b->plan_heads != n_heads) return INFLLM_PAGES_NO_PLAN;
     if (b->most == 0) return INFLLM_OK;
     if (!d_q || !d_out || !d_work) return fail(INFLLM_E_BADARG, "page_batch_attend: null pointer");
@@ -568,7 +569,9 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     P.batch = (int)b->seqs.size();
     P.n_beside = b->n_beside * c.n_kv_heads;
     P.next = (int32_t*)d_work;
-    P.scale_log2 = scale * kLog2e;
+    // (the tensor-core kernel masks scores before they are scaled: -inf times 0 is no number.  By the least normal number instead, scores
+    // of less than 2^100 are zeros beside any reference)
+    P.scale_log2 = std::max(scale * kLog2e, FLT_MIN);
     if (b->n_ctas > 0) INFLLM_TRY(paged_tc_launch(P, c.dtype, c.head_dim, b->n_ctas, s));
     INFLLM_DISPATCH_DTYPE(c.dtype, T, {
       if (b->n_row_units > 0) {

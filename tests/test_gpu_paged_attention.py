@@ -508,3 +508,33 @@ def test_attend_again_after_its_workspace_found_no_memory(monkeypatch):
                 b.attend(0, q)
     x.check(b, [200], 8)
     assert b._work.numel() > small
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-50, 1e-42, 1e-30])
+@pytest.mark.parametrize("prefix,counts", [(9000, (1,) * 40), (9001, (17, 0, 40, 33)), (0, (2000,)), (300, (1, 1)), (5000, (700, 3))])
+def test_scales_of_nearly_nothing(scale, prefix, counts):
+    """Every key that a row sees has the same share: the mean of the values, by the kernel of few rows and by the tensor cores' one."""
+    x = Kept(make((prefix + 40 * 60 + 2000) // 16, 16, 2, 128, max_tokens=32768), prefix)
+    root = x.open()
+    if prefix:
+        x.grow([root], [prefix])
+    seqs = x.fork(root, len(counts))
+    b = x.grow(seqs, list(counts))
+    x.check(b, list(counts), 8, scale=scale)
+
+
+def test_scales_that_are_none_to_base_2():
+    """Scores are scaled by scale * log2(e): where that is no number in 32 bits, neither is what would come out."""
+    from infllm_b200 import _lib as L
+
+    c = make(300, 16, 2, 128)
+    s = c.open()
+    b = c.batch(s)
+    b.extend(4)
+    k = torch.zeros((1, 2, 4, 128), dtype=torch.bfloat16, device="cuda")
+    b.write(0, k, k)
+    q = torch.zeros((1, 8, 4, 128), dtype=torch.bfloat16, device="cuda")
+    for scale in (2.4e38, 3e38, 1e39, math.inf):
+        with pytest.raises(L.InfLLMError):
+            b.attend(0, q, scale=scale)
+    assert (b.attend(0, q, scale=2.3e38) == 0).all()
