@@ -585,7 +585,8 @@ int infllm_pages_free_count(const infllm_pages* p); /* free pages */
  *             d_work is the caller's, 16-byte aligned, of the size that infllm_page_batch_plan gives.  That call works out
  *             the plan, which holds for all layers until a sequence of the cache changes: attend returns
  *             INFLLM_PAGES_NO_PLAN where there is none for n_heads.  The first attend call after it uploads the plan to
- *             d_work, which the later ones have to be given too. */
+ *             d_work, which the later ones have to be given too; it is refused on a stream that captures a graph.  Later calls may be
+ *             captured: a replay is good for as long as that plan holds and d_work is there. */
 #define INFLLM_PAGES_NO_PLAN 1
 int infllm_page_batch_create(infllm_pages* p, const int32_t* seqs, int n, infllm_page_batch** out);
 int infllm_page_batch_destroy(infllm_page_batch* b);

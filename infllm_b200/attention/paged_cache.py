@@ -245,7 +245,8 @@ class PagedBatch:
         """Attention of the step's queries (batch, n_heads, tokens, head_dim) to their sequences' keys up to their own places.
         `scale` of the scores, not negative: 1 / sqrt(head_dim) if not given.  Returns (batch, n_heads, tokens, head_dim), a view of
         (batch, tokens, n_heads, head_dim); with return_lse also the scores' log-sum-exps (batch, n_heads, tokens), fp32.  A batch's
-        calls share a workspace: on several streams, one waits for the other as for any tensor that both use."""
+        calls share a workspace: on several streams, one waits for the other as for any tensor that both use.  A step's first call is
+        refused while a CUDA graph is captured; later ones may be, for replays within the step."""
         c = self.cache
         heads = q.size(1)
         q, at, bs, hs, ts = self._rows(q, heads, "q")
@@ -269,6 +270,8 @@ class PagedBatch:
             self._work_at, self._work_stream = self._work.data_ptr(), stream
             rc = _lib_call.infllm_page_batch_attend(self.handle, layer, at, bs, hs, ts, out.data_ptr(), lse_at, heads, scale, self._work_at,
                                                     stream)
+            if rc:  # (memory of a graph that is captured is not for calls outside it)
+                self._work, self._work_at = None, 0
         elif stream != self._work_stream and self._work is not None:  # it is not to be given away before this stream is done with it
             self._work.record_stream(torch.cuda.current_stream(c.device))
         if rc:

@@ -549,7 +549,13 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     if (q_bs < 0 || q_hs < 0 || q_ts < 0 || far / 8 > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_attend: queries that lie %lld bytes apart", (long long)far * 2);
     DeviceScope scope(c.device);
     cudaStream_t s = (cudaStream_t)stream;
-    if (b->upload) INFLLM_CUDA_OK(cudaMemcpyAsync(d_work, b->plan.data(), b->plan.size() * 4, cudaMemcpyHostToDevice, s));
+    if (b->upload) {
+      // (a copy that is captured is not made, and would be made later of whatever the next plan leaves there)
+      cudaStreamCaptureStatus capture;
+      INFLLM_CUDA_OK(cudaStreamIsCapturing(s, &capture));
+      if (capture != cudaStreamCaptureStatusNone) return fail(INFLLM_E_BADARG, "page_batch_attend: a plan that is not on the device yet, on a stream that captures");
+      INFLLM_CUDA_OK(cudaMemcpyAsync(d_work, b->plan.data(), b->plan.size() * 4, cudaMemcpyHostToDevice, s));
+    }
     b->upload = false;
     PagedParams P;
     P.plane = (int64_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim * 2;

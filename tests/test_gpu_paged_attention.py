@@ -538,3 +538,31 @@ def test_scales_that_are_none_to_base_2():
         with pytest.raises(L.InfLLMError):
             b.attend(0, q, scale=scale)
     assert (b.attend(0, q, scale=2.3e38) == 0).all()
+
+
+def test_a_plan_is_not_uploaded_by_a_graph():
+    """The copy of a plan would not run while a graph is captured, and would read another plan when it is replayed; a step's later calls
+    can be captured, and are replayed within it."""
+    from infllm_b200 import _lib as L
+
+    x = Kept(make(900, 16, 2, 128), 31)
+    root = x.open()
+    x.grow([root], [9000])
+    seqs = x.fork(root, 40)
+    b = x.grow(seqs, [2] * 40)
+    q = rand(x.g, 40, 8, 2, 128)
+    torch.cuda.synchronize()
+    with pytest.raises(L.InfLLMError, match="captures"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            b.attend(0, q)
+    want = b.attend(0, q)
+    x.check(b, [2] * 40, 8)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = b.attend(0, q)
+    for _ in range(3):
+        got.fill_(NAN)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
