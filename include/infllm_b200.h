@@ -539,6 +539,7 @@ int infllm_ctx_load(infllm_ctx* ctx, const char* path, void* stream);
  * Which pages a sequence has is known on the host at once; the device has a copy of the table.  What does not fit is
  * refused (INFLLM_E_CAPACITY) before anything changes.  Pages and sequence numbers are taken lowest first, for one sequence
  * after the other.  All calls on a cache belong on one stream, or are ordered by the caller; one host thread at a time.
+ * What changes pages is refused on a stream that captures a graph.
  *
  * d_pages (n_layers, 2: keys and values, n_pages, n_kv_heads, page_size, head_dim), d_table (max_sequences, max_pages);
  * head_dim 64 or 128, page_size 16, 32, 64 or 128.  device < 0: bookkeeping only, without a GPU.

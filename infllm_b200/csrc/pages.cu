@@ -208,6 +208,15 @@ static int need_pages(const infllm_pages* p, int64_t n, const char* what) {
   return INFLLM_OK;
 }
 
+// (in a capture the changes would not be made now, and made again with every replay)
+static int need_stream(const infllm_pages* p, void* stream, const char* what) {
+  if (p->cfg.device < 0) return INFLLM_OK;
+  cudaStreamCaptureStatus capture;
+  INFLLM_CUDA_OK(cudaStreamIsCapturing((cudaStream_t)stream, &capture));
+  if (capture != cudaStreamCaptureStatusNone) return fail(INFLLM_E_BADARG, "%s: pages change, and the stream captures", what);
+  return INFLLM_OK;
+}
+
 // the lowest numbers that no sequence has
 static int need_seqs(const infllm_pages* p, int64_t n, std::vector<int32_t>* out, const char* what) {
   for (size_t i = 0; i < p->seqs.size() && (int64_t)out->size() < n; ++i)
@@ -239,7 +248,7 @@ static void cut(infllm_pages* p, int32_t seq, int64_t length) {
 }
 
 // room for counts[i] more tokens of each sequence, or for `same`
-static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* counts, int32_t same, int n, const char* what) {
+static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* counts, int32_t same, int n, void* stream, const char* what) {
   const int page = p->cfg.page_size;
   int64_t need = 0;
   for (int i = 0; i < n; ++i) {
@@ -255,6 +264,7 @@ static int extend(infllm_pages* p, const int32_t* seqs, const int32_t* counts, i
     if (more > 0 && s.length % page && p->uses[s.pages.back()] > 1) ++need;
   }
   INFLLM_TRY(need_pages(p, need, what));
+  if (need > 0) INFLLM_TRY(need_stream(p, stream, what));
   ++p->change;
   for (int i = 0; i < n; ++i) {
     PageSeq& s = p->seqs[seqs[i]];
@@ -435,6 +445,7 @@ extern "C" int infllm_pages_fork(infllm_pages* p, const int32_t* seqs, int n, in
     for (int i = 0; i < n; ++i) need += p->seqs[seqs[i]].length % page ? n_each : 0;
     INFLLM_TRY(need_pages(p, need, "pages_fork"));
     DeviceScope scope(p->cfg.device);
+    INFLLM_TRY(need_stream(p, stream, "pages_fork"));
     ++p->change;
     int at = 0;
     for (int i = 0; i < n; ++i) {
@@ -476,6 +487,7 @@ extern "C" int infllm_pages_copy(infllm_pages* p, const int32_t* seqs, int n, in
     }
     INFLLM_TRY(need_pages(into, need, "pages_copy"));
     DeviceScope scope(b.device);
+    INFLLM_TRY(need_stream(into, stream, "pages_copy"));
     ++into->change;
     for (int i = 0; i < n; ++i) {
       const PageSeq& s = p->seqs[seqs[i]];
@@ -547,6 +559,7 @@ extern "C" int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n,
     }
     INFLLM_TRY(need_pages(p, need, "pages_compact"));
     DeviceScope scope(p->cfg.device);
+    INFLLM_TRY(need_stream(p, stream, "pages_compact"));
     ++p->change, ++p->reshape;
     std::vector<int32_t> gone;
     span = spans;
@@ -649,7 +662,7 @@ extern "C" int infllm_page_batch_extend(infllm_page_batch* b, const int32_t* cou
   return guarded("page_batch_extend", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_extend"));
     DeviceScope scope(b->cache->cfg.device);
-    INFLLM_TRY(extend(b->cache, b->seqs.data(), counts, same, (int)b->seqs.size(), "page_batch_extend"));
+    INFLLM_TRY(extend(b->cache, b->seqs.data(), counts, same, (int)b->seqs.size(), stream, "page_batch_extend"));
     set_counts(b, counts, same);
     set_reach(b, reach);
     return flush(b->cache, b->cache, (cudaStream_t)stream);

@@ -566,3 +566,30 @@ def test_a_plan_is_not_uploaded_by_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_pages_do_not_change_in_a_graph():
+    """The device's copy of the table would be changed by replays alone, while the host goes on at once: refused, and nothing changes.
+    A step within pages that are there can be captured."""
+    from infllm_b200 import _lib as L
+
+    c, g = make(40, 16, 2, 128), torch.Generator(device="cuda").manual_seed(4)
+    s = c.open(2)
+    b = c.batch(s)
+    b.extend([20, 16])
+    k = rand(g, 2, 2, 1, 128)
+    torch.cuda.synchronize()
+    for call in (lambda: b.extend(1), lambda: c.fork(s, 1), lambda: c.copy(s), lambda: c.compact(s[:1], [[(3, 20)]])):
+        with pytest.raises(L.InfLLMError, match="captures"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        assert c.free_pages == 37 and [c.length(x) for x in s] == [20, 16] and c.open() == [2]
+        c.free([2])
+    graph = torch.cuda.CUDAGraph()
+    b = c.batch(s[:1])
+    with torch.cuda.graph(graph):
+        b.extend(1)
+        b.write(0, k[:1], k[:1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(c.pages[0, 0, c.page_ids(s[0])[1], :, 4], k[0, :, 0]) and torch.isnan(c.pages).sum() == c.pages.numel() - 512
