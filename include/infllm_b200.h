@@ -569,6 +569,11 @@ int infllm_pages_compact(infllm_pages* p, const int32_t* seqs, int n, const int6
 int infllm_pages_info(const infllm_pages* p, int32_t seq, int64_t* length, int64_t* position);
 int infllm_pages_row(const infllm_pages* p, int32_t seq, int32_t* out, int cap, int* n); /* its pages */
 int infllm_pages_free_count(const infllm_pages* p); /* free pages */
+/* A wait that runs out in an attention kernel is recorded for its cache too: attend returns INFLLM_E_TIMEOUT on the first call after it
+ * has got there, and so does infllm_pages_check, which waits for the stream first.  Either clears the record.
+ * infllm_pages_error_set writes it from the host, for tests of that. */
+int infllm_pages_check(infllm_pages* p, void* stream);
+int infllm_pages_error_set(infllm_pages* p, int code, int where);
 
 /* A batch (destroyed before its cache): sequences, and of each a count of newest tokens that the calls are about.  The tensors of a call have as many
  * tokens as the largest count; a sequence with fewer has its own at the end, the rows before them are not read, or written

@@ -208,6 +208,8 @@ SIGNATURES = {
     "infllm_pages_info": (c_int, [c_void_p, c_int32, POINTER(c_int64), POINTER(c_int64)]),
     "infllm_pages_row": (c_int, [c_void_p, c_int32, POINTER(c_int32), c_int, POINTER(c_int)]),
     "infllm_pages_free_count": (c_int, [c_void_p]),
+    "infllm_pages_check": (c_int, [c_void_p, c_void_p]),
+    "infllm_pages_error_set": (c_int, [c_void_p, c_int, c_int]),
     "infllm_page_batch_create": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_void_p)]),
     "infllm_page_batch_destroy": (c_int, [c_void_p]),
     "infllm_page_batch_extend": (c_int, [c_void_p, POINTER(c_int32), c_int32, POINTER(c_int64), c_void_p]),

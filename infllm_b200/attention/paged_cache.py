@@ -114,6 +114,11 @@ class PagedCache:
     def batch(self, seqs):
         return PagedBatch(self, seqs)
 
+    def check(self):
+        """Waits for the current stream, and raises InfLLMError (E_TIMEOUT) where an attention kernel has given up a wait and left
+        rows unwritten.  attend() reports that too, but of calls whose kernels have run by then."""
+        _lib.check(_lib_call.infllm_pages_check(self.handle, _lib.raw_stream(self.device)))
+
     # -- what there is
     def _info(self, seq):
         length, position = c_int64(), c_int64()

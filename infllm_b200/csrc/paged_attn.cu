@@ -21,6 +21,19 @@ namespace infllm {
 
 using namespace mma;
 
+// A block that gave up a wait has left its rows unwritten: the cache's next call says so, and clears the record.
+int check_lost(infllm_pages* p, cudaStream_t s) {
+  volatile int32_t* lost = p->lost;
+  if (!lost || lost[0] == 0) return INFLLM_OK;
+  const int code = lost[0], where = lost[1], block = lost[2];
+  lost[0] = 0;
+  int* err = nullptr;  // (also where the other kernels have theirs)
+  INFLLM_TRY(tc_get_error_ptr(&err));
+  INFLLM_CUDA_OK(cudaMemsetAsync(err, 0, 4 * sizeof(int32_t), s));
+  return fail(INFLLM_E_TIMEOUT, "a bounded wait of the attention over pages ran out in a call before (code %d, wait %d, block %d): the rows that "
+              "the block was to write are not valid", code, where, block);
+}
+
 // ------------------------------------------------------------------------------------------------------- few rows
 // Four warps share a unit's groups of 16 keys and meet in shared memory.  A token of one sequence over 131072 keys (537 MB, 8 KV heads): 86 us,
 // 6.3 TB/s, the join in it.
@@ -533,7 +546,7 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
                                         float* d_lse, int n_heads, float scale, void* d_work, void* stream) {
   return guarded("page_batch_attend", [&]() -> int {
     INFLLM_TRY(batch_alive(b, "page_batch_attend"));
-    const infllm_pages* p = b->cache;
+    infllm_pages* p = b->cache;
     const infllm_pages_config& c = p->cfg;
     if (c.device < 0) return fail(INFLLM_E_BADARG, "page_batch_attend: a cache without a device");
     if (layer < 0 || layer >= c.n_layers) return fail(INFLLM_E_BADARG, "page_batch_attend: layer %d of %d", layer, c.n_layers);
@@ -549,6 +562,7 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     if (q_bs < 0 || q_hs < 0 || q_ts < 0 || far / 8 > INT32_MAX) return fail(INFLLM_E_BADARG, "page_batch_attend: queries that lie %lld bytes apart", (long long)far * 2);
     DeviceScope scope(c.device);
     cudaStream_t s = (cudaStream_t)stream;
+    INFLLM_TRY(check_lost(p, s));
     if (b->upload) {
       // (a copy that is captured is not made, and would be made later of whatever the next plan leaves there)
       cudaStreamCaptureStatus capture;
@@ -571,6 +585,7 @@ extern "C" int infllm_page_batch_attend(infllm_page_batch* b, int layer, const v
     P.tile_unit = (const AttnUnit*)(plan + b->off_tile_unit), P.cta_unit = plan + b->off_cta;
     P.page0 = 2 * layer * c.n_pages, P.n_pages = c.n_pages;
     INFLLM_TRY(tc_get_error_ptr(&P.err));
+    P.lost = p->lost;
     P.max_pages = c.max_pages, P.page = c.page_size, P.n_kv = c.n_kv_heads, P.group = n_heads / c.n_kv_heads, P.most = b->most;
     P.batch = (int)b->seqs.size();
     P.n_beside = b->n_beside * c.n_kv_heads;

@@ -39,6 +39,7 @@ struct PagedParams {
   const int32_t* cta_unit;  // the first unit of each block
   int32_t page0, n_pages;   // the layer's first page in the map, pages from keys to values
   int* err;
+  int32_t* lost;            // the cache's own record of it, in the host's memory
   const char* pages;  // keys of the layer
   int64_t plane;      // bytes from keys to values
   const int32_t* table;

@@ -455,6 +455,12 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && *abort_flag) {
+    volatile int32_t* lost = P.lost;
+    lost[1] = *(volatile int*)(P.err + 1), lost[2] = blockIdx.x;
+    __threadfence_system();
+    lost[0] = kErrWaitTimeout;
+  }
 }
 
 int paged_tc_launch(const PagedParams& P, int dtype, int head_dim, int n_ctas, cudaStream_t s) {

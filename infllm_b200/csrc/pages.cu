@@ -8,6 +8,7 @@
 // it; where truncation left it shared, it is copied before the next token is written).
 #include <algorithm>
 #include <cstring>
+#include <mutex>
 
 #include "pages.cuh"
 
@@ -298,6 +299,28 @@ int batch_alive(const infllm_page_batch* b, const char* what) {
   return INFLLM_OK;
 }
 
+// Records that a block's last act may be to write: of the process and never given back to the system, since a kernel may outlive its
+// cache's books.
+namespace {
+std::mutex lost_mutex;
+std::vector<int32_t*> lost_free;
+}  // namespace
+
+static int take_lost(int32_t** out) {
+  constexpr int kRecords = 256;
+  std::lock_guard<std::mutex> lock(lost_mutex);
+  if (lost_free.empty()) {
+    lost_free.reserve(kRecords);
+    int32_t* block = nullptr;
+    INFLLM_CUDA_OK(cudaHostAlloc((void**)&block, kRecords * 4 * sizeof(int32_t), cudaHostAllocPortable));
+    for (int i = 0; i < kRecords; ++i) lost_free.push_back(block + 4 * i);
+  }
+  *out = lost_free.back();
+  lost_free.pop_back();
+  std::fill(*out, *out + 4, 0);
+  return INFLLM_OK;
+}
+
 // ------------------------------------------------------------------------------------------------------------ writes
 // New tokens' keys and values into their pages, keys and queries rotated to the tokens' positions on the way.  A block has
 // a token, or some where a token's rows are few; a thread has 8 dimensions of the first half of a row and the 8 that go with them in the second, so that it needs
@@ -382,6 +405,15 @@ __global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const __grid_
 // ------------------------------------------------------------------------------------------------------- entry points
 using namespace infllm;
 
+infllm_pages::~infllm_pages() {
+  if (!lost) return;
+  std::lock_guard<std::mutex> lock(lost_mutex);
+  try {
+    lost_free.push_back(lost);
+  } catch (const std::bad_alloc&) {  // (16 bytes fewer)
+  }
+}
+
 extern "C" int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages** out) {
   return guarded("pages_create", [&]() -> int {
     if (!cfg || !out) return fail(INFLLM_E_BADARG, "pages_create: null pointer");
@@ -408,6 +440,7 @@ extern "C" int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages*
       if (!scope.ok()) return fail(INFLLM_E_CUDA, "pages_create: no device %d", c.device);
       if (c.device < 0) return INFLLM_OK;
       INFLLM_CUDA_OK(cudaDeviceGetAttribute(&p->n_sm, cudaDevAttrMultiProcessorCount, c.device));
+      INFLLM_TRY(take_lost(&p->lost));
       return pages_encode_map(p);
     });
     if (rc != INFLLM_OK) {
@@ -421,6 +454,22 @@ extern "C" int infllm_pages_create(const infllm_pages_config* cfg, infllm_pages*
 
 extern "C" int infllm_pages_destroy(infllm_pages* p) {
   delete p;
+  return INFLLM_OK;
+}
+
+extern "C" int infllm_pages_check(infllm_pages* p, void* stream) {
+  return guarded("pages_check", [&]() -> int {
+    if (!p) return fail(INFLLM_E_BADARG, "pages_check: null pointer");
+    if (!p->lost) return INFLLM_OK;
+    DeviceScope scope(p->cfg.device);
+    INFLLM_CUDA_OK(cudaStreamSynchronize((cudaStream_t)stream));
+    return check_lost(p, (cudaStream_t)stream);
+  });
+}
+
+extern "C" int infllm_pages_error_set(infllm_pages* p, int code, int where) {
+  if (!p || !p->lost) return fail(INFLLM_E_BADARG, "pages_error_set: no cache with a device");
+  p->lost[1] = where, p->lost[2] = 0, p->lost[0] = code;
   return INFLLM_OK;
 }
 

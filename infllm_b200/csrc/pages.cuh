@@ -100,7 +100,9 @@ struct infllm_pages {
   std::vector<int32_t> to_pages;
   CUtensorMap map;       // of all pages (paged_tc.cu)
   int32_t n_sm = 148;
+  int32_t* lost = nullptr;  // pinned: written by a block whose wait ran out (code, wait, block), read by the next calls
 
+  ~infllm_pages();
   int32_t pages_of(int64_t tokens) const { return (int32_t)((tokens + cfg.page_size - 1) / cfg.page_size); }
 };
 
@@ -129,5 +131,6 @@ struct infllm_page_batch {
 
 namespace infllm {
 int batch_alive(const infllm_page_batch* b, const char* what);
+int check_lost(infllm_pages* p, cudaStream_t s);  // paged_attn.cu
 int pages_encode_map(infllm_pages* p);  // paged_tc.cu
 }  // namespace infllm

@@ -71,6 +71,7 @@ class SharedPromptDecoder(HeadGroupDecoder):
                 if i < max_length - 1:
                     batch.extend(1)
                     logits = self.step(nxt[:, None])
+            self.cache.check()
         finally:
             self.reset()
             self.cache.free(seqs)

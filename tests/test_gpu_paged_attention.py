@@ -593,3 +593,25 @@ def test_pages_do_not_change_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(c.pages[0, 0, c.page_ids(s[0])[1], :, 4], k[0, :, 0]) and torch.isnan(c.pages).sum() == c.pages.numel() - 512
+
+
+@pytest.mark.parametrize("how", ["attend", "check"])
+def test_a_wait_that_ran_out_is_reported(how):
+    """By the cache whose kernel gave it up, once.  (Set from the host: nothing is made to time out on the GPU.)"""
+    from infllm_b200 import _lib as L
+
+    c, other = make(40, 16, 2, 128), make(40, 16, 2, 128)
+    b, of_other = (x.batch(x.open()) for x in (c, other))
+    for x in (b, of_other):
+        x.extend(20)
+        k = torch.zeros((1, 2, 20, 128), dtype=torch.bfloat16, device="cuda")
+        x.write(0, k, k)
+    q = torch.zeros((1, 8, 20, 128), dtype=torch.bfloat16, device="cuda")
+    L.check(L.lib.infllm_pages_error_set(c.handle, 1, 712))
+    assert not torch.isnan(of_other.attend(0, q)).any()
+    other.check()
+    with pytest.raises(L.InfLLMError, match="wait 712") as e:
+        b.attend(0, q) if how == "attend" else c.check()
+    assert e.value.code == L.E_TIMEOUT
+    c.check()
+    assert not torch.isnan(b.attend(0, q)).any()

@@ -48,3 +48,25 @@ def test_what_does_not_fit_leaves_the_cache_as_it_was():
     with pytest.raises(TypeError):  # the attention type alone, without a layer of a batch
         dec.step(ids)
     assert dec.generate_many(ids, 2, max_length=2)[0].shape == (2, 2)
+
+
+def test_answers_whose_attention_gave_up_are_not_returned(monkeypatch):
+    """A wait that ran out in the last steps' kernels is reported before the answers are (set from the host)."""
+    from infllm_b200 import _lib as L
+    from infllm_b200.utils import SharedPromptDecoder
+
+    dec = SharedPromptDecoder(**SHAPE, n_pages=40, page_size=16, max_sequences=5, max_tokens=256, seed=3)
+    ids, step, calls = torch.zeros((1, 60), dtype=torch.int64, device="cuda"), dec.step, []
+
+    def last(x):
+        out = step(x)
+        calls.append(x)
+        if len(calls) == 3:  # the prompt, and two tokens
+            L.check(L.lib.infllm_pages_error_set(dec.cache.handle, 1, 722))
+        return out
+
+    monkeypatch.setattr(dec, "step", last)
+    with pytest.raises(L.InfLLMError, match="wait 722"):
+        dec.generate_many(ids, 2, max_length=3)
+    assert dec.cache.free_pages == 40
+    assert dec.generate_many(ids, 2, max_length=3)[0].shape == (2, 3)
