@@ -76,3 +76,8 @@ class SharedPromptDecoder(HeadGroupDecoder):
             self.reset()
             self.cache.free(seqs)
         return torch.stack(out, dim=1), torch.stack(trail, dim=1)
+
+    def generate(self, input_ids, max_length=64, chunk_size=8192):
+        """One greedy answer to the prompt input_ids (1, L): generated ids, and their logits (max_length, vocab)."""
+        out, trail = self.generate_many(input_ids, 1, max_length, chunk_size, temperature=0)
+        return out[0].tolist(), trail[0]

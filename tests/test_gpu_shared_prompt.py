@@ -70,3 +70,16 @@ def test_answers_whose_attention_gave_up_are_not_returned(monkeypatch):
         dec.generate_many(ids, 2, max_length=3)
     assert dec.cache.free_pages == 40
     assert dec.generate_many(ids, 2, max_length=3)[0].shape == (2, 3)
+
+
+def test_generate_is_one_greedy_answer():
+    """The decoder's own generate(): the same tokens and logits as one answer of generate_many."""
+    from infllm_b200.utils import SharedPromptDecoder
+
+    dec = SharedPromptDecoder(**SHAPE, n_pages=60, page_size=16, max_tokens=1024, seed=3, rope_base=BASE, init_std=0.05)
+    ids = torch.randint(0, SHAPE["vocab"], (1, 300), generator=torch.Generator().manual_seed(5)).cuda()
+    out, trail = dec.generate(ids, max_length=5, chunk_size=128)
+    assert len(out) == 5 and all(isinstance(x, int) for x in out) and trail.shape == (5, SHAPE["vocab"])
+    many, logits = dec.generate_many(ids, 1, max_length=5, chunk_size=128, temperature=0)
+    assert many[0].tolist() == out and torch.equal(logits[0], trail)
+    assert dec.cache.free_pages == 60
