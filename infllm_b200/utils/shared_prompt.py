@@ -28,6 +28,18 @@ class SharedPromptDecoder(HeadGroupDecoder):
         for layer in self.layers:
             layer["past"] = None
 
+    def _draw(self, logits, temperature, generator):
+        if temperature == 0:
+            nxt = logits.argmax(dim=-1)
+        else:
+            nxt = torch.multinomial(torch.softmax(logits / temperature, dim=-1), 1, generator=generator)[:, 0]
+        if self.world > 1:  # the first rank's: with other tokens than its own a rank would add another sequence's rows to the sums
+            import torch.distributed as dist
+
+            nxt = nxt.contiguous()
+            dist.broadcast(nxt, group=self.group, group_src=0)
+        return nxt
+
     def read(self, input_ids, chunk_size=8192):
         """A new sequence of the prompt input_ids (1, L): its number in the cache, and the logits of its last position."""
         if input_ids.size(1) < 1:
@@ -50,7 +62,8 @@ class SharedPromptDecoder(HeadGroupDecoder):
     @torch.inference_mode()
     def generate_many(self, input_ids, n, max_length=64, chunk_size=8192, temperature=1.0, generator=None):
         """n answers of max_length tokens to the prompt input_ids (1, L), drawn from the softmax of the logits over
-        `temperature` with the random numbers of `generator` (a CUDA generator; temperature 0: the largest logit).
+        `temperature` with the random numbers of `generator` (a CUDA generator; temperature 0: the largest logit), of several
+        ranks with the first one's.
         Returns the answers (n, max_length) and the logits that each token was drawn from (n, max_length, vocab)."""
         root, logits = self.read(input_ids, chunk_size)
         seqs = [root]
@@ -63,10 +76,7 @@ class SharedPromptDecoder(HeadGroupDecoder):
             out, trail = [], []
             for i in range(max_length):
                 trail.append(logits.clone())
-                if temperature == 0:
-                    nxt = logits.argmax(dim=-1)
-                else:
-                    nxt = torch.multinomial(torch.softmax(logits / temperature, dim=-1), 1, generator=generator)[:, 0]
+                nxt = self._draw(logits, temperature, generator)
                 out.append(nxt)
                 if i < max_length - 1:
                     batch.extend(1)
