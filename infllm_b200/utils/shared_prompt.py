@@ -60,11 +60,13 @@ class SharedPromptDecoder(HeadGroupDecoder):
         return seq[0], logits
 
     @torch.inference_mode()
-    def generate_many(self, input_ids, n, max_length=64, chunk_size=8192, temperature=1.0, generator=None):
+    def generate_many(self, input_ids, n, max_length=64, chunk_size=8192, temperature=1.0, generator=None,
+                      keep_logits=True):
         """n answers of max_length tokens to the prompt input_ids (1, L), drawn from the softmax of the logits over
         `temperature` with the random numbers of `generator` (a CUDA generator; temperature 0: the largest logit), of several
         ranks with the first one's.
-        Returns the answers (n, max_length) and the logits that each token was drawn from (n, max_length, vocab)."""
+        Returns the answers (n, max_length) and the logits that each token was drawn from (n, max_length, vocab), fp32;
+        without keep_logits, None in their place."""
         root, logits = self.read(input_ids, chunk_size)
         seqs = [root]
         try:
@@ -75,7 +77,8 @@ class SharedPromptDecoder(HeadGroupDecoder):
             logits = logits.expand(n, -1)
             out, trail = [], []
             for i in range(max_length):
-                trail.append(logits.clone())
+                if keep_logits:
+                    trail.append(logits.clone())
                 nxt = self._draw(logits, temperature, generator)
                 out.append(nxt)
                 if i < max_length - 1:
@@ -85,7 +88,7 @@ class SharedPromptDecoder(HeadGroupDecoder):
         finally:
             self.reset()
             self.cache.free(seqs)
-        return torch.stack(out, dim=1), torch.stack(trail, dim=1)
+        return torch.stack(out, dim=1), torch.stack(trail, dim=1) if keep_logits else None
 
     def generate(self, input_ids, max_length=64, chunk_size=8192):
         """One greedy answer to the prompt input_ids (1, L): generated ids, and their logits (max_length, vocab)."""

@@ -83,3 +83,29 @@ def test_generate_is_one_greedy_answer():
     many, logits = dec.generate_many(ids, 1, max_length=5, chunk_size=128, temperature=0)
     assert many[0].tolist() == out and torch.equal(logits[0], trail)
     assert dec.cache.free_pages == 60
+
+
+def test_logits_need_not_be_kept():
+    """The same answers, without memory of (n, max_length, vocab)."""
+    from infllm_b200.utils import SharedPromptDecoder
+
+    shape = dict(SHAPE, vocab=60000)
+    dec = SharedPromptDecoder(**shape, n_pages=200, page_size=16, max_tokens=1024, seed=3, rope_base=BASE, init_std=0.05)
+    ids = torch.randint(0, shape["vocab"], (1, 40), generator=torch.Generator().manual_seed(5)).cuda()
+    most = []
+    for keep in (True, False):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        base = torch.cuda.memory_allocated()
+        out, trail = dec.generate_many(ids, 30, max_length=40, generator=torch.Generator(device="cuda").manual_seed(1), keep_logits=keep)
+        torch.cuda.synchronize()
+        most.append(torch.cuda.max_memory_allocated() - base)
+        if keep:
+            want = out
+            assert trail.shape == (30, 40, shape["vocab"])
+        else:
+            assert trail is None and torch.equal(out, want)
+        del trail
+    kept = 30 * 40 * shape["vocab"] * 4
+    # a step's logits and what the draw makes of them are there in either case
+    assert most[0] >= kept and most[1] <= kept // 2
