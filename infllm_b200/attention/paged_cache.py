@@ -17,6 +17,7 @@ attention types take them.  Work goes to the current stream; all calls on a cach
 the caller."""
 import ctypes
 import math
+from array import array
 from ctypes import c_int32, c_int64
 
 import torch
@@ -27,8 +28,13 @@ from .rope import RotaryEmbeddingESM
 _lib_call = _lib.lib
 
 
+# (ctypes cuts what does not fit, which would name another sequence or count; array raises OverflowError)
 def _ids(seqs):
-    return (c_int32 * len(seqs))(*seqs)
+    return (c_int32 * len(seqs))(*array("i", seqs))
+
+
+def _long(values):
+    return (c_int64 * len(values))(*array("q", values))
 
 
 class PagedCache:
@@ -92,7 +98,7 @@ class PagedCache:
         """Cuts each sequence to a length."""
         if len(seqs) != len(lengths):
             raise ValueError(f"{len(seqs)} sequences and {len(lengths)} lengths")
-        _lib.check(_lib_call.infllm_pages_truncate(self.handle, _ids(seqs), (c_int64 * len(seqs))(*lengths), len(seqs)))
+        _lib.check(_lib_call.infllm_pages_truncate(self.handle, _ids(seqs), _long(lengths), len(seqs)))
 
     def free(self, seqs):
         """Ends sequences; pages that no other one shares are free."""
@@ -108,7 +114,7 @@ class PagedCache:
         counts = _ids([len(spans) for spans in keep])
         if len(flat) != 2 * sum(counts):
             raise ValueError("spans are pairs (start, stop)")
-        _lib.check(_lib_call.infllm_pages_compact(self.handle, _ids(seqs), len(seqs), (c_int64 * len(flat))(*flat), counts,
+        _lib.check(_lib_call.infllm_pages_compact(self.handle, _ids(seqs), len(seqs), _long(flat), counts,
                                                   _lib.raw_stream(self.device)))
 
     def batch(self, seqs):
@@ -122,7 +128,7 @@ class PagedCache:
     # -- what there is
     def _info(self, seq):
         length, position = c_int64(), c_int64()
-        _lib.check(_lib_call.infllm_pages_info(self.handle, seq, ctypes.byref(length), ctypes.byref(position)))
+        _lib.check(_lib_call.infllm_pages_info(self.handle, _ids([seq])[0], ctypes.byref(length), ctypes.byref(position)))
         return length.value, position.value
 
     def length(self, seq):
@@ -136,7 +142,7 @@ class PagedCache:
     def page_ids(self, seq):
         n = ctypes.c_int()
         out = (c_int32 * self.table.size(1))()
-        _lib.check(_lib_call.infllm_pages_row(self.handle, seq, out, len(out), ctypes.byref(n)))
+        _lib.check(_lib_call.infllm_pages_row(self.handle, _ids([seq])[0], out, len(out), ctypes.byref(n)))
         return out[:n.value]
 
     @property
@@ -171,6 +177,8 @@ class PagedBatch:
 
     def _counts(self, n):
         if isinstance(n, int):
+            if not -1 << 31 <= n < 1 << 31:
+                raise OverflowError(f"{n} tokens")
             return None, n, n
         if len(n) != self._n:
             raise ValueError(f"{self._n} sequences and {len(n)} counts")

@@ -415,3 +415,30 @@ def test_a_plan_that_found_no_memory_is_not_used_with_the_last_ones(monkeypatch)
         b.attend(0, q)
         b.attend(1, q)
         assert len(lib.seen) == 2 and all(sizes[w] >= 1 << 16 for w in lib.seen)
+
+
+def test_numbers_beyond_the_library_s_are_refused(monkeypatch):
+    """Not cut to 32 or 64 bits, where they would name another sequence or count."""
+    import torch
+
+    from infllm_b200.attention import paged_cache as M
+
+    monkeypatch.setattr(M._lib, "raw_stream", lambda device: None)
+    book = Cache()
+    c = M.PagedCache.__new__(M.PagedCache)
+    c.handle, c.device, c.head_dim, c.table = book.h, None, 64, torch.zeros((12, 10))
+    s = c.open()[0]
+    b = c.batch([s])
+    b.extend(20)
+    far = s + (1 << 32)
+    try:
+        for call in (lambda: c.free([far]), lambda: c.fork([far], 1), lambda: c.copy([far]), lambda: c.truncate([far], [3]), lambda: c.truncate([s], [1 << 64]),
+                     lambda: c.compact([far], [[]]), lambda: c.compact([s], [[(0, (1 << 64) + 4)]]), lambda: c.batch([far]), lambda: c.length(far),
+                     lambda: c.position(far), lambda: c.page_ids(far), lambda: b.extend((1 << 32) + 1), lambda: b.extend([(1 << 32) + 1]),
+                     lambda: b.plan(1 << 32), lambda: b.retract((1 << 32) + 1), lambda: b.retract([(1 << 32) + 1])):
+            with pytest.raises(OverflowError):
+                call()
+            assert c.length(s) == 20 and b.tokens == 20 and c.free_pages == 38 and c.open() == [s + 1]
+            c.free([s + 1])
+    finally:
+        c.handle = None  # (the book's)
