@@ -228,9 +228,14 @@ constexpr int kBlockWork = 8;  // worth a block
 constexpr int kGroupWork = 4;  // of a group of 16 keys for few rows, by a warp beside the products
 
 // Work of a batch, in groups of 16 keys by tiles of 16 rows and KV heads, up to which all of it goes to the kernel of few rows: that
-// is through before the tensor-core kernel has begun, and is one launch less where both would be needed.  (Eight tokens on 1000 keys,
-// 1100: 11.6 us instead of 22.6; 30 on 1000, 4500: 17.0, 24.2; 13 of 28/4 heads of 64 on 5000, 8700: 15.2, 16.5; 33 new tokens of a
-// sequence of 2000, 9100: 18.4, 18.5; five times 20 on 700, 9000: 29, 23; ten on 8000, 12300: 24.5, 18.8.)
+// is through before the tensor-core kernel has begun, and is one launch less where both would be needed.  Both ways were timed on 660
+// random batches (1 to 64 sequences, prompts of 64 to 60000 tokens, 1 to 64 new ones, six layouts of heads, half with 64 dimensions): the
+// time by few rows over that by the tensor cores is, in the median (and from the tenth to the 90th percentile, which says what the measure
+// leaves out: keys that several row tiles read, long leaves),
+//   work 1500 to 4000    0.70 (0.45 to 0.99)    4000 to 6000    0.81 (0.57 to 1.02)     6000 to 8000    0.88 (0.65 to 1.12)
+//        8000 to 10000   1.09 (0.81 to 1.36)    10000 to 13000  1.11 (0.74 to 1.47)     13000 to 20000  1.31 (0.97 to 1.75)
+// alike for 64 and 128 dimensions.  With a bound of 7000 a batch takes 3.1 % more than the better way, of 8000 or 8800 2.3 %, of 11000
+// 2.5 %, of 14000 3.5 %; always the tensor cores 25 %, never 19 %.
 constexpr int64_t kLittle = 8800;
 
 // Groups of 16 keys of a block's unit, where nodes have groups[..] of them for each KV head: so that all blocks run in one, two or
