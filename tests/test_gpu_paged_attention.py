@@ -615,3 +615,30 @@ def test_a_wait_that_ran_out_is_reported(how):
     assert e.value.code == L.E_TIMEOUT
     c.check()
     assert not torch.isnan(b.attend(0, q)).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,kv,group", [(128, 2, 4), (64, 2, 7), (128, 1, 16)])
+@pytest.mark.parametrize("prefix,tails", [(0, (24,)), (0, (1, 3, 70)), (32, (5, 9)), (300, (20, 1, 64))])
+def test_few_rows_round_their_output_alone(dtype, dim, kv, group, prefix, tails):
+    """The kernel of few rows holds a probability as two 16-bit numbers, so that the rounding of the output is the only one of 16 bits:
+    the output lies between the roundings of (o - rest) and of (o + rest), where `rest` has no rounding to 16 bits in it.
+
+    rest: of sum_j p_j |v_j| 2^-16 for what is held in 32 bits, and u^2 (2^-16, 2^-22) for what the second number leaves of p_j; fp16 has
+    a least step of 2^-24, by half of which a p_j may be off: 2^-25 sum_j |v_j| over the sum of the unnormalised p, which is at least 1."""
+    x = Kept(make((prefix + sum(tails)) // 16 + 3 * len(tails) + 2, 16, kv, dim, dtype), prefix + dim)
+    root = x.open()
+    if prefix:
+        x.grow([root], [prefix])
+    seqs = x.fork(root, len(tails))
+    b = x.grow(seqs, list(tails))
+    b.plan(1)
+    q = rand(x.g, len(seqs), kv * group, 1, dim, dtype=dtype)
+    out = b.attend(0, q)
+    least = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for i, s in enumerate(seqs):
+        k, v = (t[s].double().repeat_interleave(group, 0) for t in (x.k, x.v))
+        p = torch.softmax(q[i].double() @ k.transpose(1, 2) / math.sqrt(dim), -1)
+        want, mass = p @ v, p @ v.abs()
+        rest = (2.0 ** -16 + U[dtype] ** 2) * mass + least * v.abs().sum(1, keepdim=True)
+        assert ((want - rest).to(dtype) <= out[i]).all() and (out[i] <= (want + rest).to(dtype)).all(), i
