@@ -9,11 +9,13 @@
 // the order K0 K1 V0 K2 V1 ..; another warp issues the products.  Blocks work through a list of units of about equal work.
 // Two more warps take units of few rows (paged_rows.cuh), whose loads fit in beside the products.
 // The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
+// P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.  With
+// the output's own rounding that is an error of 2.3e-3 for bf16 where that alone is 1.7e-3.  Sums, O and partial rows are fp32.
 //
 // What bounds it: with two teams a round of one of them, 3450 cycles for 256 rows by 128 keys (by clock readings, 2048 tokens behind 28000:
 // maximum 300, exponentials 1490, hand-overs 270, then its P V and next Q K^T, 512 each, and 360 until the scores are seen), in which the
 // tensor pipe is needed for 2048; with one team the keys' bytes.  128 tokens of 32/8 heads over 131072 shared keys: 283 us for 275 GFLOP
-// as a launch by itself (0.97 PFLOP/s; each byte from HBM once, though two blocks share every key), 343 with the join, calls back to
+// as a launch by itself (0.97 PFLOP/s; each byte from HBM once, though two blocks share every key), 337 with the join, calls back to
 // back; 32 over 32768 (134 MB): 40 us, of which 8 lie before the first scores and 3 between the last tile and its rows.
 // Tried: steps of 64 keys with two buffers of scores a team (a product of 64 columns takes nearly as long as one of 128: 13 % more time), P in
 // two halves (scores 350 cycles earlier, exponentials 700 longer), an issuer that polls both teams (25 % more), sixteen softmax warps (5 to

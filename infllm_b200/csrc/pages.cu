@@ -21,7 +21,7 @@ namespace infllm {
 // pages << 16); those pages' numbers are behind them, four to an item.
 // Pages that are written were free before the call, and rows that are written belong to sequences that are not read from, so
 // that the order of the blocks does not matter.  It is bound by the bytes of the tokens, read once and written as often as there
-// are pages for them: half of two 65536-token sequences of four layers (2.1 GB) in 325 us, 6.6 TB/s; the last page of a sequence
+// are pages for them: half of two 65536-token sequences of four layers (2.1 GB) in 326 us, 6.6 TB/s; the last page of a sequence
 // for 64 forks in eight layers (268 MB written) in 47.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveAhead = 8;  // 16-byte loads of a thread in flight
