@@ -606,6 +606,62 @@ int infllm_page_batch_plan(infllm_page_batch* b, int n_heads, int64_t* work_byte
 int infllm_page_batch_attend(infllm_page_batch* b, int layer, const void* d_q, int64_t q_bs, int64_t q_hs, int64_t q_ts, void* d_out,
                              float* d_lse, int n_heads, float scale, void* d_work, void* stream);
 
+/* ------------------------------------------------------- cache in 4 bits, attention over it, eviction by attention weight
+ * (No counterpart in the reference, which moves what it does not attend to out of the device's memory.)  Keys and values of several
+ * sequences in 4 bits and a least number and a step per 32 of them; of every token and KV head its position, and a weight:
+ * what attention has given it, by which infllm_packed_evict chooses who stays.
+ *
+ * Of each 32 neighbouring numbers x of a row, in the 16-bit type T: m = min x, s = T((max x - m) / 15), and of each x the code c, the
+ * nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  It stands for T(m + s c).  A group with a number that is not finite,
+ * or with a span that is not, is NaN.
+ *
+ * The memory is the caller's, 16-byte aligned, and the library keeps nothing of its own:
+ *   d_codes    (n_layers, 2: keys and values, n_sequences, n_kv_heads, max_tokens, head_dim / 8) 32-bit words; of a word's eight
+ *              numbers 2i lies at bit 4i and 2i + 1 at bit 16 + 4i
+ *   d_scales   (the same, head_dim / 32, 2) of type T: m and s
+ *   d_weights  (n_layers, n_sequences, n_kv_heads, max_tokens) fp32
+ *   d_places   (the same) int32
+ * Which tokens a sequence has is the caller's to know: a call is given, of each of its n sequences, the slot (no two the same), the
+ * tokens that it holds, the newest included, how many newest tokens the call is about, and the position of the first of those.
+ * Tensors of a call are (batch, heads, tokens, head_dim) with strides in elements (bs, hs, ts) that are multiples of 8 and bases that
+ * are 16-byte aligned; `most` is their number of tokens, and a sequence with fewer newest tokens has them at the end: rows before
+ * those are not read, and written as zeros.  Nothing but launches on `stream`: calls may be captured, and a replay does the same
+ * again for the same sequences and lengths. */
+typedef struct infllm_packed {
+  int32_t n_layers, n_kv_heads, head_dim, n_sequences, max_tokens, dtype, device, pad;
+  void *d_codes, *d_scales;
+  float* d_weights;
+  int32_t* d_places;
+} infllm_packed;
+typedef struct infllm_packed_seq {
+  int32_t slot, length, count, position;
+} infllm_packed_seq;
+/* A layer's keys and values of the newest tokens into the cache, their weights 0; q to d_q_out (batch, tokens, n_heads, head_dim).
+ * With d_cos / d_sin (table_len, head_dim / 2) keys and queries are rotated to the tokens' positions first.  q may be NULL. */
+int infllm_packed_write(const infllm_packed* c, int layer, const infllm_packed_seq* seqs, int n, int most, const void* d_k, int64_t k_bs,
+                        int64_t k_hs, int64_t k_ts, const void* d_v, int64_t v_bs, int64_t v_hs, int64_t v_ts, const void* d_q, int64_t q_bs,
+                        int64_t q_hs, int64_t q_ts, void* d_q_out, int n_heads, const float* d_cos, const float* d_sin, int64_t table_len,
+                        void* stream);
+/* What the cache holds of the newest tokens, in T: d_k and d_v (n_layers, batch, n_kv_heads, tokens, head_dim), layers from `layer` on. */
+int infllm_packed_values(const infllm_packed* c, int layer, int n_layers, const infllm_packed_seq* seqs, int n, int most, void* d_k,
+                         void* d_v, void* stream);
+/* Attention of the newest tokens: each sees its sequence's tokens up to itself.  d_out (batch, tokens, n_heads, head_dim), d_lse (batch,
+ * tokens, n_heads) fp32 log-sum-exp of the scores, or NULL; scale is finite and not negative.  Of the newest `weigh` tokens among those
+ * the attention probabilities are summed, over them and the query heads of a KV head, and a sequence's weights become decay * weight + that
+ * sum (decay 0: the weights are not read); weigh 0: they stay as they are.  d_work, 16-byte aligned, is the call's until it is done, of
+ * the size that infllm_packed_room gives for these arguments. */
+int infllm_packed_room(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int most, int n_heads, int weigh, int64_t* work_bytes);
+int infllm_packed_attend(const infllm_packed* c, int layer, const infllm_packed_seq* seqs, int n, int most, const void* d_q, int64_t q_bs,
+                         int64_t q_hs, int64_t q_ts, void* d_out, float* d_lse, int n_heads, float scale, int weigh, float decay,
+                         void* d_work, int64_t work_bytes, void* stream);
+/* Of every layer and KV head of each sequence of more than `budget` tokens, `budget` stay, in their order: the first `sink`, the newest
+ * `recent`, and of the others those of the largest weights (of equal ones the earlier; a NaN is the largest).  They close up, with their
+ * weights and places.  `into` NULL: in place; otherwise they, or all tokens of a sequence of no more than budget, go to slot into[i],
+ * which is none of the sequences', and these stay as they are.  (seqs[i].count and .position are not looked at.)  d_work, 16-byte
+ * aligned: n_layers * n * n_kv_heads * 4 * (the most tokens that stay of a sequence, rounded up to a multiple of 4) bytes. */
+int infllm_packed_evict(const infllm_packed* c, const infllm_packed_seq* seqs, int n, const int32_t* into, int64_t budget, int64_t sink,
+                        int64_t recent, void* d_work, int64_t work_bytes, void* stream);
+
 /* ----------------------------------------------------- host logic, GPU-free
  * The LRU table alone (context_manager.py:246-265, 495-515): dict-ordered ids with stamps.
  * Exposed so that the eviction order can be tested without a device. */

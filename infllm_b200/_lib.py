@@ -44,6 +44,12 @@ class Config(ctypes.Structure):
     ]
 
 
+class Packed(ctypes.Structure):
+    _fields_ = [("n_layers", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("n_sequences", c_int32), ("max_tokens", c_int32),
+                ("dtype", c_int32), ("device", c_int32), ("pad", c_int32),
+                ("d_codes", c_void_p), ("d_scales", c_void_p), ("d_weights", c_void_p), ("d_places", c_void_p)]
+
+
 class SinkWindow(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("d_q", "d_k", "d_v", "d_past_k", "d_past_v", "d_cache_k", "d_cache_v", "d_out",
                                         "d_scratch", "d_cos", "d_sin")] + \
@@ -220,6 +226,13 @@ SIGNATURES = {
     "infllm_page_batch_plan": (c_int, [c_void_p, c_int, POINTER(c_int64)]),
     "infllm_page_batch_attend": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_float,
                                          c_void_p, c_void_p]),
+    "infllm_packed_write": (c_int, [POINTER(Packed), c_int, c_void_p, c_int, c_int] + [c_void_p, c_int64, c_int64, c_int64] * 3 +
+                            [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "infllm_packed_values": (c_int, [POINTER(Packed), c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "infllm_packed_room": (c_int, [POINTER(Packed), c_void_p, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
+    "infllm_packed_attend": (c_int, [POINTER(Packed), c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                     c_int, c_float, c_int, c_float, c_void_p, c_int64, c_void_p]),
+    "infllm_packed_evict": (c_int, [POINTER(Packed), c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "infllm_lru_create": (c_int, [c_int, POINTER(c_void_p)]),
     "infllm_lru_destroy": (c_int, [c_void_p]),
     "infllm_lru_plan": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_int32), POINTER(c_int)]),

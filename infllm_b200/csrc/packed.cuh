@@ -1,0 +1,64 @@
+// A key/value cache in 4 bits (packed.cu, packed_attn.cu): what it holds, and how numbers come out of it.
+//
+// Of each 32 neighbouring numbers x of a row, in the cache's 16-bit type T: the least m, a step s = T((max x - m) / 15), and of each
+// number a code c = the nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  A number stands for T(m + s c): one fused
+// multiply-add in T, so every kernel has the same operands, whatever its tiles.
+// A word has eight codes, number 2i at bit 4i and number 2i + 1 at bit 16 + 4i: a shift and a mask by 0x000f000f give two neighbours,
+// and the low or the high halves of two rows' words, put together, give pairs of the same number of both rows.
+#pragma once
+#include <type_traits>
+
+#include "mma_common.cuh"
+#include "pages.cuh"
+
+namespace infllm {
+
+constexpr int kPackGroup = 32;  // numbers that share (m, s)
+
+// the layer's planes and the step between a sequence's heads; rows of a head lie one behind the other
+struct PackedPlanes {
+  const char* codes;   // keys; values `codes_v` behind them.  A row has kDim / 2 bytes
+  const char* scales;  // a row has kDim / 8 bytes: (m, s) of each group
+  int64_t codes_v, scales_v;
+  int32_t max_tokens, n_kv;
+  __device__ __forceinline__ int64_t row0(int slot, int hkv) const { return ((int64_t)slot * n_kv + hkv) * max_tokens; }
+};
+
+template <typename T>
+struct Codes {
+  using T2 = typename Act<T>::T2;
+  static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  // codes as the low bits of numbers whose last place is 1: 128 + c in bf16, 1024 + c in fp16
+  static constexpr uint32_t kBias = kBf16 ? 0x43004300u : 0x64006400u;
+  static __device__ __forceinline__ T2 as2(uint32_t x) { return *reinterpret_cast<T2*>(&x); }
+  static __device__ __forceinline__ uint32_t bits(T2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+  // the pair at bits 4i and 16 + 4i of w, with least numbers m2 and steps s2
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, int i, T2 m2, T2 s2) {
+    const T2 c = __hsub2(as2(((w >> (4 * i)) & 0x000f000fu) | kBias), as2(kBias));
+    return bits(__hfma2(c, s2, m2));
+  }
+  // (m, s) in one word: pairs (m, m) and (s, s)
+  static __device__ __forceinline__ T2 least2(uint32_t sc) { return as2(__byte_perm(sc, sc, 0x1010)); }
+  static __device__ __forceinline__ T2 step2(uint32_t sc) { return as2(__byte_perm(sc, sc, 0x3232)); }
+  // of two rows' words: pairs (m of a, m of b) and (s of a, s of b)
+  static __device__ __forceinline__ T2 least2(uint32_t a, uint32_t b) { return as2(__byte_perm(a, b, 0x5410)); }
+  static __device__ __forceinline__ T2 step2(uint32_t a, uint32_t b) { return as2(__byte_perm(a, b, 0x7632)); }
+  // whether (m, s) are not both finite: all exponent bits are set in one of them
+  static __device__ __forceinline__ bool odd(uint32_t sc) {
+    constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
+    return (sc & e) == e || (sc >> 16 & e) == e;
+  }
+};
+
+// a sequence of a launch
+struct PackedSeq {
+  int32_t slot, length, count, position;  // tokens, the newest included; the newest; the position of the first of those
+};
+static_assert(sizeof(PackedSeq) == sizeof(infllm_packed_seq), "");
+
+int packed_check(const infllm_packed* c, const char* what);
+int packed_check_seqs(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int most, const char* what);
+PackedPlanes packed_planes(const infllm_packed* c, int layer);
+inline int64_t packed_rows(const infllm_packed* c) { return (int64_t)c->n_sequences * c->n_kv_heads * c->max_tokens; }  // of a layer
+
+}  // namespace infllm

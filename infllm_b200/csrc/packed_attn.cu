@@ -1,0 +1,514 @@
+// Attention of a batch of sequences over the cache in 4 bits (packed.cuh), and the weights that it gives the cache's tokens.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij) / sum_j exp(s_ij),  s_ij = scale q_i . k_j,  over the keys j up to query i's place
+//   w_j = decay w_j + sum_i p_ij, over the counted queries of all query heads of a KV head
+//
+// Keys are cut into stretches, the parts of a row joined by their log-sum-exps,
+//   M = max_p lse_p,   o = sum_p 2^(lse_p - M) o_p / sum_p 2^(lse_p - M)   (logarithms to base 2).
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "decode_warp.cuh"
+#include "packed.cuh"
+
+namespace infllm {
+
+using namespace mma;
+
+constexpr int kAttnSeqs = 128;  // of a launch
+constexpr int kAttnWarps = 4, kAttnTile = 16;
+
+struct PackedAttnSeq {
+  int32_t slot, length, count;
+  int32_t unit0, chunks, keys;  // its first unit, stretches, and keys of a stretch: unit0 + row tile * chunks + stretch
+};
+
+struct PackedAttnParams {
+  PackedPlanes at;
+  const char* q;
+  int64_t q_bs, q_hs, q_ts;  // bytes
+  char* out;
+  float* lse;
+  float *part_o, *part_lse;  // 16 rows of each unit and KV head
+  float* row_lse;            // (batch, KV head, token, query head of the KV head), to base 2: of the counted rows' weights; null: none
+  float* weights;            // of the layer
+  int32_t group, most, batch, b0, weigh;
+  float scale_log2, decay;
+  PackedAttnSeq seq[kAttnSeqs];
+};
+
+// the launch's sequence that has unit u
+__device__ __forceinline__ int seq_of(const PackedAttnParams& P, int u) {
+  int lo = 0, hi = P.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (P.seq[mid].unit0 <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// --------------------------------------------------------------------------------------------------------- a warp's part
+// Groups of 16 keys against up to 16 rows, from global memory straight into the operands of the m16n8k16 products: a thread's codes of
+// a key are those of the 32 numbers of one (m, s) (kDim 128), its codes of a value an eighth of the row.
+template <typename T, int kDim, int kNt>  // kNt: tiles of eight rows
+struct PackedWarp {
+  static constexpr int kW = kDim / 32;  // words of a key, kDim / 4 numbers, that a thread has: as many of Q's 16-byte pieces
+  static constexpr int kH = kDim / 64;  // of a value, kDim / 8 numbers
+  using C = Codes<T>;
+  const char* from[kNt];
+  uint4 qf[kNt][kW];
+  int lim[kNt];
+
+  // the rows row0 + 0 .. 15 of a sequence's new tokens
+  __device__ __forceinline__ void rows(const PackedAttnParams& P, const PackedAttnSeq& S, int b, int hkv, int row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int x = 0; x < kNt; ++x) {
+      const int r = row0 + x * 8 + g, i = r / P.group, h = r - i * P.group;
+      lim[x] = 0, from[x] = nullptr;
+      if (i < S.count) {
+        lim[x] = S.length - S.count + i + 1;
+        from[x] = P.q + (int64_t)(P.b0 + b) * P.q_bs + (int64_t)(hkv * P.group + h) * P.q_hs + (int64_t)(P.most - S.count + i) * P.q_ts + t * (kDim / 2);
+      }
+    }
+  }
+  __device__ __forceinline__ void queries() {
+#pragma unroll
+    for (int x = 0; x < kNt; ++x)
+#pragma unroll
+      for (int j = 0; j < kW; ++j) qf[x][j] = from[x] ? __ldg(reinterpret_cast<const uint4*>(from[x] + j * 16)) : make_uint4(0, 0, 0, 0);
+  }
+
+  struct Key {  // rows nt * 8 + g
+    uint32_t w[2][kW], ms[2];
+  };
+  __device__ __forceinline__ static Key key(const char* codes, const char* scales, int nk) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    Key k;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const int r = min(nt * 8 + g, nk - 1);  // (what lies behind the last key is not read: it may not be a number, and 0 times that is none)
+      if (kDim == 128) {
+        const uint4 x = ld_stream16(codes + r * 64 + t * 16);
+        k.w[nt][0] = x.x, k.w[nt][1] = x.y, k.w[nt][2 % kW] = x.z, k.w[nt][3 % kW] = x.w;
+        k.ms[nt] = *reinterpret_cast<const uint32_t*>(scales + r * 16 + t * 4);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(codes + r * 32 + t * 8);
+        k.w[nt][0] = x.x, k.w[nt][1] = x.y;
+        k.ms[nt] = *reinterpret_cast<const uint32_t*>(scales + r * 8 + (t >> 1) * 4);
+      }
+    }
+    return k;
+  }
+  // scores of rows g (and 8 + g) by keys nt * 8 + 2t, + 1
+  __device__ __forceinline__ void scores(const Key& k, float (*s)[4]) const {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const auto m2 = C::least2(k.ms[nt]), s2 = C::step2(k.ms[nt]);
+      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        const uint32_t w = k.w[nt][j];
+        const uint32_t a0[4] = {qf[0][j].x, kNt > 1 ? qf[kNt - 1][j].x : 0u, qf[0][j].y, kNt > 1 ? qf[kNt - 1][j].y : 0u};
+        mma16816<T>(s[nt], a0, C::pair(w, 0, m2, s2), C::pair(w, 1, m2, s2));
+        const uint32_t a1[4] = {qf[0][j].z, kNt > 1 ? qf[kNt - 1][j].z : 0u, qf[0][j].w, kNt > 1 ? qf[kNt - 1][j].w : 0u};
+        mma16816<T>(s[nt], a1, C::pair(w, 2, m2, s2), C::pair(w, 3, m2, s2));
+      }
+    }
+  }
+
+  struct Value {  // rows 2t, 2t + 1, 2t + 8, 2t + 9: numbers g * kDim / 8 .. of each
+    uint32_t w[4][kH], ms[4];
+  };
+  __device__ __forceinline__ static Value value(const char* codes, const char* scales, int nk) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    Value v;
+#pragma unroll
+    for (int ki = 0; ki < 4; ++ki) {
+      const int r = min(2 * t + (ki & 1) + (ki >> 1) * 8, nk - 1);
+      if (kDim == 128) {
+        const uint2 x = *reinterpret_cast<const uint2*>(codes + r * 64 + g * 8);
+        v.w[ki][0] = x.x, v.w[ki][kH - 1] = x.y;
+        v.ms[ki] = *reinterpret_cast<const uint32_t*>(scales + r * 16 + (g >> 1) * 4);
+      } else {
+        v.w[ki][0] = *reinterpret_cast<const uint32_t*>(codes + r * 32 + g * 4);
+        v.ms[ki] = *reinterpret_cast<const uint32_t*>(scales + r * 8 + (g >> 2) * 4);
+      }
+    }
+    return v;
+  }
+};
+
+// --------------------------------------------------------------------------------------------------------- attention
+// Four warps share a stretch's groups of 16 keys and meet in shared memory.  P is two 16-bit numbers, p = hi + lo, so that an output's
+// only rounding is its own.
+template <typename T, int kDim, int kNt>
+__global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_kernel(const __grid_constant__ PackedAttnParams P) {
+  using W = PackedWarp<T, kDim, kNt>;
+  using C = Codes<T>;
+  constexpr int kTiles = 4 * W::kH, kPitch = kDim + 4;
+  __shared__ __align__(16) float sm_o[kAttnWarps][8 * kNt][kPitch];
+  __shared__ float sm_m[kAttnWarps][8 * kNt], sm_l[kAttnWarps][8 * kNt];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int unit = blockIdx.x, hkv = blockIdx.y, b = seq_of(P, unit);
+  const PackedAttnSeq S = P.seq[b];
+  const int tile = (unit - S.unit0) / S.chunks, key0 = (unit - S.unit0 - tile * S.chunks) * S.keys, row0 = tile * kAttnTile;
+  // (of the last row's keys: the others see no more)
+  const int last = S.length - S.count + min(S.count, (row0 + kAttnTile - 1) / P.group + 1), key1 = min(key0 + S.keys, last);
+  const int rows = min(8 * kNt, S.count * P.group - row0);
+  W w;
+  w.rows(P, S, b, hkv, row0);
+  w.queries();
+  const int least = S.length - S.count + row0 / P.group + 1;  // keys that every row sees
+  float ot[kTiles][kNt][4], m[kNt], l[kNt];  // O^T: [0], [1] = number g * kDim / 8 + 2i of rows 2t, 2t + 1; [2], [3] = the next one
+#pragma unroll
+  for (int x = 0; x < kNt; ++x) {
+    m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) ot[i][x][0] = ot[i][x][1] = ot[i][x][2] = ot[i][x][3] = 0.f;
+  }
+  const int64_t first = P.at.row0(S.slot, hkv);
+  const char* kc = P.at.codes + first * (kDim / 2);
+  const char* ks = P.at.scales + first * (kDim / 8);
+  const char* vc = kc + P.at.codes_v;
+  const char* vs = ks + P.at.scales_v;
+#pragma unroll 1
+  for (int j0 = key0 + warp * 16; j0 < key1; j0 += kAttnWarps * 16) {
+    const int nk = min(16, key1 - j0);
+    typename W::Key k = W::key(kc + (int64_t)j0 * (kDim / 2), ks + (int64_t)j0 * (kDim / 8), nk);
+    typename W::Value v = W::value(vc + (int64_t)j0 * (kDim / 2), vs + (int64_t)j0 * (kDim / 8), nk);
+    if (j0 + 16 > least) {
+      // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and its
+      // key is no number in its place, so that the rows that see it still become none.
+      uint32_t bad = 0;
+#pragma unroll
+      for (int ki = 0; ki < 4; ++ki) {
+        const bool odd = C::odd(v.ms[ki]);
+        if (odd) v.ms[ki] = 0;
+        const uint32_t any = __ballot_sync(0xffffffffu, odd);  // of key 2t + .. in every lane with that t
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+          if (any & (0x11111111u << tt)) bad |= 1u << (2 * tt + (ki & 1) + (ki >> 1) * 8);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+        if (bad >> (nt * 8 + g) & 1) k.ms[nt] = 0x7fff7fffu;
+    }
+    float s[2][4];
+    w.scores(k, s);
+    uint32_t hi[kNt][2], lo[kNt][2];
+#pragma unroll
+    for (int x = 0; x < kNt; ++x) {  // row x * 8 + g: keys nt * 8 + 2t + e
+      float p[4], mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = j0 + (e >> 1) * 8 + 2 * t + (e & 1);
+        p[e] = key < min(w.lim[x], key1) ? s[e >> 1][x * 2 + (e & 1)] * P.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, p[e]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[x], mx), ms = mn == -INFINITY ? 0.f : mn;
+      const float al = exp2f(m[x] - ms);
+      m[x] = mn;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = exp2f(p[e] - ms);
+      l[x] = l[x] * al + (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        typename Act<T>::T2 h = Act<T>::from_f2(p[2 * e], p[2 * e + 1]);
+        hi[x][e] = *reinterpret_cast<uint32_t*>(&h);
+        const float2 f = Act<T>::to_f2(h);
+        lo[x][e] = pack2<T>(p[2 * e] - f.x, p[2 * e + 1] - f.y);
+      }
+      if (__any_sync(0xffffffffu, al != 1.f)) {
+        // this thread's columns of O^T are rows 2t and 2t + 1
+        const float a0 = __shfl_sync(0xffffffffu, al, (2 * t) * 4), a1 = __shfl_sync(0xffffffffu, al, (2 * t + 1) * 4);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) ot[i][x][0] *= a0, ot[i][x][1] *= a1, ot[i][x][2] *= a0, ot[i][x][3] *= a1;
+      }
+    }
+    // A operands: numbers of keys 2t, 2t + 1 and of 2t + 8, 2t + 9
+    const auto m01 = C::least2(v.ms[0], v.ms[1]), s01 = C::step2(v.ms[0], v.ms[1]);
+    const auto m23 = C::least2(v.ms[2], v.ms[3]), s23 = C::step2(v.ms[2], v.ms[3]);
+#pragma unroll
+    for (int j = 0; j < W::kH; ++j) {
+      const uint32_t e01 = __byte_perm(v.w[0][j], v.w[1][j], 0x5410), o01 = __byte_perm(v.w[0][j], v.w[1][j], 0x7632);
+      const uint32_t e23 = __byte_perm(v.w[2][j], v.w[3][j], 0x5410), o23 = __byte_perm(v.w[2][j], v.w[3][j], 0x7632);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a[4] = {C::pair(e01, i, m01, s01), C::pair(o01, i, m01, s01), C::pair(e23, i, m23, s23), C::pair(o23, i, m23, s23)};
+#pragma unroll
+        for (int x = 0; x < kNt; ++x) {
+          mma16816<T>(ot[j * 4 + i][x], a, hi[x][0], hi[x][1]);
+          mma16816<T>(ot[j * 4 + i][x], a, lo[x][0], lo[x][1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < kNt; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    if (l[x] != l[x] && m[x] == -INFINITY) m[x] = 0.f;  // (scores that are no numbers are not seen by the maximum)
+    if (t == 0) sm_m[warp][x * 8 + g] = m[x], sm_l[warp][x * 8 + g] = l[x];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<float2*>(&sm_o[warp][x * 8 + 2 * t + e][g * (kDim / 8) + 2 * i]) = make_float2(ot[i][x][e], ot[i][x][2 + e]);
+  }
+  __syncthreads();
+  for (int idx = tid; idx < rows * (kDim / 2); idx += kAttnWarps * 32) {  // two neighbouring numbers each
+    const int r = idx / (kDim / 2), d = idx % (kDim / 2) * 2;
+    float mx = sm_m[0][r];
+#pragma unroll
+    for (int y = 1; y < kAttnWarps; ++y) mx = fmaxf(mx, sm_m[y][r]);
+    float den = 0.f, n0 = 0.f, n1 = 0.f;
+    if (mx != -INFINITY) {
+#pragma unroll
+      for (int y = 0; y < kAttnWarps; ++y) {
+        const float wt = exp2f(sm_m[y][r] - mx);
+        den = fmaf(wt, sm_l[y][r], den);
+        n0 = fmaf(wt, sm_o[y][r][d], n0);
+        n1 = fmaf(wt, sm_o[y][r][d + 1], n1);
+      }
+      n0 /= den, n1 /= den;
+    }
+    const float lse = mx == -INFINITY ? -INFINITY : mx + log2f(den);
+    if (S.chunks > 1) {
+      const int64_t pr = ((int64_t)unit * P.at.n_kv + hkv) * kAttnTile + r;
+      *reinterpret_cast<float2*>(P.part_o + pr * kDim + d) = make_float2(n0, n1);
+      if (d == 0) P.part_lse[pr] = lse;
+    } else {
+      const int i = (row0 + r) / P.group, h = row0 + r - i * P.group;
+      const int64_t orow = ((int64_t)(P.b0 + b) * P.most + P.most - S.count + i) * (P.at.n_kv * P.group) + hkv * P.group + h;
+      *reinterpret_cast<uint32_t*>(P.out + (orow * kDim + d) * 2) = pack2<T>(n0, n1);
+      if (P.lse && d == 0) P.lse[orow] = lse * (1.f / kLog2e);
+      if (P.row_lse && d == 0) P.row_lse[((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group + row0 + r] = lse;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- the join
+// A warp per query head and token; rows without a token become zeros.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ PackedAttnParams P) {
+  constexpr int kPer = kDim / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = P.at.n_kv * P.group;
+  const int64_t at = (int64_t)blockIdx.x * 8 + warp;
+  if (at >= (int64_t)P.batch * P.most * heads) return;
+  const int h = (int)(at % heads), i = (int)(at / heads % P.most), b = (int)(at / heads / P.most), hkv = h / P.group;
+  const PackedAttnSeq S = P.seq[b];
+  const int tok = i - (P.most - S.count);
+  if (tok >= 0 && S.chunks <= 1) return;  // whole already
+  const int r = tok * P.group + h % P.group;
+  float m = -INFINITY, l = 0.f, acc[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+  const int64_t step = (int64_t)P.at.n_kv * kAttnTile;
+  const int64_t first = tok < 0 ? 0 : ((int64_t)(S.unit0 + r / kAttnTile * S.chunks) * P.at.n_kv + hkv) * kAttnTile + r % kAttnTile;
+  for (int c = 0; tok >= 0 && c < S.chunks; ++c) {
+    const int64_t row = first + c * step;
+    const float lse = P.part_lse[row];
+    if (lse == -INFINITY) continue;
+    const float mx = fmaxf(m, lse), a = exp2f(m - mx), w = exp2f(lse - mx);
+    l = l * a + w;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * a + w * P.part_o[row * kDim + lane * kPer + k];
+    m = mx;
+  }
+  const int64_t orow = ((int64_t)(P.b0 + b) * P.most + i) * heads + h;
+  const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
+  uint32_t* to = reinterpret_cast<uint32_t*>(P.out + (orow * kDim + lane * kPer) * 2);
+#pragma unroll
+  for (int k = 0; k < kPer; k += 2) to[k / 2] = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
+  const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
+  if (lane == 0 && P.lse) P.lse[orow] = lse * (1.f / kLog2e);
+  if (lane == 0 && P.row_lse && tok >= 0) P.row_lse[((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group + r] = lse;
+}
+
+// --------------------------------------------------------------------------------------------------------- the weights
+// A warp has a group of 16 keys, forms its scores with all counted rows again and adds up what they give each key.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(128) packed_weigh_kernel(const __grid_constant__ PackedAttnParams P) {
+  using W = PackedWarp<T, kDim, 2>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int b = blockIdx.z, hkv = blockIdx.y, j0 = ((int)blockIdx.x * 4 + (threadIdx.x >> 5)) * 16;
+  const PackedAttnSeq S = P.seq[b];
+  if (S.count == 0 || j0 >= S.length) return;
+  const int nk = min(16, S.length - j0);
+  const int64_t first = P.at.row0(S.slot, hkv) + j0;
+  const typename W::Key k = W::key(P.at.codes + first * (kDim / 2), P.at.scales + first * (kDim / 8), nk);
+  const float* row_lse = P.row_lse + ((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group;
+  // the rows from the first counted token, or the first that sees one of the keys, on
+  const int from = max(S.count - min(P.weigh, S.count), j0 - (S.length - S.count)) * P.group;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int row0 = from; row0 < S.count * P.group; row0 += kAttnTile) {
+    W w;
+    w.rows(P, S, b, hkv, row0);
+    w.queries();
+    float s[2][4];
+    w.scores(k, s);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = row0 + x * 8 + g;
+      if (r >= S.count * P.group) continue;
+      const float lse = row_lse[r];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = j0 + (e >> 1) * 8 + 2 * t + (e & 1);
+        if (key < w.lim[x]) sum[e] += exp2f(s[e >> 1][x * 2 + (e & 1)] * P.scale_log2 - lse);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+    const int at = (e >> 1) * 8 + 2 * t + (e & 1);
+    if (g == 0 && at < nk) P.weights[first + at] = P.decay == 0.f ? sum[e] : P.decay * P.weights[first + at] + sum[e];
+  }
+}
+
+namespace {
+
+// Keys of a unit's stretch, so that all units run in about one, two or some waves of as many as the machine holds
+int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group, int64_t resident) {
+  constexpr double kGroup = 1., kUnit = 5.;  // microseconds of a warp's 16 keys, and of a unit besides
+  int64_t most = 64;
+  for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, ceil_div(seqs[i].length, 64) * 64);
+  auto units = [&](int64_t keys) {
+    int64_t u = 0;
+    for (int i = 0; i < n; ++i) u += ceil_div((int64_t)seqs[i].count * group, kAttnTile) * ceil_div(seqs[i].length, keys);
+    return u * c->n_kv_heads;
+  };
+  int64_t best = most;
+  double least = 1e300;
+  for (int waves = 1; waves <= 6; ++waves) {
+    int64_t lo = 1, hi = most / 64;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (units(mid * 64) <= waves * resident) hi = mid;
+      else lo = mid + 1;
+    }
+    const double cost = (double)ceil_div(units(lo * 64), resident) * ((double)lo * kGroup + kUnit);
+    if (cost < least) least = cost, best = lo * 64;
+  }
+  return best;
+}
+
+struct Plan {
+  int64_t units = 0, rows = 0;  // the most of a launch; all rows
+  int64_t keys[64];
+  int64_t bytes(const infllm_packed* c, int n, int most, int n_heads, int weigh) const {
+    int64_t b = ceil_div(units * c->n_kv_heads * kAttnTile * (c->head_dim + 1) * 4, 16) * 16;
+    return b + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
+  }
+};
+
+// the units of the launch of seqs[0 .. n - 1]; fills `to` where it is given
+int64_t lay_out(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int n_heads, PackedAttnSeq* to, bool* join) {
+  const int group = n_heads / c->n_kv_heads;
+  const int64_t keys = chunk_keys(c, seqs, n, group, 148 * 4);
+  int64_t u = 0;
+  for (int i = 0; i < n; ++i) {
+    const int64_t chunks = std::max<int64_t>(1, ceil_div(seqs[i].length, keys)), tiles = ceil_div((int64_t)seqs[i].count * group, kAttnTile);
+    if (to) to[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)std::min<int64_t>(u, INT_MAX), (int32_t)chunks, (int32_t)keys};
+    if (join && chunks > 1 && seqs[i].count > 0) *join = true;
+    u += chunks * tiles;
+  }
+  return u;
+}
+
+int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int most, int n_heads, int weigh, int64_t* bytes, const char* what) {
+  INFLLM_TRY(packed_check(c, what));
+  INFLLM_TRY(packed_check_seqs(c, seqs, n, most, what));
+  if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads > 1 << 16) return fail(INFLLM_E_BADARG, "%s: %d query heads over %d KV heads", what, n_heads, c->n_kv_heads);
+  if (weigh < 0) return fail(INFLLM_E_BADARG, "%s: the weights of %d tokens", what, weigh);
+  if ((int64_t)most * n_heads > INT_MAX / 4) return fail(INFLLM_E_BADARG, "%s: %d tokens of %d heads", what, most, n_heads);
+  int64_t units = 0;
+  for (int b0 = 0; b0 < n; b0 += kAttnSeqs) units = std::max(units, lay_out(c, seqs + b0, std::min(n - b0, kAttnSeqs), n_heads, nullptr, nullptr));
+  if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
+  Plan p;
+  p.units = units;
+  *bytes = p.bytes(c, n, most, n_heads, weigh);
+  return INFLLM_OK;
+}
+
+}  // namespace
+
+}  // namespace infllm
+
+using namespace infllm;
+
+extern "C" int infllm_packed_room(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int most, int n_heads, int weigh, int64_t* work_bytes) {
+  return guarded("packed_room", [&]() -> int {
+    if (!work_bytes) return fail(INFLLM_E_BADARG, "packed_room: null pointer");
+    return check_attend(c, seqs, n, most, n_heads, weigh, work_bytes, "packed_room");
+  });
+}
+
+extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const infllm_packed_seq* seqs, int n, int most, const void* d_q,
+                                    int64_t q_bs, int64_t q_hs, int64_t q_ts, void* d_out, float* d_lse, int n_heads, float scale, int weigh,
+                                    float decay, void* d_work, int64_t work_bytes, void* stream) {
+  return guarded("packed_attend", [&]() -> int {
+    int64_t bytes = 0;
+    INFLLM_TRY(check_attend(c, seqs, n, most, n_heads, weigh, &bytes, "packed_attend"));
+    if (layer < 0 || layer >= c->n_layers) return fail(INFLLM_E_BADARG, "packed_attend: layer %d of %d", layer, c->n_layers);
+    if (!(scale >= 0.f) || !std::isfinite(scale * kLog2e)) return fail(INFLLM_E_BADARG, "packed_attend: a scale of %g", (double)scale);
+    if (!(decay >= 0.f) || !std::isfinite(decay)) return fail(INFLLM_E_BADARG, "packed_attend: a decay of %g", (double)decay);
+    if (n == 0 || most == 0) return INFLLM_OK;
+    if (!d_q || !d_out) return fail(INFLLM_E_BADARG, "packed_attend: null pointer");
+    if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 || (q_bs | q_hs | q_ts) % 8) return fail(INFLLM_E_BADARG, "packed_attend: rows must be 16-byte aligned");
+    if (work_bytes < bytes || (bytes > 0 && (!d_work || (uintptr_t)d_work % 16)))
+      return fail(INFLLM_E_BADARG, "packed_attend: a workspace of %lld bytes, 16-byte aligned", (long long)bytes);
+    DeviceScope scope(c->device);
+    cudaStream_t s = (cudaStream_t)stream;
+    PackedAttnParams P;
+    P.at = packed_planes(c, layer);
+    P.q = (const char*)d_q, P.q_bs = q_bs * 2, P.q_hs = q_hs * 2, P.q_ts = q_ts * 2;
+    P.out = (char*)d_out, P.lse = d_lse;
+    P.row_lse = weigh > 0 ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * 4) : nullptr;
+    P.weights = c->d_weights + layer * packed_rows(c);
+    P.group = n_heads / c->n_kv_heads, P.most = most, P.weigh = weigh;
+    P.scale_log2 = scale * kLog2e, P.decay = decay;
+    for (P.b0 = 0; P.b0 < n; P.b0 += kAttnSeqs) {
+      const int m = std::min(n - P.b0, kAttnSeqs);
+      const infllm_packed_seq* mine = seqs + P.b0;
+      P.batch = m;
+      bool join = false;
+      const int64_t units = lay_out(c, mine, m, n_heads, P.seq, &join);
+      int64_t longest = 0;
+      int counts = 0;
+      for (int i = 0; i < m; ++i) {
+        longest = std::max<int64_t>(longest, mine[i].length), counts = std::max(counts, mine[i].count);
+        join = join || mine[i].count < most;  // (rows without a token)
+      }
+      P.part_o = (float*)d_work, P.part_lse = P.part_o + units * c->n_kv_heads * kAttnTile * c->head_dim;
+      INFLLM_DISPATCH_DTYPE(c->dtype, T, {
+        if (units > 0) {
+          const bool few = counts * P.group <= 8;
+          auto kern = c->head_dim == 128 ? (few ? packed_rows_kernel<T, 128, 1> : packed_rows_kernel<T, 128, 2>)
+                                         : (few ? packed_rows_kernel<T, 64, 1> : packed_rows_kernel<T, 64, 2>);
+          kern<<<dim3((unsigned)units, c->n_kv_heads), kAttnWarps * 32, 0, s>>>(P);
+          INFLLM_LAUNCH_OK("packed_rows_kernel");
+        }
+        if (join) {
+          auto kern = c->head_dim == 128 ? packed_join_kernel<T, 128> : packed_join_kernel<T, 64>;
+          kern<<<(unsigned)ceil_div((int64_t)m * most * n_heads, 8), 256, 0, s>>>(P);
+          INFLLM_LAUNCH_OK("packed_join_kernel");
+        }
+        if (weigh > 0 && units > 0) {
+          auto kern = c->head_dim == 128 ? packed_weigh_kernel<T, 128> : packed_weigh_kernel<T, 64>;
+          kern<<<dim3((unsigned)ceil_div(longest, 64), c->n_kv_heads, m), 128, 0, s>>>(P);
+          INFLLM_LAUNCH_OK("packed_weigh_kernel");
+        }
+      });
+    }
+    return INFLLM_OK;
+  });
+}
