@@ -6,48 +6,20 @@
 // Keys are cut into stretches, the parts of a row joined by their log-sum-exps,
 //   M = max_p lse_p,   o = sum_p 2^(lse_p - M) o_p / sum_p 2^(lse_p - M)   (logarithms to base 2).
 #include <algorithm>
+#include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
+#include "attn_tc.cuh"
 #include "decode_warp.cuh"
-#include "packed.cuh"
+#include "packed_attn.cuh"
 
 namespace infllm {
 
 using namespace mma;
 
-constexpr int kAttnSeqs = 128;  // of a launch
 constexpr int kAttnWarps = 4, kAttnTile = 16;
-
-struct PackedAttnSeq {
-  int32_t slot, length, count;
-  int32_t unit0, chunks, keys;  // its first unit, stretches, and keys of a stretch: unit0 + row tile * chunks + stretch
-};
-
-struct PackedAttnParams {
-  PackedPlanes at;
-  const char* q;
-  int64_t q_bs, q_hs, q_ts;  // bytes
-  char* out;
-  float* lse;
-  float *part_o, *part_lse;  // 16 rows of each unit and KV head
-  float* row_lse;            // (batch, KV head, token, query head of the KV head), to base 2: of the counted rows' weights; null: none
-  float* weights;            // of the layer
-  int32_t group, most, batch, b0, weigh;
-  float scale_log2, decay;
-  PackedAttnSeq seq[kAttnSeqs];
-};
-
-// the launch's sequence that has unit u
-__device__ __forceinline__ int seq_of(const PackedAttnParams& P, int u) {
-  int lo = 0, hi = P.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (P.seq[mid].unit0 <= u) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
 
 // --------------------------------------------------------------------------------------------------------- a warp's part
 // Groups of 16 keys against up to 16 rows, from global memory straight into the operands of the m16n8k16 products: a thread's codes of
@@ -160,6 +132,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
   const int rows = min(8 * kNt, S.count * P.group - row0);
   W w;
   w.rows(P, S, b, hkv, row0);
+  chain_enter();
   w.queries();
   const int least = S.length - S.count + row0 / P.group + 1;  // keys that every row sees
   float ot[kTiles][kNt][4], m[kNt], l[kNt];  // O^T: [0], [1] = number g * kDim / 8 + 2i of rows 2t, 2t + 1; [2], [3] = the next one
@@ -293,33 +266,123 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
 }
 
 // ----------------------------------------------------------------------------------------------------------- the join
-// A warp per query head and token; rows without a token become zeros.
-template <typename T, int kDim>
-__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ PackedAttnParams P) {
-  constexpr int kPer = kDim / 32;
+// kWarps warps per query head and token share a row's parts, four of them on their way at once; rows without a token become zeros.
+template <bool kTc>
+struct JoinParams {
+  using type = PackedAttnParams;
+  static __device__ __forceinline__ const PackedAttnParams& attn(const type& p) { return p; }
+};
+template <>
+struct JoinParams<true> {
+  using type = PackedTcParams;
+  static __device__ __forceinline__ const PackedAttnParams& attn(const type& p) { return p.a; }
+};
+
+// the last block whose stretch begins at or before (unit, tile)
+__device__ __forceinline__ int block_of(const PackedTcParams& P, int u, int t) {
+  int lo = 0, hi = P.n_ctas - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (P.start[mid].x < u || (P.start[mid].x == u && P.start[mid].y <= t)) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T, int kDim, int kWarps, bool kTc>
+__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ typename JoinParams<kTc>::type All) {
+  constexpr int kPer = kDim / 32, kRows = 8 / kWarps, kAhead = 4;
+  __shared__ float sm[8][kDim + 4];
+  const PackedAttnParams& P = JoinParams<kTc>::attn(All);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = P.at.n_kv * P.group;
-  const int64_t at = (int64_t)blockIdx.x * 8 + warp;
-  if (at >= (int64_t)P.batch * P.most * heads) return;
-  const int h = (int)(at % heads), i = (int)(at / heads % P.most), b = (int)(at / heads / P.most), hkv = h / P.group;
+  const int64_t at = (int64_t)blockIdx.x * kRows + warp / kWarps;
+  const bool in = at < (int64_t)P.batch * P.most * heads;
+  const int h = in ? (int)(at % heads) : 0, i = in ? (int)(at / heads % P.most) : 0, b = in ? (int)(at / heads / P.most) : 0, hkv = h / P.group;
   const PackedAttnSeq S = P.seq[b];
-  const int tok = i - (P.most - S.count);
-  if (tok >= 0 && S.chunks <= 1) return;  // whole already
-  const int r = tok * P.group + h % P.group;
+  const int tok = i - (P.most - S.count), r = tok * P.group + h % P.group;
+  int parts = 0, block0 = 0, unit = 0;
+  bool whole = false;
+  if (in && tok >= 0) {
+    if constexpr (kTc) {
+      const int block = r / kBlockRows;
+      unit = S.unit0 + hkv * S.chunks + block;
+      block0 = block_of(All, unit, 0);
+      parts = block_of(All, unit, tiles_of(S, P.group, block) - 1) - block0 + 1;
+    } else {
+      parts = S.chunks;
+    }
+    whole = parts == 1;  // written by the unit that had all of it
+  }
+  auto row_of = [&](int c) -> int64_t {
+    if constexpr (kTc) {
+      // a block's first unit has its first slot, its last one the second
+      const int2 s = All.start[block0 + c];
+      return (int64_t)(2 * (block0 + c) + (s.x < unit)) * kBlockRows + r % kBlockRows;
+    } else {
+      return ((int64_t)(S.unit0 + r / kAttnTile * S.chunks + c) * P.at.n_kv + hkv) * kAttnTile + r % kAttnTile;
+    }
+  };
+  chain_enter();
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  const int64_t step = (int64_t)P.at.n_kv * kAttnTile;
-  const int64_t first = tok < 0 ? 0 : ((int64_t)(S.unit0 + r / kAttnTile * S.chunks) * P.at.n_kv + hkv) * kAttnTile + r % kAttnTile;
-  for (int c = 0; tok >= 0 && c < S.chunks; ++c) {
-    const int64_t row = first + c * step;
-    const float lse = P.part_lse[row];
-    if (lse == -INFINITY) continue;
-    const float mx = fmaxf(m, lse), a = exp2f(m - mx), w = exp2f(lse - mx);
-    l = l * a + w;
+  if (!whole) {
+    for (int c0 = warp % kWarps; c0 < parts; c0 += kWarps * kAhead) {
+      float lse[kAhead], v[kAhead][kPer];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * a + w * P.part_o[row * kDim + lane * kPer + k];
+      for (int e = 0; e < kAhead; ++e) {
+        const int c = c0 + e * kWarps;
+        lse[e] = -INFINITY;
+        if (c >= parts) continue;
+        const int64_t row = row_of(c);
+        lse[e] = P.part_lse[row];
+        // (partial rows of the tensor-core kernel lie in blocks of 32, four columns of all of them side by side)
+        const float* o = P.part_o + (kTc ? (row & ~(int64_t)31) * kDim + (lane * kPer / 4) * 128 + (row & 31) * 4 + lane * kPer % 4 : row * kDim + lane * kPer);
+        if (kPer == 4) *reinterpret_cast<float4*>(v[e]) = *reinterpret_cast<const float4*>(o);
+        else *reinterpret_cast<float2*>(v[e]) = *reinterpret_cast<const float2*>(o);
+      }
+      float mx = m;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) mx = fmaxf(mx, lse[e]);
+      const float ref = mx == -INFINITY ? 0.f : mx;  // (a part that is no number is not seen by the maximum)
+      const float a = exp2f(m - ref);
+      l *= a;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] *= a;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        if (lse[e] == -INFINITY) continue;
+        const float w = exp2f(lse[e] - ref);
+        l += w;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(w, v[e][k], acc[k]);
+      }
+      m = mx;
+    }
+  }
+  if (kWarps > 1) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) sm[warp][lane * kPer + k] = acc[k];
+    if (lane == 0) sm[warp][kDim] = m, sm[warp][kDim + 1] = l;
+    __syncthreads();
+    if (warp % kWarps) return;
+    float mx = m;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[warp + w][kDim]);
+    const float ms = mx == -INFINITY ? 0.f : mx, a = exp2f(m - ms);
+    l *= a;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) acc[k] *= a;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      const float wt = exp2f(sm[warp + w][kDim] - ms);
+      l = fmaf(wt, sm[warp + w][kDim + 1], l);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] = fmaf(wt, sm[warp + w][lane * kPer + k], acc[k]);
+    }
     m = mx;
   }
+  if (!in || whole) return;
   const int64_t orow = ((int64_t)(P.b0 + b) * P.most + i) * heads + h;
   const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
   uint32_t* to = reinterpret_cast<uint32_t*>(P.out + (orow * kDim + lane * kPer) * 2);
@@ -330,6 +393,19 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
   if (lane == 0 && P.row_lse && tok >= 0) P.row_lse[((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group + r] = lse;
 }
 
+template <typename T, int kDim, bool kTc>
+static int join_launch(const typename JoinParams<kTc>::type& P, const PackedAttnParams& A, int n_sm, cudaStream_t s) {
+  // as many warps to a row as one wave has room for
+  const int64_t rows = (int64_t)A.batch * A.most * A.at.n_kv * A.group, warps = n_sm * 32 / std::max<int64_t>(rows, 1);
+  auto launch = [&](auto kern, int per_row) { return launch_chained(kern, dim3((unsigned)ceil_div(rows * per_row, 8)), dim3(256), 0, s, P); };
+  if (warps >= 8) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 8, kTc>, 8));
+  else if (warps >= 4) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 4, kTc>, 4));
+  else if (warps >= 2) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 2, kTc>, 2));
+  else INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 1, kTc>, 1));
+  INFLLM_LAUNCH_OK("packed_join_kernel");
+  return INFLLM_OK;
+}
+
 // --------------------------------------------------------------------------------------------------------- the weights
 // A warp has a group of 16 keys, forms its scores with all counted rows again and adds up what they give each key.
 template <typename T, int kDim>
@@ -338,6 +414,7 @@ __global__ void __launch_bounds__(128) packed_weigh_kernel(const __grid_constant
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.z, hkv = blockIdx.y, j0 = ((int)blockIdx.x * 4 + (threadIdx.x >> 5)) * 16;
   const PackedAttnSeq S = P.seq[b];
+  chain_enter();
   if (S.count == 0 || j0 >= S.length) return;
   const int nk = min(16, S.length - j0);
   const int64_t first = P.at.row0(S.slot, hkv) + j0;
@@ -401,27 +478,87 @@ int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n,
   return best;
 }
 
-struct Plan {
-  int64_t units = 0, rows = 0;  // the most of a launch; all rows
-  int64_t keys[64];
-  int64_t bytes(const infllm_packed* c, int n, int most, int n_heads, int weigh) const {
-    int64_t b = ceil_div(units * c->n_kv_heads * kAttnTile * (c->head_dim + 1) * 4, 16) * 16;
-    return b + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
+// multiprocessors of a device (of a B200 where there is none: sizes are worked out without one, too)
+int sm_count(int device) {
+  static std::atomic<int> known[64];
+  if (device < 0 || device >= 64) return 148;
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+      cudaGetLastError();
+      return 148;
+    }
+    n = std::min(n, kMaxSms);
+    known[device].store(n, std::memory_order_relaxed);
   }
-};
+  return n;
+}
 
-// the units of the launch of seqs[0 .. n - 1]; fills `to` where it is given
-int64_t lay_out(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int n_heads, PackedAttnSeq* to, bool* join) {
-  const int group = n_heads / c->n_kv_heads;
-  const int64_t keys = chunk_keys(c, seqs, n, group, 148 * 4);
+// Work, in half microseconds
+constexpr int64_t kUnitWork = 8;   // of a unit of many rows besides its tiles
+constexpr int64_t kBlockWork = 24;  // worth a block
+int64_t tile_work(int64_t rows) { return rows > 128 ? 4 : 2; }  // of 128 keys
+
+// whether a call goes to the tensor cores: up to two tiles of rows, keys are read once or twice by the kernel of few rows
+bool many_rows(const infllm_packed_seq* seqs, int n, int group) {
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, (int64_t)seqs[i].count * group);
+  return most > 2 * kAttnTile;
+}
+
+// the units of the launch of seqs[0 .. n - 1] for few rows
+int64_t lay_out_few(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group, int n_sm, PackedAttnSeq* to, bool* join) {
+  const int64_t keys = chunk_keys(c, seqs, n, group, n_sm * 4);
   int64_t u = 0;
   for (int i = 0; i < n; ++i) {
     const int64_t chunks = std::max<int64_t>(1, ceil_div(seqs[i].length, keys)), tiles = ceil_div((int64_t)seqs[i].count * group, kAttnTile);
-    if (to) to[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)std::min<int64_t>(u, INT_MAX), (int32_t)chunks, (int32_t)keys};
-    if (join && chunks > 1 && seqs[i].count > 0) *join = true;
+    to[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)std::min<int64_t>(u, INT_MAX), (int32_t)chunks, (int32_t)keys};
+    if (chunks > 1 && seqs[i].count > 0) *join = true;
     u += chunks * tiles;
   }
   return u;
+}
+
+// the same for many rows: units are dealt out to blocks, and cut, so that all have about the same work
+int lay_out_many(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group, int n_sm, PackedAttnSeq* to, int2* start, int* n_ctas, bool* join) {
+  int64_t u = 0, work = 0;
+  auto rows_of = [&](int i, int block) { return std::min<int64_t>(kBlockRows, (int64_t)seqs[i].count * group - (int64_t)block * kBlockRows); };
+  for (int i = 0; i < n; ++i) {
+    const int64_t blocks = ceil_div((int64_t)seqs[i].count * group, kBlockRows);
+    to[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)u, (int32_t)std::max<int64_t>(blocks, 1), 0};
+    u += blocks * c->n_kv_heads;
+    if (u > INT_MAX) return fail(INFLLM_E_BADARG, "packed_attend: %lld units of work", (long long)u);
+    for (int x = 0; x < (int)blocks; ++x) work += c->n_kv_heads * (kUnitWork + tile_work(rows_of(i, x)) * tiles_of(to[i], group, x));
+  }
+  // (a cut costs a unit's start; where that was too little, so that the last block has more than the others, shares grow)
+  int64_t share = std::max(ceil_div(work, n_sm) + kUnitWork, kBlockWork), left = 0;
+  int ctas = 0;
+  for (int tries = 0; tries < 20; ++tries, share += ceil_div(share, 16)) {
+    auto begin = [&](int64_t unit, int64_t tile) {
+      start[ctas++] = make_int2((int)unit, (int)tile);
+      left = share;
+    };
+    ctas = 0, left = 0, u = 0;
+    for (int i = 0; i < n; ++i)
+      for (int h = 0; h < c->n_kv_heads; ++h)
+        for (int x = 0; seqs[i].count > 0 && x < to[i].chunks; ++x, ++u) {
+          const int64_t tiles = tiles_of(to[i], group, x), each = tile_work(rows_of(i, x));
+          int64_t at = 0;
+          while (at < tiles) {
+            // short ends stay where they are
+            if (ctas == 0 || (left < kUnitWork + 4 * each && left < kUnitWork + (tiles - at) * each && ctas < n_sm)) begin(u, at);
+            int64_t take = tiles - at;
+            if (ctas < n_sm && kUnitWork + take * each > left + 2 * each) take = std::max<int64_t>(1, std::min(take, (left - kUnitWork) / each));
+            left -= kUnitWork + take * each;
+            if (at > 0 || take < tiles) *join = true;
+            at += take;
+          }
+        }
+    if (left > -share / 16 - 8) break;
+  }
+  start[ctas] = make_int2((int)u, 0);
+  *n_ctas = ctas;
+  return INFLLM_OK;
 }
 
 int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int most, int n_heads, int weigh, int64_t* bytes, const char* what) {
@@ -430,13 +567,45 @@ int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, i
   if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads > 1 << 16) return fail(INFLLM_E_BADARG, "%s: %d query heads over %d KV heads", what, n_heads, c->n_kv_heads);
   if (weigh < 0) return fail(INFLLM_E_BADARG, "%s: the weights of %d tokens", what, weigh);
   if ((int64_t)most * n_heads > INT_MAX / 4) return fail(INFLLM_E_BADARG, "%s: %d tokens of %d heads", what, most, n_heads);
-  int64_t units = 0;
-  for (int b0 = 0; b0 < n; b0 += kAttnSeqs) units = std::max(units, lay_out(c, seqs + b0, std::min(n - b0, kAttnSeqs), n_heads, nullptr, nullptr));
-  if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
-  Plan p;
-  p.units = units;
-  *bytes = p.bytes(c, n, most, n_heads, weigh);
+  *bytes = 0;
+  if (n == 0 || most == 0) return INFLLM_OK;
+  const int group = n_heads / c->n_kv_heads;
+  const int n_sm = sm_count(c->device);
+  int64_t rows = many_rows(seqs, n, group) ? 2 * n_sm * kBlockRows : 0;
+  PackedAttnSeq to[kAttnSeqs];
+  for (int b0 = 0; b0 < n; b0 += kAttnSeqs) {
+    const int m = std::min(n - b0, kAttnSeqs);
+    if (many_rows(seqs + b0, m, group)) continue;
+    bool join = false;
+    const int64_t units = lay_out_few(c, seqs + b0, m, group, n_sm, to, &join);
+    if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
+    rows = std::max(rows, units * c->n_kv_heads * kAttnTile);
+  }
+  *bytes = ceil_div(rows * (c->head_dim + 1) * 4, 16) * 16 + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
   return INFLLM_OK;
+}
+
+template <typename T, int kDim>
+int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, int n_sm, bool join, cudaStream_t s) {
+  const int64_t units = lay_out_few(c, seqs, P.batch, P.group, n_sm, P.seq, &join);
+  int counts = 0;
+  for (int i = 0; i < P.batch; ++i) counts = std::max(counts, seqs[i].count);
+  P.part_lse = P.part_o + units * c->n_kv_heads * kAttnTile * kDim;
+  if (units > 0) {
+    auto kern = counts * P.group <= 8 ? packed_rows_kernel<T, kDim, 1> : packed_rows_kernel<T, kDim, 2>;
+    INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)units, c->n_kv_heads), dim3(kAttnWarps * 32), 0, s, P));
+    INFLLM_LAUNCH_OK("packed_rows_kernel");
+  }
+  return join ? join_launch<T, kDim, false>(P, P, n_sm, s) : INFLLM_OK;
+}
+
+template <typename T, int kDim>
+int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, int n_sm, bool join, cudaStream_t s) {
+  INFLLM_TRY(lay_out_many(c, seqs, P.a.batch, P.a.group, n_sm, P.a.seq, P.start, &P.n_ctas, &join));
+  INFLLM_TRY(tc_get_error_ptr(&P.a.err));
+  P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
+  if (P.n_ctas > 0) INFLLM_TRY(packed_tc_launch(P, c->dtype, kDim, s));
+  return join ? join_launch<T, kDim, true>(P, P.a, n_sm, s) : INFLLM_OK;
 }
 
 }  // namespace
@@ -468,43 +637,35 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
       return fail(INFLLM_E_BADARG, "packed_attend: a workspace of %lld bytes, 16-byte aligned", (long long)bytes);
     DeviceScope scope(c->device);
     cudaStream_t s = (cudaStream_t)stream;
-    PackedAttnParams P;
+    PackedTcParams Tc;
+    PackedAttnParams& P = Tc.a;
     P.at = packed_planes(c, layer);
     P.q = (const char*)d_q, P.q_bs = q_bs * 2, P.q_hs = q_hs * 2, P.q_ts = q_ts * 2;
     P.out = (char*)d_out, P.lse = d_lse;
     P.row_lse = weigh > 0 ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * 4) : nullptr;
     P.weights = c->d_weights + layer * packed_rows(c);
+    P.part_o = (float*)d_work;
     P.group = n_heads / c->n_kv_heads, P.most = most, P.weigh = weigh;
-    P.scale_log2 = scale * kLog2e, P.decay = decay;
+    // (the tensor-core kernel masks scores before it scales them: -inf times 0 is no number.  By the least normal number instead, scores
+    // of less than 2^100 are zeros beside any reference)
+    P.scale_log2 = std::max(scale * kLog2e, FLT_MIN), P.decay = decay;
+    const int n_sm = sm_count(c->device);
     for (P.b0 = 0; P.b0 < n; P.b0 += kAttnSeqs) {
-      const int m = std::min(n - P.b0, kAttnSeqs);
+      P.batch = std::min(n - P.b0, kAttnSeqs);
       const infllm_packed_seq* mine = seqs + P.b0;
-      P.batch = m;
-      bool join = false;
-      const int64_t units = lay_out(c, mine, m, n_heads, P.seq, &join);
       int64_t longest = 0;
-      int counts = 0;
-      for (int i = 0; i < m; ++i) {
-        longest = std::max<int64_t>(longest, mine[i].length), counts = std::max(counts, mine[i].count);
-        join = join || mine[i].count < most;  // (rows without a token)
+      bool empty = false, any = false;  // rows without a token, rows with one
+      for (int i = 0; i < P.batch; ++i) {
+        if (mine[i].count > 0) longest = std::max<int64_t>(longest, mine[i].length), any = true;
+        empty = empty || mine[i].count < most;
       }
-      P.part_o = (float*)d_work, P.part_lse = P.part_o + units * c->n_kv_heads * kAttnTile * c->head_dim;
+      const bool many = many_rows(mine, P.batch, P.group);
       INFLLM_DISPATCH_DTYPE(c->dtype, T, {
-        if (units > 0) {
-          const bool few = counts * P.group <= 8;
-          auto kern = c->head_dim == 128 ? (few ? packed_rows_kernel<T, 128, 1> : packed_rows_kernel<T, 128, 2>)
-                                         : (few ? packed_rows_kernel<T, 64, 1> : packed_rows_kernel<T, 64, 2>);
-          kern<<<dim3((unsigned)units, c->n_kv_heads), kAttnWarps * 32, 0, s>>>(P);
-          INFLLM_LAUNCH_OK("packed_rows_kernel");
-        }
-        if (join) {
-          auto kern = c->head_dim == 128 ? packed_join_kernel<T, 128> : packed_join_kernel<T, 64>;
-          kern<<<(unsigned)ceil_div((int64_t)m * most * n_heads, 8), 256, 0, s>>>(P);
-          INFLLM_LAUNCH_OK("packed_join_kernel");
-        }
-        if (weigh > 0 && units > 0) {
+        if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, n_sm, empty, s) : attend_many<T, 64>(Tc, mine, c, n_sm, empty, s)));
+        else INFLLM_TRY((c->head_dim == 128 ? attend_few<T, 128>(P, mine, c, n_sm, empty, s) : attend_few<T, 64>(P, mine, c, n_sm, empty, s)));
+        if (weigh > 0 && any) {
           auto kern = c->head_dim == 128 ? packed_weigh_kernel<T, 128> : packed_weigh_kernel<T, 64>;
-          kern<<<dim3((unsigned)ceil_div(longest, 64), c->n_kv_heads, m), 128, 0, s>>>(P);
+          INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)ceil_div(longest, 64), c->n_kv_heads, P.batch), dim3(128), 0, s, P));
           INFLLM_LAUNCH_OK("packed_weigh_kernel");
         }
       });

@@ -1,0 +1,519 @@
+// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that four warps
+// take out of their codes, S and O in TMEM.
+//
+// A unit is up to 256 rows of one KV head (two tiles of 128: one each for two teams of four softmax warps, a thread per row) by a
+// stretch of keys.  Four more warps bring codes from global memory through registers, a key tile ahead, and leave 16-bit numbers, swizzled
+// as the products want them, in a ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is
+// taken out once for 256 rows.  Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A
+// operand of P V from there, have 128 columns, O another 128; a unit of up to 128 rows has one team, whose S goes to the two buffers in
+// turn.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
+// P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.
+// Sums, O and partial rows are fp32.
+#include <atomic>
+
+#include "attn_tc.cuh"
+#include "packed_attn.cuh"
+#include "ring.cuh"
+#include "tc_softmax.cuh"
+
+namespace infllm {
+
+namespace xtc {
+constexpr int kStages = 5;
+constexpr int kWarpMma = 8, kWarpCodes = 9, kCodeWarps = 4;
+constexpr int kThreads = (kWarpCodes + kCodeWarps) * 32;
+enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, Q_FULL0 = EMPTY0 + kStages, S_FULL0 = Q_FULL0 + 2, P_FULL0 = S_FULL0 + 3, PV_DONE0 = P_FULL0 + 3, N_BARS = PV_DONE0 + 3 };
+// Scores and what follows from them go by channels: 0 and 1 are the teams' with the buffer of the same number, 2 is the first
+// team's with the second buffer.
+__device__ __forceinline__ int channel(bool two, int team, int i) { return two ? team : (i & 1) * 2; }
+__device__ __forceinline__ int buffer(int channel) { return channel ? 1 : 0; }
+template <int kDim>
+struct Smem {
+  static constexpr int kTileBytes = 128 * kDim * 2;  // of 128 rows, as one or two swizzled tiles of 64 dimensions
+  static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBar = kRing + kStages * kTileBytes, kTotal = kBar + 256;
+};
+// position of a key tile and of a value tile of a unit of n tiles in the ring, and what is at a position
+__device__ __forceinline__ int pos_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
+__device__ __forceinline__ int pos_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
+__device__ __forceinline__ bool is_value(int p, int n) { return p == 2 * n - 1 || (p > 0 && p % 2 == 0); }
+__device__ __forceinline__ int tile_at(int p, int n) { return p == 2 * n - 1 ? n - 1 : p % 2 ? (p + 1) / 2 : p == 0 ? 0 : p / 2 - 1; }
+
+struct Piece {  // of a unit: what a block has of it
+  int b, hkv, row0, rows;  // rows of the sequence's new tokens, up to 256
+  int tile0, n, keys;      // key tiles, and keys in them
+  int slot;                // of partial rows, -1: the unit is whole
+};
+struct Pieces {  // a block's, in turn
+  int u, t, ue, te, slot;
+  __device__ __forceinline__ explicit Pieces(const PackedTcParams& P) {
+    const int2 a = P.start[blockIdx.x], z = P.start[blockIdx.x + 1];
+    u = a.x, t = a.y, ue = z.x, te = z.y, slot = 2 * blockIdx.x;
+  }
+  __device__ __forceinline__ bool next(const PackedTcParams& P, Piece& p) {
+    if (u > ue || (u == ue && t >= te)) return false;
+    p.b = seq_of(P.a, u);
+    const PackedAttnSeq& S = P.a.seq[p.b];
+    const int local = u - S.unit0, block = local % S.chunks;
+    p.hkv = local / S.chunks;
+    p.row0 = block * kBlockRows, p.rows = min(kBlockRows, S.count * P.a.group - p.row0);
+    const int all = tiles_of(S, P.a.group, block), end = u == ue ? te : all;
+    p.tile0 = t, p.n = end - t;
+    p.keys = min(end * kKeyTile, keys_of_row(S, P.a.group, p.row0 + p.rows - 1)) - t * kKeyTile;
+    p.slot = t == 0 && end == all ? -1 : slot;
+    slot = 2 * blockIdx.x + 1;  // (only the first and the last of a block are parts)
+    if (end == all) ++u, t = 0;
+    else t = end;
+    return true;
+  }
+};
+}  // namespace xtc
+
+template <typename T, int kDim>
+__global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __grid_constant__ PackedTcParams P) {
+  using namespace xtc;
+  using L = Smem<kDim>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t s_base = smem_u32(smem), sQ = s_base + L::kQ, sRing = s_base + L::kRing, bars = s_base + L::kBar;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + N_BARS * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBar + N_BARS * 8 + 8);
+  auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* const err = P.a.err;
+
+  if (warp == 0) {
+    static_assert(N_BARS <= 32 && N_BARS * 8 + 16 <= 256, "");
+    static_assert(kCodeWarps == 4, "");
+    // the parts of four warps: tiles, queries, probabilities
+    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 || lane == Q_FULL0 || lane == Q_FULL0 + 1 || (lane >= P_FULL0 && lane < P_FULL0 + 3) ? 4u : 1u);
+    if (lane == 0) *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  constexpr uint32_t idesc_qk = make_idesc(kBf16, 128, 128, false), idesc_pv = make_idesc(kBf16, 128, kDim, true);
+  chain_enter();
+
+  if (warp >= kWarpCodes) {
+    // ======================================================================================================== numbers
+    // A lane has the 32 numbers of one (m, s): a 16-byte piece of a row of codes, of rows 32 (or 64) apart.
+    using C = Codes<T>;
+    constexpr int kGroups = kDim / 32, kPer = kGroups, kStep = 128 / kPer;
+    const int at = (warp - kWarpCodes) * 32 + lane, t = at % kGroups, r0 = at / kGroups;
+    struct Raw {
+      uint4 c[kPer];
+      uint32_t ms[kPer];
+    };
+    struct Op {
+      bool more, value, mixed;
+      int b, nk;
+      int64_t row;  // the first of the tile's in the layer
+    };
+    Pieces pieces(P);
+    Piece now;
+    int p = 0;
+    bool there = pieces.next(P, now);
+    auto next_op = [&]() {
+      Op o;
+      o.more = there;
+      if (!there) return o;
+      const PackedAttnSeq& S = P.a.seq[now.b];
+      const int i = tile_at(p, now.n), j0 = (now.tile0 + i) * kKeyTile;
+      o.value = is_value(p, now.n);
+      o.nk = min(kKeyTile, now.keys - i * kKeyTile);
+      o.mixed = j0 + kKeyTile > keys_of_row(S, P.a.group, now.row0);
+      o.row = P.a.at.row0(S.slot, now.hkv) + j0;
+      if (++p == 2 * now.n) p = 0, there = pieces.next(P, now);
+      return o;
+    };
+    auto load = [&](const Op& o, Raw& r) {
+      const char* codes = P.a.at.codes + (o.value ? P.a.at.codes_v : 0) + o.row * (kDim / 2);
+      const char* scales = P.a.at.scales + (o.value ? P.a.at.scales_v : 0) + o.row * (kDim / 8);
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        const int k = r0 + x * kStep;
+        r.c[x] = make_uint4(0, 0, 0, 0), r.ms[x] = 0;  // (what lies behind the last key is not read: zeros)
+        if (o.more && k < o.nk) {
+          r.c[x] = __ldg(reinterpret_cast<const uint4*>(codes + k * (kDim / 2) + t * 16));
+          r.ms[x] = __ldg(reinterpret_cast<const uint32_t*>(scales + k * (kDim / 8) + t * 4));
+        }
+      }
+    };
+    bool ok = true;
+    int slot = 0;
+    Raw raw;
+    Op op = next_op();
+    load(op, raw);
+    while (op.more && ok) {
+      const Op after = next_op();
+      Raw then;
+      load(after, then);
+      if (op.mixed) {
+        // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and
+        // its key is no number in its place, so that the rows that see it still become none.
+        const char* scales = P.a.at.scales + P.a.at.scales_v + op.row * (kDim / 8);
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          const int k = r0 + x * kStep;
+          if (op.value && C::odd(raw.ms[x])) raw.ms[x] = 0;
+          if (!op.value && k < op.nk)
+            for (int g = 0; g < kGroups; ++g)
+              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + k * (kDim / 8) + g * 4)))) raw.ms[x] = 0x7fff7fffu;
+        }
+      }
+      const int b = slot % kStages;
+      if (slot >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot - kStages, kStages), abort_flag, err, 751);
+      if (!ok) break;
+      unsigned char* to = smem + L::kRing + b * L::kTileBytes + (t >> 1) * kSubTileBytes;
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        const int k = r0 + x * kStep;
+        const auto m2 = C::least2(raw.ms[x]), s2 = C::step2(raw.ms[x]);
+        const uint32_t w[4] = {raw.c[x].x, raw.c[x].y, raw.c[x].z, raw.c[x].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // (16 bytes of eight lanes at a time go to eight different bank groups)
+          const int c = j ^ (t >> 1) * 2;
+          uint32_t wc = w[0];
+#pragma unroll
+          for (int y = 1; y < 4; ++y) wc = c == y ? w[y] : wc;
+          *reinterpret_cast<uint4*>(to + k * 128 + ((((t & 1) * 4 + c) ^ (k & 7)) << 4)) =
+              make_uint4(C::pair(wc, 0, m2, s2), C::pair(wc, 1, m2, s2), C::pair(wc, 2, m2, s2), C::pair(wc, 3, m2, s2));
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(FULL0 + b));
+      ++slot;
+      op = after, raw = then;
+    }
+    // nothing will be signalled in this block when it goes: the releases come behind all products
+    for (int b = 0; b < kStages && ok; ++b) {
+      const int last = ring_last(slot, kStages, b);
+      if (last >= 0) ok = warp_wait(bar(EMPTY0 + b), ring_parity(last, kStages), abort_flag, err, 752);
+    }
+    __syncwarp();
+  } else if (warp == kWarpMma) {
+    // ===================================================================================================== products
+    const bool lead = elect_one();
+    int base = 0, np[3] = {0, 0, 0}, n_one = 0, n_two = 0;  // ring position, probabilities that have been waited for, units of each team
+    bool ok = true;
+    const uint64_t ring_k = make_sdesc(sRing, 16, 1024), ring_v = make_sdesc(sRing, kSubTileBytes, 1024), qd0 = make_sdesc(sQ, 16, 1024);
+    auto arrived = [&](int pos) { ok = ok && warp_wait(bar(FULL0 + pos % kStages), ring_parity(pos, kStages), abort_flag, err, 761); };
+    auto release = [&](int pos) {
+      if (lead) tc_commit(bar(EMPTY0 + pos % kStages));
+    };
+    auto qk = [&](int q, int pos, int ch) {  // S of a team's queries
+      tc_fence_after();
+      if (lead) {
+        const uint64_t qd = qd0 + (uint64_t)(q * L::kTileBytes >> 4), kd = ring_k + (uint64_t)((pos % kStages) * L::kTileBytes >> 4);
+#pragma unroll
+        for (int ks = 0; ks < kDim / 16; ++ks) {
+          const uint64_t o = (uint64_t)(((ks >> 2) * kSubTileBytes + (ks & 3) * 32) >> 4);
+          mma_ss(tmem + buffer(ch) * 128, qd + o, kd + o, idesc_qk, ks > 0);
+        }
+        tc_commit(bar(S_FULL0 + ch));
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int team, int pos, int ch, bool first) {
+      ok = ok && warp_wait(bar(P_FULL0 + ch), np[ch] & 1, abort_flag, err, 762);
+      ++np[ch];
+      if (!ok) return;
+      tc_fence_after();
+      if (lead) {
+        const uint64_t vd = ring_v + (uint64_t)((pos % kStages) * L::kTileBytes >> 4);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) mma_ts(tmem + 256 + team * 128, tmem + buffer(ch) * 128 + 8 * ks, vd + (uint64_t)((ks * 2048) >> 4), idesc_pv, !first || ks > 0);
+        tc_commit(bar(PV_DONE0 + ch));
+      }
+      __syncwarp();
+    };
+    Pieces pieces(P);
+    Piece U;
+    while (ok && pieces.next(P, U)) {
+      const int n = U.n;
+      const bool two = U.rows > 128;
+      ok = warp_wait(bar(Q_FULL0), n_one++ & 1, abort_flag, err, 760);
+      if (two) ok = ok && warp_wait(bar(Q_FULL0 + 1), n_two++ & 1, abort_flag, err, 760);
+      if (!ok) break;
+      const int ahead = two ? 1 : 2;  // a team's buffers
+      for (int i = 0; i < ahead && i < n && ok; ++i) {
+        const int pos = base + pos_k(i);
+        arrived(pos);
+        if (!ok) break;
+        qk(0, pos, channel(two, 0, i));
+        if (two) qk(1, pos, 1);
+        release(pos);
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const int v_pos = base + pos_v(i, n), more = i + ahead, k_pos = base + pos_k(more);
+        arrived(v_pos);
+        if (!ok) break;
+        if (two) {
+          pv(0, v_pos, 0, i == 0);
+          if (ok && more < n) {
+            arrived(k_pos);
+            if (ok) qk(0, k_pos, 0);
+          }
+          if (ok) pv(1, v_pos, 1, i == 0);
+          if (!ok) break;
+          release(v_pos);
+          if (more < n) {
+            qk(1, k_pos, 1);
+            release(k_pos);
+          }
+        } else {
+          pv(0, v_pos, channel(false, 0, i), i == 0);
+          if (!ok) break;
+          release(v_pos);
+          if (more < n) {
+            arrived(k_pos);
+            if (!ok) break;
+            qk(0, k_pos, channel(false, 0, more));
+            release(k_pos);
+          }
+        }
+      }
+      base += 2 * n;
+    }
+    __syncwarp();
+  } else {
+    // ====================================================================================================== softmax
+    const int quad = warp & 3, team = warp >> 2, row = quad * 32 + lane;
+    const uint32_t lane_base = ((uint32_t)(quad * 32)) << 16;
+    const uint32_t tO = tmem + 256 + team * 128 + lane_base;
+    struct Turn {  // a unit of this team's, and this thread's row of it
+      bool more, two, in;
+      int n, key0, lim, all;
+      int64_t out, slot_row;  // row of the output; of the partial results, -1: the unit is whole
+      int64_t part;           // the first of the row's 32 in its slot's numbers
+      int64_t lse;            // of the counted rows' log-sum-exps
+      int64_t q;              // bytes from the first query's first row to its own, -1: none
+    };
+    Pieces pieces(P);
+    auto find = [&]() {  // the team's next unit
+      Turn t;
+      Piece U;
+      t.more = false;
+      while (pieces.next(P, U)) {
+        if (team == 0 || U.rows > 128) {
+          t.more = true;
+          break;
+        }
+      }
+      if (!t.more) return t;
+      const PackedAttnSeq& S = P.a.seq[U.b];
+      t.n = U.n, t.key0 = U.tile0 * kKeyTile, t.two = U.rows > 128;
+      t.in = team * 128 + row < U.rows;
+      t.lim = t.key0 + U.keys;  // rows that are none are not masked, so that whole tiles stay whole: nothing of them is written
+      t.q = t.out = t.lse = 0, t.slot_row = t.part = -1;
+      if (!t.in) t.q = -1;
+      if (t.in) {
+        const int r = U.row0 + team * 128 + row, i = r / P.a.group, h = r - i * P.a.group;
+        t.lim = min(t.lim, keys_of_row(S, P.a.group, r));
+        const int64_t b = P.a.b0 + U.b, tok = P.a.most - S.count + i;
+        t.q = b * P.a.q_bs + (int64_t)(U.hkv * P.a.group + h) * P.a.q_hs + tok * P.a.q_ts;
+        t.out = (b * P.a.most + tok) * (P.a.at.n_kv * P.a.group) + U.hkv * P.a.group + h;
+        t.lse = (b * P.a.at.n_kv + U.hkv) * P.a.most * P.a.group + r;
+      }
+      if (U.slot >= 0) {
+        t.slot_row = (int64_t)U.slot * kBlockRows + team * 128 + row;
+        t.part = ((int64_t)U.slot * kBlockRows + team * 128 + quad * 32) * kDim;
+      }
+      t.all = __reduce_min_sync(0xffffffffu, t.lim);
+      return t;
+    };
+    auto queries = [&](const Turn& t) {
+      // The warp's 32 rows, 16 bytes a lane, swizzled.  No product reads the last unit's any more: its scores have been seen.
+      constexpr int kPer = kDim / 8, kAt = 32 / kPer;
+      const int c = lane % kPer;
+      const uint32_t to = sQ + team * L::kTileBytes + quad * 32 * 128 + (c >> 3) * kSubTileBytes;
+#pragma unroll 1
+      for (int r = lane / kPer; r < 32; r += kAt) {
+        const int64_t from = __shfl_sync(0xffffffffu, t.q, r);
+        mma::cp_async16(to + r * 128 + (((c & 7) ^ (r & 7)) << 4), P.a.q + (from < 0 ? 0 : from) + c * 16, from >= 0);
+      }
+      mma::cp_async_commit();
+      mma::cp_async_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
+    };
+    int ns[3] = {0, 0, 0};  // tiles so far of each channel
+    bool ok = true;
+    Turn now = find();
+    if (now.more) queries(now);
+    while (now.more && ok) {
+      const Turn next = find();
+      const int step = now.two ? 1 : 2;
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < now.n && ok; ++i) {
+        const int ch = channel(now.two, team, i);
+        const uint32_t tS = tmem + buffer(ch) * 128 + lane_base;
+        ok = warp_wait(bar(S_FULL0 + ch), (ns[ch] + i / step) & 1, abort_flag, err, 770);
+        if (!ok) break;
+        tc_fence_after();
+        const int j0 = now.key0 + i * kKeyTile;
+        if (now.all < j0 + kKeyTile) {
+          // what a row does not see is taken out of the scores where they are
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            const int hi = now.lim - j0 - c;
+            if (__all_sync(0xffffffffu, hi >= 32)) continue;
+            uint32_t w[32];
+            tmem_ld32(tS + c, w);
+            tmem_wait_ld32(w);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) w[k] = k < hi ? w[k] : 0xff800000u;
+            tmem_st32(tS + c, w);
+          }
+          tmem_wait_st();
+        }
+        float s[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t* us = reinterpret_cast<uint32_t*>(s);
+        {
+          float b[32];
+          uint32_t* ub = reinterpret_cast<uint32_t*>(b);
+          tmem_ld32(tS + 32, ub);
+          tmem_ld32(tS + 64, us);
+          tmem_wait_ld32(ub);
+          tmem_wait_ld32(us);
+          max_chunk(b, mx);
+          tmem_ld32(tS + 96, ub);
+          max_chunk(s, mx);
+          tmem_ld32(tS, us);
+          tmem_wait_ld32(ub);
+          tmem_wait_ld32(us);
+          max_chunk(b, mx);
+          max_chunk(s, mx);
+        }
+        const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.a.scale_log2;
+        const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
+        const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
+        const bool scale_o = __any_sync(0xffffffffu, mn != m && m != -INFINITY) && i > 0;
+        l *= alpha;
+        m = mn;
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // P, packed, takes the place of scores that have been read: 16 columns for 32
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float2 e[16];
+          uint32_t pk[16];
+          arg_chunk(s, P.a.scale_log2, nm, e);
+          tmem_ld32_if(c < 3, tS + 32 * c + 32, us);
+          exp_chunk<T, 5>(e, rs, pk);
+          tmem_st16(tS + 16 * c, pk);
+          tmem_wait_ld32(us);
+        }
+        const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
+        const float sum = r.x + r.y;
+        l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
+        if (scale_o) {
+          // O has the products up to the tile before: wait for the last of them
+          const int pb = channel(now.two, team, i - 1);
+          ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (i - 1) / step) & 1, abort_flag, err, 771);
+          if (!ok) break;
+          tc_fence_after();
+          const float2 al = make_float2(alpha, alpha);
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + c, o);
+            tmem_wait_ld32(o);
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              const float2 x = fmul2(make_float2(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), al);
+              o[k] = __float_as_uint(x.x), o[k + 1] = __float_as_uint(x.y);
+            }
+            tmem_st32(tO + c, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(P_FULL0 + ch));
+      }
+      // the next unit's queries first, so that its first scores are formed while this one's rows are written
+      if (ok && next.more) queries(next);
+      if (ok) {
+        const int pb = channel(now.two, team, now.n - 1);
+        ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (now.n - 1) / step) & 1, abort_flag, err, 772);
+      }
+      if (ok) {
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
+#pragma unroll 1
+        for (int c = 0; c < kDim; c += 32) {
+          uint32_t o[32];
+          float* f = reinterpret_cast<float*>(o);
+          tmem_ld32(tO + c, o);
+          tmem_wait_ld32(o);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) f[k] *= inv;
+          if (now.in && now.slot_row >= 0) {
+            // partial rows lie in blocks of 32, four columns of all of them side by side: every store is one stretch
+            float4* to = reinterpret_cast<float4*>(P.a.part_o + now.part) + (c / 4) * 32 + lane;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to[k * 32] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+          } else if (now.in) {
+            uint4* to = reinterpret_cast<uint4*>(P.a.out + (now.out * kDim + c) * 2);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = mma::pack2<T>(f[8 * k + 2 * e], f[8 * k + 2 * e + 1]);
+              to[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (now.in) {
+          const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
+          if (now.slot_row >= 0) {
+            P.a.part_lse[now.slot_row] = lse;
+          } else {
+            if (P.a.lse) P.a.lse[now.out] = lse * (1.f / kLog2e);
+            if (P.a.row_lse) P.a.row_lse[now.lse] = lse;
+          }
+        }
+        tc_fence_before();
+      }
+      if (now.two) ns[team] += now.n;
+      else ns[0] += (now.n + 1) / 2, ns[2] += now.n / 2;
+      __syncwarp();
+      now = next;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+}
+
+int packed_tc_launch(const PackedTcParams& P, int dtype, int head_dim, cudaStream_t s) {
+  INFLLM_DISPATCH_DTYPE(dtype, T, {
+    auto kern = head_dim == 128 ? packed_tc_kernel<T, 128> : packed_tc_kernel<T, 64>;
+    const int smem = (head_dim == 128 ? xtc::Smem<128>::kTotal : xtc::Smem<64>::kTotal) + 1024;
+    static std::atomic<uint64_t> set[2];  // devices that know it, per head_dim (and, by the dispatch, type)
+    int dev = 0;
+    INFLLM_CUDA_OK(cudaGetDevice(&dev));
+    std::atomic<uint64_t>& there = set[head_dim == 128];
+    if (dev >= 64 || !(there.load(std::memory_order_relaxed) >> dev & 1)) {
+      INFLLM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (dev < 64) there.fetch_or(1ull << dev);
+    }
+    INFLLM_CUDA_OK(launch_chained(kern, dim3(P.n_ctas), dim3(xtc::kThreads), smem, s, P));
+  });
+  INFLLM_LAUNCH_OK("packed_tc_kernel");
+  return INFLLM_OK;
+}
+
+}  // namespace infllm
