@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libinfllm_b200.so")
 SOURCES = ["error.cu", "rope.cu", "retrieval.cu", "attn_general.cu", "attn_decode.cu", "attn_tc.cu", "context.cu",
            "comm.cu", "sink_window.cu", "token.cu", "pages.cu", "paged_attn.cu", "paged_tc.cu",
-           "packed.cu", "packed_attn.cu", "packed_tc.cu"]
+           "packed.cu", "packed_attn.cu", "packed_tc.cu", "packed_weigh.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",

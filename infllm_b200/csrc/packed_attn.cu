@@ -278,17 +278,6 @@ struct JoinParams<true> {
   static __device__ __forceinline__ const PackedAttnParams& attn(const type& p) { return p.a; }
 };
 
-// the last block whose stretch begins at or before (unit, tile)
-__device__ __forceinline__ int block_of(const PackedTcParams& P, int u, int t) {
-  int lo = 0, hi = P.n_ctas - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (P.start[mid].x < u || (P.start[mid].x == u && P.start[mid].y <= t)) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
 template <typename T, int kDim, int kWarps, bool kTc>
 __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ typename JoinParams<kTc>::type All) {
   constexpr int kPer = kDim / 32, kRows = 8 / kWarps, kAhead = 4;
@@ -519,45 +508,69 @@ int64_t lay_out_few(const infllm_packed* c, const infllm_packed_seq* seqs, int n
   return u;
 }
 
-// the same for many rows: units are dealt out to blocks, and cut, so that all have about the same work
-int lay_out_many(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group, int n_sm, PackedAttnSeq* to, int2* start, int* n_ctas, bool* join) {
-  int64_t u = 0, work = 0;
-  auto rows_of = [&](int i, int block) { return std::min<int64_t>(kBlockRows, (int64_t)seqs[i].count * group - (int64_t)block * kBlockRows); };
-  for (int i = 0; i < n; ++i) {
-    const int64_t blocks = ceil_div((int64_t)seqs[i].count * group, kBlockRows);
-    to[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)u, (int32_t)std::max<int64_t>(blocks, 1), 0};
-    u += blocks * c->n_kv_heads;
-    if (u > INT_MAX) return fail(INFLLM_E_BADARG, "packed_attend: %lld units of work", (long long)u);
-    for (int x = 0; x < (int)blocks; ++x) work += c->n_kv_heads * (kUnitWork + tile_work(rows_of(i, x)) * tiles_of(to[i], group, x));
-  }
+// Deals the tiles of units 0, 1, .. out to blocks, so that all have about the same work: for_each calls f(tiles, work of one).
+template <typename F>
+void deal_out(PackedTcParams& P, int n_sm, bool* join, F&& for_each) {
+  int64_t work = 0;
+  for_each([&](int64_t tiles, int64_t each) { work += kUnitWork + tiles * each; });
   // (a cut costs a unit's start; where that was too little, so that the last block has more than the others, shares grow)
   int64_t share = std::max(ceil_div(work, n_sm) + kUnitWork, kBlockWork), left = 0;
-  int ctas = 0;
+  int ctas = 0, u = 0;
+  bool cut = false;
   for (int tries = 0; tries < 20; ++tries, share += ceil_div(share, 16)) {
-    auto begin = [&](int64_t unit, int64_t tile) {
-      start[ctas++] = make_int2((int)unit, (int)tile);
-      left = share;
-    };
-    ctas = 0, left = 0, u = 0;
-    for (int i = 0; i < n; ++i)
-      for (int h = 0; h < c->n_kv_heads; ++h)
-        for (int x = 0; seqs[i].count > 0 && x < to[i].chunks; ++x, ++u) {
-          const int64_t tiles = tiles_of(to[i], group, x), each = tile_work(rows_of(i, x));
-          int64_t at = 0;
-          while (at < tiles) {
-            // short ends stay where they are
-            if (ctas == 0 || (left < kUnitWork + 4 * each && left < kUnitWork + (tiles - at) * each && ctas < n_sm)) begin(u, at);
-            int64_t take = tiles - at;
-            if (ctas < n_sm && kUnitWork + take * each > left + 2 * each) take = std::max<int64_t>(1, std::min(take, (left - kUnitWork) / each));
-            left -= kUnitWork + take * each;
-            if (at > 0 || take < tiles) *join = true;
-            at += take;
-          }
-        }
+    ctas = u = 0, left = 0, cut = false;
+    for_each([&](int64_t tiles, int64_t each) {
+      int64_t at = 0;
+      while (at < tiles) {
+        // short ends stay where they are
+        if (ctas == 0 || (left < kUnitWork + 4 * each && left < kUnitWork + (tiles - at) * each && ctas < n_sm))
+          P.start[ctas++] = make_int2(u, (int)at), left = share;
+        int64_t take = tiles - at;
+        if (ctas < n_sm && kUnitWork + take * each > left + 2 * each) take = std::max<int64_t>(1, std::min(take, (left - kUnitWork) / each));
+        left -= kUnitWork + take * each;
+        cut = cut || take < tiles;
+        at += take;
+      }
+      ++u;
+    });
     if (left > -share / 16 - 8) break;
   }
-  start[ctas] = make_int2((int)u, 0);
-  *n_ctas = ctas;
+  P.start[ctas] = make_int2(u, 0);
+  P.n_ctas = ctas;
+  *join = *join || cut;
+}
+
+int many_units(const infllm_packed* c, const infllm_packed_seq* seqs, PackedTcParams& P, int kv_units(const infllm_packed_seq&, int)) {
+  int64_t u = 0;
+  for (int i = 0; i < P.a.batch; ++i) {
+    const int blocks = kv_units(seqs[i], P.a.group);
+    P.a.seq[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)u, std::max(blocks, 1), 0};
+    u += (int64_t)blocks * c->n_kv_heads;
+    if (u > INT_MAX) return fail(INFLLM_E_BADARG, "packed_attend: %lld units of work", (long long)u);
+  }
+  return INFLLM_OK;
+}
+
+// the units of the attention of seqs[0 .. n - 1] for many rows
+int lay_out_many(const infllm_packed* c, const infllm_packed_seq* seqs, int n_sm, PackedTcParams& P, bool* join) {
+  const int group = P.a.group;
+  INFLLM_TRY(many_units(c, seqs, P, [](const infllm_packed_seq& s, int g) { return (int)ceil_div((int64_t)s.count * g, kBlockRows); }));
+  deal_out(P, n_sm, join, [&](auto&& f) {
+    for (int i = 0; i < P.a.batch; ++i)
+      for (int h = 0; h < c->n_kv_heads && seqs[i].count > 0; ++h)
+        for (int x = 0; x < P.a.seq[i].chunks; ++x) f(tiles_of(P.a.seq[i], group, x), tile_work(std::min<int64_t>(kBlockRows, (int64_t)seqs[i].count * group - (int64_t)x * kBlockRows)));
+  });
+  return INFLLM_OK;
+}
+
+// and of their weights
+int lay_out_weights(const infllm_packed* c, const infllm_packed_seq* seqs, int n_sm, PackedTcParams& P, bool* join) {
+  INFLLM_TRY(many_units(c, seqs, P, [](const infllm_packed_seq& s, int) { return s.count > 0 ? (int)ceil_div(s.length, kWeighKeys) : 0; }));
+  deal_out(P, n_sm, join, [&](auto&& f) {
+    for (int i = 0; i < P.a.batch; ++i)
+      for (int h = 0; h < c->n_kv_heads && seqs[i].count > 0; ++h)
+        for (int x = 0; x < P.a.seq[i].chunks; ++x) f(weigh_tiles(P.a.seq[i], P.a.group, P.a.weigh, x), 2);
+  });
   return INFLLM_OK;
 }
 
@@ -601,7 +614,7 @@ int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_
 
 template <typename T, int kDim>
 int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, int n_sm, bool join, cudaStream_t s) {
-  INFLLM_TRY(lay_out_many(c, seqs, P.a.batch, P.a.group, n_sm, P.a.seq, P.start, &P.n_ctas, &join));
+  INFLLM_TRY(lay_out_many(c, seqs, n_sm, P, &join));
   INFLLM_TRY(tc_get_error_ptr(&P.a.err));
   P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
   if (P.n_ctas > 0) INFLLM_TRY(packed_tc_launch(P, c->dtype, kDim, s));
@@ -663,7 +676,11 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
       INFLLM_DISPATCH_DTYPE(c->dtype, T, {
         if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, n_sm, empty, s) : attend_many<T, 64>(Tc, mine, c, n_sm, empty, s)));
         else INFLLM_TRY((c->head_dim == 128 ? attend_few<T, 128>(P, mine, c, n_sm, empty, s) : attend_few<T, 64>(P, mine, c, n_sm, empty, s)));
-        if (weigh > 0 && any) {
+        if (weigh > 0 && any && many) {
+          bool cut = false;
+          INFLLM_TRY(lay_out_weights(c, mine, n_sm, Tc, &cut));
+          INFLLM_TRY(packed_weigh_tc_launch(Tc, c->dtype, c->head_dim, cut, (int)longest, s));
+        } else if (weigh > 0 && any) {
           auto kern = c->head_dim == 128 ? packed_weigh_kernel<T, 128> : packed_weigh_kernel<T, 64>;
           INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)ceil_div(longest, 64), c->n_kv_heads, P.batch), dim3(128), 0, s, P));
           INFLLM_LAUNCH_OK("packed_weigh_kernel");

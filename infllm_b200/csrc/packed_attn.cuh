@@ -56,6 +56,45 @@ __host__ __device__ __forceinline__ int tiles_of(const PackedAttnSeq& S, int gro
   return (keys_of_row(S, group, last < rows ? last : rows - 1) + kKeyTile - 1) / kKeyTile;
 }
 
+// the weights, for many rows: units of 256 keys of a KV head (unit0 + KV head * chunks + block) by tiles of 128 counted rows that see them
+constexpr int kWeighKeys = 256;
+__host__ __device__ __forceinline__ int weigh_row0(const PackedAttnSeq& S, int group, int weigh, int block) {
+  const int counted = S.count - (weigh < S.count ? weigh : S.count), sees = block * kWeighKeys - (S.length - S.count);
+  return (counted > sees ? counted : sees) * group;
+}
+__host__ __device__ __forceinline__ int weigh_tiles(const PackedAttnSeq& S, int group, int weigh, int block) {
+  return (S.count * group - weigh_row0(S, group, weigh, block) + 127) / 128;
+}
+
+#ifdef __CUDACC__
+// the last block whose stretch begins at or before (unit, tile)
+__device__ __forceinline__ int block_of(const PackedTcParams& P, int u, int t) {
+  int lo = 0, hi = P.n_ctas - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (P.start[mid].x < u || (P.start[mid].x == u && P.start[mid].y <= t)) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// the 32 numbers of a group, codes c and (m, s), to row k of a swizzled tile; `to` is the tile's half that has group t
+template <typename T>
+__device__ __forceinline__ void put_group(unsigned char* to, int k, int t, const uint4& c, uint32_t ms) {
+  using C = Codes<T>;
+  const auto m2 = C::least2(ms), s2 = C::step2(ms);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // (the 16 bytes of eight lanes at a time go to eight different bank groups: lanes of the second half of a row are two pieces ahead)
+    const int at = j ^ (t >> 1) * 2;
+    const uint32_t x = t >> 1 ? w[j ^ 2] : w[j];
+    *reinterpret_cast<uint4*>(to + k * 128 + ((((t & 1) * 4 + at) ^ (k & 7)) << 4)) = make_uint4(C::pair(x, 0, m2, s2), C::pair(x, 1, m2, s2), C::pair(x, 2, m2, s2), C::pair(x, 3, m2, s2));
+  }
+}
+#endif
+
+int packed_weigh_tc_launch(const PackedTcParams& P, int dtype, int head_dim, bool join, int longest, cudaStream_t s);
 int packed_tc_launch(const PackedTcParams& P, int dtype, int head_dim, cudaStream_t s);
 
 }  // namespace infllm

@@ -173,21 +173,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
       if (!ok) break;
       unsigned char* to = smem + L::kRing + b * L::kTileBytes + (t >> 1) * kSubTileBytes;
 #pragma unroll
-      for (int x = 0; x < kPer; ++x) {
-        const int k = r0 + x * kStep;
-        const auto m2 = C::least2(raw.ms[x]), s2 = C::step2(raw.ms[x]);
-        const uint32_t w[4] = {raw.c[x].x, raw.c[x].y, raw.c[x].z, raw.c[x].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // (16 bytes of eight lanes at a time go to eight different bank groups)
-          const int c = j ^ (t >> 1) * 2;
-          uint32_t wc = w[0];
-#pragma unroll
-          for (int y = 1; y < 4; ++y) wc = c == y ? w[y] : wc;
-          *reinterpret_cast<uint4*>(to + k * 128 + ((((t & 1) * 4 + c) ^ (k & 7)) << 4)) =
-              make_uint4(C::pair(wc, 0, m2, s2), C::pair(wc, 1, m2, s2), C::pair(wc, 2, m2, s2), C::pair(wc, 3, m2, s2));
-        }
-      }
+      for (int x = 0; x < kPer; ++x) put_group<T>(to, r0 + x * kStep, t, raw.c[x], raw.ms[x]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(FULL0 + b));
