@@ -48,8 +48,10 @@ __device__ __forceinline__ float2 span32(const uint4& x, uint32_t quad) {
 template <typename T>
 __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_t* ms) {
   const float2 span = span32<T>(x, quad);
-  const T step = Act<T>::from_f(__fdiv_rn(span.y - span.x, 15.f)), least = Act<T>::from_f(span.x);
+  T step = Act<T>::from_f(__fdiv_rn(span.y - span.x, 15.f));
+  const T least = Act<T>::from_f(span.x);
   const float s = Act<T>::to_f(step);
+  if (Codes<T>::kBf16 && s >= 0x1p122f) step = Act<T>::from_f(NAN);
   const T* p = reinterpret_cast<const T*>(&x);
   uint32_t w = 0;
 #pragma unroll
@@ -157,7 +159,9 @@ __global__ void __launch_bounds__(256) packed_values_kernel(const __grid_constan
     const uint32_t c = reinterpret_cast<const uint32_t*>(P.at.codes + layer * P.codes_layer + val * P.at.codes_v + row * (kDim / 2))[w];
     const uint32_t ms = reinterpret_cast<const uint32_t*>(P.at.scales + layer * P.scales_layer + val * P.at.scales_v + row * (kDim / 8))[w / 4];
     const auto m2 = Codes<T>::least2(ms), s2 = Codes<T>::step2(ms);
-    out = make_uint4(Codes<T>::pair(c, 0, m2, s2), Codes<T>::pair(c, 1, m2, s2), Codes<T>::pair(c, 2, m2, s2), Codes<T>::pair(c, 3, m2, s2));
+    uint32_t v[4];
+    Codes<T>::pairs(c, m2, s2, v);
+    out = make_uint4(v[0], v[1], v[2], v[3]);
   }
   char* to = (val ? P.v : P.k) + ((((int64_t)layer * P.batch + P.b0 + blockIdx.y) * P.at.n_kv + h) * P.most + i) * (kDim * 2);
   *reinterpret_cast<uint4*>(to + w * 16) = out;

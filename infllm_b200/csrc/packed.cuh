@@ -3,8 +3,7 @@
 // Of each 32 neighbouring numbers x of a row, in the cache's 16-bit type T: the least m, a step s = T((max x - m) / 15), and of each
 // number a code c = the nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  A number stands for T(m + s c): one fused
 // multiply-add in T, so every kernel has the same operands, whatever its tiles.
-// A word has eight codes, number 2i at bit 4i and number 2i + 1 at bit 16 + 4i: a shift and a mask by 0x000f000f give two neighbours,
-// and the low or the high halves of two rows' words, put together, give pairs of the same number of both rows.
+// A word has eight codes, number 2i at bit 4i and number 2i + 1 at bit 16 + 4i: what a mask leaves are two neighbours, and the low or the high halves of two rows' words, put together, give pairs of the same number of both rows.
 #pragma once
 #include <type_traits>
 
@@ -24,29 +23,50 @@ struct PackedPlanes {
   __device__ __forceinline__ int64_t row0(int slot, int hkv) const { return ((int64_t)slot * n_kv + hkv) * max_tokens; }
 };
 
+// A word's codes come out by a mask (and a shift for the upper half of them), a product or a difference that makes them numbers, and one
+// multiply-add; the masks and shifts share the slowest pipe, so there are as few of them as can be.
+//   bf16  Bits 0 .. 7 of a number are, without its other bits, that whole number times 2^-133 (the first binade goes on where the
+//         subnormals end), so codes at bits 0 .. 3 and 4 .. 7 are c and 16 c times 2^-133; a product makes c 2^-6 of both, and the step is
+//         64 s.  (A step of 2^122 or more, which has no such product, is not held: its group is NaN.)
+//   fp16  Beside the exponent of 1024 they are 1024 + c and 1024 + 16 c.
 template <typename T>
 struct Codes {
   using T2 = typename Act<T>::T2;
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  // codes as the low bits of numbers whose last place is 1: 128 + c in bf16, 1024 + c in fp16
-  static constexpr uint32_t kBias = kBf16 ? 0x43004300u : 0x64006400u;
   static __device__ __forceinline__ T2 as2(uint32_t x) { return *reinterpret_cast<T2*>(&x); }
   static __device__ __forceinline__ uint32_t bits(T2 x) { return *reinterpret_cast<uint32_t*>(&x); }
-  // the pair at bits 4i and 16 + 4i of w, with least numbers m2 and steps s2
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int i, T2 m2, T2 s2) {
-    const T2 c = __hsub2(as2(((w >> (4 * i)) & 0x000f000fu) | kBias), as2(kBias));
-    return bits(__hfma2(c, s2, m2));
+  // the pairs at bits 4i and 16 + 4i of w, i = 0 .. 3, with least numbers m2 and steps s2
+  static __device__ __forceinline__ void pairs(uint32_t w, T2 m2, T2 s2, uint32_t* out) {
+    const uint32_t h = w >> 8;
+    out[0] = bits(__hfma2(low(w), s2, m2));
+    out[1] = bits(__hfma2(high(w), s2, m2));
+    out[2] = bits(__hfma2(low(h), s2, m2));
+    out[3] = bits(__hfma2(high(h), s2, m2));
   }
-  // (m, s) in one word: pairs (m, m) and (s, s)
+  // (m, s) in one word: pairs (m, m) and (s, s), as pairs() wants them
   static __device__ __forceinline__ T2 least2(uint32_t sc) { return as2(__byte_perm(sc, sc, 0x1010)); }
-  static __device__ __forceinline__ T2 step2(uint32_t sc) { return as2(__byte_perm(sc, sc, 0x3232)); }
+  static __device__ __forceinline__ T2 step2(uint32_t sc) { return scaled(as2(__byte_perm(sc, sc, 0x3232))); }
   // of two rows' words: pairs (m of a, m of b) and (s of a, s of b)
   static __device__ __forceinline__ T2 least2(uint32_t a, uint32_t b) { return as2(__byte_perm(a, b, 0x5410)); }
-  static __device__ __forceinline__ T2 step2(uint32_t a, uint32_t b) { return as2(__byte_perm(a, b, 0x7632)); }
+  static __device__ __forceinline__ T2 step2(uint32_t a, uint32_t b) { return scaled(as2(__byte_perm(a, b, 0x7632))); }
   // whether (m, s) are not both finite: all exponent bits are set in one of them
   static __device__ __forceinline__ bool odd(uint32_t sc) {
     constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
     return (sc & e) == e || (sc >> 16 & e) == e;
+  }
+
+ private:
+  static __device__ __forceinline__ T2 low(uint32_t w) {  // the codes at bits 0 and 16: themselves, or times 2^-6
+    if constexpr (kBf16) return __hmul2(as2(w & 0x000f000fu), as2(0x7f007f00u));  // 2^127
+    else return __hsub2(as2((w & 0x000f000fu) | 0x64006400u), as2(0x64006400u));
+  }
+  static __device__ __forceinline__ T2 high(uint32_t w) {  // at bits 4 and 20
+    if constexpr (kBf16) return __hmul2(as2(w & 0x00f000f0u), as2(0x7d007d00u));  // 2^123
+    else return __hfma2(as2((w & 0x00f000f0u) | 0x64006400u), as2(0x2c002c00u), as2(0xd400d400u));  // times 1/16, less 64
+  }
+  static __device__ __forceinline__ T2 scaled(T2 s) {
+    if constexpr (kBf16) return __hmul2(s, as2(0x42804280u));  // 64
+    else return s;
   }
 };
 

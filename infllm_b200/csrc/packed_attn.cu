@@ -21,6 +21,17 @@ using namespace mma;
 
 constexpr int kAttnWarps = 4, kAttnTile = 16;
 
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_stream4(const void* p) {
+  uint32_t r;
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+
 // --------------------------------------------------------------------------------------------------------- a warp's part
 // Groups of 16 keys against up to 16 rows, from global memory straight into the operands of the m16n8k16 products: a thread's codes of
 // a key are those of the 32 numbers of one (m, s) (kDim 128), its codes of a value an eighth of the row.
@@ -56,20 +67,21 @@ struct PackedWarp {
   struct Key {  // rows nt * 8 + g
     uint32_t w[2][kW], ms[2];
   };
+  template <bool kAll>  // all 16 keys are there
   __device__ __forceinline__ static Key key(const char* codes, const char* scales, int nk) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     Key k;
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
-      const int r = min(nt * 8 + g, nk - 1);  // (what lies behind the last key is not read: it may not be a number, and 0 times that is none)
+      const int r = kAll ? nt * 8 + g : min(nt * 8 + g, nk - 1);  // (what lies behind the last key is not read: it may not be a number, and 0 times that is none)
       if (kDim == 128) {
         const uint4 x = ld_stream16(codes + r * 64 + t * 16);
         k.w[nt][0] = x.x, k.w[nt][1] = x.y, k.w[nt][2 % kW] = x.z, k.w[nt][3 % kW] = x.w;
-        k.ms[nt] = *reinterpret_cast<const uint32_t*>(scales + r * 16 + t * 4);
+        k.ms[nt] = ld_stream4(scales + r * 16 + t * 4);
       } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(codes + r * 32 + t * 8);
+        const uint2 x = ld_stream8(codes + r * 32 + t * 8);
         k.w[nt][0] = x.x, k.w[nt][1] = x.y;
-        k.ms[nt] = *reinterpret_cast<const uint32_t*>(scales + r * 8 + (t >> 1) * 4);
+        k.ms[nt] = ld_stream4(scales + r * 8 + (t >> 1) * 4);
       }
     }
     return k;
@@ -82,11 +94,12 @@ struct PackedWarp {
       s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < kW; ++j) {
-        const uint32_t w = k.w[nt][j];
+        uint32_t v[4];
+        C::pairs(k.w[nt][j], m2, s2, v);
         const uint32_t a0[4] = {qf[0][j].x, kNt > 1 ? qf[kNt - 1][j].x : 0u, qf[0][j].y, kNt > 1 ? qf[kNt - 1][j].y : 0u};
-        mma16816<T>(s[nt], a0, C::pair(w, 0, m2, s2), C::pair(w, 1, m2, s2));
+        mma16816<T>(s[nt], a0, v[0], v[1]);
         const uint32_t a1[4] = {qf[0][j].z, kNt > 1 ? qf[kNt - 1][j].z : 0u, qf[0][j].w, kNt > 1 ? qf[kNt - 1][j].w : 0u};
-        mma16816<T>(s[nt], a1, C::pair(w, 2, m2, s2), C::pair(w, 3, m2, s2));
+        mma16816<T>(s[nt], a1, v[2], v[3]);
       }
     }
   }
@@ -94,19 +107,20 @@ struct PackedWarp {
   struct Value {  // rows 2t, 2t + 1, 2t + 8, 2t + 9: numbers g * kDim / 8 .. of each
     uint32_t w[4][kH], ms[4];
   };
+  template <bool kAll>
   __device__ __forceinline__ static Value value(const char* codes, const char* scales, int nk) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     Value v;
 #pragma unroll
     for (int ki = 0; ki < 4; ++ki) {
-      const int r = min(2 * t + (ki & 1) + (ki >> 1) * 8, nk - 1);
+      const int at = 2 * t + (ki & 1) + (ki >> 1) * 8, r = kAll ? at : min(at, nk - 1);
       if (kDim == 128) {
-        const uint2 x = *reinterpret_cast<const uint2*>(codes + r * 64 + g * 8);
+        const uint2 x = ld_stream8(codes + r * 64 + g * 8);
         v.w[ki][0] = x.x, v.w[ki][kH - 1] = x.y;
-        v.ms[ki] = *reinterpret_cast<const uint32_t*>(scales + r * 16 + (g >> 1) * 4);
+        v.ms[ki] = ld_stream4(scales + r * 16 + (g >> 1) * 4);
       } else {
-        v.w[ki][0] = *reinterpret_cast<const uint32_t*>(codes + r * 32 + g * 4);
-        v.ms[ki] = *reinterpret_cast<const uint32_t*>(scales + r * 8 + (g >> 2) * 4);
+        v.w[ki][0] = ld_stream4(codes + r * 32 + g * 4);
+        v.ms[ki] = ld_stream4(scales + r * 8 + (g >> 2) * 4);
       }
     }
     return v;
@@ -115,80 +129,62 @@ struct PackedWarp {
 
 // --------------------------------------------------------------------------------------------------------- attention
 // Four warps share a stretch's groups of 16 keys and meet in shared memory.  P is two 16-bit numbers, p = hi + lo, so that an output's
-// only rounding is its own.
+// only rounding is its own.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is
+// scaled and do lanes that share a row exchange anything.
 template <typename T, int kDim, int kNt>
-__global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_kernel(const __grid_constant__ PackedAttnParams P) {
+struct PackedRows : PackedWarp<T, kDim, kNt> {
   using W = PackedWarp<T, kDim, kNt>;
   using C = Codes<T>;
-  constexpr int kTiles = 4 * W::kH, kPitch = kDim + 4;
-  __shared__ __align__(16) float sm_o[kAttnWarps][8 * kNt][kPitch];
-  __shared__ float sm_m[kAttnWarps][8 * kNt], sm_l[kAttnWarps][8 * kNt];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int unit = blockIdx.x, hkv = blockIdx.y, b = seq_of(P, unit);
-  const PackedAttnSeq S = P.seq[b];
-  const int tile = (unit - S.unit0) / S.chunks, key0 = (unit - S.unit0 - tile * S.chunks) * S.keys, row0 = tile * kAttnTile;
-  // (of the last row's keys: the others see no more)
-  const int last = S.length - S.count + min(S.count, (row0 + kAttnTile - 1) / P.group + 1), key1 = min(key0 + S.keys, last);
-  const int rows = min(8 * kNt, S.count * P.group - row0);
-  W w;
-  w.rows(P, S, b, hkv, row0);
-  chain_enter();
-  w.queries();
-  const int least = S.length - S.count + row0 / P.group + 1;  // keys that every row sees
-  float ot[kTiles][kNt][4], m[kNt], l[kNt];  // O^T: [0], [1] = number g * kDim / 8 + 2i of rows 2t, 2t + 1; [2], [3] = the next one
+  static constexpr int kTiles = 4 * W::kH;
+  float ot[kTiles][kNt][4];  // O^T: [0], [1] = number g * kDim / 8 + 2i of rows 2t, 2t + 1; [2], [3] = the next one
+  float m[kNt], l[kNt];
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int x = 0; x < kNt; ++x) {
-    m[x] = -INFINITY, l[x] = 0.f;
+    for (int x = 0; x < kNt; ++x) {
+      m[x] = -INFINITY, l[x] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) ot[i][x][0] = ot[i][x][1] = ot[i][x][2] = ot[i][x][3] = 0.f;
-  }
-  const int64_t first = P.at.row0(S.slot, hkv);
-  const char* kc = P.at.codes + first * (kDim / 2);
-  const char* ks = P.at.scales + first * (kDim / 8);
-  const char* vc = kc + P.at.codes_v;
-  const char* vs = ks + P.at.scales_v;
-#pragma unroll 1
-  for (int j0 = key0 + warp * 16; j0 < key1; j0 += kAttnWarps * 16) {
-    const int nk = min(16, key1 - j0);
-    typename W::Key k = W::key(kc + (int64_t)j0 * (kDim / 2), ks + (int64_t)j0 * (kDim / 8), nk);
-    typename W::Value v = W::value(vc + (int64_t)j0 * (kDim / 2), vs + (int64_t)j0 * (kDim / 8), nk);
-    if (j0 + 16 > least) {
-      // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and its
-      // key is no number in its place, so that the rows that see it still become none.
-      uint32_t bad = 0;
-#pragma unroll
-      for (int ki = 0; ki < 4; ++ki) {
-        const bool odd = C::odd(v.ms[ki]);
-        if (odd) v.ms[ki] = 0;
-        const uint32_t any = __ballot_sync(0xffffffffu, odd);  // of key 2t + .. in every lane with that t
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-          if (any & (0x11111111u << tt)) bad |= 1u << (2 * tt + (ki & 1) + (ki >> 1) * 8);
-      }
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-        if (bad >> (nt * 8 + g) & 1) k.ms[nt] = 0x7fff7fffu;
+      for (int i = 0; i < kTiles; ++i) ot[i][x][0] = ot[i][x][1] = ot[i][x][2] = ot[i][x][3] = 0.f;
     }
+  }
+
+  // 16 keys from j0 on; kAll: every row sees all of them.  Otherwise those below key1, and a row those below its own limit.
+  template <bool kAll>
+  __device__ __forceinline__ void group(const typename W::Key& k, const typename W::Value& v, int j0, int key1, float scale_log2, float* logits, int64_t pitch) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
     float s[2][4];
-    w.scores(k, s);
+    this->scores(k, s);
     uint32_t hi[kNt][2], lo[kNt][2];
 #pragma unroll
     for (int x = 0; x < kNt; ++x) {  // row x * 8 + g: keys nt * 8 + 2t + e
-      float p[4], mx = -INFINITY;
+      float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = j0 + (e >> 1) * 8 + 2 * t + (e & 1);
-        p[e] = key < min(w.lim[x], key1) ? s[e >> 1][x * 2 + (e & 1)] * P.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, p[e]);
+        p[e] = s[e >> 1][x * 2 + (e & 1)] * scale_log2;
+        if (!kAll && j0 + (e >> 1) * 8 + 2 * t + (e & 1) >= min(this->lim[x], key1)) p[e] = -INFINITY;
       }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[x], mx), ms = mn == -INFINITY ? 0.f : mn;
-      const float al = exp2f(m[x] - ms);
-      m[x] = mn;
+      if (logits) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = exp2f(p[e] - ms);
-      l[x] = l[x] * al + (p[0] + p[1]) + (p[2] + p[3]);
+        for (int e = 0; e < 4; e += 2)
+          if (kAll || j0 + e * 4 + 2 * t < key1) *reinterpret_cast<float2*>(logits + j0 + e * 4) = make_float2(p[e], p[e + 1]);
+      }
+      float mx = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+      if (__any_sync(0xffffffffu, mx > m[x] + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = mx > m[x] + 8.f ? mx : m[x];
+        const float al = m[x] == -INFINITY ? 0.f : exp2f(m[x] - mn);
+        m[x] = mn;
+        l[x] *= al;
+        // this thread's columns of O^T are rows 2t and 2t + 1
+        const float a0 = __shfl_sync(0xffffffffu, al, (2 * t) * 4), a1 = __shfl_sync(0xffffffffu, al, (2 * t + 1) * 4);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) ot[i][x][0] *= a0, ot[i][x][1] *= a1, ot[i][x][2] *= a0, ot[i][x][3] *= a1;
+      }
+      const float ms = !kAll && m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = ex2(p[e] - ms);
+      l[x] += (p[0] + p[1]) + (p[2] + p[3]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         typename Act<T>::T2 h = Act<T>::from_f2(p[2 * e], p[2 * e + 1]);
@@ -196,23 +192,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
         const float2 f = Act<T>::to_f2(h);
         lo[x][e] = pack2<T>(p[2 * e] - f.x, p[2 * e + 1] - f.y);
       }
-      if (__any_sync(0xffffffffu, al != 1.f)) {
-        // this thread's columns of O^T are rows 2t and 2t + 1
-        const float a0 = __shfl_sync(0xffffffffu, al, (2 * t) * 4), a1 = __shfl_sync(0xffffffffu, al, (2 * t + 1) * 4);
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) ot[i][x][0] *= a0, ot[i][x][1] *= a1, ot[i][x][2] *= a0, ot[i][x][3] *= a1;
-      }
     }
     // A operands: numbers of keys 2t, 2t + 1 and of 2t + 8, 2t + 9
     const auto m01 = C::least2(v.ms[0], v.ms[1]), s01 = C::step2(v.ms[0], v.ms[1]);
     const auto m23 = C::least2(v.ms[2], v.ms[3]), s23 = C::step2(v.ms[2], v.ms[3]);
 #pragma unroll
     for (int j = 0; j < W::kH; ++j) {
-      const uint32_t e01 = __byte_perm(v.w[0][j], v.w[1][j], 0x5410), o01 = __byte_perm(v.w[0][j], v.w[1][j], 0x7632);
-      const uint32_t e23 = __byte_perm(v.w[2][j], v.w[3][j], 0x5410), o23 = __byte_perm(v.w[2][j], v.w[3][j], 0x7632);
+      uint32_t e01[4], o01[4], e23[4], o23[4];
+      C::pairs(__byte_perm(v.w[0][j], v.w[1][j], 0x5410), m01, s01, e01);
+      C::pairs(__byte_perm(v.w[0][j], v.w[1][j], 0x7632), m01, s01, o01);
+      C::pairs(__byte_perm(v.w[2][j], v.w[3][j], 0x5410), m23, s23, e23);
+      C::pairs(__byte_perm(v.w[2][j], v.w[3][j], 0x7632), m23, s23, o23);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a[4] = {C::pair(e01, i, m01, s01), C::pair(o01, i, m01, s01), C::pair(e23, i, m23, s23), C::pair(o23, i, m23, s23)};
+        const uint32_t a[4] = {e01[i], o01[i], e23[i], o23[i]};
 #pragma unroll
         for (int x = 0; x < kNt; ++x) {
           mma16816<T>(ot[j * 4 + i][x], a, hi[x][0], hi[x][1]);
@@ -221,6 +214,81 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
       }
     }
   }
+  static __device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  }
+};
+
+template <typename T, int kDim, int kNt>
+__global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_kernel(const __grid_constant__ PackedAttnParams P) {
+  using R = PackedRows<T, kDim, kNt>;
+  using W = typename R::W;
+  using C = Codes<T>;
+  constexpr int kTiles = R::kTiles, kPitch = kDim + 4, kStep = kAttnWarps * 16;
+  __shared__ __align__(16) float sm_o[kAttnWarps][8 * kNt][kPitch];
+  __shared__ float sm_m[kAttnWarps][8 * kNt], sm_l[kAttnWarps][8 * kNt];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int unit = blockIdx.x, hkv = blockIdx.y, b = seq_of(P, unit);
+  const PackedAttnSeq S = P.seq[b];
+  const int tile = (unit - S.unit0) / S.chunks, key0 = (unit - S.unit0 - tile * S.chunks) * S.keys, row0 = tile * kAttnTile;
+  const int rows = min(8 * kNt, S.count * P.group - row0);
+  const int key1 = min(key0 + S.keys, keys_of_row(S, P.group, row0 + rows - 1));  // (the last row's: the others see no more)
+  const int least = keys_of_row(S, P.group, row0);  // keys that every row sees
+  R w;
+  w.rows(P, S, b, hkv, row0);
+  const int64_t first = P.at.row0(S.slot, hkv);
+  const char* kc = P.at.codes + first * (kDim / 2);
+  const char* ks = P.at.scales + first * (kDim / 8);
+  const char* vc = kc + P.at.codes_v;
+  const char* vs = ks + P.at.scales_v;
+  float* logits = kNt == 1 && P.logits && g < rows ? P.logits + (((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.logit_rows + g) * P.pitch + 2 * t : nullptr;
+  chain_enter();
+  w.queries();
+  w.clear();
+  auto key = [&](int j) { return W::template key<true>(kc + (int64_t)j * (kDim / 2), ks + (int64_t)j * (kDim / 8), 16); };
+  auto value = [&](int j) { return W::template value<true>(vc + (int64_t)j * (kDim / 2), vs + (int64_t)j * (kDim / 8), 16); };
+  const int whole = min(key1, least) - 16;  // the last place of a group that all rows see all of
+  int j0 = key0 + warp * 16;
+  if (j0 <= whole) {
+    // a group is on its way while the one before it is worked on
+    typename W::Key k = key(j0);
+    typename W::Value v = value(j0);
+#pragma unroll 1
+    for (; j0 + kStep <= whole; j0 += kStep) {
+      const typename W::Key kn = key(j0 + kStep);
+      const typename W::Value vn = value(j0 + kStep);
+      w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
+      k = kn, v = vn;
+    }
+    w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
+    j0 += kStep;
+  }
+#pragma unroll 1
+  for (; j0 < key1; j0 += kStep) {
+    const int nk = min(16, key1 - j0);
+    typename W::Key k = W::template key<false>(kc + (int64_t)j0 * (kDim / 2), ks + (int64_t)j0 * (kDim / 8), nk);
+    typename W::Value v = W::template value<false>(vc + (int64_t)j0 * (kDim / 2), vs + (int64_t)j0 * (kDim / 8), nk);
+    // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and its
+    // key is no number in its place, so that the rows that see it still become none.
+    uint32_t bad = 0;
+#pragma unroll
+    for (int ki = 0; ki < 4; ++ki) {
+      const bool odd = C::odd(v.ms[ki]);
+      if (odd) v.ms[ki] = 0;
+      const uint32_t any = __ballot_sync(0xffffffffu, odd);  // of key 2t + .. in every lane with that t
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+        if (any & (0x11111111u << tt)) bad |= 1u << (2 * tt + (ki & 1) + (ki >> 1) * 8);
+    }
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+      if (bad >> (nt * 8 + g) & 1) k.ms[nt] = 0x7fff7fffu;
+    w.template group<false>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
+  }
+  float (&ot)[kTiles][kNt][4] = w.ot;
+  float (&m)[kNt] = w.m, (&l)[kNt] = w.l;
 #pragma unroll
   for (int x = 0; x < kNt; ++x) {
     l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
@@ -251,10 +319,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
       n0 /= den, n1 /= den;
     }
     const float lse = mx == -INFINITY ? -INFINITY : mx + log2f(den);
+    const int64_t pr = ((int64_t)unit * P.at.n_kv + hkv) * kAttnTile + r;
+    if (d == 0 && (S.chunks > 1 || P.logits)) P.part_lse[pr] = lse;
     if (S.chunks > 1) {
-      const int64_t pr = ((int64_t)unit * P.at.n_kv + hkv) * kAttnTile + r;
       *reinterpret_cast<float2*>(P.part_o + pr * kDim + d) = make_float2(n0, n1);
-      if (d == 0) P.part_lse[pr] = lse;
     } else {
       const int i = (row0 + r) / P.group, h = row0 + r - i * P.group;
       const int64_t orow = ((int64_t)(P.b0 + b) * P.most + P.most - S.count + i) * (P.at.n_kv * P.group) + hkv * P.group + h;
@@ -278,11 +346,52 @@ struct JoinParams<true> {
   static __device__ __forceinline__ const PackedAttnParams& attn(const type& p) { return p.a; }
 };
 
+// The weights of four keys a thread from the scores that the kernel of few rows has left, 1024 keys of a KV head a block.
+constexpr int kSumKeys = 1024;
+__device__ __forceinline__ void sum_weights(const PackedAttnParams& P, int block) {
+  __shared__ float sm_lse[8];
+  const int per = (int)(P.pitch / kSumKeys), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hkv = block / per % P.at.n_kv, b = block / per / P.at.n_kv;
+  const PackedAttnSeq S = P.seq[b];
+  const int key0 = block % per * kSumKeys, rows = S.count * P.group, from = (S.count - min(P.weigh, S.count)) * P.group;
+  chain_enter();
+  if (rows == 0 || key0 >= S.length) return;
+  if (warp < rows) {  // a row's log-sum-exp, of its parts'
+    float mx = -INFINITY, sum = 0.f;
+    auto part = [&](int c) { return P.part_lse[((int64_t)(S.unit0 + c) * P.at.n_kv + hkv) * kAttnTile + warp]; };
+    for (int c = lane; c < S.chunks; c += 32) mx = fmaxf(mx, part(c));
+    mx = warp_max(mx);
+    if (mx == -INFINITY) mx = 0.f;  // (where all are no numbers)
+    for (int c = lane; c < S.chunks; c += 32) sum += exp2f(part(c) - mx);
+    sum = warp_sum(sum);
+    if (lane == 0) sm_lse[warp] = mx + log2f(sum);
+  }
+  __syncthreads();
+  const int key = key0 + threadIdx.x * 4;
+  if (key >= S.length) return;
+  const float* from_logits = P.logits + ((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.logit_rows * P.pitch + key;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int r = from; r < rows; ++r) {
+    const float4 s = *reinterpret_cast<const float4*>(from_logits + r * P.pitch);
+    const float z = sm_lse[r];
+    w[0] += exp2f(s.x - z), w[1] += exp2f(s.y - z), w[2] += exp2f(s.z - z), w[3] += exp2f(s.w - z);
+  }
+  float* to = P.weights + P.at.row0(S.slot, hkv) + key;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (key + e < S.length) to[e] = P.decay == 0.f ? w[e] : P.decay * to[e] + w[e];
+  }
+}
+
 template <typename T, int kDim, int kWarps, bool kTc>
 __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ typename JoinParams<kTc>::type All) {
   constexpr int kPer = kDim / 32, kRows = 8 / kWarps, kAhead = 4;
   __shared__ float sm[8][kDim + 4];
   const PackedAttnParams& P = JoinParams<kTc>::attn(All);
+  if (!kTc && (int)blockIdx.x >= P.join_blocks) {
+    sum_weights(P, blockIdx.x - P.join_blocks);
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = P.at.n_kv * P.group;
   const int64_t at = (int64_t)blockIdx.x * kRows + warp / kWarps;
   const bool in = at < (int64_t)P.batch * P.most * heads;
@@ -383,10 +492,14 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
 }
 
 template <typename T, int kDim, bool kTc>
-static int join_launch(const typename JoinParams<kTc>::type& P, const PackedAttnParams& A, int n_sm, cudaStream_t s) {
+static int join_launch(typename JoinParams<kTc>::type& P, PackedAttnParams& A, bool join, int n_sm, cudaStream_t s) {
   // as many warps to a row as one wave has room for
   const int64_t rows = (int64_t)A.batch * A.most * A.at.n_kv * A.group, warps = n_sm * 32 / std::max<int64_t>(rows, 1);
-  auto launch = [&](auto kern, int per_row) { return launch_chained(kern, dim3((unsigned)ceil_div(rows * per_row, 8)), dim3(256), 0, s, P); };
+  auto launch = [&](auto kern, int per_row) {
+    A.join_blocks = join ? (int)ceil_div(rows * per_row, 8) : 0;
+    const int64_t sums = A.logits ? (int64_t)A.batch * A.at.n_kv * (A.pitch / kSumKeys) : 0;
+    return launch_chained(kern, dim3((unsigned)(A.join_blocks + sums)), dim3(256), 0, s, P);
+  };
   if (warps >= 8) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 8, kTc>, 8));
   else if (warps >= 4) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 4, kTc>, 4));
   else if (warps >= 2) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 2, kTc>, 2));
@@ -407,7 +520,7 @@ __global__ void __launch_bounds__(128) packed_weigh_kernel(const __grid_constant
   if (S.count == 0 || j0 >= S.length) return;
   const int nk = min(16, S.length - j0);
   const int64_t first = P.at.row0(S.slot, hkv) + j0;
-  const typename W::Key k = W::key(P.at.codes + first * (kDim / 2), P.at.scales + first * (kDim / 8), nk);
+  const typename W::Key k = W::template key<false>(P.at.codes + first * (kDim / 2), P.at.scales + first * (kDim / 8), nk);
   const float* row_lse = P.row_lse + ((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group;
   // the rows from the first counted token, or the first that sees one of the keys, on
   const int from = max(S.count - min(P.weigh, S.count), j0 - (S.length - S.count)) * P.group;
@@ -493,6 +606,19 @@ bool many_rows(const infllm_packed_seq* seqs, int n, int group) {
   int64_t most = 0;
   for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, (int64_t)seqs[i].count * group);
   return most > 2 * kAttnTile;
+}
+
+// whether the weights are worked out of scores that the kernel of few rows leaves: 8 bytes of a row and key, written and read, where
+// keys that are read again are kDim * 5 / 8
+bool by_logits(const infllm_packed_seq* seqs, int n, int group) {
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, (int64_t)seqs[i].count * group);
+  return most <= 8;
+}
+int64_t logit_pitch(const infllm_packed_seq* seqs, int n) {
+  int64_t longest = 0;
+  for (int i = 0; i < n; ++i) longest = std::max<int64_t>(longest, seqs[i].length);
+  return ceil_div(longest, kSumKeys) * kSumKeys;
 }
 
 // the units of the launch of seqs[0 .. n - 1] for few rows
@@ -594,7 +720,8 @@ int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, i
     if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
     rows = std::max(rows, units * c->n_kv_heads * kAttnTile);
   }
-  *bytes = ceil_div(rows * (c->head_dim + 1) * 4, 16) * 16 + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
+  *bytes = ceil_div(rows * (c->head_dim + 1) * 4, 16) * 16;
+  if (weigh > 0) *bytes += by_logits(seqs, n, group) ? (int64_t)n * most * n_heads * logit_pitch(seqs, n) * 4 : (int64_t)n * most * n_heads * 4;
   return INFLLM_OK;
 }
 
@@ -609,7 +736,7 @@ int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_
     INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)units, c->n_kv_heads), dim3(kAttnWarps * 32), 0, s, P));
     INFLLM_LAUNCH_OK("packed_rows_kernel");
   }
-  return join ? join_launch<T, kDim, false>(P, P, n_sm, s) : INFLLM_OK;
+  return join || (P.logits && units > 0) ? join_launch<T, kDim, false>(P, P, join, n_sm, s) : INFLLM_OK;
 }
 
 template <typename T, int kDim>
@@ -618,7 +745,7 @@ int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_p
   INFLLM_TRY(tc_get_error_ptr(&P.a.err));
   P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
   if (P.n_ctas > 0) INFLLM_TRY(packed_tc_launch(P, c->dtype, kDim, s));
-  return join ? join_launch<T, kDim, true>(P, P.a, n_sm, s) : INFLLM_OK;
+  return join ? join_launch<T, kDim, true>(P, P.a, true, n_sm, s) : INFLLM_OK;
 }
 
 }  // namespace
@@ -655,7 +782,9 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
     P.at = packed_planes(c, layer);
     P.q = (const char*)d_q, P.q_bs = q_bs * 2, P.q_hs = q_hs * 2, P.q_ts = q_ts * 2;
     P.out = (char*)d_out, P.lse = d_lse;
-    P.row_lse = weigh > 0 ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * 4) : nullptr;
+    P.pitch = logit_pitch(seqs, n), P.logit_rows = most * (n_heads / c->n_kv_heads);
+    P.logits = weigh > 0 && by_logits(seqs, n, n_heads / c->n_kv_heads) ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * P.pitch * 4) : nullptr;
+    P.row_lse = weigh > 0 && !P.logits ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * 4) : nullptr;
     P.weights = c->d_weights + layer * packed_rows(c);
     P.part_o = (float*)d_work;
     P.group = n_heads / c->n_kv_heads, P.most = most, P.weigh = weigh;
@@ -680,7 +809,7 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
           bool cut = false;
           INFLLM_TRY(lay_out_weights(c, mine, n_sm, Tc, &cut));
           INFLLM_TRY(packed_weigh_tc_launch(Tc, c->dtype, c->head_dim, cut, (int)longest, s));
-        } else if (weigh > 0 && any) {
+        } else if (weigh > 0 && any && !P.logits) {
           auto kern = c->head_dim == 128 ? packed_weigh_kernel<T, 128> : packed_weigh_kernel<T, 64>;
           INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)ceil_div(longest, 64), c->n_kv_heads, P.batch), dim3(128), 0, s, P));
           INFLLM_LAUNCH_OK("packed_weigh_kernel");

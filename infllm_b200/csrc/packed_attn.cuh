@@ -24,6 +24,9 @@ struct PackedAttnParams {
   float *part_o, *part_lse;  // few rows: 16 rows of each unit and KV head; many: kBlockRows rows of each block's first and last unit
   float* row_lse;            // (batch, KV head, token, query head of the KV head), to base 2: for the weights; null: none
   float* weights;            // of the layer
+  float* logits;             // (batch, KV head, row, pitch): scores to base 2 of up to 8 rows, for the weights; null: none
+  int64_t pitch;
+  int32_t logit_rows, join_blocks;  // blocks of the join; those behind them add up the weights
   int* err;
   int32_t group, most, batch, b0, weigh;
   float scale_log2, decay;
@@ -89,7 +92,9 @@ __device__ __forceinline__ void put_group(unsigned char* to, int k, int t, const
     // (the 16 bytes of eight lanes at a time go to eight different bank groups: lanes of the second half of a row are two pieces ahead)
     const int at = j ^ (t >> 1) * 2;
     const uint32_t x = t >> 1 ? w[j ^ 2] : w[j];
-    *reinterpret_cast<uint4*>(to + k * 128 + ((((t & 1) * 4 + at) ^ (k & 7)) << 4)) = make_uint4(C::pair(x, 0, m2, s2), C::pair(x, 1, m2, s2), C::pair(x, 2, m2, s2), C::pair(x, 3, m2, s2));
+    uint32_t v[4];
+    C::pairs(x, m2, s2, v);
+    *reinterpret_cast<uint4*>(to + k * 128 + ((((t & 1) * 4 + at) ^ (k & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 #endif
