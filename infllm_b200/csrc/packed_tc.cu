@@ -1,17 +1,21 @@
-// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that four warps
+// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that seven warps
 // take out of their codes, S and O in TMEM.
 //
-// A unit is up to 256 rows of one KV head (two tiles of 128: one each for two teams of four softmax warps, a thread per row) by a
-// stretch of keys.  Four more warps bring codes from global memory through registers, a key tile ahead, and leave 16-bit numbers, swizzled
-// as the products want them, in a ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is
-// taken out once for 256 rows.  Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A
-// operand of P V from there, have 128 columns, O another 128; a unit of up to 128 rows has one team, whose S goes to the two buffers in
-// turn.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
+// A unit is up to 256 rows of one KV head by a stretch of keys.  Two teams of four softmax warps, a thread per row, have 128 rows each;
+// of up to 128 rows both have all, and take the key tiles in turn: each with a maximum, a sum and an O of its own, which are put
+// together at the unit's end, where a thread reads the other team's O of its row from TMEM.  (A tile is in a team's hands for 1.1 us:
+// with one team that, not its bytes, would be a tile's time.)
+// Seven more warps bring codes from global memory through registers, tiles ahead, and leave 16-bit numbers, swizzled as the products
+// want them, in a ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is taken out once
+// for 256 rows.  Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A operand of P V from
+// there, have 128 columns, O another 128.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only
+// then O is scaled.
 // P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.
 // Sums, O and partial rows are fp32.
 #include <atomic>
 
 #include "attn_tc.cuh"
+#include "decode_warp.cuh"
 #include "packed_attn.cuh"
 #include "ring.cuh"
 #include "tc_softmax.cuh"
@@ -20,17 +24,13 @@ namespace infllm {
 
 namespace xtc {
 constexpr int kStages = 5;
-constexpr int kWarpMma = 8, kWarpCodes = 9, kCodeWarps = 4;
+constexpr int kWarpMma = 8, kWarpCodes = 9, kCodeWarps = 7;
 constexpr int kThreads = (kWarpCodes + kCodeWarps) * 32;
-enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, Q_FULL0 = EMPTY0 + kStages, S_FULL0 = Q_FULL0 + 2, P_FULL0 = S_FULL0 + 3, PV_DONE0 = P_FULL0 + 3, N_BARS = PV_DONE0 + 3 };
-// Scores and what follows from them go by channels: 0 and 1 are the teams' with the buffer of the same number, 2 is the first
-// team's with the second buffer.
-__device__ __forceinline__ int channel(bool two, int team, int i) { return two ? team : (i & 1) * 2; }
-__device__ __forceinline__ int buffer(int channel) { return channel ? 1 : 0; }
+enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, Q_FULL0 = EMPTY0 + kStages, S_FULL0 = Q_FULL0 + 2, P_FULL0 = S_FULL0 + 2, PV_DONE0 = P_FULL0 + 2, MERGE = PV_DONE0 + 2, N_BARS };
 template <int kDim>
 struct Smem {
   static constexpr int kTileBytes = 128 * kDim * 2;  // of 128 rows, as one or two swizzled tiles of 64 dimensions
-  static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBar = kRing + kStages * kTileBytes, kTotal = kBar + 256;
+  static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBar = kRing + kStages * kTileBytes, kMl = kBar + 256, kTotal = kMl + 2 * 128 * 8;
 };
 // position of a key tile and of a value tile of a unit of n tiles in the ring, and what is at a position
 __device__ __forceinline__ int pos_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
@@ -72,20 +72,22 @@ template <typename T, int kDim>
 __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __grid_constant__ PackedTcParams P) {
   using namespace xtc;
   using L = Smem<kDim>;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char smem[];  // (swizzled tiles begin on 1024 bytes, and no byte is left to shift them by)
   const uint32_t s_base = smem_u32(smem), sQ = s_base + L::kQ, sRing = s_base + L::kRing, bars = s_base + L::kBar;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + N_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBar + N_BARS * 8 + 8);
   auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* const err = P.a.err;
+  if (s_base & 1023) {
+    if (threadIdx.x == 0) record_error(err, kErrWaitTimeout, 750);
+    return;
+  }
 
   if (warp == 0) {
     static_assert(N_BARS <= 32 && N_BARS * 8 + 16 <= 256, "");
-    static_assert(kCodeWarps == 4, "");
-    // the parts of four warps: tiles, queries, probabilities
-    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 || lane == Q_FULL0 || lane == Q_FULL0 + 1 || (lane >= P_FULL0 && lane < P_FULL0 + 3) ? 4u : 1u);
+    // tiles: the warps that make them; queries and probabilities: a team's four; what the teams have of the same rows: both
+    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 ? (uint32_t)kCodeWarps : lane == Q_FULL0 || lane == Q_FULL0 + 1 || lane == P_FULL0 || lane == P_FULL0 + 1 ? 4u : lane == MERGE ? 8u : 1u);
     if (lane == 0) *abort_flag = 0;
     mbar_fence_init();
   }
@@ -103,82 +105,107 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
 
   if (warp >= kWarpCodes) {
     // ======================================================================================================== numbers
-    // A lane has the 32 numbers of one (m, s): a 16-byte piece of a row of codes, of rows 32 (or 64) apart.
+    // A thread has the 32 numbers of one (m, s): a 16-byte piece of a row of codes.  A turn is a key tile and the value tile before it; the
+    // next turn's codes are on their way through registers meanwhile, those kAhead tiles behind it to L2.
     using C = Codes<T>;
-    constexpr int kGroups = kDim / 32, kPer = kGroups, kStep = 128 / kPer;
+    constexpr int kGroups = kDim / 32, kStep = kCodeWarps * 32 / kGroups, kPer = (128 + kStep - 1) / kStep, kAhead = 4;
     const int at = (warp - kWarpCodes) * 32 + lane, t = at % kGroups, r0 = at / kGroups;
     struct Raw {
-      uint4 c[kPer];
-      uint32_t ms[kPer];
+      uint4 c[2][kPer];
+      uint32_t ms[2][kPer];
     };
-    struct Op {
-      bool more, value, mixed;
-      int b, nk;
-      int64_t row;  // the first of the tile's in the layer
+    struct Turn {
+      int i, n;      // the key tile, of the piece's
+      int keys;      // from its first one to the piece's last
+      int seen;      // of those that every row sees
+      int64_t row;   // of its first one in the layer
+      bool more;
+      __device__ __forceinline__ int there(int v) const { return v ? (i > 0 ? min(kKeyTile, keys + kKeyTile) : 0) : i < n ? min(kKeyTile, keys) : 0; }
     };
     Pieces pieces(P);
-    Piece now;
-    int p = 0;
-    bool there = pieces.next(P, now);
-    auto next_op = [&]() {
-      Op o;
-      o.more = there;
-      if (!there) return o;
-      const PackedAttnSeq& S = P.a.seq[now.b];
-      const int i = tile_at(p, now.n), j0 = (now.tile0 + i) * kKeyTile;
-      o.value = is_value(p, now.n);
-      o.nk = min(kKeyTile, now.keys - i * kKeyTile);
-      o.mixed = j0 + kKeyTile > keys_of_row(S, P.a.group, now.row0);
-      o.row = P.a.at.row0(S.slot, now.hkv) + j0;
-      if (++p == 2 * now.n) p = 0, there = pieces.next(P, now);
+    auto begin = [&]() {
+      Turn o{};
+      Piece U;
+      o.more = pieces.next(P, U);
+      if (o.more) {
+        const PackedAttnSeq& S = P.a.seq[U.b];
+        o.n = U.n, o.keys = U.keys, o.seen = keys_of_row(S, P.a.group, U.row0) - U.tile0 * kKeyTile;
+        o.row = P.a.at.row0(S.slot, U.hkv) + U.tile0 * kKeyTile;
+      }
       return o;
     };
-    auto load = [&](const Op& o, Raw& r) {
-      const char* codes = P.a.at.codes + (o.value ? P.a.at.codes_v : 0) + o.row * (kDim / 2);
-      const char* scales = P.a.at.scales + (o.value ? P.a.at.scales_v : 0) + o.row * (kDim / 8);
+    auto advance = [&](Turn& o) {
+      if (o.i < o.n) ++o.i, o.keys -= kKeyTile, o.seen -= kKeyTile, o.row += kKeyTile;
+      else o = begin();
+    };
+    const char* const codes0 = P.a.at.codes + r0 * (kDim / 2) + t * 16;
+    const char* const scales0 = P.a.at.scales + r0 * (kDim / 8) + t * 4;
+    auto load = [&](const Turn& o, Raw& r) {
 #pragma unroll
-      for (int x = 0; x < kPer; ++x) {
-        const int k = r0 + x * kStep;
-        r.c[x] = make_uint4(0, 0, 0, 0), r.ms[x] = 0;  // (what lies behind the last key is not read: zeros)
-        if (o.more && k < o.nk) {
-          r.c[x] = __ldg(reinterpret_cast<const uint4*>(codes + k * (kDim / 2) + t * 16));
-          r.ms[x] = __ldg(reinterpret_cast<const uint32_t*>(scales + k * (kDim / 8) + t * 4));
+      for (int v = 0; v < 2; ++v) {
+        const int nk = o.more ? o.there(v) : 0;
+        const int64_t row = o.row - v * kKeyTile;
+        const char* codes = codes0 + v * P.a.at.codes_v + row * (kDim / 2);
+        const char* scales = scales0 + v * P.a.at.scales_v + row * (kDim / 8);
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          r.c[v][x] = make_uint4(0, 0, 0, 0), r.ms[v][x] = 0;  // (what lies behind the last key is not read: zeros)
+          if (r0 + x * kStep < nk) {
+            r.c[v][x] = ld_stream16(codes + x * kStep * (kDim / 2));
+            r.ms[v][x] = __ldg(reinterpret_cast<const uint32_t*>(scales + x * kStep * (kDim / 8)));
+          }
         }
       }
+      // (a line of 128 bytes has the codes of two or four rows, the scales of eight or sixteen)
+      constexpr int kLine = 128 / (kDim / 2), kScaleLine = 128 / (kDim / 8), kLines = 128 / kLine, kAll = kLines + 128 / kScaleLine;
+      static_assert(2 * kAll <= kCodeWarps * 32, "");
+      const int v = at >= kAll, y = at - v * kAll, k = kAhead * kKeyTile + (y < kLines ? y * kLine : (y - kLines) * kScaleLine);
+      if (o.more && at < 2 * kAll && k < o.keys)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(y < kLines ? P.a.at.codes + v * P.a.at.codes_v + (o.row + k) * (kDim / 2)
+                                                               : P.a.at.scales + v * P.a.at.scales_v + (o.row + k) * (kDim / 8)));
     };
     bool ok = true;
     int slot = 0;
     Raw raw;
-    Op op = next_op();
-    load(op, raw);
-    while (op.more && ok) {
-      const Op after = next_op();
+    Turn now = begin();
+    load(now, raw);
+    while (now.more && ok) {
+      Turn after = now;
+      advance(after);
       Raw then;
       load(after, then);
-      if (op.mixed) {
+      if (now.seen < kKeyTile) {
         // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and
         // its key is no number in its place, so that the rows that see it still become none.
-        const char* scales = P.a.at.scales + P.a.at.scales_v + op.row * (kDim / 8);
+        const char* scales = P.a.at.scales + P.a.at.scales_v + now.row * (kDim / 8);
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
           const int k = r0 + x * kStep;
-          if (op.value && C::odd(raw.ms[x])) raw.ms[x] = 0;
-          if (!op.value && k < op.nk)
+          if (now.seen < 0 && C::odd(raw.ms[1][x])) raw.ms[1][x] = 0;
+          if (k < now.there(0))
             for (int g = 0; g < kGroups; ++g)
-              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + k * (kDim / 8) + g * 4)))) raw.ms[x] = 0x7fff7fffu;
+              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + k * (kDim / 8) + g * 4)))) raw.ms[0][x] = 0x7fff7fffu;
         }
       }
-      const int b = slot % kStages;
-      if (slot >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot - kStages, kStages), abort_flag, err, 751);
-      if (!ok) break;
-      unsigned char* to = smem + L::kRing + b * L::kTileBytes + (t >> 1) * kSubTileBytes;
+      const int first = slot;
 #pragma unroll
-      for (int x = 0; x < kPer; ++x) put_group<T>(to, r0 + x * kStep, t, raw.c[x], raw.ms[x]);
+      for (int v = 0; v < 2; ++v) {
+        if (v ? now.i == 0 : now.i == now.n) continue;
+        const int b = slot % kStages;
+        if (ok && slot >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot - kStages, kStages), abort_flag, err, 751);
+        if (ok) {
+          unsigned char* to = smem + L::kRing + b * L::kTileBytes + (t >> 1) * kSubTileBytes;
+#pragma unroll
+          for (int x = 0; x < kPer; ++x)
+            if ((x + 1) * kStep <= 128 || r0 + x * kStep < 128) put_group<T>(to, r0 + x * kStep, t, raw.c[v][x], raw.ms[v][x]);
+        }
+        ++slot;
+      }
+      if (!ok) break;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(FULL0 + b));
-      ++slot;
-      op = after, raw = then;
+      if (lane < slot - first) mbar_arrive(bar(FULL0 + (first + lane) % kStages));
+      now = after, raw = then;
     }
     // nothing will be signalled in this block when it goes: the releases come behind all products
     for (int b = 0; b < kStages && ok; ++b) {
@@ -189,36 +216,36 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
   } else if (warp == kWarpMma) {
     // ===================================================================================================== products
     const bool lead = elect_one();
-    int base = 0, np[3] = {0, 0, 0}, n_one = 0, n_two = 0;  // ring position, probabilities that have been waited for, units of each team
+    int base = 0, np[2] = {0, 0}, n_one = 0, n_two = 0;  // ring position, probabilities that have been waited for, units of each kind
     bool ok = true;
     const uint64_t ring_k = make_sdesc(sRing, 16, 1024), ring_v = make_sdesc(sRing, kSubTileBytes, 1024), qd0 = make_sdesc(sQ, 16, 1024);
     auto arrived = [&](int pos) { ok = ok && warp_wait(bar(FULL0 + pos % kStages), ring_parity(pos, kStages), abort_flag, err, 761); };
     auto release = [&](int pos) {
       if (lead) tc_commit(bar(EMPTY0 + pos % kStages));
     };
-    auto qk = [&](int q, int pos, int ch) {  // S of a team's queries
+    auto qk = [&](int q, int pos, int team) {  // S of a team, of one of the tiles of queries
       tc_fence_after();
       if (lead) {
         const uint64_t qd = qd0 + (uint64_t)(q * L::kTileBytes >> 4), kd = ring_k + (uint64_t)((pos % kStages) * L::kTileBytes >> 4);
 #pragma unroll
         for (int ks = 0; ks < kDim / 16; ++ks) {
           const uint64_t o = (uint64_t)(((ks >> 2) * kSubTileBytes + (ks & 3) * 32) >> 4);
-          mma_ss(tmem + buffer(ch) * 128, qd + o, kd + o, idesc_qk, ks > 0);
+          mma_ss(tmem + team * 128, qd + o, kd + o, idesc_qk, ks > 0);
         }
-        tc_commit(bar(S_FULL0 + ch));
+        tc_commit(bar(S_FULL0 + team));
       }
       __syncwarp();
     };
-    auto pv = [&](int team, int pos, int ch, bool first) {
-      ok = ok && warp_wait(bar(P_FULL0 + ch), np[ch] & 1, abort_flag, err, 762);
-      ++np[ch];
+    auto pv = [&](int team, int pos, bool first) {
+      ok = ok && warp_wait(bar(P_FULL0 + team), np[team] & 1, abort_flag, err, 762);
+      ++np[team];
       if (!ok) return;
       tc_fence_after();
       if (lead) {
         const uint64_t vd = ring_v + (uint64_t)((pos % kStages) * L::kTileBytes >> 4);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) mma_ts(tmem + 256 + team * 128, tmem + buffer(ch) * 128 + 8 * ks, vd + (uint64_t)((ks * 2048) >> 4), idesc_pv, !first || ks > 0);
-        tc_commit(bar(PV_DONE0 + ch));
+        for (int ks = 0; ks < 8; ++ks) mma_ts(tmem + 256 + team * 128, tmem + team * 128 + 8 * ks, vd + (uint64_t)((ks * 2048) >> 4), idesc_pv, !first || ks > 0);
+        tc_commit(bar(PV_DONE0 + team));
       }
       __syncwarp();
     };
@@ -230,12 +257,12 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
       ok = warp_wait(bar(Q_FULL0), n_one++ & 1, abort_flag, err, 760);
       if (two) ok = ok && warp_wait(bar(Q_FULL0 + 1), n_two++ & 1, abort_flag, err, 760);
       if (!ok) break;
-      const int ahead = two ? 1 : 2;  // a team's buffers
+      const int ahead = two ? 1 : 2;  // tiles that both teams, or one after the other, have scores of
       for (int i = 0; i < ahead && i < n && ok; ++i) {
         const int pos = base + pos_k(i);
         arrived(pos);
         if (!ok) break;
-        qk(0, pos, channel(two, 0, i));
+        qk(0, pos, two ? 0 : i);
         if (two) qk(1, pos, 1);
         release(pos);
       }
@@ -244,12 +271,12 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         arrived(v_pos);
         if (!ok) break;
         if (two) {
-          pv(0, v_pos, 0, i == 0);
+          pv(0, v_pos, i == 0);
           if (ok && more < n) {
             arrived(k_pos);
             if (ok) qk(0, k_pos, 0);
           }
-          if (ok) pv(1, v_pos, 1, i == 0);
+          if (ok) pv(1, v_pos, i == 0);
           if (!ok) break;
           release(v_pos);
           if (more < n) {
@@ -257,13 +284,13 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
             release(k_pos);
           }
         } else {
-          pv(0, v_pos, channel(false, 0, i), i == 0);
+          pv(i & 1, v_pos, i < 2);
           if (!ok) break;
           release(v_pos);
           if (more < n) {
             arrived(k_pos);
             if (!ok) break;
-            qk(0, k_pos, channel(false, 0, more));
+            qk(0, k_pos, i & 1);
             release(k_pos);
           }
         }
@@ -276,34 +303,29 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
     const int quad = warp & 3, team = warp >> 2, row = quad * 32 + lane;
     const uint32_t lane_base = ((uint32_t)(quad * 32)) << 16;
     const uint32_t tO = tmem + 256 + team * 128 + lane_base;
-    struct Turn {  // a unit of this team's, and this thread's row of it
+    struct Turn {  // a unit, and this thread's row of it
       bool more, two, in;
-      int n, key0, lim, all;
+      int n, mine, key0, lim, all;  // its tiles; this team's
       int64_t out, slot_row;  // row of the output; of the partial results, -1: the unit is whole
       int64_t part;           // the first of the row's 32 in its slot's numbers
       int64_t lse;            // of the counted rows' log-sum-exps
       int64_t q;              // bytes from the first query's first row to its own, -1: none
     };
     Pieces pieces(P);
-    auto find = [&]() {  // the team's next unit
+    auto find = [&]() {
       Turn t;
       Piece U;
-      t.more = false;
-      while (pieces.next(P, U)) {
-        if (team == 0 || U.rows > 128) {
-          t.more = true;
-          break;
-        }
-      }
+      t.more = pieces.next(P, U);
       if (!t.more) return t;
       const PackedAttnSeq& S = P.a.seq[U.b];
       t.n = U.n, t.key0 = U.tile0 * kKeyTile, t.two = U.rows > 128;
-      t.in = team * 128 + row < U.rows;
+      t.mine = t.two ? t.n : (t.n + 1 - team) / 2;
+      const int at = (t.two ? team * 128 : 0) + row;
+      t.in = at < U.rows;
       t.lim = t.key0 + U.keys;  // rows that are none are not masked, so that whole tiles stay whole: nothing of them is written
-      t.q = t.out = t.lse = 0, t.slot_row = t.part = -1;
-      if (!t.in) t.q = -1;
+      t.out = t.lse = 0, t.slot_row = t.part = t.q = -1;
       if (t.in) {
-        const int r = U.row0 + team * 128 + row, i = r / P.a.group, h = r - i * P.a.group;
+        const int r = U.row0 + at, i = r / P.a.group, h = r - i * P.a.group;
         t.lim = min(t.lim, keys_of_row(S, P.a.group, r));
         const int64_t b = P.a.b0 + U.b, tok = P.a.most - S.count + i;
         t.q = b * P.a.q_bs + (int64_t)(U.hkv * P.a.group + h) * P.a.q_hs + tok * P.a.q_ts;
@@ -311,8 +333,8 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         t.lse = (b * P.a.at.n_kv + U.hkv) * P.a.most * P.a.group + r;
       }
       if (U.slot >= 0) {
-        t.slot_row = (int64_t)U.slot * kBlockRows + team * 128 + row;
-        t.part = ((int64_t)U.slot * kBlockRows + team * 128 + quad * 32) * kDim;
+        t.slot_row = (int64_t)U.slot * kBlockRows + at;
+        t.part = ((int64_t)U.slot * kBlockRows + at - lane) * kDim;
       }
       t.all = __reduce_min_sync(0xffffffffu, t.lim);
       return t;
@@ -333,18 +355,18 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
     };
-    int ns[3] = {0, 0, 0};  // tiles so far of each channel
-    bool ok = true;
+    float2* const ml = reinterpret_cast<float2*>(smem + L::kMl);  // of each team's rows, where both have the same
+    int ns[2] = {0, 0}, n_merged = 0;  // tiles so far of each team; arrivals of both at MERGE
+    bool ok = true, owed = false;      // the other team may still read this one's O
+    const uint32_t tS = tmem + team * 128 + lane_base;
     Turn now = find();
-    if (now.more) queries(now);
+    if (now.more && (now.two || team == 0)) queries(now);
     while (now.more && ok) {
       const Turn next = find();
-      const int step = now.two ? 1 : 2;
       float m = -INFINITY, l = 0.f;
-      for (int i = 0; i < now.n && ok; ++i) {
-        const int ch = channel(now.two, team, i);
-        const uint32_t tS = tmem + buffer(ch) * 128 + lane_base;
-        ok = warp_wait(bar(S_FULL0 + ch), (ns[ch] + i / step) & 1, abort_flag, err, 770);
+      for (int x = 0; x < now.mine && ok; ++x) {
+        const int i = now.two ? x : 2 * x + team;
+        ok = warp_wait(bar(S_FULL0 + team), (ns[team] + x) & 1, abort_flag, err, 770);
         if (!ok) break;
         tc_fence_after();
         const int j0 = now.key0 + i * kKeyTile;
@@ -384,7 +406,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.a.scale_log2;
         const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
         const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
-        const bool scale_o = __any_sync(0xffffffffu, mn != m && m != -INFINITY) && i > 0;
+        const bool scale_o = __any_sync(0xffffffffu, mn != m && m != -INFINITY) && x > 0;
         l *= alpha;
         m = mn;
         const float nm = m == -INFINITY ? 0.f : -m;
@@ -405,8 +427,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
         if (scale_o) {
           // O has the products up to the tile before: wait for the last of them
-          const int pb = channel(now.two, team, i - 1);
-          ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (i - 1) / step) & 1, abort_flag, err, 771);
+          ok = warp_wait(bar(PV_DONE0 + team), (ns[team] + x - 1) & 1, abort_flag, err, 771);
           if (!ok) break;
           tc_fence_after();
           const float2 al = make_float2(alpha, alpha);
@@ -424,27 +445,55 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
           }
         }
         tmem_wait_st();
+        if (owed) ok = warp_wait(bar(MERGE), (n_merged - 1) & 1, abort_flag, err, 773), owed = false;
+        if (!ok) break;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(P_FULL0 + ch));
+        if (lane == 0) mbar_arrive(bar(P_FULL0 + team));
       }
-      // the next unit's queries first, so that its first scores are formed while this one's rows are written
-      if (ok && next.more) queries(next);
-      if (ok) {
-        const int pb = channel(now.two, team, now.n - 1);
-        ok = warp_wait(bar(PV_DONE0 + pb), (ns[pb] + (now.n - 1) / step) & 1, abort_flag, err, 772);
+      const bool merge = !now.two && now.n > 1;
+      // the next unit's queries first, so that its first scores are formed while this one's rows are written; where both teams
+      // have the same queries, once the other one is through with them too
+      const bool load = next.more && (next.two || team == 0);
+      if (ok && load && !merge) queries(next);
+      if (ok && now.mine > 0) ok = warp_wait(bar(PV_DONE0 + team), (ns[team] + now.mine - 1) & 1, abort_flag, err, 772);
+      // rows that both teams have a part of: each writes half of their columns
+      float mine = 1.f, theirs = 0.f;
+      if (ok && merge) {
+        ml[team * 128 + row] = make_float2(m, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(MERGE));
+        ok = warp_wait(bar(MERGE), n_merged++ & 1, abort_flag, err, 775);
+        if (ok) {
+          if (load) queries(next);
+          tc_fence_after();
+          const float2 o = ml[(team ^ 1) * 128 + row];
+          const float mx = fmaxf(m, o.x), ref = mx == -INFINITY ? 0.f : mx;
+          mine = exp2f(m - ref), theirs = exp2f(o.x - ref);
+          l = l * mine + o.y * theirs;
+          m = mx;
+        }
       }
-      if (ok) {
+      if (ok && (now.two || merge || team == 0)) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
+        mine *= inv, theirs *= inv;
 #pragma unroll 1
-        for (int c = 0; c < kDim; c += 32) {
+        for (int c = merge ? team * (kDim / 2) : 0; c < (merge && team == 0 ? kDim / 2 : kDim); c += 32) {
           uint32_t o[32];
           float* f = reinterpret_cast<float*>(o);
           tmem_ld32(tO + c, o);
           tmem_wait_ld32(o);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) f[k] *= inv;
+          for (int k = 0; k < 32; ++k) f[k] *= mine;
+          if (merge) {
+            uint32_t z[32];
+            tmem_ld32(tmem + 256 + (team ^ 1) * 128 + lane_base + c, z);
+            tmem_wait_ld32(z);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) f[k] = fmaf(__uint_as_float(z[k]), theirs, f[k]);
+          }
           if (now.in && now.slot_row >= 0) {
             // partial rows lie in blocks of 32, four columns of all of them side by side: every store is one stretch
             float4* to = reinterpret_cast<float4*>(P.a.part_o + now.part) + (c / 4) * 32 + lane;
@@ -462,7 +511,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
           }
           __syncwarp();
         }
-        if (now.in) {
+        if (now.in && (now.two || team == 0)) {
           const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
           if (now.slot_row >= 0) {
             P.a.part_lse[now.slot_row] = lse;
@@ -473,8 +522,13 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         }
         tc_fence_before();
       }
-      if (now.two) ns[team] += now.n;
-      else ns[0] += (now.n + 1) / 2, ns[2] += now.n / 2;
+      if (ok && merge) {  // both teams' O have been read: no probabilities are handed over before
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(MERGE));
+        ++n_merged, owed = true;
+      }
+      if (now.two) ns[0] += now.n, ns[1] += now.n;
+      else ns[0] += (now.n + 1) / 2, ns[1] += now.n / 2;
       __syncwarp();
       now = next;
     }
@@ -487,7 +541,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
 int packed_tc_launch(const PackedTcParams& P, int dtype, int head_dim, cudaStream_t s) {
   INFLLM_DISPATCH_DTYPE(dtype, T, {
     auto kern = head_dim == 128 ? packed_tc_kernel<T, 128> : packed_tc_kernel<T, 64>;
-    const int smem = (head_dim == 128 ? xtc::Smem<128>::kTotal : xtc::Smem<64>::kTotal) + 1024;
+    const int smem = (head_dim == 128 ? xtc::Smem<128>::kTotal : xtc::Smem<64>::kTotal);
     static std::atomic<uint64_t> set[2];  // devices that know it, per head_dim (and, by the dispatch, type)
     int dev = 0;
     INFLLM_CUDA_OK(cudaGetDevice(&dev));
