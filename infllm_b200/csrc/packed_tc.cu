@@ -107,20 +107,23 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
     // ======================================================================================================== numbers
     // A thread has the 32 numbers of one (m, s): a 16-byte piece of a row of codes.  A turn is a key tile and the value tile before it; the
     // next turn's codes are on their way through registers meanwhile, those kAhead tiles behind it to L2.
+    // (Eight lanes that write 16 bytes at a time have four rows and pieces of one half of them: eight different bank groups.)
     using C = Codes<T>;
     constexpr int kGroups = kDim / 32, kStep = kCodeWarps * 32 / kGroups, kPer = (128 + kStep - 1) / kStep, kAhead = 4;
-    const int at = (warp - kWarpCodes) * 32 + lane, t = at % kGroups, r0 = at / kGroups;
+    constexpr int kRow = kDim / 2, kScales = kDim / 8;  // bytes
+    static_assert(kStep % 8 == 0, "");
+    const int at = (warp - kWarpCodes) * 32 + lane;
+    const int t = kGroups == 4 ? (lane >> 3 & 1) * 2 + (lane & 1) : lane & 1;
+    const int r0 = (warp - kWarpCodes) * (32 / kGroups) + (kGroups == 4 ? (lane >> 4) * 4 + (lane >> 1 & 3) : lane >> 1);
     struct Raw {
-      uint4 c[2][kPer];
-      uint32_t ms[2][kPer];
+      uint32_t c[2][kPer][4], ms[2][kPer];
     };
     struct Turn {
-      int i, n;      // the key tile, of the piece's
-      int keys;      // from its first one to the piece's last
-      int seen;      // of those that every row sees
-      int64_t row;   // of its first one in the layer
       bool more;
-      __device__ __forceinline__ int there(int v) const { return v ? (i > 0 ? min(kKeyTile, keys + kKeyTile) : 0) : i < n ? min(kKeyTile, keys) : 0; }
+      int i, n;   // the key tile, of the piece's
+      int keys;   // from its first one to the piece's last
+      int seen;   // of those that every row sees
+      const char *codes, *scales;  // this thread's of the key tile's first row
     };
     Pieces pieces(P);
     auto begin = [&]() {
@@ -130,61 +133,67 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
       if (o.more) {
         const PackedAttnSeq& S = P.a.seq[U.b];
         o.n = U.n, o.keys = U.keys, o.seen = keys_of_row(S, P.a.group, U.row0) - U.tile0 * kKeyTile;
-        o.row = P.a.at.row0(S.slot, U.hkv) + U.tile0 * kKeyTile;
+        const int64_t row = P.a.at.row0(S.slot, U.hkv) + U.tile0 * kKeyTile;
+        o.codes = P.a.at.codes + row * kRow, o.scales = P.a.at.scales + row * kScales;
       }
       return o;
     };
     auto advance = [&](Turn& o) {
-      if (o.i < o.n) ++o.i, o.keys -= kKeyTile, o.seen -= kKeyTile, o.row += kKeyTile;
+      if (o.i < o.n) ++o.i, o.keys -= kKeyTile, o.seen -= kKeyTile, o.codes += kKeyTile * kRow, o.scales += kKeyTile * kScales;
       else o = begin();
     };
-    const char* const codes0 = P.a.at.codes + r0 * (kDim / 2) + t * 16;
-    const char* const scales0 = P.a.at.scales + r0 * (kDim / 8) + t * 4;
+    const int64_t to_values = P.a.at.codes_v - kKeyTile * kRow, to_value_scales = P.a.at.scales_v - kKeyTile * kScales;
+    const int in_codes = r0 * kRow + t * 16, in_scales = r0 * kScales + t * 4;
+    // lines of 128 bytes of a tile: its codes' and its scales'
+    constexpr int kLines = kRow, kAll = kLines + kScales;
+    static_assert(2 * kAll <= kCodeWarps * 32, "");
+    const bool fetch_values = at >= kAll;
+    const int line = at - fetch_values * kAll;
+    const int fetch_key = kAhead * kKeyTile + (line < kLines ? line * 128 / kRow : (line - kLines) * 128 / kScales);
+    const int64_t fetch = (line < kLines ? (int64_t)fetch_key * kRow : (int64_t)fetch_key * kScales) + (!fetch_values ? 0 : line < kLines ? P.a.at.codes_v : P.a.at.scales_v);
     auto load = [&](const Turn& o, Raw& r) {
+      // what lies behind the last key is not read: its numbers are 0 by their (m, s), whatever their codes
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        const int nk = o.more ? o.there(v) : 0;
-        const int64_t row = o.row - v * kKeyTile;
-        const char* codes = codes0 + v * P.a.at.codes_v + row * (kDim / 2);
-        const char* scales = scales0 + v * P.a.at.scales_v + row * (kDim / 8);
+        const int nk = !o.more ? 0 : v ? (o.i > 0 ? o.keys + kKeyTile : 0) : o.i < o.n ? o.keys : 0;
+        const char* codes = o.codes + in_codes + (v ? to_values : 0);
+        const char* scales = o.scales + in_scales + (v ? to_value_scales : 0);
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          r.c[v][x] = make_uint4(0, 0, 0, 0), r.ms[v][x] = 0;  // (what lies behind the last key is not read: zeros)
-          if (r0 + x * kStep < nk) {
-            r.c[v][x] = ld_stream16(codes + x * kStep * (kDim / 2));
-            r.ms[v][x] = __ldg(reinterpret_cast<const uint32_t*>(scales + x * kStep * (kDim / 8)));
-          }
+          const bool there = r0 + x * kStep < min(nk, kKeyTile);
+          r.ms[v][x] = 0;
+          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+                       "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%5];\n\t"
+                       "@p ld.global.nc.u32 %4, [%6];\n\t}"
+                       : "+r"(r.c[v][x][0]), "+r"(r.c[v][x][1]), "+r"(r.c[v][x][2]), "+r"(r.c[v][x][3]), "+r"(r.ms[v][x])
+                       : "l"(codes + x * kStep * kRow), "l"(scales + x * kStep * kScales), "r"((int)there));
         }
       }
-      // (a line of 128 bytes has the codes of two or four rows, the scales of eight or sixteen)
-      constexpr int kLine = 128 / (kDim / 2), kScaleLine = 128 / (kDim / 8), kLines = 128 / kLine, kAll = kLines + 128 / kScaleLine;
-      static_assert(2 * kAll <= kCodeWarps * 32, "");
-      const int v = at >= kAll, y = at - v * kAll, k = kAhead * kKeyTile + (y < kLines ? y * kLine : (y - kLines) * kScaleLine);
-      if (o.more && at < 2 * kAll && k < o.keys)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(y < kLines ? P.a.at.codes + v * P.a.at.codes_v + (o.row + k) * (kDim / 2)
-                                                               : P.a.at.scales + v * P.a.at.scales_v + (o.row + k) * (kDim / 8)));
+      if (o.more && at < 2 * kAll && fetch_key < o.keys) asm volatile("prefetch.global.L2 [%0];" ::"l"((line < kLines ? o.codes : o.scales) + fetch));
     };
+    uint32_t piece[4];  // of a tile: where this thread's 16 bytes go
+#pragma unroll
+    for (int j = 0; j < 4; ++j) piece[j] = (t >> 1) * kSubTileBytes + r0 * 128 + ((((t & 1) * 4 + j) ^ (r0 & 7)) << 4);
     bool ok = true;
     int slot = 0;
-    Raw raw;
+    Raw raw{}, then{};
     Turn now = begin();
     load(now, raw);
     while (now.more && ok) {
       Turn after = now;
       advance(after);
-      Raw then;
       load(after, then);
       if (now.seen < kKeyTile) {
         // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and
         // its key is no number in its place, so that the rows that see it still become none.
-        const char* scales = P.a.at.scales + P.a.at.scales_v + now.row * (kDim / 8);
+        const char* scales = now.scales + P.a.at.scales_v;
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
           const int k = r0 + x * kStep;
           if (now.seen < 0 && C::odd(raw.ms[1][x])) raw.ms[1][x] = 0;
-          if (k < now.there(0))
+          if (now.i < now.n && k < min(now.keys, kKeyTile))
             for (int g = 0; g < kGroups; ++g)
-              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + k * (kDim / 8) + g * 4)))) raw.ms[0][x] = 0x7fff7fffu;
+              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + k * kScales + g * 4)))) raw.ms[0][x] = 0x7fff7fffu;
         }
       }
       const int first = slot;
@@ -194,10 +203,18 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         const int b = slot % kStages;
         if (ok && slot >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot - kStages, kStages), abort_flag, err, 751);
         if (ok) {
-          unsigned char* to = smem + L::kRing + b * L::kTileBytes + (t >> 1) * kSubTileBytes;
+          unsigned char* to = smem + L::kRing + b * L::kTileBytes;
 #pragma unroll
-          for (int x = 0; x < kPer; ++x)
-            if ((x + 1) * kStep <= 128 || r0 + x * kStep < 128) put_group<T>(to, r0 + x * kStep, t, raw.c[v][x], raw.ms[v][x]);
+          for (int x = 0; x < kPer; ++x) {
+            if ((x + 1) * kStep > 128 && r0 + x * kStep >= 128) continue;
+            const auto m2 = C::least2(raw.ms[v][x]), s2 = C::step2(raw.ms[v][x]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+              C::pairs(raw.c[v][x][j], m2, s2, w);
+              *reinterpret_cast<uint4*>(to + piece[j] + x * kStep * 128) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
         }
         ++slot;
       }
@@ -305,6 +322,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
     const uint32_t tO = tmem + 256 + team * 128 + lane_base;
     struct Turn {  // a unit, and this thread's row of it
       bool more, two, in;
+      bool idle;  // the warp has no row of it: what it leaves in P is of rows that nobody looks at
       int n, mine, key0, lim, all;  // its tiles; this team's
       int64_t out, slot_row;  // row of the output; of the partial results, -1: the unit is whole
       int64_t part;           // the first of the row's 32 in its slot's numbers
@@ -337,6 +355,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         t.part = ((int64_t)U.slot * kBlockRows + at - lane) * kDim;
       }
       t.all = __reduce_min_sync(0xffffffffu, t.lim);
+      t.idle = at - lane >= U.rows;
       return t;
     };
     auto queries = [&](const Turn& t) {
@@ -369,6 +388,14 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         ok = warp_wait(bar(S_FULL0 + team), (ns[team] + x) & 1, abort_flag, err, 770);
         if (!ok) break;
         tc_fence_after();
+        if (now.idle) {
+          if (owed) ok = warp_wait(bar(MERGE), (n_merged - 1) & 1, abort_flag, err, 773), owed = false;
+          if (!ok) break;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(P_FULL0 + team));
+          continue;
+        }
         const int j0 = now.key0 + i * kKeyTile;
         if (now.all < j0 + kKeyTile) {
           // what a row does not see is taken out of the scores where they are
