@@ -252,18 +252,19 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
   const int whole = min(key1, least) - 16;  // the last place of a group that all rows see all of
   int j0 = key0 + warp * 16;
   if (j0 <= whole) {
-    // a group is on its way while the one before it is worked on
-    typename W::Key k = key(j0);
-    typename W::Value v = value(j0);
-#pragma unroll 1
-    for (; j0 + kStep <= whole; j0 += kStep) {
-      const typename W::Key kn = key(j0 + kStep);
-      const typename W::Value vn = value(j0 + kStep);
+    // A group is on its way while the one before it is worked on: two copies of the work, each with its own registers, as what is on
+    // its way is not to be moved, which would wait for it.
+    typename W::Key k0 = key(j0), k1;
+    typename W::Value v0 = value(j0), v1;
+    auto turn = [&](const typename W::Key& k, const typename W::Value& v, typename W::Key& kn, typename W::Value& vn) {
+      const bool more = j0 + kStep <= whole;
+      if (more) kn = key(j0 + kStep), vn = value(j0 + kStep);
       w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
-      k = kn, v = vn;
+      j0 += kStep;
+      return more;
+    };
+    while (turn(k0, v0, k1, v1) && turn(k1, v1, k0, v0)) {
     }
-    w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
-    j0 += kStep;
   }
 #pragma unroll 1
   for (; j0 < key1; j0 += kStep) {

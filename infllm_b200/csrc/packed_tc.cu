@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
     Raw raw{}, then{};
     Turn now = begin();
     load(now, raw);
-    while (now.more && ok) {
+    // (two copies of a turn, each with its own registers: what is on its way is not to be moved, which would wait for it)
+    auto turn = [&](Raw& raw, Raw& then) {
       Turn after = now;
       advance(after);
       load(after, then);
@@ -218,11 +219,14 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         }
         ++slot;
       }
-      if (!ok) break;
+      if (!ok) return false;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane < slot - first) mbar_arrive(bar(FULL0 + (first + lane) % kStages));
-      now = after, raw = then;
+      now = after;
+      return now.more;
+    };
+    while (now.more && turn(raw, then) && turn(then, raw)) {
     }
     // nothing will be signalled in this block when it goes: the releases come behind all products
     for (int b = 0; b < kStages && ok; ++b) {
