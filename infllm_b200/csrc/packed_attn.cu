@@ -19,7 +19,7 @@ namespace infllm {
 
 using namespace mma;
 
-constexpr int kAttnWarps = 4, kAttnTile = 16;
+constexpr int kAttnWarps = 4, kFewRows = 8;
 
 __device__ __forceinline__ uint2 ld_stream8(const void* p) {
   uint2 r;
@@ -32,40 +32,32 @@ __device__ __forceinline__ uint32_t ld_stream4(const void* p) {
   return r;
 }
 
-// --------------------------------------------------------------------------------------------------------- a warp's part
-// Groups of 16 keys against up to 16 rows, from global memory straight into the operands of the m16n8k16 products: a thread's codes of
-// a key are those of the 32 numbers of one (m, s) (kDim 128), its codes of a value an eighth of the row.
-template <typename T, int kDim, int kNt>  // kNt: tiles of eight rows
-struct PackedWarp {
+// ------------------------------------------------------------------------------------------------------- few rows
+// Up to eight rows of a KV head.  A warp takes groups of 16 keys, keys and values from global memory through registers into operands of the
+// m16n8k16 products:
+//   S^T = K Q^T       keys are rows: a thread's codes of a key are the numbers of one (m, s) (kDim 128) or of half a one
+//   O^T += V^T P^T    numbers of the values are rows: a thread's codes of a value are an eighth of it, and two keys' are paired as they
+//                     are taken out.  P^T is S^T's place with keys and rows exchanged: two 8 x 8 transpositions in the warp.
+// P is two 16-bit numbers, p = hi + lo, so that an output's only rounding is its own: where rows are no more than four (kFour), the other
+// four columns have the same rows again, and theirs is lo, in the same product.
+// The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled and do lanes exchange
+// anything.
+template <typename T, int kDim, bool kFour>
+struct PackedRows {
   static constexpr int kW = kDim / 32;  // words of a key, kDim / 4 numbers, that a thread has: as many of Q's 16-byte pieces
   static constexpr int kH = kDim / 64;  // of a value, kDim / 8 numbers
+  static constexpr int kRow = kDim / 2, kScales = kDim / 8, kTiles = 4 * kH;
   using C = Codes<T>;
-  const char* from[kNt];
-  uint4 qf[kNt][kW];
-  int lim[kNt];
-
-  // the rows row0 + 0 .. 15 of a sequence's new tokens
-  __device__ __forceinline__ void rows(const PackedAttnParams& P, const PackedAttnSeq& S, int b, int hkv, int row0) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int x = 0; x < kNt; ++x) {
-      const int r = row0 + x * 8 + g, i = r / P.group, h = r - i * P.group;
-      lim[x] = 0, from[x] = nullptr;
-      if (i < S.count) {
-        lim[x] = S.length - S.count + i + 1;
-        from[x] = P.q + (int64_t)(P.b0 + b) * P.q_bs + (int64_t)(hkv * P.group + h) * P.q_hs + (int64_t)(P.most - S.count + i) * P.q_ts + t * (kDim / 2);
-      }
-    }
-  }
-  __device__ __forceinline__ void queries() {
-#pragma unroll
-    for (int x = 0; x < kNt; ++x)
-#pragma unroll
-      for (int j = 0; j < kW; ++j) qf[x][j] = from[x] ? __ldg(reinterpret_cast<const uint4*>(from[x] + j * 16)) : make_uint4(0, 0, 0, 0);
-  }
+  const uint4* qf;     // row g's pieces, in shared memory: [piece][lane].  (The registers are worth more than four loads a group.)
+  int lim[2];          // keys that rows 2t and 2t + 1 see
+  float ot[kTiles][4];  // O^T: [0], [1] = number g * kDim / 8 + 2i of columns 2t, 2t + 1; [2], [3] = the next one
+  float m[2], l[2];
 
   struct Key {  // rows nt * 8 + g
     uint32_t w[2][kW], ms[2];
+  };
+  struct Value {  // rows 2t, 2t + 1, 2t + 8, 2t + 9
+    uint32_t w[4][kH], ms[4];
   };
   template <bool kAll>  // all 16 keys are there
   __device__ __forceinline__ static Key key(const char* codes, const char* scales, int nk) {
@@ -75,38 +67,17 @@ struct PackedWarp {
     for (int nt = 0; nt < 2; ++nt) {
       const int r = kAll ? nt * 8 + g : min(nt * 8 + g, nk - 1);  // (what lies behind the last key is not read: it may not be a number, and 0 times that is none)
       if (kDim == 128) {
-        const uint4 x = ld_stream16(codes + r * 64 + t * 16);
+        const uint4 x = ld_stream16(codes + r * kRow + t * 16);
         k.w[nt][0] = x.x, k.w[nt][1] = x.y, k.w[nt][2 % kW] = x.z, k.w[nt][3 % kW] = x.w;
-        k.ms[nt] = ld_stream4(scales + r * 16 + t * 4);
+        k.ms[nt] = ld_stream4(scales + r * kScales + t * 4);
       } else {
-        const uint2 x = ld_stream8(codes + r * 32 + t * 8);
+        const uint2 x = ld_stream8(codes + r * kRow + t * 8);
         k.w[nt][0] = x.x, k.w[nt][1] = x.y;
-        k.ms[nt] = ld_stream4(scales + r * 8 + (t >> 1) * 4);
+        k.ms[nt] = ld_stream4(scales + r * kScales + (t >> 1) * 4);
       }
     }
     return k;
   }
-  // scores of rows g (and 8 + g) by keys nt * 8 + 2t, + 1
-  __device__ __forceinline__ void scores(const Key& k, float (*s)[4]) const {
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const auto m2 = C::least2(k.ms[nt]), s2 = C::step2(k.ms[nt]);
-      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < kW; ++j) {
-        uint32_t v[4];
-        C::pairs(k.w[nt][j], m2, s2, v);
-        const uint32_t a0[4] = {qf[0][j].x, kNt > 1 ? qf[kNt - 1][j].x : 0u, qf[0][j].y, kNt > 1 ? qf[kNt - 1][j].y : 0u};
-        mma16816<T>(s[nt], a0, v[0], v[1]);
-        const uint32_t a1[4] = {qf[0][j].z, kNt > 1 ? qf[kNt - 1][j].z : 0u, qf[0][j].w, kNt > 1 ? qf[kNt - 1][j].w : 0u};
-        mma16816<T>(s[nt], a1, v[2], v[3]);
-      }
-    }
-  }
-
-  struct Value {  // rows 2t, 2t + 1, 2t + 8, 2t + 9: numbers g * kDim / 8 .. of each
-    uint32_t w[4][kH], ms[4];
-  };
   template <bool kAll>
   __device__ __forceinline__ static Value value(const char* codes, const char* scales, int nk) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -115,89 +86,97 @@ struct PackedWarp {
     for (int ki = 0; ki < 4; ++ki) {
       const int at = 2 * t + (ki & 1) + (ki >> 1) * 8, r = kAll ? at : min(at, nk - 1);
       if (kDim == 128) {
-        const uint2 x = ld_stream8(codes + r * 64 + g * 8);
+        const uint2 x = ld_stream8(codes + r * kRow + g * 8);
         v.w[ki][0] = x.x, v.w[ki][kH - 1] = x.y;
-        v.ms[ki] = ld_stream4(scales + r * 16 + (g >> 1) * 4);
+        v.ms[ki] = ld_stream4(scales + r * kScales + (g >> 1) * 4);
       } else {
-        v.w[ki][0] = ld_stream4(codes + r * 32 + g * 4);
-        v.ms[ki] = ld_stream4(scales + r * 8 + (g >> 2) * 4);
+        v.w[ki][0] = ld_stream4(codes + r * kRow + g * 4);
+        v.ms[ki] = ld_stream4(scales + r * kScales + (g >> 2) * 4);
       }
     }
     return v;
   }
-};
-
-// --------------------------------------------------------------------------------------------------------- attention
-// Four warps share a stretch's groups of 16 keys and meet in shared memory.  P is two 16-bit numbers, p = hi + lo, so that an output's
-// only rounding is its own.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is
-// scaled and do lanes that share a row exchange anything.
-template <typename T, int kDim, int kNt>
-struct PackedRows : PackedWarp<T, kDim, kNt> {
-  using W = PackedWarp<T, kDim, kNt>;
-  using C = Codes<T>;
-  static constexpr int kTiles = 4 * W::kH;
-  float ot[kTiles][kNt][4];  // O^T: [0], [1] = number g * kDim / 8 + 2i of rows 2t, 2t + 1; [2], [3] = the next one
-  float m[kNt], l[kNt];
 
   __device__ __forceinline__ void clear() {
+    m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
 #pragma unroll
-    for (int x = 0; x < kNt; ++x) {
-      m[x] = -INFINITY, l[x] = 0.f;
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) ot[i][x][0] = ot[i][x][1] = ot[i][x][2] = ot[i][x][3] = 0.f;
-    }
+    for (int i = 0; i < kTiles; ++i) ot[i][0] = ot[i][1] = ot[i][2] = ot[i][3] = 0.f;
+  }
+  static __device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  }
+  static __device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
   }
 
   // 16 keys from j0 on; kAll: every row sees all of them.  Otherwise those below key1, and a row those below its own limit.
+  // logits: the scores' place of this thread's first row and key g, null: none is wanted
   template <bool kAll>
-  __device__ __forceinline__ void group(const typename W::Key& k, const typename W::Value& v, int j0, int key1, float scale_log2, float* logits, int64_t pitch) {
-    const int lane = threadIdx.x & 31, t = lane & 3;
-    float s[2][4];
-    this->scores(k, s);
-    uint32_t hi[kNt][2], lo[kNt][2];
+  __device__ __forceinline__ void group(const Key& k, const Value& v, int j0, int key1, float scale_log2, float* logits, int64_t pitch, bool two) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // key g of rows 2t, 2t + 1; key g + 8
+    {
+      const auto m0 = C::least2(k.ms[0]), s0 = C::step2(k.ms[0]), m1 = C::least2(k.ms[1]), s1 = C::step2(k.ms[1]);
 #pragma unroll
-    for (int x = 0; x < kNt; ++x) {  // row x * 8 + g: keys nt * 8 + 2t + e
-      float p[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[e] = s[e >> 1][x * 2 + (e & 1)] * scale_log2;
-        if (!kAll && j0 + (e >> 1) * 8 + 2 * t + (e & 1) >= min(this->lim[x], key1)) p[e] = -INFINITY;
+      for (int j = 0; j < kW; ++j) {
+        const uint4 q = qf[j * 32];
+        uint32_t a[4], b[4];
+        C::pairs(k.w[0][j], m0, s0, a);
+        C::pairs(k.w[1][j], m1, s1, b);
+        const uint32_t x[4] = {a[0], b[0], a[1], b[1]}, y[4] = {a[2], b[2], a[3], b[3]};
+        mma16816<T>(s, x, q.x, q.y);
+        mma16816<T>(s, y, q.z, q.w);
       }
-      if (logits) {
+    }
+    if (!kAll) {
 #pragma unroll
-        for (int e = 0; e < 4; e += 2)
-          if (kAll || j0 + e * 4 + 2 * t < key1) *reinterpret_cast<float2*>(logits + j0 + e * 4) = make_float2(p[e], p[e + 1]);
-      }
-      float mx = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
-      if (__any_sync(0xffffffffu, mx > m[x] + 8.f)) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = mx > m[x] + 8.f ? mx : m[x];
-        const float al = m[x] == -INFINITY ? 0.f : exp2f(m[x] - mn);
-        m[x] = mn;
-        l[x] *= al;
-        // this thread's columns of O^T are rows 2t and 2t + 1
-        const float a0 = __shfl_sync(0xffffffffu, al, (2 * t) * 4), a1 = __shfl_sync(0xffffffffu, al, (2 * t + 1) * 4);
+      for (int e = 0; e < 4; ++e)
+        if (j0 + (e >> 1) * 8 + g >= min(lim[e & 1], key1)) s[e] = -INFINITY;
+    }
+    if (logits) {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) ot[i][x][0] *= a0, ot[i][x][1] *= a1, ot[i][x][2] *= a0, ot[i][x][3] *= a1;
-      }
-      const float ms = !kAll && m[x] == -INFINITY ? 0.f : m[x];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = ex2(p[e] - ms);
-      l[x] += (p[0] + p[1]) + (p[2] + p[3]);
+      for (int e = 0; e < 4; ++e)
+        if ((kAll || j0 + (e >> 1) * 8 + g < key1) && (!(e & 1) || two)) logits[(e & 1) * pitch + j0 + (e >> 1) * 8] = s[e] * scale_log2;
+    }
+    float mx[2] = {fmaxf(s[0], s[2]) * scale_log2, fmaxf(s[1], s[3]) * scale_log2};
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+      float al[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        typename Act<T>::T2 h = Act<T>::from_f2(p[2 * e], p[2 * e + 1]);
-        hi[x][e] = *reinterpret_cast<uint32_t*>(&h);
-        const float2 f = Act<T>::to_f2(h);
-        lo[x][e] = pack2<T>(p[2 * e] - f.x, p[2 * e + 1] - f.y);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
+        const float mn = mx[e] > m[e] + 8.f ? mx[e] : m[e];
+        al[e] = m[e] == -INFINITY ? 0.f : exp2f(m[e] - mn);
+        m[e] = mn;
+        l[e] *= al[e];
       }
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) ot[i][0] *= al[0], ot[i][1] *= al[1], ot[i][2] *= al[0], ot[i][3] *= al[1];
+    }
+    const float r0 = !kAll && m[0] == -INFINITY ? 0.f : -m[0], r1 = !kAll && m[1] == -INFINITY ? 0.f : -m[1];
+    const float p[4] = {ex2(fmaf(s[0], scale_log2, r0)), ex2(fmaf(s[1], scale_log2, r1)), ex2(fmaf(s[2], scale_log2, r0)), ex2(fmaf(s[3], scale_log2, r1))};
+    l[0] += p[0] + p[2];
+    l[1] += p[1] + p[3];
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      typename Act<T>::T2 h = Act<T>::from_f2(p[2 * e], p[2 * e + 1]);
+      hi[e] = *reinterpret_cast<uint32_t*>(&h);
+      const float2 f = Act<T>::to_f2(h);
+      lo[e] = pack2<T>(p[2 * e] - f.x, p[2 * e + 1] - f.y);
+      if (kFour) hi[e] = t < 2 ? hi[e] : lo[e];
+      hi[e] = transposed(hi[e]);
+      if (!kFour) lo[e] = transposed(lo[e]);
     }
     // A operands: numbers of keys 2t, 2t + 1 and of 2t + 8, 2t + 9
     const auto m01 = C::least2(v.ms[0], v.ms[1]), s01 = C::step2(v.ms[0], v.ms[1]);
     const auto m23 = C::least2(v.ms[2], v.ms[3]), s23 = C::step2(v.ms[2], v.ms[3]);
 #pragma unroll
-    for (int j = 0; j < W::kH; ++j) {
+    for (int j = 0; j < kH; ++j) {
       uint32_t e01[4], o01[4], e23[4], o23[4];
       C::pairs(__byte_perm(v.w[0][j], v.w[1][j], 0x5410), m01, s01, e01);
       C::pairs(__byte_perm(v.w[0][j], v.w[1][j], 0x7632), m01, s01, o01);
@@ -206,60 +185,65 @@ struct PackedRows : PackedWarp<T, kDim, kNt> {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a[4] = {e01[i], o01[i], e23[i], o23[i]};
-#pragma unroll
-        for (int x = 0; x < kNt; ++x) {
-          mma16816<T>(ot[j * 4 + i][x], a, hi[x][0], hi[x][1]);
-          mma16816<T>(ot[j * 4 + i][x], a, lo[x][0], lo[x][1]);
-        }
+        mma16816<T>(ot[j * 4 + i], a, hi[0], hi[1]);
+        if (!kFour) mma16816<T>(ot[j * 4 + i], a, lo[0], lo[1]);
       }
     }
   }
-  static __device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-  }
 };
 
-template <typename T, int kDim, int kNt>
-__global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_kernel(const __grid_constant__ PackedAttnParams P) {
-  using R = PackedRows<T, kDim, kNt>;
-  using W = typename R::W;
+// Four warps share a stretch's groups of 16 keys and meet in shared memory.
+template <typename T, int kDim, bool kFour>
+__global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const __grid_constant__ PackedAttnParams P) {
+  using R = PackedRows<T, kDim, kFour>;
   using C = Codes<T>;
-  constexpr int kTiles = R::kTiles, kPitch = kDim + 4, kStep = kAttnWarps * 16;
-  __shared__ __align__(16) float sm_o[kAttnWarps][8 * kNt][kPitch];
-  __shared__ float sm_m[kAttnWarps][8 * kNt], sm_l[kAttnWarps][8 * kNt];
+  constexpr int kPitch = kDim + 4, kStep = kAttnWarps * 16;
+  __shared__ __align__(16) float sm_o[kAttnWarps][8][kPitch];
+  __shared__ float sm_m[kAttnWarps][8], sm_l[kAttnWarps][8];
+  __shared__ uint4 sm_q[R::kW][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int unit = blockIdx.x, hkv = blockIdx.y, b = seq_of(P, unit);
   const PackedAttnSeq S = P.seq[b];
-  const int tile = (unit - S.unit0) / S.chunks, key0 = (unit - S.unit0 - tile * S.chunks) * S.keys, row0 = tile * kAttnTile;
-  const int rows = min(8 * kNt, S.count * P.group - row0);
-  const int key1 = min(key0 + S.keys, keys_of_row(S, P.group, row0 + rows - 1));  // (the last row's: the others see no more)
-  const int least = keys_of_row(S, P.group, row0);  // keys that every row sees
+  const int key0 = (unit - S.unit0) * S.keys, rows = S.count * P.group;
+  const int key1 = min(key0 + S.keys, S.length);
+  const int least = keys_of_row(S, P.group, 0);  // keys that every row sees
   R w;
-  w.rows(P, S, b, hkv, row0);
-  const int64_t first = P.at.row0(S.slot, hkv);
-  const char* kc = P.at.codes + first * (kDim / 2);
-  const char* ks = P.at.scales + first * (kDim / 8);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = kFour ? (2 * t + e) & 3 : 2 * t + e;
+    w.lim[e] = r < rows ? keys_of_row(S, P.group, r) : 0;
+  }
+  const int64_t first = P.at.row0(S.slot, hkv) + key0;  // (the stretch's first row)
+  const char* kc = P.at.codes + first * R::kRow;
+  const char* ks = P.at.scales + first * R::kScales;
   const char* vc = kc + P.at.codes_v;
   const char* vs = ks + P.at.scales_v;
-  float* logits = kNt == 1 && P.logits && g < rows ? P.logits + (((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.logit_rows + g) * P.pitch + 2 * t : nullptr;
+  float* logits = nullptr;
+  if (P.logits && 2 * t < rows) logits = P.logits + (((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.logit_rows + 2 * t) * P.pitch + g;
+  const bool two = 2 * t + 1 < rows;
   chain_enter();
-  w.queries();
+  if (warp < R::kW) {  // a piece of every row by a warp
+    const int r = kFour ? g & 3 : g, i = r / P.group, h = r - i * P.group;
+    const char* from = P.q + (int64_t)(P.b0 + b) * P.q_bs + (int64_t)(hkv * P.group + h) * P.q_hs + (int64_t)(P.most - S.count + i) * P.q_ts;
+    sm_q[warp][lane] = r < rows ? __ldg(reinterpret_cast<const uint4*>(from + t * (kDim / 2) + warp * 16)) : make_uint4(0, 0, 0, 0);
+  }
+  w.qf = &sm_q[0][lane];
   w.clear();
-  auto key = [&](int j) { return W::template key<true>(kc + (int64_t)j * (kDim / 2), ks + (int64_t)j * (kDim / 8), 16); };
-  auto value = [&](int j) { return W::template value<true>(vc + (int64_t)j * (kDim / 2), vs + (int64_t)j * (kDim / 8), 16); };
+  auto key = [&](int j) { return R::template key<true>(kc + (int64_t)(j - key0) * R::kRow, ks + (int64_t)(j - key0) * R::kScales, 16); };
+  auto value = [&](int j) { return R::template value<true>(vc + (int64_t)(j - key0) * R::kRow, vs + (int64_t)(j - key0) * R::kScales, 16); };
   const int whole = min(key1, least) - 16;  // the last place of a group that all rows see all of
   int j0 = key0 + warp * 16;
+  // A group is on its way while the one before it is worked on: two copies of the work, each with its own registers, as what is on its
+  // way is not to be moved, which would wait for it.
+  typename R::Key k0, k1;
+  typename R::Value v0, v1;
+  if (j0 <= whole) k0 = key(j0), v0 = value(j0);
+  __syncthreads();
   if (j0 <= whole) {
-    // A group is on its way while the one before it is worked on: two copies of the work, each with its own registers, as what is on
-    // its way is not to be moved, which would wait for it.
-    typename W::Key k0 = key(j0), k1;
-    typename W::Value v0 = value(j0), v1;
-    auto turn = [&](const typename W::Key& k, const typename W::Value& v, typename W::Key& kn, typename W::Value& vn) {
+    auto turn = [&](const typename R::Key& k, const typename R::Value& v, typename R::Key& kn, typename R::Value& vn) {
       const bool more = j0 + kStep <= whole;
       if (more) kn = key(j0 + kStep), vn = value(j0 + kStep);
-      w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
+      w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
       j0 += kStep;
       return more;
     };
@@ -269,8 +253,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
 #pragma unroll 1
   for (; j0 < key1; j0 += kStep) {
     const int nk = min(16, key1 - j0);
-    typename W::Key k = W::template key<false>(kc + (int64_t)j0 * (kDim / 2), ks + (int64_t)j0 * (kDim / 8), nk);
-    typename W::Value v = W::template value<false>(vc + (int64_t)j0 * (kDim / 2), vs + (int64_t)j0 * (kDim / 8), nk);
+    const int64_t at = j0 - key0;
+    typename R::Key k = R::template key<false>(kc + at * R::kRow, ks + at * R::kScales, nk);
+    typename R::Value v = R::template value<false>(vc + at * R::kRow, vs + at * R::kScales, nk);
     // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and its
     // key is no number in its place, so that the rows that see it still become none.
     uint32_t bad = 0;
@@ -286,21 +271,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
       if (bad >> (nt * 8 + g) & 1) k.ms[nt] = 0x7fff7fffu;
-    w.template group<false>(k, v, j0, key1, P.scale_log2, logits, P.pitch);
+    w.template group<false>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
   }
-  float (&ot)[kTiles][kNt][4] = w.ot;
-  float (&m)[kNt] = w.m, (&l)[kNt] = w.l;
 #pragma unroll
-  for (int x = 0; x < kNt; ++x) {
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-    if (l[x] != l[x] && m[x] == -INFINITY) m[x] = 0.f;  // (scores that are no numbers are not seen by the maximum)
-    if (t == 0) sm_m[warp][x * 8 + g] = m[x], sm_l[warp][x * 8 + g] = l[x];
+  for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i)
+    for (int o = 4; o < 32; o <<= 1) w.l[e] += __shfl_xor_sync(0xffffffffu, w.l[e], o);
+    if (w.l[e] != w.l[e] && w.m[e] == -INFINITY) w.m[e] = 0.f;  // (scores that are no numbers are not seen by the maximum)
+    if (g == 0) sm_m[warp][2 * t + e] = w.m[e], sm_l[warp][2 * t + e] = w.l[e];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float2*>(&sm_o[warp][x * 8 + 2 * t + e][g * (kDim / 8) + 2 * i]) = make_float2(ot[i][x][e], ot[i][x][2 + e]);
+    for (int i = 0; i < R::kTiles; ++i) *reinterpret_cast<float2*>(&sm_o[warp][2 * t + e][g * (kDim / 8) + 2 * i]) = make_float2(w.ot[i][e], w.ot[i][2 + e]);
   }
   __syncthreads();
   for (int idx = tid; idx < rows * (kDim / 2); idx += kAttnWarps * 32) {  // two neighbouring numbers each
@@ -314,22 +294,21 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kNt > 1 ? 3 : 4) packed_rows_
       for (int y = 0; y < kAttnWarps; ++y) {
         const float wt = exp2f(sm_m[y][r] - mx);
         den = fmaf(wt, sm_l[y][r], den);
-        n0 = fmaf(wt, sm_o[y][r][d], n0);
-        n1 = fmaf(wt, sm_o[y][r][d + 1], n1);
+        n0 = fmaf(wt, kFour ? sm_o[y][r][d] + sm_o[y][r + 4][d] : sm_o[y][r][d], n0);
+        n1 = fmaf(wt, kFour ? sm_o[y][r][d + 1] + sm_o[y][r + 4][d + 1] : sm_o[y][r][d + 1], n1);
       }
       n0 /= den, n1 /= den;
     }
     const float lse = mx == -INFINITY ? -INFINITY : mx + log2f(den);
-    const int64_t pr = ((int64_t)unit * P.at.n_kv + hkv) * kAttnTile + r;
+    const int64_t pr = ((int64_t)unit * P.at.n_kv + hkv) * kFewRows + r;
     if (d == 0 && (S.chunks > 1 || P.logits)) P.part_lse[pr] = lse;
     if (S.chunks > 1) {
       *reinterpret_cast<float2*>(P.part_o + pr * kDim + d) = make_float2(n0, n1);
     } else {
-      const int i = (row0 + r) / P.group, h = row0 + r - i * P.group;
+      const int i = r / P.group, h = r - i * P.group;
       const int64_t orow = ((int64_t)(P.b0 + b) * P.most + P.most - S.count + i) * (P.at.n_kv * P.group) + hkv * P.group + h;
       *reinterpret_cast<uint32_t*>(P.out + (orow * kDim + d) * 2) = pack2<T>(n0, n1);
       if (P.lse && d == 0) P.lse[orow] = lse * (1.f / kLog2e);
-      if (P.row_lse && d == 0) P.row_lse[((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group + row0 + r] = lse;
     }
   }
 }
@@ -359,7 +338,7 @@ __device__ __forceinline__ void sum_weights(const PackedAttnParams& P, int block
   if (rows == 0 || key0 >= S.length) return;
   if (warp < rows) {  // a row's log-sum-exp, of its parts'
     float mx = -INFINITY, sum = 0.f;
-    auto part = [&](int c) { return P.part_lse[((int64_t)(S.unit0 + c) * P.at.n_kv + hkv) * kAttnTile + warp]; };
+    auto part = [&](int c) { return P.part_lse[((int64_t)(S.unit0 + c) * P.at.n_kv + hkv) * kFewRows + warp]; };
     for (int c = lane; c < S.chunks; c += 32) mx = fmaxf(mx, part(c));
     mx = warp_max(mx);
     if (mx == -INFINITY) mx = 0.f;  // (where all are no numbers)
@@ -418,7 +397,7 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
       const int2 s = All.start[block0 + c];
       return (int64_t)(2 * (block0 + c) + (s.x < unit)) * kBlockRows + r % kBlockRows;
     } else {
-      return ((int64_t)(S.unit0 + r / kAttnTile * S.chunks + c) * P.at.n_kv + hkv) * kAttnTile + r % kAttnTile;
+      return ((int64_t)(S.unit0 + c) * P.at.n_kv + hkv) * kFewRows + r;
     }
   };
   chain_enter();
@@ -509,61 +488,16 @@ static int join_launch(typename JoinParams<kTc>::type& P, PackedAttnParams& A, b
   return INFLLM_OK;
 }
 
-// --------------------------------------------------------------------------------------------------------- the weights
-// A warp has a group of 16 keys, forms its scores with all counted rows again and adds up what they give each key.
-template <typename T, int kDim>
-__global__ void __launch_bounds__(128) packed_weigh_kernel(const __grid_constant__ PackedAttnParams P) {
-  using W = PackedWarp<T, kDim, 2>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.z, hkv = blockIdx.y, j0 = ((int)blockIdx.x * 4 + (threadIdx.x >> 5)) * 16;
-  const PackedAttnSeq S = P.seq[b];
-  chain_enter();
-  if (S.count == 0 || j0 >= S.length) return;
-  const int nk = min(16, S.length - j0);
-  const int64_t first = P.at.row0(S.slot, hkv) + j0;
-  const typename W::Key k = W::template key<false>(P.at.codes + first * (kDim / 2), P.at.scales + first * (kDim / 8), nk);
-  const float* row_lse = P.row_lse + ((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group;
-  // the rows from the first counted token, or the first that sees one of the keys, on
-  const int from = max(S.count - min(P.weigh, S.count), j0 - (S.length - S.count)) * P.group;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int row0 = from; row0 < S.count * P.group; row0 += kAttnTile) {
-    W w;
-    w.rows(P, S, b, hkv, row0);
-    w.queries();
-    float s[2][4];
-    w.scores(k, s);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = row0 + x * 8 + g;
-      if (r >= S.count * P.group) continue;
-      const float lse = row_lse[r];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = j0 + (e >> 1) * 8 + 2 * t + (e & 1);
-        if (key < w.lim[x]) sum[e] += exp2f(s[e >> 1][x * 2 + (e & 1)] * P.scale_log2 - lse);
-      }
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
-    const int at = (e >> 1) * 8 + 2 * t + (e & 1);
-    if (g == 0 && at < nk) P.weights[first + at] = P.decay == 0.f ? sum[e] : P.decay * P.weights[first + at] + sum[e];
-  }
-}
-
 namespace {
 
 // Keys of a unit's stretch, so that all units run in about one, two or some waves of as many as the machine holds
-int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group, int64_t resident) {
+int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int64_t resident) {
   constexpr double kGroup = 1., kUnit = 5.;  // microseconds of a warp's 16 keys, and of a unit besides
   int64_t most = 64;
   for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, ceil_div(seqs[i].length, 64) * 64);
   auto units = [&](int64_t keys) {
     int64_t u = 0;
-    for (int i = 0; i < n; ++i) u += ceil_div((int64_t)seqs[i].count * group, kAttnTile) * ceil_div(seqs[i].length, keys);
+    for (int i = 0; i < n; ++i) u += seqs[i].count > 0 ? ceil_div(seqs[i].length, keys) : 0;
     return u * c->n_kv_heads;
   };
   int64_t best = most;
@@ -602,35 +536,28 @@ constexpr int64_t kUnitWork = 8;   // of a unit of many rows besides its tiles
 constexpr int64_t kBlockWork = 24;  // worth a block
 int64_t tile_work(int64_t rows) { return rows > 128 ? 4 : 2; }  // of 128 keys
 
-// whether a call goes to the tensor cores: up to two tiles of rows, keys are read once or twice by the kernel of few rows
+// whether a call goes to the kernel of many rows: some sequence has more than eight
 bool many_rows(const infllm_packed_seq* seqs, int n, int group) {
   int64_t most = 0;
   for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, (int64_t)seqs[i].count * group);
-  return most > 2 * kAttnTile;
+  return most > kFewRows;
 }
-
-// whether the weights are worked out of scores that the kernel of few rows leaves: 8 bytes of a row and key, written and read, where
-// keys that are read again are kDim * 5 / 8
-bool by_logits(const infllm_packed_seq* seqs, int n, int group) {
-  int64_t most = 0;
-  for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, (int64_t)seqs[i].count * group);
-  return most <= 8;
-}
+// keys that a row of scores has room for
 int64_t logit_pitch(const infllm_packed_seq* seqs, int n) {
   int64_t longest = 0;
   for (int i = 0; i < n; ++i) longest = std::max<int64_t>(longest, seqs[i].length);
   return ceil_div(longest, kSumKeys) * kSumKeys;
 }
 
-// the units of the launch of seqs[0 .. n - 1] for few rows
-int64_t lay_out_few(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group, int n_sm, PackedAttnSeq* to, bool* join) {
-  const int64_t keys = chunk_keys(c, seqs, n, group, n_sm * 4);
+// the units of the launch of seqs[0 .. n - 1] for few rows: stretches of a sequence's keys
+int64_t lay_out_few(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int n_sm, PackedAttnSeq* to, bool* join) {
+  const int64_t keys = chunk_keys(c, seqs, n, n_sm * 4);
   int64_t u = 0;
   for (int i = 0; i < n; ++i) {
-    const int64_t chunks = std::max<int64_t>(1, ceil_div(seqs[i].length, keys)), tiles = ceil_div((int64_t)seqs[i].count * group, kAttnTile);
+    const int64_t chunks = seqs[i].count > 0 ? ceil_div(seqs[i].length, keys) : 0;
     to[i] = {seqs[i].slot, seqs[i].length, seqs[i].count, (int32_t)std::min<int64_t>(u, INT_MAX), (int32_t)chunks, (int32_t)keys};
-    if (chunks > 1 && seqs[i].count > 0) *join = true;
-    u += chunks * tiles;
+    *join = *join || chunks > 1;
+    u += chunks;
   }
   return u;
 }
@@ -709,31 +636,28 @@ int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, i
   if ((int64_t)most * n_heads > INT_MAX / 4) return fail(INFLLM_E_BADARG, "%s: %d tokens of %d heads", what, most, n_heads);
   *bytes = 0;
   if (n == 0 || most == 0) return INFLLM_OK;
-  const int group = n_heads / c->n_kv_heads;
   const int n_sm = sm_count(c->device);
-  int64_t rows = many_rows(seqs, n, group) ? 2 * n_sm * kBlockRows : 0;
-  PackedAttnSeq to[kAttnSeqs];
-  for (int b0 = 0; b0 < n; b0 += kAttnSeqs) {
-    const int m = std::min(n - b0, kAttnSeqs);
-    if (many_rows(seqs + b0, m, group)) continue;
-    bool join = false;
-    const int64_t units = lay_out_few(c, seqs + b0, m, group, n_sm, to, &join);
-    if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
-    rows = std::max(rows, units * c->n_kv_heads * kAttnTile);
+  if (many_rows(seqs, n, n_heads / c->n_kv_heads)) {
+    *bytes = (int64_t)2 * n_sm * kBlockRows * (c->head_dim + 1) * 4 + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
+    return INFLLM_OK;
   }
-  *bytes = ceil_div(rows * (c->head_dim + 1) * 4, 16) * 16;
-  if (weigh > 0) *bytes += by_logits(seqs, n, group) ? (int64_t)n * most * n_heads * logit_pitch(seqs, n) * 4 : (int64_t)n * most * n_heads * 4;
+  int64_t units = 0;
+  PackedAttnSeq to[kAttnSeqs];
+  bool join = false;
+  for (int b0 = 0; b0 < n; b0 += kAttnSeqs) units = std::max(units, lay_out_few(c, seqs + b0, std::min(n - b0, kAttnSeqs), n_sm, to, &join));
+  if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
+  *bytes = ceil_div(units * c->n_kv_heads * kFewRows * (c->head_dim + 1) * 4, 16) * 16 + (weigh > 0 ? (int64_t)n * most * n_heads * logit_pitch(seqs, n) * 4 : 0);
   return INFLLM_OK;
 }
 
 template <typename T, int kDim>
 int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, int n_sm, bool join, cudaStream_t s) {
-  const int64_t units = lay_out_few(c, seqs, P.batch, P.group, n_sm, P.seq, &join);
+  const int64_t units = lay_out_few(c, seqs, P.batch, n_sm, P.seq, &join);
   int counts = 0;
   for (int i = 0; i < P.batch; ++i) counts = std::max(counts, seqs[i].count);
-  P.part_lse = P.part_o + units * c->n_kv_heads * kAttnTile * kDim;
+  P.part_lse = P.part_o + units * c->n_kv_heads * kFewRows * kDim;
   if (units > 0) {
-    auto kern = counts * P.group <= 8 ? packed_rows_kernel<T, kDim, 1> : packed_rows_kernel<T, kDim, 2>;
+    auto kern = counts * P.group <= 4 ? packed_rows_kernel<T, kDim, true> : packed_rows_kernel<T, kDim, false>;
     INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)units, c->n_kv_heads), dim3(kAttnWarps * 32), 0, s, P));
     INFLLM_LAUNCH_OK("packed_rows_kernel");
   }
@@ -783,9 +707,11 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
     P.at = packed_planes(c, layer);
     P.q = (const char*)d_q, P.q_bs = q_bs * 2, P.q_hs = q_hs * 2, P.q_ts = q_ts * 2;
     P.out = (char*)d_out, P.lse = d_lse;
+    const bool many = many_rows(seqs, n, n_heads / c->n_kv_heads);
     P.pitch = logit_pitch(seqs, n), P.logit_rows = most * (n_heads / c->n_kv_heads);
-    P.logits = weigh > 0 && by_logits(seqs, n, n_heads / c->n_kv_heads) ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * P.pitch * 4) : nullptr;
-    P.row_lse = weigh > 0 && !P.logits ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * 4) : nullptr;
+    // (what the weights are worked out of, at the end of the workspace)
+    P.logits = weigh > 0 && !many ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * P.pitch * 4) : nullptr;
+    P.row_lse = weigh > 0 && many ? (float*)((char*)d_work + bytes - (int64_t)n * most * n_heads * 4) : nullptr;
     P.weights = c->d_weights + layer * packed_rows(c);
     P.part_o = (float*)d_work;
     P.group = n_heads / c->n_kv_heads, P.most = most, P.weigh = weigh;
@@ -802,7 +728,6 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
         if (mine[i].count > 0) longest = std::max<int64_t>(longest, mine[i].length), any = true;
         empty = empty || mine[i].count < most;
       }
-      const bool many = many_rows(mine, P.batch, P.group);
       INFLLM_DISPATCH_DTYPE(c->dtype, T, {
         if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, n_sm, empty, s) : attend_many<T, 64>(Tc, mine, c, n_sm, empty, s)));
         else INFLLM_TRY((c->head_dim == 128 ? attend_few<T, 128>(P, mine, c, n_sm, empty, s) : attend_few<T, 64>(P, mine, c, n_sm, empty, s)));
@@ -810,10 +735,6 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
           bool cut = false;
           INFLLM_TRY(lay_out_weights(c, mine, n_sm, Tc, &cut));
           INFLLM_TRY(packed_weigh_tc_launch(Tc, c->dtype, c->head_dim, cut, (int)longest, s));
-        } else if (weigh > 0 && any && !P.logits) {
-          auto kern = c->head_dim == 128 ? packed_weigh_kernel<T, 128> : packed_weigh_kernel<T, 64>;
-          INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)ceil_div(longest, 64), c->n_kv_heads, P.batch), dim3(128), 0, s, P));
-          INFLLM_LAUNCH_OK("packed_weigh_kernel");
         }
       });
     }

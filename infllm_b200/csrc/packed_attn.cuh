@@ -11,7 +11,7 @@ constexpr int kMaxSms = 160;
 struct PackedAttnSeq {
   int32_t slot, length, count;
   int32_t unit0;   // its first unit of work, and how they follow from there:
-  int32_t chunks;  // few rows: unit0 + tile of 16 rows * chunks + stretch of `keys` keys
+  int32_t chunks;  // few rows: unit0 + stretch of `keys` keys
   int32_t keys;    // many: unit0 + KV head * chunks + block of 256 rows
 };
 
@@ -21,7 +21,7 @@ struct PackedAttnParams {
   int64_t q_bs, q_hs, q_ts;  // bytes
   char* out;
   float* lse;
-  float *part_o, *part_lse;  // few rows: 16 rows of each unit and KV head; many: kBlockRows rows of each block's first and last unit
+  float *part_o, *part_lse;  // few rows: 8 of each unit and KV head; many: kBlockRows rows of each block's first and last unit
   float* row_lse;            // (batch, KV head, token, query head of the KV head), to base 2: for the weights; null: none
   float* weights;            // of the layer
   float* logits;             // (batch, KV head, row, pitch): scores to base 2 of up to 8 rows, for the weights; null: none
