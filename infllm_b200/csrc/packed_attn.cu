@@ -21,14 +21,23 @@ using namespace mma;
 
 constexpr int kAttnWarps = 4, kFewRows = 8;
 
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+// loads of 16, 8 and 4 bytes that are read once, kAt bytes behind an address
+template <int kAt>
+__device__ __forceinline__ uint4 ld_stream16(const char* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4+%5];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "n"(kAt));
   return r;
 }
-__device__ __forceinline__ uint32_t ld_stream4(const void* p) {
+template <int kAt>
+__device__ __forceinline__ uint2 ld_stream8(const char* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2+%3];" : "=r"(r.x), "=r"(r.y) : "l"(p), "n"(kAt));
+  return r;
+}
+template <int kAt>
+__device__ __forceinline__ uint32_t ld_stream4(const char* p) {
   uint32_t r;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1+%2];" : "=r"(r) : "l"(p), "n"(kAt));
   return r;
 }
 
@@ -55,47 +64,77 @@ struct PackedRows {
 
   struct Key {  // rows nt * 8 + g
     uint32_t w[2][kW], ms[2];
+    // codes and scales from here on: this thread's of row nt
+    template <int kNt>
+    __device__ __forceinline__ void load(const char* codes, const char* scales) {
+      if constexpr (kDim == 128) {
+        const uint4 x = ld_stream16<kNt * 8 * kRow>(codes);
+        w[kNt][0] = x.x, w[kNt][1] = x.y, w[kNt][2] = x.z, w[kNt][3] = x.w;
+      } else {
+        const uint2 x = ld_stream8<kNt * 8 * kRow>(codes);
+        w[kNt][0] = x.x, w[kNt][1] = x.y;
+      }
+      ms[kNt] = ld_stream4<kNt * 8 * kScales>(scales);
+    }
   };
   struct Value {  // rows 2t, 2t + 1, 2t + 8, 2t + 9
     uint32_t w[4][kH], ms[4];
+    template <int kKi>
+    __device__ __forceinline__ void load(const char* codes, const char* scales) {
+      constexpr int kR = (kKi & 1) + (kKi >> 1) * 8;
+      if constexpr (kDim == 128) {
+        const uint2 x = ld_stream8<kR * kRow>(codes);
+        w[kKi][0] = x.x, w[kKi][1] = x.y;
+      } else {
+        w[kKi][0] = ld_stream4<kR * kRow>(codes);
+      }
+      ms[kKi] = ld_stream4<kR * kScales>(scales);
+    }
   };
-  template <bool kAll>  // all 16 keys are there
-  __device__ __forceinline__ static Key key(const char* codes, const char* scales, int nk) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    Key k;
+  // where a thread's pieces of 16 keys begin, from the first one's codes and scales of keys and of values on
+  struct Place {
+    const char *kc, *ks, *vc, *vs;
+    __device__ __forceinline__ Place(const char* codes, const char* scales, int64_t codes_v, int64_t scales_v) {
+      const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+      kc = codes + g * kRow + t * (kRow / 4), ks = scales + g * kScales + (kDim == 128 ? t : t >> 1) * 4;
+      vc = codes + codes_v + 2 * t * kRow + g * (kRow / 8), vs = scales + scales_v + 2 * t * kScales + (kDim == 128 ? g >> 1 : g >> 2) * 4;
+    }
+    __device__ __forceinline__ void advance(int keys) { kc += keys * kRow, ks += keys * kScales, vc += keys * kRow, vs += keys * kScales; }
+    __device__ __forceinline__ void load(Key& k, Value& v) const {
+      k.template load<0>(kc, ks);
+      k.template load<1>(kc, ks);
+      v.template load<0>(vc, vs);
+      v.template load<1>(vc, vs);
+      v.template load<2>(vc, vs);
+      v.template load<3>(vc, vs);
+    }
+    // nk keys are there: what lies behind the last is not read, as it may not be a number, and 0 times that is none
+    __device__ __forceinline__ void load(Key& k, Value& v, int nk) const {
+      const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const int r = kAll ? nt * 8 + g : min(nt * 8 + g, nk - 1);  // (what lies behind the last key is not read: it may not be a number, and 0 times that is none)
-      if (kDim == 128) {
-        const uint4 x = ld_stream16(codes + r * kRow + t * 16);
-        k.w[nt][0] = x.x, k.w[nt][1] = x.y, k.w[nt][2 % kW] = x.z, k.w[nt][3 % kW] = x.w;
-        k.ms[nt] = ld_stream4(scales + r * kScales + t * 4);
-      } else {
-        const uint2 x = ld_stream8(codes + r * kRow + t * 8);
-        k.w[nt][0] = x.x, k.w[nt][1] = x.y;
-        k.ms[nt] = ld_stream4(scales + r * kScales + (t >> 1) * 4);
+      for (int nt = 0; nt < 2; ++nt) {
+        const int64_t back = min(nk - 1 - (nt * 8 + g), 0);  // rows from the one that would be this thread's
+        Key x;
+        if (nt == 0) x.template load<0>(kc + back * kRow, ks + back * kScales);
+        else x.template load<1>(kc + back * kRow, ks + back * kScales);
+#pragma unroll
+        for (int j = 0; j < kW; ++j) k.w[nt][j] = x.w[nt][j];
+        k.ms[nt] = x.ms[nt];
+      }
+#pragma unroll
+      for (int ki = 0; ki < 4; ++ki) {
+        const int64_t back = min(nk - 1 - (2 * t + (ki & 1) + (ki >> 1) * 8), 0);
+        Value x;
+        if (ki == 0) x.template load<0>(vc + back * kRow, vs + back * kScales);
+        else if (ki == 1) x.template load<1>(vc + back * kRow, vs + back * kScales);
+        else if (ki == 2) x.template load<2>(vc + back * kRow, vs + back * kScales);
+        else x.template load<3>(vc + back * kRow, vs + back * kScales);
+#pragma unroll
+        for (int j = 0; j < kH; ++j) v.w[ki][j] = x.w[ki][j];
+        v.ms[ki] = x.ms[ki];
       }
     }
-    return k;
-  }
-  template <bool kAll>
-  __device__ __forceinline__ static Value value(const char* codes, const char* scales, int nk) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    Value v;
-#pragma unroll
-    for (int ki = 0; ki < 4; ++ki) {
-      const int at = 2 * t + (ki & 1) + (ki >> 1) * 8, r = kAll ? at : min(at, nk - 1);
-      if (kDim == 128) {
-        const uint2 x = ld_stream8(codes + r * kRow + g * 8);
-        v.w[ki][0] = x.x, v.w[ki][kH - 1] = x.y;
-        v.ms[ki] = ld_stream4(scales + r * kScales + (g >> 1) * 4);
-      } else {
-        v.w[ki][0] = ld_stream4(codes + r * kRow + g * 4);
-        v.ms[ki] = ld_stream4(scales + r * kScales + (g >> 2) * 4);
-      }
-    }
-    return v;
-  }
+  };
 
   __device__ __forceinline__ void clear() {
     m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
@@ -114,8 +153,8 @@ struct PackedRows {
   }
 
   // 16 keys from j0 on; kAll: every row sees all of them.  Otherwise those below key1, and a row those below its own limit.
-  // logits: the scores' place of this thread's first row and key g, null: none is wanted
-  template <bool kAll>
+  // kWeigh: scores are left for the weights; logits: the place of this thread's first row's of key g, null: it has none
+  template <bool kAll, bool kWeigh>
   __device__ __forceinline__ void group(const Key& k, const Value& v, int j0, int key1, float scale_log2, float* logits, int64_t pitch, bool two) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float s[4] = {0.f, 0.f, 0.f, 0.f};  // key g of rows 2t, 2t + 1; key g + 8
@@ -137,7 +176,7 @@ struct PackedRows {
       for (int e = 0; e < 4; ++e)
         if (j0 + (e >> 1) * 8 + g >= min(lim[e & 1], key1)) s[e] = -INFINITY;
     }
-    if (logits) {
+    if (kWeigh && logits) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if ((kAll || j0 + (e >> 1) * 8 + g < key1) && (!(e & 1) || two)) logits[(e & 1) * pitch + j0 + (e >> 1) * 8] = s[e] * scale_log2;
@@ -193,7 +232,7 @@ struct PackedRows {
 };
 
 // Four warps share a stretch's groups of 16 keys and meet in shared memory.
-template <typename T, int kDim, bool kFour>
+template <typename T, int kDim, bool kFour, bool kWeigh>
 __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const __grid_constant__ PackedAttnParams P) {
   using R = PackedRows<T, kDim, kFour>;
   using C = Codes<T>;
@@ -213,13 +252,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
     const int r = kFour ? (2 * t + e) & 3 : 2 * t + e;
     w.lim[e] = r < rows ? keys_of_row(S, P.group, r) : 0;
   }
-  const int64_t first = P.at.row0(S.slot, hkv) + key0;  // (the stretch's first row)
-  const char* kc = P.at.codes + first * R::kRow;
-  const char* ks = P.at.scales + first * R::kScales;
-  const char* vc = kc + P.at.codes_v;
-  const char* vs = ks + P.at.scales_v;
+  const int64_t first = P.at.row0(S.slot, hkv) + key0 + warp * 16;  // of the stretch, this warp's first row
+  typename R::Place at(P.at.codes + first * R::kRow, P.at.scales + first * R::kScales, P.at.codes_v, P.at.scales_v);
   float* logits = nullptr;
-  if (P.logits && 2 * t < rows) logits = P.logits + (((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.logit_rows + 2 * t) * P.pitch + g;
+  if (kWeigh && 2 * t < rows) logits = P.logits + (((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.logit_rows + 2 * t) * P.pitch + g;
   const bool two = 2 * t + 1 < rows;
   chain_enter();
   if (warp < R::kW) {  // a piece of every row by a warp
@@ -229,21 +265,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
   }
   w.qf = &sm_q[0][lane];
   w.clear();
-  auto key = [&](int j) { return R::template key<true>(kc + (int64_t)(j - key0) * R::kRow, ks + (int64_t)(j - key0) * R::kScales, 16); };
-  auto value = [&](int j) { return R::template value<true>(vc + (int64_t)(j - key0) * R::kRow, vs + (int64_t)(j - key0) * R::kScales, 16); };
   const int whole = min(key1, least) - 16;  // the last place of a group that all rows see all of
   int j0 = key0 + warp * 16;
   // A group is on its way while the one before it is worked on: two copies of the work, each with its own registers, as what is on its
   // way is not to be moved, which would wait for it.
   typename R::Key k0, k1;
   typename R::Value v0, v1;
-  if (j0 <= whole) k0 = key(j0), v0 = value(j0);
+  if (j0 <= whole) at.load(k0, v0);
   __syncthreads();
   if (j0 <= whole) {
     auto turn = [&](const typename R::Key& k, const typename R::Value& v, typename R::Key& kn, typename R::Value& vn) {
       const bool more = j0 + kStep <= whole;
-      if (more) kn = key(j0 + kStep), vn = value(j0 + kStep);
-      w.template group<true>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
+      at.advance(kStep);
+      if (more) at.load(kn, vn);
+      w.template group<true, kWeigh>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
       j0 += kStep;
       return more;
     };
@@ -251,11 +286,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
     }
   }
 #pragma unroll 1
-  for (; j0 < key1; j0 += kStep) {
-    const int nk = min(16, key1 - j0);
-    const int64_t at = j0 - key0;
-    typename R::Key k = R::template key<false>(kc + at * R::kRow, ks + at * R::kScales, nk);
-    typename R::Value v = R::template value<false>(vc + at * R::kRow, vs + at * R::kScales, nk);
+  for (; j0 < key1; j0 += kStep, at.advance(kStep)) {
+    typename R::Key k;
+    typename R::Value v;
+    at.load(k, v, min(16, key1 - j0));
     // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and its
     // key is no number in its place, so that the rows that see it still become none.
     uint32_t bad = 0;
@@ -271,7 +305,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
       if (bad >> (nt * 8 + g) & 1) k.ms[nt] = 0x7fff7fffu;
-    w.template group<false>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
+    w.template group<false, kWeigh>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
   }
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -301,7 +335,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
     }
     const float lse = mx == -INFINITY ? -INFINITY : mx + log2f(den);
     const int64_t pr = ((int64_t)unit * P.at.n_kv + hkv) * kFewRows + r;
-    if (d == 0 && (S.chunks > 1 || P.logits)) P.part_lse[pr] = lse;
+    if (d == 0 && (S.chunks > 1 || kWeigh)) P.part_lse[pr] = lse;
     if (S.chunks > 1) {
       *reinterpret_cast<float2*>(P.part_o + pr * kDim + d) = make_float2(n0, n1);
     } else {
@@ -657,7 +691,8 @@ int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_
   for (int i = 0; i < P.batch; ++i) counts = std::max(counts, seqs[i].count);
   P.part_lse = P.part_o + units * c->n_kv_heads * kFewRows * kDim;
   if (units > 0) {
-    auto kern = counts * P.group <= 4 ? packed_rows_kernel<T, kDim, true> : packed_rows_kernel<T, kDim, false>;
+    auto kern = counts * P.group <= 4 ? (P.logits ? packed_rows_kernel<T, kDim, true, true> : packed_rows_kernel<T, kDim, true, false>)
+                                      : (P.logits ? packed_rows_kernel<T, kDim, false, true> : packed_rows_kernel<T, kDim, false, false>);
     INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)units, c->n_kv_heads), dim3(kAttnWarps * 32), 0, s, P));
     INFLLM_LAUNCH_OK("packed_rows_kernel");
   }
