@@ -662,6 +662,29 @@ int infllm_packed_attend(const infllm_packed* c, int layer, const infllm_packed_
 int infllm_packed_evict(const infllm_packed* c, const infllm_packed_seq* seqs, int n, const int32_t* into, int64_t budget, int64_t sink,
                         int64_t recent, void* d_work, int64_t work_bytes, void* stream);
 
+/* The bookkeeping of such a caller, without a GPU.  Five numbers of a sequence: how often it was opened and closed (odd: it is open), its
+ * tokens, the position of the next one, how many of its newest tokens are known to lie at the positions before that one, and the last
+ * change of the former, by a count of the book's.  Of a batch of n sequences, with the first of those numbers as of its beginning:
+ *   EXTEND   counts[i] more tokens (counts NULL: `same` for every sequence), which become the step's
+ *   PLAN     the newest counts[i] tokens that are there become the step's
+ *   RETRACT  takes the newest counts[i] tokens back, which have to lie in a row
+ * EXTEND and PLAN fill `table` with the step's sequences, as_of with their last changes, and info with the largest count, the rows that
+ * a rotary table has to have, and whether every token of the step lies in a row with those before it.  INFLLM_E_CAPACITY where
+ * more tokens than max_tokens were the result, INFLLM_E_BADARG for what there is not; either changes nothing.
+ * infllm_packed_book_evict: the same for infllm_packed_evict.  With apply 0 it checks the arguments, fills `table`, and sets *most to the most
+ * tokens that stay of a sequence; with apply 1 the lengths become what they are after it. */
+#define INFLLM_PACKED_EXTEND 0
+#define INFLLM_PACKED_PLAN 1
+#define INFLLM_PACKED_RETRACT 2
+typedef struct infllm_packed_book {
+  int64_t n_sequences, max_tokens, changes;
+  int64_t* state; /* (n_sequences, 5): opened, length, position, in a row, change */
+} infllm_packed_book;
+int infllm_packed_book_step(infllm_packed_book* book, int what, const int32_t* seqs, const int64_t* opened, int n, const int64_t* counts,
+                            int64_t same, infllm_packed_seq* table, int64_t* as_of, int64_t* info);
+int infllm_packed_book_evict(infllm_packed_book* book, const int32_t* seqs, int n, const int32_t* into, int64_t budget, int64_t sink,
+                             int64_t recent, infllm_packed_seq* table, int64_t* most, int apply);
+
 /* ----------------------------------------------------- host logic, GPU-free
  * The LRU table alone (context_manager.py:246-265, 495-515): dict-ordered ids with stamps.
  * Exposed so that the eviction order can be tested without a device. */

@@ -16,6 +16,7 @@ CACHE_LRU, CACHE_LRU_S = 0, 1
 MASK_NONE, MASK_WINDOW, MASK_COMPLEMENT = 0, 1, 2
 MAX_SEGMENTS = 80
 PAGES_NO_PLAN = 1
+PACKED_EXTEND, PACKED_PLAN, PACKED_RETRACT = 0, 1, 2
 PROF_ATTN, PROF_COLSUM, PROF_DECODE, PROF_TOPK, PROF_SLOTS = 0, 1, 2, 3, 4
 
 
@@ -45,9 +46,15 @@ class Config(ctypes.Structure):
 
 
 class Packed(ctypes.Structure):
+    """infllm_packed of include/infllm_b200.h."""
     _fields_ = [("n_layers", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("n_sequences", c_int32), ("max_tokens", c_int32),
                 ("dtype", c_int32), ("device", c_int32), ("pad", c_int32),
                 ("d_codes", c_void_p), ("d_scales", c_void_p), ("d_weights", c_void_p), ("d_places", c_void_p)]
+
+
+class PackedBook(ctypes.Structure):
+    """infllm_packed_book of include/infllm_b200.h."""
+    _fields_ = [("n_sequences", c_int64), ("max_tokens", c_int64), ("changes", c_int64), ("state", c_void_p)]
 
 
 class SinkWindow(ctypes.Structure):
@@ -233,6 +240,8 @@ SIGNATURES = {
     "infllm_packed_attend": (c_int, [POINTER(Packed), c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                                      c_int, c_float, c_int, c_float, c_void_p, c_int64, c_void_p]),
     "infllm_packed_evict": (c_int, [POINTER(Packed), c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "infllm_packed_book_step": (c_int, [POINTER(PackedBook), c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "infllm_packed_book_evict": (c_int, [POINTER(PackedBook), c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int]),
     "infllm_lru_create": (c_int, [c_int, POINTER(c_void_p)]),
     "infllm_lru_destroy": (c_int, [c_void_p]),
     "infllm_lru_plan": (c_int, [c_void_p, POINTER(c_int32), c_int, POINTER(c_int32), POINTER(c_int)]),

@@ -67,51 +67,47 @@ class PackedCache:
 
     def _begin(self):
         n = self.n_sequences
-        self._open, self._length, self._position = [False] * n, [0] * n, [0] * n
-        self._fresh = [0] * n  # newest tokens that lie at the positions before `_position`
-        self._opened = [0] * n  # how often
-        self._changes, self._n_changes = [0] * n, 0  # of what a sequence holds
+        self._state = (c_int64 * (5 * n))()  # of each sequence: opened, length, position, newest in a row, change
+        self._book = _lib.PackedBook(n, self.max_tokens, 0, ctypes.addressof(self._state))
+        self._book_ref = ctypes.byref(self._book)
 
     # -- sequences
     def _known(self, seqs):
         seqs = [int(s) for s in seqs]
         for s in seqs:
-            if not 0 <= s < self.n_sequences or not self._open[s]:
+            if not 0 <= s < self.n_sequences or self._state[5 * s] % 2 == 0:
                 raise ValueError(f"there is no sequence {s}")
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence twice")
         return seqs
 
-    def _change(self, s):
-        self._n_changes += 1
-        self._changes[s] = self._n_changes
-
     def open(self, n=1):
         """n new, empty sequences: their numbers, the lowest that are not in use."""
         if n < 0:
             raise ValueError(f"{n} sequences")
-        free = [s for s in range(self.n_sequences) if not self._open[s]][:n]
+        free = [s for s in range(self.n_sequences) if self._state[5 * s] % 2 == 0][:n]
         if len(free) < n:
             raise _lib.InfLLMCapacityError(_lib.E_CAPACITY, f"{n} sequences, where {len(free)} of {self.n_sequences} are free")
         for s in free:
-            self._open[s], self._length[s], self._position[s], self._fresh[s] = True, 0, 0, 0
-            self._opened[s] += 1
-            self._change(s)
+            self._set(s)
         return free
+
+    def _set(self, s):  # opened, or freed, and empty
+        self._book.changes += 1
+        self._state[5 * s:5 * s + 5] = self._state[5 * s] + 1, 0, 0, 0, self._book.changes
 
     def free(self, seqs):
         """Ends sequences."""
         for s in self._known(seqs):
-            self._open[s], self._length[s] = False, 0
-            self._change(s)
+            self._set(s)
 
     def length(self, seq):
         """Tokens that a sequence holds."""
-        return self._length[self._known([seq])[0]]
+        return self._state[5 * self._known([seq])[0] + 1]
 
     def position(self, seq):
         """The position that its next token is rotated to: the tokens that it has had (evict() takes none of them back)."""
-        return self._position[self._known([seq])[0]]
+        return self._state[5 * self._known([seq])[0] + 2]
 
     def batch(self, seqs):
         return PackedBatch(self, seqs)
@@ -122,39 +118,35 @@ class PackedCache:
         to head: `places` says it.  Keys keep the rotation that they were written with, and position() goes on from where it was.
         `into`: sequences of this cache that get what stays (all of a shorter sequence) in place of what they hold; `seqs` then
         stay as they are."""
-        seqs = self._known(seqs)
-        budget, sink, recent = int(budget), int(sink), int(recent)
-        if sink < 0 or recent < 0 or sink + recent > budget:
-            raise ValueError(f"{budget} tokens, the first {sink} and the newest {recent} among them")
-        to = None
+        n, ids, to = len(seqs), _ids(seqs), None
         if into is not None:
-            to = self._known(into)
-            if len(to) != len(seqs):
-                raise ValueError(f"{len(seqs)} sequences into {len(to)}")
-            if set(to) & set(seqs):
-                raise ValueError("a sequence into itself or another that is read")
-        most = max((min(self._length[s], budget) for s in seqs), default=0)
-        need = self.n_layers * len(seqs) * self.n_kv_heads * (-(-most // 4) * 4) * 4
-        work = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
-        table = _table([(s, self._length[s], 0, 0) for s in seqs])
-        _lib.check(_lib_call.infllm_packed_evict(self._ref, table, len(seqs), None if to is None else _ints(to), budget, sink, recent,
-                                                 work.data_ptr(), work.numel(), _lib.raw_stream(self.device)))
-        for i, s in enumerate(seqs):
-            n = self._length[s]
-            fresh = self._fresh[s] if n <= budget else min(self._fresh[s], recent)
-            d = s if to is None else to[i]
-            if to is None and n <= budget:
-                continue
-            self._length[d], self._position[d], self._fresh[d] = min(n, budget), self._position[s], fresh
-            self._change(d)
+            if len(into) != n:
+                raise ValueError(f"{n} sequences into {len(into)}")
+            to = _ids(into)
+        table, most = (c_int32 * (4 * max(n, 1)))(), c_int64()
+        _checked(_lib_call.infllm_packed_book_evict(self._book_ref, ids, n, to, budget, sink, recent, table, ctypes.byref(most), 0))
+        size = self.n_layers * n * self.n_kv_heads * (-(-most.value // 4) * 4) * 4
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
+        _lib.check(_lib_call.infllm_packed_evict(self._ref, table, n, to, budget, sink, recent, work.data_ptr(), work.numel(),
+                                                 _lib.raw_stream(self.device)))
+        _lib.check(_lib_call.infllm_packed_book_evict(self._book_ref, ids, n, to, budget, sink, recent, None, None, 1))
 
 
-def _ints(values):
-    return (c_int32 * len(values)).from_buffer(array("i", values)) if values else (c_int32 * 1)()
+def _checked(rc):
+    """What there is not, and what does not fit, as Python's own errors."""
+    if rc == _lib.E_BADARG:
+        raise ValueError(_lib_call.infllm_last_error().decode("utf-8", "replace"))
+    if rc:
+        _lib.check(rc)
 
 
-def _table(rows):  # of (slot, length, count, position)
-    return _ints([x for row in rows for x in row])
+# (ctypes cuts what does not fit: array raises OverflowError)
+def _ids(values):
+    return (c_int32 * len(values)).from_buffer(array("i", values)) if len(values) else (c_int32 * 1)()
+
+
+def _long(values):
+    return (c_int64 * len(values)).from_buffer(array("q", values)) if len(values) else (c_int64 * 1)()
 
 
 class PackedBatch:
@@ -166,82 +158,56 @@ class PackedBatch:
     def __init__(self, cache, seqs):
         self.cache, self.seqs = cache, cache._known(seqs)
         self._n = len(self.seqs)
+        self._ids = _ids(self.seqs)
+        self._opened = _long([cache._state[5 * s] for s in self.seqs])
         self.tokens = 0  # of the step's tensors
-        self._as_of = [None] * self._n  # the sequences' _changes when the step began
-        self._opened = [cache._opened[s] for s in self.seqs]
-        self._table = _table([])
-        self._whole = True  # the positions of the step's tokens are known
-        self._reach = 0  # rows that a rotary table has to have
+        self._table = (c_int32 * (4 * max(self._n, 1)))()  # of the step's sequences: slot, length, count, position
+        self._as_of = (c_int64 * max(self._n, 1))()  # the last changes of the sequences when the step began,
+        self._at = None  # and of the book; None: there is no step
+        self._info = (c_int64 * 3)()  # tokens, rows that a rotary table has to have, whether all tokens' positions are known
         self._rooms = {}  # of workspaces, by heads and counted tokens
         self._scale = 1.0 / math.sqrt(cache.head_dim)
 
-    def _counts(self, n):
-        self.cache._known(self.seqs)
-        for s, x in zip(self.seqs, self._opened):
-            if self.cache._opened[s] != x:
-                raise ValueError(f"sequence {s} of this batch has been freed")
-        if isinstance(n, int):
-            n = [n] * self._n
-        n = [int(x) for x in n]
-        if len(n) != self._n:
-            raise ValueError(f"{self._n} sequences and {len(n)} counts")
-        for x in n:
-            if x < 0:
-                raise ValueError(f"{x} tokens")
-        return n
-
-    def _step(self, counts):
-        c = self.cache
-        self.tokens = max(counts, default=0)
-        self._as_of = [c._changes[s] for s in self.seqs]
-        rows = [(s, c._length[s], n, max(c._position[s] - n, 0)) for s, n in zip(self.seqs, counts)]
-        self._table, self._rooms = _table(rows), {}
-        self._reach = max((c._position[s] for s, n in zip(self.seqs, counts) if n), default=0)
-        self._whole = all(n <= c._fresh[s] for s, n in zip(self.seqs, counts))
+    def _step(self, what, n):
+        c, counts, same = self.cache, None, n
+        if not isinstance(n, int):
+            if len(n) != self._n:
+                raise ValueError(f"{self._n} sequences and {len(n)} counts")
+            counts, same = _long(n), 0
+        elif not -1 << 63 <= n < 1 << 63:
+            raise OverflowError(f"{n} is beyond 64 bits")
+        rc = _lib_call.infllm_packed_book_step(c._book_ref, what, self._ids, self._opened, self._n, counts, same, self._table, self._as_of,
+                                               self._info)
+        if rc:
+            _checked(rc)
+        if what == _lib.PACKED_RETRACT:
+            self.tokens, self._at = 0, None
+        else:
+            self.tokens, self._at, self._rooms = self._info[0], c._book.changes, {}
 
     def _current(self):
         c = self.cache
+        if self._at == c._book.changes:
+            return
+        if self._at is None:
+            raise ValueError("no step: extend() or plan() says what it is about")
         for s, x in zip(self.seqs, self._as_of):
-            if c._changes[s] != x:
-                raise ValueError("no step, or one whose sequences another call has changed" if x is None else
-                                 f"sequence {s} has been changed since the step began")
+            if c._state[5 * s + 4] != x:
+                raise ValueError(f"sequence {s} has been changed since the step began")
+        self._at = c._book.changes
 
     def extend(self, n):
         """Room for n more tokens of every sequence, or for n[i]: they are the step's."""
-        c, counts = self.cache, self._counts(n)
-        for s, x in zip(self.seqs, counts):
-            if c._length[s] + x > c.max_tokens:
-                raise _lib.InfLLMCapacityError(_lib.E_CAPACITY, f"sequence {s} of {c._length[s]} tokens and {x} more, where {c.max_tokens} fit")
-            if c._position[s] + x > 0x7fffffff:
-                raise _lib.InfLLMCapacityError(_lib.E_CAPACITY, f"sequence {s}: a position beyond 31 bits")
-        for s, x in zip(self.seqs, counts):
-            c._length[s] += x
-            c._position[s] += x
-            c._fresh[s] += x
-            c._change(s)
-        self._step(counts)
+        self._step(_lib.PACKED_EXTEND, n)
 
     def plan(self, n):
         """The newest n tokens of every sequence, or n[i], that are there already, are the step's."""
-        c, counts = self.cache, self._counts(n)
-        for s, x in zip(self.seqs, counts):
-            if x > c._length[s]:
-                raise ValueError(f"the newest {x} tokens of sequence {s}, which has {c._length[s]}")
-        self._step(counts)
+        self._step(_lib.PACKED_PLAN, n)
 
     def retract(self, n):
         """Takes the newest n tokens of every sequence, or n[i], back, as a speculative decoder does with drafts.  They are tokens
         that were written since the last eviction, or that it kept as `recent`."""
-        c, counts = self.cache, self._counts(n)
-        for s, x in zip(self.seqs, counts):
-            if x > c._fresh[s]:
-                raise ValueError(f"{x} tokens of sequence {s}, of which the newest {c._fresh[s]} are whole")
-        for s, x in zip(self.seqs, counts):
-            c._length[s] -= x
-            c._position[s] -= x
-            c._fresh[s] -= x
-            c._change(s)
-        self.tokens, self._as_of = 0, [None] * self._n
+        self._step(_lib.PACKED_RETRACT, n)
 
     def _rows(self, t, heads, what):
         """A tensor (batch, heads, tokens, head_dim) with 16-byte aligned rows, copied if it has others; address and strides."""
@@ -271,7 +237,7 @@ class PackedBatch:
         a RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q)."""
         c = self.cache
         self._current()
-        if not self._whole:
+        if not self._info[2]:
             raise ValueError("tokens that an eviction has come after are not written again")
         k, k_at, k_bs, k_hs, k_ts = self._rows(k, c.n_kv_heads, "k")
         v, v_at, v_bs, v_hs, v_ts = self._rows(v, c.n_kv_heads, "v")
@@ -285,7 +251,7 @@ class PackedBatch:
         if rope is not None:
             if not isinstance(rope, RotaryEmbeddingESM) or rope.dim != c.head_dim:
                 raise ValueError(f"rope must be a RotaryEmbeddingESM of {c.head_dim} dimensions")
-            cos, sin = rope._tables(max(self._reach, 1), c.device)
+            cos, sin = rope._tables(max(self._info[1], 1), c.device)
             rows, cos, sin = cos.size(0), cos.data_ptr(), sin.data_ptr()
         rc = _lib_call.infllm_packed_write(c._ref, layer, self._table, self._n, self.tokens, k_at, k_bs, k_hs, k_ts, v_at, v_bs, v_hs, v_ts,
                                            q_at, q_bs, q_hs, q_ts, at, heads, cos, sin, rows, _lib.raw_stream(c.device))

@@ -516,3 +516,89 @@ extern "C" int infllm_packed_evict(const infllm_packed* c, const infllm_packed_s
     return INFLLM_OK;
   });
 }
+
+// -------------------------------------------------------------------------------------------------------- bookkeeping
+namespace {
+
+struct BookSeq {
+  int64_t opened, length, position, fresh, change;
+};
+BookSeq* book_of(infllm_packed_book* b) { return reinterpret_cast<BookSeq*>(b->state); }
+
+int book_check(const infllm_packed_book* b, const int32_t* seqs, int n, const char* what) {
+  if (!b || !b->state || b->n_sequences < 1 || b->max_tokens < 1 || n < 0 || (n > 0 && !seqs)) return fail(INFLLM_E_BADARG, "%s: no book, or %d sequences", what, n);
+  const BookSeq* s = reinterpret_cast<const BookSeq*>(b->state);
+  for (int i = 0; i < n; ++i)
+    if (seqs[i] < 0 || seqs[i] >= b->n_sequences || s[seqs[i]].opened % 2 == 0) return fail(INFLLM_E_BADARG, "there is no sequence %d", seqs[i]);
+  return INFLLM_OK;
+}
+
+}  // namespace
+
+extern "C" int infllm_packed_book_step(infllm_packed_book* book, int what, const int32_t* seqs, const int64_t* opened, int n, const int64_t* counts,
+                                       int64_t same, infllm_packed_seq* table, int64_t* as_of, int64_t* info) {
+  INFLLM_TRY(book_check(book, seqs, n, "packed_book_step"));
+  if (n > 0 && (!opened || (what != INFLLM_PACKED_RETRACT && (!table || !as_of)))) return fail(INFLLM_E_BADARG, "packed_book_step: null pointer");
+  if (what < INFLLM_PACKED_EXTEND || what > INFLLM_PACKED_RETRACT || !info) return fail(INFLLM_E_BADARG, "packed_book_step: step %d", what);
+  BookSeq* all = book_of(book);
+  for (int i = 0; i < n; ++i) {
+    const BookSeq& s = all[seqs[i]];
+    const int64_t x = counts ? counts[i] : same;
+    if (s.opened != opened[i]) return fail(INFLLM_E_BADARG, "sequence %d of this batch has been freed", seqs[i]);
+    if (x < 0) return fail(INFLLM_E_BADARG, "%lld tokens", (long long)x);
+    if (what == INFLLM_PACKED_EXTEND && x > book->max_tokens - s.length)
+      return fail(INFLLM_E_CAPACITY, "sequence %d of %lld tokens and %lld more, where %lld fit", seqs[i], (long long)s.length, (long long)x, (long long)book->max_tokens);
+    if (what == INFLLM_PACKED_EXTEND && x > INT32_MAX - s.position) return fail(INFLLM_E_CAPACITY, "sequence %d: a position beyond 31 bits", seqs[i]);
+    if (what == INFLLM_PACKED_PLAN && x > s.length) return fail(INFLLM_E_BADARG, "the newest %lld tokens of sequence %d, which has %lld", (long long)x, seqs[i], (long long)s.length);
+    if (what == INFLLM_PACKED_RETRACT && x > s.fresh)
+      return fail(INFLLM_E_BADARG, "%lld tokens of sequence %d, of which the newest %lld lie in a row", (long long)x, seqs[i], (long long)s.fresh);
+  }
+  info[0] = info[1] = 0, info[2] = 1;
+  for (int i = 0; i < n; ++i) {
+    BookSeq& s = all[seqs[i]];
+    const int64_t x = counts ? counts[i] : same, more = what == INFLLM_PACKED_EXTEND ? x : what == INFLLM_PACKED_RETRACT ? -x : 0;
+    if (what != INFLLM_PACKED_PLAN) s.length += more, s.position += more, s.fresh += more, s.change = ++book->changes;
+    if (what == INFLLM_PACKED_RETRACT) continue;
+    table[i] = {seqs[i], (int32_t)s.length, (int32_t)x, (int32_t)std::max<int64_t>(s.position - x, 0)};
+    as_of[i] = s.change;
+    info[0] = std::max(info[0], x);
+    if (x > 0) info[1] = std::max(info[1], s.position);
+    if (x > s.fresh) info[2] = 0;
+  }
+  return INFLLM_OK;
+}
+
+extern "C" int infllm_packed_book_evict(infllm_packed_book* book, const int32_t* seqs, int n, const int32_t* into, int64_t budget, int64_t sink,
+                                        int64_t recent, infllm_packed_seq* table, int64_t* most, int apply) {
+  return guarded("packed_book_evict", [&]() -> int {
+    INFLLM_TRY(book_check(book, seqs, n, "packed_book_evict"));
+    if (into) INFLLM_TRY(book_check(book, into, n, "packed_book_evict"));
+    BookSeq* all = book_of(book);
+    if (!apply) {
+      if (!most || (n > 0 && !table)) return fail(INFLLM_E_BADARG, "packed_book_evict: null pointer");
+      if (budget < 0 || sink < 0 || recent < 0 || sink > budget || recent > budget - sink)
+        return fail(INFLLM_E_BADARG, "%lld tokens stay, the first %lld and the newest %lld among them", (long long)budget, (long long)sink, (long long)recent);
+      std::vector<int32_t> names(seqs, seqs + n);
+      if (into) names.insert(names.end(), into, into + n);
+      std::sort(names.begin(), names.end());
+      for (size_t i = 1; i < names.size(); ++i)
+        if (names[i] == names[i - 1]) return fail(INFLLM_E_BADARG, "sequence %d twice", names[i]);
+      *most = 0;
+      for (int i = 0; i < n; ++i) {
+        const int64_t length = all[seqs[i]].length;
+        table[i] = {seqs[i], (int32_t)length, 0, 0};
+        *most = std::max(*most, std::min(length, budget));
+      }
+      return INFLLM_OK;
+    }
+    for (int i = 0; i < n; ++i) {
+      const BookSeq s = all[seqs[i]];
+      if (!into && s.length <= budget) continue;
+      BookSeq& to = all[into ? into[i] : seqs[i]];
+      to.length = std::min(s.length, budget), to.position = s.position;
+      to.fresh = s.length <= budget ? s.fresh : std::min(s.fresh, recent);
+      to.change = ++book->changes;
+    }
+    return INFLLM_OK;
+  });
+}

@@ -334,8 +334,7 @@ def test_offsets_past_32_bits():
     g = gen(5)
     c = make(8, 128, 40, 131072)
     assert c.codes[0, 0].numel() * 4 > 1 << 31
-    c._length[39], c._open[39] = 0, True
-    seqs = [39]
+    seqs = c.open(40)[39:]
     b = c.batch(seqs)
     b.extend(131072 - 40)
     b.extend(40)
@@ -349,7 +348,6 @@ def test_offsets_past_32_bits():
         q = rand(g, 1, 8, n, 128)
         out, lse = b.attend(0, q, return_lse=True, weigh=True, decay=0.0)
         check(c, b, [n], q, out, lse, weigh=n, before=c.weights, decay=0.0)
-    c._open[3] = True
     c.evict(seqs, 300, 100, 100, into=[3])
     assert (c.places[0, 3, :, 200:300] == c.places[0, 39, :, -100:]).all()
     want = stay_of(c.weights[0, 39], 131072, 300, 100, 100)

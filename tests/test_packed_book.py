@@ -11,12 +11,15 @@ from infllm_b200.attention import PackedCache, packed_cache
 
 
 class Calls:
-    """The library, of which calls are noted and nothing is launched."""
+    """The library, of which calls that launch something are noted and not made."""
 
     def __init__(self):
         self.seen = []
 
     def __getattr__(self, name):
+        if "book" in name or name == "infllm_last_error":
+            return getattr(L.lib, name)
+
         def call(*args):
             self.seen.append((name, args))
             return 0
@@ -45,7 +48,11 @@ def test_a_cpu_device_is_refused():
 
 
 def state(c):
-    return [list(x) for x in (c._open, c._length, c._position, c._fresh)]
+    return list(c._state)
+
+
+def fresh(c, s):  # newest tokens that are known to lie in a row
+    return c._state[5 * s + 3]
 
 
 def test_lowest_numbers_and_capacity(cache):
@@ -63,13 +70,19 @@ def test_lowest_numbers_and_capacity(cache):
         b.extend([0, 18])
     with pytest.raises(L.InfLLMCapacityError):
         b.extend(1)
+    for n in (1 << 40, [0, 1 << 62]):
+        with pytest.raises(L.InfLLMCapacityError):
+            b.extend(n)
+    for n in (1 << 63, [0, 1 << 64]):
+        with pytest.raises(OverflowError):
+            b.extend(n)
     assert state(c) == before
 
 
 @pytest.mark.parametrize("call", [
     lambda c, b: c.batch([0, 0]), lambda c, b: c.batch([3]), lambda c, b: c.batch([-1]), lambda c, b: c.batch([9]), lambda c, b: c.free([0, 0]),
     lambda c, b: c.length(3), lambda c, b: c.position(-2), lambda c, b: c.open(-1), lambda c, b: b.extend(-1), lambda c, b: b.extend([1]),
-    lambda c, b: b.plan([11, 1]), lambda c, b: b.retract(7), lambda c, b: c.evict([0, 0], 4), lambda c, b: c.evict([0], -1),
+    lambda c, b: b.extend([1, -1]), lambda c, b: b.plan([11, 1]), lambda c, b: b.retract(7), lambda c, b: c.evict([0, 0], 4), lambda c, b: c.evict([0], -1),
     lambda c, b: c.evict([0], 4, 3, 2), lambda c, b: c.evict([0], 4, -1), lambda c, b: c.evict([0], 4, 0, -1), lambda c, b: c.evict([0, 1], 4, into=[1, 2]),
     lambda c, b: c.evict([0, 1], 4, into=[2]), lambda c, b: c.evict([0], 4, into=[3]), lambda c, b: c.evict([0], 4, into=[0])])
 def test_refusals_change_nothing(cache, call):
@@ -97,15 +110,14 @@ def test_positions_go_on_behind_an_eviction(cache):
     b.retract(2)
     assert (c.length(s), c.position(s)) == (6, 16)
     b.extend(5)
-    assert list(b._table)[:4] == [s, 11, 5, 16] and b._reach == 21
+    assert list(b._table)[:4] == [s, 11, 5, 16] and b._info[1] == 21
     b.plan(11)
     with pytest.raises(ValueError, match="eviction"):
         b.write(0, None, None)
     c.evict([s], 30)  # nothing to do
     assert (c.length(s), c.position(s)) == (11, 21)
-    b.values(0) if torch.cuda.is_available() else None
     c.evict([s], 4, recent=4, into=[t])
-    assert (c.length(s), c.length(t), c.position(t), c._fresh[t]) == (11, 4, 21, 4)
+    assert (c.length(s), c.length(t), c.position(t), fresh(c, t)) == (11, 4, 21, 4)
     c.evict([s], 40, into=[t])
     assert (c.length(t), c.position(t)) == (11, 21)
 
@@ -144,26 +156,26 @@ def test_random_books_agree_with_a_restatement(cache):
             held[s] = ([], 0, 0)
         elif held:
             s = rng.choice(sorted(held))
-            rows, pos, fresh = held[s]
+            rows, pos, new = held[s]
             n = rng.randint(0, 12)
             if what == "extend" and len(rows) + n <= 50:
                 c.batch([s]).extend(n)
-                held[s] = (rows + list(range(pos, pos + n)), pos + n, fresh + n)
-            elif what == "retract" and n <= fresh:
+                held[s] = (rows + list(range(pos, pos + n)), pos + n, new + n)
+            elif what == "retract" and n <= new:
                 c.batch([s]).retract(n)
-                held[s] = (rows[:len(rows) - n], pos - n, fresh - n)
+                held[s] = (rows[:len(rows) - n], pos - n, new - n)
             elif what == "evict":
                 recent = rng.randint(0, 10)
                 budget = recent + rng.randint(0, 20)
                 c.evict([s], budget, recent=recent)
                 if len(rows) > budget:
-                    held[s] = (rows[:budget - recent] + rows[len(rows) - recent:], pos, min(fresh, recent))
+                    held[s] = (rows[:budget - recent] + rows[len(rows) - recent:], pos, min(new, recent))
             elif what == "free":
                 c.free([s])
                 del held[s]
-        for s, (rows, pos, fresh) in held.items():
-            assert (c.length(s), c.position(s), c._fresh[s]) == (len(rows), pos, fresh)
-            assert not fresh or rows[-fresh:] == list(range(pos - fresh, pos))
+        for s, (rows, pos, new) in held.items():
+            assert (c.length(s), c.position(s), fresh(c, s)) == (len(rows), pos, new)
+            assert not new or rows[-new:] == list(range(pos - new, pos))
 
 
 # ------------------------------------------------------------------------------------------------- the C entry points
