@@ -44,24 +44,42 @@ __device__ __forceinline__ float2 span32(const uint4& x, uint32_t quad) {
   return make_float2(Act<T>::to_f(a), Act<T>::to_f(b));
 }
 
-// eight numbers of a row as codes, and their group's (m, s)
+// Eight numbers of a row as codes, and their group's (m, s).
+// A quotient of 16-bit numbers' differences lies on the border between two codes, or further from it than the last place in 32 bits: so
+// a rounded quotient has the definition's code.  q0 = t / s by the reciprocal is off by some last places, and q0 + (t - q0 s) / s, whose
+// remainder is exact, is the rounded quotient wherever that is a border: five operations a number instead of a division's
+// dozen, after which writes are bound by their bytes.
 template <typename T>
 __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_t* ms) {
   const float2 span = span32<T>(x, quad);
   T step = Act<T>::from_f(__fdiv_rn(span.y - span.x, 15.f));
   const T least = Act<T>::from_f(span.x);
   const float s = Act<T>::to_f(step);
-  if (Codes<T>::kBf16 && s >= 0x1p122f) step = Act<T>::from_f(NAN);
-  const T* p = reinterpret_cast<const T*>(&x);
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // (a quotient of 16-bit numbers' differences in fp32 falls on a half only where it is one)
-    const int c = s == 0.f ? 0 : __float2int_rn(__fdiv_rn(Act<T>::to_f(p[i]) - span.x, s));
-    w |= (uint32_t)min(max(c, 0), 15) << (4 * (i >> 1) + 16 * (i & 1));
-  }
+  const bool held = s < (Codes<T>::kBf16 ? 0x1p122f : INFINITY);  // (not where one is not finite, either)
+  if (!held) step = Act<T>::from_f(NAN);
   const typename Act<T>::T2 pair = {least, step};
   *ms = *reinterpret_cast<const uint32_t*>(&pair);
+  const typename Act<T>::T2* p = reinterpret_cast<const typename Act<T>::T2*>(&x);
+  uint32_t w = 0;
+  if (!held) return 0;
+  if (s < 0x1p-100f) {  // (0, or so small that its reciprocal is not one)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = Act<T>::to_f2(p[i >> 1]);
+      const int c = s == 0.f ? 0 : __float2int_rn(__fdiv_rn((i & 1 ? f.y : f.x) - span.x, s));
+      w |= (uint32_t)min(max(c, 0), 15) << (4 * (i >> 1) + 16 * (i & 1));
+    }
+    return w;
+  }
+  const float inv = __frcp_rn(s);
+  constexpr float kMagic = 8388608.f;  // 2^23: what is added to it is rounded to a whole number, ties to even, in its low bits
+  constexpr uint32_t kMagicBits = 0x4b000000u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = Act<T>::to_f2(p[i >> 1]);
+    const float t = (i & 1 ? f.y : f.x) - span.x, q0 = t * inv, q = fmaf(fmaf(-q0, s, t), inv, q0);
+    w += (__float_as_uint(fminf(q, 15.f) + kMagic) - kMagicBits) << (4 * (i >> 1) + 16 * (i & 1));
+  }
   return w;
 }
 
@@ -141,30 +159,36 @@ struct PackReadParams {
   PackedSeq seq[kPackSeqs];
 };
 
-// a thread per word of eight numbers
+// kReadEach words of eight numbers a thread, of a head's tokens
+constexpr int kReadThreads = 256, kReadEach = 4;
 template <typename T, int kDim>
-__global__ void __launch_bounds__(256) packed_values_kernel(const __grid_constant__ PackReadParams P) {
+__global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __grid_constant__ PackReadParams P) {
   constexpr int kWords = kDim / 8;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int w = (int)(idx % kWords);
-  const int64_t r = idx / kWords;
-  const int i = (int)(r % P.most), h = (int)(r / P.most);
-  if (h >= P.at.n_kv) return;
+  const int per = (P.most * kWords + kReadThreads * kReadEach - 1) / (kReadThreads * kReadEach), h = blockIdx.x / per;
+  const int first = (blockIdx.x - h * per) * kReadThreads * kReadEach + threadIdx.x, words = P.most * kWords;
   const int layer = blockIdx.z >> 1, val = blockIdx.z & 1;
   const PackedSeq S = P.seq[blockIdx.y];
-  const int at = i - (P.most - S.count);
-  uint4 out = make_uint4(0, 0, 0, 0);
-  if (at >= 0) {
-    const int64_t row = P.at.row0(S.slot, h) + S.length - S.count + at;
-    const uint32_t c = reinterpret_cast<const uint32_t*>(P.at.codes + layer * P.codes_layer + val * P.at.codes_v + row * (kDim / 2))[w];
-    const uint32_t ms = reinterpret_cast<const uint32_t*>(P.at.scales + layer * P.scales_layer + val * P.at.scales_v + row * (kDim / 8))[w / 4];
-    const auto m2 = Codes<T>::least2(ms), s2 = Codes<T>::step2(ms);
-    uint32_t v[4];
-    Codes<T>::pairs(c, m2, s2, v);
-    out = make_uint4(v[0], v[1], v[2], v[3]);
+  const int64_t row0 = P.at.row0(S.slot, h) + S.length - P.most;  // (the tokens stand at the end)
+  const char* codes = P.at.codes + layer * P.codes_layer + val * P.at.codes_v;
+  const char* scales = P.at.scales + layer * P.scales_layer + val * P.at.scales_v;
+  uint4* to = reinterpret_cast<uint4*>(val ? P.v : P.k) + (((int64_t)layer * P.batch + P.b0 + blockIdx.y) * P.at.n_kv + h) * (int64_t)words;
+  uint32_t c[kReadEach], ms[kReadEach];
+#pragma unroll
+  for (int x = 0; x < kReadEach; ++x) {
+    const int at = first + x * kReadThreads, i = at / kWords, w = at % kWords;
+    c[x] = ms[x] = 0;  // (numbers of no token: 0)
+    if (at < words && i >= P.most - S.count) {
+      c[x] = __ldg(reinterpret_cast<const uint32_t*>(codes + (row0 + i) * (kDim / 2)) + w);
+      ms[x] = __ldg(reinterpret_cast<const uint32_t*>(scales + (row0 + i) * (kDim / 8)) + w / 4);
+    }
   }
-  char* to = (val ? P.v : P.k) + ((((int64_t)layer * P.batch + P.b0 + blockIdx.y) * P.at.n_kv + h) * P.most + i) * (kDim * 2);
-  *reinterpret_cast<uint4*>(to + w * 16) = out;
+#pragma unroll
+  for (int x = 0; x < kReadEach; ++x) {
+    const int at = first + x * kReadThreads;
+    uint32_t v[4];
+    Codes<T>::pairs(c[x], Codes<T>::least2(ms[x]), Codes<T>::step2(ms[x]), v);
+    if (at < words) to[at] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------- eviction
@@ -175,6 +199,7 @@ __global__ void __launch_bounds__(256) packed_values_kernel(const __grid_constan
 // so, in place, the blocks read kRound rows each, wait for each other, and write; what the next round reads lies behind all that
 // this one has written.
 constexpr int kEvictThreads = 256, kRound = 128, kEach = 8;
+constexpr int kEvictRoom = 10240;  // weights a block: 40 KB, so that five have room on a multiprocessor
 
 struct EvictParams {
   PackedPlanes at;
@@ -184,7 +209,7 @@ struct EvictParams {
   int64_t rows_layer;
   int32_t* stay;      // (layers, sequences, KV heads, most_stay): of the middle tokens those that stay
   int64_t seq0, n_seqs, most_stay;
-  int32_t budget, sink, recent;
+  int32_t budget, sink, recent, room;  // weights that shared memory has room for
   bool copy;
   int2 seq[kPackSeqs];   // slot, length
   int32_t into[kPackSeqs];
@@ -213,6 +238,13 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
   const bool choose = !all && k > 0;
   if (choose) {
     const int share = (late - sink + n_ctas - 1) / n_ctas, first = sink + min(me * share, late - sink), last = min(first + share, late);
+    // The share's weights, as whole numbers, in shared memory as far as there is room; the others are read again each time
+    extern __shared__ uint32_t ranks[];
+    const int room = P.room;
+#pragma unroll 8
+    for (int j = first + tid; j < min(last, first + room); j += kEvictThreads) ranks[j - first] = weight_rank(weights[j]);
+    auto rank_of = [&](int j) { return j - first < room ? ranks[j - first] : weight_rank(weights[j]); };
+    __syncthreads();
     uint32_t cut = 0;
     int need = k;
 #pragma unroll 1
@@ -222,7 +254,7 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
       mine[tid] = 0;
       __syncthreads();
       for (int j = first + tid; j < last; j += kEvictThreads) {
-        const uint32_t u = weight_rank(weights[j]);
+        const uint32_t u = rank_of(j);
         if (pass == 0 || (u ^ cut) >> (shift + 8) == 0) atomicAdd(&mine[u >> shift & 255], 1);
       }
       cluster.sync();  // (of the pass after the next, whose counts take this one's place, nobody is ahead of the next one's)
@@ -246,7 +278,7 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
     // of the tokens of weight `cut` the first `need` stay
     int larger = 0, equal = 0;
     for (int j = first + tid; j < last; j += kEvictThreads) {
-      const uint32_t u = weight_rank(weights[j]);
+      const uint32_t u = rank_of(j);
       larger += u > cut, equal += u == cut;
     }
     larger = __reduce_add_sync(0xffffffffu, larger), equal = __reduce_add_sync(0xffffffffu, equal);
@@ -271,7 +303,7 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
 #pragma unroll
       for (int x = 0; x < kEach; ++x) {
         const bool in = j0 + x < last;
-        u[x] = in ? weight_rank(weights[j0 + x]) : 0;
+        u[x] = in ? rank_of(j0 + x) : 0;
         g += in && u[x] > cut, e += in && u[x] == cut;
       }
       int sg = g, se = e;
@@ -443,8 +475,8 @@ extern "C" int infllm_packed_values(const infllm_packed* c, int layer, int n_lay
     if (layer < 0 || n_layers < 1 || layer > c->n_layers - n_layers) return fail(INFLLM_E_BADARG, "packed_values: layers %d and %d more of %d", layer, n_layers - 1, c->n_layers);
     if (n == 0 || most == 0) return INFLLM_OK;
     if (!d_k || !d_v || ((uintptr_t)d_k | (uintptr_t)d_v) % 16) return fail(INFLLM_E_BADARG, "packed_values: the outputs have to be 16-byte aligned");
-    const int64_t blocks = ceil_div((int64_t)c->n_kv_heads * most * (c->head_dim / 8), 256);
-    if (blocks > INT_MAX) return fail(INFLLM_E_BADARG, "packed_values: %d tokens of %d KV heads", most, c->n_kv_heads);
+    const int64_t words = (int64_t)most * (c->head_dim / 8), blocks = c->n_kv_heads * ceil_div(words, kReadThreads * kReadEach);
+    if (blocks > INT_MAX || words > INT_MAX - kReadThreads * kReadEach) return fail(INFLLM_E_BADARG, "packed_values: %d tokens of %d KV heads", most, c->n_kv_heads);
     DeviceScope scope(c->device);
     PackReadParams P;
     P.k = (char*)d_k, P.v = (char*)d_v;
@@ -457,7 +489,7 @@ extern "C" int infllm_packed_values(const infllm_packed* c, int layer, int n_lay
       const dim3 grid((unsigned)blocks, m, 2 * n_layers);
       INFLLM_DISPATCH_DTYPE(c->dtype, T, {
         auto kern = c->head_dim == 128 ? packed_values_kernel<T, 128> : packed_values_kernel<T, 64>;
-        kern<<<grid, 256, 0, (cudaStream_t)stream>>>(P);
+        kern<<<grid, kReadThreads, 0, (cudaStream_t)stream>>>(P);
       });
       INFLLM_LAUNCH_OK("packed_values_kernel");
     }
@@ -501,9 +533,11 @@ extern "C" int infllm_packed_evict(const infllm_packed* c, const infllm_packed_s
       const int64_t heads = (int64_t)c->n_layers * m * c->n_kv_heads;
       int ctas = 8;
       while (ctas > 1 && heads * ctas > 148 * 4) ctas /= 2;
+      P.room = (int32_t)std::min<int64_t>(ceil_div(longest, ctas), kEvictRoom);
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)(c->n_kv_heads * ctas), m, c->n_layers);
       cfg.blockDim = dim3(kEvictThreads);
+      cfg.dynamicSmemBytes = (size_t)P.room * 4;
       cfg.stream = (cudaStream_t)stream;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
