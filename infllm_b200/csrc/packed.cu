@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __gri
 // counts before it give; ties go to the earlier token.  Then the rows close up: a row's new place is never behind its old one,
 // so, in place, the blocks read kRound rows each, wait for each other, and write; what the next round reads lies behind all that
 // this one has written.
-constexpr int kEvictThreads = 256, kRound = 128, kEach = 8;
+constexpr int kEvictThreads = 256, kRound = 256, kEach = 8;
 constexpr int kEvictRoom = 10240;  // weights a block: 40 KB, so that five have room on a multiprocessor
 
 struct EvictParams {
@@ -259,7 +259,9 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
       }
       cluster.sync();  // (of the pass after the next, whose counts take this one's place, nobody is ahead of the next one's)
       int sum = 0;
-      for (int c = 0; c < n_ctas; ++c) sum += cluster.map_shared_rank(mine, c)[255 - tid];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)  // (all on their way at once)
+        if (c < n_ctas) sum += cluster.map_shared_rank(mine, c)[255 - tid];
       // digits from the largest down: how many tokens have a larger one
       int upto = sum;
 #pragma unroll
@@ -334,10 +336,10 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
   // ---- the rows close up
   constexpr int kCode = kDim / 32, kPer = kRound * kCode / kEvictThreads;  // 16-byte pieces of a row's codes; of a thread
   using Scale = typename std::conditional<kDim == 128, uint4, uint2>::type;
-  static_assert(kRound * 2 == kEvictThreads, "");
+  static_assert(kRound == kEvictThreads, "");
   const char* codes = P.at.codes + layer * P.codes_layer;
   const char* scales = P.at.scales + layer * P.scales_layer;
-  int32_t* words = reinterpret_cast<int32_t*>(tid & 1 ? P.weights : reinterpret_cast<float*>(P.places)) + layer * P.rows_layer;
+  int32_t* words[2] = {P.places + layer * P.rows_layer, reinterpret_cast<int32_t*>(P.weights) + layer * P.rows_layer};
   const int tail = all ? n : P.budget - P.recent;  // the first of the newest
 #pragma unroll 1
   for (int base = P.copy ? 0 : sink; base < kept; base += n_ctas * kRound) {
@@ -346,8 +348,8 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
     if (tid < rows) src[tid] = r0 + tid < sink ? r0 + tid : r0 + tid < tail ? stay[r0 + tid - sink] : late + r0 + tid - tail;
     __syncthreads();
     uint4 c[2][kPer];
-    Scale s;
-    int32_t word;
+    Scale s[2];
+    int32_t word[2];
     // (a row that stays where it is is not touched)
     auto moves = [&](int r) { return r < rows && (P.copy || src[r] != r0 + r); };
 #pragma unroll
@@ -358,9 +360,12 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
         for (int v = 0; v < 2; ++v) c[v][x] = *reinterpret_cast<const uint4*>(codes + v * P.at.codes_v + (from + src[r]) * (kDim / 2) + p * 16);
       }
     }
-    if (moves(tid >> 1)) {
-      s = *reinterpret_cast<const Scale*>(scales + (tid & 1) * P.at.scales_v + (from + src[tid >> 1]) * (kDim / 8));
-      word = words[from + src[tid >> 1]];
+    if (moves(tid)) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        s[v] = *reinterpret_cast<const Scale*>(scales + v * P.at.scales_v + (from + src[tid]) * (kDim / 8));
+        word[v] = words[v][from + src[tid]];
+      }
     }
     if (!P.copy) cluster.sync();
 #pragma unroll
@@ -371,9 +376,12 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
         for (int v = 0; v < 2; ++v) *reinterpret_cast<uint4*>(const_cast<char*>(codes) + v * P.at.codes_v + (to + r0 + r) * (kDim / 2) + p * 16) = c[v][x];
       }
     }
-    if (moves(tid >> 1)) {
-      *reinterpret_cast<Scale*>(const_cast<char*>(scales) + (tid & 1) * P.at.scales_v + (to + r0 + (tid >> 1)) * (kDim / 8)) = s;
-      words[to + r0 + (tid >> 1)] = word;
+    if (moves(tid)) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        *reinterpret_cast<Scale*>(const_cast<char*>(scales) + v * P.at.scales_v + (to + r0 + tid) * (kDim / 8)) = s[v];
+        words[v][to + r0 + tid] = word[v];
+      }
     }
   }
 }
