@@ -1,11 +1,11 @@
-// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that seven warps
+// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that sixteen warps
 // take out of their codes, S and O in TMEM.
 //
 // A unit is up to 256 rows of one KV head by a stretch of keys.  Two teams of four softmax warps, a thread per row, have 128 rows each;
 // of up to 128 rows both have all, and take the key tiles in turn: each with a maximum, a sum and an O of its own, which are put
 // together at the unit's end, where a thread reads the other team's O of its row from TMEM.  (A tile is in a team's hands for 1.1 us:
 // with one team that, not its bytes, would be a tile's time.)
-// Seven more warps bring codes from global memory through registers, tiles ahead, and leave 16-bit numbers, swizzled as the products
+// Sixteen more warps bring codes from global memory through registers, and leave 16-bit numbers, swizzled as the products
 // want them, in a ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is taken out once
 // for 256 rows.  Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A operand of P V from
 // there, have 128 columns, O another 128.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only
@@ -24,8 +24,8 @@ namespace infllm {
 
 namespace xtc {
 constexpr int kStages = 5;
-constexpr int kWarpMma = 8, kWarpCodes = 9, kCodeWarps = 7;
-constexpr int kThreads = (kWarpCodes + kCodeWarps) * 32;
+constexpr int kWarpCodes = 8, kCodeWarps = 8, kWarpMma = kWarpCodes + kCodeWarps;  // half of them keys, half values
+constexpr int kThreads = (kWarpMma + 1) * 32;
 enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, Q_FULL0 = EMPTY0 + kStages, S_FULL0 = Q_FULL0 + 2, P_FULL0 = S_FULL0 + 2, PV_DONE0 = P_FULL0 + 2, MERGE = PV_DONE0 + 2, N_BARS };
 template <int kDim>
 struct Smem {
@@ -68,6 +68,26 @@ struct Pieces {  // a block's, in turn
 };
 }  // namespace xtc
 
+// (16 columns at a time: the softmax warps are to do with 96 registers a thread, so that there is room for more warps)
+__device__ __forceinline__ void tmem_ld16_if(bool yes, uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %17, 0;\n\t"
+      "@p tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t}"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+      : "r"(taddr), "r"((uint32_t)yes)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               ::"memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
 template <typename T, int kDim>
 __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __grid_constant__ PackedTcParams P) {
   using namespace xtc;
@@ -87,7 +107,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
   if (warp == 0) {
     static_assert(N_BARS <= 32 && N_BARS * 8 + 16 <= 256, "");
     // tiles: the warps that make them; queries and probabilities: a team's four; what the teams have of the same rows: both
-    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 ? (uint32_t)kCodeWarps : lane == Q_FULL0 || lane == Q_FULL0 + 1 || lane == P_FULL0 || lane == P_FULL0 + 1 ? 4u : lane == MERGE ? 8u : 1u);
+    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 ? (uint32_t)kCodeWarps / 2 : lane == Q_FULL0 || lane == Q_FULL0 + 1 || lane == P_FULL0 || lane == P_FULL0 + 1 ? 4u : lane == MERGE ? 8u : 1u);
     if (lane == 0) *abort_flag = 0;
     mbar_fence_init();
   }
@@ -103,135 +123,104 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
   constexpr uint32_t idesc_qk = make_idesc(kBf16, 128, 128, false), idesc_pv = make_idesc(kBf16, 128, kDim, true);
   chain_enter();
 
-  if (warp >= kWarpCodes) {
+  if (warp >= kWarpCodes && warp < kWarpMma) {
     // ======================================================================================================== numbers
-    // A thread has the 32 numbers of one (m, s): a 16-byte piece of a row of codes.  A turn is a key tile and the value tile before it; the
-    // next turn's codes are on their way through registers meanwhile, those kAhead tiles behind it to L2.
+    // Eight warps take key tiles, eight value tiles.  A thread has the 32 numbers of one (m, s), a 16-byte piece of a row of codes, of
+    // kPer rows; the next tile's are on their way through registers while it is at work, those kAhead tiles ahead to L2.
     // (Eight lanes that write 16 bytes at a time have four rows and pieces of one half of them: eight different bank groups.)
     using C = Codes<T>;
-    constexpr int kGroups = kDim / 32, kStep = kCodeWarps * 32 / kGroups, kPer = (128 + kStep - 1) / kStep, kAhead = 4;
+    constexpr int kGroups = kDim / 32, kStep = kCodeWarps / 2 * 32 / kGroups, kPer = (128 + kStep - 1) / kStep, kAhead = 4;
     constexpr int kRow = kDim / 2, kScales = kDim / 8;  // bytes
     static_assert(kStep % 8 == 0, "");
-    const int at = (warp - kWarpCodes) * 32 + lane;
+    const bool values = warp >= kWarpCodes + kCodeWarps / 2;
+    const int w8 = (warp - kWarpCodes) % (kCodeWarps / 2), at = w8 * 32 + lane;
     const int t = kGroups == 4 ? (lane >> 3 & 1) * 2 + (lane & 1) : lane & 1;
-    const int r0 = (warp - kWarpCodes) * (32 / kGroups) + (kGroups == 4 ? (lane >> 4) * 4 + (lane >> 1 & 3) : lane >> 1);
+    const int r0 = w8 * (32 / kGroups) + (kGroups == 4 ? (lane >> 4) * 4 + (lane >> 1 & 3) : lane >> 1);
     struct Raw {
-      uint32_t c[2][kPer][4], ms[2][kPer];
-    };
-    struct Turn {
-      bool more;
-      int i, n;   // the key tile, of the piece's
-      int keys;   // from its first one to the piece's last
-      int seen;   // of those that every row sees
-      const char *codes, *scales;  // this thread's of the key tile's first row
+      uint32_t c[kPer][4], ms[kPer];
     };
     Pieces pieces(P);
+    bool more = false;
+    int i = 0, n = 0, base = 0;     // the tile of the piece's, and the piece's place in the ring
+    int keys = 0, seen = 0;         // from the tile's first one to the piece's last; of those that every row sees
+    const char *codes = nullptr, *scales = nullptr;  // this thread's of the tile's first row
     auto begin = [&]() {
-      Turn o{};
       Piece U;
-      o.more = pieces.next(P, U);
-      if (o.more) {
-        const PackedAttnSeq& S = P.a.seq[U.b];
-        o.n = U.n, o.keys = U.keys, o.seen = keys_of_row(S, P.a.group, U.row0) - U.tile0 * kKeyTile;
-        const int64_t row = P.a.at.row0(S.slot, U.hkv) + U.tile0 * kKeyTile;
-        o.codes = P.a.at.codes + row * kRow, o.scales = P.a.at.scales + row * kScales;
-      }
-      return o;
+      more = pieces.next(P, U);
+      if (!more) return;
+      const PackedAttnSeq& S = P.a.seq[U.b];
+      const int64_t row = P.a.at.row0(S.slot, U.hkv) + U.tile0 * kKeyTile;
+      base += 2 * n, i = 0, n = U.n, keys = U.keys, seen = keys_of_row(S, P.a.group, U.row0) - U.tile0 * kKeyTile;
+      codes = P.a.at.codes + (values ? P.a.at.codes_v : 0) + row * kRow + r0 * kRow + t * 16;
+      scales = P.a.at.scales + (values ? P.a.at.scales_v : 0) + row * kScales + r0 * kScales + t * 4;
     };
-    auto advance = [&](Turn& o) {
-      if (o.i < o.n) ++o.i, o.keys -= kKeyTile, o.seen -= kKeyTile, o.codes += kKeyTile * kRow, o.scales += kKeyTile * kScales;
-      else o = begin();
+    auto advance = [&]() {
+      if (i + 1 < n) ++i, keys -= kKeyTile, seen -= kKeyTile, codes += kKeyTile * kRow, scales += kKeyTile * kScales;
+      else begin();
     };
-    const int64_t to_values = P.a.at.codes_v - kKeyTile * kRow, to_value_scales = P.a.at.scales_v - kKeyTile * kScales;
-    const int in_codes = r0 * kRow + t * 16, in_scales = r0 * kScales + t * 4;
-    // lines of 128 bytes of a tile: its codes' and its scales'
+    // lines of 128 bytes of a tile kAhead tiles on: its codes' and its scales'
     constexpr int kLines = kRow, kAll = kLines + kScales;
-    static_assert(2 * kAll <= kCodeWarps * 32, "");
-    const bool fetch_values = at >= kAll;
-    const int line = at - fetch_values * kAll;
-    const int fetch_key = kAhead * kKeyTile + (line < kLines ? line * 128 / kRow : (line - kLines) * 128 / kScales);
-    const int64_t fetch = (line < kLines ? (int64_t)fetch_key * kRow : (int64_t)fetch_key * kScales) + (!fetch_values ? 0 : line < kLines ? P.a.at.codes_v : P.a.at.scales_v);
-    auto load = [&](const Turn& o, Raw& r) {
+    static_assert(kAll <= kCodeWarps / 2 * 32, "");
+    const int fetch_key = kAhead * kKeyTile + (at < kLines ? at * 128 / kRow : (at - kLines) * 128 / kScales);
+    const int fetch = at < kLines ? (fetch_key - r0) * kRow - t * 16 : (fetch_key - r0) * kScales - t * 4;  // from this thread's own
+    auto load = [&](Raw& r) {
       // what lies behind the last key is not read: its numbers are 0 by their (m, s), whatever their codes
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const int nk = !o.more ? 0 : v ? (o.i > 0 ? o.keys + kKeyTile : 0) : o.i < o.n ? o.keys : 0;
-        const char* codes = o.codes + in_codes + (v ? to_values : 0);
-        const char* scales = o.scales + in_scales + (v ? to_value_scales : 0);
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          const bool there = r0 + x * kStep < min(nk, kKeyTile);
-          r.ms[v][x] = 0;
-          asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %7, 0;\n\t"
-                       "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%5];\n\t"
-                       "@p ld.global.nc.u32 %4, [%6];\n\t}"
-                       : "+r"(r.c[v][x][0]), "+r"(r.c[v][x][1]), "+r"(r.c[v][x][2]), "+r"(r.c[v][x][3]), "+r"(r.ms[v][x])
-                       : "l"(codes + x * kStep * kRow), "l"(scales + x * kStep * kScales), "r"((int)there));
-        }
+      for (int x = 0; x < kPer; ++x) {
+        const bool there = more && r0 + x * kStep < min(keys, kKeyTile);
+        r.ms[x] = 0;
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+                     "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%5];\n\t"
+                     "@p ld.global.nc.u32 %4, [%6];\n\t}"
+                     : "+r"(r.c[x][0]), "+r"(r.c[x][1]), "+r"(r.c[x][2]), "+r"(r.c[x][3]), "+r"(r.ms[x])
+                     : "l"(codes + x * kStep * kRow), "l"(scales + x * kStep * kScales), "r"((int)there));
       }
-      if (o.more && at < 2 * kAll && fetch_key < o.keys) asm volatile("prefetch.global.L2 [%0];" ::"l"((line < kLines ? o.codes : o.scales) + fetch));
+      if (more && at < kAll && fetch_key < keys) asm volatile("prefetch.global.L2 [%0];" ::"l"((at < kLines ? codes : scales) + fetch));
     };
     uint32_t piece[4];  // of a tile: where this thread's 16 bytes go
 #pragma unroll
     for (int j = 0; j < 4; ++j) piece[j] = (t >> 1) * kSubTileBytes + r0 * 128 + ((((t & 1) * 4 + j) ^ (r0 & 7)) << 4);
-    bool ok = true;
-    int slot = 0;
-    Raw raw{}, then{};
-    Turn now = begin();
-    load(now, raw);
     // (two copies of a turn, each with its own registers: what is on its way is not to be moved, which would wait for it)
     auto turn = [&](Raw& raw, Raw& then) {
-      Turn after = now;
-      advance(after);
-      load(after, then);
-      if (now.seen < kKeyTile) {
+      const int slot = base + (values ? pos_v(i, n) : pos_k(i));
+      if (seen < kKeyTile) {
         // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and
         // its key is no number in its place, so that the rows that see it still become none.
-        const char* scales = now.scales + P.a.at.scales_v;
+        const char* other = scales - t * 4 + P.a.at.scales_v;
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          const int k = r0 + x * kStep;
-          if (now.seen < 0 && C::odd(raw.ms[1][x])) raw.ms[1][x] = 0;
-          if (now.i < now.n && k < min(now.keys, kKeyTile))
+          if (values && C::odd(raw.ms[x])) raw.ms[x] = 0;
+          if (!values && r0 + x * kStep < min(keys, kKeyTile))
             for (int g = 0; g < kGroups; ++g)
-              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + k * kScales + g * 4)))) raw.ms[0][x] = 0x7fff7fffu;
+              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(other + x * kStep * kScales + g * 4)))) raw.ms[x] = 0x7fff7fffu;
         }
       }
-      const int first = slot;
+      advance();
+      load(then);
+      const int b = slot % kStages;
+      // (a tile of the other kind, up to three places before in the ring, has not passed this one: the phase is the next one of the barrier)
+      if (slot >= kStages && !warp_wait(bar(EMPTY0 + b), ring_parity(slot - kStages, kStages), abort_flag, err, 751)) return false;
+      unsigned char* to = smem + L::kRing + b * L::kTileBytes;
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        if (v ? now.i == 0 : now.i == now.n) continue;
-        const int b = slot % kStages;
-        if (ok && slot >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot - kStages, kStages), abort_flag, err, 751);
-        if (ok) {
-          unsigned char* to = smem + L::kRing + b * L::kTileBytes;
+      for (int x = 0; x < kPer; ++x) {
+        if ((x + 1) * kStep > 128 && r0 + x * kStep >= 128) continue;
+        const auto m2 = C::least2(raw.ms[x]), s2 = C::step2(raw.ms[x]);
 #pragma unroll
-          for (int x = 0; x < kPer; ++x) {
-            if ((x + 1) * kStep > 128 && r0 + x * kStep >= 128) continue;
-            const auto m2 = C::least2(raw.ms[v][x]), s2 = C::step2(raw.ms[v][x]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
-              C::pairs(raw.c[v][x][j], m2, s2, w);
-              *reinterpret_cast<uint4*>(to + piece[j] + x * kStep * 128) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
+        for (int j = 0; j < 4; ++j) {
+          uint32_t w[4];
+          C::pairs(raw.c[x][j], m2, s2, w);
+          *reinterpret_cast<uint4*>(to + piece[j] + x * kStep * 128) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        ++slot;
       }
-      if (!ok) return false;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane < slot - first) mbar_arrive(bar(FULL0 + (first + lane) % kStages));
-      now = after;
-      return now.more;
+      if (lane == 0) mbar_arrive(bar(FULL0 + b));
+      return more;
     };
-    while (now.more && turn(raw, then) && turn(then, raw)) {
-    }
-    // nothing will be signalled in this block when it goes: the releases come behind all products
-    for (int b = 0; b < kStages && ok; ++b) {
-      const int last = ring_last(slot, kStages, b);
-      if (last >= 0) ok = warp_wait(bar(EMPTY0 + b), ring_parity(last, kStages), abort_flag, err, 752);
+    Raw raw{}, then{};
+    begin();
+    load(raw);
+    while (more && turn(raw, then) && turn(then, raw)) {
     }
     __syncwarp();
   } else if (warp == kWarpMma) {
@@ -318,8 +307,14 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
       }
       base += 2 * n;
     }
+    // Nothing will be signalled in this block when it goes: the releases come behind all products.  (That a tile has been there says that the
+    // one before it in its place had been released: the phase waited for is the next one.)
+    for (int b = 0; b < kStages && ok; ++b) {
+      const int last = ring_last(base, kStages, b);
+      if (last >= 0) ok = warp_wait(bar(EMPTY0 + b), ring_parity(last, kStages), abort_flag, err, 752);
+    }
     __syncwarp();
-  } else {
+  } else if (warp < kWarpCodes) {
     // ====================================================================================================== softmax
     const int quad = warp & 3, team = warp >> 2, row = quad * 32 + lane;
     const uint32_t lane_base = ((uint32_t)(quad * 32)) << 16;
@@ -416,24 +411,16 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
           }
           tmem_wait_st();
         }
-        float s[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint32_t* us = reinterpret_cast<uint32_t*>(s);
-        {
-          float b[32];
-          uint32_t* ub = reinterpret_cast<uint32_t*>(b);
-          tmem_ld32(tS + 32, ub);
-          tmem_ld32(tS + 64, us);
-          tmem_wait_ld32(ub);
-          tmem_wait_ld32(us);
-          max_chunk(b, mx);
-          tmem_ld32(tS + 96, ub);
-          max_chunk(s, mx);
-          tmem_ld32(tS, us);
-          tmem_wait_ld32(ub);
-          tmem_wait_ld32(us);
-          max_chunk(b, mx);
-          max_chunk(s, mx);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t w[32];
+          tmem_ld32(tS + c, w);
+          tmem_wait_ld32(w);
+          max_chunk(reinterpret_cast<const float*>(w), mx);
         }
+        uint32_t us[16];
+        tmem_ld16_if(true, tS, us);
         const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.a.scale_log2;
         const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
         const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
@@ -442,16 +429,27 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         m = mn;
         const float nm = m == -INFINITY ? 0.f : -m;
         float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // P, packed, takes the place of scores that have been read: 16 columns for 32
+        // P, packed, takes the place of scores that have been read: 8 columns for 16
+        tmem_wait_ld16(us);
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float2 e[16];
-          uint32_t pk[16];
-          arg_chunk(s, P.a.scale_log2, nm, e);
-          tmem_ld32_if(c < 3, tS + 32 * c + 32, us);
-          exp_chunk<T, 5>(e, rs, pk);
-          tmem_st16(tS + 16 * c, pk);
-          tmem_wait_ld32(us);
+        for (int c = 0; c < 8; ++c) {
+          float2 e[8];
+          uint32_t pk[8];
+          const float2 sc2 = make_float2(P.a.scale_log2, P.a.scale_log2), nm2 = make_float2(nm, nm);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            e[k] = ffma2(__uint_as_float(us[2 * k]), __uint_as_float(us[2 * k + 1]), sc2, nm2);
+            asm volatile("" : "+f"(e[k].x), "+f"(e[k].y));
+          }
+          tmem_ld16_if(c < 7, tS + 16 * c + 16, us);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float2 p = k == 7 ? ex2_poly2<5>(e[k]) : make_float2(ex2_approx(e[k].x), ex2_approx(e[k].y));
+            rs[k & 3] = fadd2(rs[k & 3], p);
+            pk[k] = mma::pack2<T>(p.x, p.y);
+          }
+          tmem_st8(tS + 8 * c, pk);
+          tmem_wait_ld16(us);
         }
         const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
         const float sum = r.x + r.y;
@@ -511,34 +509,31 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
         mine *= inv, theirs *= inv;
 #pragma unroll 1
-        for (int c = merge ? team * (kDim / 2) : 0; c < (merge && team == 0 ? kDim / 2 : kDim); c += 32) {
-          uint32_t o[32];
+        for (int c = merge ? team * (kDim / 2) : 0; c < (merge && team == 0 ? kDim / 2 : kDim); c += 16) {
+          uint32_t o[16];
           float* f = reinterpret_cast<float*>(o);
-          tmem_ld32(tO + c, o);
-          tmem_wait_ld32(o);
+          tmem_ld16_if(true, tO + c, o);
+          tmem_wait_ld16(o);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) f[k] *= mine;
+          for (int k = 0; k < 16; ++k) f[k] *= mine;
           if (merge) {
-            uint32_t z[32];
-            tmem_ld32(tmem + 256 + (team ^ 1) * 128 + lane_base + c, z);
-            tmem_wait_ld32(z);
+            uint32_t z[16];
+            tmem_ld16_if(true, tmem + 256 + (team ^ 1) * 128 + lane_base + c, z);
+            tmem_wait_ld16(z);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) f[k] = fmaf(__uint_as_float(z[k]), theirs, f[k]);
+            for (int k = 0; k < 16; ++k) f[k] = fmaf(__uint_as_float(z[k]), theirs, f[k]);
           }
           if (now.in && now.slot_row >= 0) {
             // partial rows lie in blocks of 32, four columns of all of them side by side: every store is one stretch
             float4* to = reinterpret_cast<float4*>(P.a.part_o + now.part) + (c / 4) * 32 + lane;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) to[k * 32] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            for (int k = 0; k < 4; ++k) to[k * 32] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
           } else if (now.in) {
             uint4* to = reinterpret_cast<uint4*>(P.a.out + (now.out * kDim + c) * 2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = mma::pack2<T>(f[8 * k + 2 * e], f[8 * k + 2 * e + 1]);
-              to[k] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int k = 0; k < 2; ++k)
+              to[k] = make_uint4(mma::pack2<T>(f[8 * k], f[8 * k + 1]), mma::pack2<T>(f[8 * k + 2], f[8 * k + 3]), mma::pack2<T>(f[8 * k + 4], f[8 * k + 5]),
+                                 mma::pack2<T>(f[8 * k + 6], f[8 * k + 7]));
           }
           __syncwarp();
         }
