@@ -639,6 +639,19 @@ int many_units(const infllm_packed* c, const infllm_packed_seq* seqs, PackedTcPa
   return INFLLM_OK;
 }
 
+// Bytes of the image of a launch's tiles, 0 where numbers are taken out of their codes by the blocks themselves: with an image a tile of 256
+// rows takes 1.8 us instead of 2.4, and to make one takes 0.013 us a tile of the machine's time; so it pays from about four blocks of rows
+// to a tile on.  Not beyond a gigabyte, as a cache in 4 bits is there for want of memory.
+int64_t image_bytes(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group) {
+  int64_t tiles = 0, blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    const int64_t t = seqs[i].count > 0 ? ceil_div(seqs[i].length, kKeyTile) : 0;
+    tiles += t, blocks += t * ceil_div((int64_t)seqs[i].count * group, kBlockRows);
+  }
+  const int64_t bytes = tiles * c->n_kv_heads * 2 * kKeyTile * c->head_dim * 2;
+  return blocks >= 4 * tiles && bytes <= 1 << 30 ? bytes : 0;
+}
+
 // the units of the attention of seqs[0 .. n - 1] for many rows
 int lay_out_many(const infllm_packed* c, const infllm_packed_seq* seqs, int n_sm, PackedTcParams& P, bool* join) {
   const int group = P.a.group;
@@ -671,8 +684,11 @@ int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, i
   *bytes = 0;
   if (n == 0 || most == 0) return INFLLM_OK;
   const int n_sm = sm_count(c->device);
-  if (many_rows(seqs, n, n_heads / c->n_kv_heads)) {
-    *bytes = (int64_t)2 * n_sm * kBlockRows * (c->head_dim + 1) * 4 + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
+  const int group = n_heads / c->n_kv_heads;
+  if (many_rows(seqs, n, group)) {
+    int64_t image = 0;
+    for (int b0 = 0; b0 < n; b0 += kAttnSeqs) image = std::max(image, image_bytes(c, seqs + b0, std::min(n - b0, kAttnSeqs), group));
+    *bytes = image + (int64_t)2 * n_sm * kBlockRows * (c->head_dim + 1) * 4 + (weigh > 0 ? (int64_t)n * most * n_heads * 4 : 0);
     return INFLLM_OK;
   }
   int64_t units = 0;
@@ -700,8 +716,15 @@ int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_
 }
 
 template <typename T, int kDim>
-int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, int n_sm, bool join, cudaStream_t s) {
+int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, char* work, int n_sm, bool join, cudaStream_t s) {
+  const int64_t image = image_bytes(c, seqs, P.a.batch, P.a.group);
   INFLLM_TRY(lay_out_many(c, seqs, n_sm, P, &join));
+  P.image = image > 0 ? work : nullptr, P.n_image = 0;
+  for (int i = 0; image > 0 && i < P.a.batch; ++i) {
+    P.a.seq[i].keys = P.n_image;
+    if (seqs[i].count > 0) P.n_image += c->n_kv_heads * (int)ceil_div(seqs[i].length, kKeyTile);
+  }
+  P.a.part_o = (float*)(work + image);
   INFLLM_TRY(tc_get_error_ptr(&P.a.err));
   P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
   if (P.n_ctas > 0) INFLLM_TRY(packed_tc_launch(P, c->dtype, kDim, s));
@@ -764,7 +787,7 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
         empty = empty || mine[i].count < most;
       }
       INFLLM_DISPATCH_DTYPE(c->dtype, T, {
-        if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, n_sm, empty, s) : attend_many<T, 64>(Tc, mine, c, n_sm, empty, s)));
+        if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, (char*)d_work, n_sm, empty, s) : attend_many<T, 64>(Tc, mine, c, (char*)d_work, n_sm, empty, s)));
         else INFLLM_TRY((c->head_dim == 128 ? attend_few<T, 128>(P, mine, c, n_sm, empty, s) : attend_few<T, 64>(P, mine, c, n_sm, empty, s)));
         if (weigh > 0 && any && many) {
           bool cut = false;

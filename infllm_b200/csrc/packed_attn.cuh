@@ -12,7 +12,7 @@ struct PackedAttnSeq {
   int32_t slot, length, count;
   int32_t unit0;   // its first unit of work, and how they follow from there:
   int32_t chunks;  // few rows: unit0 + stretch of `keys` keys
-  int32_t keys;    // many: unit0 + KV head * chunks + block of 256 rows
+  int32_t keys;    // many: unit0 + KV head * chunks + block of 256 rows; its first tile of the image
 };
 
 struct PackedAttnParams {
@@ -37,7 +37,8 @@ struct PackedAttnParams {
 // has those from start[c] to start[c + 1], as (unit, tile).
 struct PackedTcParams {
   PackedAttnParams a;
-  int32_t n_ctas, pad;
+  int32_t n_ctas, n_image;
+  char* image;  // prompts: n_image tiles, keys and values, as 16-bit numbers (packed_tc.cu); null: none
   int2 start[kMaxSms + 1];
 };
 

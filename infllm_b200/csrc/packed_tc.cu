@@ -1,15 +1,16 @@
-// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that sixteen warps
+// Attention over the cache in 4 bits for many rows (packed_attn.cu has the formulas): tcgen05 products of numbers that six warps
 // take out of their codes, S and O in TMEM.
 //
 // A unit is up to 256 rows of one KV head by a stretch of keys.  Two teams of four softmax warps, a thread per row, have 128 rows each;
 // of up to 128 rows both have all, and take the key tiles in turn: each with a maximum, a sum and an O of its own, which are put
 // together at the unit's end, where a thread reads the other team's O of its row from TMEM.  (A tile is in a team's hands for 1.1 us:
 // with one team that, not its bytes, would be a tile's time.)
-// Sixteen more warps bring codes from global memory through registers, and leave 16-bit numbers, swizzled as the products
-// want them, in a ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is taken out once
-// for 256 rows.  Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A operand of P V from
-// there, have 128 columns, O another 128.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only
-// then O is scaled.
+// Six more warps bring codes from global memory through registers, and leave 16-bit numbers, swizzled as the products want them, in a
+// ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is taken out once for 256 rows.
+// (Eight warps, with softmax in pieces of 16 columns to do with 96 registers: of 48 rows 4 % less, of 192 rows 8 % more.)  Prompts'
+// tiles, which many blocks of rows read, are taken out once for all of them by a kernel before, and fetched by one warp.
+// Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A operand of P V from there, have 128
+// columns, O another 128.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
 // P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.
 // Sums, O and partial rows are fp32.
 #include <atomic>
@@ -24,8 +25,11 @@ namespace infllm {
 
 namespace xtc {
 constexpr int kStages = 5;
-constexpr int kWarpCodes = 8, kCodeWarps = 8, kWarpMma = kWarpCodes + kCodeWarps;  // half of them keys, half values
-constexpr int kThreads = (kWarpMma + 1) * 32;
+// Warps: eight of softmax; six that take numbers out of their codes (half of them keys, half values), or one that fetches tiles that are
+// there already (kImage); one that issues products.  Sixteen or fewer, so that a thread has 128 registers.
+constexpr int kWarpCodes = 8, kCodeWarps = 6;
+constexpr int makers(bool image) { return image ? 1 : kCodeWarps; }
+constexpr int threads(bool image) { return (kWarpCodes + makers(image) + 1) * 32; }
 enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, Q_FULL0 = EMPTY0 + kStages, S_FULL0 = Q_FULL0 + 2, P_FULL0 = S_FULL0 + 2, PV_DONE0 = P_FULL0 + 2, MERGE = PV_DONE0 + 2, N_BARS };
 template <int kDim>
 struct Smem {
@@ -68,30 +72,11 @@ struct Pieces {  // a block's, in turn
 };
 }  // namespace xtc
 
-// (16 columns at a time: the softmax warps are to do with 96 registers a thread, so that there is room for more warps)
-__device__ __forceinline__ void tmem_ld16_if(bool yes, uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %17, 0;\n\t"
-      "@p tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t}"
-      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-      : "r"(taddr), "r"((uint32_t)yes)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               ::"memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
-
-template <typename T, int kDim>
-__global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __grid_constant__ PackedTcParams P) {
+template <typename T, int kDim, bool kImage>
+__global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(const __grid_constant__ PackedTcParams P) {
   using namespace xtc;
   using L = Smem<kDim>;
+  constexpr int kWarpMma = kWarpCodes + makers(kImage);
   extern __shared__ __align__(1024) unsigned char smem[];  // (swizzled tiles begin on 1024 bytes, and no byte is left to shift them by)
   const uint32_t s_base = smem_u32(smem), sQ = s_base + L::kQ, sRing = s_base + L::kRing, bars = s_base + L::kBar;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + N_BARS * 8);
@@ -107,7 +92,7 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
   if (warp == 0) {
     static_assert(N_BARS <= 32 && N_BARS * 8 + 16 <= 256, "");
     // tiles: the warps that make them; queries and probabilities: a team's four; what the teams have of the same rows: both
-    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 ? (uint32_t)kCodeWarps / 2 : lane == Q_FULL0 || lane == Q_FULL0 + 1 || lane == P_FULL0 || lane == P_FULL0 + 1 ? 4u : lane == MERGE ? 8u : 1u);
+    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 ? (kImage ? 1u : kCodeWarps / 2u) : lane == Q_FULL0 || lane == Q_FULL0 + 1 || lane == P_FULL0 || lane == P_FULL0 + 1 ? 4u : lane == MERGE ? 8u : 1u);
     if (lane == 0) *abort_flag = 0;
     mbar_fence_init();
   }
@@ -123,7 +108,34 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
   constexpr uint32_t idesc_qk = make_idesc(kBf16, 128, 128, false), idesc_pv = make_idesc(kBf16, 128, kDim, true);
   chain_enter();
 
-  if (warp >= kWarpCodes && warp < kWarpMma) {
+  if (kImage && warp == kWarpCodes) {
+    // ========================================================================================================== tiles
+    const bool lead = elect_one();
+    Pieces pieces(P);
+    Piece U;
+    bool ok = true;
+    int base = 0;
+    while (ok && pieces.next(P, U)) {
+      const PackedAttnSeq& S = P.a.seq[U.b];
+      const char* from = P.image + ((int64_t)S.keys + (int64_t)U.hkv * ((S.length + kKeyTile - 1) / kKeyTile) + U.tile0) * (2 * L::kTileBytes);
+      for (int p = 0; p < 2 * U.n && ok; ++p) {
+        const int b = (base + p) % kStages;
+        if (base + p >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(base + p - kStages, kStages), abort_flag, err, 751);
+        if (ok && lead) {
+          mbar_expect_tx(bar(FULL0 + b), L::kTileBytes);
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(sRing + b * L::kTileBytes), "l"(from + (int64_t)(2 * tile_at(p, U.n) + is_value(p, U.n)) * L::kTileBytes), "r"((uint32_t)L::kTileBytes), "r"(bar(FULL0 + b))
+                       : "memory");
+        }
+        __syncwarp();
+      }
+      if (ok) base += 2 * U.n;
+    }
+    if (!ok && lane == 0) {  // given up: loads on their way get a bounded chance to land
+      for (uint32_t w = 0; w < 4096; ++w) __nanosleep(64);
+    }
+    __syncwarp();
+  } else if (!kImage && warp >= kWarpCodes && warp < kWarpMma) {
     // ======================================================================================================== numbers
     // Eight warps take key tiles, eight value tiles.  A thread has the 32 numbers of one (m, s), a 16-byte piece of a row of codes, of
     // kPer rows; the next tile's are on their way through registers while it is at work, those kAhead tiles ahead to L2.
@@ -411,16 +423,24 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
           }
           tmem_wait_st();
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t w[32];
-          tmem_ld32(tS + c, w);
-          tmem_wait_ld32(w);
-          max_chunk(reinterpret_cast<const float*>(w), mx);
+        float s[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t* us = reinterpret_cast<uint32_t*>(s);
+        {
+          float b[32];
+          uint32_t* ub = reinterpret_cast<uint32_t*>(b);
+          tmem_ld32(tS + 32, ub);
+          tmem_ld32(tS + 64, us);
+          tmem_wait_ld32(ub);
+          tmem_wait_ld32(us);
+          max_chunk(b, mx);
+          tmem_ld32(tS + 96, ub);
+          max_chunk(s, mx);
+          tmem_ld32(tS, us);
+          tmem_wait_ld32(ub);
+          tmem_wait_ld32(us);
+          max_chunk(b, mx);
+          max_chunk(s, mx);
         }
-        uint32_t us[16];
-        tmem_ld16_if(true, tS, us);
         const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.a.scale_log2;
         const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
         const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
@@ -429,27 +449,16 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         m = mn;
         const float nm = m == -INFINITY ? 0.f : -m;
         float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // P, packed, takes the place of scores that have been read: 8 columns for 16
-        tmem_wait_ld16(us);
+        // P, packed, takes the place of scores that have been read: 16 columns for 32
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          float2 e[8];
-          uint32_t pk[8];
-          const float2 sc2 = make_float2(P.a.scale_log2, P.a.scale_log2), nm2 = make_float2(nm, nm);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            e[k] = ffma2(__uint_as_float(us[2 * k]), __uint_as_float(us[2 * k + 1]), sc2, nm2);
-            asm volatile("" : "+f"(e[k].x), "+f"(e[k].y));
-          }
-          tmem_ld16_if(c < 7, tS + 16 * c + 16, us);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float2 p = k == 7 ? ex2_poly2<5>(e[k]) : make_float2(ex2_approx(e[k].x), ex2_approx(e[k].y));
-            rs[k & 3] = fadd2(rs[k & 3], p);
-            pk[k] = mma::pack2<T>(p.x, p.y);
-          }
-          tmem_st8(tS + 8 * c, pk);
-          tmem_wait_ld16(us);
+        for (int c = 0; c < 4; ++c) {
+          float2 e[16];
+          uint32_t pk[16];
+          arg_chunk(s, P.a.scale_log2, nm, e);
+          tmem_ld32_if(c < 3, tS + 32 * c + 32, us);
+          exp_chunk<T, 5>(e, rs, pk);
+          tmem_st16(tS + 16 * c, pk);
+          tmem_wait_ld32(us);
         }
         const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
         const float sum = r.x + r.y;
@@ -509,31 +518,34 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
         const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
         mine *= inv, theirs *= inv;
 #pragma unroll 1
-        for (int c = merge ? team * (kDim / 2) : 0; c < (merge && team == 0 ? kDim / 2 : kDim); c += 16) {
-          uint32_t o[16];
+        for (int c = merge ? team * (kDim / 2) : 0; c < (merge && team == 0 ? kDim / 2 : kDim); c += 32) {
+          uint32_t o[32];
           float* f = reinterpret_cast<float*>(o);
-          tmem_ld16_if(true, tO + c, o);
-          tmem_wait_ld16(o);
+          tmem_ld32(tO + c, o);
+          tmem_wait_ld32(o);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) f[k] *= mine;
+          for (int k = 0; k < 32; ++k) f[k] *= mine;
           if (merge) {
-            uint32_t z[16];
-            tmem_ld16_if(true, tmem + 256 + (team ^ 1) * 128 + lane_base + c, z);
-            tmem_wait_ld16(z);
+            uint32_t z[32];
+            tmem_ld32(tmem + 256 + (team ^ 1) * 128 + lane_base + c, z);
+            tmem_wait_ld32(z);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) f[k] = fmaf(__uint_as_float(z[k]), theirs, f[k]);
+            for (int k = 0; k < 32; ++k) f[k] = fmaf(__uint_as_float(z[k]), theirs, f[k]);
           }
           if (now.in && now.slot_row >= 0) {
             // partial rows lie in blocks of 32, four columns of all of them side by side: every store is one stretch
             float4* to = reinterpret_cast<float4*>(P.a.part_o + now.part) + (c / 4) * 32 + lane;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) to[k * 32] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            for (int k = 0; k < 8; ++k) to[k * 32] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
           } else if (now.in) {
             uint4* to = reinterpret_cast<uint4*>(P.a.out + (now.out * kDim + c) * 2);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-              to[k] = make_uint4(mma::pack2<T>(f[8 * k], f[8 * k + 1]), mma::pack2<T>(f[8 * k + 2], f[8 * k + 3]), mma::pack2<T>(f[8 * k + 4], f[8 * k + 5]),
-                                 mma::pack2<T>(f[8 * k + 6], f[8 * k + 7]));
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = mma::pack2<T>(f[8 * k + 2 * e], f[8 * k + 2 * e + 1]);
+              to[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
           __syncwarp();
         }
@@ -564,22 +576,89 @@ __global__ void __launch_bounds__(xtc::kThreads, 1) packed_tc_kernel(const __gri
   if (warp == kWarpMma) tmem_dealloc(tmem, 512);
 }
 
-int packed_tc_launch(const PackedTcParams& P, int dtype, int head_dim, cudaStream_t s) {
-  INFLLM_DISPATCH_DTYPE(dtype, T, {
-    auto kern = head_dim == 128 ? packed_tc_kernel<T, 128> : packed_tc_kernel<T, 64>;
-    const int smem = (head_dim == 128 ? xtc::Smem<128>::kTotal : xtc::Smem<64>::kTotal);
-    static std::atomic<uint64_t> set[2];  // devices that know it, per head_dim (and, by the dispatch, type)
-    int dev = 0;
-    INFLLM_CUDA_OK(cudaGetDevice(&dev));
-    std::atomic<uint64_t>& there = set[head_dim == 128];
-    if (dev >= 64 || !(there.load(std::memory_order_relaxed) >> dev & 1)) {
-      INFLLM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      if (dev < 64) there.fetch_or(1ull << dev);
+// The numbers of all tiles of a launch's sequences, each as a block of the kernel above wants it in its shared memory: for prompts, whose
+// tiles many blocks read (2048 tokens behind 28000: 32 blocks of rows).  A tile of keys or of values a block: out of its codes in shared
+// memory, and from there in one piece.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(256) packed_image_kernel(const __grid_constant__ PackedTcParams P) {
+  using L = xtc::Smem<kDim>;
+  using C = Codes<T>;
+  constexpr int kGroups = kDim / 32, kPer = 128 * kGroups / 256;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  int lo = 0, hi = P.a.batch - 1;
+  const int tile = blockIdx.x;
+  while (lo < hi) {  // (the sequence's first tile is in `keys`)
+    const int mid = (lo + hi + 1) / 2;
+    if (P.a.seq[mid].keys <= tile) lo = mid;
+    else hi = mid - 1;
+  }
+  const PackedAttnSeq S = P.a.seq[lo];
+  const int tiles = (S.length + kKeyTile - 1) / kKeyTile, hkv = (tile - S.keys) / tiles, j0 = (tile - S.keys) % tiles * kKeyTile;
+  const bool mixed = j0 + kKeyTile > keys_of_row(S, P.a.group, 0);
+  chain_enter();
+  for (int value = 0; value < 2; ++value) {
+    const int64_t row = P.a.at.row0(S.slot, hkv) + j0;
+    const char* codes = P.a.at.codes + (value ? P.a.at.codes_v : 0) + row * (kDim / 2);
+    const char* scales = P.a.at.scales + row * (kDim / 8);
+    uint4 c[kPer];
+    uint32_t ms[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      const int at = threadIdx.x + x * 256, k = at / kGroups, t = at % kGroups;
+      c[x] = make_uint4(0, 0, 0, 0), ms[x] = 0;
+      if (j0 + k < S.length) {
+        c[x] = __ldg(reinterpret_cast<const uint4*>(codes + k * (kDim / 2) + t * 16));
+        ms[x] = __ldg(reinterpret_cast<const uint32_t*>(scales + (value ? P.a.at.scales_v : 0) + k * (kDim / 8) + t * 4));
+        if (mixed && value && C::odd(ms[x])) ms[x] = 0;  // (as the warps that do this without an image)
+        if (mixed && !value)
+          for (int g = 0; g < kGroups; ++g)
+            if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + P.a.at.scales_v + k * (kDim / 8) + g * 4)))) ms[x] = 0x7fff7fffu;
+      }
     }
-    INFLLM_CUDA_OK(launch_chained(kern, dim3(P.n_ctas), dim3(xtc::kThreads), smem, s, P));
-  });
+    if (value) {
+      if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // (the keys have been read from where the values go)
+      __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      const int at = threadIdx.x + x * 256, k = at / kGroups, t = at % kGroups;
+      put_group<T>(smem + (t >> 1) * kSubTileBytes, k, t, c[x], ms[x]);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(P.image + ((int64_t)2 * tile + value) * L::kTileBytes), "r"(smem_u32(smem)), "r"((uint32_t)L::kTileBytes) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+  if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+template <typename T, int kDim, bool kImage>
+static int tc_launch(const PackedTcParams& P, cudaStream_t s) {
+  auto kern = packed_tc_kernel<T, kDim, kImage>;
+  const int smem = xtc::Smem<kDim>::kTotal;
+  static std::atomic<uint64_t> set;  // devices that know it
+  int dev = 0;
+  INFLLM_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
+    INFLLM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) set.fetch_or(1ull << dev);
+  }
+  if (kImage) {
+    INFLLM_CUDA_OK(launch_chained(packed_image_kernel<T, kDim>, dim3(P.n_image), dim3(256), xtc::Smem<kDim>::kTileBytes, s, P));
+    INFLLM_LAUNCH_OK("packed_image_kernel");
+  }
+  INFLLM_CUDA_OK(launch_chained(kern, dim3(P.n_ctas), dim3(xtc::threads(kImage)), smem, s, P));
   INFLLM_LAUNCH_OK("packed_tc_kernel");
   return INFLLM_OK;
+}
+
+int packed_tc_launch(const PackedTcParams& P, int dtype, int head_dim, cudaStream_t s) {
+  INFLLM_DISPATCH_DTYPE(dtype, T, {
+    if (P.image) return head_dim == 128 ? tc_launch<T, 128, true>(P, s) : tc_launch<T, 64, true>(P, s);
+    return head_dim == 128 ? tc_launch<T, 128, false>(P, s) : tc_launch<T, 64, false>(P, s);
+  });
 }
 
 }  // namespace infllm
