@@ -348,18 +348,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
 }
 
 // ----------------------------------------------------------------------------------------------------------- the join
-// kWarps warps per query head and token share a row's parts, four of them on their way at once; rows without a token become zeros.
-template <bool kTc>
-struct JoinParams {
-  using type = PackedAttnParams;
-  static __device__ __forceinline__ const PackedAttnParams& attn(const type& p) { return p; }
-};
-template <>
-struct JoinParams<true> {
-  using type = PackedTcParams;
-  static __device__ __forceinline__ const PackedAttnParams& attn(const type& p) { return p.a; }
-};
-
 // The weights of four keys a thread from the scores that the kernel of few rows has left, 1024 keys of a KV head a block.
 constexpr int kSumKeys = 1024;
 __device__ __forceinline__ void sum_weights(const PackedAttnParams& P, int block) {
@@ -397,87 +385,54 @@ __device__ __forceinline__ void sum_weights(const PackedAttnParams& P, int block
   }
 }
 
-template <typename T, int kDim, int kWarps, bool kTc>
-__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ typename JoinParams<kTc>::type All) {
-  constexpr int kPer = kDim / 32, kRows = 8 / kWarps, kAhead = 4;
+// A row's parts, by kWarps warps that share them, four on their way at once: sum, maximum and kDim / 32 numbers a lane, in the first
+// of the warps (false in the others).  row_of(part): its row in part_lse and part_o.
+template <int kDim, int kWarps, bool kTc, typename F>
+__device__ __forceinline__ bool join_row(const PackedAttnParams& P, int parts, F&& row_of, float& m, float& l, float (&acc)[kDim / 32]) {
+  constexpr int kPer = kDim / 32, kAhead = 4;
   __shared__ float sm[8][kDim + 4];
-  const PackedAttnParams& P = JoinParams<kTc>::attn(All);
-  if (!kTc && (int)blockIdx.x >= P.join_blocks) {
-    sum_weights(P, blockIdx.x - P.join_blocks);
-    return;
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = P.at.n_kv * P.group;
-  const int64_t at = (int64_t)blockIdx.x * kRows + warp / kWarps;
-  const bool in = at < (int64_t)P.batch * P.most * heads;
-  const int h = in ? (int)(at % heads) : 0, i = in ? (int)(at / heads % P.most) : 0, b = in ? (int)(at / heads / P.most) : 0, hkv = h / P.group;
-  const PackedAttnSeq S = P.seq[b];
-  const int tok = i - (P.most - S.count), r = tok * P.group + h % P.group;
-  int parts = 0, block0 = 0, unit = 0;
-  bool whole = false;
-  if (in && tok >= 0) {
-    if constexpr (kTc) {
-      const int block = r / kBlockRows;
-      unit = S.unit0 + hkv * S.chunks + block;
-      block0 = block_of(All, unit, 0);
-      parts = block_of(All, unit, tiles_of(S, P.group, block) - 1) - block0 + 1;
-    } else {
-      parts = S.chunks;
-    }
-    whole = parts == 1;  // written by the unit that had all of it
-  }
-  auto row_of = [&](int c) -> int64_t {
-    if constexpr (kTc) {
-      // a block's first unit has its first slot, its last one the second
-      const int2 s = All.start[block0 + c];
-      return (int64_t)(2 * (block0 + c) + (s.x < unit)) * kBlockRows + r % kBlockRows;
-    } else {
-      return ((int64_t)(S.unit0 + c) * P.at.n_kv + hkv) * kFewRows + r;
-    }
-  };
-  chain_enter();
-  float m = -INFINITY, l = 0.f, acc[kPer];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  if (!whole) {
-    for (int c0 = warp % kWarps; c0 < parts; c0 += kWarps * kAhead) {
-      float lse[kAhead], v[kAhead][kPer];
+  for (int c0 = warp % kWarps; c0 < parts; c0 += kWarps * kAhead) {
+    float lse[kAhead], v[kAhead][kPer];
 #pragma unroll
-      for (int e = 0; e < kAhead; ++e) {
-        const int c = c0 + e * kWarps;
-        lse[e] = -INFINITY;
-        if (c >= parts) continue;
-        const int64_t row = row_of(c);
-        lse[e] = P.part_lse[row];
-        // (partial rows of the tensor-core kernel lie in blocks of 32, four columns of all of them side by side)
-        const float* o = P.part_o + (kTc ? (row & ~(int64_t)31) * kDim + (lane * kPer / 4) * 128 + (row & 31) * 4 + lane * kPer % 4 : row * kDim + lane * kPer);
-        if (kPer == 4) *reinterpret_cast<float4*>(v[e]) = *reinterpret_cast<const float4*>(o);
-        else *reinterpret_cast<float2*>(v[e]) = *reinterpret_cast<const float2*>(o);
-      }
-      float mx = m;
-#pragma unroll
-      for (int e = 0; e < kAhead; ++e) mx = fmaxf(mx, lse[e]);
-      const float ref = mx == -INFINITY ? 0.f : mx;  // (a part that is no number is not seen by the maximum)
-      const float a = exp2f(m - ref);
-      l *= a;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[k] *= a;
-#pragma unroll
-      for (int e = 0; e < kAhead; ++e) {
-        if (lse[e] == -INFINITY) continue;
-        const float w = exp2f(lse[e] - ref);
-        l += w;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(w, v[e][k], acc[k]);
-      }
-      m = mx;
+    for (int e = 0; e < kAhead; ++e) {
+      const int c = c0 + e * kWarps;
+      lse[e] = -INFINITY;
+      if (c >= parts) continue;
+      const int64_t row = row_of(c);
+      lse[e] = P.part_lse[row];
+      // (partial rows of the tensor-core kernel lie in blocks of 32, four columns of all of them side by side)
+      const float* o = P.part_o + (kTc ? (row & ~(int64_t)31) * kDim + (lane * kPer / 4) * 128 + (row & 31) * 4 + lane * kPer % 4 : row * kDim + lane * kPer);
+      if (kPer == 4) *reinterpret_cast<float4*>(v[e]) = *reinterpret_cast<const float4*>(o);
+      else *reinterpret_cast<float2*>(v[e]) = *reinterpret_cast<const float2*>(o);
     }
+    float mx = m;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) mx = fmaxf(mx, lse[e]);
+    const float ref = mx == -INFINITY ? 0.f : mx;  // (a part that is no number is not seen by the maximum)
+    const float a = exp2f(m - ref);
+    l *= a;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) acc[k] *= a;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (lse[e] == -INFINITY) continue;
+      const float w = exp2f(lse[e] - ref);
+      l += w;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] = fmaf(w, v[e][k], acc[k]);
+    }
+    m = mx;
   }
   if (kWarps > 1) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) sm[warp][lane * kPer + k] = acc[k];
     if (lane == 0) sm[warp][kDim] = m, sm[warp][kDim + 1] = l;
     __syncthreads();
-    if (warp % kWarps) return;
+    if (warp % kWarps) return false;
     float mx = m;
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm[warp + w][kDim]);
@@ -494,30 +449,83 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
     }
     m = mx;
   }
-  if (!in || whole) return;
-  const int64_t orow = ((int64_t)(P.b0 + b) * P.most + i) * heads + h;
+  return true;
+}
+
+// a joined row: token i (of the tensors) of query head h of the launch's sequence b; its log-sum-exp to base 2
+template <typename T, int kDim>
+__device__ __forceinline__ float write_row(const PackedAttnParams& P, int b, int i, int h, float m, float l, const float (&acc)[kDim / 32]) {
+  constexpr int kPer = kDim / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t orow = ((int64_t)(P.b0 + b) * P.most + i) * (P.at.n_kv * P.group) + h;
   const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
   uint32_t* to = reinterpret_cast<uint32_t*>(P.out + (orow * kDim + lane * kPer) * 2);
 #pragma unroll
   for (int k = 0; k < kPer; k += 2) to[k / 2] = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
   const float lse = l > 0.f ? m + log2f(l) : l == 0.f ? -INFINITY : l;
   if (lane == 0 && P.lse) P.lse[orow] = lse * (1.f / kLog2e);
-  if (lane == 0 && P.row_lse && tok >= 0) P.row_lse[((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group + r] = lse;
+  return lse;
 }
 
-template <typename T, int kDim, bool kTc>
-static int join_launch(typename JoinParams<kTc>::type& P, PackedAttnParams& A, bool join, int n_sm, cudaStream_t s) {
-  // as many warps to a row as one wave has room for
-  const int64_t rows = (int64_t)A.batch * A.most * A.at.n_kv * A.group, warps = n_sm * 32 / std::max<int64_t>(rows, 1);
-  auto launch = [&](auto kern, int per_row) {
-    A.join_blocks = join ? (int)ceil_div(rows * per_row, 8) : 0;
-    const int64_t sums = A.logits ? (int64_t)A.batch * A.at.n_kv * (A.pitch / kSumKeys) : 0;
-    return launch_chained(kern, dim3((unsigned)(A.join_blocks + sums)), dim3(256), 0, s, P);
-  };
-  if (warps >= 8) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 8, kTc>, 8));
-  else if (warps >= 4) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 4, kTc>, 4));
-  else if (warps >= 2) INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 2, kTc>, 2));
-  else INFLLM_CUDA_OK(launch(packed_join_kernel<T, kDim, 1, kTc>, 1));
+// few rows: all of a launch's rows, those without a token as zeros
+template <typename T, int kDim, int kWarps>
+__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ PackedAttnParams P) {
+  if ((int)blockIdx.x >= P.join_blocks) {
+    sum_weights(P, blockIdx.x - P.join_blocks);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, heads = P.at.n_kv * P.group;
+  const int64_t at = (int64_t)blockIdx.x * (8 / kWarps) + warp / kWarps;
+  const bool in = at < (int64_t)P.batch * P.most * heads;
+  const int h = in ? (int)(at % heads) : 0, i = in ? (int)(at / heads % P.most) : 0, b = in ? (int)(at / heads / P.most) : 0, hkv = h / P.group;
+  const PackedAttnSeq S = P.seq[b];
+  const int tok = i - (P.most - S.count), r = tok * P.group + h % P.group;
+  const bool whole = tok >= 0 && S.chunks == 1;  // written by the unit that had all of it
+  chain_enter();
+  float m, l, acc[kDim / 32];
+  const bool mine = join_row<kDim, kWarps, false>(P, in && tok >= 0 && !whole ? S.chunks : 0, [&](int c) -> int64_t { return ((int64_t)(S.unit0 + c) * P.at.n_kv + hkv) * kFewRows + r; }, m, l, acc);
+  if (mine && in && !whole) write_row<T, kDim>(P, b, i, h, m, l, acc);
+}
+
+// many rows: those of the units that were cut, a block of the grid's second dimension for each block in which a unit begins that ends in another one
+template <typename T, int kDim, int kWarps>
+__global__ void __launch_bounds__(256) packed_join_cut_kernel(const __grid_constant__ PackedTcParams All) {
+  const PackedAttnParams& P = All.a;
+  const int first = blockIdx.y, warp = threadIdx.x >> 5;
+  const int2 begin = All.start[first], end = All.start[first + 1];
+  chain_enter();
+  // the unit that the block's stretch ends in, if the stretch has its first tile and not its last
+  if (end.y == 0 || (begin.x == end.x && begin.y > 0)) return;
+  const int unit = end.x, b = seq_of(P, unit);
+  const PackedAttnSeq S = P.seq[b];
+  const int hkv = (unit - S.unit0) / S.chunks, block = (unit - S.unit0) % S.chunks, in_block = blockIdx.x * (8 / kWarps) + warp / kWarps;
+  const int r = block * kBlockRows + in_block, parts = block_of(All, unit, tiles_of(S, P.group, block) - 1) - first + 1;
+  const bool in = r < S.count * P.group;
+  // a block's first unit has its first slot, its last one the second
+  float m, l, acc[kDim / 32];
+  const bool mine = join_row<kDim, kWarps, true>(P, in ? parts : 0, [&](int c) -> int64_t { return (int64_t)(2 * (first + c) + (All.start[first + c].x < unit)) * kBlockRows + in_block; }, m, l, acc);
+  if (!mine || !in) return;
+  const int tok = r / P.group;
+  const float lse = write_row<T, kDim>(P, b, P.most - S.count + tok, hkv * P.group + r - tok * P.group, m, l, acc);
+  if ((threadIdx.x & 31) == 0 && P.row_lse) P.row_lse[((int64_t)(P.b0 + b) * P.at.n_kv + hkv) * P.most * P.group + r] = lse;
+}
+
+// rows of tokens that are none, where sequences have fewer than the tensors: a warp a row
+template <typename T, int kDim>
+__global__ void __launch_bounds__(256) packed_empty_kernel(const __grid_constant__ PackedAttnParams P) {
+  const int heads = P.at.n_kv * P.group, b = blockIdx.y;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  chain_enter();
+  if (at >= (int64_t)(P.most - P.seq[b].count) * heads) return;
+  const float none[kDim / 32] = {};
+  write_row<T, kDim>(P, b, (int)(at / heads), (int)(at % heads), -INFINITY, 0.f, none);
+}
+
+// as many warps to a row as one wave has room for
+template <typename F>
+static int by_warps(int64_t rows, int n_sm, F&& launch) {
+  const int64_t warps = n_sm * 32 / std::max<int64_t>(rows, 1);
+  INFLLM_CUDA_OK(warps >= 8 ? launch(std::integral_constant<int, 8>()) : warps >= 2 ? launch(std::integral_constant<int, 2>()) : launch(std::integral_constant<int, 1>()));
   INFLLM_LAUNCH_OK("packed_join_kernel");
   return INFLLM_OK;
 }
@@ -700,6 +708,8 @@ int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, i
   return INFLLM_OK;
 }
 
+int n_heads_of(const PackedAttnParams& P) { return P.at.n_kv * P.group; }
+
 template <typename T, int kDim>
 int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, int n_sm, bool join, cudaStream_t s) {
   const int64_t units = lay_out_few(c, seqs, P.batch, n_sm, P.seq, &join);
@@ -712,23 +722,41 @@ int attend_few(PackedAttnParams& P, const infllm_packed_seq* seqs, const infllm_
     INFLLM_CUDA_OK(launch_chained(kern, dim3((unsigned)units, c->n_kv_heads), dim3(kAttnWarps * 32), 0, s, P));
     INFLLM_LAUNCH_OK("packed_rows_kernel");
   }
-  return join || (P.logits && units > 0) ? join_launch<T, kDim, false>(P, P, join, n_sm, s) : INFLLM_OK;
+  if (!join && (!P.logits || units == 0)) return INFLLM_OK;
+  const int64_t rows = (int64_t)P.batch * P.most * n_heads_of(P);
+  return by_warps(rows, n_sm, [&](auto warps) {
+    constexpr int kWarps = decltype(warps)::value;
+    P.join_blocks = join ? (int)ceil_div(rows * kWarps, 8) : 0;
+    const int64_t sums = P.logits ? (int64_t)P.batch * P.at.n_kv * (P.pitch / kSumKeys) : 0;
+    return launch_chained(packed_join_kernel<T, kDim, kWarps>, dim3((unsigned)(P.join_blocks + sums)), dim3(256), 0, s, P);
+  });
 }
 
 template <typename T, int kDim>
-int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, char* work, int n_sm, bool join, cudaStream_t s) {
+int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_packed* c, char* work, int n_sm, cudaStream_t s) {
   const int64_t image = image_bytes(c, seqs, P.a.batch, P.a.group);
-  INFLLM_TRY(lay_out_many(c, seqs, n_sm, P, &join));
+  bool cut = false;
+  INFLLM_TRY(lay_out_many(c, seqs, n_sm, P, &cut));
   P.image = image > 0 ? work : nullptr, P.n_image = 0;
-  for (int i = 0; image > 0 && i < P.a.batch; ++i) {
+  int fewest = P.a.most, rows = 0;
+  for (int i = 0; i < P.a.batch; ++i) {
     P.a.seq[i].keys = P.n_image;
-    if (seqs[i].count > 0) P.n_image += c->n_kv_heads * (int)ceil_div(seqs[i].length, kKeyTile);
+    if (image > 0 && seqs[i].count > 0) P.n_image += c->n_kv_heads * (int)ceil_div(seqs[i].length, kKeyTile);
+    fewest = std::min(fewest, seqs[i].count), rows = std::max(rows, std::min(kBlockRows, seqs[i].count * P.a.group));
   }
-  P.a.part_o = (float*)(work + image);
+  P.a.part_o = (float*)(work + image), P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
   INFLLM_TRY(tc_get_error_ptr(&P.a.err));
-  P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
   if (P.n_ctas > 0) INFLLM_TRY(packed_tc_launch(P, c->dtype, kDim, s));
-  return join ? join_launch<T, kDim, true>(P, P.a, true, n_sm, s) : INFLLM_OK;
+  if (cut)
+    INFLLM_TRY(by_warps((int64_t)P.n_ctas * rows, n_sm, [&](auto warps) {
+      constexpr int kWarps = decltype(warps)::value;
+      return launch_chained(packed_join_cut_kernel<T, kDim, kWarps>, dim3((unsigned)ceil_div(rows * kWarps, 8), P.n_ctas), dim3(256), 0, s, P);
+    }));
+  if (fewest < P.a.most) {
+    INFLLM_CUDA_OK(launch_chained(packed_empty_kernel<T, kDim>, dim3((unsigned)ceil_div((int64_t)(P.a.most - fewest) * n_heads_of(P.a), 8), P.a.batch), dim3(256), 0, s, P.a));
+    INFLLM_LAUNCH_OK("packed_empty_kernel");
+  }
+  return INFLLM_OK;
 }
 
 }  // namespace
@@ -787,7 +815,7 @@ extern "C" int infllm_packed_attend(const infllm_packed* c, int layer, const inf
         empty = empty || mine[i].count < most;
       }
       INFLLM_DISPATCH_DTYPE(c->dtype, T, {
-        if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, (char*)d_work, n_sm, empty, s) : attend_many<T, 64>(Tc, mine, c, (char*)d_work, n_sm, empty, s)));
+        if (many) INFLLM_TRY((c->head_dim == 128 ? attend_many<T, 128>(Tc, mine, c, (char*)d_work, n_sm, s) : attend_many<T, 64>(Tc, mine, c, (char*)d_work, n_sm, s)));
         else INFLLM_TRY((c->head_dim == 128 ? attend_few<T, 128>(P, mine, c, n_sm, empty, s) : attend_few<T, 64>(P, mine, c, n_sm, empty, s)));
         if (weigh > 0 && any && many) {
           bool cut = false;

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t s_base = smem_u32(smem), sK = s_base + L::kK, sRing = s_base + L::kRing, bars = s_base + L::kBar;
-  float* const sLse = reinterpret_cast<float*>(smem + L::kLse);
+  float* const sLse = reinterpret_cast<float*>(smem + L::kLse);  // log-sum-exps of a tile's rows, negative
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + N_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBar + N_BARS * 8 + 8);
   auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
@@ -136,20 +136,25 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(K_FULL));
 
-      // query tiles, two on their way behind the one that has to be there
+      // query tiles, one on its way behind the one that has to be there
       const int rows = S.count * P.a.group;
       const int64_t q0 = (int64_t)(P.a.b0 + U.b) * P.a.q_bs + (int64_t)U.hkv * P.a.group * P.a.q_hs + (int64_t)(P.a.most - S.count) * P.a.q_ts;
       const float* row_lse = P.a.row_lse + ((int64_t)(P.a.b0 + U.b) * P.a.at.n_kv + U.hkv) * P.a.most * P.a.group;
-      constexpr int kPer = kDim / 8, kAt = 32 / kPer, kLag = 2;
+      constexpr int kPer = kDim / 8, kAt = 32 / kPer, kLag = 1;
       const int c = lane % kPer, wq = (warp - kWarpLoad) * 32;
+      // (a row's log-sum-exp is asked for a tile ahead: a tile is not to wait for it)
+      auto lse_of = [&](int r) { return r < rows ? -__ldg(row_lse + r) : -INFINITY; };  // (a row that is none gives nothing)
+      float z = lse_of(U.row0 + wq + lane);
       for (int i = 0; i < U.n + kLag && ok; ++i) {
         if (i < U.n) {
+          const float next = lse_of(U.row0 + (i + 1) * 128 + wq + lane);
           const int b = (slot + i) % kStages;
           if (slot + i >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot + i - kStages, kStages), abort_flag, err, 782);
           if (!ok) break;
           const int r = U.row0 + i * 128 + wq + lane, tok = r / P.a.group;
           const int64_t from = r < rows ? q0 + (int64_t)(r - tok * P.a.group) * P.a.q_hs + (int64_t)tok * P.a.q_ts : -1;
-          sLse[b * 128 + wq + lane] = r < rows ? __ldg(row_lse + r) : INFINITY;  // (a row that is none gives nothing)
+          sLse[b * 128 + wq + lane] = z;
+          z = next;
           const uint32_t to = sRing + b * L::kTileBytes + wq * 128 + (c >> 3) * kSubTileBytes;
 #pragma unroll 4
           for (int x = lane / kPer; x < 32; x += kAt) {
@@ -240,8 +245,8 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
               const float4 z = lse[c * 8 + x];
-              a[2 * x] = ffma2(__uint_as_float(w[4 * x]), __uint_as_float(w[4 * x + 1]), sc, make_float2(-z.x, -z.y));
-              a[2 * x + 1] = ffma2(__uint_as_float(w[4 * x + 2]), __uint_as_float(w[4 * x + 3]), sc, make_float2(-z.z, -z.w));
+              a[2 * x] = ffma2(__uint_as_float(w[4 * x]), __uint_as_float(w[4 * x + 1]), sc, make_float2(z.x, z.y));
+              a[2 * x + 1] = ffma2(__uint_as_float(w[4 * x + 2]), __uint_as_float(w[4 * x + 3]), sc, make_float2(z.z, z.w));
             }
             tmem_ld32_if(c < 3, tS + 32 * c + 32, w);
             if (last_first > row0 + 32 * c) {
