@@ -532,27 +532,35 @@ static int by_warps(int64_t rows, int n_sm, F&& launch) {
 
 namespace {
 
-// Keys of a unit's stretch, so that all units run in about one, two or some waves of as many as the machine holds
-int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int64_t resident) {
-  constexpr double kGroup = 1., kUnit = 5.;  // microseconds of a warp's 16 keys, and of a unit besides
-  int64_t most = 64;
-  for (int i = 0; i < n; ++i) most = std::max<int64_t>(most, ceil_div(seqs[i].length, 64) * 64);
+// Keys of a unit's stretch.  A multiprocessor takes kGroup microseconds to a block's 64 keys while it has blocks to spare, kTwo to two blocks'
+// and kAlone to one's; a wave of blocks costs kWave besides, and a join kJoin.  (Fitted to ten batches of 1 to 64 sequences, each with
+// stretches of 64 to 6144 keys; what is chosen takes up to 8 % more than the best of those.)
+int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int n_sm) {
+  constexpr double kGroup = .3, kTwo = .7, kAlone = .42, kWave = 2.5, kJoin = 4.;
+  int64_t most = 64, groups = 0;  // (up to 2^24 keys, so that a stretch's bytes are counted in 32 bits)
+  for (int i = 0; i < n; ++i) {
+    if (seqs[i].count == 0) continue;
+    most = std::max<int64_t>(most, std::min<int64_t>(ceil_div(seqs[i].length, 64) * 64, 1 << 24));
+    groups += ceil_div(seqs[i].length, 64);
+  }
   auto units = [&](int64_t keys) {
     int64_t u = 0;
-    for (int i = 0; i < n; ++i) u += seqs[i].count > 0 ? ceil_div(seqs[i].length, keys) : 0;
+    for (int i = 0; i < n; ++i) u += seqs[i].count > 0 ? (uint32_t)(seqs[i].length + keys - 1) / (uint32_t)keys : 0;
     return u * c->n_kv_heads;
   };
-  int64_t best = most;
+  int64_t best = most, tried = 0;
   double least = 1e300;
-  for (int waves = 1; waves <= 6; ++waves) {
-    int64_t lo = 1, hi = most / 64;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (units(mid * 64) <= waves * resident) hi = mid;
-      else lo = mid + 1;
-    }
-    const double cost = (double)ceil_div(units(lo * 64), resident) * ((double)lo * kGroup + kUnit);
-    if (cost < least) least = cost, best = lo * 64;
+  for (int each = 1; each <= 14; ++each) {  // blocks of a multiprocessor
+    const int64_t room = (int64_t)each * n_sm;
+    int64_t keys = std::min(most, std::max<int64_t>(1, groups * c->n_kv_heads / room) * 64), u = units(keys);
+    while (u > room && keys < most) keys = std::min(most, std::max(keys + 64, keys * std::min(u, 2 * room) / room / 64 * 64)), u = units(keys);
+    for (int down = 0; down < 8 && keys > 64 && units(keys - 64) == u; ++down) keys -= 64;
+    if (keys == tried) continue;
+    tried = keys;
+    const int64_t per = ceil_div(u, n_sm);
+    const double cost = (double)(keys / 64) * (per > 2 ? kGroup * (double)per : per == 2 ? kTwo : kAlone) + kWave * (double)ceil_div(per, 4) + (keys < most ? kJoin : 0.);
+    if (cost < least) least = cost, best = keys;
+    if (keys == 64) break;
   }
   return best;
 }
@@ -593,7 +601,7 @@ int64_t logit_pitch(const infllm_packed_seq* seqs, int n) {
 
 // the units of the launch of seqs[0 .. n - 1] for few rows: stretches of a sequence's keys
 int64_t lay_out_few(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int n_sm, PackedAttnSeq* to, bool* join) {
-  const int64_t keys = chunk_keys(c, seqs, n, n_sm * 4);
+  const int64_t keys = chunk_keys(c, seqs, n, n_sm);
   int64_t u = 0;
   for (int i = 0; i < n; ++i) {
     const int64_t chunks = seqs[i].count > 0 ? ceil_div(seqs[i].length, keys) : 0;
