@@ -112,6 +112,15 @@ class PackedCache:
     def batch(self, seqs):
         return PackedBatch(self, seqs)
 
+    def check(self):
+        """Waits for the device, and raises InfLLMError (E_TIMEOUT) where an attention kernel on it has given up a wait and left rows
+        unwritten."""
+        with torch.cuda.device(self.device):
+            code, where = _lib.device_error()
+        if code:
+            raise _lib.InfLLMError(_lib.E_TIMEOUT, f"a bounded wait of an attention kernel ran out in a call before (code {code}, wait {where}): the "
+                                   "rows that the block was to write are not valid")
+
     def evict(self, seqs, budget, sink=0, recent=0, into=None):
         """In every layer, each KV head of a sequence of more than `budget` tokens keeps that many, in their order: the first `sink`, the
         newest `recent`, and of the others those of the largest weights (of equal ones the earlier).  Which ones differs from head

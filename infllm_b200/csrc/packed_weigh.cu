@@ -6,7 +6,9 @@
 // at a time: keys are taken out of their codes once, queries go through a ring of tiles with their log-sum-exps.  Units are dealt out to
 // the blocks in stretches of about equal work, as (unit, tile of rows); what is cut is added up by one more kernel, in order.
 // Sums: within a tile of rows in eight numbers of 32 bits, then tile by tile, so that an error does not grow with the rows.
-// What bounds it: the exponentials, three eighths of them by a quintic on the FMA pipe.
+// What bounds it: the exponentials, a quarter of them by a quintic on the FMA pipe, and what is issued around them (128 queries by 256 keys in 2 us; without
+// exponentials 1.1).  Keys as the operand in TMEM, a warp of its own for each team's products, or three eighths or none of the exponentials by
+// the polynomial took as long.
 #include <atomic>
 
 #include "attn_tc.cuh"
@@ -55,11 +57,11 @@ struct Pieces {  // a block's, in turn
   }
 };
 
-// exponentials to base 2 of 16 pairs, added up: of every eight pairs three on the FMA pipe
+// exponentials to base 2 of 16 pairs, added up: of every four pairs one on the FMA pipe
 __device__ __forceinline__ void exp_sum(const float2* a, float2* rs) {
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const float2 p = k % 8 == 1 || k % 8 == 4 || k % 8 == 6 ? ex2_poly2<5>(a[k]) : make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
+    const float2 p = k % 4 == 3 ? ex2_poly2<5>(a[k]) : make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
     rs[k & 3] = fadd2(rs[k & 3], p);
   }
 }

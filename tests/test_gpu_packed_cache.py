@@ -269,8 +269,28 @@ def test_weights(dim, kv, heads, dtype, lengths, counts, weigh, decay):
         assert torch.equal(c.weights.nan_to_num(-5), after.nan_to_num(-5))  # the same bits again
 
 
+@pytest.mark.parametrize("dim,kv,heads,dtype", SHAPES[:4])
+@pytest.mark.parametrize("lengths,counts,weigh", [([2600], [2600], True), ([1300, 2100, 5], [900, 1, 0], 700), ([9000], [40], True), ([257, 255], [130, 255], 256)])
+def test_weights_of_long_prompts(dim, kv, heads, dtype, lengths, counts, weigh):
+    """Prompts whose tiles are taken out of their codes beforehand, units that are cut and added up in parts, and units of one tile of keys."""
+    g = gen(sum(lengths) + dim)
+    c = make(kv, dim, len(lengths) + 1, max(lengths) + 3, dtype)
+    seqs = c.open(len(lengths) + 1)[1:]
+    b = fill(c, g, seqs, lengths)
+    for s, n in zip(seqs, lengths):
+        c.weights[0, s, :, :n] = torch.rand((kv, n), generator=g, device="cuda")
+    before, most = c.weights.clone(), max(counts)
+    b.plan(counts)
+    q = rand(g, len(seqs), most, heads, dim, dtype=dtype, scale=1.5).permute(0, 2, 1, 3)
+    out, lse = b.attend(0, q, return_lse=True, weigh=weigh, decay=0.75)
+    check(c, b, counts, q, out, lse, weigh=most if weigh is True else weigh, before=before, decay=0.75)
+    c.weights.copy_(before)
+    out2, lse2 = b.attend(0, q, return_lse=True, weigh=weigh, decay=0.75)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
 @pytest.mark.parametrize("dim,kv,heads,dtype", SHAPES[:3])
-@pytest.mark.parametrize("n", [4, 200])
+@pytest.mark.parametrize("n", [4, 200, 420])
 def test_tokens_that_are_no_numbers_are_none_only_where_they_are_seen(dim, kv, heads, dtype, n):
     g = gen(9)
     c = make(kv, dim, 1, 600, dtype)
@@ -570,6 +590,23 @@ def test_many_sequences_in_one_call():
     for i in (38, 127, 128, 271, 299):
         rows = stay_of(w[0, i], lengths[i], 11, 1, 3)[0].cuda()
         assert torch.equal(c.weights[0, i, 0, :len(rows)], w[0, i, 0, rows])
+
+
+def test_a_step_without_tokens():
+    c = make(2, 64, 2, 50)
+    b = c.batch(c.open(2))
+    none = torch.empty((2, 2, 0, 64), dtype=torch.bfloat16, device="cuda")
+    for step in (b.extend, b.plan):
+        step(0)
+        assert b.write(0, none, none) is None
+        out, lse = b.attend(0, torch.empty((2, 8, 0, 64), dtype=torch.bfloat16, device="cuda"), return_lse=True, weigh=True)
+        assert out.shape == (2, 8, 0, 64) and lse.shape == (2, 8, 0)
+        assert b.values(0)[0].shape == (2, 2, 0, 64) and b.values()[1].shape == (1, 2, 2, 0, 64)
+    c.evict(b.seqs, 0)
+    c.evict([], 5)
+    empty = c.batch([])
+    empty.extend(3)
+    assert c.scales.isnan().all()
 
 
 def test_refusals_of_tensors():
