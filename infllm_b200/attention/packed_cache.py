@@ -127,6 +127,9 @@ class PackedCache:
         to head: `places` says it.  Keys keep the rotation that they were written with, and position() goes on from where it was.
         `into`: sequences of this cache that get what stays (all of a shorter sequence) in place of what they hold; `seqs` then
         stay as they are."""
+        for x in (budget, sink, recent):
+            if not -1 << 63 <= x < 1 << 63:
+                raise OverflowError(f"{x} is beyond 64 bits")
         n, ids, to = len(seqs), _ids(seqs), None
         if into is not None:
             if len(into) != n:
@@ -194,8 +197,10 @@ class PackedBatch:
         else:
             self.tokens, self._at, self._rooms = self._info[0], c._book.changes, {}
 
-    def _current(self):
+    def _layer(self, layer):
         c = self.cache
+        if not 0 <= layer < c.n_layers:
+            raise ValueError(f"layer {layer} of {c.n_layers}")
         if self._at == c._book.changes:
             return
         if self._at is None:
@@ -215,7 +220,8 @@ class PackedBatch:
 
     def retract(self, n):
         """Takes the newest n tokens of every sequence, or n[i], back, as a speculative decoder does with drafts.  They are tokens
-        that were written since the last eviction, or that it kept as `recent`."""
+        that were written since the last eviction, or that it kept as `recent`.  (What their queries have added to the weights of
+        others stays.)"""
         self._step(_lib.PACKED_RETRACT, n)
 
     def _rows(self, t, heads, what):
@@ -245,7 +251,7 @@ class PackedBatch:
         """The step's keys and values (batch, n_kv_heads, tokens, head_dim) into a layer of the cache, with weights of 0.  With `rope`,
         a RotaryEmbeddingESM, keys and queries are rotated to their positions.  Returns the queries (None without q)."""
         c = self.cache
-        self._current()
+        self._layer(layer)
         if not self._info[2]:
             raise ValueError("tokens that an eviction has come after are not written again")
         k, k_at, k_bs, k_hs, k_ts = self._rows(k, c.n_kv_heads, "k")
@@ -272,7 +278,7 @@ class PackedBatch:
         """What the cache holds of the step's tokens, in its 16-bit type: keys and values (batch, n_kv_heads, tokens, head_dim) of a layer,
         or (n_layers, batch, ..) of all."""
         c = self.cache
-        self._current()
+        self._layer(0 if layer is None else layer)
         first, n = (0, c.n_layers) if layer is None else (layer, 1)
         k, v = (torch.empty((n, self._n, c.n_kv_heads, self.tokens, c.head_dim), dtype=c.dtype, device=c.device) for _ in range(2))
         _lib.check(_lib_call.infllm_packed_values(c._ref, first, n, self._table, self._n, self.tokens, k.data_ptr(), v.data_ptr(),
@@ -287,7 +293,7 @@ class PackedBatch:
         the tokens' queries give them, summed over the queries and the query heads of a KV head: all queries' (True), or those of
         each sequence's newest `weigh` tokens of the step.  Each such call adds."""
         c = self.cache
-        self._current()
+        self._layer(layer)
         heads = q.size(1)
         q, at, bs, hs, ts = self._rows(q, heads, "q")
         out = self._out(q, heads)
@@ -296,6 +302,8 @@ class PackedBatch:
             lse = torch.empty((self._n, self.tokens, heads), dtype=torch.float32, device=c.device)
             lse_at = lse.data_ptr()
         weigh = self.tokens if weigh is True else min(int(weigh), self.tokens)
+        if weigh < 0:
+            raise ValueError(f"the weights of {weigh} tokens")
         size = self._rooms.get((heads, weigh))
         if size is None:  # the first layer of a step
             size = c_int64()

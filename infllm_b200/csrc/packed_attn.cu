@@ -550,7 +550,7 @@ int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n,
   };
   int64_t best = most, tried = 0;
   double least = 1e300;
-  for (int each = 1; each <= 14; ++each) {  // blocks of a multiprocessor
+  for (int each = 1; each <= 32; each += each < 14 ? 1 : 6) {  // blocks of a multiprocessor
     const int64_t room = (int64_t)each * n_sm;
     int64_t keys = std::min(most, std::max<int64_t>(1, groups * c->n_kv_heads / room) * 64), u = units(keys);
     while (u > room && keys < most) keys = std::min(most, std::max(keys + 64, keys * std::min(u, 2 * room) / room / 64 * 64)), u = units(keys);
@@ -558,7 +558,10 @@ int64_t chunk_keys(const infllm_packed* c, const infllm_packed_seq* seqs, int n,
     if (keys == tried) continue;
     tried = keys;
     const int64_t per = ceil_div(u, n_sm);
-    const double cost = (double)(keys / 64) * (per > 2 ? kGroup * (double)per : per == 2 ? kTwo : kAlone) + kWave * (double)ceil_div(per, 4) + (keys < most ? kJoin : 0.);
+    // (equal blocks run in waves; where lengths differ, short ones fill up what the long ones leave, but for the last)
+    const double each_full = (double)(keys / 64) * (per > 2 ? kGroup * (double)per : per == 2 ? kTwo : kAlone);
+    const double filled = kGroup * (double)(groups * c->n_kv_heads) / n_sm + kAlone * (double)(keys / 64);
+    const double cost = std::min(each_full, filled) + kWave * (double)ceil_div(per, 4) + (keys < most ? kJoin : 0.);
     if (cost < least) least = cost, best = keys;
     if (keys == 64) break;
   }
@@ -711,7 +714,8 @@ int check_attend(const infllm_packed* c, const infllm_packed_seq* seqs, int n, i
   PackedAttnSeq to[kAttnSeqs];
   bool join = false;
   for (int b0 = 0; b0 < n; b0 += kAttnSeqs) units = std::max(units, lay_out_few(c, seqs + b0, std::min(n - b0, kAttnSeqs), n_sm, to, &join));
-  if (units > INT_MAX) return fail(INFLLM_E_BADARG, "%s: %lld units of work", what, (long long)units);
+  const int64_t sums = weigh > 0 ? std::min(n, kAttnSeqs) * (int64_t)c->n_kv_heads * (logit_pitch(seqs, n) / kSumKeys) : 0;  // (blocks of a launch)
+  if (units > INT_MAX || sums > INT_MAX / 2) return fail(INFLLM_E_BADARG, "%s: %lld units of work, the weights of %lld thousand tokens", what, (long long)units, (long long)sums);
   *bytes = ceil_div(units * c->n_kv_heads * kFewRows * (c->head_dim + 1) * 4, 16) * 16 + (weigh > 0 ? (int64_t)n * most * n_heads * logit_pitch(seqs, n) * 4 : 0);
   return INFLLM_OK;
 }

@@ -616,8 +616,8 @@ def test_refusals_of_tensors():
     t = torch.zeros((1, 2, 3, 64), dtype=torch.bfloat16, device="cuda")
     for call, error in ((lambda: b.write(0, t[:, :1], t), ValueError), (lambda: b.write(0, t, t.half()), TypeError), (lambda: b.write(0, t.cpu(), t), RuntimeError),
                         (lambda: b.attend(0, t[:, :, :2]), ValueError), (lambda: b.attend(0, t.float()), TypeError), (lambda: b.write(0, t, t, rope=3), ValueError),
-                        (lambda: b.attend(1, t), RuntimeError), (lambda: b.attend(0, t[:, :0]), RuntimeError), (lambda: b.attend(0, t, scale=-1.0), RuntimeError),
-                        (lambda: b.values(1), RuntimeError), (lambda: b.write(-1, t, t), RuntimeError)):
+                        (lambda: b.attend(1, t), ValueError), (lambda: b.attend(1 << 32, t), ValueError), (lambda: b.attend(0, t, weigh=-1), ValueError), (lambda: b.attend(0, t, weigh=-1 << 40), ValueError), (lambda: b.attend(0, t[:, :0]), RuntimeError), (lambda: b.attend(0, t, scale=-1.0), RuntimeError),
+                        (lambda: b.values(1), ValueError), (lambda: b.write(-1, t, t), ValueError), (lambda: b.attend(0, t, scale=1e300), RuntimeError), (lambda: b.attend(0, t, weigh=True, decay=-0.5), RuntimeError)):
         with pytest.raises(error):
             call()
     assert c.scales.isnan().all()

@@ -95,6 +95,24 @@ def test_refusals_change_nothing(cache, call):
     assert state(c) == before and not [n for n, _ in c.calls.seen if "evict" in n]
 
 
+def test_numbers_that_do_not_fit_are_refused_not_cut(cache):
+    c = cache()
+    b = c.batch(c.open())
+    b.extend(5)
+    before = state(c)
+    for args in ((1 << 64,), (1 << 63,), (5, 1 << 64), (5, 0, -(1 << 64))):
+        with pytest.raises(OverflowError):
+            c.evict([0], *args)
+    for seqs in ([1 << 32], [-1 << 40]):
+        with pytest.raises((OverflowError, ValueError)):
+            c.evict(seqs, 3)
+        with pytest.raises(ValueError):
+            c.batch(seqs)
+    with pytest.raises(ValueError):
+        b.values(1 << 32)
+    assert state(c) == before
+
+
 def test_positions_go_on_behind_an_eviction(cache):
     c = cache()
     s, t = c.open(2)
