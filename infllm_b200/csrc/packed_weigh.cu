@@ -20,13 +20,13 @@ namespace infllm {
 
 namespace xwg {
 constexpr int kStages = 4;
-constexpr int kWarpMma = 8, kWarpLoad = 9, kLoadWarps = 4;
+constexpr int kSumWarps = 16, kWarpMma = 16, kWarpLoad = 17, kLoadWarps = 4;  // eight warps of a team: four for each half of the columns
 constexpr int kThreads = (kWarpLoad + kLoadWarps) * 32;
-enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, K_FULL = EMPTY0 + kStages, K_FREE, S_FULL0, S_FREE0 = S_FULL0 + 4, N_BARS = S_FREE0 + 4 };  // S: 2 * team + buffer
+enum { FULL0 = 0, EMPTY0 = FULL0 + kStages, K_FULL = EMPTY0 + kStages, K_FREE, S_FULL0, S_FREE0 = S_FULL0 + 4, SUMS = S_FREE0 + 4, SUMS_READ, N_BARS };  // S: 2 * team + buffer
 template <int kDim>
 struct Smem {
   static constexpr int kTileBytes = 128 * kDim * 2;
-  static constexpr int kK = 0, kRing = 2 * kTileBytes, kLse = kRing + kStages * kTileBytes, kBar = kLse + kStages * 512, kTotal = kBar + 256;
+  static constexpr int kK = 0, kRing = 2 * kTileBytes, kLse = kRing + kStages * kTileBytes, kBar = kLse + kStages * 512, kSum = kBar + 256, kTotal = kSum + kWeighKeys * 4;
 };
 
 struct Piece {
@@ -57,15 +57,30 @@ struct Pieces {  // a block's, in turn
   }
 };
 
-// exponentials to base 2 of 16 pairs, added up: of every four pairs one on the FMA pipe
+// exponentials to base 2 of eight pairs, added up: of every four pairs one on the FMA pipe
 __device__ __forceinline__ void exp_sum(const float2* a, float2* rs) {
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
+  for (int k = 0; k < 8; ++k) {
     const float2 p = k % 4 == 3 ? ex2_poly2<5>(a[k]) : make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
     rs[k & 3] = fadd2(rs[k & 3], p);
   }
 }
 }  // namespace xwg
+
+__device__ __forceinline__ void tmem_ld16_if(bool yes, uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %17, 0;\n\t"
+      "@p tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t}"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+      : "r"(taddr), "r"((uint32_t)yes)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               ::"memory");
+}
 
 template <typename T, int kDim>
 __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const __grid_constant__ PackedTcParams P) {
@@ -83,8 +98,8 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
 
   if (warp == 0) {
     static_assert(N_BARS <= 32 && N_BARS * 8 + 16 <= 256, "");
-    // tiles and keys: the four warps that load; free tiles: the products and eight warps; free scores: a team's warps
-    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 || lane == K_FULL || lane >= S_FREE0 ? 4u : lane < K_FULL ? 9u : 1u);
+    // tiles and keys: the four warps that load; free tiles: the products and the warps that sum; free scores: a team's; sums: half of them
+    if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 || lane == K_FULL ? 4u : lane < K_FULL ? kSumWarps + 1u : lane >= S_FREE0 ? kSumWarps / 2u : 1u);
     if (lane == 0) *abort_flag = 0;
     mbar_fence_init();
   }
@@ -216,9 +231,9 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
     }
   } else {
     // ========================================================================================================= sums
-    const int quad = warp & 3, team = warp >> 2;
+    const int quad = warp & 3, team = warp >> 2 & 1, half = warp >> 3;  // (a warp's place among four says which lanes of TMEM it reads)
     const uint32_t lane_base = ((uint32_t)(quad * 32)) << 16;
-    int slot = 0, used[2] = {0, 0};
+    int slot = 0, used[2] = {0, 0}, n_units = 0;
     while (ok && pieces.next(P, U)) {
       const PackedAttnSeq& S = P.a.seq[U.b];
       const bool mine = team == 0 || U.keys > 128;
@@ -233,28 +248,28 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
           ok = warp_wait(bar(S_FULL0 + s), used[buf]++ & 1, abort_flag, err, 796);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t tS = tmem + s * 128 + lane_base;
-          const int row0 = U.row0 + i * 128;
-          const float4* lse = reinterpret_cast<const float4*>(sLse + stage * 128);
+          const uint32_t tS = tmem + s * 128 + lane_base + half * 64;
+          const int row0 = U.row0 + i * 128 + half * 64;
+          const float4* lse = reinterpret_cast<const float4*>(sLse + stage * 128 + half * 64);
           float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 sc = make_float2(P.a.scale_log2, P.a.scale_log2);
-          uint32_t w[32];
-          tmem_ld32(tS, w);
+          uint32_t w[16];
+          tmem_ld16_if(true, tS, w);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld32(w);
-            float2 a[16];
+            tmem_wait_ld16(w);
+            float2 a[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const float4 z = lse[c * 8 + x];
+            for (int x = 0; x < 4; ++x) {
+              const float4 z = lse[c * 4 + x];
               a[2 * x] = ffma2(__uint_as_float(w[4 * x]), __uint_as_float(w[4 * x + 1]), sc, make_float2(z.x, z.y));
               a[2 * x + 1] = ffma2(__uint_as_float(w[4 * x + 2]), __uint_as_float(w[4 * x + 3]), sc, make_float2(z.z, z.w));
             }
-            tmem_ld32_if(c < 3, tS + 32 * c + 32, w);
-            if (last_first > row0 + 32 * c) {
-              const int hidden = first - row0 - 32 * c;  // columns of rows that do not see the key
+            tmem_ld16_if(c < 3, tS + 16 * c + 16, w);
+            if (last_first > row0 + 16 * c) {
+              const int hidden = first - row0 - 16 * c;  // columns of rows that do not see the key
 #pragma unroll
-              for (int x = 0; x < 16; ++x) {
+              for (int x = 0; x < 8; ++x) {
                 if (2 * x < hidden) a[x].x = -INFINITY;
                 if (2 * x + 1 < hidden) a[x].y = -INFINITY;
               }
@@ -272,7 +287,21 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
           mbar_arrive(bar(EMPTY0 + stage));
         }
       }
-      if (ok && k < U.keys) {
+      // the second half's sums go to the first half's warps
+      float* const halves = reinterpret_cast<float*>(smem + L::kSum);
+      if (half == 1) {
+        if (ok && n_units > 0) ok = warp_wait(bar(SUMS_READ), (n_units - 1) & 1, abort_flag, err, 797);
+        if (ok) halves[k] = sum;
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(bar(SUMS));
+      } else {
+        ok = ok && warp_wait(bar(SUMS), n_units & 1, abort_flag, err, 798);
+        if (ok) sum += halves[k];
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(bar(SUMS_READ));
+      }
+      ++n_units;
+      if (ok && half == 0 && k < U.keys) {
         if (U.slot >= 0) {
           P.a.part_o[(int64_t)U.slot * kWeighKeys + k] = sum;
         } else {
