@@ -2,13 +2,15 @@
 // probabilities, whose log-sum-exps are known, w_j = sum_i exp2(s_ij - lse_i).
 //
 // S^T = K Q^T by tcgen05: keys are the lanes of TMEM, so that a thread has a key and adds up along its row, and nothing is exchanged.  A
-// unit is 256 keys of one KV head (two tiles of 128, one each for two teams of four warps) by the counted rows that see them, 128
-// at a time: keys are taken out of their codes once, queries go through a ring of tiles with their log-sum-exps.  Units are dealt out to
-// the blocks in stretches of about equal work, as (unit, tile of rows); what is cut is added up by one more kernel, in order.
+// unit is 256 keys of one KV head (two tiles of 128, one each for two teams of eight warps, of which four have half of the columns each)
+// by the counted rows that see them, 128 at a time: keys are taken out of their codes once, queries go through a ring of tiles with their
+// log-sum-exps.  Units are dealt out to the blocks in stretches of about equal work, as (unit, tile of rows); what is cut is added up by
+// one more kernel, in order.
 // Sums: within a tile of rows in eight numbers of 32 bits, then tile by tile, so that an error does not grow with the rows.
-// What bounds it: the exponentials, a quarter of them by a quintic on the FMA pipe, and what is issued around them (128 queries by 256 keys in 2 us; without
-// exponentials 1.1).  Keys as the operand in TMEM, a warp of its own for each team's products, or three eighths or none of the exponentials by
-// the polynomial took as long.
+// What bounds it: what is issued around the exponentials, 32768 of them in 3000 cycles (a prompt of 4096 tokens, 32/8 heads: 115 us; with a
+// quarter of them by a quintic on the FMA pipe instead of an eighth 118, three eighths 125; without any 80).  By clock readings a warp is
+// at its sums for 2330 cycles of a tile, the loads' copies take 1700, the products' issue 1100.  Tried: keys as the operand in TMEM, a warp of
+// its own for each team's products, products of 64 columns (each as long); eight warps of sums instead of sixteen (5 % more).
 #include <atomic>
 
 #include "attn_tc.cuh"
@@ -57,11 +59,11 @@ struct Pieces {  // a block's, in turn
   }
 };
 
-// exponentials to base 2 of eight pairs, added up: of every four pairs one on the FMA pipe
+// exponentials to base 2 of eight pairs, added up: one pair on the FMA pipe
 __device__ __forceinline__ void exp_sum(const float2* a, float2* rs) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float2 p = k % 4 == 3 ? ex2_poly2<5>(a[k]) : make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
+    const float2 p = k == 7 ? ex2_poly2<5>(a[k]) : make_float2(ex2_approx(a[k].x), ex2_approx(a[k].y));
     rs[k & 3] = fadd2(rs[k & 3], p);
   }
 }
@@ -159,6 +161,8 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
       const float* row_lse = P.a.row_lse + ((int64_t)(P.a.b0 + U.b) * P.a.at.n_kv + U.hkv) * P.a.most * P.a.group;
       constexpr int kPer = kDim / 8, kAt = 32 / kPer, kLag = 1;
       const int c = lane % kPer, wq = (warp - kWarpLoad) * 32;
+      const int step_h = kAt % P.a.group;
+      const int64_t step = (int64_t)(kAt / P.a.group) * P.a.q_ts + step_h * P.a.q_hs, wrap = P.a.q_ts - P.a.group * P.a.q_hs;
       // (a row's log-sum-exp is asked for a tile ahead: a tile is not to wait for it)
       auto lse_of = [&](int r) { return r < rows ? -__ldg(row_lse + r) : -INFINITY; };  // (a row that is none gives nothing)
       float z = lse_of(U.row0 + wq + lane);
@@ -168,15 +172,19 @@ __global__ void __launch_bounds__(xwg::kThreads, 1) packed_weigh_tc_kernel(const
           const int b = (slot + i) % kStages;
           if (slot + i >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(slot + i - kStages, kStages), abort_flag, err, 782);
           if (!ok) break;
-          const int r = U.row0 + i * 128 + wq + lane, tok = r / P.a.group;
-          const int64_t from = r < rows ? q0 + (int64_t)(r - tok * P.a.group) * P.a.q_hs + (int64_t)tok * P.a.q_ts : -1;
           sLse[b * 128 + wq + lane] = z;
           z = next;
+          // a lane's rows are kAt apart: the next one is some heads on, and a token where those are through
           const uint32_t to = sRing + b * L::kTileBytes + wq * 128 + (c >> 3) * kSubTileBytes;
-#pragma unroll 4
-          for (int x = lane / kPer; x < 32; x += kAt) {
-            const int64_t f = __shfl_sync(0xffffffffu, from, x);
-            mma::cp_async16(to + x * 128 + (((c & 7) ^ (x & 7)) << 4), P.a.q + (f < 0 ? 0 : f) + c * 16, f >= 0);
+          const int r = U.row0 + i * 128 + wq + lane / kPer, tok = r / P.a.group, left = rows - r;
+          int h = r - tok * P.a.group;
+          const char* from = P.a.q + q0 + (int64_t)h * P.a.q_hs + (int64_t)tok * P.a.q_ts + c * 16;
+#pragma unroll
+          for (int x = 0; x < 32; x += kAt) {
+            const int row = x + lane / kPer;
+            mma::cp_async16(to + row * 128 + (((c & 7) ^ (row & 7)) << 4), x < left ? from : P.a.q, x < left);
+            from += step, h += step_h;
+            if (h >= P.a.group) h -= P.a.group, from += wrap;
           }
         }
         mma::cp_async_commit();  // (an empty one behind the last)
