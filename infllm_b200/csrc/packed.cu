@@ -97,6 +97,8 @@ __device__ __forceinline__ void pack_rotate8(uint4& lo, uint4& hi, const float* 
 
 // A thread has 8 numbers of the first half of a row and the 8 that are rotated with them; the four threads of a group of 32 agree on
 // its least number and step.
+// What bounds it: bytes, and the arithmetic of codes beside them.  8192 tokens of 32 query and 32 KV heads of 128 in fp16, rotated, 310 MB
+// in and out, 58 to 69 us: 4.5 to 5.4 TB/s (with a division a number 77).  Of 64 single tokens, 3.6 us.
 template <typename T, int kDim, bool kRope>
 __global__ void __launch_bounds__(kPackThreads) packed_write_kernel(const __grid_constant__ PackWriteParams P) {
   constexpr int kPer = kDim / 16;  // threads of a row
@@ -159,7 +161,8 @@ struct PackReadParams {
   PackedSeq seq[kPackSeqs];
 };
 
-// kReadEach words of eight numbers a thread, of a head's tokens
+// kReadEach words of eight numbers a thread, of a head's tokens: their loads are all on their way before the first is used.
+// What bounds it: the numbers' bytes, 16 bits for 5 bits read.  8192 tokens of 32 heads of 128, keys and values: 176 MB in 29 us, 6.0 TB/s.
 constexpr int kReadThreads = 256, kReadEach = 4;
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __grid_constant__ PackReadParams P) {
@@ -198,6 +201,9 @@ __global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __gri
 // counts before it give; ties go to the earlier token.  Then the rows close up: a row's new place is never behind its old one,
 // so, in place, the blocks read kRound rows each, wait for each other, and write; what the next round reads lies behind all that
 // this one has written.
+// What bounds it: bytes, where sequences and layers are many (4 sequences of 2176 tokens, 32 layers, 8 KV heads of 128, 2048 stay: 705 MB
+// in and out, 140 us into other places, 5.0 TB/s, 116 in place); otherwise the chain of passes, lists and rows, some 15 us (8 sequences of
+// 4224, 2 layers, 2048 stay: 86 MB, 28 us; one of 65536, 4 layers, 4096 stay: 50 MB, 38 us).
 constexpr int kEvictThreads = 256, kRound = 256, kEach = 8;
 constexpr int kEvictRoom = 10240;  // weights a block: 40 KB, so that five have room on a multiprocessor
 

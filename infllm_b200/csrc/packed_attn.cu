@@ -51,6 +51,13 @@ __device__ __forceinline__ uint32_t ld_stream4(const char* p) {
 // four columns have the same rows again, and theirs is lo, in the same product.
 // The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled and do lanes exchange
 // anything.
+// What bounds it: the codes' bytes, and close behind them what is issued to take numbers out of them, 397 instructions a warp for 16 keys of
+// 128 (loads alone 138 us where the kernel takes 192; without the taking out 189).  One new token of 32 sequences of 24576 tokens, 32/8
+// heads of 128 in bf16: 1.007 GB in 192 us, 5.24 TB/s; of one sequence of 131072, 168 MB in 39 us.  What brought it there from 389: loads of
+// the next 16 keys under this one's products, two copies of a turn so that their registers stay where they are, Q in shared memory (four
+// blocks a multiprocessor by registers), keys as rows of S^T so that a thread's codes have one (m, s), and addresses that run.  Tried, and
+// slower: 32 keys at a time (the kernel of then 291 instead of 286), five blocks a multiprocessor (324), lines asked for into L2 ahead
+// (275, 265), shifts and differences instead of the masks of packed.cuh (a tenth more).
 template <typename T, int kDim, bool kFour>
 struct PackedRows {
   static constexpr int kW = kDim / 32;  // words of a key, kDim / 4 numbers, that a thread has: as many of Q's 16-byte pieces
@@ -659,7 +666,7 @@ int many_units(const infllm_packed* c, const infllm_packed_seq* seqs, PackedTcPa
 }
 
 // Bytes of the image of a launch's tiles, 0 where numbers are taken out of their codes by the blocks themselves: with an image a tile of 256
-// rows takes 1.8 us instead of 2.4, and to make one takes 0.013 us a tile of the machine's time; so it pays from about four blocks of rows
+// rows takes 2.2 us instead of 2.45, and to make one takes 0.013 us a tile of the machine's time; so it pays from about four blocks of rows
 // to a tile on.  Not beyond a gigabyte, as a cache in 4 bits is there for want of memory.
 int64_t image_bytes(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group) {
   int64_t tiles = 0, blocks = 0;

@@ -7,12 +7,17 @@
 // with one team that, not its bytes, would be a tile's time.)
 // Six more warps bring codes from global memory through registers, and leave 16-bit numbers, swizzled as the products want them, in a
 // ring of tiles in the order K0 K1 V0 K2 V1 ..; both teams' products read the same tile, so that it is taken out once for 256 rows.
-// (Eight warps, with softmax in pieces of 16 columns to do with 96 registers: of 48 rows 4 % less, of 192 rows 8 % more.)  Prompts'
+// (Eight of them, with softmax in pieces of 16 columns to do with 96 registers: of 48 rows 4 % less, of 192 rows 8 % more.)  Prompts'
 // tiles, which many blocks of rows read, are taken out once for all of them by a kernel before, and fetched by one warp.
 // Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A operand of P V from there, have 128
 // columns, O another 128.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
 // P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.
 // Sums, O and partial rows are fp32.
+// What bounds it: the softmax warps' chain (scores out of TMEM, maximum, exponentials, P back) between two products of its team, with six code
+// warps beside it for issue.  2048 tokens behind 28000, 32/8 heads of 128 in bf16: 895 us with the image, 2.2 us for a tile of 256 rows by
+// 128 keys (products alone, with P as it lies there, 1.63; as fast as they can be issued, 1.1 to 1.2), 963 without.  48 tokens of 8
+// sequences of 12288 (192 rows of 8 KV heads) 124 us, 12 tokens (48 rows) 77.
+// Tried: 4, 7, 8, 10, 12, 14 and 16 code warps; registers given from warpgroup to warpgroup with 28 warps (five times slower: spills).
 #include <atomic>
 
 #include "attn_tc.cuh"

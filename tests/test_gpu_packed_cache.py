@@ -195,6 +195,23 @@ def test_a_group_that_is_not_finite_is_none(dtype):
     assert torch.equal(got.nan_to_num(-9).double(), want.nan_to_num(-9))
 
 
+@pytest.mark.parametrize("least", [0.0, -7.0, -15.0])
+def test_the_widest_steps(least):
+    """bf16: groups in steps of 2^121 and of the largest number below 2^122 are held, one of 2^122 and one that is wider (of least -7: its span is not finite) are not."""
+    c = make(1, 128, 1, 16)
+    b = c.batch(c.open())
+    b.extend(1)
+    code = torch.arange(32, device="cuda", dtype=torch.float64) % 16
+    steps = torch.tensor([2.0 ** 121, 2.0 ** 122 * (1 - 2.0 ** -8), 2.0 ** 122, 2.0 ** 125], device="cuda", dtype=torch.float64)
+    k = (steps[:, None] * (code + least)).clamp(-3.3e38, 3.3e38).to(torch.bfloat16).view(1, 1, 1, 128)
+    b.write(0, k, torch.zeros_like(k))
+    got = b.values(0)[0].view(4, 32)
+    assert got[2:].isnan().all() and c.scales[0, 0, 0, 0, 0, 2:, 1].isnan().all()
+    codes, low, step = pack64(k)
+    want = stand64(codes, low, step, torch.bfloat16).view(4, 32)[:2]
+    assert (step.view(4)[:2] < 2.0 ** 122).all() and torch.equal(got[:2].double(), want)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_every_code_and_the_borders_between_them(dtype):
     """Groups from a to b in steps of (b - a) / 15, and numbers half way between two codes."""
