@@ -292,6 +292,16 @@ def raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
+def capturing(device):
+    """Whether a device's current stream is being captured into a CUDA graph."""
+    import torch
+
+    if torch.cuda.current_device() == device.index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def stream_ptr(device=None):
     import torch
 

@@ -18,7 +18,8 @@ numbers is not finite, or where the step is not, or in bf16 is 2^122 or more, no
 Tensors are (batch, heads, tokens, head_dim) views with any strides whose rows are 16-byte aligned, as the other attention types take
 them.  Work goes to the current stream; all calls on a cache belong on one stream, or are ordered by the caller.  Inside a CUDA
 graph's capture, write, attend, values and evict are launches like others: a replay does them again for the lengths of the
-capture, while extend, retract and what evict does to lengths happen on the host, once."""
+capture, while extend, retract and what evict does to lengths happen on the host, once.  A graph reads the cache's tensors and, of
+a write with `rope`, the tables of positions that were there, which the cache keeps for it."""
 import ctypes
 import math
 from array import array
@@ -63,6 +64,7 @@ class PackedCache:
         self._c = _lib.Packed(self.n_layers, self.n_kv_heads, self.head_dim, self.n_sequences, self.max_tokens, code, self.device.index, 0,
                               self.codes.data_ptr(), self.scales.data_ptr(), self.weights.data_ptr(), self.places.data_ptr())
         self._ref = ctypes.byref(self._c)
+        self._captured = []  # rotary tables that captured writes read
         self._begin()
 
     def _begin(self):
@@ -266,8 +268,13 @@ class PackedBatch:
         if rope is not None:
             if not isinstance(rope, RotaryEmbeddingESM) or rope.dim != c.head_dim:
                 raise ValueError(f"rope must be a RotaryEmbeddingESM of {c.head_dim} dimensions")
-            cos, sin = rope._tables(max(self._info[1], 1), c.device)
-            rows, cos, sin = cos.size(0), cos.data_ptr(), sin.data_ptr()
+            need, captured = max(self._info[1], 1), _lib.capturing(c.device)
+            if captured and (rope._cos is None or rope._cos.device != c.device or need > rope._seq_len_cached):
+                raise RuntimeError(f"a rotary table of {need} positions is not there, and is not made inside a capture: write once outside of it")
+            tables = rope._tables(need, c.device)
+            if captured and all(x[0] is not tables[0] for x in c._captured):
+                c._captured.append(tables)  # (the graph goes on reading these, also when longer ones have taken their place)
+            rows, cos, sin = tables[0].size(0), tables[0].data_ptr(), tables[1].data_ptr()
         rc = _lib_call.infllm_packed_write(c._ref, layer, self._table, self._n, self.tokens, k_at, k_bs, k_hs, k_ts, v_at, v_bs, v_hs, v_ts,
                                            q_at, q_bs, q_hs, q_ts, at, heads, cos, sin, rows, _lib.raw_stream(c.device))
         if rc:

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
     __syncwarp();
   } else if (!kImage && warp >= kWarpCodes && warp < kWarpMma) {
     // ======================================================================================================== numbers
-    // Eight warps take key tiles, eight value tiles.  A thread has the 32 numbers of one (m, s), a 16-byte piece of a row of codes, of
+    // Half of the warps take key tiles, half value tiles.  A thread has the 32 numbers of one (m, s), a 16-byte piece of a row of codes, of
     // kPer rows; the next tile's are on their way through registers while it is at work, those kAhead tiles ahead to L2.
     // (Eight lanes that write 16 bytes at a time have four rows and pieces of one half of them: eight different bank groups.)
     using C = Codes<T>;

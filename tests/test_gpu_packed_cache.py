@@ -586,6 +586,36 @@ def test_a_captured_step_is_replayed(n):
         assert torch.equal(x.double().nan_to_num(-3), y.double().nan_to_num(-3))
 
 
+def test_tables_that_a_captured_write_reads():
+    """They are not made inside a capture, and stay when longer ones have taken their place."""
+    from infllm_b200.attention import RotaryEmbeddingESM
+
+    g, rope = gen(18), RotaryEmbeddingESM(128, 1e4, 1.0)
+    c = make(1, 128, 1, 200)
+    b = c.batch(c.open())
+    b.extend(20)
+    k, v = (rand(g, 1, 1, 20, 128) for _ in range(2))
+    with pytest.raises(RuntimeError, match="inside a capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            b.write(0, k, v, rope=rope)
+    assert c.scales.isnan().all() and rope._cos is None
+    b.write(0, k, v, rope=rope)
+    want = c.codes.clone(), c.scales.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.write(0, k, v, rope=rope)
+        b.write(0, k, v, rope=rope)
+    assert len(c._captured) == 1
+    shape = rope._cos.shape
+    rope._tables(5000, c.device)
+    over = [torch.full(shape, NAN, device="cuda") for _ in range(20)]  # (memory that was given back would be theirs)
+    c.codes.fill_(-1)
+    c.scales.fill_(NAN)
+    graph.replay()
+    assert torch.equal(c.codes[:, :, :, :, :20], want[0][:, :, :, :, :20]) and torch.equal(c.scales[:, :, :, :, :20], want[1][:, :, :, :, :20])
+    assert all(x.isnan().all() for x in over)
+
+
 def test_many_sequences_in_one_call():
     g = gen(15)
     c = make(1, 64, 300, 40, layers=1)
