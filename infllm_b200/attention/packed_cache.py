@@ -287,10 +287,14 @@ class PackedBatch:
         c = self.cache
         self._layer(0 if layer is None else layer)
         first, n = (0, c.n_layers) if layer is None else (layer, 1)
-        k, v = (torch.empty((n, self._n, c.n_kv_heads, self.tokens, c.head_dim), dtype=c.dtype, device=c.device) for _ in range(2))
+        size = (self._n, c.n_kv_heads, self.tokens, c.head_dim)
+        if layer is None:
+            size = (n, *size)
+        k = torch.empty(size, dtype=c.dtype, device=c.device)
+        v = torch.empty(size, dtype=c.dtype, device=c.device)
         _lib.check(_lib_call.infllm_packed_values(c._ref, first, n, self._table, self._n, self.tokens, k.data_ptr(), v.data_ptr(),
                                                   _lib.raw_stream(c.device)))
-        return (k, v) if layer is None else (k[0], v[0])
+        return k, v
 
     def attend(self, layer, q, scale=None, return_lse=False, weigh=False, decay=1.0):
         """Attention of the step's queries (batch, n_heads, tokens, head_dim) to their sequences' keys up to their own places.

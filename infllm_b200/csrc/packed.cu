@@ -46,9 +46,10 @@ __device__ __forceinline__ float2 span32(const uint4& x, uint32_t quad) {
 
 // Eight numbers of a row as codes, and their group's (m, s).
 // A quotient of 16-bit numbers' differences lies on the border between two codes, or further from it than the last place in 32 bits: so
-// a rounded quotient has the definition's code.  q0 = t / s by the reciprocal is off by some last places, and q0 + (t - q0 s) / s, whose
-// remainder is exact, is the rounded quotient wherever that is a border: five operations a number instead of a division's
-// dozen, after which writes are bound by their bytes.
+// a rounded quotient has the definition's code.  1 / s as the sum of two numbers, of which the second is what the first leaves (1 - inv s is
+// exact), is right to 2^-46; so t inv + t rest, rounded once, is the border wherever the quotient is one: three operations a number, with the
+// rounding to a whole one, instead of a division's dozen.  Steps at the ends of the range, where the reciprocal or what it leaves is
+// no normal number, or fp16's steps of less than 16 of its least ones, where a quotient may be above 15.5, are divided by.
 template <typename T>
 __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_t* ms) {
   const float2 span = span32<T>(x, quad);
@@ -62,7 +63,7 @@ __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_
   const typename Act<T>::T2* p = reinterpret_cast<const typename Act<T>::T2*>(&x);
   uint32_t w = 0;
   if (!held) return 0;
-  if (s < 0x1p-100f) {  // (0, or so small that its reciprocal is not one)
+  if (s < (Codes<T>::kBf16 ? 0x1p-100f : 0x1p-20f) || s > 0x1p90f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 f = Act<T>::to_f2(p[i >> 1]);
@@ -71,14 +72,14 @@ __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_
     }
     return w;
   }
-  const float inv = __frcp_rn(s);
+  const float inv = __frcp_rn(s), rest = fmaf(-inv, s, 1.f) * inv;
   constexpr float kMagic = 8388608.f;  // 2^23: what is added to it is rounded to a whole number, ties to even, in its low bits
   constexpr uint32_t kMagicBits = 0x4b000000u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 f = Act<T>::to_f2(p[i >> 1]);
-    const float t = (i & 1 ? f.y : f.x) - span.x, q0 = t * inv, q = fmaf(fmaf(-q0, s, t), inv, q0);
-    w += (__float_as_uint(fminf(q, 15.f) + kMagic) - kMagicBits) << (4 * (i >> 1) + 16 * (i & 1));
+    const float t = (i & 1 ? f.y : f.x) - span.x, q = fmaf(t, inv, t * rest);
+    w += (__float_as_uint(q + kMagic) - kMagicBits) << (4 * (i >> 1) + 16 * (i & 1));
   }
   return w;
 }
@@ -196,8 +197,8 @@ __global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __gri
 
 // ---------------------------------------------------------------------------------------------------------- eviction
 // Of a head's n tokens the first `sink`, the newest `recent` and the k of largest weight between them stay.  A cluster of blocks
-// has a head: the k-th largest weight by its digits of 8 bits from the top (four passes over the weights, whose counts the blocks add
-// up through each other's shared memory), then each block lists which of its share of tokens stay, at the rank that the
+// has a head: the k-th largest weight by its digits of 8 bits from the top (four passes over the weights, whose counts the blocks
+// add up through each other's shared memory: with digits of 11 bits that takes longer than the pass that they spare), then each block lists which of its share of tokens stay, at the rank that the
 // counts before it give; ties go to the earlier token.  Then the rows close up: a row's new place is never behind its old one,
 // so, in place, the blocks read kRound rows each, wait for each other, and write; what the next round reads lies behind all that
 // this one has written.
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __gri
 // in and out, 140 us into other places, 5.0 TB/s, 116 in place); otherwise the chain of passes, lists and rows, some 15 us (8 sequences of
 // 4224, 2 layers, 2048 stay: 86 MB, 28 us; one of 65536, 4 layers, 4096 stay: 50 MB, 38 us).
 constexpr int kEvictThreads = 256, kRound = 256, kEach = 8;
-constexpr int kEvictRoom = 10240;  // weights a block: 40 KB, so that five have room on a multiprocessor
+constexpr int kEvictRoom = 10240;  // weights a block: 40 KB, so that four blocks have room on a multiprocessor
+constexpr int kCounts = 4, kPitch = 256 + 8;  // counts of a digit, by lanes: weights of like size have few first digits, and wait for each other
 
 struct EvictParams {
   PackedPlanes at;
@@ -228,7 +230,7 @@ __device__ __forceinline__ uint32_t weight_rank(float w) {
 }
 
 template <int kDim>
-__global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __grid_constant__ EvictParams P) {
+__global__ void __launch_bounds__(kEvictThreads, 4) packed_evict_kernel(const __grid_constant__ EvictParams P) {
   cg::cluster_group cluster = cg::this_cluster();
   const int n_ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.x / n_ctas, b = blockIdx.y, layer = blockIdx.z;
@@ -239,30 +241,40 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
   const int64_t from = P.at.row0(slot, h), to = P.copy ? P.at.row0(P.into[b], h) : from;
   const float* weights = P.weights + layer * P.rows_layer + from;
   int32_t* stay = P.stay + (((int64_t)layer * P.n_seqs + P.seq0 + b) * P.at.n_kv + h) * P.most_stay;
-  __shared__ int hist[2][256], total[256], counts[2], warps[2][kEvictThreads / 32], found[2], src[kRound];
+  __shared__ int hist[2][256], part[kCounts][kPitch], total[kEvictThreads / 32], counts[2], warps[2][kEvictThreads / 32], found[2], src[kRound];
 
   const bool choose = !all && k > 0;
   if (choose) {
     const int share = (late - sink + n_ctas - 1) / n_ctas, first = sink + min(me * share, late - sink), last = min(first + share, late);
-    // The share's weights, as whole numbers, in shared memory as far as there is room; the others are read again each time
-    extern __shared__ uint32_t ranks[];
-    const int room = P.room;
+    // The share's weights, as whole numbers, in shared memory as far as there is room, up to a multiple of 8 with zeros, which are less than
+    // any weight's; the others are read again each time
+    extern __shared__ __align__(16) uint32_t ranks[];
+    const int held = min(last - first, P.room), beyond = first + held;
 #pragma unroll 8
-    for (int j = first + tid; j < min(last, first + room); j += kEvictThreads) ranks[j - first] = weight_rank(weights[j]);
-    auto rank_of = [&](int j) { return j - first < room ? ranks[j - first] : weight_rank(weights[j]); };
-    __syncthreads();
+    for (int j = tid; j < held; j += kEvictThreads) ranks[j] = weight_rank(weights[first + j]);
+    if (tid < (-held & 7)) ranks[held + tid] = 0;
+    auto each = [&](auto&& f) {
+#pragma unroll 2
+      for (int v = tid; v < (held + 3) / 4; v += kEvictThreads) {
+        const uint4 u = reinterpret_cast<const uint4*>(ranks)[v];
+        f(u.x), f(u.y), f(u.z), f(u.w);
+      }
+      for (int j = beyond + tid; j < last; j += kEvictThreads) f(weight_rank(weights[j]));
+    };
     uint32_t cut = 0;
     int need = k;
 #pragma unroll 1
     for (int pass = 0; pass < 4; ++pass) {
       const int shift = 24 - 8 * pass;
       int* mine = hist[pass & 1];
-      mine[tid] = 0;
+#pragma unroll
+      for (int x = 0; x < kCounts; ++x) part[x][tid] = 0;
       __syncthreads();
-      for (int j = first + tid; j < last; j += kEvictThreads) {
-        const uint32_t u = rank_of(j);
-        if (pass == 0 || (u ^ cut) >> (shift + 8) == 0) atomicAdd(&mine[u >> shift & 255], 1);
-      }
+      each([&](uint32_t u) {
+        if (pass == 0 || (u ^ cut) >> (shift + 8) == 0) atomicAdd(&part[lane % kCounts][u >> shift & 255], 1);
+      });
+      __syncthreads();
+      mine[tid] = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
       cluster.sync();  // (of the pass after the next, whose counts take this one's place, nobody is ahead of the next one's)
       int sum = 0;
 #pragma unroll
@@ -285,10 +297,7 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
     }
     // of the tokens of weight `cut` the first `need` stay
     int larger = 0, equal = 0;
-    for (int j = first + tid; j < last; j += kEvictThreads) {
-      const uint32_t u = rank_of(j);
-      larger += u > cut, equal += u == cut;
-    }
+    each([&](uint32_t u) { larger += u > cut, equal += u == cut; });
     larger = __reduce_add_sync(0xffffffffu, larger), equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) warps[0][warp] = larger, warps[1][warp] = equal;
     __syncthreads();
@@ -306,12 +315,19 @@ __global__ void __launch_bounds__(kEvictThreads) packed_evict_kernel(const __gri
 #pragma unroll 1
     for (int base = first; base < last; base += kEvictThreads * kEach) {
       const int j0 = base + tid * kEach;
-      uint32_t u[kEach];
+      alignas(16) uint32_t u[kEach];
       int g = 0, e = 0;
+      const int at = j0 - first;
+      if (at + kEach <= ((held + 7) & ~7)) {
+        *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(ranks + at);
+        *reinterpret_cast<uint4*>(u + 4) = *reinterpret_cast<const uint4*>(ranks + at + 4);
+      } else {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) u[x] = j0 + x < last ? weight_rank(weights[j0 + x]) : 0;
+      }
 #pragma unroll
       for (int x = 0; x < kEach; ++x) {
         const bool in = j0 + x < last;
-        u[x] = in ? rank_of(j0 + x) : 0;
         g += in && u[x] > cut, e += in && u[x] == cut;
       }
       int sg = g, se = e;
@@ -547,7 +563,7 @@ extern "C" int infllm_packed_evict(const infllm_packed* c, const infllm_packed_s
       const int64_t heads = (int64_t)c->n_layers * m * c->n_kv_heads;
       int ctas = 8;
       while (ctas > 1 && heads * ctas > 148 * 4) ctas /= 2;
-      P.room = (int32_t)std::min<int64_t>(ceil_div(longest, ctas), kEvictRoom);
+      P.room = (int32_t)std::min<int64_t>(ceil_div(ceil_div(longest, ctas), kEach) * kEach, kEvictRoom);
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)(c->n_kv_heads * ctas), m, c->n_layers);
       cfg.blockDim = dim3(kEvictThreads);
@@ -557,8 +573,8 @@ extern "C" int infllm_packed_evict(const infllm_packed* c, const infllm_packed_s
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim = {(unsigned)ctas, 1, 1};
       cfg.attrs = at, cfg.numAttrs = 1;
-      if (c->head_dim == 128) INFLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, packed_evict_kernel<128>, P));
-      else INFLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, packed_evict_kernel<64>, P));
+      auto kern = c->head_dim == 128 ? packed_evict_kernel<128> : packed_evict_kernel<64>;
+      INFLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, P));
       INFLLM_LAUNCH_OK("packed_evict_kernel");
     }
     return INFLLM_OK;

@@ -461,6 +461,27 @@ def test_evict(dim, kv, dtype, layers, lengths, budget, sink, recent, into, ties
 
 
 # ------------------------------------------------------------------------------------------------- a run of them together
+@pytest.mark.parametrize("n,kv,budget,sink,recent", [(20011, 600, 9001, 3, 100), (9999, 601, 9990, 0, 0), (90001, 2, 45000, 0, 500), (30, 1, 29, 0, 0)])
+@pytest.mark.parametrize("values", ["normal", "lowest"])
+def test_evict_of_more_weights_than_a_block_has_room_for(n, kv, budget, sink, recent, values):
+    g = gen(19)
+    c = make(kv, 64, 1, n)
+    s = c.open()
+    c.batch(s).extend(n)
+    w = torch.randn((kv, n), generator=g, device="cuda").exp()
+    if values == "lowest":  # one half of them less than any other, and some the least number
+        w = torch.where(w < 1, -INF, torch.where(w < 1.5, -3.4028234663852886e38, w.round()))
+    c.weights[0, 0].copy_(w)
+    c.places[0, 0].copy_(torch.arange(n, dtype=torch.int32, device="cuda").expand(kv, n))
+    c.evict(s, budget, sink, recent)
+    k = budget - sink - recent
+    order = torch.sort(w[:, sink:n - recent], dim=1, descending=True, stable=True).indices[:, :k]  # (of equal ones the earlier)
+    want = torch.cat((torch.arange(sink, device="cuda").expand(kv, sink), order.sort(1).values + sink,
+                      torch.arange(n - recent, n, device="cuda").expand(kv, recent)), 1)
+    assert c.length(s[0]) == budget and torch.equal(c.places[0, 0, :, :budget].long(), want)
+    assert torch.equal(c.weights[0, 0, :, :budget], w.gather(1, want))
+
+
 @pytest.mark.parametrize("dim,kv,heads,dtype", SHAPES[:3])
 def test_a_generation_with_evictions(dim, kv, heads, dtype):
     """A prompt, decode steps, drafts that are taken back, evictions in between: every output and weight against the formulas over what the
