@@ -35,15 +35,17 @@ __device__ __forceinline__ float2 span32(const uint4& x, uint32_t quad) {
   const T2* p = reinterpret_cast<const T2*>(&x);
   const T2 lo = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
   const T2 hi = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
-  T a = __hmin_nan(lo.x, lo.y), b = __hmax_nan(hi.x, hi.y);
+  T2 ends = {__hmin_nan(lo.x, lo.y), __hneg(__hmax_nan(hi.x, hi.y))};  // (the largest as the least of the negatives)
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    a = __hmin_nan(a, __shfl_xor_sync(quad, a, o));
-    b = __hmax_nan(b, __shfl_xor_sync(quad, b, o));
-  }
-  return make_float2(Act<T>::to_f(a), Act<T>::to_f(b));
+  for (int o = 1; o < 4; o <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(quad, ends, o));
+  return make_float2(Act<T>::to_f(ends.x), -Act<T>::to_f(ends.y));
 }
 
+// a span's fifteenth, rounded once (below, its second term would be rounded to fewer bits)
+__device__ __forceinline__ float fifteenth(float span) {
+  constexpr float kHi = 1.f / 15.f, kLo = (float)(1. / 15. - (double)kHi);
+  return span < 0x1p-90f ? __fdiv_rn(span, 15.f) : fmaf(span, kHi, span * kLo);
+}
 // Eight numbers of a row as codes, and their group's (m, s).
 // A quotient of 16-bit numbers' differences lies on the border between two codes, or further from it than the last place in 32 bits: so
 // a rounded quotient has the definition's code.  1 / s as the sum of two numbers, of which the second is what the first leaves (1 - inv s is
@@ -53,7 +55,7 @@ __device__ __forceinline__ float2 span32(const uint4& x, uint32_t quad) {
 template <typename T>
 __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_t* ms) {
   const float2 span = span32<T>(x, quad);
-  T step = Act<T>::from_f(__fdiv_rn(span.y - span.x, 15.f));
+  T step = Act<T>::from_f(fifteenth(span.y - span.x));
   const T least = Act<T>::from_f(span.x);
   const float s = Act<T>::to_f(step);
   const bool held = s < (Codes<T>::kBf16 ? 0x1p122f : INFINITY);  // (not where one is not finite, either)
@@ -72,7 +74,9 @@ __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_
     }
     return w;
   }
-  const float inv = __frcp_rn(s), rest = fmaf(-inv, s, 1.f) * inv;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float rest = fmaf(-inv, s, 1.f) * inv;
   constexpr float kMagic = 8388608.f;  // 2^23: what is added to it is rounded to a whole number, ties to even, in its low bits
   constexpr uint32_t kMagicBits = 0x4b000000u;
 #pragma unroll
@@ -98,10 +102,12 @@ __device__ __forceinline__ void pack_rotate8(uint4& lo, uint4& hi, const float* 
 
 // A thread has 8 numbers of the first half of a row and the 8 that are rotated with them; the four threads of a group of 32 agree on
 // its least number and step.
-// What bounds it: bytes, and the arithmetic of codes beside them.  8192 tokens of 32 query and 32 KV heads of 128 in fp16, rotated, 310 MB
-// in and out, 58 to 69 us: 4.5 to 5.4 TB/s (with a division a number 77).  Of 64 single tokens, 3.6 us.
+// What bounds it: bytes, and the arithmetic of codes and angles beside them.  8192 tokens of 32 query and 32 KV heads of 128 in fp16, 310 MB in
+// and out: 73 us, 4.2 TB/s, in a row of calls; 63 without angles, 60 with no arithmetic for the codes.  From 85: three operations a number
+// instead of five, 83; one exchange for both ends of a group, and no division for the step, 80; the next row ahead, 75; eight blocks a
+// multiprocessor, 73 (ten: 77; blocks of 256: 96, of 64: 73).  Of 64 single tokens, 3.6 us.
 template <typename T, int kDim, bool kRope>
-__global__ void __launch_bounds__(kPackThreads) packed_write_kernel(const __grid_constant__ PackWriteParams P) {
+__global__ void __launch_bounds__(kPackThreads, 8) packed_write_kernel(const __grid_constant__ PackWriteParams P) {
   constexpr int kPer = kDim / 16;  // threads of a row
   const int n_kv = P.at.n_kv, n_rows = P.n_heads + 2 * n_kv, per = min(n_rows * kPer, kPackThreads);  // threads of a token
   const int sub = (int)threadIdx.x / per, of_token = (int)threadIdx.x - sub * per, token = (int)blockIdx.x * P.per_block + sub;
@@ -121,21 +127,23 @@ __global__ void __launch_bounds__(kPackThreads) packed_write_kernel(const __grid
       *reinterpret_cast<float4*>(sn + k) = __ldg(reinterpret_cast<const float4*>(P.sin_t + o + k));
     }
   }
+  // (the next row is on its way while one is worked on)
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo, lo1 = lo, hi1 = lo;  // (no token: its query is not one)
+  auto load = [&](int r, uint4& a, uint4& z) {
+    if (at < 0 || r >= n_rows) return;
+    const char* src = r < P.n_heads          ? P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts
+                      : r < P.n_heads + n_kv ? P.k + bb * P.k_bs + (r - P.n_heads) * P.k_hs + i * P.k_ts
+                                             : P.v + bb * P.v_bs + (r - P.n_heads - n_kv) * P.v_hs + i * P.v_ts;
+    a = *reinterpret_cast<const uint4*>(src + c * 16), z = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
+  };
+  load(of_token / kPer, lo1, hi1);
   for (int r = of_token / kPer; r < n_rows; r += per / kPer) {
     const bool val = r >= P.n_heads + n_kv;
     const int h = r - P.n_heads - (val ? n_kv : 0);
-    const char* src;
-    if (h < 0) {
-      src = P.q + bb * P.q_bs + r * P.q_hs + i * P.q_ts;
-    } else {
-      if (at < 0) return;  // (queries come first: nothing is left of this token)
-      src = val ? P.v + bb * P.v_bs + h * P.v_hs + i * P.v_ts : P.k + bb * P.k_bs + h * P.k_hs + i * P.k_ts;
-    }
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;  // (no token: its query is not one)
-    if (at >= 0) {
-      lo = *reinterpret_cast<const uint4*>(src + c * 16), hi = *reinterpret_cast<const uint4*>(src + kDim + c * 16);
-      if (kRope && !val) pack_rotate8<T>(lo, hi, cs, sn);
-    }
+    if (h >= 0 && at < 0) return;  // (queries come first: nothing is left of this token)
+    lo = lo1, hi = hi1;
+    load(r + per / kPer, lo1, hi1);
+    if (kRope && !val && at >= 0) pack_rotate8<T>(lo, hi, cs, sn);
     if (h < 0) {
       char* to = P.q_out + ((bb * P.most + i) * P.n_heads + r) * (int64_t)(kDim * 2);
       *reinterpret_cast<uint4*>(to + c * 16) = lo;
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(kReadThreads) packed_values_kernel(const __gri
 // this one has written.
 // What bounds it: bytes, where sequences and layers are many (4 sequences of 2176 tokens, 32 layers, 8 KV heads of 128, 2048 stay: 705 MB
 // in and out, 140 us into other places, 5.0 TB/s, 116 in place); otherwise the chain of passes, lists and rows, some 15 us (8 sequences of
-// 4224, 2 layers, 2048 stay: 86 MB, 28 us; one of 65536, 4 layers, 4096 stay: 50 MB, 38 us).
+// 4224, 2 layers, 2048 stay: 86 MB, 29 us; one of 65536, 4 layers, 4096 stay: 50 MB, 34 us, 38 with weights one by one and one count).
 constexpr int kEvictThreads = 256, kRound = 256, kEach = 8;
 constexpr int kEvictRoom = 10240;  // weights a block: 40 KB, so that four blocks have room on a multiprocessor
 constexpr int kCounts = 4, kPitch = 256 + 8;  // counts of a digit, by lanes: weights of like size have few first digits, and wait for each other
