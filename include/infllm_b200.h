@@ -612,8 +612,8 @@ int infllm_page_batch_attend(infllm_page_batch* b, int layer, const void* d_q, i
  * what attention has given it, by which infllm_packed_evict chooses who stays.
  *
  * Of each 32 neighbouring numbers x of a row, in the 16-bit type T: m = min x, s = T((max x - m) / 15), and of each x the code c, the
- * nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  It stands for T(m + s c).  A group with a number that is not finite,
- * or whose step is not, or in bf16 is 2^122 or more, is NaN.
+ * nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  It stands for T(m + s c).   Where T(m + 15 s) were infinite, s
+ * is the next smaller number of T.  A group with a number that is not finite, or whose step is not, or in bf16 is 2^122 or more, is NaN.
  *
  * The memory is the caller's, 16-byte aligned, and the library keeps nothing of its own:
  *   d_codes    (n_layers, 2: keys and values, n_sequences, n_kv_heads, max_tokens, head_dim / 8) 32-bit words; of a word's eight

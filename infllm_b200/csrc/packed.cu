@@ -57,6 +57,10 @@ __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_
   const float2 span = span32<T>(x, quad);
   T step = Act<T>::from_f(fifteenth(span.y - span.x));
   const T least = Act<T>::from_f(span.x);
+  // (bf16: s < 2^122 is too little for that)
+  if constexpr (!Codes<T>::kBf16) {
+    if (__hisinf(__hfma(step, __float2half(15.f), least)) && !__hisinf(step)) step = __ushort_as_half(__half_as_ushort(step) - 1);
+  }
   const float s = Act<T>::to_f(step);
   const bool held = s < (Codes<T>::kBf16 ? 0x1p122f : INFINITY);  // (not where one is not finite, either)
   if (!held) step = Act<T>::from_f(NAN);

@@ -1,7 +1,8 @@
 // A key/value cache in 4 bits (packed.cu, packed_attn.cu): what it holds, and how numbers come out of it.
 //
 // Of each 32 neighbouring numbers x of a row, in the cache's 16-bit type T: the least m, a step s = T((max x - m) / 15), and of each
-// number a code c = the nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  A number stands for T(m + s c): one fused
+// number a code c = the nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  (Where T(m + 15 s) were infinite, s is the next
+// smaller number of T: what the cache stands for is finite wherever m and s are.)  A number stands for T(m + s c): one fused
 // multiply-add in T, so every kernel has the same operands, whatever its tiles.
 // A word has eight codes, number 2i at bit 4i and number 2i + 1 at bit 16 + 4i: what a mask leaves are two neighbours, and the low or the high halves of two rows' words, put together, give pairs of the same number of both rows.
 #pragma once

@@ -42,7 +42,11 @@ def pack64(x):
     """codes (.., dim), least and step (.., dim / 32) of rows x (.., dim), from the definition."""
     y = x.double().unflatten(-1, (-1, 32))
     least = y.amin(-1)
-    step = ((y.amax(-1) - least) / 15).float().to(x.dtype).double()
+    step = ((y.amax(-1) - least) / 15).float().to(x.dtype)
+    if x.dtype == torch.float16:  # (the next smaller one where the largest number that the group stands for were infinite)
+        over = (least + 15 * step.double()).to(x.dtype).isinf() & step.isfinite()
+        step = torch.where(over, (step.view(torch.int16) - 1).view(x.dtype), step)
+    step = step.double()
     c = torch.round((y - least[..., None]) / step[..., None])
     c = torch.where(step[..., None] == 0, torch.zeros_like(c), c).clamp(0, 15)
     return c.flatten(-2).long(), least, step
@@ -193,6 +197,44 @@ def test_a_group_that_is_not_finite_is_none(dtype):
     codes, least, step = pack64(k)
     want = torch.where(want.isnan(), NAN, stand64(codes, least, step, dtype))
     assert torch.equal(got.nan_to_num(-9).double(), want.nan_to_num(-9))
+
+
+def test_finite_numbers_stay_finite():
+    """fp16 groups at the ends of its range, whose steps are rounded up: none of what they stand for is infinite."""
+    g = gen(20)
+    c = make(1, 128, 1, 600, torch.float16)
+    b = c.batch(c.open())
+    b.extend(600)
+    k = (torch.rand((1, 1, 600, 128), generator=g, device="cuda") * 65504).half()
+    k[0, 0, :300, ::32] = 65504
+    k[0, 0, :, 1::32] = (torch.rand((600, 4), generator=g, device="cuda") * 131008 - 65504).half()
+    k[0, 0, :2, 2::32] = torch.tensor([0.0, -65504.0], device="cuda").half()[:, None]
+    b.write(0, k, -k)
+    smaller = 0
+    for got, x in zip(b.values(0), (k, -k)):
+        codes, least, step = pack64(x)
+        want = stand64(codes, least, step, torch.float16)
+        assert want.isfinite().all() and torch.equal(got.double(), want)
+        plain = ((x.double().unflatten(-1, (-1, 32)).amax(-1) - least) / 15).float().half()
+        smaller += (plain.double() != step).sum().item()
+        assert ((want - x.double()).abs() <= step.repeat_interleave(32, -1) * (0.5 + 15 * U[torch.float16]) + U[torch.float16] * want.abs()).all()
+    assert smaller > 100  # (the rule is at work)
+
+
+@pytest.mark.parametrize("n", [2, 60])
+def test_large_values_do_not_reach_rows_that_do_not_see_them(n):
+    g = gen(21)
+    c = make(1, 128, 1, 300, torch.float16)
+    b = c.batch(c.open())
+    b.extend(150 + n)
+    k, v, q = (rand(g, 1, 1, x, 128, dtype=torch.float16) for x in (150 + n, 150 + n, n))
+    v[0, 0, -1, ::2] = 65504
+    v[0, 0, -1, 1::2] = 0
+    b.write(0, k, v)
+    b.plan(n)
+    out, lse = b.attend(0, q, return_lse=True)
+    assert out.isfinite().all()
+    check(c, b, [n], q, out, lse)
 
 
 @pytest.mark.parametrize("least", [0.0, -7.0, -15.0])
