@@ -57,11 +57,12 @@ __device__ __forceinline__ uint32_t pack8(const uint4& x, uint32_t quad, uint32_
   const float2 span = span32<T>(x, quad);
   T step = Act<T>::from_f(fifteenth(span.y - span.x));
   const T least = Act<T>::from_f(span.x);
-  // (bf16: s < 2^122 is too little for that)
+  float s = Act<T>::to_f(step);
+  // m + 15 s is 16 or more above the largest number, 65504, only where s was rounded up by more than 1, so from 4096 on.  (bf16: the largest
+  // s that is held, just below 2^122, is rounded by too little.)
   if constexpr (!Codes<T>::kBf16) {
-    if (__hisinf(__hfma(step, __float2half(15.f), least)) && !__hisinf(step)) step = __ushort_as_half(__half_as_ushort(step) - 1);
+    if (s >= 4096.f && __hisinf(__hfma(step, __float2half(15.f), least)) && !__hisinf(step)) step = __ushort_as_half(__half_as_ushort(step) - 1), s = Act<T>::to_f(step);
   }
-  const float s = Act<T>::to_f(step);
   const bool held = s < (Codes<T>::kBf16 ? 0x1p122f : INFINITY);  // (not where one is not finite, either)
   if (!held) step = Act<T>::from_f(NAN);
   const typename Act<T>::T2 pair = {least, step};
