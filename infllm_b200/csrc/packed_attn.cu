@@ -48,9 +48,11 @@ __device__ __forceinline__ uint32_t ld_stream4(const char* p) {
 //   O^T += V^T P^T    numbers of the values are rows: a thread's codes of a value are an eighth of it, and two keys' are paired as they
 //                     are taken out.  P^T is S^T's place with keys and rows exchanged: two 8 x 8 transpositions in the warp.
 // P is two 16-bit numbers, p = hi + lo, so that an output's only rounding is its own: where rows are no more than four (kFour), the other
-// four columns have the same rows again, and theirs is lo, in the same product.
-// The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled and do lanes exchange
-// anything.
+// four columns have the same rows again, and theirs is lo, in the same product.  In fp16, whose numbers end at 2^-24, lo is kept times
+// 2^11, as it is that much smaller than hi wherever hi has all its digits: the other four columns are scaled at the end; with more rows the
+// products of lo are formed apart and added, a multiplication and addition of O's numbers for 16 keys.  (In fp16 217 us where 215 without, below;
+// of eight rows, 16 sequences with 64/8 heads, 139 for 134.)
+// The reference of a row is lazy (packed_attn.cuh): only where it moves O is scaled and do lanes exchange anything.
 // What bounds it: the codes' bytes, and close behind them what is issued to take numbers out of them, 397 instructions a warp for 16 keys of
 // 128 (loads alone 138 us where the kernel takes 192; without the taking out 189).  One new token of 32 sequences of 24576 tokens, 32/8
 // heads of 128 in bf16: 1.007 GB in 192 us, 5.24 TB/s; of one sequence of 131072, 168 MB in 39 us.  What brought it there from 389: loads of
@@ -63,6 +65,9 @@ struct PackedRows {
   static constexpr int kW = kDim / 32;  // words of a key, kDim / 4 numbers, that a thread has: as many of Q's 16-byte pieces
   static constexpr int kH = kDim / 64;  // of a value, kDim / 8 numbers
   static constexpr int kRow = kDim / 2, kScales = kDim / 8, kTiles = 4 * kH;
+  static constexpr float kGrow = Reference<T>::kGrow, kBelow = Reference<T>::kBelow;
+  static constexpr bool kApart = !Reference<T>::kBf16;  // lo is kept times 2^11
+  static constexpr float kLo = kApart ? 2048.f : 1.f, kUnLo = 1.f / kLo;
   using C = Codes<T>;
   const uint4* qf;     // row g's pieces, in shared memory: [piece][lane].  (The registers are worth more than four loads a group.)
   int lim[2];          // keys that rows 2t and 2t + 1 see
@@ -189,13 +194,13 @@ struct PackedRows {
         if ((kAll || j0 + (e >> 1) * 8 + g < key1) && (!(e & 1) || two)) logits[(e & 1) * pitch + j0 + (e >> 1) * 8] = s[e] * scale_log2;
     }
     float mx[2] = {fmaxf(s[0], s[2]) * scale_log2, fmaxf(s[1], s[3]) * scale_log2};
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + kGrow || mx[1] > m[1] + kGrow)) {
       float al[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
-        const float mn = mx[e] > m[e] + 8.f ? mx[e] : m[e];
+        const float mn = mx[e] > m[e] + kGrow ? mx[e] - kBelow : m[e];
         al[e] = m[e] == -INFINITY ? 0.f : exp2f(m[e] - mn);
         m[e] = mn;
         l[e] *= al[e];
@@ -213,7 +218,7 @@ struct PackedRows {
       typename Act<T>::T2 h = Act<T>::from_f2(p[2 * e], p[2 * e + 1]);
       hi[e] = *reinterpret_cast<uint32_t*>(&h);
       const float2 f = Act<T>::to_f2(h);
-      lo[e] = pack2<T>(p[2 * e] - f.x, p[2 * e + 1] - f.y);
+      lo[e] = pack2<T>((p[2 * e] - f.x) * kLo, (p[2 * e + 1] - f.y) * kLo);
       if (kFour) hi[e] = t < 2 ? hi[e] : lo[e];
       hi[e] = transposed(hi[e]);
       if (!kFour) lo[e] = transposed(lo[e]);
@@ -232,7 +237,13 @@ struct PackedRows {
       for (int i = 0; i < 4; ++i) {
         const uint32_t a[4] = {e01[i], o01[i], e23[i], o23[i]};
         mma16816<T>(ot[j * 4 + i], a, hi[0], hi[1]);
-        if (!kFour) mma16816<T>(ot[j * 4 + i], a, lo[0], lo[1]);
+        if (!kFour && !kApart) mma16816<T>(ot[j * 4 + i], a, lo[0], lo[1]);
+        if (!kFour && kApart) {
+          float z[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816<T>(z, a, lo[0], lo[1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ot[j * 4 + i][e] = fmaf(z[e], kUnLo, ot[j * 4 + i][e]);
+        }
       }
     }
   }
@@ -335,8 +346,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
       for (int y = 0; y < kAttnWarps; ++y) {
         const float wt = exp2f(sm_m[y][r] - mx);
         den = fmaf(wt, sm_l[y][r], den);
-        n0 = fmaf(wt, kFour ? sm_o[y][r][d] + sm_o[y][r + 4][d] : sm_o[y][r][d], n0);
-        n1 = fmaf(wt, kFour ? sm_o[y][r][d + 1] + sm_o[y][r + 4][d + 1] : sm_o[y][r][d + 1], n1);
+        n0 = fmaf(wt, kFour ? fmaf(sm_o[y][r + 4][d], R::kUnLo, sm_o[y][r][d]) : sm_o[y][r][d], n0);
+        n1 = fmaf(wt, kFour ? fmaf(sm_o[y][r + 4][d + 1], R::kUnLo, sm_o[y][r][d + 1]) : sm_o[y][r][d + 1], n1);
       }
       n0 /= den, n1 /= den;
     }

@@ -8,6 +8,16 @@ constexpr int kAttnSeqs = 128;  // of a launch
 constexpr int kBlockRows = 256, kKeyTile = 128;  // of the tensor-core kernels
 constexpr int kMaxSms = 160;
 
+// The reference of a row's exponentials, p = 2^(s - reference), is lazy: it moves where the maximum is more than kGrow above it, to kBelow under
+// the maximum, so that p is 2^kGrow at most, and the largest 2^kBelow or more.  fp16 has no numbers below 2^-24, and only a few digits
+// below 2^-14: its reference is as low as its largest numbers allow, or what many keys together have beside one (a first token that
+// takes nearly all attention) would be lost from the products and not from the sums.
+template <typename T>
+struct Reference {
+  static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr float kGrow = kBf16 ? 8.f : 15.f, kBelow = kBf16 ? 0.f : 11.f;
+};
+
 struct PackedAttnSeq {
   int32_t slot, length, count;
   int32_t unit0;   // its first unit of work, and how they follow from there:

@@ -10,8 +10,9 @@
 // (Eight of them, with softmax in pieces of 16 columns to do with 96 registers: of 48 rows 4 % less, of 192 rows 8 % more.)  Prompts'
 // tiles, which many blocks of rows read, are taken out once for all of them by a kernel before, and fetched by one warp.
 // Another warp issues the products.  S of a team and its P, which takes S's place in TMEM and is the A operand of P V from there, have 128
-// columns, O another 128.  The reference maximum of a row is lazy: it moves when the maximum has grown by 2^8, and only then O is scaled.
-// P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.
+// columns, O another 128.  The reference of a row is lazy (packed_attn.cuh): only where it moves O is scaled.
+// P is one 16-bit number: the A operand is 16 bits, and a second one for what is left over would be half as many products again.  (bf16: off by
+// up to 2^-8 of itself.  fp16: by 2^-11 of itself, and where it is less than 2^-25 of its row's largest, by up to 2^-36 of that.)
 // Sums, O and partial rows are fp32.
 // What bounds it: the softmax warps' chain (scores out of TMEM, maximum, exponentials, P back) between two products of its team, with six code
 // warps beside it for issue.  2048 tokens behind 28000, 32/8 heads of 128 in bf16: 895 us with the image, 2.2 us for a tile of 256 rows by
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
           max_chunk(s, mx);
         }
         const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * P.a.scale_log2;
-        const float mn = mt - m > 8.f ? mt : m;  // (from -inf: any number)
+        const float mn = mt - m > Reference<T>::kGrow ? mt - Reference<T>::kBelow : m;  // (from -inf: any number)
         const float alpha = m == -INFINITY ? 1.f : ex2_approx(m - mn);
         const bool scale_o = __any_sync(0xffffffffu, mn != m && m != -INFINITY) && x > 0;
         l *= alpha;

@@ -1,0 +1,39 @@
+"""PackedCache where numbers are at the ends of their types, or are none.  Tolerances as in test_gpu_packed_cache.py, but for what a test says itself."""
+import math
+
+import pytest
+import torch
+from test_gpu_packed_cache import INF, NAN, SHAPES, TINY, U, check, fill, formula, gen, held, make, rand
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.float16), (64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("group,n", [(1, 1), (4, 1), (4, 2), (7, 1), (4, 20), (4, 70), (4, 300)])
+@pytest.mark.parametrize("below,spread", [(11.0, 0.0), (15.0, 0.0), (17.0, 0.3), (18.0, 0.0)])
+def test_many_small_probabilities_beside_a_large_one(dim, dtype, group, n, below, spread):
+    """A token whose value is zero has nearly all of the attention; the output is what 8192 others, `below` nats less, have left.  (64
+    sequences, all the same, so that a unit of work has long stretches of them.)
+
+    Up to eight rows probabilities are as good as 32 bits, so that of the sum of p |v| only what is held in 32 bits is lost.  Of more rows each is
+    rounded to 16 bits: by u of itself, or, where an fp16 number has less bits, by half of 2^-24 in units of which the largest has
+    2^11 or more: N 2^-36 max |v| in all."""
+    g, length, kv, seqs = gen(31), 8193, 8, 64 if n < 100 else 8
+    c = make(kv, dim, seqs, length, dtype)
+    b = c.batch(c.open(seqs))
+    b.extend(length)
+    k = rand(g, 1, 1, length, dim, dtype=dtype, scale=spread)
+    v = (1 + 0.25 * torch.randn((1, 1, length, dim), generator=g, device="cuda")).to(dtype)
+    k[0, 0, 0], v[0, 0, 0] = below / math.sqrt(dim), 0
+    b.write(0, k.expand(seqs, kv, -1, -1), v.expand(seqs, kv, -1, -1))
+    b.plan(n)
+    out, lse = b.attend(0, torch.ones((seqs, kv * group, n, dim), dtype=dtype, device="cuda"), return_lse=True)
+    k, v = (x[-1:] for x in held(c, 0, seqs - 1))
+    want, mass, want_lse, p, e = formula(torch.ones((group, n, dim), device="cuda"), k, v, n, 1 / math.sqrt(dim))
+    few = group * n <= 8
+    tol = U[dtype] * want.abs() + ((0 if few else U[dtype]) + 2.0 ** -16 + 2 * e[..., None]) * mass + TINY[dtype]
+    if not few and dtype == torch.float16:
+        tol = tol + length * 2.0 ** -36 * v.abs().max()
+    err = (out[-1, -group:].double() - want).abs()
+    assert (err <= tol).all(), ((err / tol).max().item(), (err / want.abs()).max().item())
+    assert ((lse[-1, -group:].double() - want_lse).abs() <= e + 2.0 ** -20 * want_lse.abs() + 1e-6).all()
