@@ -467,8 +467,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
           tmem_wait_ld32(us);
         }
         const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
-        const float sum = r.x + r.y;
-        l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
+        l += r.x + r.y;
         if (scale_o) {
           // O has the products up to the tile before: wait for the last of them
           ok = warp_wait(bar(PV_DONE0 + team), (ns[team] + x - 1) & 1, abort_flag, err, 771);

@@ -372,8 +372,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) paged_tc_kernel(const __grid
           tmem_wait_ld32(us);
         }
         const float2 r = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
-        const float sum = r.x + r.y;
-        l += m == -INFINITY && sum < 1.f ? 0.f : sum;  // (the polynomial leaves 2^-126 of a masked key; a NaN stays one)
+        l += r.x + r.y;
         if (scale_o) {
           // O has the products up to the tile before: wait for the last of them
           const int pb = channel(now.two, team, i - 1);

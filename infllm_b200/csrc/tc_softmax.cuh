@@ -71,7 +71,8 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
 // exp2 of a pair on the FMA and integer pipes (the special-function unit does 16 per clock per SM, which bounds the
 // softmax when every exponential goes there): x = n + f with n the nearest integer (magic-number rounding) and f in
 // [-0.5, 0.5], 2^f by a polynomial whose relative error was minimised over that interval (least squares on Chebyshev
-// points), times 2^n.  A NaN stays one; arguments below -126, those of masked keys too, give 2^-126.
+// points), times 2^n.  A NaN stays one; arguments below -126.5, those of masked keys too, give 0: their n is -127, whose
+// power of two is made of no bits.  (Not 2^-126: a bf16 P has that number, and a value of 2^120 that a row does not see would reach it.)
 //   cubic    7.5e-5: a twentieth of the rounding of a bf16 P, a third to a sixth of that of an fp16 P
 //   quartic  2.6e-6
 //   quintic  2e-7 as evaluated in fp32, which is what ex2.approx has: where exp2f was
@@ -83,8 +84,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 template <int kDegree>
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   static_assert(kDegree >= 3 && kDegree <= 5, "");
-  x.x = max_nan(x.x, -126.f);
-  x.y = max_nan(x.y, -126.f);
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
   const float2 magic = make_float2(12582912.f, 12582912.f), neg_magic = make_float2(-12582912.f, -12582912.f);
   const float2 t = fadd2(x, magic);
   const float2 n = fadd2(t, neg_magic);

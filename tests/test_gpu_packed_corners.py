@@ -37,3 +37,43 @@ def test_many_small_probabilities_beside_a_large_one(dim, dtype, group, n, below
     err = (out[-1, -group:].double() - want).abs()
     assert (err <= tol).all(), ((err / tol).max().item(), (err / want.abs()).max().item())
     assert ((lse[-1, -group:].double() - want_lse).abs() <= e + 2.0 ** -20 * want_lse.abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("dim,kv,heads,dtype", [x for x in SHAPES if x[3] == torch.bfloat16])
+@pytest.mark.parametrize("length,n", [(150, 2), (150, 12), (250, 60), (900, 700), (9000, 40)])
+def test_the_largest_values_do_not_reach_rows_that_do_not_see_them(dim, kv, heads, dtype, length, n):
+    g, hidden = gen(33), n // 2
+    c = make(kv, dim, 1, length, dtype)
+    b = c.batch(c.open())
+    k, v = (rand(g, 1, kv, length, dim, dtype=dtype) for _ in range(2))
+    q = rand(g, 1, heads, n, dim, dtype=dtype)
+    b.extend(length)
+    got = []
+    for large in (0.0, 2.0 ** 120):
+        v[:, :, length - hidden:] = large
+        b.plan(length)
+        b.write(0, k, v)
+        b.plan(n)
+        got.append(b.attend(0, q)[:, :, :n - hidden])
+    assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("prefix,n", [(700, 40), (0, 2000), (9000, 300)])
+def test_the_largest_values_of_pages_do_not_reach_rows_that_do_not_see_them(prefix, n):
+    """The same of the paged cache."""
+    from infllm_b200.attention import PagedCache
+
+    g, hidden = gen(35), n // 2
+    c = PagedCache(1, 2, 128, 150, page_size=64)
+    b = c.batch(c.open())
+    b.extend(prefix + n)
+    k, v = (rand(g, 1, 2, prefix + n, 128) for _ in range(2))
+    q = rand(g, 1, 8, n, 128)
+    got = []
+    for large in (0.0, 2.0 ** 120):
+        v[:, :, prefix + n - hidden:] = large
+        b.plan(prefix + n)
+        b.write(0, k, v)
+        b.plan(n)
+        got.append(b.attend(0, q)[:, :, :n - hidden])
+    assert torch.equal(*got)
