@@ -68,6 +68,9 @@ struct PackedRows {
   static constexpr float kGrow = Reference<T>::kGrow, kBelow = Reference<T>::kBelow;
   static constexpr bool kApart = !Reference<T>::kBf16;  // lo is kept times 2^11
   static constexpr float kLo = kApart ? 2048.f : 1.f, kUnLo = 1.f / kLo;
+  // the reference before there is one: any score that fits 32 bits is above it, and what a row does not see, or does not fit, -inf, is a
+  // probability of 0 beside it
+  static constexpr float kNone = -FLT_MAX;
   using C = Codes<T>;
   const uint4* qf;     // row g's pieces, in shared memory: [piece][lane].  (The registers are worth more than four loads a group.)
   int lim[2];          // keys that rows 2t and 2t + 1 see
@@ -149,7 +152,7 @@ struct PackedRows {
   };
 
   __device__ __forceinline__ void clear() {
-    m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
+    m[0] = m[1] = kNone, l[0] = l[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) ot[i][0] = ot[i][1] = ot[i][2] = ot[i][3] = 0.f;
   }
@@ -201,15 +204,14 @@ struct PackedRows {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
         const float mn = mx[e] > m[e] + kGrow ? mx[e] - kBelow : m[e];
-        al[e] = m[e] == -INFINITY ? 0.f : exp2f(m[e] - mn);
+        al[e] = exp2f(m[e] - mn);
         m[e] = mn;
         l[e] *= al[e];
       }
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) ot[i][0] *= al[0], ot[i][1] *= al[1], ot[i][2] *= al[0], ot[i][3] *= al[1];
     }
-    const float r0 = !kAll && m[0] == -INFINITY ? 0.f : -m[0], r1 = !kAll && m[1] == -INFINITY ? 0.f : -m[1];
-    const float p[4] = {ex2(fmaf(s[0], scale_log2, r0)), ex2(fmaf(s[1], scale_log2, r1)), ex2(fmaf(s[2], scale_log2, r0)), ex2(fmaf(s[3], scale_log2, r1))};
+    const float p[4] = {ex2(fmaf(s[0], scale_log2, -m[0])), ex2(fmaf(s[1], scale_log2, -m[1])), ex2(fmaf(s[2], scale_log2, -m[0])), ex2(fmaf(s[3], scale_log2, -m[1]))};
     l[0] += p[0] + p[2];
     l[1] += p[1] + p[3];
     uint32_t hi[2], lo[2];
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
   for (int e = 0; e < 2; ++e) {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) w.l[e] += __shfl_xor_sync(0xffffffffu, w.l[e], o);
-    if (w.l[e] != w.l[e] && w.m[e] == -INFINITY) w.m[e] = 0.f;  // (scores that are no numbers are not seen by the maximum)
+    if (w.m[e] == R::kNone) w.m[e] = w.l[e] != w.l[e] ? 0.f : -INFINITY;  // (scores that are no numbers are not seen by the maximum)
     if (g == 0) sm_m[warp][2 * t + e] = w.m[e], sm_l[warp][2 * t + e] = w.l[e];
 #pragma unroll
     for (int i = 0; i < R::kTiles; ++i) *reinterpret_cast<float2*>(&sm_o[warp][2 * t + e][g * (kDim / 8) + 2 * i]) = make_float2(w.ot[i][e], w.ot[i][2 + e]);

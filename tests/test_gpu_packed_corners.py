@@ -77,3 +77,29 @@ def test_the_largest_values_of_pages_do_not_reach_rows_that_do_not_see_them(pref
         b.plan(n)
         got.append(b.attend(0, q)[:, :, :n - hidden])
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("heads", [1, 2])
+@pytest.mark.parametrize("n", [1, 3, 8, 40, 200])
+@pytest.mark.parametrize("length,some", [(300, 200), (300, 299), (5000, 4900)])
+def test_scores_of_minus_infinity_are_probabilities_of_zero(heads, n, length, some):
+    """The first `some` tokens' scores do not fit 32 bits: the others have the attention, in equal parts."""
+    g = gen(34)
+    c = make(1, 128, 1, length)
+    b = c.batch(c.open())
+    b.extend(length)
+    k = torch.zeros((1, 1, length, 128), dtype=torch.bfloat16, device="cuda")
+    k[:, :, :some] = -2.0 ** 100
+    k[:, :, 0] = 0  # (every row sees a score that fits)
+    v = rand(g, 1, 1, length, 128)
+    b.write(0, k, v)
+    b.plan(n)
+    out, lse = b.attend(0, torch.full((1, heads, n, 128), 2.0 ** 100, dtype=torch.bfloat16, device="cuda"), return_lse=True, weigh=True, decay=0.0)
+    assert (k == held(c, 0, 0)[0]).all()
+    v, at = held(c, 0, 0)[1][0], torch.arange(length, device="cuda")
+    seen = ((at >= some) | (at == 0)) & (at <= torch.arange(length - n, length, device="cuda")[:, None])
+    p = seen.double() / seen.sum(-1, keepdim=True)
+    tol = U[c.dtype] * (p @ v).abs() + (U[c.dtype] + 2.0 ** -16) * (p @ v.abs())
+    assert ((out[0].double() - p @ v).abs() <= tol).all()
+    assert ((lse[0].double() - seen.sum(-1).double().log()).abs() <= 1e-5).all()
+    assert ((c.weights[0, 0, 0].double() - heads * p.sum(0)).abs() <= 2.0 ** -18 * heads * p.sum(0)).all()
