@@ -305,34 +305,32 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 4) packed_rows_kernel(const _
     while (turn(k0, v0, k1, v1) && turn(k1, v1, k0, v0)) {
     }
   }
+  // Keys that some rows do not see: a value that is no number must not reach those, and 0 times it is none.  Its group is 0 here, and from its
+  // place on the rows that see it become none in the end, in these numbers alone.
+  int none = INT_MAX;  // the first such key, of the group that this thread's numbers are of
 #pragma unroll 1
   for (; j0 < key1; j0 += kStep, at.advance(kStep)) {
     typename R::Key k;
     typename R::Value v;
-    at.load(k, v, min(16, key1 - j0));
-    // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and its
-    // key is no number in its place, so that the rows that see it still become none.
-    uint32_t bad = 0;
+    const int nk = min(16, key1 - j0);
+    at.load(k, v, nk);
 #pragma unroll
-    for (int ki = 0; ki < 4; ++ki) {
-      const bool odd = C::odd(v.ms[ki]);
-      if (odd) v.ms[ki] = 0;
-      const uint32_t any = __ballot_sync(0xffffffffu, odd);  // of key 2t + .. in every lane with that t
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-        if (any & (0x11111111u << tt)) bad |= 1u << (2 * tt + (ki & 1) + (ki >> 1) * 8);
-    }
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-      if (bad >> (nt * 8 + g) & 1) k.ms[nt] = 0x7fff7fffu;
+    for (int ki = 0; ki < 4; ++ki)
+      if (C::odd(v.ms[ki])) v.ms[ki] = 0, none = min(none, j0 + min(2 * t + (ki & 1) + (ki >> 1) * 8, nk - 1));
     w.template group<false, kWeigh>(k, v, j0, key1, P.scale_log2, logits, P.pitch, two);
   }
+  none = min(none, __shfl_xor_sync(0xffffffffu, none, 1));
+  none = min(none, __shfl_xor_sync(0xffffffffu, none, 2));
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) w.l[e] += __shfl_xor_sync(0xffffffffu, w.l[e], o);
     if (w.m[e] == R::kNone) w.m[e] = w.l[e] != w.l[e] ? 0.f : -INFINITY;  // (scores that are no numbers are not seen by the maximum)
     if (g == 0) sm_m[warp][2 * t + e] = w.m[e], sm_l[warp][2 * t + e] = w.l[e];
+    if (none < w.lim[e]) {
+#pragma unroll
+      for (int i = 0; i < R::kTiles; ++i) w.ot[i][e] = w.ot[i][2 + e] = NAN;
+    }
 #pragma unroll
     for (int i = 0; i < R::kTiles; ++i) *reinterpret_cast<float2*>(&sm_o[warp][2 * t + e][g * (kDim / 8) + 2 * i]) = make_float2(w.ot[i][e], w.ot[i][2 + e]);
   }
@@ -678,7 +676,7 @@ int many_units(const infllm_packed* c, const infllm_packed_seq* seqs, PackedTcPa
   return INFLLM_OK;
 }
 
-// Bytes of the image of a launch's tiles, 0 where numbers are taken out of their codes by the blocks themselves: with an image a tile of 256
+// Bytes of the image of a launch's tiles, and of a word for each, 0 where numbers are taken out of their codes by the blocks themselves: with an image a tile of 256
 // rows takes 2.2 us instead of 2.45, and to make one takes 0.013 us a tile of the machine's time; so it pays from about four blocks of rows
 // to a tile on.  Not beyond a gigabyte, as a cache in 4 bits is there for want of memory.
 int64_t image_bytes(const infllm_packed* c, const infllm_packed_seq* seqs, int n, int group) {
@@ -688,7 +686,7 @@ int64_t image_bytes(const infllm_packed* c, const infllm_packed_seq* seqs, int n
     tiles += t, blocks += t * ceil_div((int64_t)seqs[i].count * group, kBlockRows);
   }
   const int64_t bytes = tiles * c->n_kv_heads * 2 * kKeyTile * c->head_dim * 2;
-  return blocks >= 4 * tiles && bytes <= 1 << 30 ? bytes : 0;
+  return blocks >= 4 * tiles && bytes <= 1 << 30 ? bytes + ceil_div(tiles * c->n_kv_heads * 4, 16) * 16 : 0;
 }
 
 // the units of the attention of seqs[0 .. n - 1] for many rows
@@ -773,9 +771,10 @@ int attend_many(PackedTcParams& P, const infllm_packed_seq* seqs, const infllm_p
   int fewest = P.a.most, rows = 0;
   for (int i = 0; i < P.a.batch; ++i) {
     P.a.seq[i].keys = P.n_image;
-    if (image > 0 && seqs[i].count > 0) P.n_image += c->n_kv_heads * (int)ceil_div(seqs[i].length, kKeyTile);
+    if (image > 0 && seqs[i].count > 0) P.n_image += c->n_kv_heads * (int)ceil_div(seqs[i].length, kKeyTile);  // (up to 16384, in a gigabyte)
     fewest = std::min(fewest, seqs[i].count), rows = std::max(rows, std::min(kBlockRows, seqs[i].count * P.a.group));
   }
+  P.odd = (int32_t*)(work + (int64_t)P.n_image * 2 * kKeyTile * kDim * 2);
   P.a.part_o = (float*)(work + image), P.a.part_lse = P.a.part_o + (int64_t)2 * n_sm * kBlockRows * kDim;
   INFLLM_TRY(tc_get_error_ptr(&P.a.err));
   if (P.n_ctas > 0) INFLLM_TRY(packed_tc_launch(P, c->dtype, kDim, s));

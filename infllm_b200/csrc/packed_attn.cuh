@@ -49,6 +49,7 @@ struct PackedTcParams {
   PackedAttnParams a;
   int32_t n_ctas, n_image;
   char* image;  // prompts: n_image tiles, keys and values, as 16-bit numbers (packed_tc.cu); null: none
+  int32_t* odd;  // of each, behind it, a multiple of 4 words: whether it has 0 where a value is no number
   int2 start[kMaxSms + 1];
 };
 

@@ -20,6 +20,7 @@
 // sequences of 12288 (192 rows of 8 KV heads) 124 us, 12 tokens (48 rows) 77.
 // Tried: 4, 7, 8, 10, 12, 14 and 16 code warps; registers given from warpgroup to warpgroup with 28 warps (five times slower: spills).
 #include <atomic>
+#include <climits>
 
 #include "attn_tc.cuh"
 #include "decode_warp.cuh"
@@ -76,6 +77,33 @@ struct Pieces {  // a block's, in turn
     return true;
   }
 };
+
+// Values that are no numbers.  In a tile that some rows do not see whole they must not reach those, and 0 times one is none: their groups
+// are 0 there, and the rows that see them become none in the end, in these 32 numbers alone.  Which those are, of a row that sees `lim` keys
+// and a block's piece `i`, is looked up here by the row's warp, once the block has met such a value: a bit for each group.  (Not inlined: 48
+// tokens of 8 sequences 123.8 us, as without; inlined 124.8.)
+template <typename T, int kDim, bool kImage>
+__device__ __noinline__ uint32_t groups_that_are_none(const PackedTcParams& P, int i, int lim) {
+  constexpr int kGroups = kDim / 32;
+  Pieces pieces(P);
+  Piece U;
+  for (int x = 0; x <= i; ++x) pieces.next(P, U);
+  const PackedAttnSeq& S = P.a.seq[U.b];
+  const uint32_t* ms = reinterpret_cast<const uint32_t*>(P.a.at.scales + P.a.at.scales_v + P.a.at.row0(S.slot, U.hkv) * (kDim / 8));
+  const int from = max(keys_of_row(S, P.a.group, kImage ? 0 : U.row0) / kKeyTile, U.tile0) * kKeyTile, to = min((U.tile0 + U.n) * kKeyTile, S.length);
+  uint32_t none = 0;
+#pragma unroll 1
+  for (int g = 0; g < kGroups; ++g) {
+    int first = INT_MAX;  // the first key whose group is none
+#pragma unroll 1
+    for (int j = from + (threadIdx.x & 31); j < to && first == INT_MAX; j += 32)
+      if (Codes<T>::odd(__ldg(ms + (int64_t)j * kGroups + g))) first = j;
+    __syncwarp();
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (first < lim) none |= 1u << g;
+  }
+  return none;
+}
 }  // namespace xtc
 
 template <typename T, int kDim, bool kImage>
@@ -87,6 +115,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
   const uint32_t s_base = smem_u32(smem), sQ = s_base + L::kQ, sRing = s_base + L::kRing, bars = s_base + L::kBar;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + N_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBar + N_BARS * 8 + 8);
+  volatile int* odd_flag = abort_flag + 1;  // a value that is no number has been left out of a tile
   auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* const err = P.a.err;
@@ -99,7 +128,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
     static_assert(N_BARS <= 32 && N_BARS * 8 + 16 <= 256, "");
     // tiles: the warps that make them; queries and probabilities: a team's four; what the teams have of the same rows: both
     if (lane < N_BARS) mbar_init(bar(lane), lane < EMPTY0 ? (kImage ? 1u : kCodeWarps / 2u) : lane == Q_FULL0 || lane == Q_FULL0 + 1 || lane == P_FULL0 || lane == P_FULL0 + 1 ? 4u : lane == MERGE ? 8u : 1u);
-    if (lane == 0) *abort_flag = 0;
+    if (lane == 0) *abort_flag = 0, *odd_flag = 0;
     mbar_fence_init();
   }
   if (warp == kWarpMma) {
@@ -125,6 +154,13 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
       const PackedAttnSeq& S = P.a.seq[U.b];
       const char* from = P.image + ((int64_t)S.keys + (int64_t)U.hkv * ((S.length + kKeyTile - 1) / kKeyTile) + U.tile0) * (2 * L::kTileBytes);
       for (int p = 0; p < 2 * U.n && ok; ++p) {
+        if (base == 0 && p == min(2 * U.n - 1, kStages - 1)) {  // (behind the first loads, and before a unit's last)
+          const int4* odd = reinterpret_cast<const int4*>(P.odd);
+          int any = 0;
+          for (int x = lane; x < P.n_image / 4; x += 32) any |= odd[x].x | odd[x].y | odd[x].z | odd[x].w;
+          for (int x = P.n_image / 4 * 4 + lane; x < P.n_image; x += 32) any |= P.odd[x];
+          if (__any_sync(0xffffffffu, any != 0) && lead) *odd_flag = 1;
+        }
         const int b = (base + p) % kStages;
         if (base + p >= kStages) ok = warp_wait(bar(EMPTY0 + b), ring_parity(base + p - kStages, kStages), abort_flag, err, 751);
         if (ok && lead) {
@@ -201,17 +237,15 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
     // (two copies of a turn, each with its own registers: what is on its way is not to be moved, which would wait for it)
     auto turn = [&](Raw& raw, Raw& then) {
       const int slot = base + (values ? pos_v(i, n) : pos_k(i));
-      if (seen < kKeyTile) {
-        // Keys that some rows do not see: what is no number must not reach those, and 0 times it is none.  Such a value is 0 here, and
-        // its key is no number in its place, so that the rows that see it still become none.
-        const char* other = scales - t * 4 + P.a.at.scales_v;
+      if (values && seen < kKeyTile) {  // (groups_that_are_none)
+        bool any = false;
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          if (values && C::odd(raw.ms[x])) raw.ms[x] = 0;
-          if (!values && r0 + x * kStep < min(keys, kKeyTile))
-            for (int g = 0; g < kGroups; ++g)
-              if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(other + x * kStep * kScales + g * 4)))) raw.ms[x] = 0x7fff7fffu;
+          const bool odd = C::odd(raw.ms[x]);
+          raw.ms[x] = odd ? 0 : raw.ms[x];
+          any = any || odd;
         }
+        if (any) *odd_flag = 1;
       }
       advance();
       load(then);
@@ -392,6 +426,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
       if (lane == 0) mbar_arrive(bar(Q_FULL0 + team));
     };
     float2* const ml = reinterpret_cast<float2*>(smem + L::kMl);  // of each team's rows, where both have the same
+    int piece = 0;                     // of the block's
     int ns[2] = {0, 0}, n_merged = 0;  // tiles so far of each team; arrivals of both at MERGE
     bool ok = true, owed = false;      // the other team may still read this one's O
     const uint32_t tS = tmem + team * 128 + lane_base;
@@ -522,14 +557,16 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : l;  // (a NaN stays one)
         mine *= inv, theirs *= inv;
+        const uint32_t none = __any_sync(0xffffffffu, *odd_flag) ? groups_that_are_none<T, kDim, kImage>(P, piece, now.lim) : 0;
 #pragma unroll 1
         for (int c = merge ? team * (kDim / 2) : 0; c < (merge && team == 0 ? kDim / 2 : kDim); c += 32) {
           uint32_t o[32];
           float* f = reinterpret_cast<float*>(o);
           tmem_ld32(tO + c, o);
           tmem_wait_ld32(o);
+          const float by = none >> (c / 32) & 1 ? NAN : mine;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) f[k] *= mine;
+          for (int k = 0; k < 32; ++k) f[k] *= by;
           if (merge) {
             uint32_t z[32];
             tmem_ld32(tmem + 256 + (team ^ 1) * 128 + lane_base + c, z);
@@ -573,7 +610,7 @@ __global__ void __launch_bounds__(xtc::threads(kImage), 1) packed_tc_kernel(cons
       if (now.two) ns[0] += now.n, ns[1] += now.n;
       else ns[0] += (now.n + 1) / 2, ns[1] += now.n / 2;
       __syncwarp();
-      now = next;
+      now = next, ++piece;
     }
   }
   tc_fence_before();
@@ -600,6 +637,7 @@ __global__ void __launch_bounds__(256) packed_image_kernel(const __grid_constant
   const PackedAttnSeq S = P.a.seq[lo];
   const int tiles = (S.length + kKeyTile - 1) / kKeyTile, hkv = (tile - S.keys) / tiles, j0 = (tile - S.keys) % tiles * kKeyTile;
   const bool mixed = j0 + kKeyTile > keys_of_row(S, P.a.group, 0);
+  bool odd = false;
   chain_enter();
   for (int value = 0; value < 2; ++value) {
     const int64_t row = P.a.at.row0(S.slot, hkv) + j0;
@@ -614,10 +652,7 @@ __global__ void __launch_bounds__(256) packed_image_kernel(const __grid_constant
       if (j0 + k < S.length) {
         c[x] = __ldg(reinterpret_cast<const uint4*>(codes + k * (kDim / 2) + t * 16));
         ms[x] = __ldg(reinterpret_cast<const uint32_t*>(scales + (value ? P.a.at.scales_v : 0) + k * (kDim / 8) + t * 4));
-        if (mixed && value && C::odd(ms[x])) ms[x] = 0;  // (as the warps that do this without an image)
-        if (mixed && !value)
-          for (int g = 0; g < kGroups; ++g)
-            if (C::odd(__ldg(reinterpret_cast<const uint32_t*>(scales + P.a.at.scales_v + k * (kDim / 8) + g * 4)))) ms[x] = 0x7fff7fffu;
+        if (mixed && value && C::odd(ms[x])) ms[x] = 0, odd = true;  // (as the warps that do this without an image)
       }
     }
     if (value) {
@@ -630,8 +665,9 @@ __global__ void __launch_bounds__(256) packed_image_kernel(const __grid_constant
       put_group<T>(smem + (t >> 1) * kSubTileBytes, k, t, c[x], ms[x]);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
+    const int any = __syncthreads_or(odd);
     if (threadIdx.x == 0) {
+      if (value) P.odd[tile] = any;
       asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(P.image + ((int64_t)2 * tile + value) * L::kTileBytes), "r"(smem_u32(smem)), "r"((uint32_t)L::kTileBytes) : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }

@@ -39,6 +39,44 @@ def test_many_small_probabilities_beside_a_large_one(dim, dtype, group, n, below
     assert ((lse[-1, -group:].double() - want_lse).abs() <= e + 2.0 ** -20 * want_lse.abs() + 1e-6).all()
 
 
+@pytest.mark.parametrize("dim,kv,heads,dtype", SHAPES[:3])
+@pytest.mark.parametrize("length,n,at", [
+    (500, 1, "newest"), (512, 1, "newest"), (500, 1, "deep"), (500, 4, "newest"), (509, 2, "middle"), (500, 40, "newest"), (500, 40, "middle"), (500, 9, "deep"),
+    (700, 200, "all"), (900, 700, "middle"), (900, 900, "all"), (20000, 1, "newest"), (20000, 40, "all"), (20000, 600, "middle"), (20000, 600, "newest")])
+def test_a_value_that_is_none_takes_its_own_dimensions_alone(dim, kv, heads, dtype, length, n, at):
+    """The 32 numbers of a value that are none: so are these dimensions of the rows that see it.  The others, log-sum-exps and weights do
+    not depend on them, and are bit for bit what they are beside a finite value."""
+    g, group = gen(32), heads // kv
+    c = make(kv, dim, 2, length + 5, dtype)
+    s = c.open(2)[1:]
+    b = c.batch(s)
+    b.extend(length)
+    k, v = (rand(g, 1, kv, length, dim, dtype=dtype) for _ in range(2))
+    places = {"newest": [length - 1], "deep": [13], "middle": [length - n // 2 - 1], "all": [length - n, length - n // 2, length - 2, length - 1]}[at]
+    places = [(x, i % (dim // 32), (kv - 1) * (1 - i % 2)) for i, x in enumerate(places)]  # token, group, KV head
+    for x, y, h in places:
+        v[0, h, x, 32 * y:32 * y + 32] = 0
+    q = rand(g, 1, heads, n, dim, dtype=dtype)
+
+    def attend():
+        b.plan(length)
+        b.write(0, k, v)
+        b.plan(n)
+        out, lse = b.attend(0, q, return_lse=True, weigh=True, decay=0.0)
+        return out, lse, c.weights[0, s[0], :, :length].clone()
+
+    fine, fine_lse, fine_weights = attend()
+    assert fine.isfinite().all() and fine_lse.isfinite().all() and fine_weights.isfinite().all()
+    want = fine.clone()
+    for i, (x, y, h) in enumerate(places):
+        v[0, h, x, 32 * y + 7] = (INF, NAN, -INF)[i % 3]
+        want[0, h * group:(h + 1) * group, max(0, x - (length - n)):, 32 * y:32 * y + 32] = NAN
+    out, lse, weights = attend()
+    assert torch.equal(lse, fine_lse) and torch.equal(weights, fine_weights)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.nan_to_num(-9), want.nan_to_num(-9))
+
+
 @pytest.mark.parametrize("dim,kv,heads,dtype", [x for x in SHAPES if x[3] == torch.bfloat16])
 @pytest.mark.parametrize("length,n", [(150, 2), (150, 12), (250, 60), (900, 700), (9000, 40)])
 def test_the_largest_values_do_not_reach_rows_that_do_not_see_them(dim, kv, heads, dtype, length, n):
