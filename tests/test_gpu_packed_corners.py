@@ -141,3 +141,28 @@ def test_scores_of_minus_infinity_are_probabilities_of_zero(heads, n, length, so
     assert ((out[0].double() - p @ v).abs() <= tol).all()
     assert ((lse[0].double() - seen.sum(-1).double().log()).abs() <= 1e-5).all()
     assert ((c.weights[0, 0, 0].double() - heads * p.sum(0)).abs() <= 2.0 ** -18 * heads * p.sum(0)).all()
+
+
+@pytest.mark.parametrize("dim,kv,heads,dtype", SHAPES[:4] + [(128, 3, 6, torch.bfloat16), (128, 1, 5, torch.float16)])
+@pytest.mark.parametrize("lengths,counts", [([1], [1]), ([15, 16, 17], [1, 1, 1]), ([64, 65, 3, 700], [1, 0, 1, 1]), ([5000], [1]), ([2049, 130], [2, 1]), ([60000], [4])])
+def test_up_to_eight_rows_round_their_output_alone(dim, kv, heads, dtype, lengths, counts):
+    """Their probabilities are as good as 32 bits: 2^-16 of sum_j p_j |v_j| beside the output's own rounding."""
+    counts = [min(x, 8 * kv // heads) for x in counts]
+    g, most = gen(sum(lengths) + dim), max(counts)
+    c = make(kv, dim, len(lengths) + 1, max(lengths) + 3, dtype)
+    seqs = c.open(len(lengths) + 1)[1:]
+    b = fill(c, g, seqs, lengths)
+    b.plan(counts)
+    q = rand(g, len(seqs), heads, most, dim, dtype=dtype, scale=1.5)
+    out, lse = b.attend(0, q, return_lse=True)
+    check(c, b, counts, q, out, lse)
+    for i, (s, n) in enumerate(zip(seqs, counts)):
+        if n:
+            k, v = held(c, 0, s)
+            want, mass, _, p, e = formula(q[i, :, most - n:], k, v, n, 1 / math.sqrt(dim))
+            err = (out[i, :, most - n:].double() - want).abs()
+            tol = U[dtype] * want.abs() + (2.0 ** -16 + 2 * e[..., None]) * mass + TINY[dtype]
+            assert (err <= tol).all(), (i, (err / tol).max().item())
+            if dtype == torch.bfloat16 and 15 <= k.size(1) <= 1000:  # (probabilities of 16 bits would not do)
+                p, v, top = p.cpu(), v.cpu().repeat_interleave(heads // kv, 0), p.amax(-1, keepdim=True).cpu()
+                assert (((p / top).to(dtype).double() * top @ v - want.cpu()).abs() > tol.cpu()).any(), i
