@@ -22,6 +22,7 @@ capture, while extend, retract and what evict does to lengths happen on the host
 a write with `rope`, the tables of positions that were there, which the cache keeps for it."""
 import ctypes
 import math
+import operator
 from array import array
 from ctypes import c_int32, c_int64
 
@@ -129,6 +130,7 @@ class PackedCache:
         to head: `places` says it.  Keys keep the rotation that they were written with, and position() goes on from where it was.
         `into`: sequences of this cache that get what stays (all of a shorter sequence) in place of what they hold; `seqs` then
         stay as they are."""
+        budget, sink, recent = (operator.index(x) for x in (budget, sink, recent))
         for x in (budget, sink, recent):
             if not -1 << 63 <= x < 1 << 63:
                 raise OverflowError(f"{x} is beyond 64 bits")
@@ -163,6 +165,15 @@ def _long(values):
     return (c_int64 * len(values)).from_buffer(array("q", values)) if len(values) else (c_int64 * 1)()
 
 
+def _one(n):
+    """Whether n, which is no int, is one number and not several: numpy's, a tensor's without dimensions."""
+    try:
+        len(n)
+    except TypeError:
+        return True
+    return False
+
+
 class PackedBatch:
     """Sequences that take a step together.  extend(), or plan(), says how many of each one's newest tokens the step is about;
     write() and attend() are then called in every layer.  Tensors have as many tokens as the largest of those counts; a
@@ -184,11 +195,13 @@ class PackedBatch:
 
     def _step(self, what, n):
         c, counts, same = self.cache, None, n
-        if not isinstance(n, int):
+        if not isinstance(n, int) and not _one(n):
             if len(n) != self._n:
                 raise ValueError(f"{self._n} sequences and {len(n)} counts")
             counts, same = _long(n), 0
-        elif not -1 << 63 <= n < 1 << 63:
+        else:
+            n = same = operator.index(n)
+        if counts is None and not -1 << 63 <= n < 1 << 63:
             raise OverflowError(f"{n} is beyond 64 bits")
         rc = _lib_call.infllm_packed_book_step(c._book_ref, what, self._ids, self._opened, self._n, counts, same, self._table, self._as_of,
                                                self._info)

@@ -3,6 +3,7 @@ import ctypes
 import random
 from ctypes import c_int32, c_int64
 
+import numpy as np
 import pytest
 import torch
 
@@ -280,3 +281,26 @@ def test_calls_without_work():
         assert call(seqs=()) == L.OK
     assert write(seqs=((1, 10, 0, 7),), most=0) == attend(seqs=((1, 10, 0, 7),), most=0) == values(seqs=((1, 10, 0, 7),), most=0) == L.OK
     assert evict(budget=10) == evict(seqs=((1, 0, 0, 0),), budget=0, sink=0, recent=0, into=[2]) == L.OK
+
+
+@pytest.mark.parametrize("number", [np.int64, np.int32, torch.tensor, np.array])
+def test_numbers_of_other_kinds(cache, number):
+    """A count that numpy or torch made is one for every sequence, an array of them one for each."""
+    c = cache()
+    b = c.batch(c.open(2))
+    b.extend(number(5))
+    assert [c.length(0), c.length(1)] == [5, 5] and b.tokens == 5
+    b.extend(np.array([3, 1]))
+    b.plan(torch.tensor([2, 1]))
+    assert [c.length(0), c.length(1)] == [8, 6] and b.tokens == 2
+    b.retract(number(1))
+    c.evict([0], number(4), number(1))
+    assert [c.length(0), c.length(1)] == [4, 5]
+    for n in (1.0, np.float64(1), torch.tensor(1.0), None):
+        with pytest.raises(TypeError):
+            b.extend(n)
+    one = c.batch([1])
+    one.extend(torch.tensor([2]))
+    with pytest.raises(ValueError):
+        b.extend(torch.tensor([2]))
+    assert [c.length(0), c.length(1)] == [4, 7]
