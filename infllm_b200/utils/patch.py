@@ -24,10 +24,15 @@ def _attention_modules(model):
 
 def patch_hf(model, attn_type: str = "inf-llm", attn_kwargs: dict = None, base=None, distance_scale=None, **kwargs):
     """Same arguments as the reference's patch_hf (patch.py:33-40).  `attn_type` is a key of ATTN_FORWRAD
-    ("inf-llm", "infinite-lm", "stream-llm"; the reference's yaml files spell the first one "inf_llm" too)."""
+    ("inf-llm", "infinite-lm", "stream-llm"; the reference's yaml files spell the first one "inf_llm" too).  "paged" and "packed"
+    are refused: their caches are of several sequences, and each step of those has to be announced to a batch (PagedBatch.extend,
+    PackedBatch.extend) before a model is called."""
     attn_kwargs = dict(attn_kwargs or {})
     attn_kwargs.update(kwargs)
     attn_type = {"inf_llm": "inf-llm", "infinite_lm": "infinite-lm", "stream_llm": "stream-llm"}.get(attn_type, attn_type)
+    if attn_type in ("paged", "packed"):
+        raise ValueError(f'patch_hf has no sequences and no steps, which attention type "{attn_type}" takes from a batch: call its cache from '
+                         "the model's own attention, or use SharedPromptDecoder or PackedStreamDecoder")
     forward = ATTN_FORWRAD[attn_type](**attn_kwargs)
     cfg = model.config
     head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
