@@ -18,11 +18,11 @@ class PackedStreamDecoder(HeadGroupDecoder):
 
     def __init__(self, n_layers, hidden, n_heads, n_kv_heads, head_dim, ffn, vocab, max_tokens, n_sequences=1, budget=None, sink=0, recent=0,
                  slack=64, decay=1.0, world=1, **kwargs):
-        super().__init__(n_layers, hidden, n_heads, n_kv_heads, head_dim, ffn, vocab, {}, world=world, attn_type="packed", **kwargs)
-        if budget is not None and not 0 <= sink + recent <= budget:
+        if budget is not None and (min(sink, recent) < 0 or sink + recent > budget):
             raise ValueError(f"{budget} tokens, the first {sink} and the newest {recent} among them")
         if budget is not None and not 0 <= slack < max_tokens - budget:
             raise ValueError(f"{budget} tokens, up to {slack} more and the next one, where {max_tokens} fit")
+        super().__init__(n_layers, hidden, n_heads, n_kv_heads, head_dim, ffn, vocab, {}, world=world, attn_type="packed", **kwargs)
         self.cache = PackedCache(n_layers, self.kv_heads, head_dim, n_sequences, max_tokens, self.dtype, self.device)
         self.budget, self.sink, self.recent, self.slack, self.decay = budget, sink, recent, slack, decay
 
