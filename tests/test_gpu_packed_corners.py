@@ -166,3 +166,42 @@ def test_up_to_eight_rows_round_their_output_alone(dim, kv, heads, dtype, length
             if dtype == torch.bfloat16 and 15 <= k.size(1) <= 1000:  # (probabilities of 16 bits would not do)
                 p, v, top = p.cpu(), v.cpu().repeat_interleave(heads // kv, 0), p.amax(-1, keepdim=True).cpu()
                 assert (((p / top).to(dtype).double() * top @ v - want.cpu()).abs() > tol.cpu()).any(), i
+
+
+@pytest.mark.parametrize("dim,kv,heads,dtype", SHAPES[:3])
+def test_a_prompt_and_single_tokens_in_one_call(dim, kv, heads, dtype):
+    """All of them go to the kernel of many rows then: each sequence's rows are the formulas', as they are alone."""
+    g, lengths, counts = gen(36), [900] + [40 + 97 * i for i in range(20)], [600] + [1] * 20
+    c = make(kv, dim, 21, max(lengths), dtype)
+    b = fill(c, g, c.open(21), lengths)
+    q = rand(g, 21, heads, 600, dim, dtype=dtype, scale=1.5)
+    c.weights.fill_(0.5)
+    before = c.weights.clone()
+    b.plan(counts)
+    out, lse = b.attend(0, q, return_lse=True, weigh=1, decay=0.5)
+    check(c, b, counts, q, out, lse, weigh=1, before=before, decay=0.5)
+    alone = c.batch(b.seqs[1:])
+    alone.plan(1)
+    out1, lse1 = alone.attend(0, q[1:, :, -1:], return_lse=True)
+    check(c, alone, [1] * 20, q[1:, :, -1:], out1, lse1)
+
+
+def test_calls_of_many_sizes_one_after_the_other():
+    """Workspaces are not cleared between calls, whose memory is the allocator's: what one has left does not reach the next."""
+    g, calls = gen(37), []
+    c = make(2, 128, 6, 3000)
+    seqs = c.open(6)
+    fill(c, g, seqs, [3000, 1, 700, 129, 2048, 31])
+    for s, n, weigh in ((seqs, 1, True), (seqs[:1], 900, True), (seqs[2:5], 100, False), (seqs[:1], 3000, 7), (seqs[4:], 8, True), (seqs[:3:2], 2, False), (seqs[1:2], 1, True)):
+        b = c.batch(s)
+        b.plan([min(n, c.length(x)) for x in s])
+        q = rand(g, len(s), 8, b.tokens, 128)
+        calls.append(lambda b=b, q=q, weigh=weigh: (*b.attend(0, q, return_lse=True, weigh=weigh, decay=0.0), c.weights[0, b.seqs].clone()))
+    want = []
+    for call in calls:
+        torch.cuda.empty_cache()
+        want.append(call())
+    for i in [0, 3, 6, 1, 5, 2, 4, 0, 6, 3, 1, 4, 2, 5, 3, 0] * 2:
+        junk = torch.full((1 << 22,), NAN, device="cuda")  # (numbers that are none in what the allocator gives next)
+        del junk
+        assert all(torch.equal(x.nan_to_num(-9), y.nan_to_num(-9)) for x, y in zip(calls[i]()[:2], want[i][:2])), i
