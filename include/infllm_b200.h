@@ -613,7 +613,8 @@ int infllm_page_batch_attend(infllm_page_batch* b, int layer, const void* d_q, i
  *
  * Of each 32 neighbouring numbers x of a row, in the 16-bit type T: m = min x, s = T((max x - m) / 15), and of each x the code c, the
  * nearest of 0 .. 15 to (x - m) / s, ties to even (0 where s is 0).  It stands for T(m + s c).   Where T(m + 15 s) were infinite, s
- * is the next smaller number of T.  A group with a number that is not finite, or whose step is not, or in bf16 is 2^122 or more, is NaN.
+ * is the next smaller number of T.  A group with a number that is not finite, or whose step is not, or in bf16 is 2^122 or more, is NaN: of a key,
+ * to every row that sees it, its log-sum-exp and the weights; of a value, in its own 32 dimensions of the rows that see it alone.
  *
  * The memory is the caller's, 16-byte aligned, and the library keeps nothing of its own:
  *   d_codes    (n_layers, 2: keys and values, n_sequences, n_kv_heads, max_tokens, head_dim / 8) 32-bit words; of a word's eight

@@ -13,7 +13,8 @@ instead of 256 (per KV head of 128 dimensions, each), and can drop tokens by the
 
 Of each 32 neighbouring numbers x of a key (rotated to its position) or value, in the cache's 16-bit type T, it holds m = min x, a step
 s = T((max x - m) / 15) and of each number 4 bits, c, the nearest of 0 .. 15 to (x - m) / s.  They stand for T(m + s c).  (Where
-T(m + 15 s) were infinite, s is the next smaller number.)  Where one of 32 numbers is not finite, or where the step is not, or in bf16 is 2^122 or more, none is a number.
+T(m + 15 s) were infinite, s is the next smaller number.)  Where one of 32 numbers is not finite, or where the step is not, or in bf16 is 2^122 or more, none is a number: of
+a value, these dimensions of the rows that see it are none, and nothing else is.
 
 Tensors are (batch, heads, tokens, head_dim) views with any strides whose rows are 16-byte aligned, as the other attention types take
 them.  Work goes to the current stream; all calls on a cache belong on one stream, or are ordered by the caller.  Inside a CUDA

@@ -50,13 +50,13 @@ __device__ __forceinline__ uint32_t ld_stream4(const char* p) {
 // P is two 16-bit numbers, p = hi + lo, so that an output's only rounding is its own: where rows are no more than four (kFour), the other
 // four columns have the same rows again, and theirs is lo, in the same product.  In fp16, whose numbers end at 2^-24, lo is kept times
 // 2^11, as it is that much smaller than hi wherever hi has all its digits: the other four columns are scaled at the end; with more rows the
-// products of lo are formed apart and added, a multiplication and addition of O's numbers for 16 keys.  (In fp16 217 us where 215 without, below;
-// of eight rows, 16 sequences with 64/8 heads, 139 for 134.)
+// products of lo are formed apart and added, a multiplication and addition of O's numbers for 16 keys.  (Without the two an fp16 call of 32
+// sequences takes 215 us instead of 217, below; of eight rows, 16 sequences with 64/8 heads, 134 instead of 139.)
 // The reference of a row is lazy (packed_attn.cuh): only where it moves O is scaled and do lanes exchange anything.
 // What bounds it: the codes' bytes, and close behind them what is issued to take numbers out of them, 397 instructions a warp for 16 keys of
-// 128 (loads alone 138 us where the kernel takes 192; without the taking out 189).  One new token of 32 sequences of 24576 tokens, 32/8
-// heads of 128 in bf16: 1.007 GB in 192 us, 5.24 TB/s; of one sequence of 131072, 168 MB in 39 us.  What brought it there from 389: loads of
-// the next 16 keys under this one's products, two copies of a turn so that their registers stay where they are, Q in shared memory (four
+// 128 (loads alone 138 us where the kernel took 192; without the taking out 189).  One new token of 32 sequences of 24576 tokens, 32/8
+// heads of 128 in bf16: 1.007 GB in 190 us, 5.30 TB/s (fp16 216); of 16, 64/8 heads, 111 (126); of one sequence of 131072, 168 MB in 39 us.
+// What brought it there from 389: loads of the next 16 keys under this one's products, two copies of a turn so that their registers stay where they are, Q in shared memory (four
 // blocks a multiprocessor by registers), keys as rows of S^T so that a thread's codes have one (m, s), and addresses that run.  Tried, and
 // slower: 32 keys at a time (the kernel of then 291 instead of 286), five blocks a multiprocessor (324), lines asked for into L2 ahead
 // (275, 265), shifts and differences instead of the masks of packed.cuh (a tenth more).

@@ -15,7 +15,7 @@
 // up to 2^-8 of itself.  fp16: by 2^-11 of itself, and where it is less than 2^-25 of its row's largest, by up to 2^-36 of that.)
 // Sums, O and partial rows are fp32.
 // What bounds it: the softmax warps' chain (scores out of TMEM, maximum, exponentials, P back) between two products of its team, with six code
-// warps beside it for issue.  2048 tokens behind 28000, 32/8 heads of 128 in bf16: 895 us with the image, 2.2 us for a tile of 256 rows by
+// warps beside it for issue.  2048 tokens behind 28000, 32/8 heads of 128 in bf16: 889 us with the image, 2.2 us for a tile of 256 rows by
 // 128 keys (products alone, with P as it lies there, 1.63; as fast as they can be issued, 1.1 to 1.2), 963 without.  48 tokens of 8
 // sequences of 12288 (192 rows of 8 KV heads) 124 us, 12 tokens (48 rows) 77.
 // Tried: 4, 7, 8, 10, 12, 14 and 16 code warps; registers given from warpgroup to warpgroup with 28 warps (five times slower: spills).
